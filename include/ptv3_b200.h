@@ -192,6 +192,79 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
                            int max_seqlen, int channels, int heads, float scale, int dtype, void* stream);
 
 /*
+ * Points of the padded rows of a plan, for ptv3_patch_attention_fwd / _bwd, and a look at the plan: every index in range,
+ * every point with one row that answers for it and at most one borrowed one (as ptv3_pad_plan writes plans), sequences that
+ * follow one another from row 0 to n_pad and are no longer than max_seqlen.  With `buckets` (2 pos_bnd + 1 int32) those
+ * are looked at too: all in [0, num_buckets).
+ *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30
+ *   rows        2 * n_pad + (n_pad - n) + 1 int32, written
+ *   status      one uint32 or NULL: PTV3_STATUS_BAD_INDEX where something does not hold (the calls that read `rows` then
+ *               stay within their tensors, and what they leave is undefined)
+ */
+int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
+                    int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* buckets, int pos_bnd,
+                    int num_buckets, int32_t* rows, uint32_t* status, void* stream);
+
+/*
+ * Patch attention that can be trained: with a learned relative position bias by buckets (maps = 1, grid_coord and
+ * table), plain (maps = 1 without them), or differential (maps = 2).  Per head of W = channels / heads values
+ *   maps = 1:  out = softmax(scale q k^T + bias) v
+ *              bias(i, j, h) = sum over axes a of table[a * num_buckets + bucket(g_i[a] - g_j[a])][h],
+ *              bucket(d) = buckets[clamp(d, -pos_bnd, pos_bnd) + pos_bnd]  (the index itself where buckets is NULL: the bias of
+ *              model.py:297-316, 372-380, 468-469)
+ *   maps = 2:  out = (softmax(scale q1 k1^T) - lam[h] softmax(scale q2 k2^T)) v, where the W values of a head's q (and k)
+ *              are q1 and q2 (k1 and k2) of W / 2 each
+ * within each patch; rows borrowed by a patch are keys there and answer for nothing.  W in {16, 32, 64}.  The gradients do
+ * not depend on the order in which anything runs.  A workspace or an `lse` belongs to one call in flight: graphs that may run at
+ * the same time need one each.
+ *   qkv, dqkv   n x 3*channels; out, dout n x channels; dtype PTV3_DTYPE_*
+ *   rows        of ptv3_patch_rows
+ *   table       3 * num_buckets x heads, lam heads: fp32 or bf16 (table_dtype, lam_dtype); gradients in the same type
+ *   lse         heads * maps * n_pad fp32: written by _fwd (may be NULL there), read by _bwd
+ *   _bwd        writes dqkv, and dtable / dlam where not NULL, from qkv, lse and dout
+ *   workspace   of _bwd
+ */
+typedef struct ptv3_patch_attention_args {
+    int64_t n, n_pad;
+    int n_seq, max_seqlen, channels, heads, maps, dtype;
+    float scale;
+    int pos_bnd, num_buckets, table_dtype, lam_dtype;
+    const void* qkv;
+    const int32_t *rows, *cu_seqlens, *grid_coord, *buckets;
+    const void *table, *lam;
+    void* out;
+    float* lse;
+    const void* dout;
+    void *dqkv, *dtable, *dlam;
+    void* workspace;
+    size_t workspace_bytes;
+} ptv3_patch_attention_args;
+
+int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* args, void* stream);
+size_t ptv3_patch_attention_workspace_bytes(const ptv3_patch_attention_args* args);
+int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* args, void* stream);
+
+/*
+ * Norms of queries and keys for each head, and their rotation by grid coordinates, in one pass over the rows of a QKV
+ * projection (either may be left out: weights NULL or grid_coord NULL); values are copied.  Per head of D values
+ *   y = x * rsqrt(mean(x^2) + eps) * weight
+ *   pairs (2 i, 2 i + 1), i < 3 p, p = D / 6:  turned by grid[i / p] * base^(-(i mod p) / p)
+ * D in {8, 16, 32, 64, 128}; the angle is taken in whole turns of 2^-64, so that far coordinates lose nothing.
+ *   qkv, out, dout, dqkv   n x 3*channels, 16-byte aligned, dtype PTV3_DTYPE_*
+ *   q_weight, k_weight     D each, PTV3_DTYPE_* weight_dtype; dq_weight, dk_weight in the same type
+ *   grid_coord             n x 3 int32
+ *   workspace              of _bwd, ptv3_qk_norm_rope_workspace_bytes, where weights are given
+ */
+int ptv3_qk_norm_rope_fwd(const void* qkv, const void* q_weight, const void* k_weight, int weight_dtype,
+                          const int32_t* grid_coord, void* out, int64_t n, int channels, int heads, float eps, double base,
+                          int dtype, void* stream);
+size_t ptv3_qk_norm_rope_workspace_bytes(int64_t n, int channels, int heads);
+int ptv3_qk_norm_rope_bwd(const void* qkv, const void* q_weight, const void* k_weight, int weight_dtype,
+                          const int32_t* grid_coord, const void* dout, void* dqkv, void* dq_weight, void* dk_weight,
+                          int64_t n, int channels, int heads, float eps, double base, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
  * Kernel map of a submanifold convolution.
  * Replaces spconv's indice-pair build behind model.py:546-552 and :767-774.
  *   indices     n x 4 int32 rows (batch, x, y, z), 16-byte aligned, each field

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(_HERE, "csrc", "libptv3_b200.so")
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_f32 = ctypes.c_float
+c_f64 = ctypes.c_double
 c_sz = ctypes.c_size_t
 c_ptr = ctypes.c_void_p
 
@@ -66,6 +67,18 @@ class BackboneArgs(ctypes.Structure):
            ("stem_bn", c_ptr), ("plain_weights", c_int)])
 
 
+class PatchAttentionArgs(ctypes.Structure):
+    """ptv3_patch_attention_args of include/ptv3_b200.h (same field order)."""
+    _fields_ = (
+        [("n", c_i64), ("n_pad", c_i64)]
+        + [(name, c_int) for name in ("n_seq", "max_seqlen", "channels", "heads", "maps", "dtype")]
+        + [("scale", c_f32)]
+        + [(name, c_int) for name in ("pos_bnd", "num_buckets", "table_dtype", "lam_dtype")]
+        + [(name, c_ptr) for name in ("qkv", "rows", "cu_seqlens", "grid_coord", "buckets", "table", "lam", "out", "lse",
+                                      "dout", "dqkv", "dtable", "dlam", "workspace")]
+        + [("workspace_bytes", c_sz)])
+
+
 # name -> (restype, argtypes); must list every symbol of include/ptv3_b200.h
 SIGNATURES = {
     "ptv3_last_error": (ctypes.c_char_p, []),
@@ -80,6 +93,16 @@ SIGNATURES = {
                                    c_int, c_f32, c_int, c_int, c_ptr, c_ptr]),
     "ptv3_attention_rpe_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_i64, c_int,
                                        c_int, c_int, c_int, c_f32, c_int, c_ptr]),
+    "ptv3_patch_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_int, c_int, c_ptr,
+                                c_ptr, c_ptr]),
+    "ptv3_patch_attention_fwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),
+    "ptv3_patch_attention_workspace_bytes": (c_sz, [ctypes.POINTER(PatchAttentionArgs)]),
+    "ptv3_patch_attention_bwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),
+    "ptv3_qk_norm_rope_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_i64, c_int, c_int, c_f32, c_f64,
+                                      c_int, c_ptr]),
+    "ptv3_qk_norm_rope_workspace_bytes": (c_sz, [c_i64, c_int, c_int]),
+    "ptv3_qk_norm_rope_bwd": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int,
+                                      c_int, c_f32, c_f64, c_int, c_ptr, c_sz, c_ptr]),
     "ptv3_kmap_workspace_bytes": (c_sz, [c_i64]),
     "ptv3_status_reset": (c_int, [c_ptr, c_ptr]),
     "ptv3_host_wait": (c_int, [c_ptr, c_ptr]),

@@ -1,0 +1,350 @@
+// Patch attention with a learned relative position bias, and differential patch attention: entry points, the map from padded rows
+// to points, and the sums behind the backward pass (patch_attn.cuh has the mathematics).
+#include "patch_attn.cuh"
+#include "../../include/ptv3_b200.h"
+
+namespace ptv3 {
+
+// ---- rows of a plan ---------------------------------------------------------------------------------------
+// Points are looked up once (rows[P] = order[pad[P]], or -1 - that where unpad[pad[P]] != P: the row was borrowed by
+// another patch and answers for nothing), so that the attention kernels load one word per row and not three in a chain.
+// Keys and values of a borrowed row have a gradient all the same, and a point has at most one such row beside its
+// own: both get a row of the backward pass's side buffer (slots 2 i and 2 i + 1).
+__global__ void __launch_bounds__(256) patch_rows_kernel(const int64_t* order, const int64_t* pad, const int64_t* unpad,
+                                                         const int32_t* cu, int n, int n_pad, int n_seq, int max_seqlen,
+                                                         const int32_t* buckets, int n_entries, int num, int32_t* rows,
+                                                         int32_t* slot, int32_t* slot_point, int32_t* taken,
+                                                         uint32_t* status)
+{
+    bool bad = false;
+    const int n_slots = n_pad - n;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < max(max(n_pad, n_seq + 1), n_entries);
+         i += gridDim.x * blockDim.x) {
+        if (i < n_pad) {
+            const int64_t pd = pad[i];
+            const bool in = pd >= 0 && pd < n;
+            const int64_t p = in ? order[pd] : -1, own = in ? unpad[pd] : -1;
+            const bool good = p >= 0 && p < n && own >= 0 && own < n_pad;
+            bad |= !good;
+            int32_t row = -1;
+            if (good) {
+                row = own == i ? (int32_t)p : -1 - (int32_t)p;
+                if (own != i && n_slots == 0) {
+                    bad = true;
+                } else if (own != i) {
+                    const int s = atomicAdd(taken, 1);
+                    bad |= pad[own] != pd || s >= n_slots;
+                    if (pad[own] == pd && s < n_slots) {
+                        slot[i] = 2 * s + 1;
+                        // (a point with two borrowed rows has no place for the second)
+                        bad |= atomicCAS(slot + own, -1, 2 * s) != -1;
+                        slot_point[s] = (int32_t)p;
+                    }
+                }
+            }
+            rows[i] = row;
+        }
+        // every point has one row that answers for it
+        if (i < n) bad |= unpad[i] < 0 || unpad[i] >= n_pad || pad[unpad[i]] != i;
+        if (i < n_seq) bad |= cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] - cu[i] > max_seqlen || (i == 0 && cu[0] != 0);
+        if (i == n_seq) bad |= cu[n_seq] != n_pad;
+        if (i < n_entries) bad |= buckets[i] < 0 || buckets[i] >= num;
+    }
+    if (bad && status) atomicOr(status, PTV3_STATUS_BAD_INDEX);
+}
+
+// ---- gradients of keys and values with a borrowed copy ------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void pa_store(T* p, float v);
+template <> __device__ __forceinline__ void pa_store<float>(float* p, float v) { *p = v; }
+template <> __device__ __forceinline__ void pa_store<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) patch_shared_kernel(const float* shared, const int32_t* slot_point, int n_slots, int C,
+                                                           T* dqkv)
+{
+    const int64_t total = (int64_t)n_slots * 2 * C;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t s = i / (2 * C), c = i % (2 * C);
+        const int p = slot_point[s];
+        if (p >= 0) pa_store(dqkv + (int64_t)p * 3 * C + C + c, shared[4 * C * s + c] + shared[4 * C * s + 2 * C + c]);
+    }
+}
+
+// ---- sums over blocks, in a fixed order ------------------------------------------------------------------------
+constexpr int PA_FOLD = 64;      // rows added by a block of the first step
+
+// out[block][i] = sum of PA_FOLD rows of in
+__global__ void __launch_bounds__(256) patch_fold_kernel(const float* in, int64_t rows, int width, float* out)
+{
+    const int64_t first = (int64_t)blockIdx.x * PA_FOLD;
+    const int count = (int)min((int64_t)PA_FOLD, rows - first);
+    const int i = blockIdx.y * 256 + threadIdx.x;
+    if (i >= width) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int r = 0; r < count; ++r) v += in[(first + r) * width + i];
+    out[(int64_t)blockIdx.x * width + i] = v;
+}
+
+// One axis and head: sums of all rows by offset, then by bucket.
+__global__ void __launch_bounds__(256) patch_table_kernel(const float* in, int64_t rows, int H, int bnd, int num,
+                                                          const int32_t* buckets, void* dtable, int bf16)
+{
+    __shared__ float sum[2 * PA_MAX_BOUND + 1];
+    __shared__ int bucket[2 * PA_MAX_BOUND + 1];
+    const int axis = blockIdx.x, h = blockIdx.y, ne = 2 * bnd + 1;
+    const int64_t width = (int64_t)H * 3 * ne;
+    for (int e = threadIdx.x; e < ne; e += 256) {
+        float v = 0.f;
+#pragma unroll 4
+        for (int64_t r = 0; r < rows; ++r) v += in[r * width + (h * 3 + axis) * ne + e];
+        sum[e] = v;
+        bucket[e] = buckets ? min(max(buckets[e], 0), num - 1) : e;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < num; b += 256) {
+        float v = 0.f;
+        for (int e = 0; e < ne; ++e)
+            if (bucket[e] == b) v += sum[e];
+        const int at = (axis * num + b) * H + h;
+        if (bf16) pa_store((__nv_bfloat16*)dtable + at, v);
+        else pa_store((float*)dtable + at, v);
+    }
+}
+
+// -sum of delta_2 over all rows, a head per block row; `parts` blocks leave partial sums, one block adds them
+__global__ void __launch_bounds__(256) patch_lam_kernel(const float* delta, int n_pad, int H, int parts, float* partial,
+                                                        void* dlam, int bf16)
+{
+    __shared__ float warp_sum[8];
+    const int h = blockIdx.y;
+    float v = 0.f;
+    if (dlam) {
+        for (int i = threadIdx.x; i < parts; i += 256) v -= partial[h * parts + i];
+    } else {
+        const float* row = delta + (int64_t)(2 * h + 1) * n_pad;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n_pad; i += (int64_t)parts * 256) v += row[i];
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 31) == 0) warp_sum[threadIdx.x / 32] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        v = 0.f;
+        for (int w = 0; w < 8; ++w) v += warp_sum[w];
+        if (!dlam) partial[h * parts + blockIdx.x] = v;
+        else if (bf16) pa_store((__nv_bfloat16*)dlam + h, v);
+        else pa_store((float*)dlam + h, v);
+    }
+}
+
+// (a caller's patch size may be more than there is)
+static int longest(const ptv3_patch_attention_args* p)
+{
+    return (int)(p->max_seqlen < p->n_pad ? p->max_seqlen : p->n_pad);
+}
+// blocks of queries of the longest sequence
+static int patch_tiles(const ptv3_patch_attention_args* p)
+{
+    return ceil_div(longest(p), patch_fma_rows(p->channels / p->heads));
+}
+
+struct PatchWorkspace {
+    float *delta, *shared, *bins, *folded, *partial;
+    size_t bytes;
+    int64_t blocks;      // of the pass over rows, heads apart
+    int parts;
+};
+
+static PatchWorkspace carve(const ptv3_patch_attention_args* p)
+{
+    Carver c(p->workspace);
+    PatchWorkspace w = {};
+    w.blocks = (int64_t)p->n_seq * patch_tiles(p);
+    w.parts = ceil_div(p->n_pad, 4096);
+    w.delta = c.take<float>((size_t)p->heads * p->maps * p->n_pad);
+    w.shared = c.take<float>((size_t)(p->n_pad - p->n) * 4 * p->channels);
+    if (p->dtable) {
+        const size_t width = (size_t)p->heads * 3 * (2 * p->pos_bnd + 1);
+        w.bins = c.take<float>((size_t)w.blocks * width);
+        w.folded = c.take<float>((size_t)ceil_div(w.blocks, PA_FOLD) * width);
+    }
+    if (p->dlam) w.partial = c.take<float>((size_t)p->heads * w.parts);
+    w.bytes = c.off;
+    return w;
+}
+
+static int check_sizes(const ptv3_patch_attention_args* p, const char* what)
+{
+    PTV3_REQUIRE(p != nullptr, PTV3_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    PTV3_REQUIRE(p->n >= 0 && p->n_pad >= p->n && p->n_seq >= 0 && p->max_seqlen >= 1 && p->channels >= 1 && p->heads >= 1 &&
+                     p->channels % p->heads == 0 && (p->maps == 1 || p->maps == 2),
+                 PTV3_ERR_INVALID_ARGUMENT, "%s: bad sizes", what);
+    const int width = p->channels / p->heads;
+    PTV3_REQUIRE(width == 16 || width == 32 || width == 64, PTV3_ERR_UNSUPPORTED,
+                 "%s: heads of %d values (supported: 16, 32, 64)", what, width);
+    PTV3_REQUIRE(p->dtype == PTV3_DTYPE_F32 || p->dtype == PTV3_DTYPE_BF16, PTV3_ERR_UNSUPPORTED, "%s: dtype %d", what,
+                 p->dtype);
+    // half of each: a point has at most two rows, and their slots are numbered in 32 bits too
+    PTV3_REQUIRE(p->n_pad < (1ll << 30) && p->n_seq < (1 << 30), PTV3_ERR_UNSUPPORTED, "%s: more than 2^30 rows", what);
+    if (p->maps == 2) {
+        PTV3_REQUIRE(!p->grid_coord && !p->table, PTV3_ERR_UNSUPPORTED, "%s: no bias with two maps", what);
+        PTV3_REQUIRE(p->lam_dtype == PTV3_DTYPE_F32 || p->lam_dtype == PTV3_DTYPE_BF16, PTV3_ERR_UNSUPPORTED,
+                     "%s: dtype %d of lam", what, p->lam_dtype);
+    } else {
+        PTV3_REQUIRE(p->n == 0 || !p->grid_coord == !p->table, PTV3_ERR_INVALID_ARGUMENT,
+                     "%s: a bias needs both coordinates and a table", what);
+    }
+    if (p->table) {
+        PTV3_REQUIRE(p->pos_bnd >= 0 && p->pos_bnd <= PA_MAX_BOUND, PTV3_ERR_UNSUPPORTED, "%s: pos_bnd %d outside [0, %d]",
+                     what, p->pos_bnd, PA_MAX_BOUND);
+        PTV3_REQUIRE(p->buckets ? p->num_buckets >= 1 && p->num_buckets <= 2 * p->pos_bnd + 1
+                                : p->num_buckets == 2 * p->pos_bnd + 1,
+                     PTV3_ERR_INVALID_ARGUMENT, "%s: %d buckets of %d offsets", what, p->num_buckets, 2 * p->pos_bnd + 1);
+        PTV3_REQUIRE(p->table_dtype == PTV3_DTYPE_F32 || p->table_dtype == PTV3_DTYPE_BF16, PTV3_ERR_UNSUPPORTED,
+                     "%s: dtype %d of the table", what, p->table_dtype);
+    }
+    PTV3_REQUIRE((int64_t)p->n_seq * patch_tiles(p) * p->heads < (1ll << 31), PTV3_ERR_UNSUPPORTED,
+                 "%s: too many blocks (%d sequences of up to %d rows, %d heads)", what, p->n_seq, longest(p), p->heads);
+    return PTV3_OK;
+}
+
+static PatchArgs device_args(const ptv3_patch_attention_args* p)
+{
+    PatchArgs a = {};
+    a.qkv = p->qkv;
+    a.out = p->out;
+    a.rows = p->rows;
+    a.slot = p->n_pad > p->n ? p->rows + p->n_pad : nullptr;
+    a.cu = p->cu_seqlens;
+    a.n_pad = (int)p->n_pad;
+    a.n_seq = p->n_seq;
+    a.max_seqlen = p->max_seqlen;
+    a.tiles = patch_tiles(p);
+    a.C = p->channels;
+    a.H = p->heads;
+    a.scale = p->scale;
+    a.grid = p->grid_coord;
+    a.table = p->table;
+    a.buckets = p->buckets;
+    a.num = p->num_buckets;
+    a.bnd = p->pos_bnd;
+    a.table_bf16 = p->table_dtype == PTV3_DTYPE_BF16;
+    while (a.copies_log2 < 5 && (3 * (2 * a.bnd + 1)) << (a.copies_log2 + 1) << 2 <= PA_TABLE_BYTES) ++a.copies_log2;
+    a.lam = p->lam;
+    a.lam_bf16 = p->lam_dtype == PTV3_DTYPE_BF16;
+    a.lse = p->lse;
+    return a;
+}
+
+}  // namespace ptv3
+
+using namespace ptv3;
+
+extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
+                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* buckets, int pos_bnd,
+                               int num_buckets, int32_t* rows, uint32_t* status, void* stream)
+{
+    PTV3_REQUIRE(n >= 0 && n_pad >= n && n_seq >= 0 && max_seqlen >= 1 && n_pad < (1ll << 30) && n_seq < (1 << 30),
+                 PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: bad sizes");
+    if (n == 0) return PTV3_OK;
+    PTV3_REQUIRE(order && pad && unpad && cu_seqlens && rows, PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: null pointer");
+    PTV3_REQUIRE(n_pad <= 2 * n, PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: %lld rows of %lld points", (long long)n_pad,
+                 (long long)n);
+    const int borrowed = (int)(n_pad - n);
+    int32_t *slot = rows + n_pad, *slot_point = slot + n_pad, *taken = slot_point + borrowed;
+    if (borrowed) {
+        // slots and their points -1, the counter 0
+        cudaError_t e = cudaMemsetAsync(slot, 0xff, (size_t)(n_pad + borrowed) * 4, (cudaStream_t)stream);
+        if (e == cudaSuccess) e = cudaMemsetAsync(taken, 0, 4, (cudaStream_t)stream);
+        PTV3_REQUIRE(e == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_rows: %s", cudaGetErrorString(e));
+    }
+    const int entries = buckets ? 2 * pos_bnd + 1 : 0;
+    const int64_t most = n_pad > n_seq + 1 ? n_pad : n_seq + 1;
+    patch_rows_kernel<<<ceil_div(most, 256), 256, 0, (cudaStream_t)stream>>>(
+        order, pad, unpad, cu_seqlens, (int)n, (int)n_pad, n_seq, max_seqlen, buckets, entries, num_buckets, rows, slot,
+        slot_point, taken, status);
+    count_launches(1);
+    return check_launch("ptv3_patch_rows");
+}
+
+extern "C" int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* p, void* stream)
+{
+    const int rc = check_sizes(p, "ptv3_patch_attention_fwd");
+    if (rc != PTV3_OK) return rc;
+    if (p->n == 0 || p->n_seq == 0) return PTV3_OK;
+    PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || p->lam), PTV3_ERR_INVALID_ARGUMENT,
+                 "ptv3_patch_attention_fwd: null pointer");
+    PatchArgs a = device_args(p);
+    const int width = a.C / a.H;
+    return launch_patch_fma(a, width, p->maps, p->dtype, PA_FWD, (cudaStream_t)stream);
+}
+
+extern "C" size_t ptv3_patch_attention_workspace_bytes(const ptv3_patch_attention_args* p)
+{
+    if (check_sizes(p, "ptv3_patch_attention_workspace_bytes") != PTV3_OK) return 0;
+    ptv3_patch_attention_args q = *p;
+    q.workspace = nullptr;
+    return carve(&q).bytes;
+}
+
+extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void* stream)
+{
+    int rc = check_sizes(p, "ptv3_patch_attention_bwd");
+    if (rc != PTV3_OK) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    PatchArgs a = device_args(p);
+    const int width = a.C / a.H;
+    if (p->n > 0 && p->n_seq > 0)
+        PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->lse && p->dout && p->dqkv && (p->maps == 1 || p->lam),
+                     PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_bwd: null pointer");
+    PTV3_REQUIRE((!p->dtable || p->table) && (!p->dlam || p->maps == 2), PTV3_ERR_INVALID_ARGUMENT,
+                 "ptv3_patch_attention_bwd: a gradient without its parameter");
+    const PatchWorkspace w = carve(p);
+    PTV3_REQUIRE(w.bytes == 0 || (p->workspace && p->workspace_bytes >= w.bytes), PTV3_ERR_WORKSPACE,
+                 "ptv3_patch_attention_bwd: workspace of %zu bytes, %zu needed", p->workspace_bytes, w.bytes);
+    const bool any = p->n > 0 && p->n_seq > 0;
+    if (any) {
+        a.dout = p->dout;
+        a.dqkv = p->dqkv;
+        a.delta = w.delta;
+        a.shared = w.shared;
+        a.bins = w.bins;
+        if ((rc = launch_patch_fma(a, width, p->maps, p->dtype, PA_ROWS, s)) != PTV3_OK) return rc;
+        if ((rc = launch_patch_fma(a, width, p->maps, p->dtype, PA_COLS, s)) != PTV3_OK) return rc;
+    }
+    const int borrowed = (int)(p->n_pad - p->n);
+    if (any && borrowed) {
+        const int32_t* slot_point = p->rows + 2 * p->n_pad;
+        const int64_t total = (int64_t)borrowed * 2 * a.C;
+        const int blocks = (int)(total > 256ll * 8 * SMS * 16 ? 8 * SMS * 16 : ceil_div(total, 256));
+        if (p->dtype == PTV3_DTYPE_F32)
+            patch_shared_kernel<float><<<blocks, 256, 0, s>>>(w.shared, slot_point, borrowed, a.C, (float*)p->dqkv);
+        else
+            patch_shared_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(w.shared, slot_point, borrowed, a.C,
+                                                                       (__nv_bfloat16*)p->dqkv);
+        count_launches(1);
+    }
+    if (p->dtable) {
+        const int64_t rows = any ? w.blocks : 0;
+        const int wide = a.H * 3 * (2 * a.bnd + 1), folded = any ? ceil_div(rows, PA_FOLD) : 0;
+        if (folded) {
+            patch_fold_kernel<<<dim3(folded, ceil_div(wide, 256)), 256, 0, s>>>(w.bins, rows, wide, w.folded);
+            count_launches(1);
+        }
+        patch_table_kernel<<<dim3(3, a.H), 256, 0, s>>>(w.folded, folded, a.H, a.bnd, a.num, a.buckets, p->dtable,
+                                                        a.table_bf16);
+        count_launches(1);
+    }
+    if (p->dlam) {
+        const int parts = any ? w.parts : 0;
+        if (parts) {
+            patch_lam_kernel<<<dim3(parts, a.H), 256, 0, s>>>(w.delta, a.n_pad, a.H, parts, w.partial, nullptr, 0);
+            count_launches(1);
+        }
+        patch_lam_kernel<<<dim3(1, a.H), 256, 0, s>>>(w.delta, a.n_pad, a.H, parts, w.partial, p->dlam, a.lam_bf16);
+        count_launches(1);
+    }
+    return check_launch("ptv3_patch_attention_bwd");
+}

@@ -1,0 +1,444 @@
+// Patch attention with bias or of two maps, forward and backward, in fp32 arithmetic on CUDA cores (patch_attn.cuh
+// has the mathematics): a thread owns a query (or, in the pass over columns, a key), the other side comes through shared memory
+// in chunks that all threads read at the same address.  Heads of 64 are shared by two neighbouring threads, so that
+// accumulators stay in registers.
+#include "patch_attn.cuh"
+#include "convert.cuh"
+#include "mma_util.cuh"
+
+namespace ptv3 {
+
+constexpr int PF_THREADS = 128;
+constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
+constexpr int PF_STEP = 8;        // of which scores are held at a time
+
+template <int W, int MAPS>
+struct PfShape {
+    static constexpr int SPLIT = W == 64 ? 2 : 1;      // threads to a row
+    static constexpr int ROWS = PF_THREADS / SPLIT;
+    static constexpr int D = W / MAPS;                 // of a map's queries and keys
+    static constexpr int DP = D / SPLIT, WP = W / SPLIT;
+};
+
+// value i of this thread's share of a row of queries or keys: map-major, the share of a map contiguous
+template <int W, int MAPS>
+__device__ __forceinline__ constexpr int pf_dim(int i, int part)
+{
+    using S = PfShape<W, MAPS>;
+    return (i / S::DP) * S::D + part * S::DP + i % S::DP;
+}
+
+// A chunk of rows in shared memory: x (queries or keys) and y (values or gradients of the result), grid coordinates
+template <typename T, int W>
+__device__ __forceinline__ void pf_stage(const PatchArgs& a, const T* x, int64_t x_stride, const T* y, int64_t y_stride,
+                                         bool owners, int start, int nk, float (*xs)[W], float (*ys)[W], int (*gs)[4])
+{
+    for (int i = threadIdx.x; i < nk * W; i += PF_THREADS) {
+        const int j = i / W, d = i % W;
+        const int e = a.rows[start + j];
+        const int64_t p = e >= 0 ? e : -(e + 1);
+        xs[j][d] = to_f<T>(x[p * x_stride + d]);
+        ys[j][d] = owners && e < 0 ? 0.f : to_f<T>(y[p * y_stride + d]);
+    }
+    if (gs)
+        for (int i = threadIdx.x; i < nk * 3; i += PF_THREADS) {
+            const int j = i / 3, e = a.rows[start + j];
+            gs[j][i % 3] = a.grid[3 * (int64_t)(e >= 0 ? e : -(e + 1)) + i % 3];
+        }
+}
+
+// places of the three look-ups of a pair (g: coordinates of the query minus those of the key)
+__device__ __forceinline__ void pf_places(const PatchArgs& a, int gx, int gy, int gz, int copy, int (&at)[3])
+{
+    const int b = a.bnd, ne = 2 * b + 1;
+    at[0] = ((min(max(gx, -b), b) + b) << a.copies_log2) + copy;
+    at[1] = ((min(max(gy, -b), b) + b + ne) << a.copies_log2) + copy;
+    at[2] = ((min(max(gz, -b), b) + b + 2 * ne) << a.copies_log2) + copy;
+}
+
+template <int W, int MAPS>
+__device__ __forceinline__ void pf_scores(const float (&q)[PfShape<W, MAPS>::WP], const float* k, int part, float scale2,
+                                          float (&s)[MAPS])
+{
+    using S = PfShape<W, MAPS>;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::DP; ++i) v = fmaf(q[m * S::DP + i], k[m * S::D + part * S::DP + i], v);
+        if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
+        s[m] = v * scale2;
+    }
+}
+template <int W, int MAPS>
+__device__ __forceinline__ float pf_dot(const float (&x)[PfShape<W, MAPS>::WP], const float* y, int part)
+{
+    using S = PfShape<W, MAPS>;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) v = fmaf(x[i], y[part * S::WP + i], v);
+    if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v;
+}
+
+// ------------------------------------------------------------------------------------------------- forward
+template <typename T, int W, int MAPS, bool BIAS>
+__global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchArgs a)
+{
+    using S = PfShape<W, MAPS>;
+    __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
+    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
+    extern __shared__ float tab[];
+    const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
+    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    int start;
+    const int L = pa_sequence(a, seq, start);
+    const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
+    if (q0 >= L) return;
+    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
+    const int e = qi < L ? a.rows[start + qi] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
+    const T* base = (const T*)a.qkv + h * W;
+    float q[S::WP], acc[MAPS][S::WP], m[MAPS], l[MAPS];
+    int g[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) q[i] = to_f<T>(base[p * stride + pf_dim<W, MAPS>(i, part)]);
+    if (BIAS)
+        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+#pragma unroll
+    for (int k = 0; k < MAPS; ++k) {
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::WP; ++i) acc[k][i] = 0.f;
+    }
+    const float scale2 = a.scale * PA_LOG2E;
+    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
+        const int nk = min(PF_CHUNK, L - c0);
+        __syncthreads();
+        pf_stage<T, W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
+        __syncthreads();
+        for (int j0 = 0; j0 < nk; j0 += PF_STEP) {
+            float s[PF_STEP][MAPS], top[MAPS];
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) top[k] = m[k];
+#pragma unroll
+            for (int j = 0; j < PF_STEP; ++j) {
+                const int jj = min(j0 + j, nk - 1);
+                pf_scores<W, MAPS>(q, Ks[jj], part, scale2, s[j]);
+                if (BIAS) {
+                    int at[3];
+                    pf_places(a, g[0] - Gs[jj][0], g[1] - Gs[jj][1], g[2] - Gs[jj][2], copy, at);
+                    s[j][0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
+                }
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    if (j0 + j >= nk) s[j][k] = -INFINITY;
+                    top[k] = fmaxf(top[k], s[j][k]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) {
+                const float fix = fast_exp2(m[k] - top[k]);
+                m[k] = top[k];
+                l[k] *= fix;
+#pragma unroll
+                for (int i = 0; i < S::WP; ++i) acc[k][i] *= fix;
+            }
+#pragma unroll
+            for (int j = 0; j < PF_STEP; ++j) {
+                const int jj = min(j0 + j, nk - 1);
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    const float pr = fast_exp2(s[j][k] - m[k]);
+                    l[k] += pr;
+#pragma unroll
+                    for (int i = 0; i < S::WP; ++i) acc[k][i] = fmaf(pr, Vs[jj][part * S::WP + i], acc[k][i]);
+                }
+            }
+        }
+    }
+    if (qi >= L) return;
+    if (a.lse && part == 0)
+#pragma unroll
+        for (int k = 0; k < MAPS; ++k) a.lse[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = m[k] + log2f(l[k]);
+    if (e < 0) return;
+    const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
+    const float w0 = 1.f / l[0], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
+    T* op = (T*)a.out + p * a.C + h * W + part * S::WP;
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) op[i] = from_f<T>(MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0);
+}
+
+// ------------------------------------------------------------------------- backward, a thread's own query
+// The first walk over the keys gives delta, the second dQ and, where the table learns, the sums of dS by offset:
+// integers in shared memory, since integer sums do not depend on the order of the additions.  Their unit follows
+// from the largest sum of |dS| that a row of this block can have (known from the first walk: at most sum P |G| +
+// |delta|), so that no bin overflows: 2^-28 of it or less with a copy of the bins to every lane.
+template <typename T, int W, int MAPS, bool BIAS>
+__global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchArgs a)
+{
+    using S = PfShape<W, MAPS>;
+    __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
+    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
+    __shared__ float largest[PF_THREADS / 32];
+    extern __shared__ float tab[];
+    const int ne = 2 * a.bnd + 1, entries = 3 * ne;
+    int* hist = (int*)(tab + (entries << a.copies_log2));
+    const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
+    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    int start;
+    const int L = pa_sequence(a, seq, start);
+    const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
+    const bool learns = BIAS && a.bins;
+    float* sums = learns ? a.bins + ((int64_t)(seq * a.tiles + tile) * a.H + h) * entries : nullptr;
+    if (q0 >= L) {
+        if (learns)
+            for (int i = threadIdx.x; i < entries; i += PF_THREADS) sums[i] = 0.f;
+        return;
+    }
+    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
+    if (learns)
+        for (int i = threadIdx.x; i < entries << a.copies_log2; i += PF_THREADS) hist[i] = 0;
+    const int e = qi < L ? a.rows[start + qi] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
+    const T* base = (const T*)a.qkv + h * W;
+    float q[S::WP], go[S::WP], dq[S::WP], lse[MAPS], delta[MAPS], coef[MAPS], total[MAPS], r = 0.f;
+    int g[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) {
+        q[i] = to_f<T>(base[p * stride + pf_dim<W, MAPS>(i, part)]);
+        go[i] = e >= 0 ? to_f<T>(((const T*)a.dout)[p * a.C + h * W + part * S::WP + i]) : 0.f;
+        dq[i] = 0.f;
+    }
+    if (BIAS)
+        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+#pragma unroll
+    for (int k = 0; k < MAPS; ++k) {
+        // a row that answers for no point has no gradient: its probabilities are taken as nothing
+        lse[k] = e >= 0 ? a.lse[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] : INFINITY;
+        delta[k] = total[k] = 0.f;
+        coef[k] = 1.f;
+    }
+    if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
+    const float scale2 = a.scale * PA_LOG2E;
+    float unit = 0.f, per_unit = 0.f;
+    for (int walk = 0; walk < 2; ++walk) {
+        for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
+            const int nk = min(PF_CHUNK, L - c0);
+            __syncthreads();
+            pf_stage<T, W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs,
+                           BIAS ? Gs : nullptr);
+            __syncthreads();
+#pragma unroll 4
+            for (int j = 0; j < nk; ++j) {
+                float s[MAPS];
+                int at[3];
+                pf_scores<W, MAPS>(q, Ks[j], part, scale2, s);
+                if (BIAS) {
+                    pf_places(a, g[0] - Gs[j][0], g[1] - Gs[j][1], g[2] - Gs[j][2], copy, at);
+                    s[0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
+                }
+                const float G = pf_dot<W, MAPS>(go, Vs[j], part);
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    const float pr = fast_exp2(s[k] - lse[k]);
+                    if (walk == 0) {
+                        delta[k] = fmaf(pr, G, delta[k]);
+                        total[k] += pr;
+                        if (BIAS) r = fmaf(pr, fabsf(G), r);
+                    } else {
+                        const float ds = coef[k] * pr * (G - delta[k]);
+#pragma unroll
+                        for (int i = 0; i < S::DP; ++i)
+                            dq[k * S::DP + i] = fmaf(ds, Ks[j][k * S::D + part * S::DP + i], dq[k * S::DP + i]);
+                        if (learns && part == 0 && e >= 0) {
+                            const int v = __float2int_rn(ds * per_unit);
+                            atomicAdd(hist + at[0], v);
+                            atomicAdd(hist + at[1], v);
+                            atomicAdd(hist + at[2], v);
+                        }
+                    }
+                }
+            }
+        }
+        if (walk == 0) {
+            // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: 3e-7 of each at
+            // a logarithm of 10 (gradient of a table of 12 000 points, off by 1.1e-6 of its norm, 3e-7 with this)
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) {
+                const float inv = e >= 0 ? 1.f / total[k] : 0.f;
+                delta[k] *= inv;
+                coef[k] *= inv;
+                if (k == 0) r *= inv;
+            }
+        }
+        if (learns && walk == 0) {
+            float top = r + fabsf(delta[0]);
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if ((threadIdx.x & 31) == 0) largest[threadIdx.x / 32] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < PF_THREADS / 32; ++i) top = fmaxf(top, largest[i]);
+            // rows that share a copy, times the largest row; half the range is left for rounding
+            unit = top * (float)(PF_THREADS >> a.copies_log2) * (1.f / 1073741824.f);
+            per_unit = unit > 0.f ? 1.f / unit : 0.f;
+            if (!(per_unit < INFINITY)) per_unit = unit = 0.f;
+        }
+    }
+    if (qi < L) {
+        if (part == 0)
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) a.delta[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = delta[k];
+        if (e >= 0) {
+            T* dst = (T*)a.dqkv + p * stride + h * W;
+#pragma unroll
+            for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = from_f<T>(dq[i] * a.scale);
+        }
+    }
+    if (learns) {
+        __syncthreads();
+        const int copies = 1 << a.copies_log2;
+        for (int i = threadIdx.x; i < entries; i += PF_THREADS) {
+            float v = 0.f;
+            for (int c = 0; c < copies; ++c) v += (float)hist[(i << a.copies_log2) + ((c + i) & (copies - 1))];
+            sums[i] = v * unit;
+        }
+    }
+}
+
+// --------------------------------------------------------------------------- backward, a thread's own key
+template <typename T, int W, int MAPS, bool BIAS>
+__global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchArgs a)
+{
+    using S = PfShape<W, MAPS>;
+    __shared__ float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
+    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
+    __shared__ float Ls[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK];
+    extern __shared__ float tab[];
+    const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
+    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    int start;
+    const int L = pa_sequence(a, seq, start);
+    const int k0 = tile * S::ROWS, kj = k0 + threadIdx.x / S::SPLIT;
+    if (k0 >= L) return;
+    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
+    const int e = kj < L ? a.rows[start + kj] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
+    const T* base = (const T*)a.qkv + h * W;
+    float k[S::WP], v[S::WP], dk[S::WP], dv[S::WP], coef[MAPS];
+    int g[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < S::WP; ++i) {
+        k[i] = to_f<T>(base[p * stride + a.C + pf_dim<W, MAPS>(i, part)]);
+        v[i] = to_f<T>(base[p * stride + 2 * a.C + part * S::WP + i]);
+        dk[i] = dv[i] = 0.f;
+    }
+    if (BIAS)
+        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+    coef[0] = 1.f;
+    if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
+    const float scale2 = a.scale * PA_LOG2E;
+    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
+        const int nq = min(PF_CHUNK, L - c0);
+        __syncthreads();
+        pf_stage<T, W>(a, base, stride, (const T*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
+        for (int i = threadIdx.x; i < nq * MAPS; i += PF_THREADS) {
+            const int m = i / nq, j = i % nq;
+            const int64_t at = (int64_t)(h * MAPS + m) * a.n_pad + start + c0 + j;
+            Ls[m][j] = a.rows[start + c0 + j] >= 0 ? a.lse[at] : INFINITY;
+            Ds[m][j] = a.delta[at];
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int j = 0; j < nq; ++j) {
+            float s[MAPS];
+            pf_scores<W, MAPS>(k, Qs[j], part, scale2, s);
+            if (BIAS) {
+                int at[3];
+                pf_places(a, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
+                s[0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
+            }
+            const float G = pf_dot<W, MAPS>(v, Os[j], part);
+            float mix = 0.f;
+#pragma unroll
+            for (int m = 0; m < MAPS; ++m) {
+                const float pr = coef[m] * fast_exp2(s[m] - Ls[m][j]);
+                const float ds = pr * (G - Ds[m][j]);
+                mix += pr;
+#pragma unroll
+                for (int i = 0; i < S::DP; ++i)
+                    dk[m * S::DP + i] = fmaf(ds, Qs[j][m * S::D + part * S::DP + i], dk[m * S::DP + i]);
+            }
+#pragma unroll
+            for (int i = 0; i < S::WP; ++i) dv[i] = fmaf(mix, Os[j][part * S::WP + i], dv[i]);
+        }
+    }
+    if (kj >= L) return;
+    const int slot = a.slot ? a.slot[start + kj] : -1;
+    if (slot >= 0) {             // this point's other row is some other patch's: added up later
+        float* dst = a.shared + (int64_t)slot * 2 * a.C + h * W;
+#pragma unroll
+        for (int i = 0; i < S::WP; ++i) {
+            dst[pf_dim<W, MAPS>(i, part)] = dk[i] * a.scale;
+            dst[a.C + part * S::WP + i] = dv[i];
+        }
+    } else if (e >= 0) {
+        T* dst = (T*)a.dqkv + p * stride + a.C + h * W;
+#pragma unroll
+        for (int i = 0; i < S::WP; ++i) {
+            dst[pf_dim<W, MAPS>(i, part)] = from_f<T>(dk[i] * a.scale);
+            dst[a.C + part * S::WP + i] = from_f<T>(dv[i]);
+        }
+    }
+}
+
+template <typename T, int W, int MAPS, bool BIAS>
+static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
+{
+    const size_t table = BIAS ? (size_t)(3 * (2 * a.bnd + 1)) << a.copies_log2 << 2 : 0;
+    const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
+    cudaError_t err = cudaSuccess;
+    if (pass == PA_FWD) {
+        if (BIAS) err = allow_smem(patch_fma_fwd_kernel<T, W, MAPS, BIAS>);
+        if (err == cudaSuccess) patch_fma_fwd_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
+    } else if (pass == PA_ROWS) {
+        if (BIAS) err = allow_smem(patch_fma_rows_kernel<T, W, MAPS, BIAS>);
+        if (err == cudaSuccess)
+            patch_fma_rows_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table * (a.bins ? 2 : 1), stream>>>(a);
+    } else {
+        if (BIAS) err = allow_smem(patch_fma_cols_kernel<T, W, MAPS, BIAS>);
+        if (err == cudaSuccess) patch_fma_cols_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
+    }
+    PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
+    count_launches(1);
+    return check_launch("ptv3_patch_attention");
+}
+
+template <typename T, int W>
+static int launch_form(const PatchArgs& a, int maps, int pass, cudaStream_t stream)
+{
+    if (maps == 2) return launch_pass<T, W, 2, false>(a, pass, stream);
+    return a.grid ? launch_pass<T, W, 1, true>(a, pass, stream) : launch_pass<T, W, 1, false>(a, pass, stream);
+}
+
+template <typename T>
+static int launch_width(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream)
+{
+    switch (width) {
+        case 16: return launch_form<T, 16>(a, maps, pass, stream);
+        case 32: return launch_form<T, 32>(a, maps, pass, stream);
+        default: return launch_form<T, 64>(a, maps, pass, stream);
+    }
+}
+
+int patch_fma_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
+
+int launch_patch_fma(const PatchArgs& a, int width, int maps, int dtype, int pass, cudaStream_t stream)
+{
+    return dtype == PTV3_DTYPE_F32 ? launch_width<float>(a, width, maps, pass, stream)
+                                   : launch_width<__nv_bfloat16>(a, width, maps, pass, stream);
+}
+
+}  // namespace ptv3

@@ -208,6 +208,99 @@ def attention_rpe(qkv, order_row, pad, unpad, cu_seqlens, grid_coord, rpe_table,
     return out
 
 
+def qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base):
+    """See ptv3_qk_norm_rope_fwd; ``functional.qk_norm_rope`` is the checked form with gradients."""
+    _lib.require_cuda(qkv, grid, q_weight, k_weight)
+    n, c3 = qkv.shape
+    out = torch.empty_like(qkv)
+    with timed("qk_norm_rope", 2.0 * qkv.numel() * qkv.element_size()):
+        _lib.check(_lib.load().ptv3_qk_norm_rope_fwd(
+            _lib.ptr(qkv), _lib.ptr(q_weight), _lib.ptr(k_weight), _lib.dtype_id(qkv if q_weight is None else q_weight),
+            _lib.ptr(grid), _lib.ptr(out), n, c3 // 3, heads, eps, base, _lib.dtype_id(qkv), _lib.stream()),
+            "ptv3_qk_norm_rope_fwd")
+    return out
+
+
+def qk_norm_rope_bwd(qkv, dout, heads, grid, q_weight, k_weight, eps, base):
+    """Gradients (dqkv, dq_weight, dk_weight); qkv may be None without weights."""
+    _lib.require_cuda(qkv, dout, grid, q_weight, k_weight)
+    lib = _lib.load()
+    n, c3 = dout.shape
+    dqkv = torch.empty_like(dout)
+    dq = dk = ws = None
+    nbytes = 0
+    if q_weight is not None:
+        dq, dk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+        nbytes = lib.ptv3_qk_norm_rope_workspace_bytes(n, c3 // 3, heads)
+        ws = _lib.workspace(nbytes, dout.device)
+    with timed("qk_norm_rope_bwd", (2.0 + (q_weight is not None)) * dout.numel() * dout.element_size()):
+        _lib.check(lib.ptv3_qk_norm_rope_bwd(
+            _lib.ptr(qkv), _lib.ptr(q_weight), _lib.ptr(k_weight), _lib.dtype_id(dout if q_weight is None else q_weight),
+            _lib.ptr(grid), _lib.ptr(dout), _lib.ptr(dqkv), _lib.ptr(dq), _lib.ptr(dk), n, c3 // 3, heads, eps, base,
+            _lib.dtype_id(dout), _lib.ptr(ws), nbytes, _lib.stream()), "ptv3_qk_norm_rope_bwd")
+    return dqkv, dq, dk
+
+
+def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, buckets=None, pos_bnd=0, num_buckets=0, status=None):
+    """Points of the padded rows of a plan as patch_attention_fwd / _bwd read them (see ptv3_patch_rows)."""
+    _lib.require_cuda(order_row, pad, unpad, cu_seqlens, buckets, status)
+    n, n_pad = order_row.numel(), pad.numel()
+    rows = torch.empty(2 * n_pad + (n_pad - n) + 1, dtype=torch.int32, device=pad.device)
+    _lib.check(_lib.load().ptv3_patch_rows(_lib.ptr(order_row), _lib.ptr(pad), _lib.ptr(unpad), _lib.ptr(cu_seqlens), n,
+                                           n_pad, cu_seqlens.numel() - 1, int(max_seqlen), _lib.ptr(buckets),
+                                           int(pos_bnd), int(num_buckets), _lib.ptr(rows), _lib.ptr(status),
+                                           _lib.stream()), "ptv3_patch_rows")
+    return rows
+
+
+def _patch_attention_args(qkv, rows, n_pad, cu, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num):
+    a = _lib.PatchAttentionArgs()
+    a.n, a.n_pad, a.n_seq, a.max_seqlen = qkv.shape[0], n_pad, cu.numel() - 1, max_seqlen
+    a.channels, a.heads, a.maps, a.dtype, a.scale = qkv.shape[1] // 3, heads, maps, _lib.dtype_id(qkv), scale
+    a.qkv, a.rows, a.cu_seqlens = qkv.data_ptr(), rows.data_ptr(), cu.data_ptr()
+    if maps == 2:
+        a.lam, a.lam_dtype = param.data_ptr(), _lib.dtype_id(param)
+    elif param is not None:
+        a.table, a.table_dtype, a.grid_coord = param.data_ptr(), _lib.dtype_id(param), grid.data_ptr()
+        a.pos_bnd, a.num_buckets, a.buckets = pos_bnd, num, _lib.ptr(buckets)
+    return a
+
+
+def patch_attention_fwd(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps=1, param=None, grid=None,
+                        buckets=None, pos_bnd=0, num_buckets=0, want_lse=False):
+    """(out (N, C), lse or None) of ptv3_patch_attention_fwd; param: the table with maps = 1, lam with maps = 2.
+    ``functional.attention_bias`` and ``functional.attention_diff`` are the checked forms with gradients."""
+    _lib.require_cuda(qkv, rows, cu_seqlens, param, grid, buckets)
+    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
+                              num_buckets)
+    out = torch.empty((qkv.shape[0], a.channels), dtype=qkv.dtype, device=qkv.device)
+    lse = torch.empty((heads * maps, n_pad), dtype=torch.float32, device=qkv.device) if want_lse else None
+    a.out, a.lse = out.data_ptr(), _lib.ptr(lse)
+    with timed("patch_attention"):
+        _lib.check(_lib.load().ptv3_patch_attention_fwd(ctypes.byref(a), _lib.stream()), "ptv3_patch_attention_fwd")
+    return out, lse
+
+
+def patch_attention_bwd(qkv, rows, n_pad, cu_seqlens, lse, dout, heads, max_seqlen, scale, maps=1, param=None, grid=None,
+                        buckets=None, pos_bnd=0, num_buckets=0, want_param=True):
+    """Gradients (dqkv, gradient of param or None) of patch_attention_fwd."""
+    _lib.require_cuda(qkv, rows, cu_seqlens, lse, dout, param, grid, buckets)
+    lib = _lib.load()
+    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
+                              num_buckets)
+    dqkv = torch.empty_like(qkv)
+    dparam = torch.empty_like(param) if want_param and param is not None else None
+    a.lse, a.dout, a.dqkv = lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr()
+    if dparam is not None:
+        setattr(a, "dlam" if maps == 2 else "dtable", dparam.data_ptr())
+    nbytes = lib.ptv3_patch_attention_workspace_bytes(ctypes.byref(a))
+    ws = _lib.workspace(nbytes, qkv.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    with timed("patch_attention_bwd"):
+        _lib.check(lib.ptv3_patch_attention_bwd(ctypes.byref(a), _lib.stream()), "ptv3_patch_attention_bwd")
+    return dqkv, dparam
+
+
 def batch_indices(offset, n, grid_coord=None, want_batch=True):
     """(batch, indices): the scene index of each of the n points (int64) and, with grid_coord, the
     (n, 4) int32 rows (batch, x, y, z) of the sparse tensor; one kernel, no device read."""

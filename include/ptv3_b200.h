@@ -194,16 +194,17 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
 /*
  * Points of the padded rows of a plan, for ptv3_patch_attention_fwd / _bwd, and a look at the plan: every index in range,
  * every point with one row that answers for it and at most one borrowed one (as ptv3_pad_plan writes plans), sequences that
- * follow one another from row 0 to n_pad and are no longer than max_seqlen.  With `buckets` (2 pos_bnd + 1 int32) those
- * are looked at too: all in [0, num_buckets).
+ * follow one another from row 0 to n_pad and are no longer than max_seqlen.  What a bias reads is looked at too, where given:
+ * `grid_coord` (n x 3 int32) within 2^22 of zero, `buckets` (2 pos_bnd + 1 int32) in [0, num_buckets).
  *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30
  *   rows        2 * n_pad + (n_pad - n) + 1 int32, written
  *   status      one uint32 or NULL: PTV3_STATUS_BAD_INDEX where something does not hold (the calls that read `rows` then
  *               stay within their tensors, and what they leave is undefined)
  */
 int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
-                    int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* buckets, int pos_bnd,
-                    int num_buckets, int32_t* rows, uint32_t* status, void* stream);
+                    int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord,
+                    const int32_t* buckets, int pos_bnd, int num_buckets, int32_t* rows, uint32_t* status,
+                    void* stream);
 
 /*
  * Patch attention that can be trained: with a learned relative position bias by buckets (maps = 1, grid_coord and
@@ -217,7 +218,7 @@ int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unp
  * within each patch; rows borrowed by a patch are keys there and answer for nothing.  W in {16, 32, 64}.  The gradients do
  * not depend on the order in which anything runs.  A workspace or an `lse` belongs to one call in flight: graphs that may run at
  * the same time need one each.
- *   qkv, dqkv   n x 3*channels; out, dout n x channels; dtype PTV3_DTYPE_*
+ *   qkv, dqkv   n x 3*channels; out, dout n x channels; 16-byte aligned, dtype PTV3_DTYPE_*
  *   rows        of ptv3_patch_rows
  *   table       3 * num_buckets x heads, lam heads: fp32 or bf16 (table_dtype, lam_dtype); gradients in the same type
  *   lse         heads * maps * n_pad fp32: written by _fwd (may be NULL there), read by _bwd

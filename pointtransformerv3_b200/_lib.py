@@ -93,8 +93,8 @@ SIGNATURES = {
                                    c_int, c_f32, c_int, c_int, c_ptr, c_ptr]),
     "ptv3_attention_rpe_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_i64, c_int,
                                        c_int, c_int, c_int, c_f32, c_int, c_ptr]),
-    "ptv3_patch_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_int, c_int, c_ptr,
-                                c_ptr, c_ptr]),
+    "ptv3_patch_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr, c_int, c_int,
+                                c_ptr, c_ptr, c_ptr]),
     "ptv3_patch_attention_fwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),
     "ptv3_patch_attention_workspace_bytes": (c_sz, [ctypes.POINTER(PatchAttentionArgs)]),
     "ptv3_patch_attention_bwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),

@@ -12,7 +12,8 @@ namespace ptv3 {
 // own: both get a row of the backward pass's side buffer (slots 2 i and 2 i + 1).
 __global__ void __launch_bounds__(256) patch_rows_kernel(const int64_t* order, const int64_t* pad, const int64_t* unpad,
                                                          const int32_t* cu, int n, int n_pad, int n_seq, int max_seqlen,
-                                                         const int32_t* buckets, int n_entries, int num, int32_t* rows,
+                                                         const int32_t* grid, const int32_t* buckets, int n_entries, int num,
+                                                         int32_t* rows,
                                                          int32_t* slot, int32_t* slot_point, int32_t* taken,
                                                          uint32_t* status)
 {
@@ -45,7 +46,11 @@ __global__ void __launch_bounds__(256) patch_rows_kernel(const int64_t* order, c
             rows[i] = row;
         }
         // every point has one row that answers for it
-        if (i < n) bad |= unpad[i] < 0 || unpad[i] >= n_pad || pad[unpad[i]] != i;
+        if (i < n) {
+            bad |= unpad[i] < 0 || unpad[i] >= n_pad || pad[unpad[i]] != i;
+            if (grid)
+                for (int c = 0; c < 3; ++c) bad |= grid[3 * (int64_t)i + c] < -PA_MAX_COORD || grid[3 * (int64_t)i + c] > PA_MAX_COORD;
+        }
         if (i < n_seq) bad |= cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] - cu[i] > max_seqlen || (i == 0 && cu[0] != 0);
         if (i == n_seq) bad |= cu[n_seq] != n_pad;
         if (i < n_entries) bad |= buckets[i] < 0 || buckets[i] >= num;
@@ -147,7 +152,14 @@ static int longest(const ptv3_patch_attention_args* p)
 // blocks of queries of the longest sequence
 static int patch_tiles(const ptv3_patch_attention_args* p)
 {
-    return ceil_div(longest(p), patch_fma_rows(p->channels / p->heads));
+    return ceil_div(longest(p), p->dtype == PTV3_DTYPE_BF16 ? patch_mma_rows() : patch_fma_rows(p->channels / p->heads));
+}
+
+static int launch_patch(const ptv3_patch_attention_args* p, const PatchArgs& a, int pass, cudaStream_t stream)
+{
+    const int width = p->channels / p->heads;
+    return p->dtype == PTV3_DTYPE_BF16 ? launch_patch_mma(a, width, p->maps, pass, stream)
+                                       : launch_patch_fma(a, width, p->maps, pass, stream);
 }
 
 struct PatchWorkspace {
@@ -243,7 +255,7 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
 using namespace ptv3;
 
 extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
-                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* buckets, int pos_bnd,
+                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord, const int32_t* buckets, int pos_bnd,
                                int num_buckets, int32_t* rows, uint32_t* status, void* stream)
 {
     PTV3_REQUIRE(n >= 0 && n_pad >= n && n_seq >= 0 && max_seqlen >= 1 && n_pad < (1ll << 30) && n_seq < (1 << 30),
@@ -263,7 +275,7 @@ extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const i
     const int entries = buckets ? 2 * pos_bnd + 1 : 0;
     const int64_t most = n_pad > n_seq + 1 ? n_pad : n_seq + 1;
     patch_rows_kernel<<<ceil_div(most, 256), 256, 0, (cudaStream_t)stream>>>(
-        order, pad, unpad, cu_seqlens, (int)n, (int)n_pad, n_seq, max_seqlen, buckets, entries, num_buckets, rows, slot,
+        order, pad, unpad, cu_seqlens, (int)n, (int)n_pad, n_seq, max_seqlen, grid_coord, buckets, entries, num_buckets, rows, slot,
         slot_point, taken, status);
     count_launches(1);
     return check_launch("ptv3_patch_rows");
@@ -274,11 +286,12 @@ extern "C" int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* p, void
     const int rc = check_sizes(p, "ptv3_patch_attention_fwd");
     if (rc != PTV3_OK) return rc;
     if (p->n == 0 || p->n_seq == 0) return PTV3_OK;
+    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
+                 "ptv3_patch_attention_fwd: unaligned rows");
     PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || p->lam), PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_fwd: null pointer");
     PatchArgs a = device_args(p);
-    const int width = a.C / a.H;
-    return launch_patch_fma(a, width, p->maps, p->dtype, PA_FWD, (cudaStream_t)stream);
+    return launch_patch(p, a, PA_FWD, (cudaStream_t)stream);
 }
 
 extern "C" size_t ptv3_patch_attention_workspace_bytes(const ptv3_patch_attention_args* p)
@@ -295,10 +308,11 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
     if (rc != PTV3_OK) return rc;
     cudaStream_t s = (cudaStream_t)stream;
     PatchArgs a = device_args(p);
-    const int width = a.C / a.H;
     if (p->n > 0 && p->n_seq > 0)
         PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->lse && p->dout && p->dqkv && (p->maps == 1 || p->lam),
                      PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_bwd: null pointer");
+    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->dout | (uintptr_t)p->dqkv) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
+                 "ptv3_patch_attention_bwd: unaligned rows");
     PTV3_REQUIRE((!p->dtable || p->table) && (!p->dlam || p->maps == 2), PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_bwd: a gradient without its parameter");
     const PatchWorkspace w = carve(p);
@@ -311,8 +325,8 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
         a.delta = w.delta;
         a.shared = w.shared;
         a.bins = w.bins;
-        if ((rc = launch_patch_fma(a, width, p->maps, p->dtype, PA_ROWS, s)) != PTV3_OK) return rc;
-        if ((rc = launch_patch_fma(a, width, p->maps, p->dtype, PA_COLS, s)) != PTV3_OK) return rc;
+        if ((rc = launch_patch(p, a, PA_ROWS, s)) != PTV3_OK) return rc;
+        if ((rc = launch_patch(p, a, PA_COLS, s)) != PTV3_OK) return rc;
     }
     const int borrowed = (int)(p->n_pad - p->n);
     if (any && borrowed) {

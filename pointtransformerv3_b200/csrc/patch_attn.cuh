@@ -21,6 +21,7 @@ namespace ptv3 {
 
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr int PA_MAX_BOUND = 512;
+constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
 constexpr int PA_TABLE_BYTES = 3 * 129 * 32 * 4;      // shared memory that copies of a head's table may take
 
 // What the kernels get: ptv3_patch_attention_args with the workspace carved up.
@@ -75,10 +76,11 @@ __device__ __forceinline__ void pa_load_table(const PatchArgs& a, int h, float* 
     }
 }
 
-int launch_patch_fma(const PatchArgs& a, int width, int maps, int dtype, int pass, cudaStream_t stream);
-
 enum { PA_FWD = 0, PA_ROWS = 1, PA_COLS = 2 };
-// query rows of a block of the pass over rows (what `bins` and `tiles` count in)
+// fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu); ..._rows: rows of a block, in which `tiles` counts
+int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
+int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int patch_fma_rows(int width);
+int patch_mma_rows();
 
 }  // namespace ptv3

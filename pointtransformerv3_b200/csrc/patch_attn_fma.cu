@@ -3,7 +3,6 @@
 // in chunks that all threads read at the same address.  Heads of 64 are shared by two neighbouring threads, so that
 // accumulators stay in registers.
 #include "patch_attn.cuh"
-#include "convert.cuh"
 #include "mma_util.cuh"
 
 namespace ptv3 {
@@ -29,16 +28,16 @@ __device__ __forceinline__ constexpr int pf_dim(int i, int part)
 }
 
 // A chunk of rows in shared memory: x (queries or keys) and y (values or gradients of the result), grid coordinates
-template <typename T, int W>
-__device__ __forceinline__ void pf_stage(const PatchArgs& a, const T* x, int64_t x_stride, const T* y, int64_t y_stride,
+template <int W>
+__device__ __forceinline__ void pf_stage(const PatchArgs& a, const float* x, int64_t x_stride, const float* y, int64_t y_stride,
                                          bool owners, int start, int nk, float (*xs)[W], float (*ys)[W], int (*gs)[4])
 {
     for (int i = threadIdx.x; i < nk * W; i += PF_THREADS) {
         const int j = i / W, d = i % W;
         const int e = a.rows[start + j];
         const int64_t p = e >= 0 ? e : -(e + 1);
-        xs[j][d] = to_f<T>(x[p * x_stride + d]);
-        ys[j][d] = owners && e < 0 ? 0.f : to_f<T>(y[p * y_stride + d]);
+        xs[j][d] = (x[p * x_stride + d]);
+        ys[j][d] = owners && e < 0 ? 0.f : (y[p * y_stride + d]);
     }
     if (gs)
         for (int i = threadIdx.x; i < nk * 3; i += PF_THREADS) {
@@ -82,7 +81,7 @@ __device__ __forceinline__ float pf_dot(const float (&x)[PfShape<W, MAPS>::WP], 
 }
 
 // ------------------------------------------------------------------------------------------------- forward
-template <typename T, int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchArgs a)
 {
     using S = PfShape<W, MAPS>;
@@ -98,11 +97,11 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
     const int e = qi < L ? a.rows[start + qi] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
-    const T* base = (const T*)a.qkv + h * W;
+    const float* base = (const float*)a.qkv + h * W;
     float q[S::WP], acc[MAPS][S::WP], m[MAPS], l[MAPS];
     int g[3] = {0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) q[i] = to_f<T>(base[p * stride + pf_dim<W, MAPS>(i, part)]);
+    for (int i = 0; i < S::WP; ++i) q[i] = (base[p * stride + pf_dim<W, MAPS>(i, part)]);
     if (BIAS)
         for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
 #pragma unroll
@@ -116,7 +115,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
         const int nk = min(PF_CHUNK, L - c0);
         __syncthreads();
-        pf_stage<T, W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
+        pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
         __syncthreads();
         for (int j0 = 0; j0 < nk; j0 += PF_STEP) {
             float s[PF_STEP][MAPS], top[MAPS];
@@ -165,9 +164,9 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (e < 0) return;
     const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
     const float w0 = 1.f / l[0], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
-    T* op = (T*)a.out + p * a.C + h * W + part * S::WP;
+    float* op = (float*)a.out + p * a.C + h * W + part * S::WP;
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) op[i] = from_f<T>(MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0);
+    for (int i = 0; i < S::WP; ++i) op[i] = (MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0);
 }
 
 // ------------------------------------------------------------------------- backward, a thread's own query
@@ -175,7 +174,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 // integers in shared memory, since integer sums do not depend on the order of the additions.  Their unit follows
 // from the largest sum of |dS| that a row of this block can have (known from the first walk: at most sum P |G| +
 // |delta|), so that no bin overflows: 2^-28 of it or less with a copy of the bins to every lane.
-template <typename T, int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchArgs a)
 {
     using S = PfShape<W, MAPS>;
@@ -202,13 +201,13 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
         for (int i = threadIdx.x; i < entries << a.copies_log2; i += PF_THREADS) hist[i] = 0;
     const int e = qi < L ? a.rows[start + qi] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
-    const T* base = (const T*)a.qkv + h * W;
+    const float* base = (const float*)a.qkv + h * W;
     float q[S::WP], go[S::WP], dq[S::WP], lse[MAPS], delta[MAPS], coef[MAPS], total[MAPS], r = 0.f;
     int g[3] = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < S::WP; ++i) {
-        q[i] = to_f<T>(base[p * stride + pf_dim<W, MAPS>(i, part)]);
-        go[i] = e >= 0 ? to_f<T>(((const T*)a.dout)[p * a.C + h * W + part * S::WP + i]) : 0.f;
+        q[i] = (base[p * stride + pf_dim<W, MAPS>(i, part)]);
+        go[i] = e >= 0 ? (((const float*)a.dout)[p * a.C + h * W + part * S::WP + i]) : 0.f;
         dq[i] = 0.f;
     }
     if (BIAS)
@@ -227,7 +226,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
         for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
             const int nk = min(PF_CHUNK, L - c0);
             __syncthreads();
-            pf_stage<T, W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs,
+            pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs,
                            BIAS ? Gs : nullptr);
             __syncthreads();
 #pragma unroll 4
@@ -292,9 +291,9 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) a.delta[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = delta[k];
         if (e >= 0) {
-            T* dst = (T*)a.dqkv + p * stride + h * W;
+            float* dst = (float*)a.dqkv + p * stride + h * W;
 #pragma unroll
-            for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = from_f<T>(dq[i] * a.scale);
+            for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = (dq[i] * a.scale);
         }
     }
     if (learns) {
@@ -309,7 +308,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 }
 
 // --------------------------------------------------------------------------- backward, a thread's own key
-template <typename T, int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchArgs a)
 {
     using S = PfShape<W, MAPS>;
@@ -326,13 +325,13 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
     const int e = kj < L ? a.rows[start + kj] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
-    const T* base = (const T*)a.qkv + h * W;
+    const float* base = (const float*)a.qkv + h * W;
     float k[S::WP], v[S::WP], dk[S::WP], dv[S::WP], coef[MAPS];
     int g[3] = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < S::WP; ++i) {
-        k[i] = to_f<T>(base[p * stride + a.C + pf_dim<W, MAPS>(i, part)]);
-        v[i] = to_f<T>(base[p * stride + 2 * a.C + part * S::WP + i]);
+        k[i] = (base[p * stride + a.C + pf_dim<W, MAPS>(i, part)]);
+        v[i] = (base[p * stride + 2 * a.C + part * S::WP + i]);
         dk[i] = dv[i] = 0.f;
     }
     if (BIAS)
@@ -343,7 +342,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
         const int nq = min(PF_CHUNK, L - c0);
         __syncthreads();
-        pf_stage<T, W>(a, base, stride, (const T*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
+        pf_stage<W>(a, base, stride, (const float*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
         for (int i = threadIdx.x; i < nq * MAPS; i += PF_THREADS) {
             const int m = i / nq, j = i % nq;
             const int64_t at = (int64_t)(h * MAPS + m) * a.n_pad + start + c0 + j;
@@ -385,60 +384,53 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
             dst[a.C + part * S::WP + i] = dv[i];
         }
     } else if (e >= 0) {
-        T* dst = (T*)a.dqkv + p * stride + a.C + h * W;
+        float* dst = (float*)a.dqkv + p * stride + a.C + h * W;
 #pragma unroll
         for (int i = 0; i < S::WP; ++i) {
-            dst[pf_dim<W, MAPS>(i, part)] = from_f<T>(dk[i] * a.scale);
-            dst[a.C + part * S::WP + i] = from_f<T>(dv[i]);
+            dst[pf_dim<W, MAPS>(i, part)] = (dk[i] * a.scale);
+            dst[a.C + part * S::WP + i] = (dv[i]);
         }
     }
 }
 
-template <typename T, int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
     const size_t table = BIAS ? (size_t)(3 * (2 * a.bnd + 1)) << a.copies_log2 << 2 : 0;
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
     cudaError_t err = cudaSuccess;
     if (pass == PA_FWD) {
-        if (BIAS) err = allow_smem(patch_fma_fwd_kernel<T, W, MAPS, BIAS>);
-        if (err == cudaSuccess) patch_fma_fwd_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
+        if (BIAS) err = allow_smem(patch_fma_fwd_kernel<W, MAPS, BIAS>);
+        if (err == cudaSuccess) patch_fma_fwd_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
     } else if (pass == PA_ROWS) {
-        if (BIAS) err = allow_smem(patch_fma_rows_kernel<T, W, MAPS, BIAS>);
+        if (BIAS) err = allow_smem(patch_fma_rows_kernel<W, MAPS, BIAS>);
         if (err == cudaSuccess)
-            patch_fma_rows_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table * (a.bins ? 2 : 1), stream>>>(a);
+            patch_fma_rows_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table * (a.bins ? 2 : 1), stream>>>(a);
     } else {
-        if (BIAS) err = allow_smem(patch_fma_cols_kernel<T, W, MAPS, BIAS>);
-        if (err == cudaSuccess) patch_fma_cols_kernel<T, W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
+        if (BIAS) err = allow_smem(patch_fma_cols_kernel<W, MAPS, BIAS>);
+        if (err == cudaSuccess) patch_fma_cols_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
     }
     PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
     count_launches(1);
     return check_launch("ptv3_patch_attention");
 }
 
-template <typename T, int W>
+template <int W>
 static int launch_form(const PatchArgs& a, int maps, int pass, cudaStream_t stream)
 {
-    if (maps == 2) return launch_pass<T, W, 2, false>(a, pass, stream);
-    return a.grid ? launch_pass<T, W, 1, true>(a, pass, stream) : launch_pass<T, W, 1, false>(a, pass, stream);
+    if (maps == 2) return launch_pass<W, 2, false>(a, pass, stream);
+    return a.grid ? launch_pass<W, 1, true>(a, pass, stream) : launch_pass<W, 1, false>(a, pass, stream);
 }
 
-template <typename T>
-static int launch_width(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream)
+int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream)
 {
     switch (width) {
-        case 16: return launch_form<T, 16>(a, maps, pass, stream);
-        case 32: return launch_form<T, 32>(a, maps, pass, stream);
-        default: return launch_form<T, 64>(a, maps, pass, stream);
+        case 16: return launch_form<16>(a, maps, pass, stream);
+        case 32: return launch_form<32>(a, maps, pass, stream);
+        default: return launch_form<64>(a, maps, pass, stream);
     }
 }
 
 int patch_fma_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
-
-int launch_patch_fma(const PatchArgs& a, int width, int maps, int dtype, int pass, cudaStream_t stream)
-{
-    return dtype == PTV3_DTYPE_F32 ? launch_width<float>(a, width, maps, pass, stream)
-                                   : launch_width<__nv_bfloat16>(a, width, maps, pass, stream);
-}
 
 }  // namespace ptv3

@@ -1,0 +1,759 @@
+// Patch attention with bias or of two maps, forward and backward, for bf16 on the tensor cores by mma.sync
+// (patch_attn.cuh has the mathematics).
+//
+// A CTA of eight warps owns 128 rows (queries, or keys in the pass over columns) of one patch and head, a warp 16 of
+// them; the other side streams through shared memory in chunks of 64 rows, gathered by cp.async through the row list, two
+// chunks ahead (three stages, one barrier a chunk).  Scores, probabilities and dS live in accumulator registers and are
+// the A operands of the next product as they lie; rounding to bf16 happens there (probabilities, dS) and where results
+// are stored, everything else is fp32.  Of a map there are 64 tensor FLOPs to an exponential at heads of 16: the exponential unit
+// and instruction issue set the pace, which is why the products stay on mma.sync.
+//
+// The bias: coordinates are kept times the size of a table entry in bytes, so a look-up is a subtraction with a
+// maximum, a minimum, a load and an addition; 32 copies of the table, one to a lane, keep loads and the integer
+// additions of the table's gradient free of bank conflicts.
+#include "patch_attn.cuh"
+#include "mma_util.cuh"
+
+namespace ptv3 {
+
+constexpr int PM_THREADS = 256, PM_WARPS = 8;
+constexpr int PM_ROWS = 128;       // of a CTA
+constexpr int PM_CHUNK = 64;       // rows of the other side in a stage
+constexpr int PM_STAGES = 3;
+constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
+constexpr float PM_LOWEST = -1e30f;
+
+template <int W>
+struct PmStage {
+    static constexpr int TILE = PM_CHUNK * W * 2;      // bytes of a matrix
+    static constexpr int AUX = 2 * TILE;               // two words of each map and row
+    static constexpr int GRID = AUX + 4 * PM_CHUNK * 4;
+    static constexpr int BYTES = GRID + PM_CHUNK * 16;
+};
+
+// byte offset of 16-byte chunk c of row r: chunks are exchanged so that the eight rows of an ldmatrix lie in different banks
+template <int W>
+__device__ __forceinline__ uint32_t pm_offset(int r, int c)
+{
+    constexpr int RB = 2 * W;
+    return (uint32_t)(r * RB + ((c ^ ((r * RB >> 7) & (RB / 16 - 1))) << 4));
+}
+
+__device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// Bias of a pair of points: coordinates in bytes of the table in shared memory
+struct PmBias {
+    int lo[3], hi[3];       // bounds of an entry's place, this lane's copy
+};
+__device__ __forceinline__ float pm_lds(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void pm_add_shared(uint32_t addr, int v)
+{
+    asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// The other side's rows: x and y (head h's W values of each), two words of each map (AUX), coordinates (BIAS)
+template <int W, int MAPS, bool AUX, bool BIAS>
+struct PmStream {
+    using S = PmStage<W>;
+    const PatchArgs& a;
+    const __nv_bfloat16 *x, *y;
+    int64_t xs, ys;
+    int start, L, h;
+    bool owners;             // rows of y that answer for no point are taken as zeros
+    unsigned char* smem;
+    int e, eg, ea, g[3];
+    float aux;
+
+    __device__ __forceinline__ int row_of(int chunk, int j) const
+    {
+        const int r = chunk * PM_CHUNK + j;
+        return r < L ? a.rows[start + r] : INT_MIN;
+    }
+    __device__ __forceinline__ void fetch_grid()
+    {
+        if (BIAS && threadIdx.x < PM_CHUNK && eg != INT_MIN) {
+            const int64_t p = eg >= 0 ? eg : -(eg + 1);
+#pragma unroll
+            for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+        }
+    }
+    __device__ __forceinline__ void fetch_aux(int chunk)
+    {
+        if (AUX && threadIdx.x < 2 * MAPS * PM_CHUNK) {
+            const int j = threadIdx.x % PM_CHUNK, what = threadIdx.x / PM_CHUNK, r = chunk * PM_CHUNK + j;
+            ea = row_of(chunk, j);
+            aux = 0.f;
+            if (r < L) aux = (what < MAPS ? a.lse : a.delta)[(int64_t)(h * MAPS + what % MAPS) * a.n_pad + start + r];
+        }
+    }
+    // what issue(chunk) needs in registers
+    __device__ __forceinline__ void fetch(int chunk)
+    {
+        e = row_of(chunk, threadIdx.x >> 2);
+        fetch_grid();
+        if (BIAS && threadIdx.x < PM_CHUNK) eg = row_of(chunk + 1, threadIdx.x);
+        fetch_aux(chunk);
+    }
+    __device__ __forceinline__ void issue(int chunk)
+    {
+        if (chunk * PM_CHUNK < L) {
+            unsigned char* st = smem + chunk % PM_STAGES * S::BYTES;
+            const int r = threadIdx.x >> 2;
+            const bool there = e != INT_MIN;
+            const int64_t p = !there ? 0 : e >= 0 ? e : -(e + 1);
+            constexpr int CPR = W / 8;
+#pragma unroll
+            for (int i = 0; i < CPR / 2; ++i) {
+                const int o = (threadIdx.x & 3) + 4 * i, c = o % CPR;
+                if (o < CPR) cp_async16_zfill(smem_u32(st) + pm_offset<W>(r, c), x + p * xs + 8 * c, there);
+                else cp_async16_zfill(smem_u32(st) + S::TILE + pm_offset<W>(r, c), y + p * ys + 8 * c,
+                                      there && !(owners && e < 0));
+            }
+            if (AUX && threadIdx.x < 2 * MAPS * PM_CHUNK) {
+                const bool lse = threadIdx.x / PM_CHUNK < MAPS;
+                // (rows that are not there, or answer for no point: probabilities of nothing)
+                ((float*)(st + S::AUX))[threadIdx.x] = ea >= 0 ? aux : lse ? INFINITY : 0.f;
+            }
+            if (BIAS && threadIdx.x < PM_CHUNK)
+                ((int4*)(st + S::GRID))[threadIdx.x] = make_int4(g[0] << (a.copies_log2 + 2), g[1] << (a.copies_log2 + 2),
+                                                                 g[2] << (a.copies_log2 + 2), 0);
+        }
+        cp_async_commit();
+    }
+    __device__ __forceinline__ void begin()
+    {
+        if (BIAS) {
+            g[0] = g[1] = g[2] = 0;
+            if (threadIdx.x < PM_CHUNK) eg = row_of(0, threadIdx.x);
+        }
+        fetch(0);
+        issue(0);
+        fetch(1);
+        issue(1);
+        fetch(2);
+    }
+    // chunk i has landed, its stage is returned; chunk i + 2 is on its way, what the one after needs is asked for
+    __device__ __forceinline__ const unsigned char* next(int i)
+    {
+        cp_async_wait<1>();
+        __syncthreads();
+        issue(i + 2);
+        fetch(i + 3);
+        return smem + i % PM_STAGES * S::BYTES;
+    }
+    __device__ __forceinline__ void end()
+    {
+        cp_async_wait<0>();
+        __syncthreads();
+    }
+};
+
+// ---- fragments ----------------------------------------------------------------------------------------------
+// A operand of 16 rows: W values of each, rows p0 and p1 of this lane (NULL: zeros)
+template <int W>
+__device__ __forceinline__ void pm_rows(const __nv_bfloat16* p0, const __nv_bfloat16* p1, uint32_t flip, uint32_t (&f)[W / 16][4])
+{
+    const int t = threadIdx.x & 3;
+#pragma unroll
+    for (int k = 0; k < W / 16; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f[k][2 * half] = p0 ? ((const uint32_t*)p0)[8 * k + 4 * half + t] ^ flip : 0u;
+            f[k][2 * half + 1] = p1 ? ((const uint32_t*)p1)[8 * k + 4 * half + t] ^ flip : 0u;
+        }
+}
+
+// s[m] = rows of this warp x 16 rows of the tile, transposed: MAPS sums of W / MAPS products each
+template <int W, int MAPS>
+__device__ __forceinline__ void pm_products(const uint32_t (&f)[W / 16][4], uint32_t tile, int row0, float (&s)[MAPS][2][4])
+{
+    const int lane = threadIdx.x & 31, r = row0 + (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[m][i][j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4(b, tile + pm_offset<W>(r, 2 * k + c));
+        if (W / MAPS == 8) {
+            // a map's eight values are one half of the fragment
+            mma_bf16_k8(s[0][0], f[k][0], f[k][1], b[0]);
+            mma_bf16_k8(s[0][1], f[k][0], f[k][1], b[2]);
+            mma_bf16_k8(s[MAPS - 1][0], f[k][2], f[k][3], b[1]);
+            mma_bf16_k8(s[MAPS - 1][1], f[k][2], f[k][3], b[3]);
+        } else {
+            const int m = k * 16 / (W / MAPS);
+            mma_bf16(s[m][0], f[k], b[0], b[1]);
+            mma_bf16(s[m][1], f[k], b[2], b[3]);
+        }
+    }
+}
+
+// acc += P x 16 rows of the tile (W values each); P of map m for the values of map m, or one P for all (MAPS = 1)
+template <int W, int MAPS>
+__device__ __forceinline__ void pm_accumulate(const uint32_t (&p)[MAPS][4], uint32_t tile, int row0, float (&acc)[W / 8][4])
+{
+    const int lane = threadIdx.x & 31, r = row0 + (lane & 15), c = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < W / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, tile + pm_offset<W>(r, 2 * k + c));
+        mma_bf16(acc[2 * k], p[2 * k * 8 / (W / MAPS)], b[0], b[1]);
+        mma_bf16(acc[2 * k + 1], p[(2 * k + 1) * 8 / (W / MAPS)], b[2], b[3]);
+    }
+}
+
+__device__ __forceinline__ void pm_pack(const float (&v)[2][4], uint32_t (&p)[4])
+{
+    p[0] = pack_bf16(v[0][0], v[0][1]);
+    p[1] = pack_bf16(v[0][2], v[0][3]);
+    p[2] = pack_bf16(v[1][0], v[1][1]);
+    p[3] = pack_bf16(v[1][2], v[1][3]);
+}
+
+// ---- bias ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void pm_bias_setup(const PatchArgs& a, uint32_t base, PmBias& b)
+{
+    const int copy = (threadIdx.x & ((1 << a.copies_log2) - 1)) * 4, step = a.copies_log2 + 2;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        b.lo[c] = (int)base + ((c * (2 * a.bnd + 1)) << step) + copy;
+        b.hi[c] = b.lo[c] + ((2 * a.bnd) << step);
+    }
+}
+// this lane's point, so that subtracting another's coordinates gives the entry's place
+__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PmBias& b, int e, int sign, int (&g)[3])
+{
+    const int64_t p = e >= 0 ? e : -(e + 1);
+#pragma unroll
+    for (int c = 0; c < 3; ++c)
+        g[c] = b.lo[c] + ((a.bnd + sign * a.grid[3 * p + c]) << (a.copies_log2 + 2));
+}
+// places of a pair's three entries; SIGN: the lane's point is the query (+1) or the key
+template <int SIGN>
+__device__ __forceinline__ void pm_places(const PmBias& b, const int (&mine)[3], const int4& other, uint32_t (&at)[3])
+{
+    const int o[3] = {other.x, other.y, other.z};
+#pragma unroll
+    for (int c = 0; c < 3; ++c)
+        at[c] = (uint32_t)min(__viaddmax_s32(mine[c], SIGN > 0 ? -o[c] : o[c], b.lo[c]), b.hi[c]);
+}
+__device__ __forceinline__ float pm_bias(const uint32_t (&at)[3], float s, float scale2)
+{
+    return fmaf(s, scale2, pm_lds(at[0])) + (pm_lds(at[1]) + pm_lds(at[2]));
+}
+
+struct PmPlace {
+    int h, tile, seq, start, L;
+};
+__device__ __forceinline__ PmPlace pm_place(const PatchArgs& a)
+{
+    PmPlace p;
+    p.h = blockIdx.x % a.H;
+    p.tile = blockIdx.x / a.H % a.tiles;
+    p.seq = blockIdx.x / a.H / a.tiles;
+    p.L = pa_sequence(a, p.seq, p.start);
+    return p;
+}
+
+// ------------------------------------------------------------------------------------------------- forward
+template <int W, int MAPS, bool BIAS, bool KEEP>
+__global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patch_mma_fwd_kernel(const PatchArgs a)
+{
+    using S = PmStage<W>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const PmPlace w = pm_place(a);
+    const int q0 = w.tile * PM_ROWS, L = w.L;
+    if (q0 >= L) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int r0 = q0 + (threadIdx.x / 32) * 16 + g, r1 = r0 + 8;
+    const int e0 = r0 < L ? a.rows[w.start + r0] : -1, e1 = r1 < L ? a.rows[w.start + r1] : -1;
+    const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
+    const int64_t stride = 3 * (int64_t)a.C;
+    const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
+    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false, smem};
+    in.begin();
+
+    float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+    PmBias bias;
+    int g0[3], g1[3];
+    if (BIAS) {
+        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
+        pm_bias_setup(a, smem_u32(tab), bias);
+        pm_bias_point(a, bias, e0, 1, g0);
+        pm_bias_point(a, bias, e1, 1, g1);
+    }
+    uint32_t q[W / 16][4];
+    // (of a negative scale the sign goes to the queries, so that larger products are larger scores)
+    pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr,
+               a.scale < 0.f ? 0x80008000u : 0u, q);
+    const float scale2 = fabsf(a.scale) * PA_LOG2E;
+    float o[MAPS][W / 8][4], sum[MAPS][4], l[MAPS][2], m[MAPS][2];
+#pragma unroll
+    for (int k = 0; k < MAPS; ++k) {
+        m[k][0] = m[k][1] = PM_LOWEST;
+        l[k][0] = l[k][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sum[k][j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < W / 8; ++i) o[k][i][j] = 0.f;
+        }
+    }
+    constexpr uint32_t ONES = 0x3f803f80u;
+    for (int i = 0; i * PM_CHUNK < L; ++i) {
+        const unsigned char* st = in.next(i);
+        if (!active) continue;
+        const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
+        const int4* gs = (const int4*)(st + S::GRID);
+        const int nk = L - i * PM_CHUNK;
+#pragma unroll
+        for (int j0 = 0; j0 < PM_CHUNK; j0 += 32) {
+            if (j0 >= nk) break;
+            float s[2][MAPS][2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
+                if (BIAS)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int4 k = gs[j0 + 16 * u + 8 * n + 2 * t + c];
+                            uint32_t at[3];
+                            pm_places<1>(bias, g0, k, at);
+                            s[u][0][n][c] = pm_bias(at, s[u][0][n][c], scale2);
+                            pm_places<1>(bias, g1, k, at);
+                            s[u][0][n][2 + c] = pm_bias(at, s[u][0][n][2 + c], scale2);
+                        }
+                if (j0 + 32 > nk)
+#pragma unroll
+                    for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (j0 + 16 * u + 8 * n + 2 * t + (c & 1) >= nk) s[u][k][n][c] = -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) {
+                float top[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(s[0][k][0][2 * r], s[0][k][0][2 * r + 1]);
+                    top[r] = fmaxf(top[r], fmaxf(s[0][k][1][2 * r], s[0][k][1][2 * r + 1]));
+                    top[r] = fmaxf(top[r], fmaxf(s[1][k][0][2 * r], s[1][k][0][2 * r + 1]));
+                    top[r] = fmaxf(top[r], fmaxf(s[1][k][1][2 * r], s[1][k][1][2 * r + 1]));
+                    if (!BIAS) top[r] *= scale2;
+                }
+                if (__any_sync(0xffffffffu, top[0] > m[k][0] + PM_LAZY || top[1] > m[k][1] + PM_LAZY)) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                        top[r] = fmaxf(m[k][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
+                        const float fix = fast_exp2(m[k][r] - top[r]);
+                        m[k][r] = top[r];
+                        l[k][r] *= fix;
+                        sum[k][2 * r] *= fix;
+#pragma unroll
+                        for (int n = 0; n < W / 8; ++n) {
+                            o[k][n][2 * r] *= fix;
+                            o[k][n][2 * r + 1] *= fix;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float v = s[u][k][n][c], top1 = m[k][c >> 1];
+                            s[u][k][n][c] = fast_exp2(BIAS ? v - top1 : fmaf(v, scale2, -top1));
+                            if (KEEP) l[k][c >> 1] += s[u][k][n][c];
+                        }
+                    uint32_t p[1][4];
+                    pm_pack(s[u][k], p[0]);
+                    pm_accumulate<W, 1>(p, vs, j0 + 16 * u, o[k]);
+                    // the sum that the result is divided by is that of the rounded probabilities
+                    mma_bf16(sum[k], p[0], ONES, ONES);
+                }
+            }
+        }
+    }
+    in.end();
+    if (!active) return;
+    if (KEEP)
+#pragma unroll
+        for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float v = l[k][r];
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                const int row = r ? r1 : r0;
+                if (t == 0 && row < L) a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = m[k][r] + log2f(v);
+            }
+    const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int e = r ? e1 : e0;
+        if (e < 0) continue;
+        const float w0 = 1.f / sum[0][2 * r], w1 = MAPS == 2 ? lam / sum[MAPS - 1][2 * r] : 0.f;
+        uint32_t* op = (uint32_t*)((__nv_bfloat16*)a.out + (int64_t)e * a.C + w.h * W);
+#pragma unroll
+        for (int n = 0; n < W / 8; ++n) {
+            float x = o[0][n][2 * r] * w0, y = o[0][n][2 * r + 1] * w0;
+            if (MAPS == 2) {
+                x -= o[MAPS - 1][n][2 * r] * w1;
+                y -= o[MAPS - 1][n][2 * r + 1] * w1;
+            }
+            op[4 * n + t] = pack_bf16(x, y);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- backward, a warp's own queries
+// Two walks over the keys: delta (and the sum of the probabilities, which undoes the rounding of the saved logarithm) first, then dQ
+// and the table's gradient, whose sums are integers in a unit of the block's largest row (patch_attn_fma.cu says why).
+template <int W, int MAPS, bool BIAS>
+__global__ void __launch_bounds__(PM_THREADS, 2) patch_mma_rows_kernel(const PatchArgs a)
+{
+    using S = PmStage<W>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float largest[PM_WARPS];
+    const PmPlace w = pm_place(a);
+    const int q0 = w.tile * PM_ROWS, L = w.L;
+    const int entries = 3 * (2 * a.bnd + 1);
+    const bool learns = BIAS && a.bins;
+    float* sums = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * entries : nullptr;
+    if (q0 >= L) {
+        if (learns)
+            for (int i = threadIdx.x; i < entries; i += PM_THREADS) sums[i] = 0.f;
+        return;
+    }
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int r0 = q0 + (threadIdx.x / 32) * 16 + g, r1 = r0 + 8;
+    const int e0 = r0 < L ? a.rows[w.start + r0] : -1, e1 = r1 < L ? a.rows[w.start + r1] : -1;
+    const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
+    const int64_t stride = 3 * (int64_t)a.C;
+    const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
+    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false, smem};
+    in.begin();
+
+    float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+    int* hist = (int*)(tab + (entries << a.copies_log2));
+    const uint32_t to_hist = (uint32_t)(entries << a.copies_log2) * 4;
+    PmBias bias;
+    int g0[3], g1[3];
+    if (BIAS) {
+        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);
+        if (learns)
+            for (int i = threadIdx.x; i < entries << a.copies_log2; i += PM_THREADS) hist[i] = 0;
+        pm_bias_setup(a, smem_u32(tab), bias);
+        pm_bias_point(a, bias, e0, 1, g0);
+        pm_bias_point(a, bias, e1, 1, g1);
+    }
+    uint32_t q[W / 16][4], go[W / 16][4];
+    pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr, 0u, q);
+    const __nv_bfloat16* gbase = (const __nv_bfloat16*)a.dout + w.h * W;
+    pm_rows<W>(e0 >= 0 ? gbase + (int64_t)e0 * a.C : nullptr, e1 >= 0 ? gbase + (int64_t)e1 * a.C : nullptr, 0u, go);
+    const float scale2 = a.scale * PA_LOG2E;
+    float lse[MAPS][2], delta[MAPS][2], total[MAPS][2], coef[MAPS][2], most[2] = {0.f, 0.f}, dq[W / 8][4];
+#pragma unroll
+    for (int n = 0; n < W / 8; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dq[n][c] = 0.f;
+#pragma unroll
+    for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const bool own = (r ? e1 : e0) >= 0;
+            lse[k][r] = own ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + (r ? r1 : r0)] : INFINITY;
+            delta[k][r] = total[k][r] = 0.f;
+            coef[k][r] = k == 1 ? -pa_param(a.lam, w.h, a.lam_bf16) : 1.f;
+        }
+    float unit = 0.f, per_unit = 0.f;
+
+    for (int walk = 0; walk < 2; ++walk) {
+        if (walk == 1) in.begin();
+        for (int i = 0; i * PM_CHUNK < L; ++i) {
+            const unsigned char* st = in.next(i);
+            if (!active) continue;
+            const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
+            const int4* gs = (const int4*)(st + S::GRID);
+            const int nk = L - i * PM_CHUNK;
+#pragma unroll 2
+            for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
+                if (j0 >= nk) break;
+                float s[MAPS][2][4], G[1][2][4];
+                uint32_t at[2][4][3];
+                pm_products<W, MAPS>(q, ks, j0, s);
+                pm_products<W, 1>(go, vs, j0, G);
+                if (BIAS)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int4 k = gs[j0 + 8 * n + 2 * t + c];
+                            pm_places<1>(bias, g0, k, at[n][c]);
+                            pm_places<1>(bias, g1, k, at[n][2 + c]);
+                        }
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float v = s[k][n][c];
+                            const int r = c >> 1;
+                            v = BIAS ? pm_bias(at[n][c], v, scale2) - lse[k][r] : fmaf(v, scale2, -lse[k][r]);
+                            if (j0 + 16 > nk && j0 + 8 * n + 2 * t + (c & 1) >= nk) v = -INFINITY;
+                            const float p = fast_exp2(v);
+                            if (walk == 0) {
+                                delta[k][r] = fmaf(p, G[0][n][c], delta[k][r]);
+                                total[k][r] += p;
+                                if (BIAS) most[r] = fmaf(p, fabsf(G[0][n][c]), most[r]);
+                            } else {
+                                s[k][n][c] = p * (G[0][n][c] - delta[k][r]);
+                            }
+                        }
+                if (walk == 1) {
+                    uint32_t p[MAPS][4];
+#pragma unroll
+                    for (int k = 0; k < MAPS; ++k) pm_pack(s[k], p[k]);
+                    pm_accumulate<W, MAPS>(p, ks, j0, dq);
+                    if (learns)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const int v = __float2int_rn(s[0][n][c] * (coef[0][c >> 1] * per_unit));
+#pragma unroll
+                                for (int x = 0; x < 3; ++x) pm_add_shared(at[n][c][x] + to_hist, v);
+                            }
+                }
+            }
+        }
+        in.end();
+        if (walk == 0) {
+            float top = 0.f;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const bool own = (r ? e1 : e0) >= 0;
+                float inv = 0.f;
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    float d = delta[k][r], s = total[k][r];
+                    d += __shfl_xor_sync(0xffffffffu, d, 1);
+                    s += __shfl_xor_sync(0xffffffffu, s, 1);
+                    d += __shfl_xor_sync(0xffffffffu, d, 2);
+                    s += __shfl_xor_sync(0xffffffffu, s, 2);
+                    inv = own ? 1.f / s : 0.f;
+                    delta[k][r] = d * inv;
+                    coef[k][r] *= inv;
+                    const int row = r ? r1 : r0;
+                    if (t == 0 && row < L)
+                        a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = delta[k][r];
+                }
+                float v = most[r];
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                top = fmaxf(top, max_nan(0.f, v * inv + fabsf(delta[0][r])));
+            }
+            if (learns) {
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+                if (lane == 0) largest[threadIdx.x / 32] = top;
+                __syncthreads();
+                for (int i = 0; i < PM_WARPS; ++i) top = max_nan(top, largest[i]);
+                // rows that share a copy (two of each warp's to a lane's), times the largest row
+                unit = top * (float)(2 * PM_WARPS << (5 - a.copies_log2)) * (1.f / 1073741824.f);
+                per_unit = unit > 0.f ? 1.f / unit : 0.f;
+                if (!(per_unit < INFINITY)) per_unit = unit = 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int e = r ? e1 : e0;
+        if (e < 0) continue;
+        uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + w.h * W);
+#pragma unroll
+        for (int n = 0; n < W / 8; ++n) {
+            const float c = coef[n * 8 / (W / MAPS)][r] * a.scale;
+            dst[4 * n + t] = pack_bf16(dq[n][2 * r] * c, dq[n][2 * r + 1] * c);
+        }
+    }
+    if (learns) {
+        const int copies = 1 << a.copies_log2;
+        for (int i = threadIdx.x; i < entries; i += PM_THREADS) {
+            float v = 0.f;
+            for (int c = 0; c < copies; ++c) v += (float)hist[(i << a.copies_log2) + ((c + i) & (copies - 1))];
+            sums[i] = v * unit;
+        }
+    }
+}
+
+// --------------------------------------------------------------------------- backward, a warp's own keys
+template <int W, int MAPS, bool BIAS>
+__global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_kernel(const PatchArgs a)
+{
+    using S = PmStage<W>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const PmPlace w = pm_place(a);
+    const int k0 = w.tile * PM_ROWS, L = w.L;
+    if (k0 >= L) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warp0 = k0 + (threadIdx.x / 32) * 16, r0 = warp0 + g, r1 = r0 + 8;
+    const bool there0 = r0 < L, there1 = r1 < L;
+    const int e0 = there0 ? a.rows[w.start + r0] : -1, e1 = there1 ? a.rows[w.start + r1] : -1;
+    const int64_t p0 = e0 >= 0 ? e0 : -(e0 + 1), p1 = e1 >= 0 ? e1 : -(e1 + 1), stride = 3 * (int64_t)a.C;
+    const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
+    PmStream<W, MAPS, true, BIAS> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
+                                        smem};
+    in.begin();
+    float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+    PmBias bias;
+    int g0[3], g1[3];
+    if (BIAS) {
+        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);
+        pm_bias_setup(a, smem_u32(tab), bias);
+        pm_bias_point(a, bias, e0, -1, g0);
+        pm_bias_point(a, bias, e1, -1, g1);
+    }
+    uint32_t kf[W / 16][4], vf[W / 16][4];
+    pm_rows<W>(there0 ? base + a.C + p0 * stride : nullptr, there1 ? base + a.C + p1 * stride : nullptr, 0u, kf);
+    pm_rows<W>(there0 ? base + 2 * a.C + p0 * stride : nullptr, there1 ? base + 2 * a.C + p1 * stride : nullptr, 0u, vf);
+    const float scale2 = a.scale * PA_LOG2E;
+    const float minus_lam = MAPS == 2 ? -pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
+    float dk[W / 8][4], dv[W / 8][4];
+#pragma unroll
+    for (int n = 0; n < W / 8; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
+
+    for (int i = 0; i * PM_CHUNK < L; ++i) {
+        const unsigned char* st = in.next(i);
+        if (warp0 >= L) continue;
+        const uint32_t qs = smem_u32(st), os = qs + S::TILE;
+        const float* aux = (const float*)(st + S::AUX);
+        const int4* gs = (const int4*)(st + S::GRID);
+        const int nq = L - i * PM_CHUNK;
+#pragma unroll 2
+        for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
+            if (j0 >= nq) break;
+            float s[MAPS][2][4], G[1][2][4], mix[2][4];
+            pm_products<W, MAPS>(kf, qs, j0, s);
+            pm_products<W, 1>(vf, os, j0, G);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int j = j0 + 8 * n + 2 * t;
+                if (BIAS)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int4 o = gs[j + c];
+                        uint32_t at[3];
+                        pm_places<-1>(bias, g0, o, at);
+                        s[0][n][c] = pm_bias(at, s[0][n][c], scale2);
+                        pm_places<-1>(bias, g1, o, at);
+                        s[0][n][2 + c] = pm_bias(at, s[0][n][2 + c], scale2);
+                    }
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    const float2 lse = *(const float2*)(aux + k * PM_CHUNK + j);
+                    const float2 delta = *(const float2*)(aux + (MAPS + k) * PM_CHUNK + j);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float ls = c & 1 ? lse.y : lse.x, d = c & 1 ? delta.y : delta.x;
+                        float p = fast_exp2(BIAS ? s[k][n][c] - ls : fmaf(s[k][n][c], scale2, -ls));
+                        if (k == 1) p *= minus_lam;
+                        mix[n][c] = k == 0 ? p : mix[n][c] + p;
+                        s[k][n][c] = p * (G[0][n][c] - d);
+                    }
+                }
+            }
+            uint32_t p[MAPS][4], x[1][4];
+            pm_pack(mix, x[0]);
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) pm_pack(s[k], p[k]);
+            pm_accumulate<W, 1>(x, os, j0, dv);
+            pm_accumulate<W, MAPS>(p, qs, j0, dk);
+        }
+    }
+    in.end();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        if (!(r ? there1 : there0)) continue;
+        const int e = r ? e1 : e0, slot = a.slot ? a.slot[w.start + (r ? r1 : r0)] : -1;
+        if (slot >= 0) {             // this point's other row is some other patch's: added up later
+            float2* dst = (float2*)(a.shared + (int64_t)slot * 2 * a.C + w.h * W);
+#pragma unroll
+            for (int n = 0; n < W / 8; ++n) {
+                dst[4 * n + t] = make_float2(dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
+                dst[a.C / 2 + 4 * n + t] = make_float2(dv[n][2 * r], dv[n][2 * r + 1]);
+            }
+        } else if (e >= 0) {
+            uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + a.C + w.h * W);
+#pragma unroll
+            for (int n = 0; n < W / 8; ++n) {
+                dst[4 * n + t] = pack_bf16(dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
+                dst[a.C / 2 + 4 * n + t] = pack_bf16(dv[n][2 * r], dv[n][2 * r + 1]);
+            }
+        }
+    }
+}
+
+template <typename K>
+static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
+{
+    const cudaError_t err = allow_smem(kern);
+    PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
+    kern<<<(unsigned)((int64_t)a.n_seq * a.tiles * a.H), PM_THREADS, smem, stream>>>(a);
+    count_launches(1);
+    return check_launch("ptv3_patch_attention");
+}
+
+template <int W, int MAPS, bool BIAS>
+static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
+{
+    const size_t table = BIAS ? (size_t)(3 * (2 * a.bnd + 1)) << a.copies_log2 << 2 : 0;
+    const size_t smem = PM_STAGES * PmStage<W>::BYTES + table;
+    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem + (a.bins ? table : 0), stream);
+    if (pass == PA_COLS) return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a, smem, stream);
+    return a.lse ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true>, a, smem, stream)
+                 : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false>, a, smem, stream);
+}
+
+template <int W>
+static int launch_form(const PatchArgs& a, int maps, int pass, cudaStream_t stream)
+{
+    if (maps == 2) return launch_pass<W, 2, false>(a, pass, stream);
+    return a.grid ? launch_pass<W, 1, true>(a, pass, stream) : launch_pass<W, 1, false>(a, pass, stream);
+}
+
+int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream)
+{
+    switch (width) {
+        case 16: return launch_form<16>(a, maps, pass, stream);
+        case 32: return launch_form<32>(a, maps, pass, stream);
+        default: return launch_form<64>(a, maps, pass, stream);
+    }
+}
+
+int patch_mma_rows() { return PM_ROWS; }
+
+}  // namespace ptv3

@@ -109,7 +109,7 @@ class _PatchAttention(torch.autograd.Function):
         qkv = _aligned(qkv)
         param = None if param is None else param.contiguous()
         with torch.cuda.device(qkv.device):
-            rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, buckets, pos_bnd, num, status)
+            rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, status)
             out, lse = ops.patch_attention_fwd(qkv, rows, pad.numel(), cu, heads, max_seqlen, scale, maps, param, grid,
                                                buckets, pos_bnd, num, want_lse=keep)
         if keep:
@@ -166,11 +166,11 @@ def attention_bias(qkv, order_row, pad, unpad, cu_seqlens, heads, max_seqlen, sc
     qkv (N, 3C), split (3, heads, D), D in 16, 32, 64, bf16 or fp32; order_row (N,), pad, unpad, cu_seqlens: one row of a serialized
     order and its patches (``ops.pad_plan``), of at most ``max_seqlen`` rows.  Scores are scale q.k (scale: D ** -0.5) plus
     the sum over the axes a of table[a * num + bucket(grid_coord[i, a] - grid_coord[j, a]), head]; table (3 num, heads), fp32 or
-    bf16, grid_coord (N, 3) integers.  ``buckets`` (2 bound + 1,) int32 gives the bucket of every offset -bound .. bound,
+    bf16, grid_coord (N, 3) integers within 2^22 of zero.  ``buckets`` (2 bound + 1,) int32 gives the bucket of every offset -bound .. bound,
     those beyond going with the outermost (``log_buckets``); without it every offset has its own, num = 2 bound + 1, which is
     the bias of ``RPE``.  Without a table there is no bias.
 
-    status: a device status word of the caller's (``ops.new_status``), in which a plan or buckets out of range are reported; the caller
+    status: a device status word of the caller's (``ops.new_status``), in which a plan, coordinates or buckets out of range are reported; the caller
     checks it when the host next waits.  Without one the call checks for itself and waits for the device.
     Gradients: qkv and table."""
     _same_device(qkv, order_row, pad, unpad, cu_seqlens, grid_coord, table, buckets, status)

@@ -241,15 +241,16 @@ def qk_norm_rope_bwd(qkv, dout, heads, grid, q_weight, k_weight, eps, base):
     return dqkv, dq, dk
 
 
-def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, buckets=None, pos_bnd=0, num_buckets=0, status=None):
+def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, grid=None, buckets=None, pos_bnd=0, num_buckets=0,
+               status=None):
     """Points of the padded rows of a plan as patch_attention_fwd / _bwd read them (see ptv3_patch_rows)."""
-    _lib.require_cuda(order_row, pad, unpad, cu_seqlens, buckets, status)
+    _lib.require_cuda(order_row, pad, unpad, cu_seqlens, grid, buckets, status)
     n, n_pad = order_row.numel(), pad.numel()
     rows = torch.empty(2 * n_pad + (n_pad - n) + 1, dtype=torch.int32, device=pad.device)
     _lib.check(_lib.load().ptv3_patch_rows(_lib.ptr(order_row), _lib.ptr(pad), _lib.ptr(unpad), _lib.ptr(cu_seqlens), n,
-                                           n_pad, cu_seqlens.numel() - 1, int(max_seqlen), _lib.ptr(buckets),
-                                           int(pos_bnd), int(num_buckets), _lib.ptr(rows), _lib.ptr(status),
-                                           _lib.stream()), "ptv3_patch_rows")
+                                           n_pad, cu_seqlens.numel() - 1, int(max_seqlen), _lib.ptr(grid),
+                                           _lib.ptr(buckets), int(pos_bnd), int(num_buckets), _lib.ptr(rows),
+                                           _lib.ptr(status), _lib.stream()), "ptv3_patch_rows")
     return rows
 
 

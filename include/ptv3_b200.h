@@ -197,7 +197,7 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
  * follow one another from row 0 to n_pad and are no longer than max_seqlen.  What a bias reads is looked at too, where given:
  * `grid_coord` (n x 3 int32) within 2^22 of zero, `buckets` (2 pos_bnd + 1 int32) in [0, num_buckets).
  *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30
- *   rows        2 * n_pad + (n_pad - n) + 1 int32, written
+ *   rows        2 * n_pad + (n_pad - n) + 1 + 3 * n_seq int32, written
  *   status      one uint32 or NULL: PTV3_STATUS_BAD_INDEX where something does not hold (the calls that read `rows` then
  *               stay within their tensors, and what they leave is undefined)
  */
@@ -221,8 +221,9 @@ int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unp
  *   qkv, dqkv   n x 3*channels; out, dout n x channels; 16-byte aligned, dtype PTV3_DTYPE_*
  *   rows        of ptv3_patch_rows
  *   table       3 * num_buckets x heads, lam heads: fp32 or bf16 (table_dtype, lam_dtype); gradients in the same type
- *   lse         heads * maps * n_pad fp32: written by _fwd (may be NULL there), read by _bwd
- *   _bwd        writes dqkv, and dtable / dlam where not NULL, from qkv, lse and dout
+ *   lse         2 * heads * maps * n_pad fp32, and with maps = 2 second, n x channels like out: what _bwd needs of the softmax
+ *               and of the second map, written by _fwd (not where lse is NULL)
+ *   _bwd        writes dqkv, and dtable / dlam where not NULL, from qkv, out, lse, second and dout
  *   workspace   of _bwd
  */
 typedef struct ptv3_patch_attention_args {
@@ -235,6 +236,7 @@ typedef struct ptv3_patch_attention_args {
     const void *table, *lam;
     void* out;
     float* lse;
+    void* second;
     const void* dout;
     void *dqkv, *dtable, *dlam;
     void* workspace;

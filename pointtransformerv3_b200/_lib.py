@@ -75,7 +75,7 @@ class PatchAttentionArgs(ctypes.Structure):
         + [("scale", c_f32)]
         + [(name, c_int) for name in ("pos_bnd", "num_buckets", "table_dtype", "lam_dtype")]
         + [(name, c_ptr) for name in ("qkv", "rows", "cu_seqlens", "grid_coord", "buckets", "table", "lam", "out", "lse",
-                                      "dout", "dqkv", "dtable", "dlam", "workspace")]
+                                      "second", "dout", "dqkv", "dtable", "dlam", "workspace")]
         + [("workspace_bytes", c_sz)])
 
 

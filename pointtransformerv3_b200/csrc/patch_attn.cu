@@ -58,6 +58,50 @@ __global__ void __launch_bounds__(256) patch_rows_kernel(const int64_t* order, c
     if (bad && status) atomicOr(status, PTV3_STATUS_BAD_INDEX);
 }
 
+// Largest offset of two points of a sequence along each axis: a block per sequence
+__global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, const int32_t* cu, const int32_t* grid, int n_pad,
+                                                           int max_seqlen, int32_t* extent)
+{
+    __shared__ int lo_s[4][3], hi_s[4][3];
+    const PatchArgs a = {nullptr, nullptr, rows, nullptr, cu, n_pad, 0, max_seqlen};
+    int start, lo[3], hi[3];
+    const int L = pa_sequence(a, blockIdx.x, start);
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        lo[c] = PA_MAX_COORD;
+        hi[c] = -PA_MAX_COORD;
+    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < L; i += 128) {
+        const int e = rows[start + i];
+        const int64_t p = e >= 0 ? e : -(e + 1);
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+            const int v = min(max(grid[3 * p + c], -PA_MAX_COORD), PA_MAX_COORD);
+            lo[c] = min(lo[c], v);
+            hi[c] = max(hi[c], v);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        lo[c] = __reduce_min_sync(0xffffffffu, lo[c]);
+        hi[c] = __reduce_max_sync(0xffffffffu, hi[c]);
+        if ((threadIdx.x & 31) == 0) {
+            lo_s[threadIdx.x / 32][c] = lo[c];
+            hi_s[threadIdx.x / 32][c] = hi[c];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        int l = lo_s[0][threadIdx.x], h = hi_s[0][threadIdx.x];
+        for (int w = 1; w < 4; ++w) {
+            l = min(l, lo_s[w][threadIdx.x]);
+            h = max(h, hi_s[w][threadIdx.x]);
+        }
+        extent[3 * blockIdx.x + threadIdx.x] = max(h - l, 0);
+    }
+}
+
 // ---- gradients of keys and values with a borrowed copy ------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void pa_store(T* p, float v);
@@ -163,9 +207,9 @@ static int launch_patch(const ptv3_patch_attention_args* p, const PatchArgs& a, 
 }
 
 struct PatchWorkspace {
-    float *delta, *shared, *bins, *folded, *partial;
+    float *delta, *reach, *shared, *bins, *folded, *partial;
     size_t bytes;
-    int64_t blocks;      // of the pass over rows, heads apart
+    int64_t blocks;      // of a pass, heads apart
     int parts;
 };
 
@@ -178,6 +222,7 @@ static PatchWorkspace carve(const ptv3_patch_attention_args* p)
     w.delta = c.take<float>((size_t)p->heads * p->maps * p->n_pad);
     w.shared = c.take<float>((size_t)(p->n_pad - p->n) * 4 * p->channels);
     if (p->dtable) {
+        w.reach = c.take<float>((size_t)p->heads * p->n_pad);
         const size_t width = (size_t)p->heads * 3 * (2 * p->pos_bnd + 1);
         w.bins = c.take<float>((size_t)w.blocks * width);
         w.folded = c.take<float>((size_t)ceil_div(w.blocks, PA_FOLD) * width);
@@ -196,6 +241,7 @@ static int check_sizes(const ptv3_patch_attention_args* p, const char* what)
     const int width = p->channels / p->heads;
     PTV3_REQUIRE(width == 16 || width == 32 || width == 64, PTV3_ERR_UNSUPPORTED,
                  "%s: heads of %d values (supported: 16, 32, 64)", what, width);
+    PTV3_REQUIRE(p->scale != 0.f && p->scale - p->scale == 0.f, PTV3_ERR_INVALID_ARGUMENT, "%s: scale %g", what, p->scale);
     PTV3_REQUIRE(p->dtype == PTV3_DTYPE_F32 || p->dtype == PTV3_DTYPE_BF16, PTV3_ERR_UNSUPPORTED, "%s: dtype %d", what,
                  p->dtype);
     // half of each: a point has at most two rows, and their slots are numbered in 32 bits too
@@ -243,7 +289,8 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
     a.num = p->num_buckets;
     a.bnd = p->pos_bnd;
     a.table_bf16 = p->table_dtype == PTV3_DTYPE_BF16;
-    while (a.copies_log2 < 5 && (3 * (2 * a.bnd + 1)) << (a.copies_log2 + 1) << 2 <= PA_TABLE_BYTES) ++a.copies_log2;
+    a.extent = p->grid_coord ? p->rows + 2 * p->n_pad + (p->n_pad - p->n) + 1 : nullptr;
+    a.second = p->second;
     a.lam = p->lam;
     a.lam_bf16 = p->lam_dtype == PTV3_DTYPE_BF16;
     a.lse = p->lse;
@@ -278,6 +325,11 @@ extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const i
         order, pad, unpad, cu_seqlens, (int)n, (int)n_pad, n_seq, max_seqlen, grid_coord, buckets, entries, num_buckets, rows, slot,
         slot_point, taken, status);
     count_launches(1);
+    if (grid_coord && n_seq > 0) {
+        patch_extent_kernel<<<n_seq, 128, 0, (cudaStream_t)stream>>>(rows, cu_seqlens, grid_coord, (int)n_pad, max_seqlen,
+                                                                      taken + 1);
+        count_launches(1);
+    }
     return check_launch("ptv3_patch_rows");
 }
 
@@ -286,10 +338,10 @@ extern "C" int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* p, void
     const int rc = check_sizes(p, "ptv3_patch_attention_fwd");
     if (rc != PTV3_OK) return rc;
     if (p->n == 0 || p->n_seq == 0) return PTV3_OK;
-    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
+    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out | (uintptr_t)p->second) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_fwd: unaligned rows");
-    PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || p->lam), PTV3_ERR_INVALID_ARGUMENT,
-                 "ptv3_patch_attention_fwd: null pointer");
+    PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || (p->lam && (!p->lse || p->second))),
+                 PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_fwd: null pointer");
     PatchArgs a = device_args(p);
     return launch_patch(p, a, PA_FWD, (cudaStream_t)stream);
 }
@@ -309,9 +361,11 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
     cudaStream_t s = (cudaStream_t)stream;
     PatchArgs a = device_args(p);
     if (p->n > 0 && p->n_seq > 0)
-        PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->lse && p->dout && p->dqkv && (p->maps == 1 || p->lam),
+        PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && p->lse && p->dout && p->dqkv &&
+                         (p->maps == 1 || (p->lam && p->second)),
                      PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_bwd: null pointer");
-    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->dout | (uintptr_t)p->dqkv) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
+    PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out | (uintptr_t)p->second | (uintptr_t)p->dout | (uintptr_t)p->dqkv) &
+                  15) == 0, PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_bwd: unaligned rows");
     PTV3_REQUIRE((!p->dtable || p->table) && (!p->dlam || p->maps == 2), PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_bwd: a gradient without its parameter");
@@ -324,6 +378,7 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
         a.dqkv = p->dqkv;
         a.delta = w.delta;
         a.shared = w.shared;
+        a.reach = w.reach;
         a.bins = w.bins;
         if ((rc = launch_patch(p, a, PA_ROWS, s)) != PTV3_OK) return rc;
         if ((rc = launch_patch(p, a, PA_COLS, s)) != PTV3_OK) return rc;

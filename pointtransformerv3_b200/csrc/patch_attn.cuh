@@ -7,10 +7,19 @@
 //   dV = A^T dO,  dQ_m = scale dS_m K_m,  dK_m = scale dS_m^T Q_m,  dlam = -sum_i delta_2,
 //   dtable[a][b] = sum of dS_1 over the pairs whose offset along axis a falls into bucket b
 //
-// A backward pass is two kernels, one that walks keys for each block of queries (delta, dQ, dtable) and one that walks
-// queries for each block of keys (dK, dV): both compute scores and probabilities again from the saved logarithm
+// A backward pass is two kernels, one that walks keys for each block of queries (delta, dQ) and one that walks
+// queries for each block of keys (dK, dV, dtable): both compute scores and probabilities again from the saved logarithm
 // of the softmax's sum, nothing of size L x L is stored and no float is added atomically, so results do not
 // depend on the order of anything.
+//
+// delta in one walk: the stored result gives an estimate, delta' = dO . O (dO . O2 for the second map, whose O2 the
+// forward pass leaves too), which is off by the rounding of O alone.  With E = sum_j P (G - delta'),
+// delta = delta' + E and dQ = sum_j P (G - delta') K - E sum_j P K, exact however far the values' mean is from zero and
+// however peaked a row is.  (A walk of its own for delta: 632 us for the differential rows of 100 000 x 64, DELTA_ONE.)
+//
+// dtable: a pair adds its dS to three bins, as integers in shared memory, since integer sums do not depend on the order
+// of the additions.  Their unit follows from what the queries of a window can add at most, sum_j |dS_ij| <= sum_j P |G -
+// delta'| + |E| (`reach`), so that no bin overflows; after a window the bins go into floats.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -22,7 +31,8 @@ namespace ptv3 {
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr int PA_MAX_BOUND = 512;
 constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
-constexpr int PA_TABLE_BYTES = 3 * 129 * 32 * 4;      // shared memory that copies of a head's table may take
+constexpr int PA_TABLE_BYTES = 360 * 32 * 4;          // shared memory that copies of a head's table may take
+constexpr int PA_WINDOW = 256;                        // queries between two clearings of the bins
 
 // What the kernels get: ptv3_patch_attention_args with the workspace carved up.
 struct PatchArgs {
@@ -37,15 +47,18 @@ struct PatchArgs {
     const void* table;          // (3 num) x H
     const int32_t* buckets;     // 2 bnd + 1, or NULL: every offset its own
     int num, bnd, table_bf16;
-    int copies_log2;            // the table in shared memory: that many copies, interleaved, one per lane or so
+    const int32_t* extent;      // n_seq x 3: largest offset within a sequence along each axis
     const void* lam;            // H
     int lam_bf16;
-    float* lse;                 // (H maps) x n_pad: log2 of the sum, or NULL
+    float* lse;                 // (H maps) x n_pad: log2 of the softmax's sum (bf16), or twice that: its reference
+                                // value in log2, then one over the sum (fp32); or NULL
     const void* dout;
     void* dqkv;
+    void* second;               // n x C: O2, with two maps
     float* delta;               // (H maps) x n_pad
+    float* reach;               // H x n_pad: no row's sum of |dS| is larger; or NULL
     float* shared;              // rows of (dK, dV), 2C
-    float* bins;                // per block of queries: H x 3 (2 bnd + 1), or NULL
+    float* bins;                // per block of keys: H x 3 (2 bnd + 1), or NULL
 };
 
 // rows [start, start + L) of a sequence; L = 0 for what ptv3_patch_rows reports
@@ -62,17 +75,105 @@ __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
     return bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : ((const float*)p)[i];
 }
 
-// This head's table in shared memory, in powers of two: entry e of axis a at ((a (2 bnd + 1) + e) << copies) + copy.
-// A lane reads the copy of its number: with 32 copies look-ups of a warp never meet in a bank.
-__device__ __forceinline__ void pa_load_table(const PatchArgs& a, int h, float* tab, int tid, int threads)
+// This head's table in shared memory, in powers of two, of the offsets that occur in a sequence: axis a holds offsets
+// -reach[a] .. reach[a], entry e of it at (first[a] + e) copies + copy.  A lane reads the copy of its number: with 32
+// copies, which most patches leave room for, look-ups of a warp never meet in a bank.
+struct PatchTable {
+    int reach[3], first[3], entries, copies_log2;
+};
+__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq)
 {
-    const int ne = 2 * a.bnd + 1, copies = 1 << a.copies_log2;
-    for (int i = tid; i < 3 * ne; i += threads) {
-        const int axis = i / ne, e = i - axis * ne;
+    PatchTable t;
+    t.entries = 0;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        t.reach[c] = min(a.bnd, a.extent[3 * seq + c]);
+        t.first[c] = t.entries;
+        t.entries += 2 * t.reach[c] + 1;
+    }
+    t.copies_log2 = 0;
+    while (t.copies_log2 < 5 && t.entries << (t.copies_log2 + 3) <= PA_TABLE_BYTES) ++t.copies_log2;
+    return t;
+}
+// axis and offset + bnd of an entry
+__device__ __forceinline__ void pa_entry(const PatchArgs& a, const PatchTable& t, int i, int& axis, int& e)
+{
+    axis = i >= t.first[2] ? 2 : i >= t.first[1] ? 1 : 0;
+    e = i - (axis == 2 ? t.first[2] - a.bnd + t.reach[2] : axis == 1 ? t.first[1] - a.bnd + t.reach[1] : t.reach[0] - a.bnd);
+}
+__device__ __forceinline__ void pa_load_table(const PatchArgs& a, const PatchTable& t, int h, float* tab, int tid,
+                                              int threads)
+{
+    const int copies = 1 << t.copies_log2;
+    for (int i = tid; i < t.entries; i += threads) {
+        int axis, e;
+        pa_entry(a, t, i, axis, e);
         int b = a.buckets ? a.buckets[e] : e;
         b = min(max(b, 0), a.num - 1);                     // (ptv3_patch_rows reports one out of range)
         const float v = pa_param(a.table, (axis * a.num + b) * a.H + h, a.table_bf16) * PA_LOG2E;
-        for (int c = 0; c < copies; ++c) tab[(i << a.copies_log2) + ((c + tid) & (copies - 1))] = v;
+        for (int c = 0; c < copies; ++c) tab[(i << t.copies_log2) + ((c + tid) & (copies - 1))] = v;
+    }
+}
+// most bytes that pa_load_table fills, and words of the entries themselves
+static inline size_t pa_table_bytes(const PatchArgs& a)
+{
+    const size_t all = (size_t)(3 * (2 * a.bnd + 1)) * 32 * 4;
+    return all < PA_TABLE_BYTES ? all : PA_TABLE_BYTES;
+}
+
+// What the queries [q0, q0 + PA_WINDOW) of a sequence can add to a bin at most, as a unit in which 2^30 of it are that.
+// With QUADS lane t of four adds queries 2 t and 2 t + 1 of every eight, to copies of its own where there are four and
+// more: the largest of four sums.  All threads of a block of 32 `WARPS`; `part`: WARPS x 4 floats
+template <int WARPS, bool QUADS>
+__device__ __forceinline__ float pa_unit(const PatchArgs& a, const PatchTable& table, int h, int start, int L, int q0,
+                                         float* part)
+{
+    float v = 0.f;
+    for (int j = threadIdx.x; j < PA_WINDOW; j += 32 * WARPS)
+        if (q0 + j < L) v += a.reach[(int64_t)h * a.n_pad + start + q0 + j];
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    v += __shfl_xor_sync(0xffffffffu, v, 16);
+    __syncthreads();
+    if ((threadIdx.x & 31) < 8 && (threadIdx.x & 1) == 0) part[(threadIdx.x / 32) * 4 + (threadIdx.x & 31) / 2] = v;
+    __syncthreads();
+    float top = 0.f, all = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        float sum = 0.f;
+        for (int w = 0; w < WARPS; ++w) sum += part[4 * w + t];
+        top = fmaxf(top, sum);
+        all += sum;                        // (a NaN among them is kept by this one)
+    }
+    return (QUADS && table.copies_log2 >= 2 && all == all ? top : all) * (1.f / 1073741824.f);
+}
+__device__ __forceinline__ float pa_per_unit(float unit)
+{
+    const float v = unit > 0.f ? 1.f / unit : 0.f;
+    return v < INFINITY ? v : 0.f;
+}
+// bins into floats, bins cleared
+__device__ __forceinline__ void pa_flush(const PatchTable& t, int* hist, float* sums, float unit, int threads)
+{
+    const int copies = 1 << t.copies_log2;
+    for (int i = threadIdx.x; i < t.entries; i += threads) {
+        float v = 0.f;
+        for (int c = 0; c < copies; ++c) {
+            int* at = hist + (i << t.copies_log2) + ((c + i) & (copies - 1));
+            v += (float)*at;
+            *at = 0;
+        }
+        sums[i] = fmaf(v, unit, sums[i]);
+    }
+}
+// a block's sums of all offsets
+__device__ __forceinline__ void pa_store_bins(const PatchArgs& a, const PatchTable& t, const float* sums, float* bins, int threads)
+{
+    const int ne = 2 * a.bnd + 1;
+    for (int i = threadIdx.x; i < 3 * ne; i += threads) {
+        const int axis = i / ne, d = i - axis * ne - a.bnd, r = axis == 0 ? t.reach[0] : axis == 1 ? t.reach[1] : t.reach[2];
+        const int first = axis == 0 ? 0 : axis == 1 ? t.first[1] : t.first[2];
+        bins[i] = d >= -r && d <= r ? sums[first + d + r] : 0.f;
     }
 }
 

@@ -46,18 +46,17 @@ __device__ __forceinline__ void pf_stage(const PatchArgs& a, const float* x, int
         }
 }
 
-// places of the three look-ups of a pair (g: coordinates of the query minus those of the key)
-__device__ __forceinline__ void pf_places(const PatchArgs& a, int gx, int gy, int gz, int copy, int (&at)[3])
+// places of the three look-ups of a pair (d: coordinates of the query minus those of the key)
+__device__ __forceinline__ void pf_places(const PatchTable& t, int dx, int dy, int dz, int copy, int (&at)[3])
 {
-    const int b = a.bnd, ne = 2 * b + 1;
-    at[0] = ((min(max(gx, -b), b) + b) << a.copies_log2) + copy;
-    at[1] = ((min(max(gy, -b), b) + b + ne) << a.copies_log2) + copy;
-    at[2] = ((min(max(gz, -b), b) + b + 2 * ne) << a.copies_log2) + copy;
+    const int d[3] = {dx, dy, dz};
+#pragma unroll
+    for (int c = 0; c < 3; ++c)
+        at[c] = ((min(max(d[c], -t.reach[c]), t.reach[c]) + t.reach[c] + t.first[c]) << t.copies_log2) + copy;
 }
 
 template <int W, int MAPS>
-__device__ __forceinline__ void pf_scores(const float (&q)[PfShape<W, MAPS>::WP], const float* k, int part, float scale2,
-                                          float (&s)[MAPS])
+__device__ __forceinline__ void pf_scores(const float (&q)[PfShape<W, MAPS>::WP], const float* k, int part, float (&s)[MAPS])
 {
     using S = PfShape<W, MAPS>;
 #pragma unroll
@@ -66,7 +65,7 @@ __device__ __forceinline__ void pf_scores(const float (&q)[PfShape<W, MAPS>::WP]
 #pragma unroll
         for (int i = 0; i < S::DP; ++i) v = fmaf(q[m * S::DP + i], k[m * S::D + part * S::DP + i], v);
         if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
-        s[m] = v * scale2;
+        s[m] = v;
     }
 }
 template <int W, int MAPS>
@@ -89,12 +88,17 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
-    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    const int part = threadIdx.x % S::SPLIT;
     int start;
     const int L = pa_sequence(a, seq, start);
     const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
     if (q0 >= L) return;
-    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
+    PatchTable table = {};
+    if (BIAS) {
+        table = pa_table(a, seq);
+        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
+    }
+    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
     const int e = qi < L ? a.rows[start + qi] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
         for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
-        m[k] = -INFINITY;
+        m[k] = -1e30f;          // (finite: scores may all be -inf)
         l[k] = 0.f;
 #pragma unroll
         for (int i = 0; i < S::WP; ++i) acc[k][i] = 0.f;
@@ -124,16 +128,16 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 #pragma unroll
             for (int j = 0; j < PF_STEP; ++j) {
                 const int jj = min(j0 + j, nk - 1);
-                pf_scores<W, MAPS>(q, Ks[jj], part, scale2, s[j]);
+                pf_scores<W, MAPS>(q, Ks[jj], part, s[j]);
                 if (BIAS) {
                     int at[3];
-                    pf_places(a, g[0] - Gs[jj][0], g[1] - Gs[jj][1], g[2] - Gs[jj][2], copy, at);
-                    s[j][0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
+                    pf_places(table, g[0] - Gs[jj][0], g[1] - Gs[jj][1], g[2] - Gs[jj][2], copy, at);
+                    s[j][0] = fmaf(s[j][0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
                 }
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
-                    if (j0 + j >= nk) s[j][k] = -INFINITY;
-                    top[k] = fmaxf(top[k], s[j][k]);
+                    if (j0 + j >= nk) s[j][k] = BIAS || scale2 > 0.f ? -INFINITY : INFINITY;
+                    top[k] = fmaxf(top[k], BIAS ? s[j][k] : s[j][k] * scale2);
                 }
             }
 #pragma unroll
@@ -144,167 +148,129 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 #pragma unroll
                 for (int i = 0; i < S::WP; ++i) acc[k][i] *= fix;
             }
+            float sum[MAPS] = {};      // of a step's, so that rounding does not grow with every key
 #pragma unroll
             for (int j = 0; j < PF_STEP; ++j) {
                 const int jj = min(j0 + j, nk - 1);
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
-                    const float pr = fast_exp2(s[j][k] - m[k]);
-                    l[k] += pr;
+                    const float pr = fast_exp2(BIAS ? s[j][k] - m[k] : fmaf(s[j][k], scale2, -m[k]));
+                    sum[k] += pr;
 #pragma unroll
                     for (int i = 0; i < S::WP; ++i) acc[k][i] = fmaf(pr, Vs[jj][part * S::WP + i], acc[k][i]);
                 }
             }
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) l[k] += sum[k];
         }
     }
-    if (qi >= L) return;
+    if (e < 0) return;
     if (a.lse && part == 0)
 #pragma unroll
-        for (int k = 0; k < MAPS; ++k) a.lse[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = m[k] + log2f(l[k]);
-    if (e < 0) return;
+        for (int k = 0; k < MAPS; ++k) {
+            float* to = a.lse + (int64_t)(h * MAPS + k) * a.n_pad + start + qi;
+            *to = m[k];
+            to[(int64_t)a.H * MAPS * a.n_pad] = 1.f / l[k];
+        }
     const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
     const float w0 = 1.f / l[0], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
     float* op = (float*)a.out + p * a.C + h * W + part * S::WP;
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) op[i] = (MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0);
+    for (int i = 0; i < S::WP; ++i) op[i] = MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0;
+    if (MAPS == 2 && a.lse) {
+        const float w2 = 1.f / l[MAPS - 1];
+        float* o2 = (float*)a.second + p * a.C + h * W + part * S::WP;
+#pragma unroll
+        for (int i = 0; i < S::WP; ++i) o2[i] = acc[MAPS - 1][i] * w2;
+    }
 }
 
 // ------------------------------------------------------------------------- backward, a thread's own query
-// The first walk over the keys gives delta, the second dQ and, where the table learns, the sums of dS by offset:
-// integers in shared memory, since integer sums do not depend on the order of the additions.  Their unit follows
-// from the largest sum of |dS| that a row of this block can have (known from the first walk: at most sum P |G| +
-// |delta|), so that no bin overflows: 2^-28 of it or less with a copy of the bins to every lane.
+// (in fp32 the stored results give delta itself, and the softmax's sum is kept as such: no estimate to correct)
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchArgs a)
 {
     using S = PfShape<W, MAPS>;
     __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
-    __shared__ float largest[PF_THREADS / 32];
     extern __shared__ float tab[];
-    const int ne = 2 * a.bnd + 1, entries = 3 * ne;
-    int* hist = (int*)(tab + (entries << a.copies_log2));
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
-    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    const int part = threadIdx.x % S::SPLIT;
     int start;
     const int L = pa_sequence(a, seq, start);
     const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
-    const bool learns = BIAS && a.bins;
-    float* sums = learns ? a.bins + ((int64_t)(seq * a.tiles + tile) * a.H + h) * entries : nullptr;
-    if (q0 >= L) {
-        if (learns)
-            for (int i = threadIdx.x; i < entries; i += PF_THREADS) sums[i] = 0.f;
-        return;
+    if (q0 >= L) return;
+    PatchTable table = {};
+    if (BIAS) {
+        table = pa_table(a, seq);
+        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
-    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
-    if (learns)
-        for (int i = threadIdx.x; i < entries << a.copies_log2; i += PF_THREADS) hist[i] = 0;
+    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
     const int e = qi < L ? a.rows[start + qi] : -1;
-    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
+    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C, all = (int64_t)a.H * MAPS * a.n_pad;
     const float* base = (const float*)a.qkv + h * W;
-    float q[S::WP], go[S::WP], dq[S::WP], lse[MAPS], delta[MAPS], coef[MAPS], total[MAPS], r = 0.f;
+    const int64_t own = p * a.C + h * W + part * S::WP;        // this thread's share of a row of C
+    float q[S::WP], go[S::WP], dq[S::WP], ref[MAPS], by[MAPS], delta[MAPS], reach = 0.f;
     int g[3] = {0, 0, 0};
+    float d1 = 0.f, d2 = 0.f;
 #pragma unroll
     for (int i = 0; i < S::WP; ++i) {
-        q[i] = (base[p * stride + pf_dim<W, MAPS>(i, part)]);
-        go[i] = e >= 0 ? (((const float*)a.dout)[p * a.C + h * W + part * S::WP + i]) : 0.f;
+        q[i] = base[p * stride + pf_dim<W, MAPS>(i, part)];
+        go[i] = e >= 0 ? ((const float*)a.dout)[own + i] : 0.f;
+        d1 = fmaf(go[i], e >= 0 ? ((const float*)a.out)[own + i] : 0.f, d1);
+        if (MAPS == 2) d2 = fmaf(go[i], e >= 0 ? ((const float*)a.second)[own + i] : 0.f, d2);
         dq[i] = 0.f;
+    }
+    if (S::SPLIT == 2) {
+        d1 += __shfl_xor_sync(0xffffffffu, d1, 1);
+        d2 += __shfl_xor_sync(0xffffffffu, d2, 1);
     }
     if (BIAS)
         for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+    const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
+    delta[0] = MAPS == 2 ? fmaf(lam, d2, d1) : d1;
+    if (MAPS == 2) delta[MAPS - 1] = d2;
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
+        const int64_t at = (int64_t)(h * MAPS + k) * a.n_pad + start + qi;
         // a row that answers for no point has no gradient: its probabilities are taken as nothing
-        lse[k] = e >= 0 ? a.lse[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] : INFINITY;
-        delta[k] = total[k] = 0.f;
-        coef[k] = 1.f;
+        ref[k] = e >= 0 ? a.lse[at] : INFINITY;
+        by[k] = e >= 0 ? a.lse[at + all] : 0.f;
+        if (qi < L && part == 0) a.delta[at] = delta[k];
     }
-    if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
     const float scale2 = a.scale * PA_LOG2E;
-    float unit = 0.f, per_unit = 0.f;
-    for (int walk = 0; walk < 2; ++walk) {
-        for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
-            const int nk = min(PF_CHUNK, L - c0);
-            __syncthreads();
-            pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs,
-                           BIAS ? Gs : nullptr);
-            __syncthreads();
+    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
+        const int nk = min(PF_CHUNK, L - c0);
+        __syncthreads();
+        pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
+        __syncthreads();
 #pragma unroll 4
-            for (int j = 0; j < nk; ++j) {
-                float s[MAPS];
+        for (int j = 0; j < nk; ++j) {
+            float s[MAPS];
+            pf_scores<W, MAPS>(q, Ks[j], part, s);
+            if (BIAS) {
                 int at[3];
-                pf_scores<W, MAPS>(q, Ks[j], part, scale2, s);
-                if (BIAS) {
-                    pf_places(a, g[0] - Gs[j][0], g[1] - Gs[j][1], g[2] - Gs[j][2], copy, at);
-                    s[0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
-                }
-                const float G = pf_dot<W, MAPS>(go, Vs[j], part);
-#pragma unroll
-                for (int k = 0; k < MAPS; ++k) {
-                    const float pr = fast_exp2(s[k] - lse[k]);
-                    if (walk == 0) {
-                        delta[k] = fmaf(pr, G, delta[k]);
-                        total[k] += pr;
-                        if (BIAS) r = fmaf(pr, fabsf(G), r);
-                    } else {
-                        const float ds = coef[k] * pr * (G - delta[k]);
-#pragma unroll
-                        for (int i = 0; i < S::DP; ++i)
-                            dq[k * S::DP + i] = fmaf(ds, Ks[j][k * S::D + part * S::DP + i], dq[k * S::DP + i]);
-                        if (learns && part == 0 && e >= 0) {
-                            const int v = __float2int_rn(ds * per_unit);
-                            atomicAdd(hist + at[0], v);
-                            atomicAdd(hist + at[1], v);
-                            atomicAdd(hist + at[2], v);
-                        }
-                    }
-                }
+                pf_places(table, g[0] - Gs[j][0], g[1] - Gs[j][1], g[2] - Gs[j][2], copy, at);
+                s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
             }
-        }
-        if (walk == 0) {
-            // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: 3e-7 of each at
-            // a logarithm of 10 (gradient of a table of 12 000 points, off by 1.1e-6 of its norm, 3e-7 with this)
+            const float G = pf_dot<W, MAPS>(go, Vs[j], part);
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) {
-                const float inv = e >= 0 ? 1.f / total[k] : 0.f;
-                delta[k] *= inv;
-                coef[k] *= inv;
-                if (k == 0) r *= inv;
+                const float ds = fast_exp2(BIAS ? s[k] - ref[k] : fmaf(s[k], scale2, -ref[k])) * (G - delta[k]);
+                if (BIAS) reach += fabsf(ds);
+#pragma unroll
+                for (int i = 0; i < S::DP; ++i)
+                    dq[k * S::DP + i] = fmaf(ds, Ks[j][k * S::D + part * S::DP + i], dq[k * S::DP + i]);
             }
         }
-        if (learns && walk == 0) {
-            float top = r + fabsf(delta[0]);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if ((threadIdx.x & 31) == 0) largest[threadIdx.x / 32] = top;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < PF_THREADS / 32; ++i) top = fmaxf(top, largest[i]);
-            // rows that share a copy, times the largest row; half the range is left for rounding
-            unit = top * (float)(PF_THREADS >> a.copies_log2) * (1.f / 1073741824.f);
-            per_unit = unit > 0.f ? 1.f / unit : 0.f;
-            if (!(per_unit < INFINITY)) per_unit = unit = 0.f;
-        }
     }
-    if (qi < L) {
-        if (part == 0)
+    if (BIAS && a.reach && qi < L && part == 0) a.reach[(int64_t)h * a.n_pad + start + qi] = reach * by[0];
+    if (e < 0) return;
+    by[0] *= a.scale;
+    if (MAPS == 2) by[MAPS - 1] *= -lam * a.scale;
+    float* dst = (float*)a.dqkv + p * stride + h * W;
 #pragma unroll
-            for (int k = 0; k < MAPS; ++k) a.delta[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = delta[k];
-        if (e >= 0) {
-            float* dst = (float*)a.dqkv + p * stride + h * W;
-#pragma unroll
-            for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = (dq[i] * a.scale);
-        }
-    }
-    if (learns) {
-        __syncthreads();
-        const int copies = 1 << a.copies_log2;
-        for (int i = threadIdx.x; i < entries; i += PF_THREADS) {
-            float v = 0.f;
-            for (int c = 0; c < copies; ++c) v += (float)hist[(i << a.copies_log2) + ((c + i) & (copies - 1))];
-            sums[i] = v * unit;
-        }
-    }
+    for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = dq[i] * by[i / S::DP];
 }
 
 // --------------------------------------------------------------------------- backward, a thread's own key
@@ -314,15 +280,34 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     using S = PfShape<W, MAPS>;
     __shared__ float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
-    __shared__ float Ls[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK];
+    // reference value, (-lam) / sum and delta of every query
+    __shared__ float Ms[MAPS][PF_CHUNK], Is[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK], unit_part[PF_THREADS / 8];
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
-    const int part = threadIdx.x % S::SPLIT, copy = threadIdx.x & ((1 << a.copies_log2) - 1);
+    const int part = threadIdx.x % S::SPLIT;
     int start;
     const int L = pa_sequence(a, seq, start);
     const int k0 = tile * S::ROWS, kj = k0 + threadIdx.x / S::SPLIT;
-    if (k0 >= L) return;
-    if (BIAS) pa_load_table(a, h, tab, threadIdx.x, PF_THREADS);
+    const bool learns = BIAS && a.bins;
+    float* bins = learns ? a.bins + ((int64_t)(seq * a.tiles + tile) * a.H + h) * 3 * (2 * a.bnd + 1) : nullptr;
+    if (k0 >= L) {
+        if (learns)
+            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PF_THREADS) bins[i] = 0.f;
+        return;
+    }
+    PatchTable table = {};
+    if (BIAS) {
+        table = pa_table(a, seq);
+        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
+    }
+    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1), words = BIAS ? table.entries << table.copies_log2 : 0;
+    int* hist = (int*)tab + words;
+    float* sums = tab + 2 * words;
+    if (learns) {
+        for (int i = threadIdx.x; i < words; i += PF_THREADS) hist[i] = 0;
+        for (int i = threadIdx.x; i < table.entries; i += PF_THREADS) sums[i] = 0.f;
+    }
+    float unit = 0.f, per_unit = 0.f;
     const int e = kj < L ? a.rows[start + kj] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;
@@ -342,30 +327,42 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
         const int nq = min(PF_CHUNK, L - c0);
         __syncthreads();
+        if (learns && c0 % PA_WINDOW == 0) {
+            if (c0) pa_flush(table, hist, sums, unit, PF_THREADS);
+            unit = pa_unit<PF_THREADS / 32, false>(a, table, h, start, L, c0, unit_part);
+            per_unit = pa_per_unit(unit);
+        }
         pf_stage<W>(a, base, stride, (const float*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
         for (int i = threadIdx.x; i < nq * MAPS; i += PF_THREADS) {
             const int m = i / nq, j = i % nq;
             const int64_t at = (int64_t)(h * MAPS + m) * a.n_pad + start + c0 + j;
-            Ls[m][j] = a.rows[start + c0 + j] >= 0 ? a.lse[at] : INFINITY;
+            const bool own = a.rows[start + c0 + j] >= 0;
+            Ms[m][j] = own ? a.lse[at] : INFINITY;
+            Is[m][j] = own ? a.lse[at + (int64_t)a.H * MAPS * a.n_pad] * coef[m] : 0.f;
             Ds[m][j] = a.delta[at];
         }
         __syncthreads();
 #pragma unroll 4
         for (int j = 0; j < nq; ++j) {
             float s[MAPS];
-            pf_scores<W, MAPS>(k, Qs[j], part, scale2, s);
+            int at[3];
+            pf_scores<W, MAPS>(k, Qs[j], part, s);
             if (BIAS) {
-                int at[3];
-                pf_places(a, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
-                s[0] += tab[at[0]] + tab[at[1]] + tab[at[2]];
+                pf_places(table, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
+                s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
             }
             const float G = pf_dot<W, MAPS>(v, Os[j], part);
             float mix = 0.f;
 #pragma unroll
             for (int m = 0; m < MAPS; ++m) {
-                const float pr = coef[m] * fast_exp2(s[m] - Ls[m][j]);
+                const float pr = Is[m][j] * fast_exp2(BIAS ? s[m] - Ms[m][j] : fmaf(s[m], scale2, -Ms[m][j]));
                 const float ds = pr * (G - Ds[m][j]);
                 mix += pr;
+                if (learns && part == 0 && kj < L) {
+                    const int v = __float2int_rn(ds * per_unit);
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) atomicAdd(hist + at[c], v);
+                }
 #pragma unroll
                 for (int i = 0; i < S::DP; ++i)
                     dk[m * S::DP + i] = fmaf(ds, Qs[j][m * S::D + part * S::DP + i], dk[m * S::DP + i]);
@@ -373,6 +370,12 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 #pragma unroll
             for (int i = 0; i < S::WP; ++i) dv[i] = fmaf(mix, Os[j][part * S::WP + i], dv[i]);
         }
+    }
+    if (learns) {
+        __syncthreads();
+        pa_flush(table, hist, sums, unit, PF_THREADS);
+        __syncthreads();
+        pa_store_bins(a, table, sums, bins, PF_THREADS);
     }
     if (kj >= L) return;
     const int slot = a.slot ? a.slot[start + kj] : -1;
@@ -396,20 +399,18 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
-    const size_t table = BIAS ? (size_t)(3 * (2 * a.bnd + 1)) << a.copies_log2 << 2 : 0;
+    const size_t table = BIAS ? pa_table_bytes(a) : 0;
+    // in the pass over columns beside the table: its bins, and their sums
+    const size_t cols = table + (a.bins ? table + (size_t)(3 * (2 * a.bnd + 1)) * 4 : 0);
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
-    cudaError_t err = cudaSuccess;
-    if (pass == PA_FWD) {
-        if (BIAS) err = allow_smem(patch_fma_fwd_kernel<W, MAPS, BIAS>);
-        if (err == cudaSuccess) patch_fma_fwd_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
-    } else if (pass == PA_ROWS) {
-        if (BIAS) err = allow_smem(patch_fma_rows_kernel<W, MAPS, BIAS>);
-        if (err == cudaSuccess)
-            patch_fma_rows_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table * (a.bins ? 2 : 1), stream>>>(a);
-    } else {
-        if (BIAS) err = allow_smem(patch_fma_cols_kernel<W, MAPS, BIAS>);
-        if (err == cudaSuccess) patch_fma_cols_kernel<W, MAPS, BIAS><<<grid, PF_THREADS, table, stream>>>(a);
-    }
+    auto go = [&](auto kern, size_t smem) {
+        const cudaError_t e = BIAS ? allow_smem(kern) : cudaSuccess;
+        if (e == cudaSuccess) kern<<<grid, PF_THREADS, smem, stream>>>(a);
+        return e;
+    };
+    const cudaError_t err = pass == PA_FWD    ? go(patch_fma_fwd_kernel<W, MAPS, BIAS>, table)
+                            : pass == PA_ROWS ? go(patch_fma_rows_kernel<W, MAPS, BIAS>, table)
+                                              : go(patch_fma_cols_kernel<W, MAPS, BIAS>, cols);
     PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
     count_launches(1);
     return check_launch("ptv3_patch_attention");

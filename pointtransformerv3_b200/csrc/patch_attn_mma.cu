@@ -28,7 +28,7 @@ struct PmStage {
     static constexpr int TILE = PM_CHUNK * W * 2;      // bytes of a matrix
     static constexpr int AUX = 2 * TILE;               // two words of each map and row
     static constexpr int GRID = AUX + 4 * PM_CHUNK * 4;
-    static constexpr int BYTES = GRID + PM_CHUNK * 16;
+    static constexpr int BYTES = GRID + 3 * PM_CHUNK * 4;
 };
 
 // byte offset of 16-byte chunk c of row r: chunks are exchanged so that the eight rows of an ldmatrix lie in different banks
@@ -70,6 +70,7 @@ struct PmStream {
     int64_t xs, ys;
     int start, L, h;
     bool owners;             // rows of y that answer for no point are taken as zeros
+    int step;                // coordinates are kept times 2^step
     unsigned char* smem;
     int e, eg, ea, g[3];
     float aux;
@@ -125,8 +126,8 @@ struct PmStream {
                 ((float*)(st + S::AUX))[threadIdx.x] = ea >= 0 ? aux : lse ? INFINITY : 0.f;
             }
             if (BIAS && threadIdx.x < PM_CHUNK)
-                ((int4*)(st + S::GRID))[threadIdx.x] = make_int4(g[0] << (a.copies_log2 + 2), g[1] << (a.copies_log2 + 2),
-                                                                 g[2] << (a.copies_log2 + 2), 0);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) ((int*)(st + S::GRID))[c * PM_CHUNK + threadIdx.x] = g[c] << step;
         }
         cp_async_commit();
     }
@@ -225,31 +226,38 @@ __device__ __forceinline__ void pm_pack(const float (&v)[2][4], uint32_t (&p)[4]
 }
 
 // ---- bias ---------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void pm_bias_setup(const PatchArgs& a, uint32_t base, PmBias& b)
+__device__ __forceinline__ void pm_bias_setup(const PatchTable& t, uint32_t base, PmBias& b)
 {
-    const int copy = (threadIdx.x & ((1 << a.copies_log2) - 1)) * 4, step = a.copies_log2 + 2;
+    const int copy = (threadIdx.x & ((1 << t.copies_log2) - 1)) * 4, step = t.copies_log2 + 2;
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-        b.lo[c] = (int)base + ((c * (2 * a.bnd + 1)) << step) + copy;
-        b.hi[c] = b.lo[c] + ((2 * a.bnd) << step);
+        b.lo[c] = (int)base + (t.first[c] << step) + copy;
+        b.hi[c] = b.lo[c] + ((2 * t.reach[c]) << step);
     }
 }
 // this lane's point, so that subtracting another's coordinates gives the entry's place
-__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PmBias& b, int e, int sign, int (&g)[3])
+__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTable& t, const PmBias& b, int e, int sign,
+                                              int (&g)[3])
 {
     const int64_t p = e >= 0 ? e : -(e + 1);
 #pragma unroll
     for (int c = 0; c < 3; ++c)
-        g[c] = b.lo[c] + ((a.bnd + sign * a.grid[3 * p + c]) << (a.copies_log2 + 2));
+        g[c] = b.lo[c] + ((t.reach[c] + sign * a.grid[3 * p + c]) << (t.copies_log2 + 2));
 }
-// places of a pair's three entries; SIGN: the lane's point is the query (+1) or the key
+// places of the entries of four pairs (rows g0, g1 of this lane and two of the other side); SIGN: the lane's point is
+// the query (+1) or the key
 template <int SIGN>
-__device__ __forceinline__ void pm_places(const PmBias& b, const int (&mine)[3], const int4& other, uint32_t (&at)[3])
+__device__ __forceinline__ void pm_places(const PmBias& b, const int (&g0)[3], const int (&g1)[3], const int* gs, int j,
+                                          uint32_t (&at)[4][3])
 {
-    const int o[3] = {other.x, other.y, other.z};
 #pragma unroll
-    for (int c = 0; c < 3; ++c)
-        at[c] = (uint32_t)min(__viaddmax_s32(mine[c], SIGN > 0 ? -o[c] : o[c], b.lo[c]), b.hi[c]);
+    for (int c = 0; c < 3; ++c) {
+        const int2 o = *(const int2*)(gs + c * PM_CHUNK + j);
+        at[0][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
+        at[1][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.y, b.lo[c]), b.hi[c]);
+        at[2][c] = (uint32_t)min(__viaddmax_s32(g1[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
+        at[3][c] = (uint32_t)min(__viaddmax_s32(g1[c], -SIGN * o.y, b.lo[c]), b.hi[c]);
+    }
 }
 __device__ __forceinline__ float pm_bias(const uint32_t (&at)[3], float s, float scale2)
 {
@@ -284,17 +292,19 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
-    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false, smem};
+    PatchTable table = {};
+    if (BIAS) table = pa_table(a, w.seq);
+    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+                                         table.copies_log2 + 2, smem};
     in.begin();
-
-    float* tab = (float*)(smem + PM_STAGES * S::BYTES);
     PmBias bias;
     int g0[3], g1[3];
     if (BIAS) {
-        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
-        pm_bias_setup(a, smem_u32(tab), bias);
-        pm_bias_point(a, bias, e0, 1, g0);
-        pm_bias_point(a, bias, e1, 1, g1);
+        float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
+        pm_bias_setup(table, smem_u32(tab), bias);
+        pm_bias_point(a, table, bias, e0, 1, g0);
+        pm_bias_point(a, table, bias, e1, 1, g1);
     }
     uint32_t q[W / 16][4];
     // (of a negative scale the sign goes to the queries, so that larger products are larger scores)
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
         const unsigned char* st = in.next(i);
         if (!active) continue;
         const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
-        const int4* gs = (const int4*)(st + S::GRID);
+        const int* gs = (const int*)(st + S::GRID);
         const int nk = L - i * PM_CHUNK;
 #pragma unroll
         for (int j0 = 0; j0 < PM_CHUNK; j0 += 32) {
@@ -329,16 +339,12 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
                 pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
                 if (BIAS)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2; ++n) {
+                        uint32_t at[4][3];
+                        pm_places<1>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int4 k = gs[j0 + 16 * u + 8 * n + 2 * t + c];
-                            uint32_t at[3];
-                            pm_places<1>(bias, g0, k, at);
-                            s[u][0][n][c] = pm_bias(at, s[u][0][n][c], scale2);
-                            pm_places<1>(bias, g1, k, at);
-                            s[u][0][n][2 + c] = pm_bias(at, s[u][0][n][2 + c], scale2);
-                        }
+                        for (int c = 0; c < 4; ++c) s[u][0][n][c] = pm_bias(at[c], s[u][0][n][c], scale2);
+                    }
                 if (j0 + 32 > nk)
 #pragma unroll
                     for (int k = 0; k < MAPS; ++k)
@@ -422,188 +428,195 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
                 y -= o[MAPS - 1][n][2 * r + 1] * w1;
             }
             op[4 * n + t] = pack_bf16(x, y);
+            if (MAPS == 2 && KEEP) {
+                const float w2 = 1.f / sum[MAPS - 1][2 * r];
+                ((uint32_t*)((__nv_bfloat16*)a.second + (int64_t)e * a.C + w.h * W))[4 * n + t] =
+                    pack_bf16(o[MAPS - 1][n][2 * r] * w2, o[MAPS - 1][n][2 * r + 1] * w2);
+            }
         }
     }
 }
 
 // ------------------------------------------------------------------------- backward, a warp's own queries
-// Two walks over the keys: delta (and the sum of the probabilities, which undoes the rounding of the saved logarithm) first, then dQ
-// and the table's gradient, whose sums are integers in a unit of the block's largest row (patch_attn_fma.cu says why).
+// acc1 += P1 x the tile's rows, acc2 += P2 x them (each map's for its own values)
+template <int W, int MAPS>
+__device__ __forceinline__ void pm_accumulate2(const uint32_t (&p1)[MAPS][4], const uint32_t (&p2)[MAPS][4], uint32_t tile,
+                                               int row0, float (&acc1)[W / 8][4], float (&acc2)[W / 8][4])
+{
+    const int lane = threadIdx.x & 31, r = row0 + (lane & 15), c = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < W / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, tile + pm_offset<W>(r, 2 * k + c));
+        constexpr int D = W / MAPS;
+        mma_bf16(acc1[2 * k], p1[16 * k / D], b[0], b[1]);
+        mma_bf16(acc1[2 * k + 1], p1[(16 * k + 8) / D], b[2], b[3]);
+        mma_bf16(acc2[2 * k], p2[16 * k / D], b[0], b[1]);
+        mma_bf16(acc2[2 * k + 1], p2[(16 * k + 8) / D], b[2], b[3]);
+    }
+}
+// row g and row g + 8 of two fragments: sums of products over the four lanes that hold them
+template <int W>
+__device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], const uint32_t (&y)[W / 16][4], float (&d)[2])
+{
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < W / 16; ++k)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float x0, x1, y0, y1;
+                unpack2(unpack_bf16x2(x[k][2 * half + r]), x0, x1);
+                unpack2(unpack_bf16x2(y[k][2 * half + r]), y0, y1);
+                v = fmaf(x0, y0, fmaf(x1, y1, v));
+            }
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        d[r] = v + __shfl_xor_sync(0xffffffffu, v, 2);
+    }
+}
+
 template <int W, int MAPS, bool BIAS>
-__global__ void __launch_bounds__(PM_THREADS, 2) patch_mma_rows_kernel(const PatchArgs a)
+__global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_kernel(const PatchArgs a)
 {
     using S = PmStage<W>;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float largest[PM_WARPS];
     const PmPlace w = pm_place(a);
     const int q0 = w.tile * PM_ROWS, L = w.L;
-    const int entries = 3 * (2 * a.bnd + 1);
-    const bool learns = BIAS && a.bins;
-    float* sums = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * entries : nullptr;
-    if (q0 >= L) {
-        if (learns)
-            for (int i = threadIdx.x; i < entries; i += PM_THREADS) sums[i] = 0.f;
-        return;
-    }
+    if (q0 >= L) return;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int r0 = q0 + (threadIdx.x / 32) * 16 + g, r1 = r0 + 8;
     const int e0 = r0 < L ? a.rows[w.start + r0] : -1, e1 = r1 < L ? a.rows[w.start + r1] : -1;
     const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
-    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false, smem};
+    PatchTable table = {};
+    if (BIAS) table = pa_table(a, w.seq);
+    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+                                         table.copies_log2 + 2, smem};
     in.begin();
-
-    float* tab = (float*)(smem + PM_STAGES * S::BYTES);
-    int* hist = (int*)(tab + (entries << a.copies_log2));
-    const uint32_t to_hist = (uint32_t)(entries << a.copies_log2) * 4;
     PmBias bias;
     int g0[3], g1[3];
     if (BIAS) {
-        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);
-        if (learns)
-            for (int i = threadIdx.x; i < entries << a.copies_log2; i += PM_THREADS) hist[i] = 0;
-        pm_bias_setup(a, smem_u32(tab), bias);
-        pm_bias_point(a, bias, e0, 1, g0);
-        pm_bias_point(a, bias, e1, 1, g1);
+        float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
+        pm_bias_setup(table, smem_u32(tab), bias);
+        pm_bias_point(a, table, bias, e0, 1, g0);
+        pm_bias_point(a, table, bias, e1, 1, g1);
     }
     uint32_t q[W / 16][4], go[W / 16][4];
+    // rows of a matrix of C columns, this head's; zeros for rows that answer for no point
+    auto own_rows = [&](const void* m, uint32_t (&f)[W / 16][4]) {
+        const __nv_bfloat16* p = (const __nv_bfloat16*)m + w.h * W;
+        pm_rows<W>(e0 >= 0 ? p + (int64_t)e0 * a.C : nullptr, e1 >= 0 ? p + (int64_t)e1 * a.C : nullptr, 0u, f);
+    };
+    own_rows(a.dout, go);
+    float lse[MAPS][2], shift[MAPS][2], E[MAPS][2], total[MAPS][2], most[2] = {0.f, 0.f};
+    const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
+    own_rows(a.out, q);
+    pm_row_dots<W>(go, q, shift[0]);
+    if (MAPS == 2) {
+        own_rows(a.second, q);
+        pm_row_dots<W>(go, q, shift[MAPS - 1]);
+        shift[0][0] += lam * shift[MAPS - 1][0];
+        shift[0][1] += lam * shift[MAPS - 1][1];
+    }
     pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr, 0u, q);
-    const __nv_bfloat16* gbase = (const __nv_bfloat16*)a.dout + w.h * W;
-    pm_rows<W>(e0 >= 0 ? gbase + (int64_t)e0 * a.C : nullptr, e1 >= 0 ? gbase + (int64_t)e1 * a.C : nullptr, 0u, go);
     const float scale2 = a.scale * PA_LOG2E;
-    float lse[MAPS][2], delta[MAPS][2], total[MAPS][2], coef[MAPS][2], most[2] = {0.f, 0.f}, dq[W / 8][4];
+    float dq[W / 8][4], pk[W / 8][4];
 #pragma unroll
     for (int n = 0; n < W / 8; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dq[n][c] = 0.f;
+        for (int c = 0; c < 4; ++c) dq[n][c] = pk[n][c] = 0.f;
 #pragma unroll
     for (int k = 0; k < MAPS; ++k)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const bool own = (r ? e1 : e0) >= 0;
             lse[k][r] = own ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + (r ? r1 : r0)] : INFINITY;
-            delta[k][r] = total[k][r] = 0.f;
-            coef[k][r] = k == 1 ? -pa_param(a.lam, w.h, a.lam_bf16) : 1.f;
+            E[k][r] = total[k][r] = 0.f;
         }
-    float unit = 0.f, per_unit = 0.f;
 
-    for (int walk = 0; walk < 2; ++walk) {
-        if (walk == 1) in.begin();
-        for (int i = 0; i * PM_CHUNK < L; ++i) {
-            const unsigned char* st = in.next(i);
-            if (!active) continue;
-            const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
-            const int4* gs = (const int4*)(st + S::GRID);
-            const int nk = L - i * PM_CHUNK;
+    for (int i = 0; i * PM_CHUNK < L; ++i) {
+        const unsigned char* st = in.next(i);
+        if (!active) continue;
+        const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
+        const int* gs = (const int*)(st + S::GRID);
+        const int nk = L - i * PM_CHUNK;
 #pragma unroll 2
-            for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
-                if (j0 >= nk) break;
-                float s[MAPS][2][4], G[1][2][4];
-                uint32_t at[2][4][3];
-                pm_products<W, MAPS>(q, ks, j0, s);
-                pm_products<W, 1>(go, vs, j0, G);
-                if (BIAS)
+        for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
+            if (j0 >= nk) break;
+            float s[MAPS][2][4], G[1][2][4];
+            pm_products<W, MAPS>(q, ks, j0, s);
+            pm_products<W, 1>(go, vs, j0, G);
+            if (BIAS)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2; ++n) {
+                    uint32_t at[4][3];
+                    pm_places<1>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int4 k = gs[j0 + 8 * n + 2 * t + c];
-                            pm_places<1>(bias, g0, k, at[n][c]);
-                            pm_places<1>(bias, g1, k, at[n][2 + c]);
-                        }
+                    for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
+                }
+            if (j0 + 16 > nk)
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float v = s[k][n][c];
-                            const int r = c >> 1;
-                            v = BIAS ? pm_bias(at[n][c], v, scale2) - lse[k][r] : fmaf(v, scale2, -lse[k][r]);
-                            if (j0 + 16 > nk && j0 + 8 * n + 2 * t + (c & 1) >= nk) v = -INFINITY;
-                            const float p = fast_exp2(v);
-                            if (walk == 0) {
-                                delta[k][r] = fmaf(p, G[0][n][c], delta[k][r]);
-                                total[k][r] += p;
-                                if (BIAS) most[r] = fmaf(p, fabsf(G[0][n][c]), most[r]);
-                            } else {
-                                s[k][n][c] = p * (G[0][n][c] - delta[k][r]);
-                            }
-                        }
-                if (walk == 1) {
-                    uint32_t p[MAPS][4];
+                        for (int c = 0; c < 4; ++c)
+                            if (j0 + 8 * n + 2 * t + (c & 1) >= nk) s[k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
+            uint32_t p[MAPS][4], d[MAPS][4];
 #pragma unroll
-                    for (int k = 0; k < MAPS; ++k) pm_pack(s[k], p[k]);
-                    pm_accumulate<W, MAPS>(p, ks, j0, dq);
-                    if (learns)
+            for (int k = 0; k < MAPS; ++k) {
+                float ds[2][4];
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const int v = __float2int_rn(s[0][n][c] * (coef[0][c >> 1] * per_unit));
-#pragma unroll
-                                for (int x = 0; x < 3; ++x) pm_add_shared(at[n][c][x] + to_hist, v);
-                            }
-                }
+                    for (int c = 0; c < 4; ++c) {
+                        const int r = c >> 1;
+                        const float v = s[k][n][c];
+                        const float pr = fast_exp2(BIAS ? v - lse[k][r] : fmaf(v, scale2, -lse[k][r]));
+                        s[k][n][c] = pr;
+                        total[k][r] += pr;
+                        ds[n][c] = pr * (G[0][n][c] - shift[k][r]);
+                        E[k][r] += ds[n][c];
+                        if (BIAS) most[r] += fabsf(ds[n][c]);
+                    }
+                pm_pack(s[k], p[k]);
+                pm_pack(ds, d[k]);
             }
-        }
-        in.end();
-        if (walk == 0) {
-            float top = 0.f;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const bool own = (r ? e1 : e0) >= 0;
-                float inv = 0.f;
-#pragma unroll
-                for (int k = 0; k < MAPS; ++k) {
-                    float d = delta[k][r], s = total[k][r];
-                    d += __shfl_xor_sync(0xffffffffu, d, 1);
-                    s += __shfl_xor_sync(0xffffffffu, s, 1);
-                    d += __shfl_xor_sync(0xffffffffu, d, 2);
-                    s += __shfl_xor_sync(0xffffffffu, s, 2);
-                    inv = own ? 1.f / s : 0.f;
-                    delta[k][r] = d * inv;
-                    coef[k][r] *= inv;
-                    const int row = r ? r1 : r0;
-                    if (t == 0 && row < L)
-                        a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = delta[k][r];
-                }
-                float v = most[r];
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                top = fmaxf(top, max_nan(0.f, v * inv + fabsf(delta[0][r])));
-            }
-            if (learns) {
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-                if (lane == 0) largest[threadIdx.x / 32] = top;
-                __syncthreads();
-                for (int i = 0; i < PM_WARPS; ++i) top = max_nan(top, largest[i]);
-                // rows that share a copy (two of each warp's to a lane's), times the largest row
-                unit = top * (float)(2 * PM_WARPS << (5 - a.copies_log2)) * (1.f / 1073741824.f);
-                per_unit = unit > 0.f ? 1.f / unit : 0.f;
-                if (!(per_unit < INFINITY)) per_unit = unit = 0.f;
-            }
+            pm_accumulate2<W, MAPS>(d, p, ks, j0, dq, pk);
         }
     }
+    in.end();
+    auto quad = [](float v) {
+        v += __shfl_xor_sync(0xffffffffu, v, 1);
+        return v + __shfl_xor_sync(0xffffffffu, v, 2);
+    };
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int e = r ? e1 : e0;
+        const int e = r ? e1 : e0, row = r ? r1 : r0;
+        float by[MAPS], eps[MAPS];
+#pragma unroll
+        for (int k = 0; k < MAPS; ++k) {
+            // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: divided out
+            const float sum = quad(total[k][r]), inv = e >= 0 ? 1.f / sum : 0.f;
+            eps[k] = quad(E[k][r]) * inv;
+            by[k] = inv * a.scale * (k == 1 ? -lam : 1.f);
+            if (t == 0 && row < L)
+                a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = e >= 0 ? shift[k][r] + eps[k] : 0.f;
+            if (BIAS && a.reach) {
+                const float reach = quad(most[r]) * inv + fabsf(eps[0]);
+                if (t == 0 && row < L) a.reach[(int64_t)w.h * a.n_pad + w.start + row] = e >= 0 ? reach : 0.f;
+            }
+        }
         if (e < 0) continue;
         uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + w.h * W);
 #pragma unroll
         for (int n = 0; n < W / 8; ++n) {
-            const float c = coef[n * 8 / (W / MAPS)][r] * a.scale;
-            dst[4 * n + t] = pack_bf16(dq[n][2 * r] * c, dq[n][2 * r + 1] * c);
-        }
-    }
-    if (learns) {
-        const int copies = 1 << a.copies_log2;
-        for (int i = threadIdx.x; i < entries; i += PM_THREADS) {
-            float v = 0.f;
-            for (int c = 0; c < copies; ++c) v += (float)hist[(i << a.copies_log2) + ((c + i) & (copies - 1))];
-            sums[i] = v * unit;
+            const int k = n * 8 / (W / MAPS);
+            dst[4 * n + t] = pack_bf16((dq[n][2 * r] - eps[k] * pk[n][2 * r]) * by[k],
+                                       (dq[n][2 * r + 1] - eps[k] * pk[n][2 * r + 1]) * by[k]);
         }
     }
 }
@@ -615,25 +628,42 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     using S = PmStage<W>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
+    __shared__ float part[4 * PM_WARPS];
     const int k0 = w.tile * PM_ROWS, L = w.L;
-    if (k0 >= L) return;
+    const bool learns = BIAS && a.bins;
+    float* bins = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * 3 * (2 * a.bnd + 1) : nullptr;
+    if (k0 >= L) {
+        if (learns)
+            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PM_THREADS) bins[i] = 0.f;
+        return;
+    }
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int warp0 = k0 + (threadIdx.x / 32) * 16, r0 = warp0 + g, r1 = r0 + 8;
     const bool there0 = r0 < L, there1 = r1 < L;
     const int e0 = there0 ? a.rows[w.start + r0] : -1, e1 = there1 ? a.rows[w.start + r1] : -1;
     const int64_t p0 = e0 >= 0 ? e0 : -(e0 + 1), p1 = e1 >= 0 ? e1 : -(e1 + 1), stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
+    PatchTable table = {};
+    if (BIAS) table = pa_table(a, w.seq);
     PmStream<W, MAPS, true, BIAS> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
-                                        smem};
+                                        table.copies_log2 + 2, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);
+    int* hist = (int*)(tab + (BIAS ? table.entries << table.copies_log2 : 0));
+    float* sums = (float*)hist + (hist - (int*)tab);
+    const uint32_t to_hist = smem_u32(hist) - smem_u32(tab);
     PmBias bias;
     int g0[3], g1[3];
+    float unit = 0.f, per_unit = 0.f;
     if (BIAS) {
-        pa_load_table(a, w.h, tab, threadIdx.x, PM_THREADS);
-        pm_bias_setup(a, smem_u32(tab), bias);
-        pm_bias_point(a, bias, e0, -1, g0);
-        pm_bias_point(a, bias, e1, -1, g1);
+        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
+        pm_bias_setup(table, smem_u32(tab), bias);
+        pm_bias_point(a, table, bias, e0, -1, g0);
+        pm_bias_point(a, table, bias, e1, -1, g1);
+        if (learns) {
+            for (int i = threadIdx.x; i < table.entries << table.copies_log2; i += PM_THREADS) hist[i] = 0;
+            for (int i = threadIdx.x; i < table.entries; i += PM_THREADS) sums[i] = 0.f;
+        }
     }
     uint32_t kf[W / 16][4], vf[W / 16][4];
     pm_rows<W>(there0 ? base + a.C + p0 * stride : nullptr, there1 ? base + a.C + p1 * stride : nullptr, 0u, kf);
@@ -647,11 +677,19 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
 
     for (int i = 0; i * PM_CHUNK < L; ++i) {
+        if (learns && i % (PA_WINDOW / PM_CHUNK) == 0) {
+            if (i) {
+                __syncthreads();
+                pa_flush(table, hist, sums, unit, PM_THREADS);
+            }
+            unit = pa_unit<PM_WARPS, true>(a, table, w.h, w.start, L, i * PM_CHUNK, part);
+            per_unit = pa_per_unit(unit);
+        }
         const unsigned char* st = in.next(i);
         if (warp0 >= L) continue;
         const uint32_t qs = smem_u32(st), os = qs + S::TILE;
         const float* aux = (const float*)(st + S::AUX);
-        const int4* gs = (const int4*)(st + S::GRID);
+        const int* gs = (const int*)(st + S::GRID);
         const int nq = L - i * PM_CHUNK;
 #pragma unroll 2
         for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
@@ -662,16 +700,12 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int j = j0 + 8 * n + 2 * t;
-                if (BIAS)
+                uint32_t at[4][3];
+                if (BIAS) {
+                    pm_places<-1>(bias, g0, g1, gs, j, at);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int4 o = gs[j + c];
-                        uint32_t at[3];
-                        pm_places<-1>(bias, g0, o, at);
-                        s[0][n][c] = pm_bias(at, s[0][n][c], scale2);
-                        pm_places<-1>(bias, g1, o, at);
-                        s[0][n][2 + c] = pm_bias(at, s[0][n][2 + c], scale2);
-                    }
+                    for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
+                }
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
                     const float2 lse = *(const float2*)(aux + k * PM_CHUNK + j);
@@ -685,6 +719,15 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
                         s[k][n][c] = p * (G[0][n][c] - d);
                     }
                 }
+                // (rows beyond the patch have no key: their lanes add nothing)
+                if (learns)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (c < 2 ? there0 : there1) {
+                            const int v = __float2int_rn(s[0][n][c] * per_unit);
+#pragma unroll
+                            for (int x = 0; x < 3; ++x) pm_add_shared(at[c][x] + to_hist, v);
+                        }
             }
             uint32_t p[MAPS][4], x[1][4];
             pm_pack(mix, x[0]);
@@ -695,6 +738,11 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         }
     }
     in.end();
+    if (learns) {
+        pa_flush(table, hist, sums, unit, PM_THREADS);
+        __syncthreads();
+        pa_store_bins(a, table, sums, bins, PM_THREADS);
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         if (!(r ? there1 : there0)) continue;
@@ -730,10 +778,12 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
-    const size_t table = BIAS ? (size_t)(3 * (2 * a.bnd + 1)) << a.copies_log2 << 2 : 0;
+    const size_t table = BIAS ? pa_table_bytes(a) : 0;
     const size_t smem = PM_STAGES * PmStage<W>::BYTES + table;
-    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem + (a.bins ? table : 0), stream);
-    if (pass == PA_COLS) return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a, smem, stream);
+    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem, stream);
+    if (pass == PA_COLS)      // the bins, and their sums
+        return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a,
+                      smem + (a.bins ? table + (size_t)(3 * (2 * a.bnd + 1)) * 4 : 0), stream);
     return a.lse ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true>, a, smem, stream)
                  : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false>, a, smem, stream);
 }

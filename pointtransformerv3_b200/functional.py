@@ -110,21 +110,21 @@ class _PatchAttention(torch.autograd.Function):
         param = None if param is None else param.contiguous()
         with torch.cuda.device(qkv.device):
             rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, status)
-            out, lse = ops.patch_attention_fwd(qkv, rows, pad.numel(), cu, heads, max_seqlen, scale, maps, param, grid,
-                                               buckets, pos_bnd, num, want_lse=keep)
+            out, lse, second = ops.patch_attention_fwd(qkv, rows, pad.numel(), cu, heads, max_seqlen, scale, maps, param,
+                                                       grid, buckets, pos_bnd, num, want_lse=keep)
         if keep:
-            ctx.save_for_backward(qkv, param, rows, cu, grid, buckets, lse)
+            ctx.save_for_backward(qkv, param, rows, cu, grid, buckets, out, lse, second)
             ctx.args = pad.numel(), heads, max_seqlen, scale, maps, pos_bnd, num
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, param, rows, cu, grid, buckets, lse = ctx.saved_tensors
+        qkv, param, rows, cu, grid, buckets, out, lse, second = ctx.saved_tensors
         n_pad, heads, max_seqlen, scale, maps, pos_bnd, num = ctx.args
         with torch.cuda.device(dout.device):
-            dqkv, dparam = ops.patch_attention_bwd(qkv, rows, n_pad, cu, lse, _aligned(dout), heads, max_seqlen, scale,
-                                                   maps, param, grid, buckets, pos_bnd, num,
+            dqkv, dparam = ops.patch_attention_bwd(qkv, rows, n_pad, cu, out, lse, second, _aligned(dout), heads,
+                                                   max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,
                                                    want_param=ctx.needs_input_grad[1])
         return (dqkv, dparam) + (None,) * 8
 
@@ -143,6 +143,8 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         raise ValueError("max_seqlen %d" % max_seqlen)
     if scale is None:
         scale = (D // maps) ** -0.5
+    if not (math.isfinite(scale) and scale):
+        raise ValueError("scale %r" % scale)
     geometry = tuple(t.contiguous() for t in (order_row, pad, unpad, cu_seqlens))
     own = status is None
     if own:

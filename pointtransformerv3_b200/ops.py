@@ -246,7 +246,7 @@ def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, grid=None, buckets
     """Points of the padded rows of a plan as patch_attention_fwd / _bwd read them (see ptv3_patch_rows)."""
     _lib.require_cuda(order_row, pad, unpad, cu_seqlens, grid, buckets, status)
     n, n_pad = order_row.numel(), pad.numel()
-    rows = torch.empty(2 * n_pad + (n_pad - n) + 1, dtype=torch.int32, device=pad.device)
+    rows = torch.empty(2 * n_pad + (n_pad - n) + 1 + 3 * (cu_seqlens.numel() - 1), dtype=torch.int32, device=pad.device)
     _lib.check(_lib.load().ptv3_patch_rows(_lib.ptr(order_row), _lib.ptr(pad), _lib.ptr(unpad), _lib.ptr(cu_seqlens), n,
                                            n_pad, cu_seqlens.numel() - 1, int(max_seqlen), _lib.ptr(grid),
                                            _lib.ptr(buckets), int(pos_bnd), int(num_buckets), _lib.ptr(rows),
@@ -269,29 +269,31 @@ def _patch_attention_args(qkv, rows, n_pad, cu, heads, max_seqlen, scale, maps, 
 
 def patch_attention_fwd(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps=1, param=None, grid=None,
                         buckets=None, pos_bnd=0, num_buckets=0, want_lse=False):
-    """(out (N, C), lse or None) of ptv3_patch_attention_fwd; param: the table with maps = 1, lam with maps = 2.
+    """(out (N, C), lse, second) of ptv3_patch_attention_fwd, the last two for patch_attention_bwd (or None); param: the table with maps = 1, lam with maps = 2.
     ``functional.attention_bias`` and ``functional.attention_diff`` are the checked forms with gradients."""
     _lib.require_cuda(qkv, rows, cu_seqlens, param, grid, buckets)
     a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
                               num_buckets)
     out = torch.empty((qkv.shape[0], a.channels), dtype=qkv.dtype, device=qkv.device)
-    lse = torch.empty((heads * maps, n_pad), dtype=torch.float32, device=qkv.device) if want_lse else None
-    a.out, a.lse = out.data_ptr(), _lib.ptr(lse)
+    lse = torch.empty((2 * heads * maps, n_pad), dtype=torch.float32, device=qkv.device) if want_lse else None
+    second = torch.empty_like(out) if want_lse and maps == 2 else None
+    a.out, a.lse, a.second = out.data_ptr(), _lib.ptr(lse), _lib.ptr(second)
     with timed("patch_attention"):
         _lib.check(_lib.load().ptv3_patch_attention_fwd(ctypes.byref(a), _lib.stream()), "ptv3_patch_attention_fwd")
-    return out, lse
+    return out, lse, second
 
 
-def patch_attention_bwd(qkv, rows, n_pad, cu_seqlens, lse, dout, heads, max_seqlen, scale, maps=1, param=None, grid=None,
-                        buckets=None, pos_bnd=0, num_buckets=0, want_param=True):
+def patch_attention_bwd(qkv, rows, n_pad, cu_seqlens, out, lse, second, dout, heads, max_seqlen, scale, maps=1,
+                        param=None, grid=None, buckets=None, pos_bnd=0, num_buckets=0, want_param=True):
     """Gradients (dqkv, gradient of param or None) of patch_attention_fwd."""
-    _lib.require_cuda(qkv, rows, cu_seqlens, lse, dout, param, grid, buckets)
+    _lib.require_cuda(qkv, rows, cu_seqlens, out, lse, second, dout, param, grid, buckets)
     lib = _lib.load()
     a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
                               num_buckets)
     dqkv = torch.empty_like(qkv)
     dparam = torch.empty_like(param) if want_param and param is not None else None
-    a.lse, a.dout, a.dqkv = lse.data_ptr(), dout.data_ptr(), dqkv.data_ptr()
+    a.out, a.lse, a.second = out.data_ptr(), lse.data_ptr(), _lib.ptr(second)
+    a.dout, a.dqkv = dout.data_ptr(), dqkv.data_ptr()
     if dparam is not None:
         setattr(a, "dlam" if maps == 2 else "dtable", dparam.data_ptr())
     nbytes = lib.ptv3_patch_attention_workspace_bytes(ctypes.byref(a))

@@ -65,7 +65,7 @@ def attention(qkv, order, pad, unpad, cu, heads, scale, maps=1, param=None, grid
         for m in range(maps):
             qm, km = q[..., m * D:(m + 1) * D], k[..., m * D:(m + 1) * D]
             s = qm @ km.transpose(1, 2) * scale
-            size = qm.abs() @ km.abs().transpose(1, 2) * scale
+            size = qm.abs() @ km.abs().transpose(1, 2) * abs(scale)
             if maps == 1 and param is not None:
                 bias = bias_of(param.double(), grid[pts], grid[pts], bound, buckets)
                 s = s + bias
@@ -92,14 +92,14 @@ def attention(qkv, order, pad, unpad, cu, heads, scale, maps=1, param=None, grid
             coef = 1.0 if m == 0 else -lam
             delta = (P * G).sum(-1, keepdim=True)
             dS = coef * P * (G - delta)
-            # what errors of P and G are relative to
+            # what errors of P and G are relative to (these sums are of absolute values, the scale's too)
             err = (P if m == 0 else lam.abs() * P) * (Ga + (P * Ga).sum(-1, keepdim=True))
             dq[..., at] = dS @ k[..., at] * scale
             dk[..., at] = dS.transpose(1, 2) @ q[..., at] * scale
-            dq_p[..., at] = dS.abs() @ k[..., at].abs() * scale
-            dk_p[..., at] = dS.abs().transpose(1, 2) @ q[..., at].abs() * scale
-            dq_e[..., at] = err @ k[..., at].abs() * scale
-            dk_e[..., at] = err.transpose(1, 2) @ q[..., at].abs() * scale
+            dq_p[..., at] = dS.abs() @ k[..., at].abs() * abs(scale)
+            dk_p[..., at] = dS.abs().transpose(1, 2) @ q[..., at].abs() * abs(scale)
+            dq_e[..., at] = err @ k[..., at].abs() * abs(scale)
+            dk_e[..., at] = err.transpose(1, 2) @ q[..., at].abs() * abs(scale)
             if maps == 2 and m == 1:
                 dparam -= delta.sum((1, 2))
                 dparam_e += (P * Ga).sum((1, 2))

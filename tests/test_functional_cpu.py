@@ -55,6 +55,8 @@ def test_cpu_tensors_are_refused():
     (lambda: F.attention_bias(t(8, 48), t(8), *args()[1:], 1, 8), "int64"),
     (lambda: F.attention_bias(t(8, 48), *args(), 1, 0), "max_seqlen"),
     (lambda: F.attention_diff(t(8, 48), t(2), *args(), 1, 8), "lam"),
+    (lambda: F.attention_bias(t(8, 48), *args(), 1, 8, 0.0), "scale"),
+    (lambda: F.attention_diff(t(8, 48), t(1), *args(), 1, 8, float("inf")), "scale"),
 ])
 def test_refusals(call, word):
     with pytest.raises(ValueError, match=word):

@@ -133,6 +133,33 @@ def test_diff_weights_and_peaks(dtype, lam, offset, size):
         R.check(got, ref, name, 32, p["longest"], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("scale", [-0.3, 0.01, 1.7])
+def test_scales(dtype, scale):
+    p = plan([150, 40], 64)
+    out, dqkv, dtable, ref = run_bias(p, 32, 2, dtype, dtype, 5, scale=scale)
+    for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dtable)):
+        R.check(got, ref, name, 16, p["longest"], dtype)
+    qkv, lam = normal(190, 192, seed=1, dtype=dtype).requires_grad_(), torch.tensor([0.6], device="cuda", requires_grad=True)
+    dout = normal(190, 64, seed=2, dtype=dtype)
+    out = F.attention_diff(qkv, lam, *geometry(p), 1, 64, scale)
+    dqkv, dlam = torch.autograd.grad(out, (qkv, lam), dout)
+    ref = R.attention(qkv.detach(), *geometry(p), 1, scale, 2, lam.detach(), dout=dout)
+    for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dlam)):
+        R.check(got, ref, name, 64, p["longest"], dtype)
+
+
+def test_a_learned_table_follows_far_and_uneven_patches():
+    """Patches whose points lie within a few cells beside ones that span thousands, and a table for offsets up to 512."""
+    p = plan([256, 256, 300], 256)
+    p["grid"][256:512] *= 400
+    p["grid"][512:] *= 45
+    for dtype in DTYPES:
+        out, dqkv, dtable, ref = run_bias(p, 32, 2, dtype, dtype, 512)
+        for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dtable)):
+            R.check(got, ref, name, 16, p["longest"], dtype)
+
+
 # --------------------------------------------------------------------------- norms and rotation
 def run_qk(n, heads, D, dtype, weight_dtype, norm, rope, extent=65536, seed=7):
     qkv = normal(n, 3 * heads * D, seed=seed, dtype=dtype).requires_grad_()
@@ -375,6 +402,10 @@ def test_bad_plans_are_reported():
     pad = p["pad"].clone()
     pad[140:142] = pad[100]
     bad(pad=pad)
+    grid = p["grid"].clone()
+    grid[17, 1] = 2 ** 22 + 1
+    with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):
+        F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=grid, table=torch.ones(9, H, device="cuda"))
     buckets, num = F.log_buckets(12, device="cuda")
     buckets[3] = num
     with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):

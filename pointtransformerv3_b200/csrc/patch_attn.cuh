@@ -15,7 +15,7 @@
 // delta in one walk: the stored result gives an estimate, delta' = dO . O (dO . O2 for the second map, whose O2 the
 // forward pass leaves too), which is off by the rounding of O alone.  With E = sum_j P (G - delta'),
 // delta = delta' + E and dQ = sum_j P (G - delta') K - E sum_j P K, exact however far the values' mean is from zero and
-// however peaked a row is.  (A walk of its own for delta: 632 us for the differential rows of 100 000 x 64, DELTA_ONE.)
+// however peaked a row is.  (A walk of its own for delta: 632 us for the differential rows of 100 000 x 64 where this takes 376.)
 //
 // dtable: a pair adds its dS to three bins, as integers in shared memory, since integer sums do not depend on the order
 // of the additions.  Their unit follows from what the queries of a window can add at most, sum_j |dS_ij| <= sum_j P |G -
@@ -32,7 +32,6 @@ constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr int PA_MAX_BOUND = 512;
 constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
 constexpr int PA_TABLE_BYTES = 360 * 32 * 4;          // shared memory that copies of a head's table may take
-constexpr int PA_WINDOW = 256;                        // queries between two clearings of the bins
 
 // What the kernels get: ptv3_patch_attention_args with the workspace carved up.
 struct PatchArgs {
@@ -81,7 +80,7 @@ __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
 struct PatchTable {
     int reach[3], first[3], entries, copies_log2;
 };
-__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq)
+__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int most_log2 = 5)
 {
     PatchTable t;
     t.entries = 0;
@@ -92,7 +91,7 @@ __device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq)
         t.entries += 2 * t.reach[c] + 1;
     }
     t.copies_log2 = 0;
-    while (t.copies_log2 < 5 && t.entries << (t.copies_log2 + 3) <= PA_TABLE_BYTES) ++t.copies_log2;
+    while (t.copies_log2 < most_log2 && t.entries << (t.copies_log2 + 3) <= PA_TABLE_BYTES) ++t.copies_log2;
     return t;
 }
 // axis and offset + bnd of an entry
@@ -121,15 +120,15 @@ static inline size_t pa_table_bytes(const PatchArgs& a)
     return all < PA_TABLE_BYTES ? all : PA_TABLE_BYTES;
 }
 
-// What the queries [q0, q0 + PA_WINDOW) of a sequence can add to a bin at most, as a unit in which 2^30 of it are that.
+// What the queries [q0, q0 + WINDOW) of a sequence can add to a bin at most, as a unit in which 2^30 of it are that.
 // With QUADS lane t of four adds queries 2 t and 2 t + 1 of every eight, to copies of its own where there are four and
 // more: the largest of four sums.  All threads of a block of 32 `WARPS`; `part`: WARPS x 4 floats
-template <int WARPS, bool QUADS>
+template <int WARPS, int WINDOW, bool QUADS>
 __device__ __forceinline__ float pa_unit(const PatchArgs& a, const PatchTable& table, int h, int start, int L, int q0,
                                          float* part)
 {
     float v = 0.f;
-    for (int j = threadIdx.x; j < PA_WINDOW; j += 32 * WARPS)
+    for (int j = threadIdx.x; j < WINDOW; j += 32 * WARPS)
         if (q0 + j < L) v += a.reach[(int64_t)h * a.n_pad + start + q0 + j];
     v += __shfl_xor_sync(0xffffffffu, v, 1);
     v += __shfl_xor_sync(0xffffffffu, v, 8);

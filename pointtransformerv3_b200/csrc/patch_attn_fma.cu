@@ -10,6 +10,8 @@ namespace ptv3 {
 constexpr int PF_THREADS = 128;
 constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
 constexpr int PF_STEP = 8;        // of which scores are held at a time
+constexpr int PF_WINDOW = 32;     // queries between two clearings of the bins: the unit is that much finer
+constexpr int PF_COPIES_LOG2 = 4; // few copies of them, so that clearing costs little
 
 template <int W, int MAPS>
 struct PfShape {
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq);
+        table = pa_table(a, seq, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq);
+        table = pa_table(a, seq, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     }
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq);
+        table = pa_table(a, seq, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1), words = BIAS ? table.entries << table.copies_log2 : 0;
@@ -327,11 +329,6 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
         const int nq = min(PF_CHUNK, L - c0);
         __syncthreads();
-        if (learns && c0 % PA_WINDOW == 0) {
-            if (c0) pa_flush(table, hist, sums, unit, PF_THREADS);
-            unit = pa_unit<PF_THREADS / 32, false>(a, table, h, start, L, c0, unit_part);
-            per_unit = pa_per_unit(unit);
-        }
         pf_stage<W>(a, base, stride, (const float*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
         for (int i = threadIdx.x; i < nq * MAPS; i += PF_THREADS) {
             const int m = i / nq, j = i % nq;
@@ -344,6 +341,14 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
         __syncthreads();
 #pragma unroll 4
         for (int j = 0; j < nq; ++j) {
+            if (learns && j % PF_WINDOW == 0) {
+                if (c0 + j) {
+                    __syncthreads();
+                    pa_flush(table, hist, sums, unit, PF_THREADS);
+                }
+                unit = pa_unit<PF_THREADS / 32, PF_WINDOW, false>(a, table, h, start, L, c0 + j, unit_part);
+                per_unit = pa_per_unit(unit);
+            }
             float s[MAPS];
             int at[3];
             pf_scores<W, MAPS>(k, Qs[j], part, s);

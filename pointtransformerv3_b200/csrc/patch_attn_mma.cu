@@ -20,6 +20,7 @@ constexpr int PM_THREADS = 256, PM_WARPS = 8;
 constexpr int PM_ROWS = 128;       // of a CTA
 constexpr int PM_CHUNK = 64;       // rows of the other side in a stage
 constexpr int PM_STAGES = 3;
+constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
 constexpr float PM_LOWEST = -1e30f;
 
@@ -677,12 +678,12 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
 
     for (int i = 0; i * PM_CHUNK < L; ++i) {
-        if (learns && i % (PA_WINDOW / PM_CHUNK) == 0) {
+        if (learns && i % (PM_WINDOW / PM_CHUNK) == 0) {
             if (i) {
                 __syncthreads();
                 pa_flush(table, hist, sums, unit, PM_THREADS);
             }
-            unit = pa_unit<PM_WARPS, true>(a, table, w.h, w.start, L, i * PM_CHUNK, part);
+            unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * PM_CHUNK, part);
             per_unit = pa_per_unit(unit);
         }
         const unsigned char* st = in.next(i);

@@ -4,11 +4,14 @@
 //   y = x r w,  r = rsqrt(mean(x^2) + eps);   (z_2i, z_2i+1) = R(angle_i) (y_2i, y_2i+1)
 //   backward:  dy = R(-angle) dz,  dw = sum over rows and heads of dy x r,  dx = r (dy w - x r mean(dy w x r))
 //
-// Bound by memory: a thread owns 16 bytes of a row, a head's sum of squares is a shuffle over the neighbouring lanes that
-// hold it.  The angles of a row serve all its heads and both of q and k, so a block computes them once, into shared
-// memory.  An angle is a coordinate times a frequency, up to 65 535 radians and more, of which only the fraction of a turn counts:
-// the frequency is held in turns as a 64-bit fraction, the product modulo 2^64 is exact, and its upper half is the
-// angle to 2^-32 of a turn (a float product would be off by 65 535 2^-24 = 0.004 radians).
+// Bound by memory and, in 16 bits, as much by instructions: a thread keeps one 16-byte column of the rows that it visits,
+// so that its head's place, its weights and its part (query, key, value) are settled once, and works on packed pairs of floats; a head's sum of
+// squares is a shuffle over the neighbouring lanes that hold it.  The angles of a row serve all its heads and both of q and k, so a block
+// computes them once, into shared memory.  An angle is a coordinate times a frequency, up to 65 535 radians and more, of which
+// only the fraction of a turn counts: the frequency is held in turns as a 64-bit fraction, the product modulo 2^64 is exact,
+// and its upper half is the angle to 2^-32 of a turn (a float product would be off by 65 535 2^-24 = 0.004 radians).
+// 407 678 x 64 forward, bf16: 81 us with threads that walked vectors of a row in order (176 instructions a vector), QK_ONE
+// here; 105 505 x 128 backward 96 (318), 64 here.
 #include <math.h>
 
 #include "common.cuh"
@@ -17,30 +20,38 @@
 
 namespace ptv3 {
 
-constexpr int QK_THREADS = 256;
-constexpr int QK_UNROLL = 4;          // vectors of a thread per block of rows
+constexpr int QK_THREADS = 384;       // a multiple of the vectors of most rows (3 channels / 8 or / 4)
+constexpr int QK_PASSES = 4;          // rows of a thread per round
 constexpr int QK_MAX_FREQ = 21;       // frequencies of an axis, D = 128
+
+// floor(i / d) for i d < 2^32 as a product
+struct QkDiv {
+    uint32_t d, m;
+    __host__ QkDiv(uint32_t d = 1) : d(d), m(d == 1 ? 0 : (uint32_t)((0xffffffffull + d) / d)) {}
+    __device__ int operator()(int i) const { return d == 1 ? i : (int)__umulhi((uint32_t)i, m); }
+};
 
 struct QkArgs {
     const void *qkv, *qw, *kw;
     const int32_t* grid;
     const void* dout;
     void* out;
-    float* partial;        // blocks x 2 D
+    float* partial;        // (blocks, 2 D)
     int64_t n;
     int vec_row, vec_c;    // 16-byte vectors of a row, of a third of it
-    int rows;              // of a block
+    int columns, rows;     // of a block at a time: vectors, rows
     int D, p, w_bf16;
     float eps;
+    QkDiv by_pairs, by_p;
     uint64_t freq[QK_MAX_FREQ];     // in turns, times 2^64
 };
 
-// cos and sin of every pair's angle for the rows of a block
+// cos and sin of every pair's angle for `rows` rows
 __device__ __forceinline__ void qk_angles(const QkArgs& a, int64_t row0, int rows, float2* cs)
 {
     const int pairs = 3 * a.p;
     for (int i = threadIdx.x; i < rows * pairs; i += QK_THREADS) {
-        const int r = i / pairs, j = i - r * pairs, axis = j / a.p;
+        const int r = a.by_pairs(i), j = i - r * pairs, axis = a.by_p(j);
         const uint64_t turn = (uint64_t)(int64_t)a.grid[3 * (row0 + r) + axis] * a.freq[j - axis * a.p];
         // signed fraction of a turn, of which sincospif wants twice as many half turns
         const float half = (float)(int32_t)(turn >> 32) * (2.f / 4294967296.f);
@@ -48,16 +59,50 @@ __device__ __forceinline__ void qk_angles(const QkArgs& a, int64_t row0, int row
     }
 }
 
+// 16 bytes as packed pairs of floats
+template <typename T> struct QkPairs;
+template <> struct QkPairs<float> {
+    static constexpr int N = 2;
+    __device__ static void load(const uint4& r, uint64_t* p)
+    {
+        p[0] = pack2u(r.x, r.y);
+        p[1] = pack2u(r.z, r.w);
+    }
+    __device__ static uint4 store(const uint64_t* p)
+    {
+        return make_uint4((uint32_t)p[0], (uint32_t)(p[0] >> 32), (uint32_t)p[1], (uint32_t)(p[1] >> 32));
+    }
+};
+template <> struct QkPairs<__nv_bfloat16> {
+    static constexpr int N = 4;
+    __device__ static void load(const uint4& r, uint64_t* p)
+    {
+        p[0] = unpack_bf16x2(r.x);
+        p[1] = unpack_bf16x2(r.y);
+        p[2] = unpack_bf16x2(r.z);
+        p[3] = unpack_bf16x2(r.w);
+    }
+    __device__ static uint32_t one(uint64_t p)
+    {
+        float x, y;
+        unpack2(p, x, y);
+        return pack_bf16(x, y);
+    }
+    __device__ static uint4 store(const uint64_t* p) { return make_uint4(one(p[0]), one(p[1]), one(p[2]), one(p[3])); }
+};
+
+// the first `turned` pairs rotated
 template <int N>
-__device__ __forceinline__ void qk_rotate(float (&y)[N], const float2* cs, int first, int pairs, float sign)
+__device__ __forceinline__ void qk_rotate(uint64_t (&y)[N], const float2* cs, int turned, bool back)
 {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i)
-        if (first + i < pairs) {
-            const float2 t = cs[first + i];
-            const float u = y[2 * i], v = y[2 * i + 1], s = t.y * sign;
-            y[2 * i] = u * t.x - v * s;
-            y[2 * i + 1] = u * s + v * t.x;
+    for (int i = 0; i < N; ++i)
+        if (i < turned) {
+            const float2 t = cs[i];
+            const float s = back ? -t.y : t.y;
+            float u, v;
+            unpack2(y[i], u, v);
+            y[i] = pack2(fmaf(u, t.x, -v * s), fmaf(u, s, v * t.x));
         }
 }
 
@@ -69,119 +114,119 @@ __device__ __forceinline__ float qk_head_sum(float v, int lanes)
 }
 
 template <typename T, bool NORM, bool BACK>
-__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkArgs a)
+__global__ void __launch_bounds__(QK_THREADS, NORM && BACK ? 2 : 3) qk_norm_rope_kernel(const QkArgs a)
 {
-    using V = Vec<T>;
-    using Raw = typename V::Raw;
-    extern __shared__ float2 cs[];
-    const int lanes = a.D / V::N;                       // of a head: a power of two that divides a warp
-    const int at = threadIdx.x % lanes * V::N;          // this thread's place in a head, always the same one
+    using P = QkPairs<T>;
+    constexpr int N = P::N;
+    extern __shared__ float2 angles[];
+    __shared__ float sums[NORM && BACK ? QK_THREADS : 1][2 * N + 1];
+    const int lanes = a.D / (2 * N);                    // of a head: a power of two that divides a warp
     const int pairs = a.grid ? 3 * a.p : 0;
-    float w[2][V::N], dw[2][V::N];
+    // this thread's column, and its row among those of a pass (threads beyond the last have none)
+    const int c = blockIdx.y * QK_THREADS + threadIdx.x % a.columns, r0 = threadIdx.x / a.columns;
+    const bool have = c < a.vec_row && r0 < a.rows;
+    const int part = !have ? 2 : c < a.vec_c ? 0 : c < 2 * a.vec_c ? 1 : 2;
+    const int first = threadIdx.x % lanes * N;          // pair of its head (all threads of a head have such neighbours)
+    const int turned = part == 2 ? 0 : pairs - first;
+    uint64_t w[N], dw[N];
     if (NORM) {
+        const void* weights = part == 0 ? a.qw : a.kw;
 #pragma unroll
-        for (int i = 0; i < V::N; ++i) {
-            w[0][i] = a.w_bf16 ? __bfloat162float(((const __nv_bfloat16*)a.qw)[at + i]) : ((const float*)a.qw)[at + i];
-            w[1][i] = a.w_bf16 ? __bfloat162float(((const __nv_bfloat16*)a.kw)[at + i]) : ((const float*)a.kw)[at + i];
-            dw[0][i] = dw[1][i] = 0.f;
+        for (int i = 0; i < N; ++i) {
+            w[i] = a.w_bf16 ? unpack_bf16x2(((const uint32_t*)weights)[first + i])
+                            : pack2(((const float*)weights)[2 * (first + i)], ((const float*)weights)[2 * (first + i) + 1]);
+            dw[i] = 0;
         }
     }
-    const Raw* in = (const Raw*)a.qkv;
-    const Raw* grad = (const Raw*)a.dout;
-    Raw* out = (Raw*)a.out;
-    for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < a.n; row0 += (int64_t)gridDim.x * a.rows) {
-        const int rows = (int)min((int64_t)a.rows, a.n - row0);
-        const int count = rows * a.vec_row;
-        const int64_t base = row0 * a.vec_row;
+    const uint4* in = (const uint4*)a.qkv;
+    const uint4* grad = (const uint4*)a.dout;
+    uint4* out = (uint4*)a.out;
+    const int rows = a.rows * QK_PASSES;
+    int turn = 0;
+    for (int64_t row0 = (int64_t)blockIdx.x * rows; row0 < a.n; row0 += (int64_t)gridDim.x * rows, turn ^= 1) {
+        const int left = (int)min((int64_t)rows, a.n - row0);
+        // two sets of angles in turn: nobody is still reading the one before the last
+        float2* cs = angles + turn * rows * pairs;
+        uint4 x[QK_PASSES], g[QK_PASSES];
+        const int64_t base = (row0 + r0) * a.vec_row + c, step = (int64_t)a.rows * a.vec_row;
+        // (rows are asked for ahead of their angles, so that one latency hides the other)
+#pragma unroll
+        for (int u = 0; u < QK_PASSES; ++u)
+            if (have && r0 + u * a.rows < left) {
+                if (BACK) g[u] = grad[base + u * step];
+                if (!BACK || (NORM && part != 2)) x[u] = in[base + u * step];
+            }
         if (pairs) {
-            __syncthreads();
-            qk_angles(a, row0, rows, cs);
+            qk_angles(a, row0, left, cs);
             __syncthreads();
         }
-        for (int first = 0; first < count; first += QK_THREADS * QK_UNROLL) {
-            Raw x[QK_UNROLL], gx[QK_UNROLL];
 #pragma unroll
-            for (int u = 0; u < QK_UNROLL; ++u) {
-                const int i = first + u * QK_THREADS + threadIdx.x;
-                if (i < count) {
-                    if (BACK) gx[u] = grad[base + i];
-                    if (!BACK || NORM) x[u] = in[base + i];
-                }
+        for (int u = 0; u < QK_PASSES; ++u) {
+            const int r = r0 + u * a.rows;
+            const bool live = have && r < left;
+            const float2* turns = cs + (live ? r * pairs + first : 0);
+            uint64_t y[N], z[N];
+            float inv = 0.f;
+            if (!BACK || NORM) P::load(x[u], y);
+            if (NORM) {
+                uint64_t s = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) s = fma2(y[i], y[i], s);
+                inv = rsqrtf(qk_head_sum(hsum2(s), lanes) / (float)a.D + a.eps);
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = mul2(y[i], pack2(inv, inv));
             }
+            if (!BACK) {
+                if (NORM)
 #pragma unroll
-            for (int u = 0; u < QK_UNROLL; ++u) {
-                const int i = first + u * QK_THREADS + threadIdx.x;
-                const bool live = i < count;
-                const int r = live ? i / a.vec_row : 0, c = i - r * a.vec_row;
-                // (all lanes of a head are queries, keys or values together, but lanes of a warp need not be)
-                const int part = live ? (c < a.vec_c ? 0 : c < 2 * a.vec_c ? 1 : 2) : 2;
-                float y[V::N], g[V::N];
-                if (!BACK) {
-                    V::unpack(x[u], y);
-                    if (NORM) {
-                        float s = 0.f;
+                    for (int i = 0; i < N; ++i) y[i] = mul2(y[i], w[i]);
+                qk_rotate(y, turns, turned, false);
+                if (live) out[base + u * step] = part == 2 ? x[u] : P::store(y);
+            } else {
+                P::load(g[u], z);
+                qk_rotate(z, turns, turned, true);
+                if (NORM) {
+                    uint64_t m = 0;
 #pragma unroll
-                        for (int k = 0; k < V::N; ++k) s = fmaf(y[k], y[k], s);
-                        const float inv = rsqrtf(qk_head_sum(s, lanes) / (float)a.D + a.eps);
-#pragma unroll
-                        for (int k = 0; k < V::N; ++k) y[k] *= inv * (part == 0 ? w[0][k] : w[1][k]);
+                    for (int i = 0; i < N; ++i) {
+                        if (live) dw[i] = fma2(z[i], y[i], dw[i]);
+                        z[i] = mul2(z[i], w[i]);
+                        m = fma2(z[i], y[i], m);
                     }
-                    qk_rotate(y, cs + r * pairs, at / 2, pairs, 1.f);
-                    if (live) out[base + i] = part == 2 ? x[u] : V::pack(y);
-                } else {
-                    V::unpack(gx[u], g);
-                    qk_rotate(g, cs + r * pairs, at / 2, pairs, -1.f);
-                    if (NORM) {
-                        V::unpack(x[u], y);
-                        float s = 0.f, m = 0.f;
+                    const float mean = -qk_head_sum(hsum2(m), lanes) / (float)a.D;
 #pragma unroll
-                        for (int k = 0; k < V::N; ++k) s = fmaf(y[k], y[k], s);
-                        const float inv = rsqrtf(qk_head_sum(s, lanes) / (float)a.D + a.eps);
-#pragma unroll
-                        for (int k = 0; k < V::N; ++k) {
-                            y[k] *= inv;
-                            if (part == 0) dw[0][k] = fmaf(g[k], y[k], dw[0][k]);
-                            if (part == 1) dw[1][k] = fmaf(g[k], y[k], dw[1][k]);
-                            g[k] *= part == 0 ? w[0][k] : w[1][k];
-                            m = fmaf(g[k], y[k], m);
-                        }
-                        m = qk_head_sum(m, lanes) / (float)a.D;
-#pragma unroll
-                        for (int k = 0; k < V::N; ++k) g[k] = inv * (g[k] - y[k] * m);
-                    }
-                    if (live) out[base + i] = part == 2 ? gx[u] : V::pack(g);
+                    for (int i = 0; i < N; ++i) z[i] = mul2(fma2(y[i], pack2(mean, mean), z[i]), pack2(inv, inv));
                 }
+                if (live) out[base + u * step] = part == 2 ? g[u] : P::store(z);
             }
         }
     }
     if (NORM && BACK) {
-        // sums of a block: lanes of one place in a head, then the warps, in a fixed order
-        __shared__ float sums[QK_THREADS / 32][2 * 128];
+        // a block's sums: its threads of one part and place, in their order
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int k = 0; k < V::N; ++k) {
-                float v = dw[q][k];
-                for (int d = lanes; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-                if ((threadIdx.x & 31) < lanes) sums[threadIdx.x / 32][q * a.D + at + k] = v;
-            }
+        for (int i = 0; i < N; ++i) unpack2(dw[i], sums[threadIdx.x][2 * i], sums[threadIdx.x][2 * i + 1]);
         __syncthreads();
+        const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
         for (int i = threadIdx.x; i < 2 * a.D; i += QK_THREADS) {
+            const int key = i >= a.D, d = i - key * a.D;
+            const int lo = max(key * a.vec_c - (int)blockIdx.y * QK_THREADS, 0);
+            const int hi = min((key + 1) * a.vec_c - (int)blockIdx.y * QK_THREADS, a.columns);
             float v = 0.f;
-#pragma unroll
-            for (int k = 0; k < QK_THREADS / 32; ++k) v += sums[k][i];
-            a.partial[(int64_t)blockIdx.x * 2 * a.D + i] = v;
+            for (int r = 0; r < a.rows; ++r)
+                for (int k = lo + d / (2 * N); k < hi; k += lanes) v += sums[r * a.columns + k][d % (2 * N)];
+            a.partial[block * 2 * a.D + i] = v;
         }
     }
 }
 
 // weights' gradients: a warp per value adds the blocks' sums
-__global__ void __launch_bounds__(QK_THREADS) qk_weights_kernel(const float* partial, int blocks, int D, void* dq, void* dk,
+__global__ void __launch_bounds__(256) qk_weights_kernel(const float* partial, int blocks, int D, void* dq, void* dk,
                                                                 int bf16)
 {
-    const int i = (blockIdx.x * QK_THREADS + threadIdx.x) / 32, lane = threadIdx.x & 31;
+    const int i = (blockIdx.x * 256 + threadIdx.x) / 32, lane = threadIdx.x & 31;
     if (i >= 2 * D) return;
     float v = 0.f;
+#pragma unroll 8
     for (int b = lane; b < blocks; b += 32) v += partial[(int64_t)b * 2 * D + i];
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -191,14 +236,13 @@ __global__ void __launch_bounds__(QK_THREADS) qk_weights_kernel(const float* par
     else ((float*)to)[i % D] = v;
 }
 
-constexpr int QK_MAX_BLOCKS = SMS * 8;
-
-// rows of a block, and how many blocks: a block's vectors once through its threads, on long inputs a few times over
-static int qk_rows(int vec_row) { return vec_row >= QK_THREADS * QK_UNROLL ? 1 : QK_THREADS * QK_UNROLL / vec_row; }
-static int qk_blocks(int64_t n, int vec_row)
+// Blocks of rows: as many as are resident; and of columns, for rows of more vectors than a block has threads
+constexpr int QK_MAX_BLOCKS = SMS * 3;
+static dim3 qk_grid(int64_t n, int vec_row)
 {
-    const int64_t b = (n + qk_rows(vec_row) - 1) / qk_rows(vec_row);
-    return (int)(b < QK_MAX_BLOCKS ? b : QK_MAX_BLOCKS);
+    const int rows = (vec_row < QK_THREADS ? QK_THREADS / vec_row : 1) * QK_PASSES, wide = ceil_div(vec_row, QK_THREADS);
+    const int64_t b = (n + rows - 1) / rows, most = ceil_div(QK_MAX_BLOCKS, wide);
+    return dim3((unsigned)(b < most ? b : most), wide);
 }
 
 static int qk_check(const char* what, const void* qkv, const void* qw, const void* kw, int weight_dtype,
@@ -212,7 +256,7 @@ static int qk_check(const char* what, const void* qkv, const void* qw, const voi
     PTV3_REQUIRE((dtype == PTV3_DTYPE_F32 || dtype == PTV3_DTYPE_BF16) &&
                      (weight_dtype == PTV3_DTYPE_F32 || weight_dtype == PTV3_DTYPE_BF16),
                  PTV3_ERR_UNSUPPORTED, "%s: dtypes %d, %d", what, dtype, weight_dtype);
-    PTV3_REQUIRE(channels <= 1 << 20, PTV3_ERR_UNSUPPORTED, "%s: %d channels", what, channels);
+    PTV3_REQUIRE(channels <= 1 << 16, PTV3_ERR_UNSUPPORTED, "%s: %d channels", what, channels);
     PTV3_REQUIRE(!qw == !kw && (qw || grid), PTV3_ERR_INVALID_ARGUMENT,
                  "%s: weights of both queries and keys, coordinates, or all three", what);
     PTV3_REQUIRE(!grid || base > 0, PTV3_ERR_INVALID_ARGUMENT, "%s: base %g", what, base);
@@ -233,11 +277,14 @@ static QkArgs qk_args(const void* qkv, const void* qw, const void* kw, int weigh
     a.n = n;
     a.vec_c = channels * (dtype == PTV3_DTYPE_F32 ? 4 : 2) / 16;
     a.vec_row = 3 * a.vec_c;
-    a.rows = qk_rows(a.vec_row);
+    a.columns = a.vec_row < QK_THREADS ? a.vec_row : QK_THREADS;
+    a.rows = QK_THREADS / a.columns;
     a.D = channels / heads;
     a.p = a.D / 6;
     a.w_bf16 = weight_dtype == PTV3_DTYPE_BF16;
     a.eps = eps;
+    a.by_pairs = QkDiv(3 * a.p);
+    a.by_p = QkDiv(a.p);
     // 2^64 base^(-k/p) / 2 pi; whole turns of frequencies above one turn a cell fall away
     for (int k = 0; grid && k < a.p; ++k) {
         const double turns = pow(base, -(double)k / a.p) * 0.15915494309189533577;
@@ -249,10 +296,10 @@ static QkArgs qk_args(const void* qkv, const void* qw, const void* kw, int weigh
 template <typename T, bool BACK>
 static int launch_qk(const QkArgs& a, const char* what, cudaStream_t stream)
 {
-    const int blocks = qk_blocks(a.n, a.vec_row);
-    const size_t smem = a.grid ? (size_t)a.rows * 3 * a.p * sizeof(float2) : 0;
-    if (a.qw) qk_norm_rope_kernel<T, true, BACK><<<blocks, QK_THREADS, smem, stream>>>(a);
-    else qk_norm_rope_kernel<T, false, BACK><<<blocks, QK_THREADS, smem, stream>>>(a);
+    const dim3 grid = qk_grid(a.n, a.vec_row);
+    const size_t smem = a.grid ? (size_t)a.rows * QK_PASSES * 3 * a.p * 2 * sizeof(float2) : 0;
+    if (a.qw) qk_norm_rope_kernel<T, true, BACK><<<grid, QK_THREADS, smem, stream>>>(a);
+    else qk_norm_rope_kernel<T, false, BACK><<<grid, QK_THREADS, smem, stream>>>(a);
     count_launches(1);
     return check_launch(what);
 }
@@ -276,7 +323,10 @@ extern "C" int ptv3_qk_norm_rope_fwd(const void* qkv, const void* q_weight, cons
 extern "C" size_t ptv3_qk_norm_rope_workspace_bytes(int64_t n, int channels, int heads)
 {
     if (n <= 0 || channels < 1 || heads < 1) return 0;
-    return (size_t)QK_MAX_BLOCKS * 2 * (channels / heads) * sizeof(float);
+    const dim3 most = qk_grid(n, 3 * channels * 4 / 16), least = qk_grid(n, 3 * channels * 2 / 16);     // fp32, bf16
+    const size_t blocks = (size_t)most.x * most.y > (size_t)least.x * least.y ? (size_t)most.x * most.y
+                                                                             : (size_t)least.x * least.y;
+    return blocks * 2 * (channels / heads) * sizeof(float);
 }
 
 extern "C" int ptv3_qk_norm_rope_bwd(const void* qkv, const void* q_weight, const void* k_weight, int weight_dtype,
@@ -304,8 +354,9 @@ extern "C" int ptv3_qk_norm_rope_bwd(const void* qkv, const void* q_weight, cons
         if (rc != PTV3_OK) return rc;
     }
     if (q_weight) {
-        qk_weights_kernel<<<ceil_div(2 * a.D * 32, QK_THREADS), QK_THREADS, 0, s>>>(
-            a.partial, n > 0 ? qk_blocks(n, a.vec_row) : 0, a.D, dq_weight, dk_weight, a.w_bf16);
+        const dim3 grid = qk_grid(n, a.vec_row);
+        qk_weights_kernel<<<ceil_div(2 * a.D * 32, 256), 256, 0, s>>>(a.partial, n > 0 ? (int)(grid.x * grid.y) : 0, a.D,
+                                                                      dq_weight, dk_weight, a.w_bf16);
         count_launches(1);
     }
     return check_launch(what);

@@ -11,6 +11,7 @@ All of them run on the current stream of the tensors' device, keep nothing betwe
 that is captured wants leaves which no eager graph holds at that time (``x.detach().requires_grad_()``): torch ties a leaf's
 gradient to the stream of the graph that met it first.  Gradients are of first order, and the same bits on every run.
 """
+import contextlib
 import math
 
 import torch
@@ -34,9 +35,22 @@ def log_buckets(bound, exact=8, per_octave=4, device=None):
 
 def _same_device(first, *others):
     _lib.require_cuda(first, *others)
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError("tensors on %s and %s" % (first.device, t.device))
+        if t is not None and t.device != device:
+            raise ValueError("tensors on %s and %s" % (device, t.device))
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes the tensors' device the current one, where it is another (the guard costs as much as a launch)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _aligned(t):
@@ -61,11 +75,7 @@ def _int32(t, shape, what):
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, grid, q_weight, k_weight, heads, eps, base):
-        qkv = _aligned(qkv)
-        if q_weight is not None:
-            q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
-        with torch.cuda.device(qkv.device):
-            out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
+        out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
         ctx.save_for_backward(qkv if q_weight is not None else None, grid, q_weight, k_weight)
         ctx.args = heads, eps, base
         return out
@@ -75,7 +85,7 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, grid, q_weight, k_weight = ctx.saved_tensors
         heads, eps, base = ctx.args
-        with torch.cuda.device(dout.device):
+        with _on(dout.device):
             dqkv, dq, dk = ops.qk_norm_rope_bwd(qkv, _aligned(dout), heads, grid, q_weight, k_weight, eps, base)
         return dqkv, None, dq, dk, None, None, None
 
@@ -97,24 +107,31 @@ def qk_norm_rope(qkv, heads, grid_coord=None, q_weight=None, k_weight=None, eps=
         raise ValueError("weights must be (%d,) of one type" % D)
     if grid_coord is not None:
         grid_coord = _int32(grid_coord, (qkv.shape[0], 3), "grid_coord")
-    return _QkNormRope.apply(qkv, grid_coord, q_weight, k_weight, int(heads), float(eps), float(base))
+    qkv = _aligned(qkv)
+    if q_weight is not None:
+        q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    with _on(qkv.device):
+        if not _wants_grad(qkv, q_weight, k_weight):
+            return ops.qk_norm_rope_fwd(qkv, int(heads), grid_coord, q_weight, k_weight, float(eps), float(base))
+        return _QkNormRope.apply(qkv, grid_coord, q_weight, k_weight, int(heads), float(eps), float(base))
 
 
 # --------------------------------------------------------------------------- attention
+def _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, keep):
+    order, pad, unpad, cu = geometry
+    grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
+    rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, status)
+    return (rows,) + ops.patch_attention_fwd(qkv, rows, pad.shape[0], cu, heads, max_seqlen, scale, maps, param, grid,
+                                             buckets, pos_bnd, num, want_lse=keep)
+
+
 class _PatchAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, keep):
-        order, pad, unpad, cu = geometry
+    def forward(ctx, qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status):
+        rows, out, lse, second = _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, True)
         grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
-        qkv = _aligned(qkv)
-        param = None if param is None else param.contiguous()
-        with torch.cuda.device(qkv.device):
-            rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, status)
-            out, lse, second = ops.patch_attention_fwd(qkv, rows, pad.numel(), cu, heads, max_seqlen, scale, maps, param,
-                                                       grid, buckets, pos_bnd, num, want_lse=keep)
-        if keep:
-            ctx.save_for_backward(qkv, param, rows, cu, grid, buckets, out, lse, second)
-            ctx.args = pad.numel(), heads, max_seqlen, scale, maps, pos_bnd, num
+        ctx.save_for_backward(qkv, param, rows, geometry[3], grid, buckets, out, lse, second)
+        ctx.args = geometry[1].shape[0], heads, max_seqlen, scale, maps, pos_bnd, num
         return out
 
     @staticmethod
@@ -122,11 +139,11 @@ class _PatchAttention(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, param, rows, cu, grid, buckets, out, lse, second = ctx.saved_tensors
         n_pad, heads, max_seqlen, scale, maps, pos_bnd, num = ctx.args
-        with torch.cuda.device(dout.device):
+        with _on(dout.device):
             dqkv, dparam = ops.patch_attention_bwd(qkv, rows, n_pad, cu, out, lse, second, _aligned(dout), heads,
                                                    max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,
                                                    want_param=ctx.needs_input_grad[1])
-        return (dqkv, dparam) + (None,) * 8
+        return (dqkv, dparam) + (None,) * 7
 
 
 def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seqlen, scale, maps, status):
@@ -146,17 +163,19 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
     if not (math.isfinite(scale) and scale):
         raise ValueError("scale %r" % scale)
     geometry = tuple(t.contiguous() for t in (order_row, pad, unpad, cu_seqlens))
+    qkv, param = _aligned(qkv), None if param is None else param.contiguous()
     own = status is None
-    if own:
-        if torch.cuda.is_current_stream_capturing():
-            raise ValueError("a captured call needs a status word of the caller's: one of its own is read at once")
-        with torch.cuda.device(qkv.device):
+    if own and torch.cuda.is_current_stream_capturing():
+        raise ValueError("a captured call needs a status word of the caller's: one of its own is read at once")
+    with _on(qkv.device):
+        if own:
             status = ops.new_status(qkv.device)
-    # (the logarithms of the sums are only wanted where a backward pass may follow)
-    keep = torch.is_grad_enabled() and (qkv.requires_grad or (param is not None and param.requires_grad))
-    out = _PatchAttention.apply(qkv, param, geometry, bias, int(heads), int(max_seqlen), float(scale), maps, status, keep)
-    if own:
-        with torch.cuda.device(qkv.device):
+        args = (qkv, param, geometry, bias, int(heads), int(max_seqlen), float(scale), maps, status)
+        if _wants_grad(qkv, param):
+            out = _PatchAttention.apply(*args)
+        else:
+            out = _patch_forward(*args, False)[1]
+        if own:
             _lib.raise_on_status(status, "ptv3_patch_attention_fwd")
     return out
 

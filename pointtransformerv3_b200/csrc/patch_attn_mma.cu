@@ -18,18 +18,23 @@ namespace ptv3 {
 
 constexpr int PM_THREADS = 256, PM_WARPS = 8;
 constexpr int PM_ROWS = 128;       // of a CTA
-constexpr int PM_CHUNK = 64;       // rows of the other side in a stage
+// Rows of the other side in a stage.  Warps meet once a chunk: with 64 rows instead of 256 the three kernels of 100 000 x 64,
+// differential, take 333, 378 and 386 us instead of 311, 343 and 349; a bias needs the room for its table.
+template <int W, bool BIAS>
+struct PmChunk {
+    static constexpr int N = W == 16 && !BIAS ? 256 : 64;
+};
 constexpr int PM_STAGES = 3;
 constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
 constexpr float PM_LOWEST = -1e30f;
 
-template <int W>
+template <int W, int CH>
 struct PmStage {
-    static constexpr int TILE = PM_CHUNK * W * 2;      // bytes of a matrix
+    static constexpr int TILE = CH * W * 2;            // bytes of a matrix
     static constexpr int AUX = 2 * TILE;               // two words of each map and row
-    static constexpr int GRID = AUX + 4 * PM_CHUNK * 4;
-    static constexpr int BYTES = GRID + 3 * PM_CHUNK * 4;
+    static constexpr int GRID = AUX + 4 * CH * 4;
+    static constexpr int BYTES = GRID + 3 * CH * 4;
 };
 
 // byte offset of 16-byte chunk c of row r: chunks are exchanged so that the eight rows of an ldmatrix lie in different banks
@@ -65,7 +70,9 @@ __device__ __forceinline__ void pm_add_shared(uint32_t addr, int v)
 // The other side's rows: x and y (head h's W values of each), two words of each map (AUX), coordinates (BIAS)
 template <int W, int MAPS, bool AUX, bool BIAS>
 struct PmStream {
-    using S = PmStage<W>;
+    static constexpr int CH = PmChunk<W, BIAS>::N;
+    static constexpr int NR = CH / 64, NA = AUX ? (2 * MAPS * CH + PM_THREADS - 1) / PM_THREADS : 1;
+    using S = PmStage<W, CH>;
     const PatchArgs& a;
     const __nv_bfloat16 *x, *y;
     int64_t xs, ys;
@@ -73,17 +80,17 @@ struct PmStream {
     bool owners;             // rows of y that answer for no point are taken as zeros
     int step;                // coordinates are kept times 2^step
     unsigned char* smem;
-    int e, eg, ea, g[3];
-    float aux;
+    int e[NR], eg, ea[NA], g[3];
+    float aux[NA];
 
     __device__ __forceinline__ int row_of(int chunk, int j) const
     {
-        const int r = chunk * PM_CHUNK + j;
+        const int r = chunk * CH + j;
         return r < L ? a.rows[start + r] : INT_MIN;
     }
     __device__ __forceinline__ void fetch_grid()
     {
-        if (BIAS && threadIdx.x < PM_CHUNK && eg != INT_MIN) {
+        if (BIAS && threadIdx.x < CH && eg != INT_MIN) {
             const int64_t p = eg >= 0 ? eg : -(eg + 1);
 #pragma unroll
             for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
@@ -91,44 +98,54 @@ struct PmStream {
     }
     __device__ __forceinline__ void fetch_aux(int chunk)
     {
-        if (AUX && threadIdx.x < 2 * MAPS * PM_CHUNK) {
-            const int j = threadIdx.x % PM_CHUNK, what = threadIdx.x / PM_CHUNK, r = chunk * PM_CHUNK + j;
-            ea = row_of(chunk, j);
-            aux = 0.f;
-            if (r < L) aux = (what < MAPS ? a.lse : a.delta)[(int64_t)(h * MAPS + what % MAPS) * a.n_pad + start + r];
-        }
+        if (AUX)
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int k = threadIdx.x + i * PM_THREADS, j = k % CH, what = k / CH, r = chunk * CH + j;
+                ea[i] = k < 2 * MAPS * CH ? row_of(chunk, j) : INT_MIN;
+                aux[i] = 0.f;
+                if (ea[i] != INT_MIN)
+                    aux[i] = (what < MAPS ? a.lse : a.delta)[(int64_t)(h * MAPS + what % MAPS) * a.n_pad + start + r];
+            }
     }
     // what issue(chunk) needs in registers
     __device__ __forceinline__ void fetch(int chunk)
     {
-        e = row_of(chunk, threadIdx.x >> 2);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) e[i] = row_of(chunk, (threadIdx.x >> 2) + 64 * i);
         fetch_grid();
-        if (BIAS && threadIdx.x < PM_CHUNK) eg = row_of(chunk + 1, threadIdx.x);
+        if (BIAS && threadIdx.x < CH) eg = row_of(chunk + 1, threadIdx.x);
         fetch_aux(chunk);
     }
     __device__ __forceinline__ void issue(int chunk)
     {
-        if (chunk * PM_CHUNK < L) {
+        if (chunk * CH < L) {
             unsigned char* st = smem + chunk % PM_STAGES * S::BYTES;
-            const int r = threadIdx.x >> 2;
-            const bool there = e != INT_MIN;
-            const int64_t p = !there ? 0 : e >= 0 ? e : -(e + 1);
             constexpr int CPR = W / 8;
 #pragma unroll
-            for (int i = 0; i < CPR / 2; ++i) {
-                const int o = (threadIdx.x & 3) + 4 * i, c = o % CPR;
-                if (o < CPR) cp_async16_zfill(smem_u32(st) + pm_offset<W>(r, c), x + p * xs + 8 * c, there);
-                else cp_async16_zfill(smem_u32(st) + S::TILE + pm_offset<W>(r, c), y + p * ys + 8 * c,
-                                      there && !(owners && e < 0));
-            }
-            if (AUX && threadIdx.x < 2 * MAPS * PM_CHUNK) {
-                const bool lse = threadIdx.x / PM_CHUNK < MAPS;
-                // (rows that are not there, or answer for no point: probabilities of nothing)
-                ((float*)(st + S::AUX))[threadIdx.x] = ea >= 0 ? aux : lse ? INFINITY : 0.f;
-            }
-            if (BIAS && threadIdx.x < PM_CHUNK)
+            for (int n = 0; n < NR; ++n) {
+                const int r = (threadIdx.x >> 2) + 64 * n;
+                const bool there = e[n] != INT_MIN;
+                const int64_t p = !there ? 0 : e[n] >= 0 ? e[n] : -(e[n] + 1);
 #pragma unroll
-                for (int c = 0; c < 3; ++c) ((int*)(st + S::GRID))[c * PM_CHUNK + threadIdx.x] = g[c] << step;
+                for (int i = 0; i < CPR / 2; ++i) {
+                    const int o = (threadIdx.x & 3) + 4 * i, c = o % CPR;
+                    if (o < CPR) cp_async16_zfill(smem_u32(st) + pm_offset<W>(r, c), x + p * xs + 8 * c, there);
+                    else cp_async16_zfill(smem_u32(st) + S::TILE + pm_offset<W>(r, c), y + p * ys + 8 * c,
+                                          there && !(owners && e[n] < 0));
+                }
+            }
+            if (AUX)
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    const int k = threadIdx.x + i * PM_THREADS;
+                    // negated; rows that are not there, or answer for no point: probabilities of nothing
+                    if (k < 2 * MAPS * CH)
+                        ((float*)(st + S::AUX))[k] = ea[i] >= 0 ? -aux[i] : k < MAPS * CH ? -INFINITY : 0.f;
+                }
+            if (BIAS && threadIdx.x < CH)
+#pragma unroll
+                for (int c = 0; c < 3; ++c) ((int*)(st + S::GRID))[c * CH + threadIdx.x] = g[c] << step;
         }
         cp_async_commit();
     }
@@ -136,7 +153,7 @@ struct PmStream {
     {
         if (BIAS) {
             g[0] = g[1] = g[2] = 0;
-            if (threadIdx.x < PM_CHUNK) eg = row_of(0, threadIdx.x);
+            if (threadIdx.x < CH) eg = row_of(0, threadIdx.x);
         }
         fetch(0);
         issue(0);
@@ -218,14 +235,6 @@ __device__ __forceinline__ void pm_accumulate(const uint32_t (&p)[MAPS][4], uint
     }
 }
 
-__device__ __forceinline__ void pm_pack(const float (&v)[2][4], uint32_t (&p)[4])
-{
-    p[0] = pack_bf16(v[0][0], v[0][1]);
-    p[1] = pack_bf16(v[0][2], v[0][3]);
-    p[2] = pack_bf16(v[1][0], v[1][1]);
-    p[3] = pack_bf16(v[1][2], v[1][3]);
-}
-
 // ---- bias ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void pm_bias_setup(const PatchTable& t, uint32_t base, PmBias& b)
 {
@@ -247,13 +256,13 @@ __device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTab
 }
 // places of the entries of four pairs (rows g0, g1 of this lane and two of the other side); SIGN: the lane's point is
 // the query (+1) or the key
-template <int SIGN>
+template <int SIGN, int CH>
 __device__ __forceinline__ void pm_places(const PmBias& b, const int (&g0)[3], const int (&g1)[3], const int* gs, int j,
                                           uint32_t (&at)[4][3])
 {
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-        const int2 o = *(const int2*)(gs + c * PM_CHUNK + j);
+        const int2 o = *(const int2*)(gs + c * CH + j);
         at[0][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
         at[1][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.y, b.lo[c]), b.hi[c]);
         at[2][c] = (uint32_t)min(__viaddmax_s32(g1[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
@@ -264,6 +273,21 @@ __device__ __forceinline__ float pm_bias(const uint32_t (&at)[3], float s, float
 {
     return fmaf(s, scale2, pm_lds(at[0])) + (pm_lds(at[1]) + pm_lds(at[2]));
 }
+
+__device__ __forceinline__ float pm_max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of both
+__device__ __forceinline__ uint64_t pm_exp2(uint64_t x)
+{
+    float a, b;
+    unpack2(x, a, b);
+    return pack2(fast_exp2(a), fast_exp2(b));
+}
+__device__ __forceinline__ uint64_t pm_both(float v) { return pack2(v, v); }
 
 struct PmPlace {
     int h, tile, seq, start, L;
@@ -282,7 +306,8 @@ __device__ __forceinline__ PmPlace pm_place(const PatchArgs& a)
 template <int W, int MAPS, bool BIAS, bool KEEP>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patch_mma_fwd_kernel(const PatchArgs a)
 {
-    using S = PmStage<W>;
+    constexpr int CH = PmChunk<W, BIAS>::N;
+    using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
     const int q0 = w.tile * PM_ROWS, L = w.L;
@@ -312,11 +337,12 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr,
                a.scale < 0.f ? 0x80008000u : 0u, q);
     const float scale2 = fabsf(a.scale) * PA_LOG2E;
-    float o[MAPS][W / 8][4], sum[MAPS][4], l[MAPS][2], m[MAPS][2];
+    float o[MAPS][W / 8][4], sum[MAPS][4], m[MAPS][2];
+    uint64_t l[MAPS][2];
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
         m[k][0] = m[k][1] = PM_LOWEST;
-        l[k][0] = l[k][1] = 0.f;
+        l[k][0] = l[k][1] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             sum[k][j] = 0.f;
@@ -325,28 +351,29 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
         }
     }
     constexpr uint32_t ONES = 0x3f803f80u;
-    for (int i = 0; i * PM_CHUNK < L; ++i) {
+    constexpr int KG = 32;      // keys whose scores are held at a time
+    for (int i = 0; i * CH < L; ++i) {
         const unsigned char* st = in.next(i);
         if (!active) continue;
         const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
         const int* gs = (const int*)(st + S::GRID);
-        const int nk = L - i * PM_CHUNK;
-#pragma unroll
-        for (int j0 = 0; j0 < PM_CHUNK; j0 += 32) {
+        const int nk = L - i * CH;
+#pragma unroll 2
+        for (int j0 = 0; j0 < CH; j0 += KG) {
             if (j0 >= nk) break;
-            float s[2][MAPS][2][4];
+            float s[KG / 16][MAPS][2][4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < KG / 16; ++u) {
                 pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
                 if (BIAS)
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         uint32_t at[4][3];
-                        pm_places<1>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
+                        pm_places<1, CH>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) s[u][0][n][c] = pm_bias(at[c], s[u][0][n][c], scale2);
                     }
-                if (j0 + 32 > nk)
+                if (j0 + KG > nk)
 #pragma unroll
                     for (int k = 0; k < MAPS; ++k)
 #pragma unroll
@@ -361,9 +388,11 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     top[r] = fmaxf(s[0][k][0][2 * r], s[0][k][0][2 * r + 1]);
-                    top[r] = fmaxf(top[r], fmaxf(s[0][k][1][2 * r], s[0][k][1][2 * r + 1]));
-                    top[r] = fmaxf(top[r], fmaxf(s[1][k][0][2 * r], s[1][k][0][2 * r + 1]));
-                    top[r] = fmaxf(top[r], fmaxf(s[1][k][1][2 * r], s[1][k][1][2 * r + 1]));
+#pragma unroll
+                    for (int u = 0; u < KG / 16; ++u)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            if (u + n) top[r] = pm_max3(top[r], s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
                     if (!BIAS) top[r] *= scale2;
                 }
                 if (__any_sync(0xffffffffu, top[0] > m[k][0] + PM_LAZY || top[1] > m[k][1] + PM_LAZY)) {
@@ -373,7 +402,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
                         top[r] = fmaxf(m[k][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
                         const float fix = fast_exp2(m[k][r] - top[r]);
                         m[k][r] = top[r];
-                        l[k][r] *= fix;
+                        l[k][r] = mul2(l[k][r], pm_both(fix));
                         sum[k][2 * r] *= fix;
 #pragma unroll
                         for (int n = 0; n < W / 8; ++n) {
@@ -383,17 +412,20 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < KG / 16; ++u) {
+                    uint32_t p[1][4];
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float v = s[u][k][n][c], top1 = m[k][c >> 1];
-                            s[u][k][n][c] = fast_exp2(BIAS ? v - top1 : fmaf(v, scale2, -top1));
-                            if (KEEP) l[k][c >> 1] += s[u][k][n][c];
+                        for (int r = 0; r < 2; ++r) {
+                            const uint64_t v = pack2(s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
+                            const uint64_t e = pm_exp2(BIAS ? add2(v, pm_both(-m[k][r]))
+                                                            : fma2(v, pm_both(scale2), pm_both(-m[k][r])));
+                            if (KEEP) l[k][r] = add2(l[k][r], e);
+                            float x, y;
+                            unpack2(e, x, y);
+                            p[0][2 * n + r] = pack_bf16(x, y);
                         }
-                    uint32_t p[1][4];
-                    pm_pack(s[u][k], p[0]);
                     pm_accumulate<W, 1>(p, vs, j0 + 16 * u, o[k]);
                     // the sum that the result is divided by is that of the rounded probabilities
                     mma_bf16(sum[k], p[0], ONES, ONES);
@@ -408,7 +440,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
         for (int k = 0; k < MAPS; ++k)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float v = l[k][r];
+                float v = hsum2(l[k][r]);
                 v += __shfl_xor_sync(0xffffffffu, v, 1);
                 v += __shfl_xor_sync(0xffffffffu, v, 2);
                 const int row = r ? r1 : r0;
@@ -480,7 +512,8 @@ __device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], cons
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_kernel(const PatchArgs a)
 {
-    using S = PmStage<W>;
+    constexpr int CH = PmChunk<W, BIAS>::N;
+    using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
     const int q0 = w.tile * PM_ROWS, L = w.L;
@@ -512,7 +545,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
         pm_rows<W>(e0 >= 0 ? p + (int64_t)e0 * a.C : nullptr, e1 >= 0 ? p + (int64_t)e1 * a.C : nullptr, 0u, f);
     };
     own_rows(a.dout, go);
-    float lse[MAPS][2], shift[MAPS][2], E[MAPS][2], total[MAPS][2], most[2] = {0.f, 0.f};
+    float lse[MAPS][2], shift[MAPS][2], most[2] = {0.f, 0.f};
+    uint64_t E[MAPS][2], total[MAPS][2];
     const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
     own_rows(a.out, q);
     pm_row_dots<W>(go, q, shift[0]);
@@ -535,17 +569,17 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
         for (int r = 0; r < 2; ++r) {
             const bool own = (r ? e1 : e0) >= 0;
             lse[k][r] = own ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + (r ? r1 : r0)] : INFINITY;
-            E[k][r] = total[k][r] = 0.f;
+            E[k][r] = total[k][r] = 0;
         }
 
-    for (int i = 0; i * PM_CHUNK < L; ++i) {
+    for (int i = 0; i * CH < L; ++i) {
         const unsigned char* st = in.next(i);
         if (!active) continue;
         const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
         const int* gs = (const int*)(st + S::GRID);
-        const int nk = L - i * PM_CHUNK;
+        const int nk = L - i * CH;
 #pragma unroll 2
-        for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
+        for (int j0 = 0; j0 < CH; j0 += 16) {
             if (j0 >= nk) break;
             float s[MAPS][2][4], G[1][2][4];
             pm_products<W, MAPS>(q, ks, j0, s);
@@ -554,7 +588,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     uint32_t at[4][3];
-                    pm_places<1>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
+                    pm_places<1, CH>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
                 }
@@ -568,24 +602,24 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
                             if (j0 + 8 * n + 2 * t + (c & 1) >= nk) s[k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
             uint32_t p[MAPS][4], d[MAPS][4];
 #pragma unroll
-            for (int k = 0; k < MAPS; ++k) {
-                float ds[2][4];
+            for (int k = 0; k < MAPS; ++k)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int r = c >> 1;
-                        const float v = s[k][n][c];
-                        const float pr = fast_exp2(BIAS ? v - lse[k][r] : fmaf(v, scale2, -lse[k][r]));
-                        s[k][n][c] = pr;
-                        total[k][r] += pr;
-                        ds[n][c] = pr * (G[0][n][c] - shift[k][r]);
-                        E[k][r] += ds[n][c];
-                        if (BIAS) most[r] += fabsf(ds[n][c]);
+                    for (int r = 0; r < 2; ++r) {
+                        const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
+                        const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][r]))
+                                                         : fma2(v, pm_both(scale2), pm_both(-lse[k][r])));
+                        total[k][r] = add2(total[k][r], pr);
+                        const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), pm_both(-shift[k][r])));
+                        E[k][r] = add2(E[k][r], ds);
+                        float x, y;
+                        unpack2(pr, x, y);
+                        p[k][2 * n + r] = pack_bf16(x, y);
+                        unpack2(ds, x, y);
+                        d[k][2 * n + r] = pack_bf16(x, y);
+                        if (BIAS) most[r] += fabsf(x) + fabsf(y);
                     }
-                pm_pack(s[k], p[k]);
-                pm_pack(ds, d[k]);
-            }
             pm_accumulate2<W, MAPS>(d, p, ks, j0, dq, pk);
         }
     }
@@ -601,8 +635,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
 #pragma unroll
         for (int k = 0; k < MAPS; ++k) {
             // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: divided out
-            const float sum = quad(total[k][r]), inv = e >= 0 ? 1.f / sum : 0.f;
-            eps[k] = quad(E[k][r]) * inv;
+            const float sum = quad(hsum2(total[k][r])), inv = e >= 0 ? 1.f / sum : 0.f;
+            eps[k] = quad(hsum2(E[k][r])) * inv;
             by[k] = inv * a.scale * (k == 1 ? -lam : 1.f);
             if (t == 0 && row < L)
                 a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = e >= 0 ? shift[k][r] + eps[k] : 0.f;
@@ -626,7 +660,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_kernel(const PatchArgs a)
 {
-    using S = PmStage<W>;
+    constexpr int CH = PmChunk<W, BIAS>::N;
+    using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
     __shared__ float part[4 * PM_WARPS];
@@ -677,13 +712,13 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
 #pragma unroll
         for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
 
-    for (int i = 0; i * PM_CHUNK < L; ++i) {
-        if (learns && i % (PM_WINDOW / PM_CHUNK) == 0) {
+    for (int i = 0; i * CH < L; ++i) {
+        if (learns && i % (PM_WINDOW / CH) == 0) {
             if (i) {
                 __syncthreads();
                 pa_flush(table, hist, sums, unit, PM_THREADS);
             }
-            unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * PM_CHUNK, part);
+            unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
             per_unit = pa_per_unit(unit);
         }
         const unsigned char* st = in.next(i);
@@ -691,11 +726,13 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         const uint32_t qs = smem_u32(st), os = qs + S::TILE;
         const float* aux = (const float*)(st + S::AUX);
         const int* gs = (const int*)(st + S::GRID);
-        const int nq = L - i * PM_CHUNK;
+        const int nq = L - i * CH;
 #pragma unroll 2
-        for (int j0 = 0; j0 < PM_CHUNK; j0 += 16) {
+        for (int j0 = 0; j0 < CH; j0 += 16) {
             if (j0 >= nq) break;
-            float s[MAPS][2][4], G[1][2][4], mix[2][4];
+            float s[MAPS][2][4], G[1][2][4];
+            uint64_t mix[2][2];
+            uint32_t p[MAPS][4], pm[1][4];
             pm_products<W, MAPS>(kf, qs, j0, s);
             pm_products<W, 1>(vf, os, j0, G);
 #pragma unroll
@@ -703,22 +740,36 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
                 const int j = j0 + 8 * n + 2 * t;
                 uint32_t at[4][3];
                 if (BIAS) {
-                    pm_places<-1>(bias, g0, g1, gs, j, at);
+                    pm_places<-1, CH>(bias, g0, g1, gs, j, at);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
                 }
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
-                    const float2 lse = *(const float2*)(aux + k * PM_CHUNK + j);
-                    const float2 delta = *(const float2*)(aux + (MAPS + k) * PM_CHUNK + j);
+                    // (negated as they are staged)
+                    const uint64_t lse = *(const uint64_t*)(aux + k * CH + j);
+                    const uint64_t delta = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float ls = c & 1 ? lse.y : lse.x, d = c & 1 ? delta.y : delta.x;
-                        float p = fast_exp2(BIAS ? s[k][n][c] - ls : fmaf(s[k][n][c], scale2, -ls));
-                        if (k == 1) p *= minus_lam;
-                        mix[n][c] = k == 0 ? p : mix[n][c] + p;
-                        s[k][n][c] = p * (G[0][n][c] - d);
+                    for (int r = 0; r < 2; ++r) {
+                        const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
+                        uint64_t pr = pm_exp2(BIAS ? add2(v, lse) : fma2(v, pm_both(scale2), lse));
+                        if (k == 1) pr = mul2(pr, pm_both(minus_lam));
+                        mix[n][r] = k == 0 ? pr : add2(mix[n][r], pr);
+                        const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), delta));
+                        float x, y;
+                        unpack2(ds, x, y);
+                        p[k][2 * n + r] = pack_bf16(x, y);
+                        if (BIAS) {
+                            s[0][n][2 * r] = x;
+                            s[0][n][2 * r + 1] = y;
+                        }
                     }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x, y;
+                    unpack2(mix[n][r], x, y);
+                    pm[0][2 * n + r] = pack_bf16(x, y);
                 }
                 // (rows beyond the patch have no key: their lanes add nothing)
                 if (learns)
@@ -730,11 +781,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
                             for (int x = 0; x < 3; ++x) pm_add_shared(at[c][x] + to_hist, v);
                         }
             }
-            uint32_t p[MAPS][4], x[1][4];
-            pm_pack(mix, x[0]);
-#pragma unroll
-            for (int k = 0; k < MAPS; ++k) pm_pack(s[k], p[k]);
-            pm_accumulate<W, 1>(x, os, j0, dv);
+            pm_accumulate<W, 1>(pm, os, j0, dv);
             pm_accumulate<W, MAPS>(p, qs, j0, dk);
         }
     }
@@ -780,7 +827,7 @@ template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
     const size_t table = BIAS ? pa_table_bytes(a) : 0;
-    const size_t smem = PM_STAGES * PmStage<W>::BYTES + table;
+    const size_t smem = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES + table;
     if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem, stream);
     if (pass == PA_COLS)      // the bins, and their sums
         return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a,

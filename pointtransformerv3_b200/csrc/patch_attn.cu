@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, 
                                                            int max_seqlen, int32_t* extent)
 {
     __shared__ int lo_s[4][3], hi_s[4][3];
-    const PatchArgs a = {nullptr, nullptr, rows, nullptr, cu, n_pad, 0, max_seqlen};
+    PatchArgs a = {nullptr, nullptr, rows, nullptr, cu, n_pad, 0, max_seqlen};
+    a.grid = grid;
     int start, lo[3], hi[3];
     const int L = pa_sequence(a, blockIdx.x, start);
 #pragma unroll
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, 
         const int64_t p = e >= 0 ? e : -(e + 1);
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-            const int v = min(max(grid[3 * p + c], -PA_MAX_COORD), PA_MAX_COORD);
+            const int v = pa_coord(a, p, c);
             lo[c] = min(lo[c], v);
             hi[c] = max(hi[c], v);
         }

@@ -31,7 +31,8 @@ namespace ptv3 {
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr int PA_MAX_BOUND = 512;
 constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
-constexpr int PA_TABLE_BYTES = 360 * 32 * 4;          // shared memory that copies of a head's table may take
+// shared memory that copies of a head's table may take: so that two CTAs fit an SM, and with its bins beside it
+constexpr int PA_TABLE_BYTES = 80 * 1024, PA_TABLE_BYTES_BINS = 352 * 32 * 4;
 
 // What the kernels get: ptv3_patch_attention_args with the workspace carved up.
 struct PatchArgs {
@@ -69,6 +70,12 @@ __device__ __forceinline__ int pa_sequence(const PatchArgs& a, int seq, int& sta
     return ok ? end - start : 0;
 }
 
+// a coordinate of a bias (ptv3_patch_rows reports one out of range; places in the table stay within it all the same)
+__device__ __forceinline__ int pa_coord(const PatchArgs& a, int64_t p, int c)
+{
+    return min(max(a.grid[3 * p + c], -PA_MAX_COORD), PA_MAX_COORD);
+}
+
 __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
 {
     return bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : ((const float*)p)[i];
@@ -76,50 +83,52 @@ __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
 
 // This head's table in shared memory, in powers of two, of the offsets that occur in a sequence: axis a holds offsets
 // -reach[a] .. reach[a], entry e of it at (first[a] + e) copies + copy.  A lane reads the copy of its number: with 32
-// copies, which most patches leave room for, look-ups of a warp never meet in a bank.
+// copies, which most patches leave room for, look-ups of a warp never meet in a bank.  Offsets beyond the bound repeat its
+// outermost entries, as long as that leaves room for eight copies: no look-up then has to be clamped.
 struct PatchTable {
     int reach[3], first[3], entries, copies_log2;
+    bool clamps;
 };
-__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int most_log2 = 5)
+__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int bytes, int most_log2 = 5)
 {
     PatchTable t;
-    t.entries = 0;
+    t.clamps = false;
+    for (int k = 0; k < 2; ++k) {
+        t.entries = 0;
 #pragma unroll
-    for (int c = 0; c < 3; ++c) {
-        t.reach[c] = min(a.bnd, a.extent[3 * seq + c]);
-        t.first[c] = t.entries;
-        t.entries += 2 * t.reach[c] + 1;
+        for (int c = 0; c < 3; ++c) {
+            t.reach[c] = a.extent[3 * seq + c];
+            if (k) t.reach[c] = min(a.bnd, t.reach[c]);
+            t.first[c] = t.entries;
+            t.entries += 2 * t.reach[c] + 1;
+        }
+        if (t.entries <= bytes >> 5) break;
+        t.clamps = true;
     }
     t.copies_log2 = 0;
-    while (t.copies_log2 < most_log2 && t.entries << (t.copies_log2 + 3) <= PA_TABLE_BYTES) ++t.copies_log2;
+    while (t.copies_log2 < most_log2 && t.entries << (t.copies_log2 + 3) <= bytes) ++t.copies_log2;
     return t;
 }
-// axis and offset + bnd of an entry
-__device__ __forceinline__ void pa_entry(const PatchArgs& a, const PatchTable& t, int i, int& axis, int& e)
+// axis and offset of an entry
+__device__ __forceinline__ void pa_entry(const PatchTable& t, int i, int& axis, int& d)
 {
     axis = i >= t.first[2] ? 2 : i >= t.first[1] ? 1 : 0;
-    e = i - (axis == 2 ? t.first[2] - a.bnd + t.reach[2] : axis == 1 ? t.first[1] - a.bnd + t.reach[1] : t.reach[0] - a.bnd);
+    d = i - (axis == 2 ? t.first[2] + t.reach[2] : axis == 1 ? t.first[1] + t.reach[1] : t.reach[0]);
 }
 __device__ __forceinline__ void pa_load_table(const PatchArgs& a, const PatchTable& t, int h, float* tab, int tid,
                                               int threads)
 {
     const int copies = 1 << t.copies_log2;
     for (int i = tid; i < t.entries; i += threads) {
-        int axis, e;
-        pa_entry(a, t, i, axis, e);
+        int axis, d;
+        pa_entry(t, i, axis, d);
+        const int e = min(max(d, -a.bnd), a.bnd) + a.bnd;
         int b = a.buckets ? a.buckets[e] : e;
         b = min(max(b, 0), a.num - 1);                     // (ptv3_patch_rows reports one out of range)
         const float v = pa_param(a.table, (axis * a.num + b) * a.H + h, a.table_bf16) * PA_LOG2E;
         for (int c = 0; c < copies; ++c) tab[(i << t.copies_log2) + ((c + tid) & (copies - 1))] = v;
     }
 }
-// most bytes that pa_load_table fills, and words of the entries themselves
-static inline size_t pa_table_bytes(const PatchArgs& a)
-{
-    const size_t all = (size_t)(3 * (2 * a.bnd + 1)) * 32 * 4;
-    return all < PA_TABLE_BYTES ? all : PA_TABLE_BYTES;
-}
-
 // What the queries [q0, q0 + WINDOW) of a sequence can add to a bin at most, as a unit in which 2^30 of it are that.
 // With QUADS lane t of four adds queries 2 t and 2 t + 1 of every eight, to copies of its own where there are four and
 // more: the largest of four sums.  All threads of a block of 32 `WARPS`; `part`: WARPS x 4 floats
@@ -165,14 +174,17 @@ __device__ __forceinline__ void pa_flush(const PatchTable& t, int* hist, float* 
         sums[i] = fmaf(v, unit, sums[i]);
     }
 }
-// a block's sums of all offsets
+// a block's sums of all offsets within the bound, those beyond with the outermost
 __device__ __forceinline__ void pa_store_bins(const PatchArgs& a, const PatchTable& t, const float* sums, float* bins, int threads)
 {
     const int ne = 2 * a.bnd + 1;
     for (int i = threadIdx.x; i < 3 * ne; i += threads) {
         const int axis = i / ne, d = i - axis * ne - a.bnd, r = axis == 0 ? t.reach[0] : axis == 1 ? t.reach[1] : t.reach[2];
-        const int first = axis == 0 ? 0 : axis == 1 ? t.first[1] : t.first[2];
-        bins[i] = d >= -r && d <= r ? sums[first + d + r] : 0.f;
+        const float* at = sums + (axis == 0 ? 0 : axis == 1 ? t.first[1] : t.first[2]) + r;
+        const int lo = d == -a.bnd ? -r : max(d, -r), hi = d == a.bnd ? r : min(d, r);
+        float v = 0.f;
+        for (int k = lo; k <= hi; ++k) v += at[k];
+        bins[i] = v;
     }
 }
 

@@ -12,6 +12,7 @@ constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
 constexpr int PF_STEP = 8;        // of which scores are held at a time
 constexpr int PF_WINDOW = 32;     // queries between two clearings of the bins: the unit is that much finer
 constexpr int PF_COPIES_LOG2 = 4; // few copies of them, so that clearing costs little
+constexpr int PF_TABLE_BYTES = PA_TABLE_BYTES_BINS / 2;
 
 template <int W, int MAPS>
 struct PfShape {
@@ -44,7 +45,7 @@ __device__ __forceinline__ void pf_stage(const PatchArgs& a, const float* x, int
     if (gs)
         for (int i = threadIdx.x; i < nk * 3; i += PF_THREADS) {
             const int j = i / 3, e = a.rows[start + j];
-            gs[j][i % 3] = a.grid[3 * (int64_t)(e >= 0 ? e : -(e + 1)) + i % 3];
+            gs[j][i % 3] = pa_coord(a, e >= 0 ? e : -(e + 1), i % 3);
         }
 }
 
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 #pragma unroll
     for (int i = 0; i < S::WP; ++i) q[i] = (base[p * stride + pf_dim<W, MAPS>(i, part)]);
     if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
         m[k] = -1e30f;          // (finite: scores may all be -inf)
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -228,7 +229,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
         d2 += __shfl_xor_sync(0xffffffffu, d2, 1);
     }
     if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
     const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
     delta[0] = MAPS == 2 ? fmaf(lam, d2, d1) : d1;
     if (MAPS == 2) delta[MAPS - 1] = d2;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     }
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1), words = BIAS ? table.entries << table.copies_log2 : 0;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
         dk[i] = dv[i] = 0.f;
     }
     if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
     coef[0] = 1.f;
     if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
     const float scale2 = a.scale * PA_LOG2E;
@@ -404,9 +405,9 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
-    const size_t table = BIAS ? pa_table_bytes(a) : 0;
+    const size_t table = BIAS ? PF_TABLE_BYTES : 0;
     // in the pass over columns beside the table: its bins, and their sums
-    const size_t cols = table + (a.bins ? table + (size_t)(3 * (2 * a.bnd + 1)) * 4 : 0);
+    const size_t cols = table * (a.bins ? 3 : 1);
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
     auto go = [&](auto kern, size_t smem) {
         const cudaError_t e = BIAS ? allow_smem(kern) : cudaSuccess;

@@ -27,6 +27,11 @@ struct PmChunk {
 constexpr int PM_STAGES = 3;
 constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
+// sums of the bins: entries of a table of eight copies, or of the largest bound (patch_attn.cuh)
+static int pm_sums_bytes(int bnd)
+{
+    return (3 * (2 * bnd + 1) > PA_TABLE_BYTES_BINS / 32 ? 3 * (2 * bnd + 1) : PA_TABLE_BYTES_BINS / 32) * 4;
+}
 constexpr float PM_LOWEST = -1e30f;
 
 template <int W, int CH>
@@ -88,12 +93,17 @@ struct PmStream {
         const int r = chunk * CH + j;
         return r < L ? a.rows[start + r] : INT_MIN;
     }
+    // (of rows beyond the last the last one's: places in the table stay within it)
+    __device__ __forceinline__ int grid_row(int chunk) const
+    {
+        return a.rows[start + min(chunk * CH + (int)threadIdx.x, L - 1)];
+    }
     __device__ __forceinline__ void fetch_grid()
     {
-        if (BIAS && threadIdx.x < CH && eg != INT_MIN) {
+        if (BIAS && threadIdx.x < CH) {
             const int64_t p = eg >= 0 ? eg : -(eg + 1);
 #pragma unroll
-            for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
+            for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
         }
     }
     __device__ __forceinline__ void fetch_aux(int chunk)
@@ -114,7 +124,7 @@ struct PmStream {
 #pragma unroll
         for (int i = 0; i < NR; ++i) e[i] = row_of(chunk, (threadIdx.x >> 2) + 64 * i);
         fetch_grid();
-        if (BIAS && threadIdx.x < CH) eg = row_of(chunk + 1, threadIdx.x);
+        if (BIAS && threadIdx.x < CH) eg = grid_row(chunk + 1);
         fetch_aux(chunk);
     }
     __device__ __forceinline__ void issue(int chunk)
@@ -151,10 +161,7 @@ struct PmStream {
     }
     __device__ __forceinline__ void begin()
     {
-        if (BIAS) {
-            g[0] = g[1] = g[2] = 0;
-            if (threadIdx.x < CH) eg = row_of(0, threadIdx.x);
-        }
+        if (BIAS && threadIdx.x < CH) eg = grid_row(0);
         fetch(0);
         issue(0);
         fetch(1);
@@ -235,6 +242,14 @@ __device__ __forceinline__ void pm_accumulate(const uint32_t (&p)[MAPS][4], uint
     }
 }
 
+// whether places in the table have to be held within it
+struct PmYes {
+    static constexpr bool value = true;
+};
+struct PmNo {
+    static constexpr bool value = false;
+};
+
 // ---- bias ---------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void pm_bias_setup(const PatchTable& t, uint32_t base, PmBias& b)
 {
@@ -245,33 +260,43 @@ __device__ __forceinline__ void pm_bias_setup(const PatchTable& t, uint32_t base
         b.hi[c] = b.lo[c] + ((2 * t.reach[c]) << step);
     }
 }
-// this lane's point, so that subtracting another's coordinates gives the entry's place
-__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTable& t, const PmBias& b, int e, int sign,
-                                              int (&g)[3])
+// row r's point, so that subtracting another's coordinates gives the entry's place
+__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTable& t, const PmBias& b, int start, int L, int r,
+                                              int sign, int (&g)[3])
 {
-    const int64_t p = e >= 0 ? e : -(e + 1);
+    const int e = a.rows[start + min(r, L - 1)];
 #pragma unroll
     for (int c = 0; c < 3; ++c)
-        g[c] = b.lo[c] + ((t.reach[c] + sign * a.grid[3 * p + c]) << (t.copies_log2 + 2));
+        g[c] = b.lo[c] + ((t.reach[c] + sign * pa_coord(a, e >= 0 ? e : -(e + 1), c)) << (t.copies_log2 + 2));
 }
 // places of the entries of four pairs (rows g0, g1 of this lane and two of the other side); SIGN: the lane's point is
 // the query (+1) or the key
-template <int SIGN, int CH>
+template <int SIGN, int CH, bool CLAMP>
 __device__ __forceinline__ void pm_places(const PmBias& b, const int (&g0)[3], const int (&g1)[3], const int* gs, int j,
                                           uint32_t (&at)[4][3])
 {
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
         const int2 o = *(const int2*)(gs + c * CH + j);
-        at[0][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
-        at[1][c] = (uint32_t)min(__viaddmax_s32(g0[c], -SIGN * o.y, b.lo[c]), b.hi[c]);
-        at[2][c] = (uint32_t)min(__viaddmax_s32(g1[c], -SIGN * o.x, b.lo[c]), b.hi[c]);
-        at[3][c] = (uint32_t)min(__viaddmax_s32(g1[c], -SIGN * o.y, b.lo[c]), b.hi[c]);
+        auto place = [&](int mine, int other) {
+            return (uint32_t)(CLAMP ? min(__viaddmax_s32(mine, -SIGN * other, b.lo[c]), b.hi[c]) : mine - SIGN * other);
+        };
+        at[0][c] = place(g0[c], o.x);
+        at[1][c] = place(g0[c], o.y);
+        at[2][c] = place(g1[c], o.x);
+        at[3][c] = place(g1[c], o.y);
     }
 }
-__device__ __forceinline__ float pm_bias(const uint32_t (&at)[3], float s, float scale2)
+// scores and biases of four pairs, in powers of two
+__device__ __forceinline__ void pm_bias(const uint32_t (&at)[4][3], float scale2, float (&s)[4])
 {
-    return fmaf(s, scale2, pm_lds(at[0])) + (pm_lds(at[1]) + pm_lds(at[2]));
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+        uint64_t t[3];
+#pragma unroll
+        for (int c = 0; c < 3; ++c) t[c] = pack2(pm_lds(at[r][c]), pm_lds(at[r + 1][c]));
+        unpack2(add2(fma2(pack2(s[r], s[r + 1]), pack2(scale2, scale2), t[0]), add2(t[1], t[2])), s[r], s[r + 1]);
+    }
 }
 
 __device__ __forceinline__ float pm_max3(float a, float b, float c)
@@ -319,7 +344,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq);
+    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES);
     PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
@@ -329,8 +354,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, e0, 1, g0);
-        pm_bias_point(a, table, bias, e1, 1, g1);
+        pm_bias_point(a, table, bias, w.start, L, r0, 1, g0);
+        pm_bias_point(a, table, bias, w.start, L, r1, 1, g1);
     }
     uint32_t q[W / 16][4];
     // (of a negative scale the sign goes to the queries, so that larger products are larger scores)
@@ -352,87 +377,91 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     }
     constexpr uint32_t ONES = 0x3f803f80u;
     constexpr int KG = 32;      // keys whose scores are held at a time
-    for (int i = 0; i * CH < L; ++i) {
-        const unsigned char* st = in.next(i);
-        if (!active) continue;
-        const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
-        const int* gs = (const int*)(st + S::GRID);
-        const int nk = L - i * CH;
+    auto walk = [&](auto clamp) {
+        constexpr bool CLAMP = decltype(clamp)::value;
+        for (int i = 0; i * CH < L; ++i) {
+            const unsigned char* st = in.next(i);
+            if (!active) continue;
+            const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
+            const int* gs = (const int*)(st + S::GRID);
+            const int nk = L - i * CH;
 #pragma unroll 2
-        for (int j0 = 0; j0 < CH; j0 += KG) {
-            if (j0 >= nk) break;
-            float s[KG / 16][MAPS][2][4];
-#pragma unroll
-            for (int u = 0; u < KG / 16; ++u) {
-                pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
-                if (BIAS)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        uint32_t at[4][3];
-                        pm_places<1, CH>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) s[u][0][n][c] = pm_bias(at[c], s[u][0][n][c], scale2);
-                    }
-                if (j0 + KG > nk)
-#pragma unroll
-                    for (int k = 0; k < MAPS; ++k)
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (j0 + 16 * u + 8 * n + 2 * t + (c & 1) >= nk) s[u][k][n][c] = -INFINITY;
-            }
-#pragma unroll
-            for (int k = 0; k < MAPS; ++k) {
-                float top[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(s[0][k][0][2 * r], s[0][k][0][2 * r + 1]);
-#pragma unroll
-                    for (int u = 0; u < KG / 16; ++u)
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-                            if (u + n) top[r] = pm_max3(top[r], s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
-                    if (!BIAS) top[r] *= scale2;
-                }
-                if (__any_sync(0xffffffffu, top[0] > m[k][0] + PM_LAZY || top[1] > m[k][1] + PM_LAZY)) {
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                        top[r] = fmaxf(m[k][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
-                        const float fix = fast_exp2(m[k][r] - top[r]);
-                        m[k][r] = top[r];
-                        l[k][r] = mul2(l[k][r], pm_both(fix));
-                        sum[k][2 * r] *= fix;
-#pragma unroll
-                        for (int n = 0; n < W / 8; ++n) {
-                            o[k][n][2 * r] *= fix;
-                            o[k][n][2 * r + 1] *= fix;
-                        }
-                    }
-                }
+            for (int j0 = 0; j0 < CH; j0 += KG) {
+                if (j0 >= nk) break;
+                float s[KG / 16][MAPS][2][4];
 #pragma unroll
                 for (int u = 0; u < KG / 16; ++u) {
-                    uint32_t p[1][4];
+                    pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
+                    if (BIAS)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                        for (int n = 0; n < 2; ++n) {
+                            uint32_t at[4][3];
+                            pm_places<1, CH, CLAMP>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
+                            pm_bias(at, scale2, s[u][0][n]);
+                        }
+                    if (j0 + KG > nk)
+#pragma unroll
+                        for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    if (j0 + 16 * u + 8 * n + 2 * t + (c & 1) >= nk) s[u][k][n][c] = -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    float top[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        top[r] = fmaxf(s[0][k][0][2 * r], s[0][k][0][2 * r + 1]);
+#pragma unroll
+                        for (int u = 0; u < KG / 16; ++u)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+                                if (u + n) top[r] = pm_max3(top[r], s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
+                        if (!BIAS) top[r] *= scale2;
+                    }
+                    if (__any_sync(0xffffffffu, top[0] > m[k][0] + PM_LAZY || top[1] > m[k][1] + PM_LAZY)) {
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const uint64_t v = pack2(s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
-                            const uint64_t e = pm_exp2(BIAS ? add2(v, pm_both(-m[k][r]))
-                                                            : fma2(v, pm_both(scale2), pm_both(-m[k][r])));
-                            if (KEEP) l[k][r] = add2(l[k][r], e);
-                            float x, y;
-                            unpack2(e, x, y);
-                            p[0][2 * n + r] = pack_bf16(x, y);
+                            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                            top[r] = fmaxf(m[k][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
+                            const float fix = fast_exp2(m[k][r] - top[r]);
+                            m[k][r] = top[r];
+                            l[k][r] = mul2(l[k][r], pm_both(fix));
+                            sum[k][2 * r] *= fix;
+#pragma unroll
+                            for (int n = 0; n < W / 8; ++n) {
+                                o[k][n][2 * r] *= fix;
+                                o[k][n][2 * r + 1] *= fix;
+                            }
                         }
-                    pm_accumulate<W, 1>(p, vs, j0 + 16 * u, o[k]);
-                    // the sum that the result is divided by is that of the rounded probabilities
-                    mma_bf16(sum[k], p[0], ONES, ONES);
+                    }
+#pragma unroll
+                    for (int u = 0; u < KG / 16; ++u) {
+                        uint32_t p[1][4];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const uint64_t v = pack2(s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
+                                const uint64_t e = pm_exp2(BIAS ? add2(v, pm_both(-m[k][r]))
+                                                                : fma2(v, pm_both(scale2), pm_both(-m[k][r])));
+                                if (KEEP) l[k][r] = add2(l[k][r], e);
+                                float x, y;
+                                unpack2(e, x, y);
+                                p[0][2 * n + r] = pack_bf16(x, y);
+                            }
+                        pm_accumulate<W, 1>(p, vs, j0 + 16 * u, o[k]);
+                        // the sum that the result is divided by is that of the rounded probabilities
+                        mma_bf16(sum[k], p[0], ONES, ONES);
+                    }
                 }
             }
         }
-    }
+    };
+    if (BIAS && table.clamps) walk(PmYes());
+    else walk(PmNo());
     in.end();
     if (!active) return;
     if (KEEP)
@@ -525,7 +554,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq);
+    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES);
     PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
@@ -535,8 +564,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, e0, 1, g0);
-        pm_bias_point(a, table, bias, e1, 1, g1);
+        pm_bias_point(a, table, bias, w.start, L, r0, 1, g0);
+        pm_bias_point(a, table, bias, w.start, L, r1, 1, g1);
     }
     uint32_t q[W / 16][4], go[W / 16][4];
     // rows of a matrix of C columns, this head's; zeros for rows that answer for no point
@@ -572,57 +601,61 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
             E[k][r] = total[k][r] = 0;
         }
 
-    for (int i = 0; i * CH < L; ++i) {
-        const unsigned char* st = in.next(i);
-        if (!active) continue;
-        const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
-        const int* gs = (const int*)(st + S::GRID);
-        const int nk = L - i * CH;
+    auto walk = [&](auto clamp) {
+        constexpr bool CLAMP = decltype(clamp)::value;
+        for (int i = 0; i * CH < L; ++i) {
+            const unsigned char* st = in.next(i);
+            if (!active) continue;
+            const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
+            const int* gs = (const int*)(st + S::GRID);
+            const int nk = L - i * CH;
 #pragma unroll 2
-        for (int j0 = 0; j0 < CH; j0 += 16) {
-            if (j0 >= nk) break;
-            float s[MAPS][2][4], G[1][2][4];
-            pm_products<W, MAPS>(q, ks, j0, s);
-            pm_products<W, 1>(go, vs, j0, G);
-            if (BIAS)
+            for (int j0 = 0; j0 < CH; j0 += 16) {
+                if (j0 >= nk) break;
+                float s[MAPS][2][4], G[1][2][4];
+                pm_products<W, MAPS>(q, ks, j0, s);
+                pm_products<W, 1>(go, vs, j0, G);
+                if (BIAS)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    uint32_t at[4][3];
-                    pm_places<1, CH>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
+                    for (int n = 0; n < 2; ++n) {
+                        uint32_t at[4][3];
+                        pm_places<1, CH, CLAMP>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
+                        pm_bias(at, scale2, s[0][n]);
+                    }
+                if (j0 + 16 > nk)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
-                }
-            if (j0 + 16 > nk)
+                    for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (j0 + 8 * n + 2 * t + (c & 1) >= nk) s[k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
+                uint32_t p[MAPS][4], d[MAPS][4];
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (j0 + 8 * n + 2 * t + (c & 1) >= nk) s[k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
-            uint32_t p[MAPS][4], d[MAPS][4];
-#pragma unroll
-            for (int k = 0; k < MAPS; ++k)
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
-                        const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][r]))
-                                                         : fma2(v, pm_both(scale2), pm_both(-lse[k][r])));
-                        total[k][r] = add2(total[k][r], pr);
-                        const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), pm_both(-shift[k][r])));
-                        E[k][r] = add2(E[k][r], ds);
-                        float x, y;
-                        unpack2(pr, x, y);
-                        p[k][2 * n + r] = pack_bf16(x, y);
-                        unpack2(ds, x, y);
-                        d[k][2 * n + r] = pack_bf16(x, y);
-                        if (BIAS) most[r] += fabsf(x) + fabsf(y);
-                    }
-            pm_accumulate2<W, MAPS>(d, p, ks, j0, dq, pk);
+                        for (int r = 0; r < 2; ++r) {
+                            const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
+                            const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][r]))
+                                                             : fma2(v, pm_both(scale2), pm_both(-lse[k][r])));
+                            total[k][r] = add2(total[k][r], pr);
+                            const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), pm_both(-shift[k][r])));
+                            E[k][r] = add2(E[k][r], ds);
+                            float x, y;
+                            unpack2(pr, x, y);
+                            p[k][2 * n + r] = pack_bf16(x, y);
+                            unpack2(ds, x, y);
+                            d[k][2 * n + r] = pack_bf16(x, y);
+                            if (BIAS) most[r] += fabsf(x) + fabsf(y);
+                        }
+                pm_accumulate2<W, MAPS>(d, p, ks, j0, dq, pk);
+            }
         }
-    }
+    };
+    if (BIAS && table.clamps) walk(PmYes());
+    else walk(PmNo());
     in.end();
     auto quad = [](float v) {
         v += __shfl_xor_sync(0xffffffffu, v, 1);
@@ -680,7 +713,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     const int64_t p0 = e0 >= 0 ? e0 : -(e0 + 1), p1 = e1 >= 0 ? e1 : -(e1 + 1), stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq);
+    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES_BINS);
     PmStream<W, MAPS, true, BIAS> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
                                         table.copies_log2 + 2, smem};
     in.begin();
@@ -694,8 +727,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     if (BIAS) {
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, e0, -1, g0);
-        pm_bias_point(a, table, bias, e1, -1, g1);
+        pm_bias_point(a, table, bias, w.start, L, r0, -1, g0);
+        pm_bias_point(a, table, bias, w.start, L, r1, -1, g1);
         if (learns) {
             for (int i = threadIdx.x; i < table.entries << table.copies_log2; i += PM_THREADS) hist[i] = 0;
             for (int i = threadIdx.x; i < table.entries; i += PM_THREADS) sums[i] = 0.f;
@@ -712,79 +745,83 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
 #pragma unroll
         for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
 
-    for (int i = 0; i * CH < L; ++i) {
-        if (learns && i % (PM_WINDOW / CH) == 0) {
-            if (i) {
-                __syncthreads();
-                pa_flush(table, hist, sums, unit, PM_THREADS);
-            }
-            unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
-            per_unit = pa_per_unit(unit);
-        }
-        const unsigned char* st = in.next(i);
-        if (warp0 >= L) continue;
-        const uint32_t qs = smem_u32(st), os = qs + S::TILE;
-        const float* aux = (const float*)(st + S::AUX);
-        const int* gs = (const int*)(st + S::GRID);
-        const int nq = L - i * CH;
-#pragma unroll 2
-        for (int j0 = 0; j0 < CH; j0 += 16) {
-            if (j0 >= nq) break;
-            float s[MAPS][2][4], G[1][2][4];
-            uint64_t mix[2][2];
-            uint32_t p[MAPS][4], pm[1][4];
-            pm_products<W, MAPS>(kf, qs, j0, s);
-            pm_products<W, 1>(vf, os, j0, G);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int j = j0 + 8 * n + 2 * t;
-                uint32_t at[4][3];
-                if (BIAS) {
-                    pm_places<-1, CH>(bias, g0, g1, gs, j, at);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) s[0][n][c] = pm_bias(at[c], s[0][n][c], scale2);
+    auto walk = [&](auto clamp) {
+        constexpr bool CLAMP = decltype(clamp)::value;
+        for (int i = 0; i * CH < L; ++i) {
+            if (learns && i % (PM_WINDOW / CH) == 0) {
+                if (i) {
+                    __syncthreads();
+                    pa_flush(table, hist, sums, unit, PM_THREADS);
                 }
+                unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
+                per_unit = pa_per_unit(unit);
+            }
+            const unsigned char* st = in.next(i);
+            if (warp0 >= L) continue;
+            const uint32_t qs = smem_u32(st), os = qs + S::TILE;
+            const float* aux = (const float*)(st + S::AUX);
+            const int* gs = (const int*)(st + S::GRID);
+            const int nq = L - i * CH;
+#pragma unroll 2
+            for (int j0 = 0; j0 < CH; j0 += 16) {
+                if (j0 >= nq) break;
+                float s[MAPS][2][4], G[1][2][4];
+                uint64_t mix[2][2];
+                uint32_t p[MAPS][4], pm[1][4];
+                pm_products<W, MAPS>(kf, qs, j0, s);
+                pm_products<W, 1>(vf, os, j0, G);
 #pragma unroll
-                for (int k = 0; k < MAPS; ++k) {
-                    // (negated as they are staged)
-                    const uint64_t lse = *(const uint64_t*)(aux + k * CH + j);
-                    const uint64_t delta = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
+                for (int n = 0; n < 2; ++n) {
+                    const int j = j0 + 8 * n + 2 * t;
+                    uint32_t at[4][3];
+                    if (BIAS) {
+                        pm_places<-1, CH, CLAMP>(bias, g0, g1, gs, j, at);
+                        pm_bias(at, scale2, s[0][n]);
+                    }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
-                        uint64_t pr = pm_exp2(BIAS ? add2(v, lse) : fma2(v, pm_both(scale2), lse));
-                        if (k == 1) pr = mul2(pr, pm_both(minus_lam));
-                        mix[n][r] = k == 0 ? pr : add2(mix[n][r], pr);
-                        const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), delta));
-                        float x, y;
-                        unpack2(ds, x, y);
-                        p[k][2 * n + r] = pack_bf16(x, y);
-                        if (BIAS) {
-                            s[0][n][2 * r] = x;
-                            s[0][n][2 * r + 1] = y;
+                    for (int k = 0; k < MAPS; ++k) {
+                        // (negated as they are staged)
+                        const uint64_t lse = *(const uint64_t*)(aux + k * CH + j);
+                        const uint64_t delta = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
+                            uint64_t pr = pm_exp2(BIAS ? add2(v, lse) : fma2(v, pm_both(scale2), lse));
+                            if (k == 1) pr = mul2(pr, pm_both(minus_lam));
+                            mix[n][r] = k == 0 ? pr : add2(mix[n][r], pr);
+                            const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), delta));
+                            float x, y;
+                            unpack2(ds, x, y);
+                            p[k][2 * n + r] = pack_bf16(x, y);
+                            if (BIAS) {
+                                s[0][n][2 * r] = x;
+                                s[0][n][2 * r + 1] = y;
+                            }
                         }
                     }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float x, y;
+                        unpack2(mix[n][r], x, y);
+                        pm[0][2 * n + r] = pack_bf16(x, y);
+                    }
+                    // (rows beyond the patch have no key: their lanes add nothing)
+                    if (learns)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (c < 2 ? there0 : there1) {
+                                const int v = __float2int_rn(s[0][n][c] * per_unit);
+#pragma unroll
+                                for (int x = 0; x < 3; ++x) pm_add_shared(at[c][x] + to_hist, v);
+                            }
                 }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x, y;
-                    unpack2(mix[n][r], x, y);
-                    pm[0][2 * n + r] = pack_bf16(x, y);
-                }
-                // (rows beyond the patch have no key: their lanes add nothing)
-                if (learns)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (c < 2 ? there0 : there1) {
-                            const int v = __float2int_rn(s[0][n][c] * per_unit);
-#pragma unroll
-                            for (int x = 0; x < 3; ++x) pm_add_shared(at[c][x] + to_hist, v);
-                        }
+                pm_accumulate<W, 1>(pm, os, j0, dv);
+                pm_accumulate<W, MAPS>(p, qs, j0, dk);
             }
-            pm_accumulate<W, 1>(pm, os, j0, dv);
-            pm_accumulate<W, MAPS>(p, qs, j0, dk);
         }
-    }
+    };
+    if (BIAS && table.clamps) walk(PmYes());
+    else walk(PmNo());
     in.end();
     if (learns) {
         pa_flush(table, hist, sums, unit, PM_THREADS);
@@ -826,12 +863,11 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
-    const size_t table = BIAS ? pa_table_bytes(a) : 0;
-    const size_t smem = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES + table;
+    const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES, smem = stages + (BIAS ? PA_TABLE_BYTES : 0);
     if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem, stream);
-    if (pass == PA_COLS)      // the bins, and their sums
+    if (pass == PA_COLS)      // the table, its bins, and their sums
         return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a,
-                      smem + (a.bins ? table + (size_t)(3 * (2 * a.bnd + 1)) * 4 : 0), stream);
+                      stages + (BIAS ? PA_TABLE_BYTES_BINS * (a.bins ? 2 : 1) + (a.bins ? pm_sums_bytes(a.bnd) : 0) : 0), stream);
     return a.lse ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true>, a, smem, stream)
                  : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false>, a, smem, stream);
 }

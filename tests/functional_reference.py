@@ -51,7 +51,7 @@ def attention(qkv, order, pad, unpad, cu, heads, scale, maps=1, param=None, grid
     dqkv, dqkv_p, dqkv_e = (torch.zeros(n, 3 * c, **z) for _ in range(3))
     dparam = None if param is None else torch.zeros_like(param, dtype=torch.float64)
     dparam_e = None if param is None else torch.zeros_like(dparam)
-    top = 0.0
+    top = bias_top = 0.0
     answers = torch.full((pad.shape[0],), -1, dtype=torch.int64, device=qkv.device)
     answers[unpad] = order
     ends = cu.tolist()
@@ -69,7 +69,9 @@ def attention(qkv, order, pad, unpad, cu, heads, scale, maps=1, param=None, grid
             if maps == 1 and param is not None:
                 bias = bias_of(param.double(), grid[pts], grid[pts], bound, buckets)
                 s = s + bias
-                size = size + 3 * param.double().abs().max()
+                largest = torch.where(param.isfinite(), param, 0).double().abs().max()
+                size = size + 3 * largest
+                bias_top = max(bias_top, float(largest))
             score = max(score, float(size.max()))
             e = torch.exp(s - s.amax(-1, keepdim=True))
             probs.append(e / e.sum(-1, keepdim=True))
@@ -117,7 +119,7 @@ def attention(qkv, order, pad, unpad, cu, heads, scale, maps=1, param=None, grid
         dqkv.index_add_(0, pts, flat(dq, dk, dv))
         dqkv_p.index_add_(0, pts, flat(dq_p, dk_p, dv_p))
         dqkv_e.index_add_(0, pts, flat(dq_e, dk_e, dv_p))
-    res = dict(top=top, out=(out, out_p, out_p))
+    res = dict(top=top, bias_top=bias_top, out=(out, out_p, out_p))
     if dout is not None:
         res["dqkv"] = (dqkv, dqkv_p, dqkv_e)
         if param is not None:
@@ -135,6 +137,8 @@ def tolerances(res, name, dtype, width, longest, features=None):
     e32 = 2.0 ** -24
     eps = 4 * ((width + 8) * e32 * max(1.0, res["top"]) + longest * e32 + 2.0 ** -21) + 2 * width * e32
     rounding = HALF_STEP[torch.bfloat16] if features == torch.bfloat16 else 0.0
+    if rounding:      # a table's entries enter bf16 scores as two bf16 parts, 2^-16 of an entry, three to a score; twice as above
+        eps += 2 * 3 * 2.0 ** -16 * res["bias_top"]
     return HALF_STEP[dtype] * value.abs() * (1 + 2.0 ** -7) + rounding * 1.01 * product + eps * sums + 1e-30
 
 

@@ -160,6 +160,44 @@ def test_a_learned_table_follows_far_and_uneven_patches():
             R.check(got, ref, name, 16, p["longest"], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_buckets_that_mask(dtype):
+    """Entries of minus infinity take keys out of a row, entries of the type's lowest value do the same, and a row that they leave
+    without a key is NaN, as softmax has it; the others keep their values and gradients."""
+    p = plan([256, 300], 128, extent=9)
+    C, H, bound = 32, 2, 5
+    qkv = normal(p["n"], 3 * C, seed=1, dtype=dtype)
+    table = normal(3 * (2 * bound + 1), H, seed=2, dtype=dtype, scale=0.5)
+    for low in (float("-inf"), torch.finfo(dtype).min):
+        masked = table.clone()
+        masked[[0, 1, 9, 13, 31], :] = low                 # (offsets of zero, which every row has with itself, stay)
+        x, w = qkv.clone().requires_grad_(), masked.clone().requires_grad_()
+        dout = normal(p["n"], C, seed=3, dtype=dtype)
+        out = F.attention_bias(x, *geometry(p), H, p["longest"], grid_coord=p["grid"], table=w)
+        got = (out,) + torch.autograd.grad(out, (x, w), dout)
+        minus = torch.where(masked < -1e30, torch.full_like(masked, float("-inf")), masked)
+        ref = R.attention(qkv, *geometry(p), H, 0.25, 1, minus, p["grid"], bound, None, dout)
+        for name, t in zip(("out", "dqkv", "dparam"), got):
+            R.check(t, ref, name, 16, p["longest"], dtype, name)
+    nothing = torch.full_like(table, float("-inf"))
+    out = F.attention_bias(qkv, *geometry(p), H, p["longest"], grid_coord=p["grid"], table=nothing)
+    assert bool(out.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_ordered_points(dtype):
+    """Points along a curve, whose neighbours in the order share coordinates, and ones that all share them."""
+    g = torch.arange(700)
+    for grid in (torch.stack([g // 64, g // 8 % 8, g % 8], 1), torch.stack([g // 350, g * 0 + 3, g * 0 - 5], 1),
+                 torch.stack([g, -g, g % 9], 1)):
+        p = plan([700], 256)
+        p["order"] = torch.arange(700, device="cuda")
+        p["grid"] = grid.int().cuda()
+        out, dqkv, dtable, ref = run_bias(p, 32, 2, dtype, dtype, 31)
+        for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dtable)):
+            R.check(got, ref, name, 16, p["longest"], dtype)
+
+
 # --------------------------------------------------------------------------- norms and rotation
 def run_qk(n, heads, D, dtype, weight_dtype, norm, rope, extent=65536, seed=7):
     qkv = normal(n, 3 * heads * D, seed=seed, dtype=dtype).requires_grad_()

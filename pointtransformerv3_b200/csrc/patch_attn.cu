@@ -63,7 +63,11 @@ __global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, 
                                                            int max_seqlen, int32_t* extent)
 {
     __shared__ int lo_s[4][3], hi_s[4][3];
-    PatchArgs a = {nullptr, nullptr, rows, nullptr, cu, n_pad, 0, max_seqlen};
+    PatchArgs a = {};
+    a.rows = rows;
+    a.cu = cu;
+    a.n_pad = n_pad;
+    a.max_seqlen = max_seqlen;
     a.grid = grid;
     int start, lo[3], hi[3];
     const int L = pa_sequence(a, blockIdx.x, start);
@@ -194,7 +198,7 @@ static int longest(const ptv3_patch_attention_args* p)
 {
     return (int)(p->max_seqlen < p->n_pad ? p->max_seqlen : p->n_pad);
 }
-// blocks of queries of the longest sequence
+// blocks of the longest sequence
 static int patch_tiles(const ptv3_patch_attention_args* p)
 {
     return ceil_div(longest(p), p->dtype == PTV3_DTYPE_BF16 ? patch_mma_rows() : patch_fma_rows(p->channels / p->heads));

@@ -31,8 +31,8 @@ namespace ptv3 {
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 constexpr int PA_MAX_BOUND = 512;
 constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
-// shared memory that copies of a head's table may take: so that two CTAs fit an SM, and with its bins beside it
-constexpr int PA_TABLE_BYTES = 80 * 1024, PA_TABLE_BYTES_BINS = 352 * 32 * 4;
+constexpr int PA_TABLE_BYTES = 80 * 1024;             // shared memory for a head's table, so that two CTAs fit an SM;
+constexpr int PA_BINS_BYTES = 2 * 352 * 32 * 4;       // for a table and its bins beside it
 
 // What the kernels get: ptv3_patch_attention_args with the workspace carved up.
 struct PatchArgs {
@@ -84,12 +84,13 @@ __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
 // This head's table in shared memory, in powers of two, of the offsets that occur in a sequence: axis a holds offsets
 // -reach[a] .. reach[a], entry e of it at (first[a] + e) copies + copy.  A lane reads the copy of its number: with 32
 // copies, which most patches leave room for, look-ups of a warp never meet in a bank.  Offsets beyond the bound repeat its
-// outermost entries, as long as that leaves room for eight copies: no look-up then has to be clamped.
+// outermost entries, as long as that leaves room for eight copies: no look-up then has to be clamped.  With `bins`, there
+// are as many copies of the bins, or half.
 struct PatchTable {
-    int reach[3], first[3], entries, copies_log2;
+    int reach[3], first[3], entries, copies_log2, bins_log2;
     bool clamps;
 };
-__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int bytes, int most_log2 = 5)
+__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int bytes, bool bins, int most_log2 = 5)
 {
     PatchTable t;
     t.clamps = false;
@@ -102,11 +103,14 @@ __device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int 
             t.first[c] = t.entries;
             t.entries += 2 * t.reach[c] + 1;
         }
-        if (t.entries <= bytes >> 5) break;
+        if (t.entries <= bytes >> (bins ? 6 : 5)) break;
         t.clamps = true;
     }
-    t.copies_log2 = 0;
-    while (t.copies_log2 < most_log2 && t.entries << (t.copies_log2 + 3) <= bytes) ++t.copies_log2;
+    t.copies_log2 = t.bins_log2 = most_log2;
+    while (t.bins_log2 > 0 && 4 * ((t.entries << t.copies_log2) + (bins ? t.entries << t.bins_log2 : 0)) > bytes) {
+        if (bins && t.bins_log2 == t.copies_log2) --t.bins_log2;
+        else t.copies_log2 = t.bins_log2 = bins ? t.bins_log2 : t.bins_log2 - 1;
+    }
     return t;
 }
 // axis and offset of an entry
@@ -153,7 +157,7 @@ __device__ __forceinline__ float pa_unit(const PatchArgs& a, const PatchTable& t
         top = fmaxf(top, sum);
         all += sum;                        // (a NaN among them is kept by this one)
     }
-    return (QUADS && table.copies_log2 >= 2 && all == all ? top : all) * (1.f / 1073741824.f);
+    return (QUADS && table.bins_log2 >= 2 && all == all ? top : all) * (1.f / 1073741824.f);
 }
 __device__ __forceinline__ float pa_per_unit(float unit)
 {
@@ -163,11 +167,11 @@ __device__ __forceinline__ float pa_per_unit(float unit)
 // bins into floats, bins cleared
 __device__ __forceinline__ void pa_flush(const PatchTable& t, int* hist, float* sums, float unit, int threads)
 {
-    const int copies = 1 << t.copies_log2;
+    const int copies = 1 << t.bins_log2;
     for (int i = threadIdx.x; i < t.entries; i += threads) {
         float v = 0.f;
         for (int c = 0; c < copies; ++c) {
-            int* at = hist + (i << t.copies_log2) + ((c + i) & (copies - 1));
+            int* at = hist + (i << t.bins_log2) + ((c + i) & (copies - 1));
             v += (float)*at;
             *at = 0;
         }
@@ -189,7 +193,8 @@ __device__ __forceinline__ void pa_store_bins(const PatchArgs& a, const PatchTab
 }
 
 enum { PA_FWD = 0, PA_ROWS = 1, PA_COLS = 2 };
-// fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu); ..._rows: rows of a block, in which `tiles` counts
+// fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu); ..._rows: rows of a block that has bins (a launch may take another
+// number where it has none, and sets `tiles`)
 int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int patch_fma_rows(int width);

@@ -12,7 +12,7 @@ constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
 constexpr int PF_STEP = 8;        // of which scores are held at a time
 constexpr int PF_WINDOW = 32;     // queries between two clearings of the bins: the unit is that much finer
 constexpr int PF_COPIES_LOG2 = 4; // few copies of them, so that clearing costs little
-constexpr int PF_TABLE_BYTES = PA_TABLE_BYTES_BINS / 2;
+constexpr int PF_TABLE_BYTES = 22 * 1024, PF_BINS_BYTES = 2 * PF_TABLE_BYTES;
 
 template <int W, int MAPS>
 struct PfShape {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, false, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, false, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -300,14 +300,15 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     }
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_BINS_BYTES, true, PF_COPIES_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
-    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1), words = BIAS ? table.entries << table.copies_log2 : 0;
-    int* hist = (int*)tab + words;
-    float* sums = tab + 2 * words;
+    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
+    const int fewer = table.copies_log2 - table.bins_log2;      // (0 or 1) copies of the bins than of the table
+    int* hist = (int*)tab + (BIAS ? table.entries << table.copies_log2 : 0);
+    float* sums = (float*)hist + (BIAS ? table.entries << table.bins_log2 : 0);
     if (learns) {
-        for (int i = threadIdx.x; i < words; i += PF_THREADS) hist[i] = 0;
+        for (int i = threadIdx.x; i < table.entries << table.bins_log2; i += PF_THREADS) hist[i] = 0;
         for (int i = threadIdx.x; i < table.entries; i += PF_THREADS) sums[i] = 0.f;
     }
     float unit = 0.f, per_unit = 0.f;
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
                 if (learns && part == 0 && kj < L) {
                     const int v = __float2int_rn(ds * per_unit);
 #pragma unroll
-                    for (int c = 0; c < 3; ++c) atomicAdd(hist + at[c], v);
+                    for (int c = 0; c < 3; ++c) atomicAdd(hist + (at[c] >> fewer), v);
                 }
 #pragma unroll
                 for (int i = 0; i < S::DP; ++i)
@@ -406,8 +407,8 @@ template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
 {
     const size_t table = BIAS ? PF_TABLE_BYTES : 0;
-    // in the pass over columns beside the table: its bins, and their sums
-    const size_t cols = table * (a.bins ? 3 : 1);
+    // in the pass over columns beside the table: its bins, and their sums (of every entry, at least a copy each)
+    const size_t cols = BIAS ? PF_BINS_BYTES + PF_TABLE_BYTES : 0;
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
     auto go = [&](auto kern, size_t smem) {
         const cudaError_t e = BIAS ? allow_smem(kern) : cudaSuccess;

@@ -27,10 +27,10 @@ struct PmChunk {
 constexpr int PM_STAGES = 3;
 constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
-// sums of the bins: entries of a table of eight copies, or of the largest bound (patch_attn.cuh)
+// bytes for the sums of the bins: entries of a table of eight copies, or of the largest bound (patch_attn.cuh)
 static int pm_sums_bytes(int bnd)
 {
-    return (3 * (2 * bnd + 1) > PA_TABLE_BYTES_BINS / 32 ? 3 * (2 * bnd + 1) : PA_TABLE_BYTES_BINS / 32) * 4;
+    return (3 * (2 * bnd + 1) > PA_BINS_BYTES / 64 ? 3 * (2 * bnd + 1) : PA_BINS_BYTES / 64) * 4;
 }
 constexpr float PM_LOWEST = -1e30f;
 
@@ -199,46 +199,63 @@ __device__ __forceinline__ void pm_rows(const __nv_bfloat16* p0, const __nv_bflo
         }
 }
 
-// s[m] = rows of this warp x 16 rows of the tile, transposed: MAPS sums of W / MAPS products each
-template <int W, int MAPS>
-__device__ __forceinline__ void pm_products(const uint32_t (&f)[W / 16][4], uint32_t tile, int row0, float (&s)[MAPS][2][4])
+// s[rt][m] = 16 rows of this warp x 16 rows of the tile, transposed: MAPS sums of W / MAPS products each
+template <int W, int MAPS, int RT>
+__device__ __forceinline__ void pm_products(const uint32_t (&f)[RT][W / 16][4], uint32_t tile, int row0,
+                                            float (&s)[RT][MAPS][2][4])
 {
     const int lane = threadIdx.x & 31, r = row0 + (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m)
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int m = 0; m < MAPS; ++m)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[m][i][j] = 0.f;
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[x][m][i][j] = 0.f;
 #pragma unroll
     for (int k = 0; k < W / 16; ++k) {
         uint32_t b[4];
         ldmatrix_x4(b, tile + pm_offset<W>(r, 2 * k + c));
-        if (W / MAPS == 8) {
-            // a map's eight values are one half of the fragment
-            mma_bf16_k8(s[0][0], f[k][0], f[k][1], b[0]);
-            mma_bf16_k8(s[0][1], f[k][0], f[k][1], b[2]);
-            mma_bf16_k8(s[MAPS - 1][0], f[k][2], f[k][3], b[1]);
-            mma_bf16_k8(s[MAPS - 1][1], f[k][2], f[k][3], b[3]);
-        } else {
-            const int m = k * 16 / (W / MAPS);
-            mma_bf16(s[m][0], f[k], b[0], b[1]);
-            mma_bf16(s[m][1], f[k], b[2], b[3]);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            if (W / MAPS == 8) {
+                // a map's eight values are one half of the fragment
+                mma_bf16_k8(s[x][0][0], f[x][k][0], f[x][k][1], b[0]);
+                mma_bf16_k8(s[x][0][1], f[x][k][0], f[x][k][1], b[2]);
+                mma_bf16_k8(s[x][MAPS - 1][0], f[x][k][2], f[x][k][3], b[1]);
+                mma_bf16_k8(s[x][MAPS - 1][1], f[x][k][2], f[x][k][3], b[3]);
+            } else {
+                const int m = k * 16 / (W / MAPS);
+                mma_bf16(s[x][m][0], f[x][k], b[0], b[1]);
+                mma_bf16(s[x][m][1], f[x][k], b[2], b[3]);
+            }
         }
     }
 }
 
-// acc += P x 16 rows of the tile (W values each); P of map m for the values of map m, or one P for all (MAPS = 1)
-template <int W, int MAPS>
-__device__ __forceinline__ void pm_accumulate(const uint32_t (&p)[MAPS][4], uint32_t tile, int row0, float (&acc)[W / 8][4])
+// acc += P x 16 rows of the tile (W values each); P of map m for the values of map m, or one P for all (MAPS = 1).  With
+// `acc2` the same of P2 to that.
+template <int W, int MAPS, int RT, bool TWO = false>
+__device__ __forceinline__ void pm_accumulate(const uint32_t (&p)[RT][MAPS][4], uint32_t tile, int row0,
+                                              float (&acc)[RT][W / 8][4], const uint32_t (&p2)[RT][MAPS][4],
+                                              float (&acc2)[RT][W / 8][4])
 {
+    constexpr int D = W / MAPS;
     const int lane = threadIdx.x & 31, r = row0 + (lane & 15), c = lane >> 4;
 #pragma unroll
     for (int k = 0; k < W / 16; ++k) {
         uint32_t b[4];
         ldmatrix_x4_trans(b, tile + pm_offset<W>(r, 2 * k + c));
-        mma_bf16(acc[2 * k], p[2 * k * 8 / (W / MAPS)], b[0], b[1]);
-        mma_bf16(acc[2 * k + 1], p[(2 * k + 1) * 8 / (W / MAPS)], b[2], b[3]);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            mma_bf16(acc[x][2 * k], p[x][16 * k / D], b[0], b[1]);
+            mma_bf16(acc[x][2 * k + 1], p[x][(16 * k + 8) / D], b[2], b[3]);
+            if (TWO) {
+                mma_bf16(acc2[x][2 * k], p2[x][16 * k / D], b[0], b[1]);
+                mma_bf16(acc2[x][2 * k + 1], p2[x][(16 * k + 8) / D], b[2], b[3]);
+            }
+        }
     }
 }
 
@@ -269,22 +286,27 @@ __device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTab
     for (int c = 0; c < 3; ++c)
         g[c] = b.lo[c] + ((t.reach[c] + sign * pa_coord(a, e >= 0 ? e : -(e + 1), c)) << (t.copies_log2 + 2));
 }
-// places of the entries of four pairs (rows g0, g1 of this lane and two of the other side); SIGN: the lane's point is
+// coordinates of the other side's rows j and j + 1
+template <int CH>
+__device__ __forceinline__ void pm_coords(const int* gs, int j, int2 (&o)[3])
+{
+#pragma unroll
+    for (int c = 0; c < 3; ++c) o[c] = *(const int2*)(gs + c * CH + j);
+}
+// places of the entries of four pairs (rows g[0], g[1] of this lane and two of the other side); SIGN: the lane's point is
 // the query (+1) or the key
-template <int SIGN, int CH, bool CLAMP>
-__device__ __forceinline__ void pm_places(const PmBias& b, const int (&g0)[3], const int (&g1)[3], const int* gs, int j,
-                                          uint32_t (&at)[4][3])
+template <int SIGN, bool CLAMP>
+__device__ __forceinline__ void pm_places(const PmBias& b, const int (&g)[2][3], const int2 (&o)[3], uint32_t (&at)[4][3])
 {
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-        const int2 o = *(const int2*)(gs + c * CH + j);
         auto place = [&](int mine, int other) {
             return (uint32_t)(CLAMP ? min(__viaddmax_s32(mine, -SIGN * other, b.lo[c]), b.hi[c]) : mine - SIGN * other);
         };
-        at[0][c] = place(g0[c], o.x);
-        at[1][c] = place(g0[c], o.y);
-        at[2][c] = place(g1[c], o.x);
-        at[3][c] = place(g1[c], o.y);
+        at[0][c] = place(g[0][c], o[c].x);
+        at[1][c] = place(g[0][c], o[c].y);
+        at[2][c] = place(g[1][c], o[c].x);
+        at[3][c] = place(g[1][c], o[c].y);
     }
 }
 // scores and biases of four pairs, in powers of two
@@ -326,135 +348,179 @@ __device__ __forceinline__ PmPlace pm_place(const PatchArgs& a)
     p.L = pa_sequence(a, p.seq, p.start);
     return p;
 }
+// this lane's rows of the RT tiles of its warp: row g + 8 r of tile x
+template <int RT>
+struct PmOwn {
+    int row[RT][2], e[RT][2];      // e: of the row list, -1 for rows that are not there
+    bool any;                      // whether one of the warp's answers for a point
+    __device__ __forceinline__ void load(const PatchArgs& a, const PmPlace& w, int first)
+    {
+        any = false;
+#pragma unroll
+        for (int x = 0; x < RT; ++x)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                row[x][r] = first + (int)(threadIdx.x / 32) * 16 * RT + 16 * x + ((threadIdx.x & 31) >> 2) + 8 * r;
+                e[x][r] = row[x][r] < w.L ? a.rows[w.start + row[x][r]] : -1;
+                any |= e[x][r] >= 0;
+            }
+        any = __any_sync(0xffffffffu, any);
+    }
+};
+// fragments of a matrix's rows (this head's W values from `base` on), zeros for rows that answer for no point
+template <int W, int RT>
+__device__ __forceinline__ void pm_own_rows(const PmOwn<RT>& own, const __nv_bfloat16* base, int64_t stride, uint32_t flip,
+                                            uint32_t (&f)[RT][W / 16][4])
+{
+#pragma unroll
+    for (int x = 0; x < RT; ++x)
+        pm_rows<W>(own.e[x][0] >= 0 ? base + own.e[x][0] * stride : nullptr,
+                   own.e[x][1] >= 0 ? base + own.e[x][1] * stride : nullptr, flip, f[x]);
+}
 
 // ------------------------------------------------------------------------------------------------- forward
-template <int W, int MAPS, bool BIAS, bool KEEP>
+template <int W, int MAPS, bool BIAS, bool KEEP, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patch_mma_fwd_kernel(const PatchArgs a)
 {
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
-    const int q0 = w.tile * PM_ROWS, L = w.L;
+    const int q0 = w.tile * PM_ROWS * RT, L = w.L;
     if (q0 >= L) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r0 = q0 + (threadIdx.x / 32) * 16 + g, r1 = r0 + 8;
-    const int e0 = r0 < L ? a.rows[w.start + r0] : -1, e1 = r1 < L ? a.rows[w.start + r1] : -1;
-    const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
+    const int t = threadIdx.x & 3;
+    PmOwn<RT> own;
+    own.load(a, w, q0);
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES);
+    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES, false);
     PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
-    int g0[3], g1[3];
+    int point[RT][2][3];
     if (BIAS) {
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, w.start, L, r0, 1, g0);
-        pm_bias_point(a, table, bias, w.start, L, r1, 1, g1);
+#pragma unroll
+        for (int x = 0; x < RT; ++x)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], 1, point[x][r]);
     }
-    uint32_t q[W / 16][4];
+    uint32_t q[RT][W / 16][4];
     // (of a negative scale the sign goes to the queries, so that larger products are larger scores)
-    pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr,
-               a.scale < 0.f ? 0x80008000u : 0u, q);
+    pm_own_rows<W, RT>(own, base, stride, a.scale < 0.f ? 0x80008000u : 0u, q);
     const float scale2 = fabsf(a.scale) * PA_LOG2E;
-    float o[MAPS][W / 8][4], sum[MAPS][4], m[MAPS][2];
-    uint64_t l[MAPS][2];
+    float o[MAPS][RT][W / 8][4], sum[MAPS][RT][4], m[MAPS][RT][2];
+    uint64_t l[MAPS][RT][2];
 #pragma unroll
-    for (int k = 0; k < MAPS; ++k) {
-        m[k][0] = m[k][1] = PM_LOWEST;
-        l[k][0] = l[k][1] = 0;
+    for (int k = 0; k < MAPS; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            sum[k][j] = 0.f;
+        for (int x = 0; x < RT; ++x) {
+            m[k][x][0] = m[k][x][1] = PM_LOWEST;
+            l[k][x][0] = l[k][x][1] = 0;
 #pragma unroll
-            for (int i = 0; i < W / 8; ++i) o[k][i][j] = 0.f;
+            for (int j = 0; j < 4; ++j) {
+                sum[k][x][j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < W / 8; ++i) o[k][x][i][j] = 0.f;
+            }
         }
-    }
     constexpr uint32_t ONES = 0x3f803f80u;
-    constexpr int KG = 32;      // keys whose scores are held at a time
+    constexpr int KG = 32 / RT;      // keys whose scores are held at a time
     auto walk = [&](auto clamp) {
         constexpr bool CLAMP = decltype(clamp)::value;
         for (int i = 0; i * CH < L; ++i) {
             const unsigned char* st = in.next(i);
-            if (!active) continue;
+            if (!own.any) continue;
             const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
             const int* gs = (const int*)(st + S::GRID);
             const int nk = L - i * CH;
 #pragma unroll 2
             for (int j0 = 0; j0 < CH; j0 += KG) {
                 if (j0 >= nk) break;
-                float s[KG / 16][MAPS][2][4];
+                float s[KG / 16][RT][MAPS][2][4];
 #pragma unroll
                 for (int u = 0; u < KG / 16; ++u) {
-                    pm_products<W, MAPS>(q, ks, j0 + 16 * u, s[u]);
+                    pm_products<W, MAPS, RT>(q, ks, j0 + 16 * u, s[u]);
                     if (BIAS)
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
-                            uint32_t at[4][3];
-                            pm_places<1, CH, CLAMP>(bias, g0, g1, gs, j0 + 16 * u + 8 * n + 2 * t, at);
-                            pm_bias(at, scale2, s[u][0][n]);
+                            int2 g[3];
+                            pm_coords<CH>(gs, j0 + 16 * u + 8 * n + 2 * t, g);
+#pragma unroll
+                            for (int x = 0; x < RT; ++x) {
+                                uint32_t at[4][3];
+                                pm_places<1, CLAMP>(bias, point[x], g, at);
+                                pm_bias(at, scale2, s[u][x][0][n]);
+                            }
                         }
                     if (j0 + KG > nk)
 #pragma unroll
-                        for (int k = 0; k < MAPS; ++k)
+                        for (int x = 0; x < RT; ++x)
 #pragma unroll
-                            for (int n = 0; n < 2; ++n)
+                            for (int k = 0; k < MAPS; ++k)
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    if (j0 + 16 * u + 8 * n + 2 * t + (c & 1) >= nk) s[u][k][n][c] = -INFINITY;
+                                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c)
+                                        if (j0 + 16 * u + 8 * n + 2 * t + (c & 1) >= nk) s[u][x][k][n][c] = -INFINITY;
                 }
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
-                    float top[2];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        top[r] = fmaxf(s[0][k][0][2 * r], s[0][k][0][2 * r + 1]);
-#pragma unroll
-                        for (int u = 0; u < KG / 16; ++u)
-#pragma unroll
-                            for (int n = 0; n < 2; ++n)
-                                if (u + n) top[r] = pm_max3(top[r], s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
-                        if (!BIAS) top[r] *= scale2;
-                    }
-                    if (__any_sync(0xffffffffu, top[0] > m[k][0] + PM_LAZY || top[1] > m[k][1] + PM_LAZY)) {
+                    for (int x = 0; x < RT; ++x) {
+                        float top[2];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                            top[r] = fmaxf(m[k][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
-                            const float fix = fast_exp2(m[k][r] - top[r]);
-                            m[k][r] = top[r];
-                            l[k][r] = mul2(l[k][r], pm_both(fix));
-                            sum[k][2 * r] *= fix;
+                            top[r] = fmaxf(s[0][x][k][0][2 * r], s[0][x][k][0][2 * r + 1]);
 #pragma unroll
-                            for (int n = 0; n < W / 8; ++n) {
-                                o[k][n][2 * r] *= fix;
-                                o[k][n][2 * r + 1] *= fix;
+                            for (int u = 0; u < KG / 16; ++u)
+#pragma unroll
+                                for (int n = 0; n < 2; ++n)
+                                    if (u + n) top[r] = pm_max3(top[r], s[u][x][k][n][2 * r], s[u][x][k][n][2 * r + 1]);
+                            if (!BIAS) top[r] *= scale2;
+                        }
+                        if (__any_sync(0xffffffffu, top[0] > m[k][x][0] + PM_LAZY || top[1] > m[k][x][1] + PM_LAZY)) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                                top[r] = fmaxf(m[k][x][r], fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)));
+                                const float fix = fast_exp2(m[k][x][r] - top[r]);
+                                m[k][x][r] = top[r];
+                                l[k][x][r] = mul2(l[k][x][r], pm_both(fix));
+                                sum[k][x][2 * r] *= fix;
+#pragma unroll
+                                for (int n = 0; n < W / 8; ++n) {
+                                    o[k][x][n][2 * r] *= fix;
+                                    o[k][x][n][2 * r + 1] *= fix;
+                                }
                             }
                         }
                     }
 #pragma unroll
                     for (int u = 0; u < KG / 16; ++u) {
-                        uint32_t p[1][4];
+                        uint32_t p[RT][1][4];
 #pragma unroll
-                        for (int n = 0; n < 2; ++n)
+                        for (int x = 0; x < RT; ++x) {
 #pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                const uint64_t v = pack2(s[u][k][n][2 * r], s[u][k][n][2 * r + 1]);
-                                const uint64_t e = pm_exp2(BIAS ? add2(v, pm_both(-m[k][r]))
-                                                                : fma2(v, pm_both(scale2), pm_both(-m[k][r])));
-                                if (KEEP) l[k][r] = add2(l[k][r], e);
-                                float x, y;
-                                unpack2(e, x, y);
-                                p[0][2 * n + r] = pack_bf16(x, y);
-                            }
-                        pm_accumulate<W, 1>(p, vs, j0 + 16 * u, o[k]);
-                        // the sum that the result is divided by is that of the rounded probabilities
-                        mma_bf16(sum[k], p[0], ONES, ONES);
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) {
+                                    const uint64_t v = pack2(s[u][x][k][n][2 * r], s[u][x][k][n][2 * r + 1]);
+                                    const uint64_t e = pm_exp2(BIAS ? add2(v, pm_both(-m[k][x][r]))
+                                                                    : fma2(v, pm_both(scale2), pm_both(-m[k][x][r])));
+                                    if (KEEP) l[k][x][r] = add2(l[k][x][r], e);
+                                    float y, z;
+                                    unpack2(e, y, z);
+                                    p[x][0][2 * n + r] = pack_bf16(y, z);
+                                }
+                            // the sum that the result is divided by is that of the rounded probabilities
+                            mma_bf16(sum[k][x], p[x][0], ONES, ONES);
+                        }
+                        pm_accumulate<W, 1, RT>(p, vs, j0 + 16 * u, o[k], p, o[k]);
                     }
                 }
             }
@@ -463,60 +529,41 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     if (BIAS && table.clamps) walk(PmYes());
     else walk(PmNo());
     in.end();
-    if (!active) return;
-    if (KEEP)
-#pragma unroll
-        for (int k = 0; k < MAPS; ++k)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float v = hsum2(l[k][r]);
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                const int row = r ? r1 : r0;
-                if (t == 0 && row < L) a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = m[k][r] + log2f(v);
-            }
+    if (!own.any) return;
     const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int e = r ? e1 : e0;
-        if (e < 0) continue;
-        const float w0 = 1.f / sum[0][2 * r], w1 = MAPS == 2 ? lam / sum[MAPS - 1][2 * r] : 0.f;
-        uint32_t* op = (uint32_t*)((__nv_bfloat16*)a.out + (int64_t)e * a.C + w.h * W);
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-        for (int n = 0; n < W / 8; ++n) {
-            float x = o[0][n][2 * r] * w0, y = o[0][n][2 * r + 1] * w0;
-            if (MAPS == 2) {
-                x -= o[MAPS - 1][n][2 * r] * w1;
-                y -= o[MAPS - 1][n][2 * r + 1] * w1;
-            }
-            op[4 * n + t] = pack_bf16(x, y);
-            if (MAPS == 2 && KEEP) {
-                const float w2 = 1.f / sum[MAPS - 1][2 * r];
-                ((uint32_t*)((__nv_bfloat16*)a.second + (int64_t)e * a.C + w.h * W))[4 * n + t] =
-                    pack_bf16(o[MAPS - 1][n][2 * r] * w2, o[MAPS - 1][n][2 * r + 1] * w2);
+        for (int r = 0; r < 2; ++r) {
+            const int e = own.e[x][r];
+            if (KEEP)
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    float v = hsum2(l[k][x][r]);
+                    v += __shfl_xor_sync(0xffffffffu, v, 1);
+                    v += __shfl_xor_sync(0xffffffffu, v, 2);
+                    if (t == 0 && e >= 0)
+                        a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r]] = m[k][x][r] + log2f(v);
+                }
+            if (e < 0) continue;
+            const float w0 = 1.f / sum[0][x][2 * r], w2 = 1.f / sum[MAPS - 1][x][2 * r], w1 = lam * w2;
+            const int64_t at = (int64_t)e * a.C + w.h * W;
+#pragma unroll
+            for (int n = 0; n < W / 8; ++n) {
+                float y = o[0][x][n][2 * r] * w0, z = o[0][x][n][2 * r + 1] * w0;
+                if (MAPS == 2) {
+                    y -= o[MAPS - 1][x][n][2 * r] * w1;
+                    z -= o[MAPS - 1][x][n][2 * r + 1] * w1;
+                }
+                ((uint32_t*)((__nv_bfloat16*)a.out + at))[4 * n + t] = pack_bf16(y, z);
+                if (MAPS == 2 && KEEP)
+                    ((uint32_t*)((__nv_bfloat16*)a.second + at))[4 * n + t] =
+                        pack_bf16(o[MAPS - 1][x][n][2 * r] * w2, o[MAPS - 1][x][n][2 * r + 1] * w2);
             }
         }
-    }
 }
 
 // ------------------------------------------------------------------------- backward, a warp's own queries
-// acc1 += P1 x the tile's rows, acc2 += P2 x them (each map's for its own values)
-template <int W, int MAPS>
-__device__ __forceinline__ void pm_accumulate2(const uint32_t (&p1)[MAPS][4], const uint32_t (&p2)[MAPS][4], uint32_t tile,
-                                               int row0, float (&acc1)[W / 8][4], float (&acc2)[W / 8][4])
-{
-    const int lane = threadIdx.x & 31, r = row0 + (lane & 15), c = lane >> 4;
-#pragma unroll
-    for (int k = 0; k < W / 16; ++k) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, tile + pm_offset<W>(r, 2 * k + c));
-        constexpr int D = W / MAPS;
-        mma_bf16(acc1[2 * k], p1[16 * k / D], b[0], b[1]);
-        mma_bf16(acc1[2 * k + 1], p1[(16 * k + 8) / D], b[2], b[3]);
-        mma_bf16(acc2[2 * k], p2[16 * k / D], b[0], b[1]);
-        mma_bf16(acc2[2 * k + 1], p2[(16 * k + 8) / D], b[2], b[3]);
-    }
-}
 // row g and row g + 8 of two fragments: sums of products over the four lanes that hold them
 template <int W>
 __device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], const uint32_t (&y)[W / 16][4], float (&d)[2])
@@ -538,119 +585,134 @@ __device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], cons
     }
 }
 
-template <int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_kernel(const PatchArgs a)
 {
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
-    const int q0 = w.tile * PM_ROWS, L = w.L;
+    const int q0 = w.tile * PM_ROWS * RT, L = w.L;
     if (q0 >= L) return;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r0 = q0 + (threadIdx.x / 32) * 16 + g, r1 = r0 + 8;
-    const int e0 = r0 < L ? a.rows[w.start + r0] : -1, e1 = r1 < L ? a.rows[w.start + r1] : -1;
-    const bool active = __any_sync(0xffffffffu, e0 >= 0 || e1 >= 0);
+    const int t = threadIdx.x & 3;
+    PmOwn<RT> own;
+    own.load(a, w, q0);
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES);
+    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES, false);
     PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
-    int g0[3], g1[3];
+    int point[RT][2][3];
     if (BIAS) {
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, w.start, L, r0, 1, g0);
-        pm_bias_point(a, table, bias, w.start, L, r1, 1, g1);
+#pragma unroll
+        for (int x = 0; x < RT; ++x)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], 1, point[x][r]);
     }
-    uint32_t q[W / 16][4], go[W / 16][4];
-    // rows of a matrix of C columns, this head's; zeros for rows that answer for no point
-    auto own_rows = [&](const void* m, uint32_t (&f)[W / 16][4]) {
-        const __nv_bfloat16* p = (const __nv_bfloat16*)m + w.h * W;
-        pm_rows<W>(e0 >= 0 ? p + (int64_t)e0 * a.C : nullptr, e1 >= 0 ? p + (int64_t)e1 * a.C : nullptr, 0u, f);
-    };
-    own_rows(a.dout, go);
-    float lse[MAPS][2], shift[MAPS][2], most[2] = {0.f, 0.f};
-    uint64_t E[MAPS][2], total[MAPS][2];
+    uint32_t q[RT][W / 16][4], go[RT][W / 16][4];
+    float lse[MAPS][RT][2], shift[MAPS][RT][2], most[RT][2];
+    uint64_t E[MAPS][RT][2], total[MAPS][RT][2];
     const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
-    own_rows(a.out, q);
-    pm_row_dots<W>(go, q, shift[0]);
+    pm_own_rows<W, RT>(own, (const __nv_bfloat16*)a.dout + w.h * W, a.C, 0u, go);
+    pm_own_rows<W, RT>(own, (const __nv_bfloat16*)a.out + w.h * W, a.C, 0u, q);
+#pragma unroll
+    for (int x = 0; x < RT; ++x) pm_row_dots<W>(go[x], q[x], shift[0][x]);
     if (MAPS == 2) {
-        own_rows(a.second, q);
-        pm_row_dots<W>(go, q, shift[MAPS - 1]);
-        shift[0][0] += lam * shift[MAPS - 1][0];
-        shift[0][1] += lam * shift[MAPS - 1][1];
-    }
-    pm_rows<W>(e0 >= 0 ? base + e0 * stride : nullptr, e1 >= 0 ? base + e1 * stride : nullptr, 0u, q);
-    const float scale2 = a.scale * PA_LOG2E;
-    float dq[W / 8][4], pk[W / 8][4];
+        pm_own_rows<W, RT>(own, (const __nv_bfloat16*)a.second + w.h * W, a.C, 0u, q);
 #pragma unroll
-    for (int n = 0; n < W / 8; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) dq[n][c] = pk[n][c] = 0.f;
-#pragma unroll
-    for (int k = 0; k < MAPS; ++k)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const bool own = (r ? e1 : e0) >= 0;
-            lse[k][r] = own ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + (r ? r1 : r0)] : INFINITY;
-            E[k][r] = total[k][r] = 0;
+        for (int x = 0; x < RT; ++x) {
+            pm_row_dots<W>(go[x], q[x], shift[MAPS - 1][x]);
+            shift[0][x][0] += lam * shift[MAPS - 1][x][0];
+            shift[0][x][1] += lam * shift[MAPS - 1][x][1];
         }
+    }
+    pm_own_rows<W, RT>(own, base, stride, 0u, q);
+    const float scale2 = a.scale * PA_LOG2E;
+    float dq[RT][W / 8][4], pk[RT][W / 8][4];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        most[x][0] = most[x][1] = 0.f;
+#pragma unroll
+        for (int n = 0; n < W / 8; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) dq[x][n][c] = pk[x][n][c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                lse[k][x][r] = own.e[x][r] >= 0 ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r]]
+                                                : INFINITY;
+                E[k][x][r] = total[k][x][r] = 0;
+            }
+    }
 
     auto walk = [&](auto clamp) {
         constexpr bool CLAMP = decltype(clamp)::value;
         for (int i = 0; i * CH < L; ++i) {
             const unsigned char* st = in.next(i);
-            if (!active) continue;
+            if (!own.any) continue;
             const uint32_t ks = smem_u32(st), vs = ks + S::TILE;
             const int* gs = (const int*)(st + S::GRID);
             const int nk = L - i * CH;
-#pragma unroll 2
+#pragma unroll (2 / RT)
             for (int j0 = 0; j0 < CH; j0 += 16) {
                 if (j0 >= nk) break;
-                float s[MAPS][2][4], G[1][2][4];
-                pm_products<W, MAPS>(q, ks, j0, s);
-                pm_products<W, 1>(go, vs, j0, G);
+                float s[RT][MAPS][2][4], G[RT][1][2][4];
+                pm_products<W, MAPS, RT>(q, ks, j0, s);
+                pm_products<W, 1, RT>(go, vs, j0, G);
                 if (BIAS)
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        uint32_t at[4][3];
-                        pm_places<1, CH, CLAMP>(bias, g0, g1, gs, j0 + 8 * n + 2 * t, at);
-                        pm_bias(at, scale2, s[0][n]);
+                        int2 g[3];
+                        pm_coords<CH>(gs, j0 + 8 * n + 2 * t, g);
+#pragma unroll
+                        for (int x = 0; x < RT; ++x) {
+                            uint32_t at[4][3];
+                            pm_places<1, CLAMP>(bias, point[x], g, at);
+                            pm_bias(at, scale2, s[x][0][n]);
+                        }
                     }
                 if (j0 + 16 > nk)
+#pragma unroll
+                    for (int x = 0; x < RT; ++x)
+#pragma unroll
+                        for (int k = 0; k < MAPS; ++k)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    if (j0 + 8 * n + 2 * t + (c & 1) >= nk)
+                                        s[x][k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
+                uint32_t p[RT][MAPS][4], d[RT][MAPS][4];
+#pragma unroll
+                for (int x = 0; x < RT; ++x)
 #pragma unroll
                     for (int k = 0; k < MAPS; ++k)
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (j0 + 8 * n + 2 * t + (c & 1) >= nk) s[k][n][c] = BIAS || a.scale > 0.f ? -INFINITY : INFINITY;
-                uint32_t p[MAPS][4], d[MAPS][4];
-#pragma unroll
-                for (int k = 0; k < MAPS; ++k)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
-                            const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][r]))
-                                                             : fma2(v, pm_both(scale2), pm_both(-lse[k][r])));
-                            total[k][r] = add2(total[k][r], pr);
-                            const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), pm_both(-shift[k][r])));
-                            E[k][r] = add2(E[k][r], ds);
-                            float x, y;
-                            unpack2(pr, x, y);
-                            p[k][2 * n + r] = pack_bf16(x, y);
-                            unpack2(ds, x, y);
-                            d[k][2 * n + r] = pack_bf16(x, y);
-                            if (BIAS) most[r] += fabsf(x) + fabsf(y);
-                        }
-                pm_accumulate2<W, MAPS>(d, p, ks, j0, dq, pk);
+                            for (int r = 0; r < 2; ++r) {
+                                const uint64_t v = pack2(s[x][k][n][2 * r], s[x][k][n][2 * r + 1]);
+                                const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][x][r]))
+                                                                 : fma2(v, pm_both(scale2), pm_both(-lse[k][x][r])));
+                                total[k][x][r] = add2(total[k][x][r], pr);
+                                const uint64_t ds = mul2(pr, add2(pack2(G[x][0][n][2 * r], G[x][0][n][2 * r + 1]),
+                                                                  pm_both(-shift[k][x][r])));
+                                E[k][x][r] = add2(E[k][x][r], ds);
+                                float y, z;
+                                unpack2(pr, y, z);
+                                p[x][k][2 * n + r] = pack_bf16(y, z);
+                                unpack2(ds, y, z);
+                                d[x][k][2 * n + r] = pack_bf16(y, z);
+                                if (BIAS) most[x][r] += fabsf(y) + fabsf(z);
+                            }
+                pm_accumulate<W, MAPS, RT, true>(d, ks, j0, dq, p, pk);
             }
         }
     };
@@ -662,43 +724,45 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
         return v + __shfl_xor_sync(0xffffffffu, v, 2);
     };
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int e = r ? e1 : e0, row = r ? r1 : r0;
-        float by[MAPS], eps[MAPS];
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-        for (int k = 0; k < MAPS; ++k) {
-            // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: divided out
-            const float sum = quad(hsum2(total[k][r])), inv = e >= 0 ? 1.f / sum : 0.f;
-            eps[k] = quad(hsum2(E[k][r])) * inv;
-            by[k] = inv * a.scale * (k == 1 ? -lam : 1.f);
-            if (t == 0 && row < L)
-                a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = e >= 0 ? shift[k][r] + eps[k] : 0.f;
-            if (BIAS && a.reach) {
-                const float reach = quad(most[r]) * inv + fabsf(eps[0]);
-                if (t == 0 && row < L) a.reach[(int64_t)w.h * a.n_pad + w.start + row] = e >= 0 ? reach : 0.f;
+        for (int r = 0; r < 2; ++r) {
+            const int e = own.e[x][r], row = own.row[x][r];
+            float by[MAPS], eps[MAPS];
+#pragma unroll
+            for (int k = 0; k < MAPS; ++k) {
+                // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: divided out
+                const float sum = quad(hsum2(total[k][x][r])), inv = e >= 0 ? 1.f / sum : 0.f;
+                eps[k] = quad(hsum2(E[k][x][r])) * inv;
+                by[k] = inv * a.scale * (k == 1 ? -lam : 1.f);
+                if (t == 0 && row < L)
+                    a.delta[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + row] = e >= 0 ? shift[k][x][r] + eps[k] : 0.f;
+                if (BIAS && a.reach) {
+                    const float reach = quad(most[x][r]) * inv + fabsf(eps[0]);
+                    if (t == 0 && row < L) a.reach[(int64_t)w.h * a.n_pad + w.start + row] = e >= 0 ? reach : 0.f;
+                }
+            }
+            if (e < 0) continue;
+            uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + w.h * W);
+#pragma unroll
+            for (int n = 0; n < W / 8; ++n) {
+                const int k = n * 8 / (W / MAPS);
+                dst[4 * n + t] = pack_bf16((dq[x][n][2 * r] - eps[k] * pk[x][n][2 * r]) * by[k],
+                                           (dq[x][n][2 * r + 1] - eps[k] * pk[x][n][2 * r + 1]) * by[k]);
             }
         }
-        if (e < 0) continue;
-        uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + w.h * W);
-#pragma unroll
-        for (int n = 0; n < W / 8; ++n) {
-            const int k = n * 8 / (W / MAPS);
-            dst[4 * n + t] = pack_bf16((dq[n][2 * r] - eps[k] * pk[n][2 * r]) * by[k],
-                                       (dq[n][2 * r + 1] - eps[k] * pk[n][2 * r + 1]) * by[k]);
-        }
-    }
 }
 
 // --------------------------------------------------------------------------- backward, a warp's own keys
-template <int W, int MAPS, bool BIAS>
+template <int W, int MAPS, bool BIAS, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_kernel(const PatchArgs a)
 {
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
-    const PmPlace w = pm_place(a);
     __shared__ float part[4 * PM_WARPS];
-    const int k0 = w.tile * PM_ROWS, L = w.L;
+    const PmPlace w = pm_place(a);
+    const int k0 = w.tile * PM_ROWS * RT, L = w.L;
     const bool learns = BIAS && a.bins;
     float* bins = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * 3 * (2 * a.bnd + 1) : nullptr;
     if (k0 >= L) {
@@ -706,44 +770,59 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
             for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PM_THREADS) bins[i] = 0.f;
         return;
     }
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int warp0 = k0 + (threadIdx.x / 32) * 16, r0 = warp0 + g, r1 = r0 + 8;
-    const bool there0 = r0 < L, there1 = r1 < L;
-    const int e0 = there0 ? a.rows[w.start + r0] : -1, e1 = there1 ? a.rows[w.start + r1] : -1;
-    const int64_t p0 = e0 >= 0 ? e0 : -(e0 + 1), p1 = e1 >= 0 ? e1 : -(e1 + 1), stride = 3 * (int64_t)a.C;
+    const int t = threadIdx.x & 3, warp0 = k0 + (int)(threadIdx.x / 32) * 16 * RT;
+    PmOwn<RT> own;
+    own.load(a, w, k0);
+    const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES_BINS);
+    if (BIAS) table = pa_table(a, w.seq, PA_BINS_BYTES, true);
     PmStream<W, MAPS, true, BIAS> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
                                         table.copies_log2 + 2, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);
     int* hist = (int*)(tab + (BIAS ? table.entries << table.copies_log2 : 0));
-    float* sums = (float*)hist + (hist - (int*)tab);
-    const uint32_t to_hist = smem_u32(hist) - smem_u32(tab);
+    float* sums = (float*)hist + (BIAS ? table.entries << table.bins_log2 : 0);
+    // from an entry's place to its bin's, in copies of this lane's number
+    const int fewer = table.copies_log2 - table.bins_log2, lane = threadIdx.x & 31;
+    const uint32_t to_hist = smem_u32(hist) + 4 * (lane & ((1 << table.bins_log2) - 1)) -
+                             ((smem_u32(tab) + 4 * (lane & ((1 << table.copies_log2) - 1))) >> fewer);
     PmBias bias;
-    int g0[3], g1[3];
+    int point[RT][2][3];
     float unit = 0.f, per_unit = 0.f;
     if (BIAS) {
         pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
         pm_bias_setup(table, smem_u32(tab), bias);
-        pm_bias_point(a, table, bias, w.start, L, r0, -1, g0);
-        pm_bias_point(a, table, bias, w.start, L, r1, -1, g1);
+#pragma unroll
+        for (int x = 0; x < RT; ++x)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], -1, point[x][r]);
         if (learns) {
-            for (int i = threadIdx.x; i < table.entries << table.copies_log2; i += PM_THREADS) hist[i] = 0;
+            for (int i = threadIdx.x; i < table.entries << table.bins_log2; i += PM_THREADS) hist[i] = 0;
             for (int i = threadIdx.x; i < table.entries; i += PM_THREADS) sums[i] = 0.f;
         }
     }
-    uint32_t kf[W / 16][4], vf[W / 16][4];
-    pm_rows<W>(there0 ? base + a.C + p0 * stride : nullptr, there1 ? base + a.C + p1 * stride : nullptr, 0u, kf);
-    pm_rows<W>(there0 ? base + 2 * a.C + p0 * stride : nullptr, there1 ? base + 2 * a.C + p1 * stride : nullptr, 0u, vf);
+    uint32_t kf[RT][W / 16][4], vf[RT][W / 16][4];
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+        const __nv_bfloat16* p[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int e = own.e[x][r];
+            p[r] = own.row[x][r] < L ? base + a.C + (e >= 0 ? e : -(e + 1)) * stride : nullptr;
+        }
+        pm_rows<W>(p[0], p[1], 0u, kf[x]);
+        pm_rows<W>(p[0] ? p[0] + a.C : nullptr, p[1] ? p[1] + a.C : nullptr, 0u, vf[x]);
+    }
     const float scale2 = a.scale * PA_LOG2E;
     const float minus_lam = MAPS == 2 ? -pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
-    float dk[W / 8][4], dv[W / 8][4];
+    float dk[RT][W / 8][4], dv[RT][W / 8][4];
 #pragma unroll
-    for (int n = 0; n < W / 8; ++n)
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
+        for (int n = 0; n < W / 8; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) dk[x][n][c] = dv[x][n][c] = 0.f;
 
     auto walk = [&](auto clamp) {
         constexpr bool CLAMP = decltype(clamp)::value;
@@ -762,61 +841,62 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
             const float* aux = (const float*)(st + S::AUX);
             const int* gs = (const int*)(st + S::GRID);
             const int nq = L - i * CH;
-#pragma unroll 2
+#pragma unroll (2 / RT)
             for (int j0 = 0; j0 < CH; j0 += 16) {
                 if (j0 >= nq) break;
-                float s[MAPS][2][4], G[1][2][4];
-                uint64_t mix[2][2];
-                uint32_t p[MAPS][4], pm[1][4];
-                pm_products<W, MAPS>(kf, qs, j0, s);
-                pm_products<W, 1>(vf, os, j0, G);
+                float s[RT][MAPS][2][4], G[RT][1][2][4];
+                uint32_t p[RT][MAPS][4], pm[RT][1][4];
+                pm_products<W, MAPS, RT>(kf, qs, j0, s);
+                pm_products<W, 1, RT>(vf, os, j0, G);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int j = j0 + 8 * n + 2 * t;
-                    uint32_t at[4][3];
-                    if (BIAS) {
-                        pm_places<-1, CH, CLAMP>(bias, g0, g1, gs, j, at);
-                        pm_bias(at, scale2, s[0][n]);
-                    }
+                    int2 g[3];
+                    if (BIAS) pm_coords<CH>(gs, j, g);
+                    uint64_t lse[MAPS], delta[MAPS];      // (negated as they are staged)
 #pragma unroll
                     for (int k = 0; k < MAPS; ++k) {
-                        // (negated as they are staged)
-                        const uint64_t lse = *(const uint64_t*)(aux + k * CH + j);
-                        const uint64_t delta = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
+                        lse[k] = *(const uint64_t*)(aux + k * CH + j);
+                        delta[k] = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
+                    }
+#pragma unroll
+                    for (int x = 0; x < RT; ++x) {
+                        uint32_t at[4][3];
+                        if (BIAS) {
+                            pm_places<-1, CLAMP>(bias, point[x], g, at);
+                            pm_bias(at, scale2, s[x][0][n]);
+                        }
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const uint64_t v = pack2(s[k][n][2 * r], s[k][n][2 * r + 1]);
-                            uint64_t pr = pm_exp2(BIAS ? add2(v, lse) : fma2(v, pm_both(scale2), lse));
-                            if (k == 1) pr = mul2(pr, pm_both(minus_lam));
-                            mix[n][r] = k == 0 ? pr : add2(mix[n][r], pr);
-                            const uint64_t ds = mul2(pr, add2(pack2(G[0][n][2 * r], G[0][n][2 * r + 1]), delta));
-                            float x, y;
-                            unpack2(ds, x, y);
-                            p[k][2 * n + r] = pack_bf16(x, y);
-                            if (BIAS) {
-                                s[0][n][2 * r] = x;
-                                s[0][n][2 * r + 1] = y;
+                            uint64_t mix = 0;
+#pragma unroll
+                            for (int k = 0; k < MAPS; ++k) {
+                                const uint64_t v = pack2(s[x][k][n][2 * r], s[x][k][n][2 * r + 1]);
+                                uint64_t pr = pm_exp2(BIAS ? add2(v, lse[k]) : fma2(v, pm_both(scale2), lse[k]));
+                                if (k == 1) pr = mul2(pr, pm_both(minus_lam));
+                                mix = k == 0 ? pr : add2(mix, pr);
+                                const uint64_t ds = mul2(pr, add2(pack2(G[x][0][n][2 * r], G[x][0][n][2 * r + 1]), delta[k]));
+                                float y, z;
+                                unpack2(ds, y, z);
+                                p[x][k][2 * n + r] = pack_bf16(y, z);
+                                // (rows beyond the patch have no key: their lanes add nothing)
+                                if (learns && own.row[x][r] < L) {
+                                    const int vy = __float2int_rn(y * per_unit), vz = __float2int_rn(z * per_unit);
+#pragma unroll
+                                    for (int c = 0; c < 3; ++c) {
+                                        pm_add_shared((at[2 * r][c] >> fewer) + to_hist, vy);
+                                        pm_add_shared((at[2 * r + 1][c] >> fewer) + to_hist, vz);
+                                    }
+                                }
                             }
+                            float y, z;
+                            unpack2(mix, y, z);
+                            pm[x][0][2 * n + r] = pack_bf16(y, z);
                         }
                     }
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float x, y;
-                        unpack2(mix[n][r], x, y);
-                        pm[0][2 * n + r] = pack_bf16(x, y);
-                    }
-                    // (rows beyond the patch have no key: their lanes add nothing)
-                    if (learns)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (c < 2 ? there0 : there1) {
-                                const int v = __float2int_rn(s[0][n][c] * per_unit);
-#pragma unroll
-                                for (int x = 0; x < 3; ++x) pm_add_shared(at[c][x] + to_hist, v);
-                            }
                 }
-                pm_accumulate<W, 1>(pm, os, j0, dv);
-                pm_accumulate<W, MAPS>(p, qs, j0, dk);
+                pm_accumulate<W, 1, RT>(pm, os, j0, dv, pm, dv);
+                pm_accumulate<W, MAPS, RT>(p, qs, j0, dk, p, dk);
             }
         }
     };
@@ -829,25 +909,27 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         pa_store_bins(a, table, sums, bins, PM_THREADS);
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (!(r ? there1 : there0)) continue;
-        const int e = r ? e1 : e0, slot = a.slot ? a.slot[w.start + (r ? r1 : r0)] : -1;
-        if (slot >= 0) {             // this point's other row is some other patch's: added up later
-            float2* dst = (float2*)(a.shared + (int64_t)slot * 2 * a.C + w.h * W);
+    for (int x = 0; x < RT; ++x)
 #pragma unroll
-            for (int n = 0; n < W / 8; ++n) {
-                dst[4 * n + t] = make_float2(dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
-                dst[a.C / 2 + 4 * n + t] = make_float2(dv[n][2 * r], dv[n][2 * r + 1]);
-            }
-        } else if (e >= 0) {
-            uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + a.C + w.h * W);
+        for (int r = 0; r < 2; ++r) {
+            if (own.row[x][r] >= L) continue;
+            const int e = own.e[x][r], slot = a.slot ? a.slot[w.start + own.row[x][r]] : -1;
+            if (slot >= 0) {             // this point's other row is some other patch's: added up later
+                float2* dst = (float2*)(a.shared + (int64_t)slot * 2 * a.C + w.h * W);
 #pragma unroll
-            for (int n = 0; n < W / 8; ++n) {
-                dst[4 * n + t] = pack_bf16(dk[n][2 * r] * a.scale, dk[n][2 * r + 1] * a.scale);
-                dst[a.C / 2 + 4 * n + t] = pack_bf16(dv[n][2 * r], dv[n][2 * r + 1]);
+                for (int n = 0; n < W / 8; ++n) {
+                    dst[4 * n + t] = make_float2(dk[x][n][2 * r] * a.scale, dk[x][n][2 * r + 1] * a.scale);
+                    dst[a.C / 2 + 4 * n + t] = make_float2(dv[x][n][2 * r], dv[x][n][2 * r + 1]);
+                }
+            } else if (e >= 0) {
+                uint32_t* dst = (uint32_t*)((__nv_bfloat16*)a.dqkv + e * stride + a.C + w.h * W);
+#pragma unroll
+                for (int n = 0; n < W / 8; ++n) {
+                    dst[4 * n + t] = pack_bf16(dk[x][n][2 * r] * a.scale, dk[x][n][2 * r + 1] * a.scale);
+                    dst[a.C / 2 + 4 * n + t] = pack_bf16(dv[x][n][2 * r], dv[x][n][2 * r + 1]);
+                }
             }
         }
-    }
 }
 
 template <typename K>
@@ -860,16 +942,36 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
     return check_launch("ptv3_patch_attention");
 }
 
-template <int W, int MAPS, bool BIAS>
-static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
+// Rows of a block, in tiles of 128: with two tiles to a warp what it reads of the other side serves twice the rows, where
+// registers allow it (heads of 16) and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and 397;
+// columns of the differential backward, 100 000 x 64, 347 and 321.  Not so forward without a bias (312, 326), rows (341, 465; with a
+// bias 464, 455) and columns with a bias (882, 891), and forward with a bias of 6 760 x 128 (64, 65).
+static int row_tiles(int64_t n_seq, int64_t longest, int heads, int width, int maps, bool bias, int pass)
 {
+    const int64_t blocks = n_seq * heads * ((longest + 2 * PM_ROWS - 1) / (2 * PM_ROWS));
+    return width == 16 && blocks >= 2 * SMS && (bias ? pass == PA_FWD : maps == 2 && pass == PA_COLS) ? 2 : 1;
+}
+
+template <int W, int MAPS, bool BIAS>
+static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
+{
+    PatchArgs a = args;
+    const int longest = a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad;
+    const int rt = row_tiles(a.n_seq, longest, a.H, W, MAPS, BIAS, pass);
+    a.tiles = ceil_div(longest, rt * PM_ROWS);
+    constexpr int FWD2 = W == 16 && BIAS ? 2 : 1, COLS2 = W == 16 && MAPS == 2 ? 2 : 1;
     const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES, smem = stages + (BIAS ? PA_TABLE_BYTES : 0);
-    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS>, a, smem, stream);
-    if (pass == PA_COLS)      // the table, its bins, and their sums
-        return launch(patch_mma_cols_kernel<W, MAPS, BIAS>, a,
-                      stages + (BIAS ? PA_TABLE_BYTES_BINS * (a.bins ? 2 : 1) + (a.bins ? pm_sums_bytes(a.bnd) : 0) : 0), stream);
-    return a.lse ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true>, a, smem, stream)
-                 : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false>, a, smem, stream);
+    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS, 1>, a, smem, stream);
+    if (pass == PA_COLS) {      // the table, its bins, and their sums
+        const size_t with_bins = stages + (BIAS ? PA_BINS_BYTES + pm_sums_bytes(a.bnd) : 0);
+        return rt == 2 ? launch(patch_mma_cols_kernel<W, MAPS, BIAS, COLS2>, a, with_bins, stream)
+                       : launch(patch_mma_cols_kernel<W, MAPS, BIAS, 1>, a, with_bins, stream);
+    }
+    if (a.lse)
+        return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, FWD2>, a, smem, stream)
+                       : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, 1>, a, smem, stream);
+    return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, FWD2>, a, smem, stream)
+                   : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, 1>, a, smem, stream);
 }
 
 template <int W>

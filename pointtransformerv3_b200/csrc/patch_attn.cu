@@ -198,10 +198,13 @@ static int longest(const ptv3_patch_attention_args* p)
 {
     return (int)(p->max_seqlen < p->n_pad ? p->max_seqlen : p->n_pad);
 }
-// blocks of the longest sequence
-static int patch_tiles(const ptv3_patch_attention_args* p)
+// blocks that leave bins, heads apart
+static int64_t bin_blocks(const ptv3_patch_attention_args* p)
 {
-    return ceil_div(longest(p), p->dtype == PTV3_DTYPE_BF16 ? patch_mma_rows() : patch_fma_rows(p->channels / p->heads));
+    const int width = p->channels / p->heads;
+    return (int64_t)p->n_seq * ceil_div(longest(p), p->dtype == PTV3_DTYPE_BF16
+                                                        ? patch_mma_cols_rows(p->n_seq, longest(p), p->heads, width)
+                                                        : patch_fma_cols_rows(width));
 }
 
 static int launch_patch(const ptv3_patch_attention_args* p, const PatchArgs& a, int pass, cudaStream_t stream)
@@ -214,7 +217,7 @@ static int launch_patch(const ptv3_patch_attention_args* p, const PatchArgs& a, 
 struct PatchWorkspace {
     float *delta, *reach, *shared, *bins, *folded, *partial;
     size_t bytes;
-    int64_t blocks;      // of a pass, heads apart
+    int64_t blocks;      // that leave bins, heads apart
     int parts;
 };
 
@@ -222,7 +225,7 @@ static PatchWorkspace carve(const ptv3_patch_attention_args* p)
 {
     Carver c(p->workspace);
     PatchWorkspace w = {};
-    w.blocks = (int64_t)p->n_seq * patch_tiles(p);
+    w.blocks = bin_blocks(p);
     w.parts = ceil_div(p->n_pad, 4096);
     w.delta = c.take<float>((size_t)p->heads * p->maps * p->n_pad);
     w.shared = c.take<float>((size_t)(p->n_pad - p->n) * 4 * p->channels);
@@ -268,7 +271,7 @@ static int check_sizes(const ptv3_patch_attention_args* p, const char* what)
         PTV3_REQUIRE(p->table_dtype == PTV3_DTYPE_F32 || p->table_dtype == PTV3_DTYPE_BF16, PTV3_ERR_UNSUPPORTED,
                      "%s: dtype %d of the table", what, p->table_dtype);
     }
-    PTV3_REQUIRE((int64_t)p->n_seq * patch_tiles(p) * p->heads < (1ll << 31), PTV3_ERR_UNSUPPORTED,
+    PTV3_REQUIRE((int64_t)p->n_seq * ceil_div(longest(p), 64) * p->heads < (1ll << 31), PTV3_ERR_UNSUPPORTED,
                  "%s: too many blocks (%d sequences of up to %d rows, %d heads)", what, p->n_seq, longest(p), p->heads);
     return PTV3_OK;
 }
@@ -284,7 +287,6 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
     a.n_pad = (int)p->n_pad;
     a.n_seq = p->n_seq;
     a.max_seqlen = p->max_seqlen;
-    a.tiles = patch_tiles(p);
     a.C = p->channels;
     a.H = p->heads;
     a.scale = p->scale;

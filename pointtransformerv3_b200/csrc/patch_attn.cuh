@@ -193,11 +193,11 @@ __device__ __forceinline__ void pa_store_bins(const PatchArgs& a, const PatchTab
 }
 
 enum { PA_FWD = 0, PA_ROWS = 1, PA_COLS = 2 };
-// fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu); ..._rows: rows of a block that has bins (a launch may take another
-// number where it has none, and sets `tiles`)
+// fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu): a pass queued, `tiles` set by the rows that its blocks have
 int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
-int patch_fma_rows(int width);
-int patch_mma_rows();
+// rows of a block of the pass over columns with a bias, whose blocks leave bins
+int patch_fma_cols_rows(int width);
+int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width);
 
 }  // namespace ptv3

@@ -404,11 +404,13 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 }
 
 template <int W, int MAPS, bool BIAS>
-static int launch_pass(const PatchArgs& a, int pass, cudaStream_t stream)
+static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
 {
+    PatchArgs a = args;
     const size_t table = BIAS ? PF_TABLE_BYTES : 0;
     // in the pass over columns beside the table: its bins, and their sums (of every entry, at least a copy each)
     const size_t cols = BIAS ? PF_BINS_BYTES + PF_TABLE_BYTES : 0;
+    a.tiles = ceil_div(a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad, PfShape<W, MAPS>::ROWS);
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
     auto go = [&](auto kern, size_t smem) {
         const cudaError_t e = BIAS ? allow_smem(kern) : cudaSuccess;
@@ -440,5 +442,7 @@ int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStre
 }
 
 int patch_fma_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
+
+int patch_fma_cols_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
 
 }  // namespace ptv3

@@ -234,6 +234,35 @@ __device__ __forceinline__ void pm_products(const uint32_t (&f)[RT][W / 16][4], 
     }
 }
 
+// the same for 8 rows of the tile
+template <int W, int MAPS, int RT>
+__device__ __forceinline__ void pm_products8(const uint32_t (&f)[RT][W / 16][4], uint32_t tile, int row0, float (&s)[RT][MAPS][4])
+{
+    const int lane = threadIdx.x & 31, r = row0 + (lane & 7), c = (lane >> 3) & 1;
+#pragma unroll
+    for (int x = 0; x < RT; ++x)
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[x][m][j] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W / 16; ++k) {
+        uint32_t b0, b1;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];\n"
+                     : "=r"(b0), "=r"(b1)
+                     : "r"(tile + pm_offset<W>(r, 2 * k + c)));
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            if (W / MAPS == 8) {
+                mma_bf16_k8(s[x][0], f[x][k][0], f[x][k][1], b0);
+                mma_bf16_k8(s[x][MAPS - 1], f[x][k][2], f[x][k][3], b1);
+            } else {
+                mma_bf16(s[x][k * 16 / (W / MAPS)], f[x][k], b0, b1);
+            }
+        }
+    }
+}
+
 // acc += P x 16 rows of the tile (W values each); P of map m for the values of map m, or one P for all (MAPS = 1).  With
 // `acc2` the same of P2 to that.
 template <int W, int MAPS, int RT, bool TWO = false>
@@ -844,13 +873,13 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
 #pragma unroll (2 / RT)
             for (int j0 = 0; j0 < CH; j0 += 16) {
                 if (j0 >= nq) break;
-                float s[RT][MAPS][2][4], G[RT][1][2][4];
                 uint32_t p[RT][MAPS][4], pm[RT][1][4];
-                pm_products<W, MAPS, RT>(kf, qs, j0, s);
-                pm_products<W, 1, RT>(vf, os, j0, G);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const int j = j0 + 8 * n + 2 * t;
+                    float s[RT][MAPS][4], G[RT][1][4];
+                    pm_products8<W, MAPS, RT>(kf, qs, j0 + 8 * n, s);
+                    pm_products8<W, 1, RT>(vf, os, j0 + 8 * n, G);
                     int2 g[3];
                     if (BIAS) pm_coords<CH>(gs, j, g);
                     uint64_t lse[MAPS], delta[MAPS];      // (negated as they are staged)
@@ -864,18 +893,18 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
                         uint32_t at[4][3];
                         if (BIAS) {
                             pm_places<-1, CLAMP>(bias, point[x], g, at);
-                            pm_bias(at, scale2, s[x][0][n]);
+                            pm_bias(at, scale2, s[x][0]);
                         }
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             uint64_t mix = 0;
 #pragma unroll
                             for (int k = 0; k < MAPS; ++k) {
-                                const uint64_t v = pack2(s[x][k][n][2 * r], s[x][k][n][2 * r + 1]);
+                                const uint64_t v = pack2(s[x][k][2 * r], s[x][k][2 * r + 1]);
                                 uint64_t pr = pm_exp2(BIAS ? add2(v, lse[k]) : fma2(v, pm_both(scale2), lse[k]));
                                 if (k == 1) pr = mul2(pr, pm_both(minus_lam));
                                 mix = k == 0 ? pr : add2(mix, pr);
-                                const uint64_t ds = mul2(pr, add2(pack2(G[x][0][n][2 * r], G[x][0][n][2 * r + 1]), delta[k]));
+                                const uint64_t ds = mul2(pr, add2(pack2(G[x][0][2 * r], G[x][0][2 * r + 1]), delta[k]));
                                 float y, z;
                                 unpack2(ds, y, z);
                                 p[x][k][2 * n + r] = pack_bf16(y, z);
@@ -943,13 +972,17 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 }
 
 // Rows of a block, in tiles of 128: with two tiles to a warp what it reads of the other side serves twice the rows, where
-// registers allow it (heads of 16) and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and 397;
-// columns of the differential backward, 100 000 x 64, 347 and 321.  Not so forward without a bias (312, 326), rows (341, 465; with a
-// bias 464, 455) and columns with a bias (882, 891), and forward with a bias of 6 760 x 128 (64, 65).
+// registers allow it (heads of 16) and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and
+// 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of two maps 347 and 320.  Not so forward and rows
+// without a bias (312 and 326, 341 and 465).
 static int row_tiles(int64_t n_seq, int64_t longest, int heads, int width, int maps, bool bias, int pass)
 {
     const int64_t blocks = n_seq * heads * ((longest + 2 * PM_ROWS - 1) / (2 * PM_ROWS));
-    return width == 16 && blocks >= 2 * SMS && (bias ? pass == PA_FWD : maps == 2 && pass == PA_COLS) ? 2 : 1;
+    return width == 16 && blocks >= 2 * SMS && (bias || (maps == 2 && pass == PA_COLS)) ? 2 : 1;
+}
+int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width)
+{
+    return PM_ROWS * row_tiles(n_seq, longest, heads, width, 1, true, PA_COLS);
 }
 
 template <int W, int MAPS, bool BIAS>
@@ -959,18 +992,20 @@ static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
     const int longest = a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad;
     const int rt = row_tiles(a.n_seq, longest, a.H, W, MAPS, BIAS, pass);
     a.tiles = ceil_div(longest, rt * PM_ROWS);
-    constexpr int FWD2 = W == 16 && BIAS ? 2 : 1, COLS2 = W == 16 && MAPS == 2 ? 2 : 1;
+    constexpr int TWO = W == 16 && BIAS ? 2 : 1, COLS2 = W == 16 && (MAPS == 2 || BIAS) ? 2 : 1;
     const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES, smem = stages + (BIAS ? PA_TABLE_BYTES : 0);
-    if (pass == PA_ROWS) return launch(patch_mma_rows_kernel<W, MAPS, BIAS, 1>, a, smem, stream);
+    if (pass == PA_ROWS)
+        return rt == 2 ? launch(patch_mma_rows_kernel<W, MAPS, BIAS, TWO>, a, smem, stream)
+                       : launch(patch_mma_rows_kernel<W, MAPS, BIAS, 1>, a, smem, stream);
     if (pass == PA_COLS) {      // the table, its bins, and their sums
         const size_t with_bins = stages + (BIAS ? PA_BINS_BYTES + pm_sums_bytes(a.bnd) : 0);
         return rt == 2 ? launch(patch_mma_cols_kernel<W, MAPS, BIAS, COLS2>, a, with_bins, stream)
                        : launch(patch_mma_cols_kernel<W, MAPS, BIAS, 1>, a, with_bins, stream);
     }
     if (a.lse)
-        return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, FWD2>, a, smem, stream)
+        return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, TWO>, a, smem, stream)
                        : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, 1>, a, smem, stream);
-    return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, FWD2>, a, smem, stream)
+    return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, TWO>, a, smem, stream)
                    : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, 1>, a, smem, stream);
 }
 
@@ -989,7 +1024,5 @@ int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStre
         default: return launch_form<64>(a, maps, pass, stream);
     }
 }
-
-int patch_mma_rows() { return PM_ROWS; }
 
 }  // namespace ptv3

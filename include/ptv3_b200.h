@@ -197,13 +197,14 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
  * follow one another from row 0 to n_pad and are no longer than max_seqlen.  What a bias reads is looked at too, where given:
  * `grid_coord` (n x 3 int32) within 2^22 of zero, `buckets` (2 pos_bnd + 1 int32) in [0, num_buckets).
  *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30
+ *   backward    not zero: for a backward pass too (what ptv3_patch_attention_bwd reads of `rows` is written)
  *   rows        2 * n_pad + (n_pad - n) + 1 + 3 * n_seq int32, written
  *   status      one uint32 or NULL: PTV3_STATUS_BAD_INDEX where something does not hold (the calls that read `rows` then
  *               stay within their tensors, and what they leave is undefined)
  */
 int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
                     int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord,
-                    const int32_t* buckets, int pos_bnd, int num_buckets, int32_t* rows, uint32_t* status,
+                    const int32_t* buckets, int pos_bnd, int num_buckets, int backward, int32_t* rows, uint32_t* status,
                     void* stream);
 
 /*

@@ -4,6 +4,7 @@ There is no fallback: if the shared library is missing or a call fails, an
 exception is raised."""
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -67,16 +68,11 @@ class BackboneArgs(ctypes.Structure):
            ("stem_bn", c_ptr), ("plain_weights", c_int)])
 
 
-class PatchAttentionArgs(ctypes.Structure):
-    """ptv3_patch_attention_args of include/ptv3_b200.h (same field order)."""
-    _fields_ = (
-        [("n", c_i64), ("n_pad", c_i64)]
-        + [(name, c_int) for name in ("n_seq", "max_seqlen", "channels", "heads", "maps", "dtype")]
-        + [("scale", c_f32)]
-        + [(name, c_int) for name in ("pos_bnd", "num_buckets", "table_dtype", "lam_dtype")]
-        + [(name, c_ptr) for name in ("qkv", "rows", "cu_seqlens", "grid_coord", "buckets", "table", "lam", "out", "lse",
-                                      "second", "dout", "dqkv", "dtable", "dlam", "workspace")]
-        + [("workspace_bytes", c_sz)])
+# ptv3_patch_attention_args of include/ptv3_b200.h (same field order, native alignment): n, n_pad; n_seq, max_seqlen,
+# channels, heads, maps, dtype; scale; pos_bnd, num_buckets, table_dtype, lam_dtype; qkv, rows, cu_seqlens, grid_coord,
+# buckets, table, lam, out, lse, second, dout, dqkv, dtable, dlam, workspace; workspace_bytes.  Packed in one go: filling
+# a ctypes structure field by field costs as much as two launches.
+PATCH_ATTENTION_ARGS = struct.Struct("@qq6if4i15PN")
 
 
 # name -> (restype, argtypes); must list every symbol of include/ptv3_b200.h
@@ -94,10 +90,10 @@ SIGNATURES = {
     "ptv3_attention_rpe_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_i64, c_int,
                                        c_int, c_int, c_int, c_f32, c_int, c_ptr]),
     "ptv3_patch_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr, c_int, c_int,
-                                c_ptr, c_ptr, c_ptr]),
-    "ptv3_patch_attention_fwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),
-    "ptv3_patch_attention_workspace_bytes": (c_sz, [ctypes.POINTER(PatchAttentionArgs)]),
-    "ptv3_patch_attention_bwd": (c_int, [ctypes.POINTER(PatchAttentionArgs), c_ptr]),
+                                c_int, c_ptr, c_ptr, c_ptr]),
+    "ptv3_patch_attention_fwd": (c_int, [c_ptr, c_ptr]),
+    "ptv3_patch_attention_workspace_bytes": (c_sz, [c_ptr]),
+    "ptv3_patch_attention_bwd": (c_int, [c_ptr, c_ptr]),
     "ptv3_qk_norm_rope_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_i64, c_int, c_int, c_f32, c_f64,
                                       c_int, c_ptr]),
     "ptv3_qk_norm_rope_workspace_bytes": (c_sz, [c_i64, c_int, c_int]),

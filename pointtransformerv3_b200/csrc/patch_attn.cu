@@ -9,80 +9,45 @@ namespace ptv3 {
 // Points are looked up once (rows[P] = order[pad[P]], or -1 - that where unpad[pad[P]] != P: the row was borrowed by
 // another patch and answers for nothing), so that the attention kernels load one word per row and not three in a chain.
 // Keys and values of a borrowed row have a gradient all the same, and a point has at most one such row beside its
-// own: both get a row of the backward pass's side buffer (slots 2 i and 2 i + 1).
-__global__ void __launch_bounds__(256) patch_rows_kernel(const int64_t* order, const int64_t* pad, const int64_t* unpad,
-                                                         const int32_t* cu, int n, int n_pad, int n_seq, int max_seqlen,
-                                                         const int32_t* grid, const int32_t* buckets, int n_entries, int num,
-                                                         int32_t* rows,
-                                                         int32_t* slot, int32_t* slot_point, int32_t* taken,
-                                                         uint32_t* status)
-{
-    bool bad = false;
-    const int n_slots = n_pad - n;
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < max(max(n_pad, n_seq + 1), n_entries);
-         i += gridDim.x * blockDim.x) {
-        if (i < n_pad) {
-            const int64_t pd = pad[i];
-            const bool in = pd >= 0 && pd < n;
-            const int64_t p = in ? order[pd] : -1, own = in ? unpad[pd] : -1;
-            const bool good = p >= 0 && p < n && own >= 0 && own < n_pad;
-            bad |= !good;
-            int32_t row = -1;
-            if (good) {
-                row = own == i ? (int32_t)p : -1 - (int32_t)p;
-                if (own != i && n_slots == 0) {
-                    bad = true;
-                } else if (own != i) {
-                    const int s = atomicAdd(taken, 1);
-                    bad |= pad[own] != pd || s >= n_slots;
-                    if (pad[own] == pd && s < n_slots) {
-                        slot[i] = 2 * s + 1;
-                        // (a point with two borrowed rows has no place for the second)
-                        bad |= atomicCAS(slot + own, -1, 2 * s) != -1;
-                        slot_point[s] = (int32_t)p;
-                    }
-                }
-            }
-            rows[i] = row;
-        }
-        // every point has one row that answers for it
-        if (i < n) {
-            bad |= unpad[i] < 0 || unpad[i] >= n_pad || pad[unpad[i]] != i;
-            if (grid)
-                for (int c = 0; c < 3; ++c) bad |= grid[3 * (int64_t)i + c] < -PA_MAX_COORD || grid[3 * (int64_t)i + c] > PA_MAX_COORD;
-        }
-        if (i < n_seq) bad |= cu[i] < 0 || cu[i + 1] < cu[i] || cu[i + 1] - cu[i] > max_seqlen || (i == 0 && cu[0] != 0);
-        if (i == n_seq) bad |= cu[n_seq] != n_pad;
-        if (i < n_entries) bad |= buckets[i] < 0 || buckets[i] >= num;
-    }
-    if (bad && status) atomicOr(status, PTV3_STATUS_BAD_INDEX);
-}
+// own: for a backward pass both get a row of its side buffer (slots 2 i and 2 i + 1; `slot` comes in filled with -1, and so
+// does the counter behind it).  With a bias the first blocks take a sequence each, and find the largest offset of two of its
+// points along each axis.
+// (Only this kernel lets the one behind it start early: blocks of the attention kernels that come while others of their kind
+// run are placed where there is room at that time, not evenly; 12 000 x 32 in fp32, all three passes: 208 us, 255 so.)
+struct PatchPlan {
+    const int64_t *order, *pad, *unpad;
+    const int32_t *cu, *grid, *buckets;
+    int n, n_pad, n_seq, max_seqlen, n_entries, num, n_extents;
+    int32_t *rows, *slot, *extent;      // slot: n_pad, then a point for each of n_pad - n, then the counter; or NULL
+    uint32_t* status;
+};
 
-// Largest offset of two points of a sequence along each axis: a block per sequence
-__global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, const int32_t* cu, const int32_t* grid, int n_pad,
-                                                           int max_seqlen, int32_t* extent)
+__device__ __forceinline__ void patch_extent(const PatchPlan& p, int seq)
 {
-    __shared__ int lo_s[4][3], hi_s[4][3];
+    __shared__ int lo_s[8][3], hi_s[8][3];
+    int lo[3], hi[3];
     PatchArgs a = {};
-    a.rows = rows;
-    a.cu = cu;
-    a.n_pad = n_pad;
-    a.max_seqlen = max_seqlen;
-    a.grid = grid;
-    int start, lo[3], hi[3];
-    const int L = pa_sequence(a, blockIdx.x, start);
+    a.cu = p.cu;
+    a.grid = p.grid;
+    a.n_pad = p.n_pad;
+    a.max_seqlen = p.max_seqlen;
+    int start;
+    const int L = pa_sequence(a, seq, start);
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
         lo[c] = PA_MAX_COORD;
         hi[c] = -PA_MAX_COORD;
     }
 #pragma unroll 4
-    for (int i = threadIdx.x; i < L; i += 128) {
-        const int e = rows[start + i];
-        const int64_t p = e >= 0 ? e : -(e + 1);
+    for (int i = threadIdx.x; i < L; i += 256) {
+        const int64_t pd = p.pad[start + i];
+        int64_t e = pd >= 0 && pd < p.n ? p.order[pd] : 0;
+        if (e < 0 || e >= p.n || p.unpad[pd >= 0 && pd < p.n ? pd : 0] < 0 ||
+            p.unpad[pd >= 0 && pd < p.n ? pd : 0] >= p.n_pad)
+            e = 0;                               // (what such a row is taken as: point 0)
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-            const int v = pa_coord(a, p, c);
+            const int v = pa_coord(a, e, c);
             lo[c] = min(lo[c], v);
             hi[c] = max(hi[c], v);
         }
@@ -99,12 +64,63 @@ __global__ void __launch_bounds__(128) patch_extent_kernel(const int32_t* rows, 
     __syncthreads();
     if (threadIdx.x < 3) {
         int l = lo_s[0][threadIdx.x], h = hi_s[0][threadIdx.x];
-        for (int w = 1; w < 4; ++w) {
+        for (int w = 1; w < 8; ++w) {
             l = min(l, lo_s[w][threadIdx.x]);
             h = max(h, hi_s[w][threadIdx.x]);
         }
-        extent[3 * blockIdx.x + threadIdx.x] = max(h - l, 0);
+        p.extent[3 * seq + threadIdx.x] = max(h - l, 0);
     }
+}
+
+__global__ void __launch_bounds__(256) patch_rows_kernel(const PatchPlan p)
+{
+    pdl_launch_next();
+    pdl_wait();
+    if ((int)blockIdx.x < p.n_extents) {
+        patch_extent(p, blockIdx.x);
+        return;
+    }
+    bool bad = false;
+    const int n_slots = p.n_pad - p.n;
+    int32_t *slot_point = p.slot + p.n_pad, *taken = slot_point + n_slots;
+    const int most = max(max(p.n_pad, p.n_seq + 1), p.n_entries);
+    for (int i = ((int)blockIdx.x - p.n_extents) * 256 + (int)threadIdx.x; i < most;
+         i += ((int)gridDim.x - p.n_extents) * 256) {
+        if (i < p.n_pad) {
+            const int64_t pd = p.pad[i];
+            const bool in = pd >= 0 && pd < p.n;
+            const int64_t e = in ? p.order[pd] : -1, own = in ? p.unpad[pd] : -1;
+            const bool good = e >= 0 && e < p.n && own >= 0 && own < p.n_pad;
+            bad |= !good;
+            if (good && own != i) {
+                const bool right = n_slots > 0 && p.pad[own] == pd;
+                bad |= !right;
+                if (right && p.slot) {
+                    const int s = atomicAdd(taken, 1) + 1;
+                    bad |= s >= n_slots;
+                    if (s < n_slots) {
+                        p.slot[i] = 2 * s + 1;
+                        // (a point with two borrowed rows has no place for the second)
+                        bad |= atomicCAS(p.slot + own, -1, 2 * s) != -1;
+                        slot_point[s] = (int32_t)e;
+                    }
+                }
+            }
+            p.rows[i] = !good ? -1 : own == i ? (int32_t)e : -1 - (int32_t)e;
+        }
+        if (i < p.n) {
+            // every point has one row that answers for it
+            bad |= p.unpad[i] < 0 || p.unpad[i] >= p.n_pad || p.pad[p.unpad[i]] != i;
+            if (p.grid)
+                for (int c = 0; c < 3; ++c)
+                    bad |= p.grid[3 * (int64_t)i + c] < -PA_MAX_COORD || p.grid[3 * (int64_t)i + c] > PA_MAX_COORD;
+        }
+        if (i < p.n_seq)
+            bad |= p.cu[i] < 0 || p.cu[i + 1] < p.cu[i] || p.cu[i + 1] - p.cu[i] > p.max_seqlen || (i == 0 && p.cu[0] != 0);
+        if (i == p.n_seq) bad |= p.cu[p.n_seq] != p.n_pad;
+        if (i < p.n_entries) bad |= p.buckets[i] < 0 || p.buckets[i] >= p.num;
+    }
+    if (bad && p.status) atomicOr(p.status, PTV3_STATUS_BAD_INDEX);
 }
 
 // ---- gradients of keys and values with a borrowed copy ------------------------------------------------------
@@ -117,6 +133,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) patch_shared_kernel(const float* shared, const int32_t* slot_point, int n_slots, int C,
                                                            T* dqkv)
 {
+    pdl_wait();
     const int64_t total = (int64_t)n_slots * 2 * C;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t s = i / (2 * C), c = i % (2 * C);
@@ -131,6 +148,7 @@ constexpr int PA_FOLD = 64;      // rows added by a block of the first step
 // out[block][i] = sum of PA_FOLD rows of in
 __global__ void __launch_bounds__(256) patch_fold_kernel(const float* in, int64_t rows, int width, float* out)
 {
+    pdl_wait();
     const int64_t first = (int64_t)blockIdx.x * PA_FOLD;
     const int count = (int)min((int64_t)PA_FOLD, rows - first);
     const int i = blockIdx.y * 256 + threadIdx.x;
@@ -145,6 +163,7 @@ __global__ void __launch_bounds__(256) patch_fold_kernel(const float* in, int64_
 __global__ void __launch_bounds__(256) patch_table_kernel(const float* in, int64_t rows, int H, int bnd, int num,
                                                           const int32_t* buckets, void* dtable, int bf16)
 {
+    pdl_wait();
     __shared__ float sum[2 * PA_MAX_BOUND + 1];
     __shared__ int bucket[2 * PA_MAX_BOUND + 1];
     const int axis = blockIdx.x, h = blockIdx.y, ne = 2 * bnd + 1;
@@ -167,18 +186,21 @@ __global__ void __launch_bounds__(256) patch_table_kernel(const float* in, int64
     }
 }
 
-// -sum of delta_2 over all rows, a head per block row; `parts` blocks leave partial sums, one block adds them
-__global__ void __launch_bounds__(256) patch_lam_kernel(const float* delta, int n_pad, int H, int parts, float* partial,
-                                                        void* dlam, int bf16)
+// -sum of delta_2 over all rows, a head per block row: `parts` blocks leave partial sums, a block of a second launch
+// adds them (the result in place of them); with one part that one launch does it all
+__global__ void __launch_bounds__(256) patch_lam_kernel(const float* delta, int n_pad, int parts, float* partial, void* dlam,
+                                                        int bf16)
 {
+    pdl_wait();
     __shared__ float warp_sum[8];
     const int h = blockIdx.y;
     float v = 0.f;
-    if (dlam) {
-        for (int i = threadIdx.x; i < parts; i += 256) v -= partial[h * parts + i];
+    if (dlam && parts > 1) {
+        for (int i = threadIdx.x; i < parts; i += 256) v += partial[h * parts + i];
     } else {
         const float* row = delta + (int64_t)(2 * h + 1) * n_pad;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n_pad; i += (int64_t)parts * 256) v += row[i];
+#pragma unroll 4
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n_pad; i += (int64_t)parts * 256) v -= row[i];
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -226,14 +248,14 @@ static PatchWorkspace carve(const ptv3_patch_attention_args* p)
     Carver c(p->workspace);
     PatchWorkspace w = {};
     w.blocks = bin_blocks(p);
-    w.parts = ceil_div(p->n_pad, 4096);
+    w.parts = p->n_pad > 16384 ? ceil_div(p->n_pad, 4096) : 1;
     w.delta = c.take<float>((size_t)p->heads * p->maps * p->n_pad);
     w.shared = c.take<float>((size_t)(p->n_pad - p->n) * 4 * p->channels);
     if (p->dtable) {
         w.reach = c.take<float>((size_t)p->heads * p->n_pad);
         const size_t width = (size_t)p->heads * 3 * (2 * p->pos_bnd + 1);
         w.bins = c.take<float>((size_t)w.blocks * width);
-        w.folded = c.take<float>((size_t)ceil_div(w.blocks, PA_FOLD) * width);
+        w.folded = c.take<float>(w.blocks > PA_FOLD ? (size_t)ceil_div(w.blocks, PA_FOLD) * width : 0);
     }
     if (p->dlam) w.partial = c.take<float>((size_t)p->heads * w.parts);
     w.bytes = c.off;
@@ -309,8 +331,9 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
 using namespace ptv3;
 
 extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
-                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord, const int32_t* buckets, int pos_bnd,
-                               int num_buckets, int32_t* rows, uint32_t* status, void* stream)
+                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord,
+                               const int32_t* buckets, int pos_bnd, int num_buckets, int backward, int32_t* rows,
+                               uint32_t* status, void* stream)
 {
     PTV3_REQUIRE(n >= 0 && n_pad >= n && n_seq >= 0 && max_seqlen >= 1 && n_pad < (1ll << 30) && n_seq < (1 << 30),
                  PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: bad sizes");
@@ -319,24 +342,17 @@ extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const i
     PTV3_REQUIRE(n_pad <= 2 * n, PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: %lld rows of %lld points", (long long)n_pad,
                  (long long)n);
     const int borrowed = (int)(n_pad - n);
-    int32_t *slot = rows + n_pad, *slot_point = slot + n_pad, *taken = slot_point + borrowed;
-    if (borrowed) {
-        // slots and their points -1, the counter 0
-        cudaError_t e = cudaMemsetAsync(slot, 0xff, (size_t)(n_pad + borrowed) * 4, (cudaStream_t)stream);
-        if (e == cudaSuccess) e = cudaMemsetAsync(taken, 0, 4, (cudaStream_t)stream);
+    PatchPlan p = {order, pad, unpad, cu_seqlens, grid_coord, buckets, (int)n, (int)n_pad, n_seq, max_seqlen,
+                   buckets ? 2 * pos_bnd + 1 : 0, num_buckets, grid_coord ? n_seq : 0, rows,
+                   backward && borrowed ? rows + n_pad : nullptr, rows + 2 * n_pad + borrowed + 1, status};
+    if (p.slot) {
+        const cudaError_t e = cudaMemsetAsync(p.slot, 0xff, (size_t)(n_pad + borrowed + 1) * 4, (cudaStream_t)stream);
         PTV3_REQUIRE(e == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_rows: %s", cudaGetErrorString(e));
     }
-    const int entries = buckets ? 2 * pos_bnd + 1 : 0;
     const int64_t most = n_pad > n_seq + 1 ? n_pad : n_seq + 1;
-    patch_rows_kernel<<<ceil_div(most, 256), 256, 0, (cudaStream_t)stream>>>(
-        order, pad, unpad, cu_seqlens, (int)n, (int)n_pad, n_seq, max_seqlen, grid_coord, buckets, entries, num_buckets, rows, slot,
-        slot_point, taken, status);
+    launch_dependent(patch_rows_kernel, dim3((unsigned)(p.n_extents + ceil_div(most, 256))), dim3(256), 0,
+                     (cudaStream_t)stream, p);
     count_launches(1);
-    if (grid_coord && n_seq > 0) {
-        patch_extent_kernel<<<n_seq, 128, 0, (cudaStream_t)stream>>>(rows, cu_seqlens, grid_coord, (int)n_pad, max_seqlen,
-                                                                      taken + 1);
-        count_launches(1);
-    }
     return check_launch("ptv3_patch_rows");
 }
 
@@ -396,30 +412,37 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
         const int64_t total = (int64_t)borrowed * 2 * a.C;
         const int blocks = (int)(total > 256ll * 8 * SMS * 16 ? 8 * SMS * 16 : ceil_div(total, 256));
         if (p->dtype == PTV3_DTYPE_F32)
-            patch_shared_kernel<float><<<blocks, 256, 0, s>>>(w.shared, slot_point, borrowed, a.C, (float*)p->dqkv);
+            launch_dependent(patch_shared_kernel<float>, dim3(blocks), dim3(256), 0, s, w.shared, slot_point, borrowed, a.C,
+                             (float*)p->dqkv);
         else
-            patch_shared_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(w.shared, slot_point, borrowed, a.C,
-                                                                       (__nv_bfloat16*)p->dqkv);
+            launch_dependent(patch_shared_kernel<__nv_bfloat16>, dim3(blocks), dim3(256), 0, s, w.shared, slot_point, borrowed,
+                             a.C, (__nv_bfloat16*)p->dqkv);
         count_launches(1);
     }
     if (p->dtable) {
-        const int64_t rows = any ? w.blocks : 0;
-        const int wide = a.H * 3 * (2 * a.bnd + 1), folded = any ? ceil_div(rows, PA_FOLD) : 0;
-        if (folded) {
-            patch_fold_kernel<<<dim3(folded, ceil_div(wide, 256)), 256, 0, s>>>(w.bins, rows, wide, w.folded);
+        const int wide = a.H * 3 * (2 * a.bnd + 1);
+        const float* sums = w.bins;
+        int64_t rows = any ? w.blocks : 0;
+        if (rows > PA_FOLD) {
+            const int folded = ceil_div(rows, PA_FOLD);
+            launch_dependent(patch_fold_kernel, dim3(folded, ceil_div(wide, 256)), dim3(256), 0, s, w.bins, rows, wide, w.folded);
             count_launches(1);
+            sums = w.folded;
+            rows = folded;
         }
-        patch_table_kernel<<<dim3(3, a.H), 256, 0, s>>>(w.folded, folded, a.H, a.bnd, a.num, a.buckets, p->dtable,
-                                                        a.table_bf16);
+        launch_dependent(patch_table_kernel, dim3(3, a.H), dim3(256), 0, s, sums, rows, a.H, a.bnd, a.num, a.buckets,
+                         p->dtable, a.table_bf16);
         count_launches(1);
     }
     if (p->dlam) {
-        const int parts = any ? w.parts : 0;
-        if (parts) {
-            patch_lam_kernel<<<dim3(parts, a.H), 256, 0, s>>>(w.delta, a.n_pad, a.H, parts, w.partial, nullptr, 0);
+        // short launches in one step
+        if (any && w.parts > 1) {
+            launch_dependent(patch_lam_kernel, dim3(w.parts, a.H), dim3(256), 0, s, w.delta, a.n_pad, w.parts, w.partial,
+                             nullptr, 0);
             count_launches(1);
         }
-        patch_lam_kernel<<<dim3(1, a.H), 256, 0, s>>>(w.delta, a.n_pad, a.H, parts, w.partial, p->dlam, a.lam_bf16);
+        launch_dependent(patch_lam_kernel, dim3(1, a.H), dim3(256), 0, s, w.delta, any ? a.n_pad : 0, w.parts, w.partial,
+                         p->dlam, a.lam_bf16);
         count_launches(1);
     }
     return check_launch("ptv3_patch_attention_bwd");

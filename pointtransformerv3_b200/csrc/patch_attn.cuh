@@ -84,17 +84,17 @@ __device__ __forceinline__ float pa_param(const void* p, int i, int bf16)
 // This head's table in shared memory, in powers of two, of the offsets that occur in a sequence: axis a holds offsets
 // -reach[a] .. reach[a], entry e of it at (first[a] + e) copies + copy.  A lane reads the copy of its number: with 32
 // copies, which most patches leave room for, look-ups of a warp never meet in a bank.  Offsets beyond the bound repeat its
-// outermost entries, as long as that leaves room for eight copies: no look-up then has to be clamped.  With `bins`, there
+// outermost entries (`far`), as long as that leaves room for eight copies: no look-up then has to be clamped.  With `bins`, there
 // are as many copies of the bins, or half.
 struct PatchTable {
     int reach[3], first[3], entries, copies_log2, bins_log2;
     bool clamps;
 };
-__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int bytes, bool bins, int most_log2 = 5)
+__device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int bytes, bool bins, bool far = true, int bins_most = 5)
 {
     PatchTable t;
     t.clamps = false;
-    for (int k = 0; k < 2; ++k) {
+    for (int k = far ? 0 : 1; k < 2; ++k) {
         t.entries = 0;
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
@@ -106,8 +106,9 @@ __device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int 
         if (t.entries <= bytes >> (bins ? 6 : 5)) break;
         t.clamps = true;
     }
-    t.copies_log2 = t.bins_log2 = most_log2;
-    while (t.bins_log2 > 0 && 4 * ((t.entries << t.copies_log2) + (bins ? t.entries << t.bins_log2 : 0)) > bytes) {
+    t.copies_log2 = 5;
+    t.bins_log2 = bins ? bins_most : 5;
+    while (t.copies_log2 > 0 && 4 * ((t.entries << t.copies_log2) + (bins ? t.entries << t.bins_log2 : 0)) > bytes) {
         if (bins && t.bins_log2 == t.copies_log2) --t.bins_log2;
         else t.copies_log2 = t.bins_log2 = bins ? t.bins_log2 : t.bins_log2 - 1;
     }

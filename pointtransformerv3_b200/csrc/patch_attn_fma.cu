@@ -11,8 +11,8 @@ constexpr int PF_THREADS = 128;
 constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
 constexpr int PF_STEP = 8;        // of which scores are held at a time
 constexpr int PF_WINDOW = 32;     // queries between two clearings of the bins: the unit is that much finer
-constexpr int PF_COPIES_LOG2 = 4; // few copies of them, so that clearing costs little
-constexpr int PF_TABLE_BYTES = 22 * 1024, PF_BINS_BYTES = 2 * PF_TABLE_BYTES;
+constexpr int PF_BINS_LOG2 = 4;   // 16 copies of them, so that clearing costs little
+constexpr int PF_TABLE_BYTES = 32 * 1024, PF_BINS_BYTES = 48 * 1024;      // for the table; for the table and its bins
 
 template <int W, int MAPS>
 struct PfShape {
@@ -86,6 +86,7 @@ __device__ __forceinline__ float pf_dot(const float (&x)[PfShape<W, MAPS>::WP], 
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchArgs a)
 {
+    pdl_wait();
     using S = PfShape<W, MAPS>;
     __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, false, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchArgs a)
 {
+    pdl_wait();
     using S = PfShape<W, MAPS>;
     __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     if (q0 >= L) return;
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, false, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -280,6 +282,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchArgs a)
 {
+    pdl_wait();
     using S = PfShape<W, MAPS>;
     __shared__ float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     }
     PatchTable table = {};
     if (BIAS) {
-        table = pa_table(a, seq, PF_BINS_BYTES, true, PF_COPIES_LOG2);
+        table = pa_table(a, seq, PF_BINS_BYTES, true, false, PF_BINS_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
     }
     const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
@@ -407,15 +410,15 @@ template <int W, int MAPS, bool BIAS>
 static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
 {
     PatchArgs a = args;
-    const size_t table = BIAS ? PF_TABLE_BYTES : 0;
-    // in the pass over columns beside the table: its bins, and their sums (of every entry, at least a copy each)
-    const size_t cols = BIAS ? PF_BINS_BYTES + PF_TABLE_BYTES : 0;
+    // the table; in the pass over columns the table, its bins and their sums
+    const size_t entries = BIAS ? 3 * (2 * a.bnd + 1) : 0, full = entries * 32 * 4, both = full + full / 2;
+    const size_t table = full < PF_TABLE_BYTES ? full : PF_TABLE_BYTES;
+    const size_t cols = (both < PF_BINS_BYTES ? both : PF_BINS_BYTES) + entries * 4;
     a.tiles = ceil_div(a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad, PfShape<W, MAPS>::ROWS);
     const unsigned grid = (unsigned)((int64_t)a.n_seq * a.tiles * a.H);
     auto go = [&](auto kern, size_t smem) {
         const cudaError_t e = BIAS ? allow_smem(kern) : cudaSuccess;
-        if (e == cudaSuccess) kern<<<grid, PF_THREADS, smem, stream>>>(a);
-        return e;
+        return e == cudaSuccess ? launch_dependent(kern, dim3(grid), dim3(PF_THREADS), smem, stream, a) : e;
     };
     const cudaError_t err = pass == PA_FWD    ? go(patch_fma_fwd_kernel<W, MAPS, BIAS>, table)
                             : pass == PA_ROWS ? go(patch_fma_rows_kernel<W, MAPS, BIAS>, table)

@@ -411,6 +411,7 @@ __device__ __forceinline__ void pm_own_rows(const PmOwn<RT>& own, const __nv_bfl
 template <int W, int MAPS, bool BIAS, bool KEEP, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patch_mma_fwd_kernel(const PatchArgs a)
 {
+    pdl_wait();
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -420,6 +421,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     const int t = threadIdx.x & 3;
     PmOwn<RT> own;
     own.load(a, w, q0);
+    if (!__syncthreads_or(own.any)) return;         // (a scene's last patch may end in borrowed rows alone)
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
@@ -617,6 +619,7 @@ __device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], cons
 template <int W, int MAPS, bool BIAS, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_kernel(const PatchArgs a)
 {
+    pdl_wait();
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -786,6 +789,7 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
 template <int W, int MAPS, bool BIAS, int RT>
 __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_kernel(const PatchArgs a)
 {
+    pdl_wait();
     constexpr int CH = PmChunk<W, BIAS>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -966,7 +970,7 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 {
     const cudaError_t err = allow_smem(kern);
     PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
-    kern<<<(unsigned)((int64_t)a.n_seq * a.tiles * a.H), PM_THREADS, smem, stream>>>(a);
+    launch_dependent(kern, dim3((unsigned)((int64_t)a.n_seq * a.tiles * a.H)), dim3(PM_THREADS), smem, stream, a);
     count_launches(1);
     return check_launch("ptv3_patch_attention");
 }

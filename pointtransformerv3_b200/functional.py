@@ -120,7 +120,7 @@ def qk_norm_rope(qkv, heads, grid_coord=None, q_weight=None, k_weight=None, eps=
 def _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, keep):
     order, pad, unpad, cu = geometry
     grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
-    rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, status)
+    rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, keep, status)
     return (rows,) + ops.patch_attention_fwd(qkv, rows, pad.shape[0], cu, heads, max_seqlen, scale, maps, param, grid,
                                              buckets, pos_bnd, num, want_lse=keep)
 

@@ -242,44 +242,45 @@ def qk_norm_rope_bwd(qkv, dout, heads, grid, q_weight, k_weight, eps, base):
 
 
 def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, grid=None, buckets=None, pos_bnd=0, num_buckets=0,
-               status=None):
+               backward=False, status=None):
     """Points of the padded rows of a plan as patch_attention_fwd / _bwd read them (see ptv3_patch_rows)."""
     _lib.require_cuda(order_row, pad, unpad, cu_seqlens, grid, buckets, status)
-    n, n_pad = order_row.numel(), pad.numel()
-    rows = torch.empty(2 * n_pad + (n_pad - n) + 1 + 3 * (cu_seqlens.numel() - 1), dtype=torch.int32, device=pad.device)
-    _lib.check(_lib.load().ptv3_patch_rows(_lib.ptr(order_row), _lib.ptr(pad), _lib.ptr(unpad), _lib.ptr(cu_seqlens), n,
-                                           n_pad, cu_seqlens.numel() - 1, int(max_seqlen), _lib.ptr(grid),
-                                           _lib.ptr(buckets), int(pos_bnd), int(num_buckets), _lib.ptr(rows),
-                                           _lib.ptr(status), _lib.stream()), "ptv3_patch_rows")
+    n, n_pad, n_seq = order_row.shape[0], pad.shape[0], cu_seqlens.shape[0] - 1
+    rows = torch.empty(3 * n_pad - n + 1 + 3 * n_seq, dtype=torch.int32, device=pad.device)
+    ptr = _lib.ptr
+    _lib.check(_lib.load().ptv3_patch_rows(order_row.data_ptr(), pad.data_ptr(), unpad.data_ptr(), cu_seqlens.data_ptr(), n,
+                                           n_pad, n_seq, max_seqlen, ptr(grid), ptr(buckets), pos_bnd, num_buckets, backward,
+                                           rows.data_ptr(), ptr(status), _lib.stream()), "ptv3_patch_rows")
     return rows
 
 
-def _patch_attention_args(qkv, rows, n_pad, cu, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num):
-    a = _lib.PatchAttentionArgs()
-    a.n, a.n_pad, a.n_seq, a.max_seqlen = qkv.shape[0], n_pad, cu.numel() - 1, max_seqlen
-    a.channels, a.heads, a.maps, a.dtype, a.scale = qkv.shape[1] // 3, heads, maps, _lib.dtype_id(qkv), scale
-    a.qkv, a.rows, a.cu_seqlens = qkv.data_ptr(), rows.data_ptr(), cu.data_ptr()
-    if maps == 2:
-        a.lam, a.lam_dtype = param.data_ptr(), _lib.dtype_id(param)
-    elif param is not None:
-        a.table, a.table_dtype, a.grid_coord = param.data_ptr(), _lib.dtype_id(param), grid.data_ptr()
-        a.pos_bnd, a.num_buckets, a.buckets = pos_bnd, num, _lib.ptr(buckets)
-    return a
+def _patch_attention_args(qkv, rows, n_pad, cu, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,
+                          out, lse, second, dout=None, dqkv=None, dparam=None, workspace=None):
+    """The packed ptv3_patch_attention_args of a call; param and dparam: the table's or lam's."""
+    def ptr(t):
+        return 0 if t is None else t.data_ptr()
+    kind = 0 if param is None else _lib.dtype_id(param)
+    table, dtable, lam, dlam = (ptr(param), ptr(dparam), 0, 0) if maps == 1 else (0, 0, ptr(param), ptr(dparam))
+    return _lib.PATCH_ATTENTION_ARGS.pack(
+        qkv.shape[0], n_pad, cu.shape[0] - 1, max_seqlen, qkv.shape[1] // 3, heads, maps, _lib.dtype_id(qkv), scale, pos_bnd,
+        num, kind, kind, qkv.data_ptr(), rows.data_ptr(), cu.data_ptr(), ptr(grid), ptr(buckets), table, lam, out.data_ptr(),
+        ptr(lse), ptr(second), ptr(dout), ptr(dqkv), dtable, dlam, ptr(workspace),
+        0 if workspace is None else workspace.numel())
 
 
 def patch_attention_fwd(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps=1, param=None, grid=None,
                         buckets=None, pos_bnd=0, num_buckets=0, want_lse=False):
-    """(out (N, C), lse, second) of ptv3_patch_attention_fwd, the last two for patch_attention_bwd (or None); param: the table with maps = 1, lam with maps = 2.
+    """(out (N, C), lse, second) of ptv3_patch_attention_fwd, the last two for patch_attention_bwd (or None); param: the
+    table with maps = 1, lam with maps = 2.
     ``functional.attention_bias`` and ``functional.attention_diff`` are the checked forms with gradients."""
     _lib.require_cuda(qkv, rows, cu_seqlens, param, grid, buckets)
-    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
-                              num_buckets)
-    out = torch.empty((qkv.shape[0], a.channels), dtype=qkv.dtype, device=qkv.device)
+    out = torch.empty((qkv.shape[0], qkv.shape[1] // 3), dtype=qkv.dtype, device=qkv.device)
     lse = torch.empty((2 * heads * maps, n_pad), dtype=torch.float32, device=qkv.device) if want_lse else None
     second = torch.empty_like(out) if want_lse and maps == 2 else None
-    a.out, a.lse, a.second = out.data_ptr(), _lib.ptr(lse), _lib.ptr(second)
+    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
+                              num_buckets, out, lse, second)
     with timed("patch_attention"):
-        _lib.check(_lib.load().ptv3_patch_attention_fwd(ctypes.byref(a), _lib.stream()), "ptv3_patch_attention_fwd")
+        _lib.check(_lib.load().ptv3_patch_attention_fwd(a, _lib.stream()), "ptv3_patch_attention_fwd")
     return out, lse, second
 
 
@@ -288,19 +289,14 @@ def patch_attention_bwd(qkv, rows, n_pad, cu_seqlens, out, lse, second, dout, he
     """Gradients (dqkv, gradient of param or None) of patch_attention_fwd."""
     _lib.require_cuda(qkv, rows, cu_seqlens, out, lse, second, dout, param, grid, buckets)
     lib = _lib.load()
-    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
-                              num_buckets)
     dqkv = torch.empty_like(qkv)
     dparam = torch.empty_like(param) if want_param and param is not None else None
-    a.out, a.lse, a.second = out.data_ptr(), lse.data_ptr(), _lib.ptr(second)
-    a.dout, a.dqkv = dout.data_ptr(), dqkv.data_ptr()
-    if dparam is not None:
-        setattr(a, "dlam" if maps == 2 else "dtable", dparam.data_ptr())
-    nbytes = lib.ptv3_patch_attention_workspace_bytes(ctypes.byref(a))
-    ws = _lib.workspace(nbytes, qkv.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    args = (qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num_buckets, out,
+            lse, second, dout, dqkv, dparam)
+    ws = _lib.workspace(lib.ptv3_patch_attention_workspace_bytes(_patch_attention_args(*args)), qkv.device)
+    a = _patch_attention_args(*args, ws)
     with timed("patch_attention_bwd"):
-        _lib.check(lib.ptv3_patch_attention_bwd(ctypes.byref(a), _lib.stream()), "ptv3_patch_attention_bwd")
+        _lib.check(lib.ptv3_patch_attention_bwd(a, _lib.stream()), "ptv3_patch_attention_bwd")
     return dqkv, dparam
 
 

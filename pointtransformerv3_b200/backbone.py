@@ -129,7 +129,7 @@ class NativeBackbone:
             blocks = (_lib.BlockArgs * max(1, len(mods)))()
             order_index, patch = (ctypes.c_int * max(1, len(mods)))(), (ctypes.c_int * max(1, len(mods)))()
             for j, m in enumerate(mods):
-                _require(type(m) is M.Block and m._fusable_form() and not m.attn.enable_rpe
+                _require(type(m) is M.Block and m._fusable_form() and m.attn.plain
                          and type(m.attn) is M.SerializedAttention and m._native_static_ok(self.dtype, f32=self.f32)
                          and m.channels < spconv.PAIR_PATH_MIN_CHANNELS)
                 args = m._native_args(self.dtype, m.attn.qkv.weight.device)
@@ -150,7 +150,7 @@ class NativeBackbone:
         got = []
         for m in self.blocks:
             t = m.attn
-            got.append((t.algo, t.scale, t.order_index, t.enable_flash,
+            got.append((t.algo, t.scale, t.order_index, t.enable_flash, t.plain,
                         t.patch_size if t.enable_flash else t.patch_size_max))
         for p in self.pools:
             got.append((p.stride, p.reduce))

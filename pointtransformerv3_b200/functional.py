@@ -76,15 +76,15 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, grid, q_weight, k_weight, heads, eps, base):
         out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
-        ctx.save_for_backward(qkv if q_weight is not None else None, grid, q_weight, k_weight)
-        ctx.args = heads, eps, base
+        ctx.save_for_backward(qkv if q_weight is not None else None, q_weight, k_weight)
+        ctx.args = grid, heads, eps, base          # (index tensors may have been made in inference mode)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, grid, q_weight, k_weight = ctx.saved_tensors
-        heads, eps, base = ctx.args
+        qkv, q_weight, k_weight = ctx.saved_tensors
+        grid, heads, eps, base = ctx.args
         with _on(dout.device):
             dqkv, dq, dk = ops.qk_norm_rope_bwd(qkv, _aligned(dout), heads, grid, q_weight, k_weight, eps, base)
         return dqkv, None, dq, dk, None, None, None
@@ -130,15 +130,15 @@ class _PatchAttention(torch.autograd.Function):
     def forward(ctx, qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status):
         rows, out, lse, second = _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, True)
         grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
-        ctx.save_for_backward(qkv, param, rows, geometry[3], grid, buckets, out, lse, second)
-        ctx.args = geometry[1].shape[0], heads, max_seqlen, scale, maps, pos_bnd, num
+        ctx.save_for_backward(qkv, param, out, lse, second)
+        ctx.args = rows, geometry[1].shape[0], geometry[3], heads, max_seqlen, scale, maps, grid, buckets, pos_bnd, num
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, param, rows, cu, grid, buckets, out, lse, second = ctx.saved_tensors
-        n_pad, heads, max_seqlen, scale, maps, pos_bnd, num = ctx.args
+        qkv, param, out, lse, second = ctx.saved_tensors
+        rows, n_pad, cu, heads, max_seqlen, scale, maps, grid, buckets, pos_bnd, num = ctx.args
         with _on(dout.device):
             dqkv, dparam = ops.patch_attention_bwd(qkv, rows, n_pad, cu, out, lse, second, _aligned(dout), heads,
                                                    max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,

@@ -10,7 +10,7 @@ from functools import partial
 import torch
 import torch.nn as nn
 
-from . import _lib, backbone, ops
+from . import _lib, backbone, functional, ops
 from . import sparse as spconv
 from .point import AttrDict, Point, offset2bincount
 
@@ -131,20 +131,27 @@ def _is_bn_gelu(norm, act):
 class RPE(nn.Module):
     """Relative position bias table (model.py:297-316).  The lookup and the sum
     over the three axes happen inside the attention kernel; ``forward`` keeps the
-    reference's tensor form for stand-alone use."""
+    reference's tensor form for stand-alone use.  ``bound``: offsets up to that many cells, in buckets that
+    widen with the distance (``functional.log_buckets``), instead of one entry for each of the near ones."""
 
-    def __init__(self, patch_size, num_heads):
+    def __init__(self, patch_size, num_heads, bound=None):
         super().__init__()
         self.patch_size = patch_size
         self.num_heads = num_heads
-        self.pos_bnd = int((4 * patch_size) ** (1 / 3) * 2)
+        self.pos_bnd = int((4 * patch_size) ** (1 / 3) * 2) if bound is None else int(bound)
         self.rpe_num = 2 * self.pos_bnd + 1
+        buckets = None
+        if bound is not None:
+            buckets, self.rpe_num = functional.log_buckets(self.pos_bnd)
+        self.register_buffer("buckets", buckets, persistent=False)
         self.rpe_table = nn.Parameter(torch.zeros(3 * self.rpe_num, num_heads))
         nn.init.trunc_normal_(self.rpe_table, std=0.02)
 
     def forward(self, coord):
-        idx = (coord.clamp(-self.pos_bnd, self.pos_bnd) + self.pos_bnd
-               + torch.arange(3, device=coord.device) * self.rpe_num)
+        idx = coord.clamp(-self.pos_bnd, self.pos_bnd) + self.pos_bnd
+        if self.buckets is not None:
+            idx = self.buckets[idx.long()]
+        idx = idx + torch.arange(3, device=coord.device) * self.rpe_num
         out = self.rpe_table.index_select(0, idx.reshape(-1))
         out = out.view(idx.shape + (-1,)).sum(3)
         return out.permute(0, 3, 1, 2)
@@ -155,16 +162,27 @@ class SerializedAttention(PointModule):
     (model.py:319-490).  Both settings of ``enable_flash`` run the same CUDA
     kernel; the flag keeps the reference's patch-size rule: off -> patch =
     min(smallest scene, patch_size) re-evaluated per call (model.py:441-444),
-    on -> patch = patch_size with shorter scenes as one short sequence."""
+    on -> patch = patch_size with shorter scenes as one short sequence.
+
+    In training mode the module has gradients, of its parameters and of the features it is given (heads of 16, 32 or
+    64 channels, no ``attn_drop``).  Options beyond the reference's, in either mode:
+    ``qk_norm``        queries and keys of every head divided by their root mean square, times a learned weight;
+    ``enable_rope``    queries and keys rotated by the grid coordinates (``rope_base``: of the frequencies);
+    ``rpe_bound``      the bias of ``enable_rpe`` over offsets up to that many cells, in widening buckets;
+    ``differential``   the difference of two softmax maps of half a head's queries and keys each, the second times
+                       a learned weight for each head (from ``differential_init`` on); not with a bias."""
 
     def __init__(self, channels, num_heads, patch_size, qkv_bias=True, qk_scale=None, attn_drop=0.0,
                  proj_drop=0.0, order_index=0, enable_rpe=False, enable_flash=True,
-                 upcast_attention=True, upcast_softmax=True):
+                 upcast_attention=True, upcast_softmax=True, qk_norm=False, enable_rope=False, rope_base=100.0,
+                 rpe_bound=None, differential=False, differential_init=0.5):
         super().__init__()
         assert channels % num_heads == 0
         self.channels = channels
         self.num_heads = num_heads
-        self.scale = qk_scale or (channels // num_heads) ** -0.5
+        self.maps = 2 if differential else 1
+        width = channels // num_heads // self.maps        # of a map's queries and keys
+        self.scale = qk_scale or width ** -0.5
         self.order_index = order_index
         self.upcast_attention = upcast_attention
         self.upcast_softmax = upcast_softmax
@@ -182,8 +200,19 @@ class SerializedAttention(PointModule):
         self.qkv = nn.Linear(channels, channels * 3, bias=qkv_bias)
         self.proj = nn.Linear(channels, channels)
         self.proj_drop = nn.Dropout(proj_drop)
-        self.rpe = RPE(patch_size, num_heads) if self.enable_rpe else None
+        assert rpe_bound is None or enable_rpe, "rpe_bound is the bound of enable_rpe's bias"
+        assert not (differential and enable_rpe), "Set enable_rpe to False with differential attention"
+        self.rpe = RPE(patch_size, num_heads, rpe_bound) if self.enable_rpe else None
+        self.enable_rope, self.rope_base = enable_rope, rope_base
+        self.q_norm = nn.Parameter(torch.ones(width)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(width)) if qk_norm else None
+        self.lam = nn.Parameter(torch.full((num_heads,), float(differential_init))) if differential else None
         self.algo = 0
+
+    @property
+    def plain(self):
+        """Whether this is the attention that the one-call block and backbone know."""
+        return not (self.enable_rpe or self.enable_rope or self.q_norm is not None or self.lam is not None)
 
     @torch.no_grad()
     def get_padding_and_inverse(self, point):
@@ -205,10 +234,23 @@ class SerializedAttention(PointModule):
     def core(self, point, qkv):
         """Patch attention of an already projected (N, 3C) qkv matrix over
         ``point``'s serialized order; the output projection is not applied."""
-        assert not self.training, "inference only"
+        assert not (self.training and self.attn_drop), "no dropout of probabilities"
         if not self.enable_flash:
             self.patch_size = min(min(point.host_counts()), self.patch_size_max)
         pad, unpad, cu_seqlens = self.get_padding_and_inverse(point)
+        with torch.set_grad_enabled(self.training and torch.is_grad_enabled()):
+            if self.q_norm is not None or self.enable_rope:
+                qkv = functional.qk_norm_rope(qkv, self.num_heads * self.maps, point.grid_coord if self.enable_rope else None,
+                                              self.q_norm, self.k_norm, base=self.rope_base)
+            geometry = (point.serialized_order[self.order_index], pad, unpad, cu_seqlens, self.num_heads, self.patch_size,
+                        self.scale)
+            if self.lam is not None:
+                return functional.attention_diff(qkv, self.lam, *geometry, status=point.device_status())
+            if self.training or (self.enable_rpe and self.rpe.buckets is not None):
+                bias = {}
+                if self.enable_rpe:
+                    bias = dict(grid_coord=point.grid_coord, table=self.rpe.rpe_table, buckets=self.rpe.buckets)
+                return functional.attention_bias(qkv, *geometry, status=point.device_status(), **bias)
         if self.enable_rpe:
             return ops.attention_rpe(qkv, point.serialized_order[self.order_index], pad, unpad, cu_seqlens,
                                      point.grid_coord, self.rpe.rpe_table, self.rpe.pos_bnd, self.num_heads,
@@ -219,6 +261,8 @@ class SerializedAttention(PointModule):
 
     def attend(self, point, feat):
         """qkv projection, patch attention and output projection of ``feat``."""
+        if self.training:
+            return self.proj_drop(self.proj(self.core(point, self.qkv(feat))))
         status = point.device_status()
         return self.proj_drop(_linear_op(self.core(point, _linear_op(feat, self.qkv, status)), self.proj, status))
 
@@ -249,7 +293,8 @@ class Block(PointModule):
     def __init__(self, channels, num_heads, patch_size=48, mlp_ratio=4.0, qkv_bias=True, qk_scale=None,
                  attn_drop=0.0, proj_drop=0.0, drop_path=0.0, norm_layer=nn.LayerNorm, act_layer=nn.GELU,
                  pre_norm=True, order_index=0, cpe_indice_key=None, enable_rpe=False, enable_flash=True,
-                 upcast_attention=True, upcast_softmax=True):
+                 upcast_attention=True, upcast_softmax=True, attn_options=None):
+        """``attn_options``: options of ``SerializedAttention`` beyond the reference's, by name."""
         super().__init__()
         self.channels = channels
         self.pre_norm = pre_norm
@@ -263,7 +308,7 @@ class Block(PointModule):
             channels=channels, patch_size=patch_size, num_heads=num_heads, qkv_bias=qkv_bias,
             qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=proj_drop, order_index=order_index,
             enable_rpe=enable_rpe, enable_flash=enable_flash, upcast_attention=upcast_attention,
-            upcast_softmax=upcast_softmax)
+            upcast_softmax=upcast_softmax, **(attn_options or {}))
         self.norm2 = PointSequential(norm_layer(channels))
         self.mlp = PointSequential(MLP(in_channels=channels, hidden_channels=int(channels * mlp_ratio),
                                        out_channels=channels, act_layer=act_layer, drop=proj_drop))
@@ -372,7 +417,7 @@ class Block(PointModule):
         shortcut, sparse = point.feat, point.sparse_conv_feat
         attn = self.attn
         dt = shortcut.dtype
-        if ops.TIMERS is not None or attn.enable_rpe or not self._native_static_ok(dt):
+        if ops.TIMERS is not None or not attn.plain or not self._native_static_ok(dt):
             return None
         args = self._native_args(dt, shortcut.device)
         if args is None:
@@ -662,7 +707,8 @@ _PLAN_STREAMS = {}      # (device, stream) -> planning stream
 
 
 class PointTransformerV3(PointModule):
-    """The backbone (model.py:786-982); constructor arguments as in the reference."""
+    """The backbone (model.py:786-982); constructor arguments as in the reference, and ``attn_options`` for the
+    options of ``SerializedAttention`` beyond it, by name (all attention modules get them)."""
 
     def __init__(self, in_channels=6, order=("z", "z-trans", "hilbert", "hilbert-trans"), stride=(2, 2, 2, 2),
                  enc_depths=(2, 2, 2, 6, 2), enc_channels=(32, 64, 128, 256, 512),
@@ -673,7 +719,7 @@ class PointTransformerV3(PointModule):
                  enable_rpe=False, enable_flash=True, upcast_attention=False, upcast_softmax=False,
                  cls_mode=False, pdnorm_bn=False, pdnorm_ln=False, pdnorm_decouple=True,
                  pdnorm_adaptive=False, pdnorm_affine=True,
-                 pdnorm_conditions=("ScanNet", "S3DIS", "Structured3D")):
+                 pdnorm_conditions=("ScanNet", "S3DIS", "Structured3D"), attn_options=None):
         super().__init__()
         self.num_stages = len(enc_depths)
         self.order = [order] if isinstance(order, str) else order
@@ -725,7 +771,8 @@ class PointTransformerV3(PointModule):
                               drop_path=enc_drop_path_[i], norm_layer=ln_layer, act_layer=act_layer,
                               pre_norm=pre_norm, order_index=i % len(self.order),
                               cpe_indice_key=f"stage{s}", enable_rpe=enable_rpe, enable_flash=enable_flash,
-                              upcast_attention=upcast_attention, upcast_softmax=upcast_softmax),
+                              upcast_attention=upcast_attention, upcast_softmax=upcast_softmax,
+                              attn_options=attn_options),
                         name=f"block{i}")
             if len(enc) != 0:
                 self.enc.add(module=enc, name=f"enc{s}")
@@ -749,7 +796,7 @@ class PointTransformerV3(PointModule):
                                   pre_norm=pre_norm, order_index=i % len(self.order),
                                   cpe_indice_key=f"stage{s}", enable_rpe=enable_rpe,
                                   enable_flash=enable_flash, upcast_attention=upcast_attention,
-                                  upcast_softmax=upcast_softmax), name=f"block{i}")
+                                  upcast_softmax=upcast_softmax, attn_options=attn_options), name=f"block{i}")
                 self.dec.add(module=dec, name=f"dec{s}")
 
     def _side_stream(self, device):

@@ -58,28 +58,70 @@ __device__ __forceinline__ void pf_places(const PatchTable& t, int dx, int dy, i
         at[c] = ((min(max(d[c], -t.reach[c]), t.reach[c]) + t.reach[c] + t.first[c]) << t.copies_log2) + copy;
 }
 
+// A thread's share of a row as packed pairs: half the multiply-adds to issue (20 011 x 64, differential, fp32: forward 127 us with
+// single ones, rows 133, columns 205; 111, 112 and 169 so).
+template <int N>
+__device__ __forceinline__ uint64_t pf_sum(const uint64_t (&x)[N], int first, const float* y, int n)
+{
+    uint64_t v = 0;
+    const ulonglong2* y2 = (const ulonglong2*)y;
+#pragma unroll
+    for (int i = 0; i < n / 4; ++i) {
+        const ulonglong2 p = y2[i];
+        v = fma2(x[first + 2 * i], p.x, fma2(x[first + 2 * i + 1], p.y, v));
+    }
+    return v;
+}
 template <int W, int MAPS>
-__device__ __forceinline__ void pf_scores(const float (&q)[PfShape<W, MAPS>::WP], const float* k, int part, float (&s)[MAPS])
+__device__ __forceinline__ void pf_scores(const uint64_t (&q)[PfShape<W, MAPS>::WP / 2], const float* k, int part,
+                                          float (&s)[MAPS])
 {
     using S = PfShape<W, MAPS>;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < S::DP; ++i) v = fmaf(q[m * S::DP + i], k[m * S::D + part * S::DP + i], v);
+        float v = hsum2(pf_sum(q, m * S::DP / 2, k + m * S::D + part * S::DP, S::DP));
         if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
         s[m] = v;
     }
 }
 template <int W, int MAPS>
-__device__ __forceinline__ float pf_dot(const float (&x)[PfShape<W, MAPS>::WP], const float* y, int part)
+__device__ __forceinline__ float pf_dot(const uint64_t (&x)[PfShape<W, MAPS>::WP / 2], const float* y, int part)
 {
     using S = PfShape<W, MAPS>;
-    float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < S::WP; ++i) v = fmaf(x[i], y[part * S::WP + i], v);
+    float v = hsum2(pf_sum(x, 0, y + part * S::WP, S::WP));
     if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
     return v;
+}
+// acc[first ..] += f y over n values
+template <int N>
+__device__ __forceinline__ void pf_add(uint64_t (&acc)[N], int first, float f, const float* y, int n)
+{
+    const uint64_t f2 = pack2(f, f);
+    const ulonglong2* y2 = (const ulonglong2*)y;
+#pragma unroll
+    for (int i = 0; i < n / 4; ++i) {
+        const ulonglong2 p = y2[i];
+        acc[first + 2 * i] = fma2(f2, p.x, acc[first + 2 * i]);
+        acc[first + 2 * i + 1] = fma2(f2, p.y, acc[first + 2 * i + 1]);
+    }
+}
+// pair i of a share of a row of queries or keys, and that of a contiguous share
+template <int W, int MAPS>
+__device__ __forceinline__ uint64_t pf_pair(const float* row, int i, int part)
+{
+    const float2 v = *(const float2*)(row + pf_dim<W, MAPS>(2 * i, part));
+    return pack2(v.x, v.y);
+}
+__device__ __forceinline__ uint64_t pf_pair(const float* share, int i)
+{
+    const float2 v = ((const float2*)share)[i];
+    return pack2(v.x, v.y);
+}
+__device__ __forceinline__ void pf_put(float* to, uint64_t v, float f)
+{
+    float x, y;
+    unpack2(v, x, y);
+    *(float2*)to = make_float2(x * f, y * f);
 }
 
 // ------------------------------------------------------------------------------------------------- forward
@@ -88,7 +130,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
+    __shared__ __align__(16) float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
@@ -106,10 +148,12 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     const int e = qi < L ? a.rows[start + qi] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;
-    float q[S::WP], acc[MAPS][S::WP], m[MAPS], l[MAPS];
+    constexpr int NP = S::WP / 2;
+    uint64_t q[NP], acc[MAPS][NP];
+    float m[MAPS], l[MAPS];
     int g[3] = {0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) q[i] = (base[p * stride + pf_dim<W, MAPS>(i, part)]);
+    for (int i = 0; i < NP; ++i) q[i] = pf_pair<W, MAPS>(base + p * stride, i, part);
     if (BIAS)
         for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
 #pragma unroll
@@ -117,7 +161,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
         m[k] = -1e30f;          // (finite: scores may all be -inf)
         l[k] = 0.f;
 #pragma unroll
-        for (int i = 0; i < S::WP; ++i) acc[k][i] = 0.f;
+        for (int i = 0; i < NP; ++i) acc[k][i] = 0;
     }
     const float scale2 = a.scale * PA_LOG2E;
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
@@ -150,7 +194,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
                 m[k] = top[k];
                 l[k] *= fix;
 #pragma unroll
-                for (int i = 0; i < S::WP; ++i) acc[k][i] *= fix;
+                for (int i = 0; i < NP; ++i) acc[k][i] = mul2(acc[k][i], pack2(fix, fix));
             }
             float sum[MAPS] = {};      // of a step's, so that rounding does not grow with every key
 #pragma unroll
@@ -160,8 +204,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
                 for (int k = 0; k < MAPS; ++k) {
                     const float pr = fast_exp2(BIAS ? s[j][k] - m[k] : fmaf(s[j][k], scale2, -m[k]));
                     sum[k] += pr;
-#pragma unroll
-                    for (int i = 0; i < S::WP; ++i) acc[k][i] = fmaf(pr, Vs[jj][part * S::WP + i], acc[k][i]);
+                    pf_add(acc[k], 0, pr, &Vs[jj][part * S::WP], S::WP);
                 }
             }
 #pragma unroll
@@ -180,12 +223,15 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     const float w0 = 1.f / l[0], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
     float* op = (float*)a.out + p * a.C + h * W + part * S::WP;
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) op[i] = MAPS == 2 ? acc[0][i] * w0 - acc[MAPS - 1][i] * w1 : acc[0][i] * w0;
+    for (int i = 0; i < NP; ++i) {
+        const uint64_t v = mul2(acc[0][i], pack2(w0, w0));
+        pf_put(op + 2 * i, MAPS == 2 ? fma2(acc[MAPS - 1][i], pack2(-w1, -w1), v) : v, 1.f);
+    }
     if (MAPS == 2 && a.lse) {
         const float w2 = 1.f / l[MAPS - 1];
         float* o2 = (float*)a.second + p * a.C + h * W + part * S::WP;
 #pragma unroll
-        for (int i = 0; i < S::WP; ++i) o2[i] = acc[MAPS - 1][i] * w2;
+        for (int i = 0; i < NP; ++i) pf_put(o2 + 2 * i, acc[MAPS - 1][i], w2);
     }
 }
 
@@ -196,7 +242,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
+    __shared__ __align__(16) float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
@@ -215,17 +261,19 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C, all = (int64_t)a.H * MAPS * a.n_pad;
     const float* base = (const float*)a.qkv + h * W;
     const int64_t own = p * a.C + h * W + part * S::WP;        // this thread's share of a row of C
-    float q[S::WP], go[S::WP], dq[S::WP], ref[MAPS], by[MAPS], delta[MAPS], reach = 0.f;
+    constexpr int NP = S::WP / 2;
+    uint64_t q[NP], go[NP], dq[NP], sum1 = 0, sum2 = 0;
+    float ref[MAPS], by[MAPS], delta[MAPS], reach = 0.f;
     int g[3] = {0, 0, 0};
-    float d1 = 0.f, d2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) {
-        q[i] = base[p * stride + pf_dim<W, MAPS>(i, part)];
-        go[i] = e >= 0 ? ((const float*)a.dout)[own + i] : 0.f;
-        d1 = fmaf(go[i], e >= 0 ? ((const float*)a.out)[own + i] : 0.f, d1);
-        if (MAPS == 2) d2 = fmaf(go[i], e >= 0 ? ((const float*)a.second)[own + i] : 0.f, d2);
-        dq[i] = 0.f;
+    for (int i = 0; i < NP; ++i) {
+        q[i] = pf_pair<W, MAPS>(base + p * stride, i, part);
+        go[i] = e >= 0 ? pf_pair((const float*)a.dout + own, i) : 0;
+        sum1 = fma2(go[i], e >= 0 ? pf_pair((const float*)a.out + own, i) : 0, sum1);
+        if (MAPS == 2) sum2 = fma2(go[i], e >= 0 ? pf_pair((const float*)a.second + own, i) : 0, sum2);
+        dq[i] = 0;
     }
+    float d1 = hsum2(sum1), d2 = hsum2(sum2);
     if (S::SPLIT == 2) {
         d1 += __shfl_xor_sync(0xffffffffu, d1, 1);
         d2 += __shfl_xor_sync(0xffffffffu, d2, 1);
@@ -263,9 +311,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
             for (int k = 0; k < MAPS; ++k) {
                 const float ds = fast_exp2(BIAS ? s[k] - ref[k] : fmaf(s[k], scale2, -ref[k])) * (G - delta[k]);
                 if (BIAS) reach += fabsf(ds);
-#pragma unroll
-                for (int i = 0; i < S::DP; ++i)
-                    dq[k * S::DP + i] = fmaf(ds, Ks[j][k * S::D + part * S::DP + i], dq[k * S::DP + i]);
+                pf_add(dq, k * S::DP / 2, ds, &Ks[j][k * S::D + part * S::DP], S::DP);
             }
         }
     }
@@ -275,7 +321,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     if (MAPS == 2) by[MAPS - 1] *= -lam * a.scale;
     float* dst = (float*)a.dqkv + p * stride + h * W;
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) dst[pf_dim<W, MAPS>(i, part)] = dq[i] * by[i / S::DP];
+    for (int i = 0; i < NP; ++i) pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dq[i], by[2 * i / S::DP]);
 }
 
 // --------------------------------------------------------------------------- backward, a thread's own key
@@ -284,7 +330,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
+    __shared__ __align__(16) float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
     // reference value, (-lam) / sum and delta of every query
     __shared__ float Ms[MAPS][PF_CHUNK], Is[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK], unit_part[PF_THREADS / 8];
@@ -318,13 +364,15 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     const int e = kj < L ? a.rows[start + kj] : -1;
     const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;
-    float k[S::WP], v[S::WP], dk[S::WP], dv[S::WP], coef[MAPS];
+    constexpr int NP = S::WP / 2;
+    uint64_t k[NP], v[NP], dk[NP], dv[NP];
+    float coef[MAPS];
     int g[3] = {0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < S::WP; ++i) {
-        k[i] = (base[p * stride + a.C + pf_dim<W, MAPS>(i, part)]);
-        v[i] = (base[p * stride + 2 * a.C + part * S::WP + i]);
-        dk[i] = dv[i] = 0.f;
+    for (int i = 0; i < NP; ++i) {
+        k[i] = pf_pair<W, MAPS>(base + p * stride + a.C, i, part);
+        v[i] = pf_pair(base + p * stride + 2 * a.C + part * S::WP, i);
+        dk[i] = dv[i] = 0;
     }
     if (BIAS)
         for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
@@ -373,12 +421,9 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
 #pragma unroll
                     for (int c = 0; c < 3; ++c) atomicAdd(hist + (at[c] >> fewer), v);
                 }
-#pragma unroll
-                for (int i = 0; i < S::DP; ++i)
-                    dk[m * S::DP + i] = fmaf(ds, Qs[j][m * S::D + part * S::DP + i], dk[m * S::DP + i]);
+                pf_add(dk, m * S::DP / 2, ds, &Qs[j][m * S::D + part * S::DP], S::DP);
             }
-#pragma unroll
-            for (int i = 0; i < S::WP; ++i) dv[i] = fmaf(mix, Os[j][part * S::WP + i], dv[i]);
+            pf_add(dv, 0, mix, &Os[j][part * S::WP], S::WP);
         }
     }
     if (learns) {
@@ -392,16 +437,16 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     if (slot >= 0) {             // this point's other row is some other patch's: added up later
         float* dst = a.shared + (int64_t)slot * 2 * a.C + h * W;
 #pragma unroll
-        for (int i = 0; i < S::WP; ++i) {
-            dst[pf_dim<W, MAPS>(i, part)] = dk[i] * a.scale;
-            dst[a.C + part * S::WP + i] = dv[i];
+        for (int i = 0; i < NP; ++i) {
+            pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dk[i], a.scale);
+            pf_put(dst + a.C + part * S::WP + 2 * i, dv[i], 1.f);
         }
     } else if (e >= 0) {
         float* dst = (float*)a.dqkv + p * stride + a.C + h * W;
 #pragma unroll
-        for (int i = 0; i < S::WP; ++i) {
-            dst[pf_dim<W, MAPS>(i, part)] = (dk[i] * a.scale);
-            dst[a.C + part * S::WP + i] = (dv[i]);
+        for (int i = 0; i < NP; ++i) {
+            pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dk[i], a.scale);
+            pf_put(dst + a.C + part * S::WP + 2 * i, dv[i], 1.f);
         }
     }
 }

@@ -192,22 +192,6 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
                            int max_seqlen, int channels, int heads, float scale, int dtype, void* stream);
 
 /*
- * Points of the padded rows of a plan, for ptv3_patch_attention_fwd / _bwd, and a look at the plan: every index in range,
- * every point with one row that answers for it and at most one borrowed one (as ptv3_pad_plan writes plans), sequences that
- * follow one another from row 0 to n_pad and are no longer than max_seqlen.  What a bias reads is looked at too, where given:
- * `grid_coord` (n x 3 int32) within 2^22 of zero, `buckets` (2 pos_bnd + 1 int32) in [0, num_buckets).
- *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30
- *   backward    not zero: for a backward pass too (what ptv3_patch_attention_bwd reads of `rows` is written)
- *   rows        2 * n_pad + (n_pad - n) + 1 + 3 * n_seq int32, written
- *   status      one uint32 or NULL: PTV3_STATUS_BAD_INDEX where something does not hold (the calls that read `rows` then
- *               stay within their tensors, and what they leave is undefined)
- */
-int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
-                    int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord,
-                    const int32_t* buckets, int pos_bnd, int num_buckets, int backward, int32_t* rows, uint32_t* status,
-                    void* stream);
-
-/*
  * Patch attention that can be trained: with a learned relative position bias by buckets (maps = 1, grid_coord and
  * table), plain (maps = 1 without them), or differential (maps = 2).  Per head of W = channels / heads values
  *   maps = 1:  out = softmax(scale q k^T + bias) v
@@ -220,7 +204,13 @@ int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unp
  * not depend on the order in which anything runs.  A workspace or an `lse` belongs to one call in flight: graphs that may run at
  * the same time need one each.
  *   qkv, dqkv   n x 3*channels; out, dout n x channels; 16-byte aligned, dtype PTV3_DTYPE_*
- *   rows        of ptv3_patch_rows
+ *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30; read by _fwd (cu_seqlens by _bwd too)
+ *   rows        2 * n_pad + (n_pad - n) + 1 + 3 * n_seq int32: what the kernels need of the plan, written by _fwd, read by _bwd
+ *   grid_coord  n x 3 int32 within 2^22 of zero; buckets 2 pos_bnd + 1 int32 in [0, num_buckets)
+ *   status      one uint32 or NULL: _fwd ORs PTV3_STATUS_BAD_INDEX into it where the plan or the bias does not hold: an index out
+ *               of range, a point without one row that answers for it or with more than one borrowed row, sequences that do
+ *               not follow one another from row 0 to n_pad or are longer than max_seqlen, coordinates or buckets out of
+ *               range.  All accesses stay within the tensors then, and what is left in them is undefined
  *   table       3 * num_buckets x heads, lam heads: fp32 or bf16 (table_dtype, lam_dtype); gradients in the same type
  *   lse         2 * heads * maps * n_pad fp32, and with maps = 2 second, n x channels like out: what _bwd needs of the softmax
  *               and of the second map, written by _fwd (not where lse is NULL)
@@ -233,8 +223,11 @@ typedef struct ptv3_patch_attention_args {
     float scale;
     int pos_bnd, num_buckets, table_dtype, lam_dtype;
     const void* qkv;
-    const int32_t *rows, *cu_seqlens, *grid_coord, *buckets;
+    const int64_t *order, *pad, *unpad;
+    const int32_t *cu_seqlens, *grid_coord, *buckets;
     const void *table, *lam;
+    int32_t* rows;
+    uint32_t* status;
     void* out;
     float* lse;
     void* second;

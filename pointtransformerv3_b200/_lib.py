@@ -69,10 +69,10 @@ class BackboneArgs(ctypes.Structure):
 
 
 # ptv3_patch_attention_args of include/ptv3_b200.h (same field order, native alignment): n, n_pad; n_seq, max_seqlen,
-# channels, heads, maps, dtype; scale; pos_bnd, num_buckets, table_dtype, lam_dtype; qkv, rows, cu_seqlens, grid_coord,
-# buckets, table, lam, out, lse, second, dout, dqkv, dtable, dlam, workspace; workspace_bytes.  Packed in one go: filling
-# a ctypes structure field by field costs as much as two launches.
-PATCH_ATTENTION_ARGS = struct.Struct("@qq6if4i15PN")
+# channels, heads, maps, dtype; scale; pos_bnd, num_buckets, table_dtype, lam_dtype; qkv, order, pad, unpad,
+# cu_seqlens, grid_coord, buckets, table, lam, rows, status, out, lse, second, dout, dqkv, dtable, dlam, workspace;
+# workspace_bytes.  Packed in one go: filling a ctypes structure field by field costs as much as two launches.
+PATCH_ATTENTION_ARGS = struct.Struct("@qq6if4i19PN")
 
 
 # name -> (restype, argtypes); must list every symbol of include/ptv3_b200.h
@@ -89,8 +89,6 @@ SIGNATURES = {
                                    c_int, c_f32, c_int, c_int, c_ptr, c_ptr]),
     "ptv3_attention_rpe_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_ptr, c_i64, c_int,
                                        c_int, c_int, c_int, c_f32, c_int, c_ptr]),
-    "ptv3_patch_rows": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr, c_int, c_int,
-                                c_int, c_ptr, c_ptr, c_ptr]),
     "ptv3_patch_attention_fwd": (c_int, [c_ptr, c_ptr]),
     "ptv3_patch_attention_workspace_bytes": (c_sz, [c_ptr]),
     "ptv3_patch_attention_bwd": (c_int, [c_ptr, c_ptr]),

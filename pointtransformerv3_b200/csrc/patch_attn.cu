@@ -265,7 +265,7 @@ static PatchWorkspace carve(const ptv3_patch_attention_args* p)
 static int check_sizes(const ptv3_patch_attention_args* p, const char* what)
 {
     PTV3_REQUIRE(p != nullptr, PTV3_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
-    PTV3_REQUIRE(p->n >= 0 && p->n_pad >= p->n && p->n_seq >= 0 && p->max_seqlen >= 1 && p->channels >= 1 && p->heads >= 1 &&
+    PTV3_REQUIRE(p->n >= 0 && p->n_pad >= p->n && p->n_pad <= 2 * p->n && p->n_seq >= 0 && p->max_seqlen >= 1 && p->channels >= 1 && p->heads >= 1 &&
                      p->channels % p->heads == 0 && (p->maps == 1 || p->maps == 2),
                  PTV3_ERR_INVALID_ARGUMENT, "%s: bad sizes", what);
     const int width = p->channels / p->heads;
@@ -330,43 +330,35 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
 
 using namespace ptv3;
 
-extern "C" int ptv3_patch_rows(const int64_t* order, const int64_t* pad, const int64_t* unpad, const int32_t* cu_seqlens,
-                               int64_t n, int64_t n_pad, int n_seq, int max_seqlen, const int32_t* grid_coord,
-                               const int32_t* buckets, int pos_bnd, int num_buckets, int backward, int32_t* rows,
-                               uint32_t* status, void* stream)
+// the plan's rows, for the attention kernel behind it in the stream
+static int launch_rows(const ptv3_patch_attention_args* a, cudaStream_t stream)
 {
-    PTV3_REQUIRE(n >= 0 && n_pad >= n && n_seq >= 0 && max_seqlen >= 1 && n_pad < (1ll << 30) && n_seq < (1 << 30),
-                 PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: bad sizes");
-    if (n == 0) return PTV3_OK;
-    PTV3_REQUIRE(order && pad && unpad && cu_seqlens && rows, PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: null pointer");
-    PTV3_REQUIRE(n_pad <= 2 * n, PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_rows: %lld rows of %lld points", (long long)n_pad,
-                 (long long)n);
+    const int64_t n = a->n, n_pad = a->n_pad;
     const int borrowed = (int)(n_pad - n);
-    PatchPlan p = {order, pad, unpad, cu_seqlens, grid_coord, buckets, (int)n, (int)n_pad, n_seq, max_seqlen,
-                   buckets ? 2 * pos_bnd + 1 : 0, num_buckets, grid_coord ? n_seq : 0, rows,
-                   backward && borrowed ? rows + n_pad : nullptr, rows + 2 * n_pad + borrowed + 1, status};
+    PatchPlan p = {a->order, a->pad, a->unpad, a->cu_seqlens, a->grid_coord, a->buckets, (int)n, (int)n_pad, a->n_seq,
+                   a->max_seqlen, a->buckets ? 2 * a->pos_bnd + 1 : 0, a->num_buckets, a->grid_coord ? a->n_seq : 0, a->rows,
+                   a->lse && borrowed ? a->rows + n_pad : nullptr, a->rows + 2 * n_pad + borrowed + 1, a->status};
     if (p.slot) {
-        const cudaError_t e = cudaMemsetAsync(p.slot, 0xff, (size_t)(n_pad + borrowed + 1) * 4, (cudaStream_t)stream);
-        PTV3_REQUIRE(e == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_rows: %s", cudaGetErrorString(e));
+        const cudaError_t e = cudaMemsetAsync(p.slot, 0xff, (size_t)(n_pad + borrowed + 1) * 4, stream);
+        PTV3_REQUIRE(e == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention_fwd: %s", cudaGetErrorString(e));
     }
-    const int64_t most = n_pad > n_seq + 1 ? n_pad : n_seq + 1;
-    launch_dependent(patch_rows_kernel, dim3((unsigned)(p.n_extents + ceil_div(most, 256))), dim3(256), 0,
-                     (cudaStream_t)stream, p);
+    const int64_t most = n_pad > a->n_seq + 1 ? n_pad : a->n_seq + 1;
+    launch_dependent(patch_rows_kernel, dim3((unsigned)(p.n_extents + ceil_div(most, 256))), dim3(256), 0, stream, p);
     count_launches(1);
-    return check_launch("ptv3_patch_rows");
+    return check_launch("ptv3_patch_attention_fwd");
 }
 
 extern "C" int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* p, void* stream)
 {
-    const int rc = check_sizes(p, "ptv3_patch_attention_fwd");
+    int rc = check_sizes(p, "ptv3_patch_attention_fwd");
     if (rc != PTV3_OK) return rc;
     if (p->n == 0 || p->n_seq == 0) return PTV3_OK;
     PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out | (uintptr_t)p->second) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_fwd: unaligned rows");
-    PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || (p->lam && (!p->lse || p->second))),
+    PTV3_REQUIRE(p->qkv && p->order && p->pad && p->unpad && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || (p->lam && (!p->lse || p->second))),
                  PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_fwd: null pointer");
-    PatchArgs a = device_args(p);
-    return launch_patch(p, a, PA_FWD, (cudaStream_t)stream);
+    if ((rc = launch_rows(p, (cudaStream_t)stream)) != PTV3_OK) return rc;
+    return launch_patch(p, device_args(p), PA_FWD, (cudaStream_t)stream);
 }
 
 extern "C" size_t ptv3_patch_attention_workspace_bytes(const ptv3_patch_attention_args* p)
@@ -384,7 +376,7 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
     cudaStream_t s = (cudaStream_t)stream;
     PatchArgs a = device_args(p);
     if (p->n > 0 && p->n_seq > 0)
-        PTV3_REQUIRE(p->qkv && p->rows && p->cu_seqlens && p->out && p->lse && p->dout && p->dqkv &&
+        PTV3_REQUIRE(p->qkv && p->order && p->pad && p->unpad && p->rows && p->cu_seqlens && p->out && p->lse && p->dout && p->dqkv &&
                          (p->maps == 1 || (p->lam && p->second)),
                      PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_bwd: null pointer");
     PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out | (uintptr_t)p->second | (uintptr_t)p->dout | (uintptr_t)p->dqkv) &

@@ -61,7 +61,7 @@ struct PatchArgs {
     float* bins;                // per block of keys: H x 3 (2 bnd + 1), or NULL
 };
 
-// rows [start, start + L) of a sequence; L = 0 for what ptv3_patch_rows reports
+// rows [start, start + L) of a sequence; L = 0 for what patch_rows_kernel reports
 __device__ __forceinline__ int pa_sequence(const PatchArgs& a, int seq, int& start)
 {
     start = a.cu[seq];
@@ -70,7 +70,7 @@ __device__ __forceinline__ int pa_sequence(const PatchArgs& a, int seq, int& sta
     return ok ? end - start : 0;
 }
 
-// a coordinate of a bias (ptv3_patch_rows reports one out of range; places in the table stay within it all the same)
+// a coordinate of a bias (patch_rows_kernel reports one out of range; places in the table stay within it all the same)
 __device__ __forceinline__ int pa_coord(const PatchArgs& a, int64_t p, int c)
 {
     return min(max(a.grid[3 * p + c], -PA_MAX_COORD), PA_MAX_COORD);
@@ -129,7 +129,7 @@ __device__ __forceinline__ void pa_load_table(const PatchArgs& a, const PatchTab
         pa_entry(t, i, axis, d);
         const int e = min(max(d, -a.bnd), a.bnd) + a.bnd;
         int b = a.buckets ? a.buckets[e] : e;
-        b = min(max(b, 0), a.num - 1);                     // (ptv3_patch_rows reports one out of range)
+        b = min(max(b, 0), a.num - 1);                     // (patch_rows_kernel reports one out of range)
         const float v = pa_param(a.table, (axis * a.num + b) * a.H + h, a.table_bf16) * PA_LOG2E;
         for (int c = 0; c < copies; ++c) tab[(i << t.copies_log2) + ((c + tid) & (copies - 1))] = v;
     }

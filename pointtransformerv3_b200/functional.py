@@ -77,7 +77,7 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, qkv, grid, q_weight, k_weight, heads, eps, base):
         out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
         ctx.save_for_backward(qkv if q_weight is not None else None, q_weight, k_weight)
-        ctx.args = grid, heads, eps, base          # (index tensors may have been made in inference mode)
+        ctx.args = grid, heads, eps, base          # (coordinates may have been made in inference mode)
         return out
 
     @staticmethod
@@ -117,32 +117,22 @@ def qk_norm_rope(qkv, heads, grid_coord=None, q_weight=None, k_weight=None, eps=
 
 
 # --------------------------------------------------------------------------- attention
-def _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, keep):
-    order, pad, unpad, cu = geometry
-    grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
-    rows = ops.patch_rows(order, pad, unpad, cu, max_seqlen, grid, buckets, pos_bnd, num, keep, status)
-    return (rows,) + ops.patch_attention_fwd(qkv, rows, pad.shape[0], cu, heads, max_seqlen, scale, maps, param, grid,
-                                             buckets, pos_bnd, num, want_lse=keep)
-
-
 class _PatchAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status):
-        rows, out, lse, second = _patch_forward(qkv, param, geometry, bias, heads, max_seqlen, scale, maps, status, True)
-        grid, buckets, pos_bnd, num = bias if bias is not None else (None, None, 0, 0)
+    def forward(ctx, qkv, param, plan, heads, max_seqlen, scale, maps, bias, status):
+        out, rows, lse, second = ops.patch_attention_fwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, status, True)
         ctx.save_for_backward(qkv, param, out, lse, second)
-        ctx.args = rows, geometry[1].shape[0], geometry[3], heads, max_seqlen, scale, maps, grid, buckets, pos_bnd, num
+        ctx.args = plan, heads, max_seqlen, scale, maps, bias, rows      # (index tensors may have been made in inference mode)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         qkv, param, out, lse, second = ctx.saved_tensors
-        rows, n_pad, cu, heads, max_seqlen, scale, maps, grid, buckets, pos_bnd, num = ctx.args
+        plan, heads, max_seqlen, scale, maps, bias, rows = ctx.args
         with _on(dout.device):
-            dqkv, dparam = ops.patch_attention_bwd(qkv, rows, n_pad, cu, out, lse, second, _aligned(dout), heads,
-                                                   max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,
-                                                   want_param=ctx.needs_input_grad[1])
+            dqkv, dparam = ops.patch_attention_bwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, out, rows, lse,
+                                                   second, _aligned(dout), ctx.needs_input_grad[1])
         return (dqkv, dparam) + (None,) * 7
 
 
@@ -162,7 +152,7 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         scale = (D // maps) ** -0.5
     if not (math.isfinite(scale) and scale):
         raise ValueError("scale %r" % scale)
-    geometry = tuple(t.contiguous() for t in (order_row, pad, unpad, cu_seqlens))
+    plan = tuple(t.contiguous() for t in (order_row, pad, unpad, cu_seqlens))
     qkv, param = _aligned(qkv), None if param is None else param.contiguous()
     own = status is None
     if own and torch.cuda.is_current_stream_capturing():
@@ -170,11 +160,10 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
     with _on(qkv.device):
         if own:
             status = ops.new_status(qkv.device)
-        args = (qkv, param, geometry, bias, int(heads), int(max_seqlen), float(scale), maps, status)
         if _wants_grad(qkv, param):
-            out = _PatchAttention.apply(*args)
+            out = _PatchAttention.apply(qkv, param, plan, int(heads), int(max_seqlen), float(scale), maps, bias, status)
         else:
-            out = _patch_forward(*args, False)[1]
+            out = ops.patch_attention_fwd(qkv, plan, int(heads), int(max_seqlen), float(scale), maps, param, bias, status)[0]
         if own:
             _lib.raise_on_status(status, "ptv3_patch_attention_fwd")
     return out

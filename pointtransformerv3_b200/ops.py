@@ -241,62 +241,53 @@ def qk_norm_rope_bwd(qkv, dout, heads, grid, q_weight, k_weight, eps, base):
     return dqkv, dq, dk
 
 
-def patch_rows(order_row, pad, unpad, cu_seqlens, max_seqlen, grid=None, buckets=None, pos_bnd=0, num_buckets=0,
-               backward=False, status=None):
-    """Points of the padded rows of a plan as patch_attention_fwd / _bwd read them (see ptv3_patch_rows)."""
-    _lib.require_cuda(order_row, pad, unpad, cu_seqlens, grid, buckets, status)
-    n, n_pad, n_seq = order_row.shape[0], pad.shape[0], cu_seqlens.shape[0] - 1
-    rows = torch.empty(3 * n_pad - n + 1 + 3 * n_seq, dtype=torch.int32, device=pad.device)
-    ptr = _lib.ptr
-    _lib.check(_lib.load().ptv3_patch_rows(order_row.data_ptr(), pad.data_ptr(), unpad.data_ptr(), cu_seqlens.data_ptr(), n,
-                                           n_pad, n_seq, max_seqlen, ptr(grid), ptr(buckets), pos_bnd, num_buckets, backward,
-                                           rows.data_ptr(), ptr(status), _lib.stream()), "ptv3_patch_rows")
-    return rows
-
-
-def _patch_attention_args(qkv, rows, n_pad, cu, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num,
-                          out, lse, second, dout=None, dqkv=None, dparam=None, workspace=None):
-    """The packed ptv3_patch_attention_args of a call; param and dparam: the table's or lam's."""
+def _patch_attention_args(qkv, plan, rows, heads, max_seqlen, scale, maps, param, bias, out, lse, second, status=None,
+                          dout=None, dqkv=None, dparam=None, workspace=None):
+    """The packed ptv3_patch_attention_args of a call; plan: (order, pad, unpad, cu_seqlens); bias: (grid_coord, buckets,
+    bound, number of buckets) or None; param and dparam: the table's or lam's."""
     def ptr(t):
         return 0 if t is None else t.data_ptr()
+    order, pad, unpad, cu = plan
+    grid, buckets, bound, num = bias if bias is not None else (None, None, 0, 0)
     kind = 0 if param is None else _lib.dtype_id(param)
     table, dtable, lam, dlam = (ptr(param), ptr(dparam), 0, 0) if maps == 1 else (0, 0, ptr(param), ptr(dparam))
+    n, c3 = qkv.shape
     return _lib.PATCH_ATTENTION_ARGS.pack(
-        qkv.shape[0], n_pad, cu.shape[0] - 1, max_seqlen, qkv.shape[1] // 3, heads, maps, _lib.dtype_id(qkv), scale, pos_bnd,
-        num, kind, kind, qkv.data_ptr(), rows.data_ptr(), cu.data_ptr(), ptr(grid), ptr(buckets), table, lam, out.data_ptr(),
-        ptr(lse), ptr(second), ptr(dout), ptr(dqkv), dtable, dlam, ptr(workspace),
-        0 if workspace is None else workspace.numel())
+        n, pad.shape[0], cu.shape[0] - 1, max_seqlen, c3 // 3, heads, maps, _lib.dtype_id(qkv), scale, bound, num, kind, kind,
+        qkv.data_ptr(), order.data_ptr(), pad.data_ptr(), unpad.data_ptr(), cu.data_ptr(), ptr(grid), ptr(buckets), table, lam,
+        rows.data_ptr(), ptr(status), out.data_ptr(), ptr(lse), ptr(second), ptr(dout), ptr(dqkv), dtable, dlam,
+        ptr(workspace), 0 if workspace is None else workspace.shape[0])
 
 
-def patch_attention_fwd(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps=1, param=None, grid=None,
-                        buckets=None, pos_bnd=0, num_buckets=0, want_lse=False):
-    """(out (N, C), lse, second) of ptv3_patch_attention_fwd, the last two for patch_attention_bwd (or None); param: the
-    table with maps = 1, lam with maps = 2.
-    ``functional.attention_bias`` and ``functional.attention_diff`` are the checked forms with gradients."""
-    _lib.require_cuda(qkv, rows, cu_seqlens, param, grid, buckets)
-    out = torch.empty((qkv.shape[0], qkv.shape[1] // 3), dtype=qkv.dtype, device=qkv.device)
-    lse = torch.empty((2 * heads * maps, n_pad), dtype=torch.float32, device=qkv.device) if want_lse else None
-    second = torch.empty_like(out) if want_lse and maps == 2 else None
-    a = _patch_attention_args(qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd,
-                              num_buckets, out, lse, second)
+def patch_attention_fwd(qkv, plan, heads, max_seqlen, scale, maps=1, param=None, bias=None, status=None, keep=False):
+    """(out (N, C), rows, lse, second) of ptv3_patch_attention_fwd, the last two with ``keep``, for patch_attention_bwd.
+    plan: (order, pad, unpad, cu_seqlens); param: the table with maps = 1, lam with maps = 2; bias: (grid_coord, buckets or
+    None, bound, number of buckets).  ``functional.attention_bias`` and ``functional.attention_diff`` are the checked forms
+    with gradients."""
+    _lib.require_cuda(qkv, *plan, param, status)
+    n, c3 = qkv.shape
+    n_pad, dev = plan[1].shape[0], qkv.device
+    rows = torch.empty(3 * n_pad - n + 1 + 3 * (plan[3].shape[0] - 1), dtype=torch.int32, device=dev)
+    out = torch.empty((n, c3 // 3), dtype=qkv.dtype, device=dev)
+    lse = torch.empty((2 * heads * maps, n_pad), dtype=torch.float32, device=dev) if keep else None
+    second = torch.empty_like(out) if keep and maps == 2 else None
+    args = _patch_attention_args(qkv, plan, rows, heads, max_seqlen, scale, maps, param, bias, out, lse, second, status)
     with timed("patch_attention"):
-        _lib.check(_lib.load().ptv3_patch_attention_fwd(a, _lib.stream()), "ptv3_patch_attention_fwd")
-    return out, lse, second
+        _lib.check(_lib.load().ptv3_patch_attention_fwd(args, _lib.stream()), "ptv3_patch_attention_fwd")
+    return out, rows, lse, second
 
 
-def patch_attention_bwd(qkv, rows, n_pad, cu_seqlens, out, lse, second, dout, heads, max_seqlen, scale, maps=1,
-                        param=None, grid=None, buckets=None, pos_bnd=0, num_buckets=0, want_param=True):
+def patch_attention_bwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, out, rows, lse, second, dout, want_param=True):
     """Gradients (dqkv, gradient of param or None) of patch_attention_fwd."""
-    _lib.require_cuda(qkv, rows, cu_seqlens, out, lse, second, dout, param, grid, buckets)
+    _lib.require_cuda(qkv, *plan, out, rows, lse, second, dout, param)
     lib = _lib.load()
     dqkv = torch.empty_like(qkv)
     dparam = torch.empty_like(param) if want_param and param is not None else None
-    args = (qkv, rows, n_pad, cu_seqlens, heads, max_seqlen, scale, maps, param, grid, buckets, pos_bnd, num_buckets, out,
-            lse, second, dout, dqkv, dparam)
+    args = (qkv, plan, rows, heads, max_seqlen, scale, maps, param, bias, out, lse, second, None, dout, dqkv, dparam)
     ws = _lib.workspace(lib.ptv3_patch_attention_workspace_bytes(_patch_attention_args(*args)), qkv.device)
-    a = _patch_attention_args(*args, ws)
     with timed("patch_attention_bwd"):
-        _lib.check(lib.ptv3_patch_attention_bwd(a, _lib.stream()), "ptv3_patch_attention_bwd")
+        _lib.check(lib.ptv3_patch_attention_bwd(_patch_attention_args(*args, ws), _lib.stream()),
+                   "ptv3_patch_attention_bwd")
     return dqkv, dparam
 
 

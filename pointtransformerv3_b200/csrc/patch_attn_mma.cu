@@ -976,13 +976,13 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 }
 
 // Rows of a block, in tiles of 128: with two tiles to a warp what it reads of the other side serves twice the rows, where
-// registers allow it (heads of 16) and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and
+// registers allow it (heads of 16), patches fill such blocks and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and
 // 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of two maps 347 and 320.  Not so forward and rows
 // without a bias (312 and 326, 341 and 465).
 static int row_tiles(int64_t n_seq, int64_t longest, int heads, int width, int maps, bool bias, int pass)
 {
     const int64_t blocks = n_seq * heads * ((longest + 2 * PM_ROWS - 1) / (2 * PM_ROWS));
-    return width == 16 && blocks >= 2 * SMS && (bias || (maps == 2 && pass == PA_COLS)) ? 2 : 1;
+    return width == 16 && longest >= 2 * PM_ROWS && blocks >= 2 * SMS && (bias || (maps == 2 && pass == PA_COLS)) ? 2 : 1;
 }
 int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width)
 {

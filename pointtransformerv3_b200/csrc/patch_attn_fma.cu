@@ -10,7 +10,8 @@ namespace ptv3 {
 constexpr int PF_THREADS = 128;
 constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
 constexpr int PF_STEP = 8;        // of which scores are held at a time
-constexpr int PF_WINDOW = 32;     // queries between two clearings of the bins: the unit is that much finer
+constexpr int PF_WINDOW = 8;      // queries between two clearings of the bins: the unit is that much finer (gradient of a
+                                  // table, patches of 1 024, off by 4e-6 of its norm with 32, 6e-7 with 8)
 constexpr int PF_BINS_LOG2 = 4;   // 16 copies of them, so that clearing costs little
 constexpr int PF_TABLE_BYTES = 32 * 1024, PF_BINS_BYTES = 48 * 1024;      // for the table; for the table and its bins
 
@@ -236,7 +237,9 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 }
 
 // ------------------------------------------------------------------------- backward, a thread's own query
-// (in fp32 the stored results give delta itself, and the softmax's sum is kept as such: no estimate to correct)
+// (in fp32 the stored results give delta as close as dQ needs it, and the softmax's sum is kept as such.  What is left, the
+// sum of P (G - delta), goes into the delta that the columns read: the same error for all of a row's keys adds up
+// in the table's gradient, 2e-6 of its norm with patches of 1 024 without this.)
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchArgs a)
 {
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     const int64_t own = p * a.C + h * W + part * S::WP;        // this thread's share of a row of C
     constexpr int NP = S::WP / 2;
     uint64_t q[NP], go[NP], dq[NP], sum1 = 0, sum2 = 0;
-    float ref[MAPS], by[MAPS], delta[MAPS], reach = 0.f;
+    float ref[MAPS], by[MAPS], delta[MAPS], left[MAPS] = {}, reach = 0.f;
     int g[3] = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -289,7 +292,6 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
         // a row that answers for no point has no gradient: its probabilities are taken as nothing
         ref[k] = e >= 0 ? a.lse[at] : INFINITY;
         by[k] = e >= 0 ? a.lse[at + all] : 0.f;
-        if (qi < L && part == 0) a.delta[at] = delta[k];
     }
     const float scale2 = a.scale * PA_LOG2E;
     for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
@@ -310,12 +312,18 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) {
                 const float ds = fast_exp2(BIAS ? s[k] - ref[k] : fmaf(s[k], scale2, -ref[k])) * (G - delta[k]);
+                left[k] += ds;
                 if (BIAS) reach += fabsf(ds);
                 pf_add(dq, k * S::DP / 2, ds, &Ks[j][k * S::D + part * S::DP], S::DP);
             }
         }
     }
-    if (BIAS && a.reach && qi < L && part == 0) a.reach[(int64_t)h * a.n_pad + start + qi] = reach * by[0];
+    if (qi < L && part == 0) {
+#pragma unroll
+        for (int k = 0; k < MAPS; ++k)
+            a.delta[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = fmaf(left[k], by[k], delta[k]);
+        if (BIAS && a.reach) a.reach[(int64_t)h * a.n_pad + start + qi] = (reach + fabsf(left[0])) * by[0];
+    }
     if (e < 0) return;
     by[0] *= a.scale;
     if (MAPS == 2) by[MAPS - 1] *= -lam * a.scale;
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     __shared__ __align__(16) float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
     __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
     // reference value, (-lam) / sum and delta of every query
-    __shared__ float Ms[MAPS][PF_CHUNK], Is[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK], unit_part[PF_THREADS / 8];
+    __shared__ float Ms[MAPS][PF_CHUNK], Is[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK], units[PF_CHUNK / PF_WINDOW];
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
     const int part = threadIdx.x % S::SPLIT;
@@ -391,39 +399,49 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
             Is[m][j] = own ? a.lse[at + (int64_t)a.H * MAPS * a.n_pad] * coef[m] : 0.f;
             Ds[m][j] = a.delta[at];
         }
+        if (learns && threadIdx.x < PF_CHUNK) {
+            // what the queries of a window can add to a bin at most is 2^31 units, less what rounding may add
+            float r = threadIdx.x < nq ? a.reach[(int64_t)h * a.n_pad + start + c0 + threadIdx.x] : 0.f;
+#pragma unroll
+            for (int d = 1; d < PF_WINDOW; d <<= 1) r += __shfl_xor_sync(0xffffffffu, r, d);
+            if (threadIdx.x % PF_WINDOW == 0) units[threadIdx.x / PF_WINDOW] = r * (1.f / 2147000000.f);
+        }
         __syncthreads();
-#pragma unroll 4
-        for (int j = 0; j < nq; ++j) {
-            if (learns && j % PF_WINDOW == 0) {
-                if (c0 + j) {
+        for (int j0 = 0; j0 < nq; j0 += PF_WINDOW) {
+            if (learns) {
+                if (c0 + j0) {
                     __syncthreads();
                     pa_flush(table, hist, sums, unit, PF_THREADS);
+                    __syncthreads();
                 }
-                unit = pa_unit<PF_THREADS / 32, PF_WINDOW, false>(a, table, h, start, L, c0 + j, unit_part);
+                unit = units[j0 / PF_WINDOW];
                 per_unit = pa_per_unit(unit);
             }
-            float s[MAPS];
-            int at[3];
-            pf_scores<W, MAPS>(k, Qs[j], part, s);
-            if (BIAS) {
-                pf_places(table, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
-                s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
-            }
-            const float G = pf_dot<W, MAPS>(v, Os[j], part);
-            float mix = 0.f;
-#pragma unroll
-            for (int m = 0; m < MAPS; ++m) {
-                const float pr = Is[m][j] * fast_exp2(BIAS ? s[m] - Ms[m][j] : fmaf(s[m], scale2, -Ms[m][j]));
-                const float ds = pr * (G - Ds[m][j]);
-                mix += pr;
-                if (learns && part == 0 && kj < L) {
-                    const int v = __float2int_rn(ds * per_unit);
-#pragma unroll
-                    for (int c = 0; c < 3; ++c) atomicAdd(hist + (at[c] >> fewer), v);
+#pragma unroll 4
+            for (int j = j0; j < min(j0 + PF_WINDOW, nq); ++j) {
+                float s[MAPS];
+                int at[3];
+                pf_scores<W, MAPS>(k, Qs[j], part, s);
+                if (BIAS) {
+                    pf_places(table, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
+                    s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
                 }
-                pf_add(dk, m * S::DP / 2, ds, &Qs[j][m * S::D + part * S::DP], S::DP);
+                const float G = pf_dot<W, MAPS>(v, Os[j], part);
+                float mix = 0.f;
+#pragma unroll
+                for (int m = 0; m < MAPS; ++m) {
+                    const float pr = Is[m][j] * fast_exp2(BIAS ? s[m] - Ms[m][j] : fmaf(s[m], scale2, -Ms[m][j]));
+                    const float ds = pr * (G - Ds[m][j]);
+                    mix += pr;
+                    if (learns && part == 0 && kj < L) {
+                        const int v = __float2int_rn(ds * per_unit);
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) atomicAdd(hist + (at[c] >> fewer), v);
+                    }
+                    pf_add(dk, m * S::DP / 2, ds, &Qs[j][m * S::D + part * S::DP], S::DP);
+                }
+                pf_add(dv, 0, mix, &Os[j][part * S::WP], S::WP);
             }
-            pf_add(dv, 0, mix, &Os[j][part * S::WP], S::WP);
         }
     }
     if (learns) {

@@ -66,8 +66,10 @@ def _check_qkv(qkv, heads):
 
 
 def _int32(t, shape, what):
-    if tuple(t.shape) != shape:
-        raise ValueError("%s must be %s, got %s" % (what, shape, tuple(t.shape)))
+    if tuple(t.shape) != shape or t.is_floating_point() or t.is_complex():
+        raise ValueError("%s must be integers %s, got %s %s" % (what, shape, t.dtype, tuple(t.shape)))
+    if t.dtype == torch.int64:        # beyond 32 bits: held at their ends, not wrapped into the range
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 
@@ -94,7 +96,7 @@ def qk_norm_rope(qkv, heads, grid_coord=None, q_weight=None, k_weight=None, eps=
     """Queries and keys of a QKV matrix normalised and rotated, values as they are.
 
     qkv (N, 3C), split (3, heads, D).  With ``q_weight`` and ``k_weight`` (D,) every head's query and key is divided by its
-    root mean square (``eps`` added to the mean square) and multiplied by the weight.  With ``grid_coord`` (N, 3) integers the
+    root mean square (``eps`` added to the mean square) and multiplied by the weight.  With ``grid_coord`` (N, 3) integers of 32 bits the
     pairs (2i, 2i+1), i < 3p, p = D // 6, are then turned by grid_coord[i // p] * base ** (-(i % p) / p), so that scores
     depend on the offset between two points; values beyond 6p are left.  D in 8, 16, 32, 64, 128; bf16 or fp32.  For
     ``attention_diff``, whose heads have two queries and two keys, pass twice its number of heads.  Returns a matrix like qkv."""
@@ -146,6 +148,8 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         raise ValueError("cu_seqlens must be a row of int32")
     if any(t.dtype != torch.int64 for t in (order_row, pad, unpad)):
         raise ValueError("order_row, pad and unpad must be int64")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 word")
     if int(max_seqlen) < 1:
         raise ValueError("max_seqlen %d" % max_seqlen)
     if scale is None:

@@ -38,7 +38,9 @@ def test_cpu_tensors_are_refused():
     (lambda: F.qk_norm_rope(t(4, 48), 1, None, t(16)), "or all three"),
     (lambda: F.qk_norm_rope(t(4, 48), 1, None, t(16), t(8)), r"\(16,\)"),
     (lambda: F.qk_norm_rope(t(4, 48), 1, None, t(16), t(16, dtype=torch.bfloat16)), "of one type"),
-    (lambda: F.qk_norm_rope(t(4, 48), 1, t(3, 3)), "grid_coord"),
+    (lambda: F.qk_norm_rope(t(4, 48), 1, t(3, 3, dtype=torch.int32)), "grid_coord"),
+    (lambda: F.qk_norm_rope(t(4, 48), 1, t(4, 3)), "integers"),
+    (lambda: F.attention_bias(t(8, 48), *args(), 1, 8, status=t(1)), "int32 word"),
     (lambda: F.attention_bias(t(8, 48), *args(), 1, 8, table=t(9, 1)), "needs grid_coord"),
     (lambda: F.attention_bias(t(8, 48), *args(), 1, 8, grid_coord=t(8, 3)), "needs a table"),
     (lambda: F.attention_bias(t(8, 48), *args(), 1, 8, grid_coord=t(8, 3), table=t(9, 2)), "1 heads"),

@@ -341,6 +341,24 @@ def test_empty_batch_and_only_needed_gradients():
         assert torch.equal(out, F.attention_bias(qkv, *geometry(p), 2, 32, grid_coord=p["grid"], table=table))
 
 
+def test_sequences_of_no_rows_and_a_table_used_twice():
+    """Patches of no rows between others, and one table in two calls, whose gradients add up."""
+    p = plan([100, 30], 64)
+    cu = p["cu"].tolist()
+    cu = torch.tensor(cu[:1] + cu[:1] + cu[1:2] * 3 + cu[2:] + cu[-1:], dtype=torch.int32, device="cuda")
+    for dtype in DTYPES:
+        qkv, table = normal(130, 96, seed=1, dtype=dtype), normal(33, 2, seed=2, dtype=dtype).requires_grad_()
+        dout = normal(130, 32, seed=3, dtype=dtype)
+
+        def step(ends, times):
+            out = sum(F.attention_bias(qkv, p["order"], p["pad"], p["unpad"], ends, 2, 64, grid_coord=p["grid"], table=table)
+                      for _ in range(times))
+            return out, torch.autograd.grad(out, table, dout)[0]
+        (a, da), (b, db), (c, dc) = step(p["cu"], 1), step(cu, 1), step(p["cu"], 2)
+        assert torch.equal(a, b) and torch.equal(da, db)
+        assert torch.equal(dc, 2 * da) and torch.equal(c, 2 * a)
+
+
 def test_strided_unaligned_and_other_stream():
     p = plan([150, 80], 64)
     n, C, H = p["n"], 32, 2
@@ -442,6 +460,8 @@ def test_bad_plans_are_reported():
     grid[17, 1] = 2 ** 22 + 1
     with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):
         F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=grid, table=torch.ones(9, H, device="cuda"))
+    with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):      # (not wrapped into 32 bits)
+        F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=p["grid"].long() + 2 ** 32, table=torch.ones(9, H, device="cuda"))
     buckets, num = F.log_buckets(12, device="cuda")
     buckets[3] = num
     with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):

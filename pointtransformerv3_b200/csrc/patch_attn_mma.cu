@@ -1,8 +1,8 @@
 // Patch attention with bias or of two maps, forward and backward, for bf16 on the tensor cores by mma.sync
 // (patch_attn.cuh has the mathematics).
 //
-// A CTA of eight warps owns 128 rows (queries, or keys in the pass over columns) of one patch and head, a warp 16 of
-// them; the other side streams through shared memory in chunks of 64 rows, gathered by cp.async through the row list, two
+// A CTA of eight warps (or four) owns 128 rows (queries, or keys in the pass over columns) of one patch and head, a warp 16
+// of them (or 32); the other side streams through shared memory in chunks of 64 rows, gathered by cp.async through the row list, two
 // chunks ahead (three stages, one barrier a chunk).  Scores, probabilities and dS live in accumulator registers and are
 // the A operands of the next product as they lie; rounding to bf16 happens there (probabilities, dS) and where results
 // are stored, everything else is fp32.  Of a map there are 64 tensor FLOPs to an exponential at heads of 16: the exponential unit
@@ -16,21 +16,24 @@
 
 namespace ptv3 {
 
-constexpr int PM_THREADS = 256, PM_WARPS = 8;
-constexpr int PM_ROWS = 128;       // of a CTA
 // Rows of the other side in a stage.  Warps meet once a chunk: with 64 rows instead of 256 the three kernels of 100 000 x 64,
 // differential, take 333, 378 and 386 us instead of 311, 343 and 349; a bias needs the room for its table.
-template <int W, bool BIAS>
+template <int W, bool BIAS, int NT>
 struct PmChunk {
-    static constexpr int N = W == 16 && !BIAS ? 256 : 64;
+    static constexpr int N = W == 16 && !BIAS && NT == 256 ? 256 : 64;
+};
+// Shared memory of a table, and of a table and its bins: smaller CTAs share an SM with more
+template <int NT>
+struct PmTableBytes {
+    static constexpr int TABLE = PA_TABLE_BYTES * NT / 256, BINS = PA_BINS_BYTES * NT / 256;
 };
 constexpr int PM_STAGES = 3;
 constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
 // bytes for the sums of the bins: entries of a table of eight copies, or of the largest bound (patch_attn.cuh)
-static int pm_sums_bytes(int bnd)
+static int pm_sums_bytes(int bnd, int bins_bytes)
 {
-    return (3 * (2 * bnd + 1) > PA_BINS_BYTES / 64 ? 3 * (2 * bnd + 1) : PA_BINS_BYTES / 64) * 4;
+    return (3 * (2 * bnd + 1) > bins_bytes / 64 ? 3 * (2 * bnd + 1) : bins_bytes / 64) * 4;
 }
 constexpr float PM_LOWEST = -1e30f;
 
@@ -73,10 +76,10 @@ __device__ __forceinline__ void pm_add_shared(uint32_t addr, int v)
 }
 
 // The other side's rows: x and y (head h's W values of each), two words of each map (AUX), coordinates (BIAS)
-template <int W, int MAPS, bool AUX, bool BIAS>
+template <int W, int MAPS, bool AUX, bool BIAS, int NT>
 struct PmStream {
-    static constexpr int CH = PmChunk<W, BIAS>::N;
-    static constexpr int NR = CH / 64, NA = AUX ? (2 * MAPS * CH + PM_THREADS - 1) / PM_THREADS : 1;
+    static constexpr int CH = PmChunk<W, BIAS, NT>::N;
+    static constexpr int RPP = NT / 4, NR = CH / RPP, NA = AUX ? (2 * MAPS * CH + NT - 1) / NT : 1;
     using S = PmStage<W, CH>;
     const PatchArgs& a;
     const __nv_bfloat16 *x, *y;
@@ -111,7 +114,7 @@ struct PmStream {
         if (AUX)
 #pragma unroll
             for (int i = 0; i < NA; ++i) {
-                const int k = threadIdx.x + i * PM_THREADS, j = k % CH, what = k / CH, r = chunk * CH + j;
+                const int k = threadIdx.x + i * NT, j = k % CH, what = k / CH, r = chunk * CH + j;
                 ea[i] = k < 2 * MAPS * CH ? row_of(chunk, j) : INT_MIN;
                 aux[i] = 0.f;
                 if (ea[i] != INT_MIN)
@@ -122,7 +125,7 @@ struct PmStream {
     __device__ __forceinline__ void fetch(int chunk)
     {
 #pragma unroll
-        for (int i = 0; i < NR; ++i) e[i] = row_of(chunk, (threadIdx.x >> 2) + 64 * i);
+        for (int i = 0; i < NR; ++i) e[i] = row_of(chunk, (threadIdx.x >> 2) + RPP * i);
         fetch_grid();
         if (BIAS && threadIdx.x < CH) eg = grid_row(chunk + 1);
         fetch_aux(chunk);
@@ -134,7 +137,7 @@ struct PmStream {
             constexpr int CPR = W / 8;
 #pragma unroll
             for (int n = 0; n < NR; ++n) {
-                const int r = (threadIdx.x >> 2) + 64 * n;
+                const int r = (threadIdx.x >> 2) + RPP * n;
                 const bool there = e[n] != INT_MIN;
                 const int64_t p = !there ? 0 : e[n] >= 0 ? e[n] : -(e[n] + 1);
 #pragma unroll
@@ -148,7 +151,7 @@ struct PmStream {
             if (AUX)
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
-                    const int k = threadIdx.x + i * PM_THREADS;
+                    const int k = threadIdx.x + i * NT;
                     // negated; rows that are not there, or answer for no point: probabilities of nothing
                     if (k < 2 * MAPS * CH)
                         ((float*)(st + S::AUX))[k] = ea[i] >= 0 ? -aux[i] : k < MAPS * CH ? -INFINITY : 0.f;
@@ -408,15 +411,15 @@ __device__ __forceinline__ void pm_own_rows(const PmOwn<RT>& own, const __nv_bfl
 }
 
 // ------------------------------------------------------------------------------------------------- forward
-template <int W, int MAPS, bool BIAS, bool KEEP, int RT>
-__global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patch_mma_fwd_kernel(const PatchArgs a)
+template <int W, int MAPS, bool BIAS, bool KEEP, int RT, int NT>
+__global__ void __launch_bounds__(NT, (W == 64 && MAPS == 2 ? 256 : 512) / NT) patch_mma_fwd_kernel(const PatchArgs a)
 {
     pdl_wait();
-    constexpr int CH = PmChunk<W, BIAS>::N;
+    constexpr int CH = PmChunk<W, BIAS, NT>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
-    const int q0 = w.tile * PM_ROWS * RT, L = w.L;
+    const int q0 = w.tile * (NT / 2) * RT, L = w.L;
     if (q0 >= L) return;
     const int t = threadIdx.x & 3;
     PmOwn<RT> own;
@@ -425,15 +428,15 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 && MAPS == 2 ? 1 : 2) patc
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES, false);
-    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+    if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
+    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
     int point[RT][2][3];
     if (BIAS) {
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
-        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);      // (the first chunk's barrier stands behind it)
+        pa_load_table(a, table, w.h, tab, threadIdx.x, NT);      // (the first chunk's barrier stands behind it)
         pm_bias_setup(table, smem_u32(tab), bias);
 #pragma unroll
         for (int x = 0; x < RT; ++x)
@@ -616,15 +619,15 @@ __device__ __forceinline__ void pm_row_dots(const uint32_t (&x)[W / 16][4], cons
     }
 }
 
-template <int W, int MAPS, bool BIAS, int RT>
-__global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_kernel(const PatchArgs a)
+template <int W, int MAPS, bool BIAS, int RT, int NT>
+__global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows_kernel(const PatchArgs a)
 {
     pdl_wait();
-    constexpr int CH = PmChunk<W, BIAS>::N;
+    constexpr int CH = PmChunk<W, BIAS, NT>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     const PmPlace w = pm_place(a);
-    const int q0 = w.tile * PM_ROWS * RT, L = w.L;
+    const int q0 = w.tile * (NT / 2) * RT, L = w.L;
     if (q0 >= L) return;
     const int t = threadIdx.x & 3;
     PmOwn<RT> own;
@@ -632,15 +635,15 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_TABLE_BYTES, false);
-    PmStream<W, MAPS, false, BIAS> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+    if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
+    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
     int point[RT][2][3];
     if (BIAS) {
         float* tab = (float*)(smem + PM_STAGES * S::BYTES);
-        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
+        pa_load_table(a, table, w.h, tab, threadIdx.x, NT);
         pm_bias_setup(table, smem_u32(tab), bias);
 #pragma unroll
         for (int x = 0; x < RT; ++x)
@@ -786,21 +789,21 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_rows_ke
 }
 
 // --------------------------------------------------------------------------- backward, a warp's own keys
-template <int W, int MAPS, bool BIAS, int RT>
-__global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_kernel(const PatchArgs a)
+template <int W, int MAPS, bool BIAS, int RT, int NT>
+__global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_cols_kernel(const PatchArgs a)
 {
     pdl_wait();
-    constexpr int CH = PmChunk<W, BIAS>::N;
+    constexpr int CH = PmChunk<W, BIAS, NT>::N;
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float part[4 * PM_WARPS];
+    __shared__ float part[4 * NT / 32];
     const PmPlace w = pm_place(a);
-    const int k0 = w.tile * PM_ROWS * RT, L = w.L;
+    const int k0 = w.tile * (NT / 2) * RT, L = w.L;
     const bool learns = BIAS && a.bins;
     float* bins = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * 3 * (2 * a.bnd + 1) : nullptr;
     if (k0 >= L) {
         if (learns)
-            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PM_THREADS) bins[i] = 0.f;
+            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += NT) bins[i] = 0.f;
         return;
     }
     const int t = threadIdx.x & 3, warp0 = k0 + (int)(threadIdx.x / 32) * 16 * RT;
@@ -809,8 +812,8 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     const int64_t stride = 3 * (int64_t)a.C;
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
-    if (BIAS) table = pa_table(a, w.seq, PA_BINS_BYTES, true);
-    PmStream<W, MAPS, true, BIAS> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
+    if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::BINS, true);
+    PmStream<W, MAPS, true, BIAS, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
                                         table.copies_log2 + 2, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);
@@ -824,15 +827,15 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     int point[RT][2][3];
     float unit = 0.f, per_unit = 0.f;
     if (BIAS) {
-        pa_load_table(a, table, w.h, tab, threadIdx.x, PM_THREADS);
+        pa_load_table(a, table, w.h, tab, threadIdx.x, NT);
         pm_bias_setup(table, smem_u32(tab), bias);
 #pragma unroll
         for (int x = 0; x < RT; ++x)
 #pragma unroll
             for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], -1, point[x][r]);
         if (learns) {
-            for (int i = threadIdx.x; i < table.entries << table.bins_log2; i += PM_THREADS) hist[i] = 0;
-            for (int i = threadIdx.x; i < table.entries; i += PM_THREADS) sums[i] = 0.f;
+            for (int i = threadIdx.x; i < table.entries << table.bins_log2; i += NT) hist[i] = 0;
+            for (int i = threadIdx.x; i < table.entries; i += NT) sums[i] = 0.f;
         }
     }
     uint32_t kf[RT][W / 16][4], vf[RT][W / 16][4];
@@ -863,9 +866,9 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
             if (learns && i % (PM_WINDOW / CH) == 0) {
                 if (i) {
                     __syncthreads();
-                    pa_flush(table, hist, sums, unit, PM_THREADS);
+                    pa_flush(table, hist, sums, unit, NT);
                 }
-                unit = pa_unit<PM_WARPS, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
+                unit = pa_unit<NT / 32, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
                 per_unit = pa_per_unit(unit);
             }
             const unsigned char* st = in.next(i);
@@ -937,9 +940,9 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
     else walk(PmNo());
     in.end();
     if (learns) {
-        pa_flush(table, hist, sums, unit, PM_THREADS);
+        pa_flush(table, hist, sums, unit, NT);
         __syncthreads();
-        pa_store_bins(a, table, sums, bins, PM_THREADS);
+        pa_store_bins(a, table, sums, bins, NT);
     }
 #pragma unroll
     for (int x = 0; x < RT; ++x)
@@ -965,28 +968,50 @@ __global__ void __launch_bounds__(PM_THREADS, W == 64 ? 1 : 2) patch_mma_cols_ke
         }
 }
 
-template <typename K>
+template <int NT, typename K>
 static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 {
     const cudaError_t err = allow_smem(kern);
     PTV3_REQUIRE(err == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention: %s", cudaGetErrorString(err));
-    launch_dependent(kern, dim3((unsigned)((int64_t)a.n_seq * a.tiles * a.H)), dim3(PM_THREADS), smem, stream, a);
+    launch_dependent(kern, dim3((unsigned)((int64_t)a.n_seq * a.tiles * a.H)), dim3(NT), smem, stream, a);
     count_launches(1);
     return check_launch("ptv3_patch_attention");
 }
 
-// Rows of a block, in tiles of 128: with two tiles to a warp what it reads of the other side serves twice the rows, where
-// registers allow it (heads of 16), patches fill such blocks and launches are long.  us with one and with two: forward with a bias, 120 000 x 64, 489 and
-// 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of two maps 347 and 320.  Not so forward and rows
-// without a bias (312 and 326, 341 and 465).
-static int row_tiles(int64_t n_seq, int64_t longest, int heads, int width, int maps, bool bias, int pass)
+// What a block is.  Eight warps of a row tile each; two tiles to a warp, so that what it reads of the other side serves twice the
+// rows, where registers allow it (heads of 16), patches fill such blocks and launches are long.  us with one and with two:
+// forward with a bias, 120 000 x 64, 489 and 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of
+// two maps 347 and 320; not so forward and rows without a bias (312 and 326, 341 and 465).  Four warps where patches are short
+// (60 000 x 64 in patches of 48, two maps, the three passes: 62, 70 and 74 us with eight, 34, 38 and 36) or blocks without a bias
+// few (1 560 x 256 forward 33 and 27.5; with a bias, 6 760 x 128, 68 and 72).
+struct PmForm {
+    int threads, tiles;      // tiles of a warp
+    int rows() const { return threads / 2 * tiles; }
+};
+static PmForm block_form(int64_t n_seq, int64_t longest, int heads, int width, int maps, bool bias, int pass)
 {
-    const int64_t blocks = n_seq * heads * ((longest + 2 * PM_ROWS - 1) / (2 * PM_ROWS));
-    return width == 16 && longest >= 2 * PM_ROWS && blocks >= 2 * SMS && (bias || (maps == 2 && pass == PA_COLS)) ? 2 : 1;
+    auto blocks = [&](int rows) { return n_seq * heads * ((longest + rows - 1) / rows); };
+    if (longest <= 64 || (!bias && blocks(128) < 2 * SMS)) return PmForm{128, 1};
+    const bool two = width == 16 && longest >= 256 && blocks(256) >= 2 * SMS && (bias || (maps == 2 && pass == PA_COLS));
+    return PmForm{256, two ? 2 : 1};
 }
 int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width)
 {
-    return PM_ROWS * row_tiles(n_seq, longest, heads, width, 1, true, PA_COLS);
+    return block_form(n_seq, longest, heads, width, 1, true, PA_COLS).rows();
+}
+
+template <int W, int MAPS, bool BIAS, int RT, int NT>
+static int launch_block(const PatchArgs& a, int pass, cudaStream_t stream)
+{
+    const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS, NT>::N>::BYTES;
+    const size_t smem = stages + (BIAS ? PmTableBytes<NT>::TABLE : 0);
+    constexpr int ROWS2 = BIAS ? RT : 1;      // (two tiles to a warp: columns alone without a bias)
+    if (pass == PA_ROWS) return launch<NT>(patch_mma_rows_kernel<W, MAPS, BIAS, ROWS2, NT>, a, smem, stream);
+    if (pass == PA_COLS)      // the table, its bins, and their sums
+        return launch<NT>(patch_mma_cols_kernel<W, MAPS, BIAS, RT, NT>, a,
+                          stages + (BIAS ? PmTableBytes<NT>::BINS + pm_sums_bytes(a.bnd, PmTableBytes<NT>::BINS) : 0), stream);
+    return a.lse ? launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, true, ROWS2, NT>, a, smem, stream)
+                 : launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, false, ROWS2, NT>, a, smem, stream);
 }
 
 template <int W, int MAPS, bool BIAS>
@@ -994,23 +1019,12 @@ static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
 {
     PatchArgs a = args;
     const int longest = a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad;
-    const int rt = row_tiles(a.n_seq, longest, a.H, W, MAPS, BIAS, pass);
-    a.tiles = ceil_div(longest, rt * PM_ROWS);
-    constexpr int TWO = W == 16 && BIAS ? 2 : 1, COLS2 = W == 16 && (MAPS == 2 || BIAS) ? 2 : 1;
-    const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS>::N>::BYTES, smem = stages + (BIAS ? PA_TABLE_BYTES : 0);
-    if (pass == PA_ROWS)
-        return rt == 2 ? launch(patch_mma_rows_kernel<W, MAPS, BIAS, TWO>, a, smem, stream)
-                       : launch(patch_mma_rows_kernel<W, MAPS, BIAS, 1>, a, smem, stream);
-    if (pass == PA_COLS) {      // the table, its bins, and their sums
-        const size_t with_bins = stages + (BIAS ? PA_BINS_BYTES + pm_sums_bytes(a.bnd) : 0);
-        return rt == 2 ? launch(patch_mma_cols_kernel<W, MAPS, BIAS, COLS2>, a, with_bins, stream)
-                       : launch(patch_mma_cols_kernel<W, MAPS, BIAS, 1>, a, with_bins, stream);
-    }
-    if (a.lse)
-        return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, TWO>, a, smem, stream)
-                       : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, true, 1>, a, smem, stream);
-    return rt == 2 ? launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, TWO>, a, smem, stream)
-                   : launch(patch_mma_fwd_kernel<W, MAPS, BIAS, false, 1>, a, smem, stream);
+    const PmForm form = block_form(a.n_seq, longest, a.H, W, MAPS, BIAS, pass);
+    a.tiles = ceil_div(longest, form.rows());
+    constexpr int RT = W == 16 && (BIAS || MAPS == 2) ? 2 : 1;
+    if (form.threads == 128) return launch_block<W, MAPS, BIAS, 1, 128>(a, pass, stream);
+    return form.tiles == 2 ? launch_block<W, MAPS, BIAS, RT, 256>(a, pass, stream)
+                           : launch_block<W, MAPS, BIAS, 1, 256>(a, pass, stream);
 }
 
 template <int W>

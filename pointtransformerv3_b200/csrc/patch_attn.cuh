@@ -15,7 +15,7 @@
 // delta in one walk: the stored result gives an estimate, delta' = dO . O (dO . O2 for the second map, whose O2 the
 // forward pass leaves too), which is off by the rounding of O alone.  With E = sum_j P (G - delta'),
 // delta = delta' + E and dQ = sum_j P (G - delta') K - E sum_j P K, exact however far the values' mean is from zero and
-// however peaked a row is.  (A walk of its own for delta: 632 us for the differential rows of 100 000 x 64 where this takes 376.)
+// however peaked a row is.  (A walk of its own for delta: 632 us for the differential rows of 100 000 x 64 where one walk took 376.)
 //
 // dtable: a pair adds its dS to three bins, as integers in shared memory, since integer sums do not depend on the order
 // of the additions.  Their unit follows from what the queries of a window can add at most, sum_j |dS_ij| <= sum_j P |G -
@@ -135,9 +135,9 @@ __device__ __forceinline__ void pa_load_table(const PatchArgs& a, const PatchTab
     }
 }
 // What the queries [q0, q0 + WINDOW) of a sequence can add to a bin at most, as a unit in which 2^30 of it are that.
-// With QUADS lane t of four adds queries 2 t and 2 t + 1 of every eight, to copies of its own where there are four and
+// Lane t of four adds queries 2 t and 2 t + 1 of every eight, to copies of its own where there are four and
 // more: the largest of four sums.  All threads of a block of 32 `WARPS`; `part`: WARPS x 4 floats
-template <int WARPS, int WINDOW, bool QUADS>
+template <int WARPS, int WINDOW>
 __device__ __forceinline__ float pa_unit(const PatchArgs& a, const PatchTable& table, int h, int start, int L, int q0,
                                          float* part)
 {
@@ -158,7 +158,7 @@ __device__ __forceinline__ float pa_unit(const PatchArgs& a, const PatchTable& t
         top = fmaxf(top, sum);
         all += sum;                        // (a NaN among them is kept by this one)
     }
-    return (QUADS && table.bins_log2 >= 2 && all == all ? top : all) * (1.f / 1073741824.f);
+    return (table.bins_log2 >= 2 && all == all ? top : all) * (1.f / 1073741824.f);
 }
 __device__ __forceinline__ float pa_per_unit(float unit)
 {

@@ -1,122 +1,190 @@
 // Patch attention with bias or of two maps, forward and backward, in fp32 arithmetic on CUDA cores (patch_attn.cuh
-// has the mathematics): a thread owns a query (or, in the pass over columns, a key), the other side comes through shared memory
-// in chunks that all threads read at the same address.  Heads of 64 are shared by two neighbouring threads, so that
-// accumulators stay in registers.
+// has the mathematics): a thread owns a query (or, in the pass over columns, a key), the other side streams through shared
+// memory in chunks that all threads read at the same address, gathered by cp.async a chunk ahead.  Heads of 64 are shared by two
+// neighbouring threads, so that accumulators stay in registers.
+#include <type_traits>
+
 #include "patch_attn.cuh"
 #include "mma_util.cuh"
 
 namespace ptv3 {
 
-constexpr int PF_THREADS = 128;
-constexpr int PF_CHUNK = 64;      // rows of the other side in shared memory
-constexpr int PF_STEP = 8;        // of which scores are held at a time
+constexpr int PF_STEP = 8;        // keys whose scores are held at a time
 constexpr int PF_WINDOW = 8;      // queries between two clearings of the bins: the unit is that much finer (gradient of a
                                   // table, patches of 1 024, off by 4e-6 of its norm with 32, 6e-7 with 8)
 constexpr int PF_BINS_LOG2 = 4;   // 16 copies of them, so that clearing costs little
 constexpr int PF_TABLE_BYTES = 32 * 1024, PF_BINS_BYTES = 48 * 1024;      // for the table; for the table and its bins
 
+constexpr int PF_THREADS = 128;
+
+// A thread has a row, or half of one of 64 values.  (Two rows to a thread halve its reads of shared memory and leave too few
+// threads: 20 000 x 64 in heads of 16, forward, rows and columns 320, 298 and 400 us instead of 268, 265 and 334.  Two threads to a
+// row of 16: 291, 337 and 436.)
 template <int W, int MAPS>
 struct PfShape {
     static constexpr int SPLIT = W == 64 ? 2 : 1;      // threads to a row
     static constexpr int ROWS = PF_THREADS / SPLIT;
+    static constexpr int CHUNK = W == 16 ? 64 : 32;    // rows of the other side in a stage of shared memory
     static constexpr int D = W / MAPS;                 // of a map's queries and keys
-    static constexpr int DP = D / SPLIT, WP = W / SPLIT;
+    static constexpr int DP = D / SPLIT, WP = W / SPLIT, NP = WP / 2;
+    // axes of the bias that a thread looks up: two threads of a row share them, their sums meet in the score's
+    static constexpr int AXES = SPLIT == 1 ? 3 : 2;
 };
 
-// value i of this thread's share of a row of queries or keys: map-major, the share of a map contiguous
+// value i of this thread's share of a row of queries or keys: map-major, of a map every SPLIT-th four values
 template <int W, int MAPS>
 __device__ __forceinline__ constexpr int pf_dim(int i, int part)
 {
     using S = PfShape<W, MAPS>;
-    return (i / S::DP) * S::D + part * S::DP + i % S::DP;
+    const int m = i / S::DP, k = i % S::DP;
+    return m * S::D + (k / 4 * S::SPLIT + part) * 4 + k % 4;
 }
 
-// A chunk of rows in shared memory: x (queries or keys) and y (values or gradients of the result), grid coordinates
-template <int W>
-__device__ __forceinline__ void pf_stage(const PatchArgs& a, const float* x, int64_t x_stride, const float* y, int64_t y_stride,
-                                         bool owners, int start, int nk, float (*xs)[W], float (*ys)[W], int (*gs)[4])
+// Two stages of the other side: x (queries or keys) and y (values or gradients of the result), grid coordinates, and of every
+// query and map its reference value, its coefficient over the sum, and delta
+template <int W, int MAPS, bool BIAS, bool COLS>
+struct PfStages {
+    using S = PfShape<W, MAPS>;
+    static constexpr int N = S::CHUNK;
+    float x[2][N][W], y[2][N][W];
+    int4 g[2][BIAS ? N : 1];
+    float4 aux[2][COLS ? MAPS : 1][COLS ? N : 1];
+    float unit[2][COLS && BIAS ? N / PF_WINDOW : 1];
+};
+
+// rows [c0, c0 + nk) of a sequence into a stage; matrices arrive behind cp_async_wait
+template <int W, int MAPS, bool BIAS, bool COLS>
+__device__ __forceinline__ void pf_stage(const PatchArgs& a, PfStages<W, MAPS, BIAS, COLS>& st, int k, const float* x, int64_t xs,
+                                         const float* y, int64_t ys, int start, int c0, int L, int h, const float (&coef)[MAPS])
 {
-    for (int i = threadIdx.x; i < nk * W; i += PF_THREADS) {
-        const int j = i / W, d = i % W;
-        const int e = a.rows[start + j];
+    using S = PfShape<W, MAPS>;
+    const int nk = min(S::CHUNK, L - c0);
+    constexpr int C4 = W / 4;
+    for (int i = threadIdx.x; i < nk * C4; i += PF_THREADS) {
+        const int j = i / C4, d = i % C4 * 4;
+        const int e = a.rows[start + c0 + j];
         const int64_t p = e >= 0 ? e : -(e + 1);
-        xs[j][d] = (x[p * x_stride + d]);
-        ys[j][d] = owners && e < 0 ? 0.f : (y[p * y_stride + d]);
+        cp_async16(smem_u32(&st.x[k][j][d]), x + p * xs + d);
+        cp_async16_zfill(smem_u32(&st.y[k][j][d]), y + p * ys + d, !COLS || e >= 0);
     }
-    if (gs)
-        for (int i = threadIdx.x; i < nk * 3; i += PF_THREADS) {
-            const int j = i / 3, e = a.rows[start + j];
-            gs[j][i % 3] = pa_coord(a, e >= 0 ? e : -(e + 1), i % 3);
+    cp_async_commit();
+    if (BIAS)
+        for (int j = threadIdx.x; j < nk; j += PF_THREADS) {
+            const int e = a.rows[start + c0 + j];
+            const int64_t p = e >= 0 ? e : -(e + 1);
+            st.g[k][j] = make_int4(pa_coord(a, p, 0), pa_coord(a, p, 1), pa_coord(a, p, 2), 0);
         }
-}
-
-// places of the three look-ups of a pair (d: coordinates of the query minus those of the key)
-__device__ __forceinline__ void pf_places(const PatchTable& t, int dx, int dy, int dz, int copy, int (&at)[3])
-{
-    const int d[3] = {dx, dy, dz};
+    if (COLS) {
+        for (int i = threadIdx.x; i < nk * MAPS; i += PF_THREADS) {
+            const int m = i / nk, j = i % nk;
+            const int64_t at = (int64_t)(h * MAPS + m) * a.n_pad + start + c0 + j;
+            // a row that answers for no point has no gradient: its probabilities are taken as nothing
+            const bool own = a.rows[start + c0 + j] >= 0;
+            st.aux[k][m][j] = make_float4(own ? a.lse[at] : INFINITY,
+                                          own ? a.lse[at + (int64_t)a.H * MAPS * a.n_pad] * coef[m] : 0.f, a.delta[at], 0.f);
+        }
+        if (BIAS && a.bins && threadIdx.x < S::CHUNK) {
+            // what the queries of a window can add to a bin at most is 2^31 units, less what rounding may add
+            float r = threadIdx.x < nk ? a.reach[(int64_t)h * a.n_pad + start + c0 + threadIdx.x] : 0.f;
 #pragma unroll
-    for (int c = 0; c < 3; ++c)
-        at[c] = ((min(max(d[c], -t.reach[c]), t.reach[c]) + t.reach[c] + t.first[c]) << t.copies_log2) + copy;
+            for (int d = 1; d < PF_WINDOW; d <<= 1) r += __shfl_xor_sync(0xffffffffu, r, d);
+            if (threadIdx.x % PF_WINDOW == 0) st.unit[k][threadIdx.x / PF_WINDOW] = r * (1.f / 2147000000.f);
+        }
+    }
 }
 
-// A thread's share of a row as packed pairs: half the multiply-adds to issue (20 011 x 64, differential, fp32: forward 127 us with
-// single ones, rows 133, columns 205; 111, 112 and 169 so).
+// This thread's look-ups: places in shared memory and clamped reach of its axes, coordinates of its rows along them
+template <int W, int MAPS>
+struct PfBias {
+    using S = PfShape<W, MAPS>;
+    int axis[S::AXES], reach[S::AXES], base[S::AXES], g[S::AXES], log2;
+    bool idle;          // the last axis is none: of two threads the second has one axis
+    __device__ __forceinline__ void set(const PatchTable& t, int part)
+    {
+        log2 = t.copies_log2;
+        idle = part == 1;
+#pragma unroll
+        for (int i = 0; i < S::AXES; ++i) {
+            const int c = part ? 2 : i;
+            axis[i] = c;
+            reach[i] = c == 0 ? t.reach[0] : c == 1 ? t.reach[1] : t.reach[2];
+            const int first = c == 0 ? t.first[0] : c == 1 ? t.first[1] : t.first[2];
+            base[i] = ((reach[i] + first) << log2) + (threadIdx.x & ((1 << log2) - 1));
+        }
+    }
+    // places for the pair of this thread's row and a row of the other side; s: 1 where the own row is the query, or -1
+    __device__ __forceinline__ void places(const int4& other, int s, int (&at)[S::AXES]) const
+    {
+#pragma unroll
+        for (int i = 0; i < S::AXES; ++i) {
+            const int o = S::SPLIT == 1 ? (i == 0 ? other.x : i == 1 ? other.y : other.z) : ((const int*)&other)[axis[i]];
+            const int d = s * (g[i] - o);
+            at[i] = (min(max(d, -reach[i]), reach[i]) << log2) + base[i];
+        }
+    }
+    __device__ __forceinline__ float look(const float* tab, const int (&at)[S::AXES]) const
+    {
+        if (S::AXES == 3) return tab[at[0]] + (tab[at[1]] + tab[at[2]]);
+        return tab[at[0]] + (idle ? 0.f : tab[at[1]]);
+    }
+};
+
+// A thread's share of a row as packed pairs: half the multiply-adds to issue.
+template <int SPLIT, int N>
+__device__ __forceinline__ void pf_load(uint64_t (&v)[N], const float* row, int part)
+{
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const ulonglong2 p = *(const ulonglong2*)(row + (i * SPLIT + part) * 4);
+        v[2 * i] = p.x;
+        v[2 * i + 1] = p.y;
+    }
+}
 template <int N>
-__device__ __forceinline__ uint64_t pf_sum(const uint64_t (&x)[N], int first, const float* y, int n)
+__device__ __forceinline__ float pf_dot(const uint64_t (&x)[N], const uint64_t (&y)[N], int first, int n)
 {
     uint64_t v = 0;
-    const ulonglong2* y2 = (const ulonglong2*)y;
 #pragma unroll
-    for (int i = 0; i < n / 4; ++i) {
-        const ulonglong2 p = y2[i];
-        v = fma2(x[first + 2 * i], p.x, fma2(x[first + 2 * i + 1], p.y, v));
-    }
+    for (int i = 0; i < n; ++i) v = fma2(x[first + i], y[first + i], v);
+    return hsum2(v);
+}
+template <int SPLIT>
+__device__ __forceinline__ float pf_meet(float v)      // sum over the threads of a row
+{
+#pragma unroll
+    for (int d = 1; d < SPLIT; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-template <int W, int MAPS>
-__device__ __forceinline__ void pf_scores(const uint64_t (&q)[PfShape<W, MAPS>::WP / 2], const float* k, int part,
-                                          float (&s)[MAPS])
-{
-    using S = PfShape<W, MAPS>;
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-        float v = hsum2(pf_sum(q, m * S::DP / 2, k + m * S::D + part * S::DP, S::DP));
-        if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
-        s[m] = v;
-    }
-}
-template <int W, int MAPS>
-__device__ __forceinline__ float pf_dot(const uint64_t (&x)[PfShape<W, MAPS>::WP / 2], const float* y, int part)
-{
-    using S = PfShape<W, MAPS>;
-    float v = hsum2(pf_sum(x, 0, y + part * S::WP, S::WP));
-    if (S::SPLIT == 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
-    return v;
-}
-// acc[first ..] += f y over n values
+// acc[first ..] += f y[first ..] over n pairs
 template <int N>
-__device__ __forceinline__ void pf_add(uint64_t (&acc)[N], int first, float f, const float* y, int n)
+__device__ __forceinline__ void pf_add(uint64_t (&acc)[N], int first, float f, const uint64_t (&y)[N], int n)
 {
     const uint64_t f2 = pack2(f, f);
-    const ulonglong2* y2 = (const ulonglong2*)y;
 #pragma unroll
-    for (int i = 0; i < n / 4; ++i) {
-        const ulonglong2 p = y2[i];
-        acc[first + 2 * i] = fma2(f2, p.x, acc[first + 2 * i]);
-        acc[first + 2 * i + 1] = fma2(f2, p.y, acc[first + 2 * i + 1]);
+    for (int i = 0; i < n; ++i) acc[first + i] = fma2(f2, y[first + i], acc[first + i]);
+}
+// acc = fix acc + sum of f[j][k] times row j over a step: in a sum of its own first, so that rounding grows with the number of
+// steps and not of rows (differential result over patches of 1 024: 1.4e-6 of its norm otherwise, in the same time)
+template <int SPLIT, int N, int F>
+__device__ __forceinline__ void pf_step_add(uint64_t (&acc)[N], float fix, const float (&f)[PF_STEP][F], int k,
+                                            const float* const (&rows)[PF_STEP], int part)
+{
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+        uint64_t t[4];
+#pragma unroll
+        for (int j = 0; j < PF_STEP; ++j) {
+            const uint64_t f2 = pack2(f[j][k], f[j][k]);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const ulonglong2 y = *(const ulonglong2*)(rows[j] + ((c + i) / 2 * SPLIT + part) * 4);
+                t[i] = j ? fma2(f2, y.x, t[i]) : mul2(f2, y.x);
+                t[i + 1] = j ? fma2(f2, y.y, t[i + 1]) : mul2(f2, y.y);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[c + i] = fma2(acc[c + i], pack2(fix, fix), t[i]);
     }
-}
-// pair i of a share of a row of queries or keys, and that of a contiguous share
-template <int W, int MAPS>
-__device__ __forceinline__ uint64_t pf_pair(const float* row, int i, int part)
-{
-    const float2 v = *(const float2*)(row + pf_dim<W, MAPS>(2 * i, part));
-    return pack2(v.x, v.y);
-}
-__device__ __forceinline__ uint64_t pf_pair(const float* share, int i)
-{
-    const float2 v = ((const float2*)share)[i];
-    return pack2(v.x, v.y);
 }
 __device__ __forceinline__ void pf_put(float* to, uint64_t v, float f)
 {
@@ -131,8 +199,8 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ __align__(16) float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
-    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
+    constexpr int NP = S::NP, HP = S::DP / 2;
+    __shared__ __align__(16) PfStages<W, MAPS, BIAS, false> st;
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
     const int part = threadIdx.x % S::SPLIT;
@@ -140,23 +208,25 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     const int L = pa_sequence(a, seq, start);
     const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
     if (q0 >= L) return;
-    PatchTable table = {};
-    if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
-        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
-    }
-    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
-    const int e = qi < L ? a.rows[start + qi] : -1;
-    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
+    const bool busy = q0 + threadIdx.x / 32 * 32 / S::SPLIT < L;          // (warps with no row at all only gather)
+    const int64_t stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;
-    constexpr int NP = S::WP / 2;
+    const float none[MAPS] = {};
+    pf_stage(a, st, 0, base + a.C, stride, base + 2 * a.C, stride, start, 0, L, h, none);
+    PfBias<W, MAPS> bias;
+    if (BIAS) {
+        const PatchTable table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
+        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
+        bias.set(table, part);
+    }
     uint64_t q[NP], acc[MAPS][NP];
     float m[MAPS], l[MAPS];
-    int g[3] = {0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < NP; ++i) q[i] = pf_pair<W, MAPS>(base + p * stride, i, part);
+    const int e = qi < L ? a.rows[start + qi] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1);
+    pf_load<S::SPLIT>(q, base + p * stride, part);
     if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
+#pragma unroll
+        for (int i = 0; i < S::AXES; ++i) bias.g[i] = pa_coord(a, p, bias.axis[i]);
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
         m[k] = -1e30f;          // (finite: scores may all be -inf)
@@ -165,54 +235,58 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
         for (int i = 0; i < NP; ++i) acc[k][i] = 0;
     }
     const float scale2 = a.scale * PA_LOG2E;
-    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
-        const int nk = min(PF_CHUNK, L - c0);
+    for (int c0 = 0, cur = 0; c0 < L; c0 += S::CHUNK, cur ^= 1) {
+        const int nk = min(S::CHUNK, L - c0);
+        cp_async_wait<0>();
         __syncthreads();
-        pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
-        __syncthreads();
-        for (int j0 = 0; j0 < nk; j0 += PF_STEP) {
-            float s[PF_STEP][MAPS], top[MAPS];
+        if (c0 + S::CHUNK < L)
+            pf_stage(a, st, cur ^ 1, base + a.C, stride, base + 2 * a.C, stride, start, c0 + S::CHUNK, L, h, none);
+        if (!busy) continue;
+        auto step = [&](int j0, auto whole) {
+            constexpr bool full = decltype(whole)::value;
+            float s[PF_STEP][MAPS], top[MAPS], sum[MAPS] = {};
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) top[k] = m[k];
 #pragma unroll
             for (int j = 0; j < PF_STEP; ++j) {
-                const int jj = min(j0 + j, nk - 1);
-                pf_scores<W, MAPS>(q, Ks[jj], part, s[j]);
-                if (BIAS) {
-                    int at[3];
-                    pf_places(table, g[0] - Gs[jj][0], g[1] - Gs[jj][1], g[2] - Gs[jj][2], copy, at);
-                    s[j][0] = fmaf(s[j][0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
-                }
+                const int jj = full ? j0 + j : min(j0 + j, nk - 1);
+                uint64_t key[NP];
+                pf_load<S::SPLIT>(key, st.x[cur][jj], part);
 #pragma unroll
                 for (int k = 0; k < MAPS; ++k) {
-                    if (j0 + j >= nk) s[j][k] = BIAS || scale2 > 0.f ? -INFINITY : INFINITY;
+                    float v = pf_dot(q, key, k * HP, HP);
+                    if (BIAS) {
+                        int at[S::AXES];
+                        bias.places(st.g[cur][jj], 1, at);
+                        v = fmaf(v, scale2, bias.look(tab, at));
+                    }
+                    s[j][k] = pf_meet<S::SPLIT>(v);
                     top[k] = fmaxf(top[k], BIAS ? s[j][k] : s[j][k] * scale2);
                 }
             }
+            const float* rows[PF_STEP];
+#pragma unroll
+            for (int j = 0; j < PF_STEP; ++j) rows[j] = st.y[cur][full ? j0 + j : min(j0 + j, nk - 1)];
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) {
                 const float fix = fast_exp2(m[k] - top[k]);
                 m[k] = top[k];
-                l[k] *= fix;
 #pragma unroll
-                for (int i = 0; i < NP; ++i) acc[k][i] = mul2(acc[k][i], pack2(fix, fix));
-            }
-            float sum[MAPS] = {};      // of a step's, so that rounding does not grow with every key
-#pragma unroll
-            for (int j = 0; j < PF_STEP; ++j) {
-                const int jj = min(j0 + j, nk - 1);
-#pragma unroll
-                for (int k = 0; k < MAPS; ++k) {
-                    const float pr = fast_exp2(BIAS ? s[j][k] - m[k] : fmaf(s[j][k], scale2, -m[k]));
-                    sum[k] += pr;
-                    pf_add(acc[k], 0, pr, &Vs[jj][part * S::WP], S::WP);
+                for (int j = 0; j < PF_STEP; ++j) {
+                    s[j][k] = fast_exp2(BIAS ? s[j][k] - m[k] : fmaf(s[j][k], scale2, -m[k]));
+                    if (!full && j0 + j >= nk) s[j][k] = 0.f;
+                    sum[k] += s[j][k];
                 }
+                l[k] = fmaf(l[k], fix, sum[k]);
+                pf_step_add<S::SPLIT>(acc[k], fix, s, k, rows, part);
             }
-#pragma unroll
-            for (int k = 0; k < MAPS; ++k) l[k] += sum[k];
-        }
+        };
+        int j0 = 0;
+        for (; j0 + PF_STEP <= nk; j0 += PF_STEP) step(j0, std::true_type());
+        if (j0 < nk) step(j0, std::false_type());
     }
     if (e < 0) return;
+    const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
     if (a.lse && part == 0)
 #pragma unroll
         for (int k = 0; k < MAPS; ++k) {
@@ -220,23 +294,18 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
             *to = m[k];
             to[(int64_t)a.H * MAPS * a.n_pad] = 1.f / l[k];
         }
-    const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
-    const float w0 = 1.f / l[0], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
-    float* op = (float*)a.out + p * a.C + h * W + part * S::WP;
+    const float w0 = 1.f / l[0], w2 = 1.f / l[MAPS - 1], w1 = MAPS == 2 ? lam / l[MAPS - 1] : 0.f;
+    const int64_t own = (int64_t)e * a.C + h * W;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
+        const int d = pf_dim<W, 1>(2 * i, part);
         const uint64_t v = mul2(acc[0][i], pack2(w0, w0));
-        pf_put(op + 2 * i, MAPS == 2 ? fma2(acc[MAPS - 1][i], pack2(-w1, -w1), v) : v, 1.f);
-    }
-    if (MAPS == 2 && a.lse) {
-        const float w2 = 1.f / l[MAPS - 1];
-        float* o2 = (float*)a.second + p * a.C + h * W + part * S::WP;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) pf_put(o2 + 2 * i, acc[MAPS - 1][i], w2);
+        pf_put((float*)a.out + own + d, MAPS == 2 ? fma2(acc[MAPS - 1][i], pack2(-w1, -w1), v) : v, 1.f);
+        if (MAPS == 2 && a.lse) pf_put((float*)a.second + own + d, acc[MAPS - 1][i], w2);
     }
 }
 
-// ------------------------------------------------------------------------- backward, a thread's own query
+// ------------------------------------------------------------------------- backward, a thread's own queries
 // (in fp32 the stored results give delta as close as dQ needs it, and the softmax's sum is kept as such.  What is left, the
 // sum of P (G - delta), goes into the delta that the columns read: the same error for all of a row's keys adds up
 // in the table's gradient, 2e-6 of its norm with patches of 1 024 without this.)
@@ -245,8 +314,8 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ __align__(16) float Ks[PF_CHUNK][W], Vs[PF_CHUNK][W];
-    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
+    constexpr int NP = S::NP, HP = S::DP / 2;
+    __shared__ __align__(16) PfStages<W, MAPS, BIAS, false> st;
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
     const int part = threadIdx.x % S::SPLIT;
@@ -254,94 +323,105 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_rows_kernel(const PatchA
     const int L = pa_sequence(a, seq, start);
     const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / S::SPLIT;
     if (q0 >= L) return;
-    PatchTable table = {};
-    if (BIAS) {
-        table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
-        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
-    }
-    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
-    const int e = qi < L ? a.rows[start + qi] : -1;
-    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C, all = (int64_t)a.H * MAPS * a.n_pad;
+    const bool busy = q0 + threadIdx.x / 32 * 32 / S::SPLIT < L;
+    const int64_t stride = 3 * (int64_t)a.C, all = (int64_t)a.H * MAPS * a.n_pad;
     const float* base = (const float*)a.qkv + h * W;
-    const int64_t own = p * a.C + h * W + part * S::WP;        // this thread's share of a row of C
-    constexpr int NP = S::WP / 2;
-    uint64_t q[NP], go[NP], dq[NP], sum1 = 0, sum2 = 0;
-    float ref[MAPS], by[MAPS], delta[MAPS], left[MAPS] = {}, reach = 0.f;
-    int g[3] = {0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        q[i] = pf_pair<W, MAPS>(base + p * stride, i, part);
-        go[i] = e >= 0 ? pf_pair((const float*)a.dout + own, i) : 0;
-        sum1 = fma2(go[i], e >= 0 ? pf_pair((const float*)a.out + own, i) : 0, sum1);
-        if (MAPS == 2) sum2 = fma2(go[i], e >= 0 ? pf_pair((const float*)a.second + own, i) : 0, sum2);
-        dq[i] = 0;
+    const float none[MAPS] = {};
+    pf_stage(a, st, 0, base + a.C, stride, base + 2 * a.C, stride, start, 0, L, h, none);
+    PfBias<W, MAPS> bias;
+    if (BIAS) {
+        const PatchTable table = pa_table(a, seq, PF_TABLE_BYTES, false, false);
+        pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
+        bias.set(table, part);
     }
-    float d1 = hsum2(sum1), d2 = hsum2(sum2);
-    if (S::SPLIT == 2) {
-        d1 += __shfl_xor_sync(0xffffffffu, d1, 1);
-        d2 += __shfl_xor_sync(0xffffffffu, d2, 1);
-    }
-    if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
     const float lam = MAPS == 2 ? pa_param(a.lam, h, a.lam_bf16) : 0.f;
+    uint64_t q[NP], go[NP], dq[NP];
+    float ref[MAPS], delta[MAPS], left[MAPS] = {}, reach = 0.f;
+    int e = qi < L ? a.rows[start + qi] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1);
+    pf_load<S::SPLIT>(q, base + p * stride, part);
+    float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) go[i] = dq[i] = 0;
+    if (e >= 0) {
+        uint64_t o[NP];
+        pf_load<S::SPLIT>(go, (const float*)a.dout + p * a.C + h * W, part);
+        pf_load<S::SPLIT>(o, (const float*)a.out + p * a.C + h * W, part);
+        d1 = pf_dot(go, o, 0, NP);
+        if (MAPS == 2) {
+            pf_load<S::SPLIT>(o, (const float*)a.second + p * a.C + h * W, part);
+            d2 = pf_dot(go, o, 0, NP);
+        }
+    }
+    d1 = pf_meet<S::SPLIT>(d1);
+    if (MAPS == 2) d2 = pf_meet<S::SPLIT>(d2);
     delta[0] = MAPS == 2 ? fmaf(lam, d2, d1) : d1;
     if (MAPS == 2) delta[MAPS - 1] = d2;
+    if (BIAS)
 #pragma unroll
-    for (int k = 0; k < MAPS; ++k) {
-        const int64_t at = (int64_t)(h * MAPS + k) * a.n_pad + start + qi;
+        for (int i = 0; i < S::AXES; ++i) bias.g[i] = pa_coord(a, p, bias.axis[i]);
+#pragma unroll
+    for (int k = 0; k < MAPS; ++k)
         // a row that answers for no point has no gradient: its probabilities are taken as nothing
-        ref[k] = e >= 0 ? a.lse[at] : INFINITY;
-        by[k] = e >= 0 ? a.lse[at + all] : 0.f;
-    }
+        ref[k] = e >= 0 ? a.lse[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] : INFINITY;
     const float scale2 = a.scale * PA_LOG2E;
-    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
-        const int nk = min(PF_CHUNK, L - c0);
+    for (int c0 = 0, cur = 0; c0 < L; c0 += S::CHUNK, cur ^= 1) {
+        const int nk = min(S::CHUNK, L - c0);
+        cp_async_wait<0>();
         __syncthreads();
-        pf_stage<W>(a, base + a.C, stride, base + 2 * a.C, stride, false, start + c0, nk, Ks, Vs, BIAS ? Gs : nullptr);
-        __syncthreads();
-#pragma unroll 4
+        if (c0 + S::CHUNK < L)
+            pf_stage(a, st, cur ^ 1, base + a.C, stride, base + 2 * a.C, stride, start, c0 + S::CHUNK, L, h, none);
+        if (!busy) continue;
+#pragma unroll (W == 16 ? 2 : 1)
         for (int j = 0; j < nk; ++j) {
-            float s[MAPS];
-            pf_scores<W, MAPS>(q, Ks[j], part, s);
-            if (BIAS) {
-                int at[3];
-                pf_places(table, g[0] - Gs[j][0], g[1] - Gs[j][1], g[2] - Gs[j][2], copy, at);
-                s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
-            }
-            const float G = pf_dot<W, MAPS>(go, Vs[j], part);
+            uint64_t key[NP], val[NP];
+            pf_load<S::SPLIT>(key, st.x[cur][j], part);
+            pf_load<S::SPLIT>(val, st.y[cur][j], part);
+            const float G = pf_meet<S::SPLIT>(pf_dot(go, val, 0, NP));
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) {
-                const float ds = fast_exp2(BIAS ? s[k] - ref[k] : fmaf(s[k], scale2, -ref[k])) * (G - delta[k]);
+                float s = pf_dot(q, key, k * HP, HP);
+                if (BIAS) {
+                    int at[S::AXES];
+                    bias.places(st.g[cur][j], 1, at);
+                    s = fmaf(s, scale2, bias.look(tab, at));
+                }
+                s = pf_meet<S::SPLIT>(s);
+                const float ds = fast_exp2(BIAS ? s - ref[k] : fmaf(s, scale2, -ref[k])) * (G - delta[k]);
                 left[k] += ds;
                 if (BIAS) reach += fabsf(ds);
-                pf_add(dq, k * S::DP / 2, ds, &Ks[j][k * S::D + part * S::DP], S::DP);
+                pf_add(dq, k * HP, ds, key, HP);
             }
         }
     }
-    if (qi < L && part == 0) {
+    if (qi >= L) return;
+    // (read again where registers decide how many CTAs an SM holds: 20 000 x 64 with a bias 358 -> 315 us)
+    if (W == 16) e = a.rows[start + qi];
+    float by[MAPS];
 #pragma unroll
-        for (int k = 0; k < MAPS; ++k)
-            a.delta[(int64_t)(h * MAPS + k) * a.n_pad + start + qi] = fmaf(left[k], by[k], delta[k]);
-        if (BIAS && a.reach) a.reach[(int64_t)h * a.n_pad + start + qi] = (reach + fabsf(left[0])) * by[0];
+    for (int k = 0; k < MAPS; ++k) {
+        const int64_t at = (int64_t)(h * MAPS + k) * a.n_pad + start + qi;
+        by[k] = e >= 0 ? a.lse[at + all] : 0.f;
+        if (part == 0) a.delta[at] = fmaf(left[k], by[k], delta[k]);
     }
+    if (BIAS && a.reach && part == 0)
+        a.reach[(int64_t)h * a.n_pad + start + qi] = (reach + fabsf(left[0])) * by[0];
     if (e < 0) return;
     by[0] *= a.scale;
     if (MAPS == 2) by[MAPS - 1] *= -lam * a.scale;
-    float* dst = (float*)a.dqkv + p * stride + h * W;
+    float* dst = (float*)a.dqkv + (int64_t)e * stride + h * W;
 #pragma unroll
     for (int i = 0; i < NP; ++i) pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dq[i], by[2 * i / S::DP]);
 }
 
-// --------------------------------------------------------------------------- backward, a thread's own key
+// --------------------------------------------------------------------------- backward, a thread's own keys
 template <int W, int MAPS, bool BIAS>
 __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchArgs a)
 {
     pdl_wait();
     using S = PfShape<W, MAPS>;
-    __shared__ __align__(16) float Qs[PF_CHUNK][W], Os[PF_CHUNK][W];
-    __shared__ int Gs[BIAS ? PF_CHUNK : 1][4];
-    // reference value, (-lam) / sum and delta of every query
-    __shared__ float Ms[MAPS][PF_CHUNK], Is[MAPS][PF_CHUNK], Ds[MAPS][PF_CHUNK], units[PF_CHUNK / PF_WINDOW];
+    constexpr int NP = S::NP, HP = S::DP / 2;
+    __shared__ __align__(16) PfStages<W, MAPS, BIAS, true> st;
     extern __shared__ float tab[];
     const int h = blockIdx.x % a.H, tile = blockIdx.x / a.H % a.tiles, seq = blockIdx.x / a.H / a.tiles;
     const int part = threadIdx.x % S::SPLIT;
@@ -355,12 +435,21 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
             for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PF_THREADS) bins[i] = 0.f;
         return;
     }
+    const bool busy = k0 + threadIdx.x / 32 * 32 / S::SPLIT < L;
+    const int64_t stride = 3 * (int64_t)a.C;
+    const float* base = (const float*)a.qkv + h * W;
+    const float* dout = (const float*)a.dout + h * W;
+    float coef[MAPS];
+    coef[0] = 1.f;
+    if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
+    pf_stage(a, st, 0, base, stride, dout, a.C, start, 0, L, h, coef);
     PatchTable table = {};
+    PfBias<W, MAPS> bias;
     if (BIAS) {
         table = pa_table(a, seq, PF_BINS_BYTES, true, false, PF_BINS_LOG2);
         pa_load_table(a, table, h, tab, threadIdx.x, PF_THREADS);
+        bias.set(table, part);
     }
-    const int copy = threadIdx.x & ((1 << table.copies_log2) - 1);
     const int fewer = table.copies_log2 - table.bins_log2;      // (0 or 1) copies of the bins than of the table
     int* hist = (int*)tab + (BIAS ? table.entries << table.copies_log2 : 0);
     float* sums = (float*)hist + (BIAS ? table.entries << table.bins_log2 : 0);
@@ -369,44 +458,22 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
         for (int i = threadIdx.x; i < table.entries; i += PF_THREADS) sums[i] = 0.f;
     }
     float unit = 0.f, per_unit = 0.f;
-    const int e = kj < L ? a.rows[start + kj] : -1;
-    const int64_t p = e >= 0 ? e : -(e + 1), stride = 3 * (int64_t)a.C;
-    const float* base = (const float*)a.qkv + h * W;
-    constexpr int NP = S::WP / 2;
     uint64_t k[NP], v[NP], dk[NP], dv[NP];
-    float coef[MAPS];
-    int g[3] = {0, 0, 0};
+    const int e = kj < L ? a.rows[start + kj] : -1;
+    const int64_t p = e >= 0 ? e : -(e + 1);
+    pf_load<S::SPLIT>(k, base + p * stride + a.C, part);
+    pf_load<S::SPLIT>(v, base + p * stride + 2 * a.C, part);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        k[i] = pf_pair<W, MAPS>(base + p * stride + a.C, i, part);
-        v[i] = pf_pair(base + p * stride + 2 * a.C + part * S::WP, i);
-        dk[i] = dv[i] = 0;
-    }
+    for (int i = 0; i < NP; ++i) dk[i] = dv[i] = 0;
     if (BIAS)
-        for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
-    coef[0] = 1.f;
-    if (MAPS == 2) coef[MAPS - 1] = -pa_param(a.lam, h, a.lam_bf16);
-    const float scale2 = a.scale * PA_LOG2E;
-    for (int c0 = 0; c0 < L; c0 += PF_CHUNK) {
-        const int nq = min(PF_CHUNK, L - c0);
-        __syncthreads();
-        pf_stage<W>(a, base, stride, (const float*)a.dout + h * W, a.C, true, start + c0, nq, Qs, Os, BIAS ? Gs : nullptr);
-        for (int i = threadIdx.x; i < nq * MAPS; i += PF_THREADS) {
-            const int m = i / nq, j = i % nq;
-            const int64_t at = (int64_t)(h * MAPS + m) * a.n_pad + start + c0 + j;
-            const bool own = a.rows[start + c0 + j] >= 0;
-            Ms[m][j] = own ? a.lse[at] : INFINITY;
-            Is[m][j] = own ? a.lse[at + (int64_t)a.H * MAPS * a.n_pad] * coef[m] : 0.f;
-            Ds[m][j] = a.delta[at];
-        }
-        if (learns && threadIdx.x < PF_CHUNK) {
-            // what the queries of a window can add to a bin at most is 2^31 units, less what rounding may add
-            float r = threadIdx.x < nq ? a.reach[(int64_t)h * a.n_pad + start + c0 + threadIdx.x] : 0.f;
 #pragma unroll
-            for (int d = 1; d < PF_WINDOW; d <<= 1) r += __shfl_xor_sync(0xffffffffu, r, d);
-            if (threadIdx.x % PF_WINDOW == 0) units[threadIdx.x / PF_WINDOW] = r * (1.f / 2147000000.f);
-        }
+        for (int i = 0; i < S::AXES; ++i) bias.g[i] = pa_coord(a, p, bias.axis[i]);
+    const float scale2 = a.scale * PA_LOG2E;
+    for (int c0 = 0, cur = 0; c0 < L; c0 += S::CHUNK, cur ^= 1) {
+        const int nq = min(S::CHUNK, L - c0);
+        cp_async_wait<0>();
         __syncthreads();
+        if (c0 + S::CHUNK < L) pf_stage(a, st, cur ^ 1, base, stride, dout, a.C, start, c0 + S::CHUNK, L, h, coef);
         for (int j0 = 0; j0 < nq; j0 += PF_WINDOW) {
             if (learns) {
                 if (c0 + j0) {
@@ -414,33 +481,39 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
                     pa_flush(table, hist, sums, unit, PF_THREADS);
                     __syncthreads();
                 }
-                unit = units[j0 / PF_WINDOW];
+                unit = st.unit[cur][j0 / PF_WINDOW];
                 per_unit = pa_per_unit(unit);
             }
+            if (!busy) continue;
 #pragma unroll 4
             for (int j = j0; j < min(j0 + PF_WINDOW, nq); ++j) {
-                float s[MAPS];
-                int at[3];
-                pf_scores<W, MAPS>(k, Qs[j], part, s);
-                if (BIAS) {
-                    pf_places(table, Gs[j][0] - g[0], Gs[j][1] - g[1], Gs[j][2] - g[2], copy, at);
-                    s[0] = fmaf(s[0], scale2, tab[at[0]]) + (tab[at[1]] + tab[at[2]]);
-                }
-                const float G = pf_dot<W, MAPS>(v, Os[j], part);
+                uint64_t qs[NP], os[NP];
+                pf_load<S::SPLIT>(qs, st.x[cur][j], part);
+                pf_load<S::SPLIT>(os, st.y[cur][j], part);
+                const float G = pf_meet<S::SPLIT>(pf_dot(v, os, 0, NP));
                 float mix = 0.f;
 #pragma unroll
                 for (int m = 0; m < MAPS; ++m) {
-                    const float pr = Is[m][j] * fast_exp2(BIAS ? s[m] - Ms[m][j] : fmaf(s[m], scale2, -Ms[m][j]));
-                    const float ds = pr * (G - Ds[m][j]);
-                    mix += pr;
-                    if (learns && part == 0 && kj < L) {
-                        const int v = __float2int_rn(ds * per_unit);
-#pragma unroll
-                        for (int c = 0; c < 3; ++c) atomicAdd(hist + (at[c] >> fewer), v);
+                    const float4 x = st.aux[cur][m][j];
+                    int at[S::AXES];
+                    float s = pf_dot(k, qs, m * HP, HP);
+                    if (BIAS) {
+                        bias.places(st.g[cur][j], -1, at);
+                        s = fmaf(s, scale2, bias.look(tab, at));
                     }
-                    pf_add(dk, m * S::DP / 2, ds, &Qs[j][m * S::D + part * S::DP], S::DP);
+                    s = pf_meet<S::SPLIT>(s);
+                    const float pr = x.y * fast_exp2(BIAS ? s - x.x : fmaf(s, scale2, -x.x));
+                    const float ds = pr * (G - x.z);
+                    mix += pr;
+                    if (learns && kj < L) {
+                        const int add = __float2int_rn(ds * per_unit);
+#pragma unroll
+                        for (int i = 0; i < S::AXES; ++i)
+                            if (!(bias.idle && i == 1)) atomicAdd(hist + (at[i] >> fewer), add);
+                    }
+                    pf_add(dk, m * HP, ds, qs, HP);
                 }
-                pf_add(dv, 0, mix, &Os[j][part * S::WP], S::WP);
+                pf_add(dv, 0, mix, os, NP);
             }
         }
     }
@@ -452,20 +525,13 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     }
     if (kj >= L) return;
     const int slot = a.slot ? a.slot[start + kj] : -1;
-    if (slot >= 0) {             // this point's other row is some other patch's: added up later
-        float* dst = a.shared + (int64_t)slot * 2 * a.C + h * W;
+    if (slot < 0 && e < 0) return;
+    // where a point's other row is some other patch's, both are added up later
+    float* dst = slot >= 0 ? a.shared + (int64_t)slot * 2 * a.C + h * W : (float*)a.dqkv + (int64_t)e * stride + a.C + h * W;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dk[i], a.scale);
-            pf_put(dst + a.C + part * S::WP + 2 * i, dv[i], 1.f);
-        }
-    } else if (e >= 0) {
-        float* dst = (float*)a.dqkv + p * stride + a.C + h * W;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dk[i], a.scale);
-            pf_put(dst + a.C + part * S::WP + 2 * i, dv[i], 1.f);
-        }
+    for (int i = 0; i < NP; ++i) {
+        pf_put(dst + pf_dim<W, MAPS>(2 * i, part), dk[i], a.scale);
+        pf_put(dst + a.C + pf_dim<W, 1>(2 * i, part), dv[i], 1.f);
     }
 }
 
@@ -507,8 +573,9 @@ int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStre
     }
 }
 
-int patch_fma_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
-
-int patch_fma_cols_rows(int width) { return width == 64 ? PF_THREADS / 2 : PF_THREADS; }
+int patch_fma_cols_rows(int width)
+{
+    return width == 16 ? PfShape<16, 1>::ROWS : width == 32 ? PfShape<32, 1>::ROWS : PfShape<64, 1>::ROWS;
+}
 
 }  // namespace ptv3

@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_cols
                     __syncthreads();
                     pa_flush(table, hist, sums, unit, NT);
                 }
-                unit = pa_unit<NT / 32, PM_WINDOW, true>(a, table, w.h, w.start, L, i * CH, part);
+                unit = pa_unit<NT / 32, PM_WINDOW>(a, table, w.h, w.start, L, i * CH, part);
                 per_unit = pa_per_unit(unit);
             }
             const unsigned char* st = in.next(i);

@@ -74,7 +74,6 @@ __device__ __forceinline__ void patch_extent(const PatchPlan& p, int seq)
 
 __global__ void __launch_bounds__(256) patch_rows_kernel(const PatchPlan p)
 {
-    pdl_launch_next();
     pdl_wait();
     if ((int)blockIdx.x < p.n_extents) {
         patch_extent(p, blockIdx.x);
@@ -226,7 +225,7 @@ static int64_t bin_blocks(const ptv3_patch_attention_args* p)
     const int width = p->channels / p->heads;
     return (int64_t)p->n_seq * ceil_div(longest(p), p->dtype == PTV3_DTYPE_BF16
                                                         ? patch_mma_cols_rows(p->n_seq, longest(p), p->heads, width)
-                                                        : patch_fma_cols_rows(width));
+                                                        : patch_fma_cols_rows(longest(p), width));
 }
 
 static int launch_patch(const ptv3_patch_attention_args* p, const PatchArgs& a, int pass, cudaStream_t stream)

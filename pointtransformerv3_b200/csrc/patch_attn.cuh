@@ -198,7 +198,7 @@ enum { PA_FWD = 0, PA_ROWS = 1, PA_COLS = 2 };
 int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 // rows of a block of the pass over columns with a bias, whose blocks leave bins
-int patch_fma_cols_rows(int width);
+int patch_fma_cols_rows(int64_t longest, int width);
 int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width);
 
 }  // namespace ptv3

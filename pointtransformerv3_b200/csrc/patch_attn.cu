@@ -12,8 +12,8 @@ namespace ptv3 {
 // own: for a backward pass both get a row of its side buffer (slots 2 i and 2 i + 1; `slot` comes in filled with -1, and so
 // does the counter behind it).  With a bias the first blocks take a sequence each, and find the largest offset of two of its
 // points along each axis.
-// (Only this kernel lets the one behind it start early: blocks of the attention kernels that come while others of their kind
-// run are placed where there is room at that time, not evenly; 12 000 x 32 in fp32, all three passes: 208 us, 255 so.)
+// (Neither this kernel nor the attention kernels let the one behind them start early: blocks that come while others run are placed
+// where there is room at that time, not evenly.  12 000 x 32 in fp32, forward and backward: 167 us, 191 if this one did.)
 struct PatchPlan {
     const int64_t *order, *pad, *unpad;
     const int32_t *cu, *grid, *buckets;

@@ -3,7 +3,7 @@
 ``qk_norm_rope`` prepares the rows of a QKV projection (norms of queries and keys for each head, rotation by grid
 coordinates), ``attention_bias`` and ``attention_diff`` are attention cores within the patches of a serialized order, with a
 learned relative position bias by buckets or as the difference of two softmax maps.  They take the index tensors that
-``ops.attention`` takes; ``SerializedAttention`` calls them for its options ``qk_norm``, ``rope``, ``enable_rpe`` (in training) and
+``ops.attention`` takes; ``SerializedAttention`` calls them for its options ``qk_norm``, ``enable_rope``, ``enable_rpe`` (in training) and
 ``differential``.
 
 All of them run on the current stream of the tensors' device, keep nothing between calls, and can be captured into a graph (with a
@@ -59,6 +59,16 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _versions(*tensors):
+    """What autograd compares for the tensors that it keeps; those made in inference mode are no tensors that it would keep."""
+    return [None if t is None or t.is_inference() else t._version for t in tensors]
+
+
+def _unchanged(versions, *tensors):
+    if _versions(*tensors) != versions:
+        raise RuntimeError("coordinates, buckets or sequences that a gradient needs were modified in place since the forward pass")
+
+
 def _check_qkv(qkv, heads):
     if qkv.dim() != 2 or qkv.shape[1] % 3 or heads < 1 or (qkv.shape[1] // 3) % heads:
         raise ValueError("qkv must be (N, 3C), C a multiple of %d heads: got %s" % (heads, tuple(qkv.shape)))
@@ -80,6 +90,7 @@ class _QkNormRope(torch.autograd.Function):
         out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
         ctx.save_for_backward(qkv if q_weight is not None else None, q_weight, k_weight)
         ctx.args = grid, heads, eps, base          # (coordinates may have been made in inference mode)
+        ctx.versions = _versions(grid)
         return out
 
     @staticmethod
@@ -87,6 +98,7 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, q_weight, k_weight = ctx.saved_tensors
         grid, heads, eps, base = ctx.args
+        _unchanged(ctx.versions, grid)
         with _on(dout.device):
             dqkv, dq, dk = ops.qk_norm_rope_bwd(qkv, _aligned(dout), heads, grid, q_weight, k_weight, eps, base)
         return dqkv, None, dq, dk, None, None, None
@@ -125,6 +137,7 @@ class _PatchAttention(torch.autograd.Function):
         out, rows, lse, second = ops.patch_attention_fwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, status, True)
         ctx.save_for_backward(qkv, param, out, lse, second)
         ctx.args = plan, heads, max_seqlen, scale, maps, bias, rows      # (index tensors may have been made in inference mode)
+        ctx.versions = _versions(plan[3], *(bias or ())[:2])
         return out
 
     @staticmethod
@@ -132,6 +145,7 @@ class _PatchAttention(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, param, out, lse, second = ctx.saved_tensors
         plan, heads, max_seqlen, scale, maps, bias, rows = ctx.args
+        _unchanged(ctx.versions, plan[3], *(bias or ())[:2])
         with _on(dout.device):
             dqkv, dparam = ops.patch_attention_bwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, out, rows, lse,
                                                    second, _aligned(dout), ctx.needs_input_grad[1])
@@ -152,6 +166,7 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         raise ValueError("status must be an int32 word")
     if int(max_seqlen) < 1:
         raise ValueError("max_seqlen %d" % max_seqlen)
+    max_seqlen = min(int(max_seqlen), 2 ** 31 - 1)
     if scale is None:
         scale = (D // maps) ** -0.5
     if not (math.isfinite(scale) and scale):
@@ -165,9 +180,9 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         if own:
             status = ops.new_status(qkv.device)
         if _wants_grad(qkv, param):
-            out = _PatchAttention.apply(qkv, param, plan, int(heads), int(max_seqlen), float(scale), maps, bias, status)
+            out = _PatchAttention.apply(qkv, param, plan, int(heads), max_seqlen, float(scale), maps, bias, status)
         else:
-            out = ops.patch_attention_fwd(qkv, plan, int(heads), int(max_seqlen), float(scale), maps, param, bias, status)[0]
+            out = ops.patch_attention_fwd(qkv, plan, int(heads), max_seqlen, float(scale), maps, param, bias, status)[0]
         if own:
             _lib.raise_on_status(status, "ptv3_patch_attention_fwd")
     return out

@@ -468,3 +468,40 @@ def test_bad_plans_are_reported():
         F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=p["grid"], table=torch.ones(3 * num, H, device="cuda"), buckets=buckets)
     # and a good one is good, with a patch size beyond all scenes too
     F.attention_diff(qkv, lam, *geometry(plan([130, 20], 2048)), H, 2048)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("counts,patch", [([700, 600], 256), ([900, 1, 399], 65), ([1300], 1024), ([420] * 3, 512)],
+                         ids=lambda v: str(v)[:20])
+def test_many_heads(counts, patch, dtype):
+    """Launches with a block for more than half of the SMs, which are laid out differently from short ones."""
+    p = plan(counts, patch)
+    for width, H in ((16, 8), (32, 9)):
+        for run in (lambda: run_bias(p, width * H, H, dtype, dtype, 9), lambda: run_diff(p, width * H, H, dtype, dtype)):
+            out, dqkv, dparam, ref = run()
+            for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dparam)):
+                R.check(got, ref, name, width, p["longest"], dtype, "width %d" % width)
+
+
+def test_index_tensors_that_change_before_the_gradient():
+    """A gradient of coordinates, buckets or sequences other than the forward pass's is refused, as autograd does for its own."""
+    p = plan([100, 30], 64)
+    H = 2
+    qkv, table = normal(130, 96, seed=1).requires_grad_(), normal(33, H, seed=2).requires_grad_()
+    buckets, num = F.log_buckets(12, device="cuda")
+    wide = normal(3 * num, H, seed=3).requires_grad_()
+    for name in ("grid", "cu", "buckets"):
+        q = dict(p, grid=p["grid"].clone(), cu=p["cu"].clone(), buckets=buckets.clone())
+        outs = [F.attention_bias(qkv, *geometry(q), H, 64, grid_coord=q["grid"], table=wide, buckets=q["buckets"])]
+        if name == "grid":
+            outs.append(F.qk_norm_rope(qkv, H, q["grid"]))
+        q[name].add_(0)
+        for out in outs:
+            with pytest.raises(RuntimeError, match="modified in place"):
+                torch.autograd.grad(out, qkv, torch.ones_like(out))
+    out = F.attention_bias(qkv, *geometry(p), H, 2 ** 40, grid_coord=p["grid"], table=table)      # (a patch size beyond all)
+    assert torch.equal(out, F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=p["grid"], table=table))
+    with torch.inference_mode():
+        grid = p["grid"].clone()
+    out = F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=grid, table=table)
+    torch.autograd.grad(out, qkv, torch.ones_like(out))

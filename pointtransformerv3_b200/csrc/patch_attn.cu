@@ -264,7 +264,7 @@ static PatchWorkspace carve(const ptv3_patch_attention_args* p)
 static int check_sizes(const ptv3_patch_attention_args* p, const char* what)
 {
     PTV3_REQUIRE(p != nullptr, PTV3_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
-    PTV3_REQUIRE(p->n >= 0 && p->n_pad >= p->n && p->n_pad <= 2 * p->n && p->n_seq >= 0 && p->max_seqlen >= 1 && p->channels >= 1 && p->heads >= 1 &&
+    PTV3_REQUIRE(p->n >= 0 && p->n_pad >= p->n && p->n_pad <= 2 * p->n && p->n_seq >= (p->n > 0) && p->max_seqlen >= 1 && p->channels >= 1 && p->heads >= 1 &&
                      p->channels % p->heads == 0 && (p->maps == 1 || p->maps == 2),
                  PTV3_ERR_INVALID_ARGUMENT, "%s: bad sizes", what);
     const int width = p->channels / p->heads;
@@ -351,7 +351,7 @@ extern "C" int ptv3_patch_attention_fwd(const ptv3_patch_attention_args* p, void
 {
     int rc = check_sizes(p, "ptv3_patch_attention_fwd");
     if (rc != PTV3_OK) return rc;
-    if (p->n == 0 || p->n_seq == 0) return PTV3_OK;
+    if (p->n == 0) return PTV3_OK;
     PTV3_REQUIRE((((uintptr_t)p->qkv | (uintptr_t)p->out | (uintptr_t)p->second) & 15) == 0, PTV3_ERR_INVALID_ARGUMENT,
                  "ptv3_patch_attention_fwd: unaligned rows");
     PTV3_REQUIRE(p->qkv && p->order && p->pad && p->unpad && p->rows && p->cu_seqlens && p->out && (p->maps == 1 || (p->lam && (!p->lse || p->second))),
@@ -374,7 +374,7 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
     if (rc != PTV3_OK) return rc;
     cudaStream_t s = (cudaStream_t)stream;
     PatchArgs a = device_args(p);
-    if (p->n > 0 && p->n_seq > 0)
+    if (p->n > 0)
         PTV3_REQUIRE(p->qkv && p->order && p->pad && p->unpad && p->rows && p->cu_seqlens && p->out && p->lse && p->dout && p->dqkv &&
                          (p->maps == 1 || (p->lam && p->second)),
                      PTV3_ERR_INVALID_ARGUMENT, "ptv3_patch_attention_bwd: null pointer");
@@ -386,7 +386,7 @@ extern "C" int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* p, void
     const PatchWorkspace w = carve(p);
     PTV3_REQUIRE(w.bytes == 0 || (p->workspace && p->workspace_bytes >= w.bytes), PTV3_ERR_WORKSPACE,
                  "ptv3_patch_attention_bwd: workspace of %zu bytes, %zu needed", p->workspace_bytes, w.bytes);
-    const bool any = p->n > 0 && p->n_seq > 0;
+    const bool any = p->n > 0;
     if (any) {
         a.dout = p->dout;
         a.dqkv = p->dqkv;

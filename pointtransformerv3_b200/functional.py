@@ -158,8 +158,8 @@ def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seql
         raise ValueError("heads of %d values (supported: 16, 32, 64)" % D)
     if order_row.shape != (n,) or unpad.shape != (n,) or pad.dim() != 1 or not n <= pad.shape[0] <= 2 * n:
         raise ValueError("order_row and unpad must be (%d,), pad %d to %d rows" % (n, n, 2 * n))
-    if cu_seqlens.dim() != 1 or cu_seqlens.dtype != torch.int32:
-        raise ValueError("cu_seqlens must be a row of int32")
+    if cu_seqlens.dim() != 1 or cu_seqlens.dtype != torch.int32 or cu_seqlens.shape[0] < (2 if n else 1):
+        raise ValueError("cu_seqlens must be a row of int32, the ends of one sequence and more")
     if any(t.dtype != torch.int64 for t in (order_row, pad, unpad)):
         raise ValueError("order_row, pad and unpad must be int64")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):

@@ -106,3 +106,9 @@ def test_the_references_gradients_are_those_of_differences():
                     moved[at] = moved[at] + s * step
                     ends.append(float((f(*moved)["out"][0] * dout).sum()))
                 assert abs((ends[0] - ends[1]) / (2 * h) - float((res[name][0] * step).sum())) < 1e-5
+
+
+def test_points_without_sequences_are_refused():
+    for ends in (t(1, dtype=torch.int32), t(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="one sequence"):
+            F.attention_bias(t(8, 48), *args()[:3], ends, 1, 8)

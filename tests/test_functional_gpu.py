@@ -505,3 +505,14 @@ def test_index_tensors_that_change_before_the_gradient():
         grid = p["grid"].clone()
     out = F.attention_bias(qkv, *geometry(p), H, 64, grid_coord=grid, table=table)
     torch.autograd.grad(out, qkv, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("width,H", [(16, 17), (32, 9)])
+def test_long_launches(width, H, dtype):
+    """Enough patches of more than 256 rows for blocks whose warps own two row tiles."""
+    p = plan([3000, 1100], 512)
+    for run in (lambda: run_bias(p, width * H, H, dtype, dtype, 9), lambda: run_diff(p, width * H, H, dtype, dtype)):
+        out, dqkv, dparam, ref = run()
+        for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dparam)):
+            R.check(got, ref, name, width, p["longest"], dtype)

@@ -412,7 +412,7 @@ __device__ __forceinline__ void pm_own_rows(const PmOwn<RT>& own, const __nv_bfl
 
 // ------------------------------------------------------------------------------------------------- forward
 template <int W, int MAPS, bool BIAS, bool KEEP, int RT, int NT>
-__global__ void __launch_bounds__(NT, (W == 64 && MAPS == 2 ? 256 : 512) / NT) patch_mma_fwd_kernel(const PatchArgs a)
+__global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 : 512) / NT) patch_mma_fwd_kernel(const PatchArgs a)
 {
     pdl_wait();
     constexpr int CH = PmChunk<W, BIAS, NT>::N;
@@ -983,7 +983,9 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 // forward with a bias, 120 000 x 64, 489 and 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of
 // two maps 347 and 320; not so forward and rows without a bias (312 and 326, 341 and 465).  Heads of 32, 100 000 x 64: columns with a
 // bias, a CTA to an SM, 671 and 523 (10 000 x 64: 110 and 84), of two maps in blocks of four warps, three to an SM, 266 and 233
-// (20 000 x 64: 78 and 68; 10 000 x 64 42 and 41); forward and rows are slower or as fast (with a bias 238 and 281, 289 and 300).  Four warps where patches are short
+// (20 000 x 64: 78 and 68; 10 000 x 64 42 and 41); forward and rows are slower or as fast (with a bias 238 and 281, 289 and 300).  Heads
+// of 64, a CTA to an SM: forward with a bias 231 and 174 (20 000 x 64: 74 and 58); columns with a bias 410 and 383, of two maps 261 and
+// 228, but 202 and 247, 122 and 149 at 40 000 x 64, whose 160 blocks are two rounds: one tile.  Four warps where patches are short
 // (60 000 x 64 in patches of 48, two maps, the three passes: 62, 70 and 74 us with eight, 34, 38 and 36) or blocks without a bias
 // few (1 560 x 256 forward 33 and 27.5; with a bias, 6 760 x 128, 68 and 72).
 struct PmForm {
@@ -995,8 +997,10 @@ static PmForm block_form(int64_t n_seq, int64_t longest, int heads, int width, i
     auto blocks = [&](int rows) { return n_seq * heads * ((longest + rows - 1) / rows); };
     if (longest <= 64 || (!bias && blocks(128) < 2 * SMS)) return PmForm{128, 1};
     const int least = width == 16 ? 2 * SMS : bias ? SMS / 2 : SMS;
-    const bool two = longest >= 256 && blocks(256) >= least &&
-                     (width == 16 ? bias || (maps == 2 && pass == PA_COLS) : width == 32 && pass == PA_COLS && (bias || maps == 2));
+    const bool suits = width == 16   ? bias || (maps == 2 && pass == PA_COLS)
+                       : width == 32 ? pass == PA_COLS && (bias || maps == 2)
+                                     : pass == PA_FWD && bias;
+    const bool two = suits && longest >= 256 && blocks(256) >= least;
     return PmForm{two && width == 32 && !bias ? 128 : 256, two ? 2 : 1};
 }
 int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width)
@@ -1009,13 +1013,14 @@ static int launch_block(const PatchArgs& a, int pass, cudaStream_t stream)
 {
     const size_t stages = PM_STAGES * PmStage<W, PmChunk<W, BIAS, NT>::N>::BYTES;
     const size_t smem = stages + (BIAS ? PmTableBytes<NT>::TABLE : 0);
-    constexpr int ROWS2 = BIAS && W == 16 ? RT : 1;      // (two tiles to a warp: columns alone without a bias or in heads of 32)
+    // (block_form has what takes two tiles)
+    constexpr int ROWS2 = BIAS && W == 16 ? RT : 1, FWD2 = BIAS && W != 32 ? RT : 1, COLS2 = W == 64 ? 1 : RT;
     if (pass == PA_ROWS) return launch<NT>(patch_mma_rows_kernel<W, MAPS, BIAS, ROWS2, NT>, a, smem, stream);
     if (pass == PA_COLS)      // the table, its bins, and their sums
-        return launch<NT>(patch_mma_cols_kernel<W, MAPS, BIAS, RT, NT>, a,
+        return launch<NT>(patch_mma_cols_kernel<W, MAPS, BIAS, COLS2, NT>, a,
                           stages + (BIAS ? PmTableBytes<NT>::BINS + pm_sums_bytes(a.bnd, PmTableBytes<NT>::BINS) : 0), stream);
-    return a.lse ? launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, true, ROWS2, NT>, a, smem, stream)
-                 : launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, false, ROWS2, NT>, a, smem, stream);
+    return a.lse ? launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, true, FWD2, NT>, a, smem, stream)
+                 : launch<NT>(patch_mma_fwd_kernel<W, MAPS, BIAS, false, FWD2, NT>, a, smem, stream);
 }
 
 template <int W, int MAPS, bool BIAS>
@@ -1025,7 +1030,7 @@ static int launch_pass(const PatchArgs& args, int pass, cudaStream_t stream)
     const int longest = a.max_seqlen < a.n_pad ? a.max_seqlen : a.n_pad;
     const PmForm form = block_form(a.n_seq, longest, a.H, W, MAPS, BIAS, pass);
     a.tiles = ceil_div(longest, form.rows());
-    constexpr int RT = (W <= 32 && BIAS) || (W == 16 && MAPS == 2) ? 2 : 1, RT4 = W == 32 && MAPS == 2 ? 2 : 1;
+    constexpr int RT = BIAS || (W == 16 && MAPS == 2) ? 2 : 1, RT4 = W == 32 && MAPS == 2 ? 2 : 1;
     if (form.threads == 128)
         return form.tiles == 2 ? launch_block<W, MAPS, BIAS, RT4, 128>(a, pass, stream)
                                : launch_block<W, MAPS, BIAS, 1, 128>(a, pass, stream);

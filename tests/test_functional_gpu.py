@@ -516,3 +516,16 @@ def test_long_launches(width, H, dtype):
         out, dqkv, dparam, ref = run()
         for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dparam)):
             R.check(got, ref, name, width, p["longest"], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_long_launches_of_wide_heads(dtype):
+    p = plan([1400, 800], 512)
+    for H in (8, 11):
+        out, dqkv, dtable, ref = run_bias(p, 64 * H, H, dtype, dtype, 9)
+        for name, got in (("out", out), ("dqkv", dqkv), ("dparam", dtable)):
+            R.check(got, ref, name, 64, p["longest"], dtype)
+        with torch.no_grad():
+            qkv, table = normal(p["n"], 192 * H, seed=1, dtype=dtype), normal(57, H, seed=2, dtype=dtype, scale=0.5)
+            alone = F.attention_bias(qkv, *geometry(p), H, 512, grid_coord=p["grid"], table=table)
+        assert torch.equal(alone, out)

@@ -248,7 +248,7 @@ int ptv3_patch_attention_bwd(const ptv3_patch_attention_args* args, void* stream
  *   pairs (2 i, 2 i + 1), i < 3 p, p = D / 6:  turned by grid[i / p] * base^(-(i mod p) / p)
  * D in {8, 16, 32, 64, 128}; the angle is taken in whole turns of 2^-64, so that far coordinates lose nothing.
  *   qkv, out, dout, dqkv   n x 3*channels, 16-byte aligned, dtype PTV3_DTYPE_*
- *   q_weight, k_weight     D each, PTV3_DTYPE_* weight_dtype; dq_weight, dk_weight in the same type
+ *   q_weight, k_weight     D each, PTV3_DTYPE_* weight_dtype, aligned to that type; dq_weight, dk_weight in the same type
  *   grid_coord             n x 3 int32
  *   workspace              of _bwd, ptv3_qk_norm_rope_workspace_bytes, where weights are given
  */

@@ -91,6 +91,15 @@ template <> struct QkPairs<__nv_bfloat16> {
     __device__ static uint4 store(const uint64_t* p) { return make_uint4(one(p[0]), one(p[1]), one(p[2]), one(p[3])); }
 };
 
+// Weights i and i + 1 as a pair.  A vector of weights is wherever its caller has it (a slice of a buffer of all parameters), so it
+// is read value by value: 16-bit weights start on 2 bytes.  A thread does this once.
+__device__ __forceinline__ uint64_t qk_weights(const void* weights, int i, int bf16)
+{
+    if (!bf16) return pack2(((const float*)weights)[i], ((const float*)weights)[i + 1]);
+    const __nv_bfloat16* w = (const __nv_bfloat16*)weights;
+    return pack2(__bfloat162float(w[i]), __bfloat162float(w[i + 1]));
+}
+
 // the first `turned` pairs rotated
 template <int N>
 __device__ __forceinline__ void qk_rotate(uint64_t (&y)[N], const float2* cs, int turned, bool back)
@@ -133,8 +142,7 @@ __global__ void __launch_bounds__(QK_THREADS, NORM && BACK ? 2 : 3) qk_norm_rope
         const void* weights = part == 0 ? a.qw : a.kw;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            w[i] = a.w_bf16 ? unpack_bf16x2(((const uint32_t*)weights)[first + i])
-                            : pack2(((const float*)weights)[2 * (first + i)], ((const float*)weights)[2 * (first + i) + 1]);
+            w[i] = qk_weights(weights, 2 * (first + i), a.w_bf16);
             dw[i] = 0;
         }
     }
@@ -259,6 +267,8 @@ static int qk_check(const char* what, const void* qkv, const void* qw, const voi
     PTV3_REQUIRE(channels <= 1 << 16, PTV3_ERR_UNSUPPORTED, "%s: %d channels", what, channels);
     PTV3_REQUIRE(!qw == !kw && (qw || grid), PTV3_ERR_INVALID_ARGUMENT,
                  "%s: weights of both queries and keys, coordinates, or all three", what);
+    PTV3_REQUIRE((((uintptr_t)qw | (uintptr_t)kw) & (weight_dtype == PTV3_DTYPE_BF16 ? 1 : 3)) == 0,
+                 PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned weights", what);
     PTV3_REQUIRE(!grid || base > 0, PTV3_ERR_INVALID_ARGUMENT, "%s: base %g", what, base);
     PTV3_REQUIRE(n == 0 || (qkv && out && (((uintptr_t)qkv | (uintptr_t)out) & 15) == 0), PTV3_ERR_INVALID_ARGUMENT,
                  "%s: null or unaligned rows", what);

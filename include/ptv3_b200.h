@@ -205,7 +205,9 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
  * the same time need one each.
  *   qkv, dqkv   n x 3*channels; out, dout n x channels; 16-byte aligned, dtype PTV3_DTYPE_*
  *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30; read by _fwd (cu_seqlens by _bwd too)
- *   rows        2 * n_pad + (n_pad - n) + 1 + 3 * n_seq int32: what the kernels need of the plan, written by _fwd, read by _bwd
+ *   rows        2 * n_pad + (n_pad - n) + 1 + 6 * n_seq int32: what the kernels need of the plan, written by _fwd, read by _bwd.
+ *               Where coordinates, buckets or cu_seqlens have changed in between, the gradients are undefined, and accesses
+ *               stay within the tensors all the same
  *   grid_coord  n x 3 int32 within 2^22 of zero; buckets 2 pos_bnd + 1 int32 in [0, num_buckets)
  *   status      one uint32 or NULL: _fwd ORs PTV3_STATUS_BAD_INDEX into it where the plan or the bias does not hold: an index out
  *               of range, a point without one row that answers for it or with more than one borrowed row, sequences that do

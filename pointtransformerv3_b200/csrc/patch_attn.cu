@@ -68,7 +68,8 @@ __device__ __forceinline__ void patch_extent(const PatchPlan& p, int seq)
             l = min(l, lo_s[w][threadIdx.x]);
             h = max(h, hi_s[w][threadIdx.x]);
         }
-        p.extent[3 * seq + threadIdx.x] = max(h - l, 0);
+        p.extent[6 * seq + threadIdx.x] = max(h - l, 0);
+        p.extent[6 * seq + 3 + threadIdx.x] = l;
     }
 }
 

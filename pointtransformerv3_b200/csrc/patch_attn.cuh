@@ -25,6 +25,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "patch_place.cuh"
 
 namespace ptv3 {
 
@@ -47,7 +48,7 @@ struct PatchArgs {
     const void* table;          // (3 num) x H
     const int32_t* buckets;     // 2 bnd + 1, or NULL: every offset its own
     int num, bnd, table_bf16;
-    const int32_t* extent;      // n_seq x 3: largest offset within a sequence along each axis
+    const int32_t* extent;      // n_seq x 6: largest offset within a sequence along each axis, and its lowest coordinates
     const void* lam;            // H
     int lam_bf16;
     float* lse;                 // (H maps) x n_pad: log2 of the softmax's sum (bf16), or twice that: its reference
@@ -98,7 +99,7 @@ __device__ __forceinline__ PatchTable pa_table(const PatchArgs& a, int seq, int 
         t.entries = 0;
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-            t.reach[c] = a.extent[3 * seq + c];
+            t.reach[c] = a.extent[6 * seq + c];
             if (k) t.reach[c] = min(a.bnd, t.reach[c]);
             t.first[c] = t.entries;
             t.entries += 2 * t.reach[c] + 1;

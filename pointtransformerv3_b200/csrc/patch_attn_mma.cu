@@ -60,6 +60,23 @@ __device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t
                  : "r"(a0), "r"(a1), "r"(b0));
 }
 
+// a coordinate in its sequence's box (of what the plan's rows hold, not of the coordinates as they are now)
+__device__ __forceinline__ int pm_box(const PatchArgs& a, int seq, int coord, int c)
+{
+    return pa_held(coord, a.extent[6 * seq + 3 + c], a.extent[6 * seq + c]);
+}
+struct PmPlace {
+    int h, tile, seq, start, L;
+};
+__device__ __forceinline__ PmPlace pm_place(const PatchArgs& a)
+{
+    PmPlace p;
+    p.h = blockIdx.x % a.H;
+    p.tile = blockIdx.x / a.H % a.tiles;
+    p.seq = blockIdx.x / a.H / a.tiles;
+    p.L = pa_sequence(a, p.seq, p.start);
+    return p;
+}
 // Bias of a pair of points: coordinates in bytes of the table in shared memory
 struct PmBias {
     int lo[3], hi[3];       // bounds of an entry's place, this lane's copy
@@ -84,7 +101,7 @@ struct PmStream {
     const PatchArgs& a;
     const __nv_bfloat16 *x, *y;
     int64_t xs, ys;
-    int start, L, h;
+    int seq, start, L, h;
     bool owners;             // rows of y that answer for no point are taken as zeros
     int step;                // coordinates are kept times 2^step
     unsigned char* smem;
@@ -106,7 +123,7 @@ struct PmStream {
         if (BIAS && threadIdx.x < CH) {
             const int64_t p = eg >= 0 ? eg : -(eg + 1);
 #pragma unroll
-            for (int c = 0; c < 3; ++c) g[c] = pa_coord(a, p, c);
+            for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
         }
     }
     __device__ __forceinline__ void fetch_aux(int chunk)
@@ -158,7 +175,8 @@ struct PmStream {
                 }
             if (BIAS && threadIdx.x < CH)
 #pragma unroll
-                for (int c = 0; c < 3; ++c) ((int*)(st + S::GRID))[c * CH + threadIdx.x] = g[c] << step;
+                for (int c = 0; c < 3; ++c)
+                    ((int*)(st + S::GRID))[c * CH + threadIdx.x] = pa_other(pm_box(a, seq, g[c], c), step);
         }
         cp_async_commit();
     }
@@ -310,13 +328,14 @@ __device__ __forceinline__ void pm_bias_setup(const PatchTable& t, uint32_t base
     }
 }
 // row r's point, so that subtracting another's coordinates gives the entry's place
-__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTable& t, const PmBias& b, int start, int L, int r,
+__device__ __forceinline__ void pm_bias_point(const PatchArgs& a, const PatchTable& t, const PmBias& b, const PmPlace& w, int r,
                                               int sign, int (&g)[3])
 {
-    const int e = a.rows[start + min(r, L - 1)];
+    const int e = a.rows[w.start + min(r, w.L - 1)];
+    const int64_t p = e >= 0 ? e : -(e + 1);
 #pragma unroll
     for (int c = 0; c < 3; ++c)
-        g[c] = b.lo[c] + ((t.reach[c] + sign * pa_coord(a, e >= 0 ? e : -(e + 1), c)) << (t.copies_log2 + 2));
+        g[c] = pa_mine(b.lo[c], t.reach[c], pm_box(a, w.seq, a.grid[3 * p + c], c), sign, t.copies_log2 + 2);
 }
 // coordinates of the other side's rows j and j + 1
 template <int CH>
@@ -368,18 +387,6 @@ __device__ __forceinline__ uint64_t pm_exp2(uint64_t x)
 }
 __device__ __forceinline__ uint64_t pm_both(float v) { return pack2(v, v); }
 
-struct PmPlace {
-    int h, tile, seq, start, L;
-};
-__device__ __forceinline__ PmPlace pm_place(const PatchArgs& a)
-{
-    PmPlace p;
-    p.h = blockIdx.x % a.H;
-    p.tile = blockIdx.x / a.H % a.tiles;
-    p.seq = blockIdx.x / a.H / a.tiles;
-    p.L = pa_sequence(a, p.seq, p.start);
-    return p;
-}
 // this lane's rows of the RT tiles of its warp: row g + 8 r of tile x
 template <int RT>
 struct PmOwn {
@@ -429,7 +436,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
-    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
 #pragma unroll
         for (int x = 0; x < RT; ++x)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], 1, point[x][r]);
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w, own.row[x][r], 1, point[x][r]);
     }
     uint32_t q[RT][W / 16][4];
     // (of a negative scale the sign goes to the queries, so that larger products are larger scores)
@@ -636,7 +643,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
-    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.start, L, w.h, false,
+    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
                                          table.copies_log2 + 2, smem};
     in.begin();
     PmBias bias;
@@ -648,7 +655,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
 #pragma unroll
         for (int x = 0; x < RT; ++x)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], 1, point[x][r]);
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w, own.row[x][r], 1, point[x][r]);
     }
     uint32_t q[RT][W / 16][4], go[RT][W / 16][4];
     float lse[MAPS][RT][2], shift[MAPS][RT][2], most[RT][2];
@@ -813,7 +820,7 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::BINS, true);
-    PmStream<W, MAPS, true, BIAS, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.start, L, w.h, true,
+    PmStream<W, MAPS, true, BIAS, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.seq, w.start, L, w.h, true,
                                         table.copies_log2 + 2, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);
@@ -832,7 +839,7 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
 #pragma unroll
         for (int x = 0; x < RT; ++x)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w.start, L, own.row[x][r], -1, point[x][r]);
+            for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w, own.row[x][r], -1, point[x][r]);
         if (learns) {
             for (int i = threadIdx.x; i < table.entries << table.bins_log2; i += NT) hist[i] = 0;
             for (int i = threadIdx.x; i < table.entries; i += NT) sums[i] = 0.f;

@@ -59,9 +59,14 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _kept(t):
+    """An index tensor as a backward pass keeps it.  One made in inference mode counts no changes, so it is copied."""
+    return t.clone() if t is not None and t.is_inference() else t
+
+
 def _versions(*tensors):
-    """What autograd compares for the tensors that it keeps; those made in inference mode are no tensors that it would keep."""
-    return [None if t is None or t.is_inference() else t._version for t in tensors]
+    """What autograd compares for the tensors that it keeps."""
+    return [None if t is None else t._version for t in tensors]
 
 
 def _unchanged(versions, *tensors):
@@ -89,7 +94,8 @@ class _QkNormRope(torch.autograd.Function):
     def forward(ctx, qkv, grid, q_weight, k_weight, heads, eps, base):
         out = ops.qk_norm_rope_fwd(qkv, heads, grid, q_weight, k_weight, eps, base)
         ctx.save_for_backward(qkv if q_weight is not None else None, q_weight, k_weight)
-        ctx.args = grid, heads, eps, base          # (coordinates may have been made in inference mode)
+        grid = _kept(grid)
+        ctx.args = grid, heads, eps, base
         ctx.versions = _versions(grid)
         return out
 
@@ -136,7 +142,10 @@ class _PatchAttention(torch.autograd.Function):
     def forward(ctx, qkv, param, plan, heads, max_seqlen, scale, maps, bias, status):
         out, rows, lse, second = ops.patch_attention_fwd(qkv, plan, heads, max_seqlen, scale, maps, param, bias, status, True)
         ctx.save_for_backward(qkv, param, out, lse, second)
-        ctx.args = plan, heads, max_seqlen, scale, maps, bias, rows      # (index tensors may have been made in inference mode)
+        plan = plan[:3] + (_kept(plan[3]),)
+        if bias is not None:
+            bias = (_kept(bias[0]), _kept(bias[1])) + bias[2:]
+        ctx.args = plan, heads, max_seqlen, scale, maps, bias, rows
         ctx.versions = _versions(plan[3], *(bias or ())[:2])
         return out
 

@@ -1,7 +1,10 @@
 """What the trainable operators ask of their arguments: what is refused on the host, and what kernels may not assume."""
+import ctypes
 import os
 import re
+import subprocess
 
+import numpy as np
 import pytest
 
 from conftest import ROOT
@@ -31,3 +34,40 @@ def test_weights_off_their_own_type_are_refused(dtype, step):
                                                        dtype, rows, 1 << 20, None)):
             with pytest.raises(_lib.Ptv3Error, match="unaligned weights"):
                 _lib.check(call(), "ptv3_qk_norm_rope")
+
+
+@pytest.fixture(scope="module")
+def places(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("hostmath") / "libpatch_place_host.so")
+    subprocess.check_call(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-o", so,
+                           os.path.join(ROOT, "tests", "hostmath", "patch_place_host.cpp")])
+    lib = ctypes.CDLL(so)
+    i, p = ctypes.c_int, ctypes.c_void_p
+    lib.host_places.argtypes = [p, p, ctypes.c_int64, i, i, i, i, i, i, p]
+
+    def call(mine, other, lowest, extent, first, reach, sign, step):
+        out = np.empty(mine.size, dtype=np.int32)
+        lib.host_places(mine.ctypes.data, other.ctypes.data, mine.size, lowest, extent, first, reach, sign, step, out.ctypes.data)
+        return out
+    return call
+
+
+@pytest.mark.parametrize("lowest,extent", [(0, 0), (0, 11), (-40, 117), (2 ** 22, 0), (-2 ** 22, 2 ** 23)])
+def test_look_ups_stay_in_the_table_whatever_the_coordinates_are(places, lowest, extent):
+    """The plan's rows hold a sequence's box.  Points of the box find the entry of their offset; coordinates that have changed since,
+    anything of 32 bits, find some entry of the table.  (Of the largest extent only what is held within the table afterwards
+    is computed: no sum passes 32 bits.)"""
+    rng = np.random.default_rng(7)
+    step, first = 5 + 2, 51200 + 4 * 31
+    inside = rng.integers(lowest, lowest + extent + 1, size=(2, 5000)).astype(np.int32)
+    ends = np.array([-2 ** 31, 2 ** 31 - 1, 0, lowest, lowest + extent], dtype=np.int32)
+    outside = rng.integers(-2 ** 31, 2 ** 31, size=(2, 5000)).astype(np.int32)
+    outside[0, :25], outside[1, :25] = np.repeat(ends, 5), np.tile(ends, 5)
+    reach = min(extent, 1024)
+    for sign in (1, -1):
+        got = places(inside[0], inside[1], lowest, extent, first, reach, sign, step)
+        want = first + ((reach + sign * (inside[0].astype(np.int64) - inside[1])) << step)
+        assert (got == want).all()
+        got = places(outside[0], outside[1], lowest, extent, first, reach, sign, step)
+        far = (extent - reach) << step              # (beyond the table only where look-ups are held afterwards)
+        assert got.min() >= first - far and got.max() <= first + ((2 * reach) << step) + far

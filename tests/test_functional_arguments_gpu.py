@@ -4,6 +4,7 @@ import torch
 
 import functional_reference as R
 from pointtransformerv3_b200 import functional as F
+from pointtransformerv3_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,63 @@ def test_weights_from_a_buffer_of_parameters(D, dtype):
         q, k = buffer[first:first + D], buffer[first + D + 1:first + 2 * D + 1]
         assert (q.data_ptr() - buffer.data_ptr()) == first * buffer.element_size()
         assert all(torch.equal(a, b) for a, b in zip(run(q, k), run(q.clone(), k.clone())))
+
+
+def patches(counts, patch, seed=0, extent=12):
+    """A batch of scenes in random order, their patches and coordinates."""
+    g = torch.Generator().manual_seed(seed)
+    order, at = [], 0
+    for c in counts:
+        order.append(torch.randperm(c, generator=g) + at)
+        at += c
+    pad, unpad, cu = ops.pad_plan(torch.cumsum(torch.tensor(counts), 0).cuda(), counts, patch)
+    grid = torch.randint(0, extent, (at, 3), generator=g, dtype=torch.int32).cuda()
+    return dict(n=at, geometry=(torch.cat(order).cuda(), pad, unpad, cu), grid=grid, longest=min(max(counts), patch))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_index_tensors_of_inference_mode_are_kept_as_they_were(dtype):
+    """They count no changes, so a gradient has a copy of them: it is the one of the forward pass's coordinates, buckets and
+    sequences, whatever they hold by then."""
+    p = patches([150, 60], 64)
+    H, C = 2, 32
+    with torch.inference_mode():
+        grid, cu = p["grid"].clone(), p["geometry"][3].clone()
+        buckets, num = F.log_buckets(10)
+        buckets = buckets.cuda()
+    qkv = normal(p["n"], 3 * C, seed=1, dtype=dtype).requires_grad_()
+    table, w = normal(3 * num, H, seed=2).requires_grad_(), torch.ones(C // H, device="cuda")
+    dout = normal(p["n"], C, seed=3, dtype=dtype)
+    args = p["geometry"][:3] + (cu, H, p["longest"])
+    outs = [F.attention_bias(qkv, *args, grid_coord=grid, table=table, buckets=buckets),
+            F.qk_norm_rope(qkv, H, grid, w, w)]
+
+    def grads():
+        return (torch.autograd.grad(outs[0], (qkv, table), dout, retain_graph=True)
+                + torch.autograd.grad(outs[1], qkv, qkv.detach(), retain_graph=True))
+    first = grads()
+    with torch.inference_mode():
+        grid.mul_(300)
+        buckets.zero_()
+        cu.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(first, grads()))
+
+
+@pytest.mark.parametrize("width", [16, 32, 64])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_coordinates_that_change_unseen_stay_in_the_table(width, dtype):
+    """Written behind torch's back, coordinates make a gradient of nothing in particular; it reads and writes what it owns, and with the
+    coordinates back it is what it was."""
+    p = patches([300, 77], 128)
+    qkv = normal(p["n"], 3 * 2 * width, seed=1, dtype=dtype).requires_grad_()
+    table, dout = normal(3 * 63, 2, seed=2).requires_grad_(), normal(p["n"], 2 * width, seed=3, dtype=dtype)
+    out = F.attention_bias(qkv, *p["geometry"], 2, p["longest"], grid_coord=p["grid"], table=table)
+
+    def grads():
+        return torch.autograd.grad(out, (qkv, table), dout, retain_graph=True)
+    first, grid = grads(), p["grid"].clone()
+    for change in (lambda g: g * 1000 - 7, lambda g: g - 2 ** 31, lambda g: 2 ** 31 - 1 - g):
+        p["grid"].data.copy_(change(grid.long()).clamp(-2 ** 31, 2 ** 31 - 1))
+        assert all(bool(t.isfinite().all()) for t in grads())
+    p["grid"].data.copy_(grid)
+    assert all(torch.equal(a, b) for a, b in zip(first, grads()))

@@ -9,12 +9,14 @@ learned relative position bias by buckets or as the difference of two softmax ma
 All of them run on the current stream of the tensors' device, keep nothing between calls, and can be captured into a graph (with a
 ``status`` word of the caller's: one that they make themselves is read at once, which waits for the device).  A backward pass
 that is captured wants leaves which no eager graph holds at that time (``x.detach().requires_grad_()``): torch ties a leaf's
-gradient to the stream of the graph that met it first.  Gradients are of first order, and the same bits on every run.
+gradient to the stream of the graph that met it first.  Gradients are of first order and backward, and the same bits on every run;
+tensors with a tangent of forward-mode differentiation are refused.
 """
 import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -47,6 +49,12 @@ _HERE = contextlib.nullcontext()
 def _on(device):
     """Makes the tensors' device the current one, where it is another (the guard costs as much as a launch)."""
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _no_tangents(*tensors):
+    """Refuses tensors with a tangent: the kernels would return results without one, which torch takes as a derivative of zero."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("no forward-mode derivatives")
 
 
 def _wants_grad(*tensors):
@@ -119,6 +127,7 @@ def qk_norm_rope(qkv, heads, grid_coord=None, q_weight=None, k_weight=None, eps=
     depend on the offset between two points; values beyond 6p are left.  D in 8, 16, 32, 64, 128; bf16 or fp32.  For
     ``attention_diff``, whose heads have two queries and two keys, pass twice its number of heads.  Returns a matrix like qkv."""
     _same_device(qkv, grid_coord, q_weight, k_weight)
+    _no_tangents(qkv, q_weight, k_weight)
     _check_qkv(qkv, heads)
     D = qkv.shape[1] // 3 // heads
     if (q_weight is None) != (k_weight is None) or (q_weight is None and grid_coord is None):
@@ -162,6 +171,7 @@ class _PatchAttention(torch.autograd.Function):
 
 
 def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seqlen, scale, maps, status):
+    _no_tangents(qkv, param)
     n, D = qkv.shape[0], qkv.shape[1] // 3 // heads
     if D not in (16, 32, 64):
         raise ValueError("heads of %d values (supported: 16, 32, 64)" % D)

@@ -6,9 +6,12 @@ import subprocess
 
 import numpy as np
 import pytest
+import torch
+from torch.autograd import forward_ad
 
 from conftest import ROOT
 from pointtransformerv3_b200 import _lib
+from pointtransformerv3_b200 import functional as F
 
 
 def _source(name):
@@ -71,3 +74,39 @@ def test_look_ups_stay_in_the_table_whatever_the_coordinates_are(places, lowest,
         got = places(outside[0], outside[1], lowest, extent, first, reach, sign, step)
         far = (extent - reach) << step              # (beyond the table only where look-ups are held afterwards)
         assert got.min() >= first - far and got.max() <= first + ((2 * reach) << step) + far
+
+
+class _Cuda(torch.Tensor):
+    """A CPU tensor that says it is on the GPU, for checks that come before any kernel."""
+    is_cuda = True
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Cuda)
+
+
+def plan(n=8):
+    return [t(n, dtype=torch.int64) for _ in range(3)] + [t(2, dtype=torch.int32)]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("call", [
+    lambda d: F.qk_norm_rope(d(t(8, 48)), 1, None, t(16), t(16)),
+    lambda d: F.qk_norm_rope(t(8, 48), 1, None, d(t(16)), t(16)),
+    lambda d: F.qk_norm_rope(t(8, 48), 1, None, t(16), d(t(16))),
+    lambda d: F.attention_bias(d(t(8, 48)), *plan(), 1, 8),
+    lambda d: F.attention_bias(t(8, 48), *plan(), 1, 8, grid_coord=t(8, 3, dtype=torch.int32), table=d(t(9, 1))),
+    lambda d: F.attention_diff(d(t(8, 48)), t(1), *plan(), 1, 8),
+    lambda d: F.attention_diff(t(8, 48), d(t(1)), *plan(), 1, 8),
+])
+def test_tangents_are_refused(call, grad):
+    """Forward-mode derivatives would be lost, with a graph and without one."""
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(lambda x: forward_ad.make_dual(x.requires_grad_(grad), torch.ones_like(x)))
+
+
+def test_a_level_without_tangents_is_no_reason_to_refuse():
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="max_seqlen"):          # (the check behind)
+            F.attention_bias(t(8, 48), *plan(), 1, 0)

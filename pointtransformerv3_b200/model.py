@@ -165,7 +165,9 @@ class SerializedAttention(PointModule):
     on -> patch = patch_size with shorter scenes as one short sequence.
 
     In training mode the module has gradients, of its parameters and of the features it is given (heads of 16, 32 or
-    64 channels, no ``attn_drop``).  Options beyond the reference's, in either mode:
+    64 channels, no ``attn_drop``).  Options beyond the reference's, in either mode, with gradients in evaluation too
+    where autograd is on (``core`` by itself has a graph in training mode only, and without options evaluation runs
+    the inference kernels, which have none):
     ``qk_norm``        queries and keys of every head divided by their root mean square, times a learned weight;
     ``enable_rope``    queries and keys rotated by the grid coordinates (``rope_base``: of the frequencies);
     ``rpe_bound``      the bias of ``enable_rpe`` over offsets up to that many cells, in widening buckets;
@@ -214,6 +216,13 @@ class SerializedAttention(PointModule):
         """Whether this is the attention that the one-call block and backbone know."""
         return not (self.enable_rpe or self.enable_rope or self.q_norm is not None or self.lam is not None)
 
+    def _learns(self, feat):
+        """Whether a call has gradients: in training mode, and with options beyond the reference's wherever autograd asks."""
+        options = (self.q_norm is not None or self.enable_rope or self.lam is not None
+                   or (self.enable_rpe and self.rpe.buckets is not None))
+        return self.training or (options and torch.is_grad_enabled()
+                                 and (feat.requires_grad or any(p.requires_grad for p in self.parameters())))
+
     @torch.no_grad()
     def get_padding_and_inverse(self, point):
         """model.py:382-438; cached in the Point under the reference's keys.
@@ -234,11 +243,14 @@ class SerializedAttention(PointModule):
     def core(self, point, qkv):
         """Patch attention of an already projected (N, 3C) qkv matrix over
         ``point``'s serialized order; the output projection is not applied."""
+        return self._core(point, qkv, self.training)
+
+    def _core(self, point, qkv, learns):
         assert not (self.training and self.attn_drop), "no dropout of probabilities"
         if not self.enable_flash:
             self.patch_size = min(min(point.host_counts()), self.patch_size_max)
         pad, unpad, cu_seqlens = self.get_padding_and_inverse(point)
-        with torch.set_grad_enabled(self.training and torch.is_grad_enabled()):
+        with torch.set_grad_enabled(learns and torch.is_grad_enabled()):
             if self.q_norm is not None or self.enable_rope:
                 qkv = functional.qk_norm_rope(qkv, self.num_heads * self.maps, point.grid_coord if self.enable_rope else None,
                                               self.q_norm, self.k_norm, base=self.rope_base)
@@ -246,7 +258,7 @@ class SerializedAttention(PointModule):
                         self.scale)
             if self.lam is not None:
                 return functional.attention_diff(qkv, self.lam, *geometry, status=point.device_status())
-            if self.training or (self.enable_rpe and self.rpe.buckets is not None):
+            if learns or (self.enable_rpe and self.rpe.buckets is not None):
                 bias = {}
                 if self.enable_rpe:
                     bias = dict(grid_coord=point.grid_coord, table=self.rpe.rpe_table, buckets=self.rpe.buckets)
@@ -261,8 +273,8 @@ class SerializedAttention(PointModule):
 
     def attend(self, point, feat):
         """qkv projection, patch attention and output projection of ``feat``."""
-        if self.training:
-            return self.proj_drop(self.proj(self.core(point, self.qkv(feat))))
+        if self._learns(feat):
+            return self.proj_drop(self.proj(self._core(point, self.qkv(feat), True)))
         status = point.device_status()
         return self.proj_drop(_linear_op(self.core(point, _linear_op(feat, self.qkv, status)), self.proj, status))
 

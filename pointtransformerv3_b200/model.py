@@ -458,6 +458,7 @@ class Block(PointModule):
         status = point.device_status()
         C, dt = self.channels, shortcut.dtype
         attn, lin = self.attn, self.cpe[1]
+        assert not attn.training, "inference only"          # (no operator around it has a gradient)
         # the convolution reads the sparse tensor's features, which differ from
         # `feat` right after an unpooling (model.py:233-236, 744-746)
         x = self.cpe[0](sparse).features

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import pointtransformerv3_b200 as P
 from helpers import rel_l2
 from test_attention_options_gpu import OPTIONS, module, reference, scene
 
@@ -39,3 +40,18 @@ def test_gradients_in_evaluation(name, dtype):
     with torch.no_grad():
         out = att(pt).feat
     assert not out.requires_grad and rel_l2(out, want) < tol
+
+
+def test_a_block_does_not_train_its_attention_alone():
+    """Operators around the attention have no gradients, so a block in evaluation refuses an attention in training."""
+    torch.manual_seed(0)
+    block = P.Block(64, 4, 128, cpe_indice_key="s", upcast_attention=False, upcast_softmax=False,
+                    attn_options=dict(qk_norm=True)).cuda().eval()
+    pt, feat, _ = scene([200], 5, 64, torch.float32)
+    pt.feat = feat
+    pt.sparsify()
+    with torch.no_grad():
+        block(P.Point(dict(pt)))
+    block.attn.train()
+    with pytest.raises(AssertionError, match="inference only"):
+        block(P.Point(dict(pt)))

@@ -214,6 +214,7 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
  *               not follow one another from row 0 to n_pad or are longer than max_seqlen, coordinates or buckets out of
  *               range.  All accesses stay within the tensors then, and what is left in them is undefined
  *   table       3 * num_buckets x heads, lam heads: fp32 or bf16 (table_dtype, lam_dtype); gradients in the same type
+ *               (finite entries beyond 2.9e37 in size count as that, so that a score of three is finite)
  *   lse         2 * heads * maps * n_pad fp32, and with maps = 2 second, n x channels like out: what _bwd needs of the softmax
  *               and of the second map, written by _fwd (not where lse is NULL)
  *   _bwd        writes dqkv, and dtable / dlam where not NULL, from qkv, out, lse, second and dout

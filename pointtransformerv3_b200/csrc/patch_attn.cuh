@@ -8,8 +8,8 @@
 //   dtable[a][b] = sum of dS_1 over the pairs whose offset along axis a falls into bucket b
 //
 // A backward pass is two kernels, one that walks keys for each block of queries (delta, dQ) and one that walks
-// queries for each block of keys (dK, dV, dtable): both compute scores and probabilities again from the saved logarithm
-// of the softmax's sum, nothing of size L x L is stored and no float is added atomically, so results do not
+// queries for each block of keys (dK, dV, dtable): both compute scores and probabilities again from the softmax's saved
+// reference value and sum, nothing of size L x L is stored and no float is added atomically, so results do not
 // depend on the order of anything.
 //
 // delta in one walk: the stored result gives an estimate, delta' = dO . O (dO . O2 for the second map, whose O2 the
@@ -30,6 +30,11 @@
 namespace ptv3 {
 
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
+// Where a running maximum starts: no finite score is lower, and what it leaves of a sum (2^(start - score)) is 0 or, at that score, 1.
+constexpr float PA_LOWEST = -3.402823466e38f;
+// Finite entries of a table are held within this, in powers of two, so that three of them and a product are finite: a row whose
+// every key is masked by the lowest value of a type is softmax's row of its least masked keys, as it is in 64 bits.
+constexpr float PA_FAR = 4.2535296e37f;               // 2^125
 constexpr int PA_MAX_BOUND = 512;
 constexpr int PA_MAX_COORD = 1 << 22;                 // coordinates of a bias lie within this of zero
 constexpr int PA_TABLE_BYTES = 80 * 1024;             // shared memory for a head's table, so that two CTAs fit an SM;
@@ -51,8 +56,8 @@ struct PatchArgs {
     const int32_t* extent;      // n_seq x 6: largest offset within a sequence along each axis, and its lowest coordinates
     const void* lam;            // H
     int lam_bf16;
-    float* lse;                 // (H maps) x n_pad: log2 of the softmax's sum (bf16), or twice that: its reference
-                                // value in log2, then one over the sum (fp32); or NULL
+    float* lse;                 // twice (H maps) x n_pad: the softmax's reference value in log2, then one over its sum (not the
+                                // logarithm of the sum, in which a reference far from zero leaves no bits for the sum); or NULL
     const void* dout;
     void* dqkv;
     void* second;               // n x C: O2, with two maps
@@ -131,7 +136,8 @@ __device__ __forceinline__ void pa_load_table(const PatchArgs& a, const PatchTab
         const int e = min(max(d, -a.bnd), a.bnd) + a.bnd;
         int b = a.buckets ? a.buckets[e] : e;
         b = min(max(b, 0), a.num - 1);                     // (patch_rows_kernel reports one out of range)
-        const float v = pa_param(a.table, (axis * a.num + b) * a.H + h, a.table_bf16) * PA_LOG2E;
+        const float entry = pa_param(a.table, (axis * a.num + b) * a.H + h, a.table_bf16);
+        const float v = fabsf(entry) < INFINITY ? fminf(fmaxf(entry * PA_LOG2E, -PA_FAR), PA_FAR) : entry;
         for (int c = 0; c < copies; ++c) tab[(i << t.copies_log2) + ((c + tid) & (copies - 1))] = v;
     }
 }

@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
         for (int i = 0; i < bias.AXES; ++i) bias.g[i] = pa_coord(a, p, bias.axis[i]);
 #pragma unroll
     for (int k = 0; k < MAPS; ++k) {
-        m[k] = -1e30f;          // (finite: scores may all be -inf)
+        m[k] = PA_LOWEST;       // (finite: scores may all be -inf)
         l[k] = 0.f;
         since[k] = 1.f;
 #pragma unroll

@@ -29,19 +29,19 @@ struct PmTableBytes {
 };
 constexpr int PM_STAGES = 3;
 constexpr int PM_WINDOW = 256;     // queries between two clearings of the table's bins
+constexpr float PM_NEAR = 1024.f;  // references this near zero leave the sum's logarithm 2^-14 of a power of two: less than bf16 shows
 constexpr float PM_LAZY = 8.f;     // slack of the running maximum, in powers of two
 // bytes for the sums of the bins: entries of a table of eight copies, or of the largest bound (patch_attn.cuh)
 static int pm_sums_bytes(int bnd, int bins_bytes)
 {
     return (3 * (2 * bnd + 1) > bins_bytes / 64 ? 3 * (2 * bnd + 1) : bins_bytes / 64) * 4;
 }
-constexpr float PM_LOWEST = -1e30f;
 
 template <int W, int CH>
 struct PmStage {
     static constexpr int TILE = CH * W * 2;            // bytes of a matrix
-    static constexpr int AUX = 2 * TILE;               // two words of each map and row
-    static constexpr int GRID = AUX + 4 * CH * 4;
+    static constexpr int AUX = 2 * TILE;               // three words of each map and row
+    static constexpr int GRID = AUX + 3 * CH * 4;      // coordinates, where there is a bias and one map; or the second map's words
     static constexpr int BYTES = GRID + 3 * CH * 4;
 };
 
@@ -92,11 +92,18 @@ __device__ __forceinline__ void pm_add_shared(uint32_t addr, int v)
     asm volatile("red.shared.add.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// The other side's rows: x and y (head h's W values of each), two words of each map (AUX), coordinates (BIAS)
+// The other side's rows: x and y (head h's W values of each), three words of each map (AUX), coordinates (BIAS).  The words are
+// r, f and -delta of P = f 2^(score + r): near zero r takes the logarithm of the softmax's sum in, and f is 1 or -lam; a reference
+// further off has no bits for it, so f is that over the sum, and the chunk is marked.  (100 000 x 64, columns: of two maps 320 us, 364 with f
+// multiplied always.  With a bias, whose tables mask, always: 809 us, 783 without f.)  Words and coordinates are spread over the threads
+// of a block, so that no warp comes late to a chunk (rows 447 -> 432 us).
 template <int W, int MAPS, bool AUX, bool BIAS, int NT>
 struct PmStream {
     static constexpr int CH = PmChunk<W, BIAS, NT>::N;
-    static constexpr int RPP = NT / 4, NR = CH / RPP, NA = AUX ? (2 * MAPS * CH + NT - 1) / NT : 1;
+    static constexpr int RPP = NT / 4, NR = CH / RPP, NG = BIAS ? (3 * CH + NT - 1) / NT : 1;
+    // with a bias a thread has one word at a time, otherwise the three of a row
+    static constexpr int NA = !AUX ? 1 : ((BIAS ? 3 : MAPS) * CH + NT - 1) / NT, AW = BIAS ? 1 : 3;
+    static_assert(!(BIAS && MAPS == 2), "coordinates lie where the second map's words do");
     using S = PmStage<W, CH>;
     const PatchArgs& a;
     const __nv_bfloat16 *x, *y;
@@ -104,38 +111,56 @@ struct PmStream {
     int seq, start, L, h;
     bool owners;             // rows of y that answer for no point are taken as zeros
     int step;                // coordinates are kept times 2^step
+    float second;            // factor of the second map
+    int* marks;              // of the stages: 1 + the last chunk there with a reference far from zero
     unsigned char* smem;
-    int e[NR], eg, ea[NA], g[3];
-    float aux[NA];
+    int e[NR], eg[NG], ea[NA], g[NG], lowest[NG], extent[NG];
+    float aux[NA][AW];
 
     __device__ __forceinline__ int row_of(int chunk, int j) const
     {
         const int r = chunk * CH + j;
         return r < L ? a.rows[start + r] : INT_MIN;
     }
+    // this thread's i-th coordinate of a chunk: of row k % CH along axis k / CH
+    static __device__ __forceinline__ int grid_slot(int i) { return threadIdx.x + i * NT; }
     // (of rows beyond the last the last one's: places in the table stay within it)
-    __device__ __forceinline__ int grid_row(int chunk) const
+    __device__ __forceinline__ void fetch_rows(int chunk)
     {
-        return a.rows[start + min(chunk * CH + (int)threadIdx.x, L - 1)];
+        if (BIAS)
+#pragma unroll
+            for (int i = 0; i < NG; ++i)
+                if (grid_slot(i) < 3 * CH) eg[i] = a.rows[start + min(chunk * CH + grid_slot(i) % CH, L - 1)];
     }
     __device__ __forceinline__ void fetch_grid()
     {
-        if (BIAS && threadIdx.x < CH) {
-            const int64_t p = eg >= 0 ? eg : -(eg + 1);
+        if (BIAS)
 #pragma unroll
-            for (int c = 0; c < 3; ++c) g[c] = a.grid[3 * p + c];
-        }
+            for (int i = 0; i < NG; ++i)
+                if (grid_slot(i) < 3 * CH)
+                    g[i] = a.grid[3 * (int64_t)(eg[i] >= 0 ? eg[i] : -(eg[i] + 1)) + grid_slot(i) / CH];
     }
+    // its i-th word, or three (with a bias other threads than the first have two of these)
+    static __device__ __forceinline__ int aux_slot(int i) { return (BIAS ? (threadIdx.x + NT - CH) % NT : threadIdx.x) + i * NT; }
     __device__ __forceinline__ void fetch_aux(int chunk)
     {
+        const int64_t all = (int64_t)a.H * MAPS * a.n_pad;
         if (AUX)
 #pragma unroll
             for (int i = 0; i < NA; ++i) {
-                const int k = threadIdx.x + i * NT, j = k % CH, what = k / CH, r = chunk * CH + j;
-                ea[i] = k < 2 * MAPS * CH ? row_of(chunk, j) : INT_MIN;
-                aux[i] = 0.f;
-                if (ea[i] != INT_MIN)
-                    aux[i] = (what < MAPS ? a.lse : a.delta)[(int64_t)(h * MAPS + what % MAPS) * a.n_pad + start + r];
+                const int k = aux_slot(i), what = k / CH;
+                ea[i] = k < (BIAS ? 3 : MAPS) * CH ? row_of(chunk, k % CH) : INT_MIN;
+#pragma unroll
+                for (int c = 0; c < AW; ++c) aux[i][c] = 0.f;
+                if (ea[i] < 0) continue;
+                const int64_t at = (int64_t)(h * MAPS + (BIAS ? 0 : what)) * a.n_pad + start + chunk * CH + k % CH;
+                if (BIAS) {
+                    aux[i][0] = what == 2 ? a.delta[at] : a.lse[what == 1 ? at + all : at];
+                } else {
+                    aux[i][0] = a.lse[at];
+                    aux[i][AW / 2] = a.lse[at + all];
+                    aux[i][AW - 1] = a.delta[at];
+                }
             }
     }
     // what issue(chunk) needs in registers
@@ -144,7 +169,7 @@ struct PmStream {
 #pragma unroll
         for (int i = 0; i < NR; ++i) e[i] = row_of(chunk, (threadIdx.x >> 2) + RPP * i);
         fetch_grid();
-        if (BIAS && threadIdx.x < CH) eg = grid_row(chunk + 1);
+        fetch_rows(chunk + 1);
         fetch_aux(chunk);
     }
     __device__ __forceinline__ void issue(int chunk)
@@ -168,21 +193,39 @@ struct PmStream {
             if (AUX)
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
-                    const int k = threadIdx.x + i * NT;
-                    // negated; rows that are not there, or answer for no point: probabilities of nothing
-                    if (k < 2 * MAPS * CH)
-                        ((float*)(st + S::AUX))[k] = ea[i] >= 0 ? -aux[i] : k < MAPS * CH ? -INFINITY : 0.f;
+                    const int k = aux_slot(i);
+                    float* to = (float*)(st + S::AUX) + k;
+                    // rows that are not there, or answer for no point: probabilities of nothing
+                    const bool there = ea[i] >= 0;
+                    if (BIAS) {
+                        if (k < 3 * CH) to[0] = k < CH && !there ? -INFINITY : k / CH == 1 ? aux[i][0] : -aux[i][0];
+                    } else if (k < MAPS * CH) {
+                        const bool far = there && !(fabsf(aux[i][0]) < PM_NEAR);
+                        const float f = k < CH ? 1.f : second, inv = aux[i][AW / 2];
+                        to[0] = !there ? -INFINITY : far ? -aux[i][0] : log2f(inv) - aux[i][0];
+                        to[MAPS * CH] = !there ? 0.f : far ? f * inv : f;
+                        to[2 * MAPS * CH] = -aux[i][AW - 1];
+                        if (far) marks[chunk % PM_STAGES] = chunk + 1;
+                    }
                 }
-            if (BIAS && threadIdx.x < CH)
+            if (BIAS)
 #pragma unroll
-                for (int c = 0; c < 3; ++c)
-                    ((int*)(st + S::GRID))[c * CH + threadIdx.x] = pa_other(pm_box(a, seq, g[c], c), step);
+                for (int i = 0; i < NG; ++i)
+                    if (grid_slot(i) < 3 * CH)
+                        ((int*)(st + S::GRID))[grid_slot(i)] = pa_other(pa_held(g[i], lowest[i], extent[i]), step);
         }
         cp_async_commit();
     }
     __device__ __forceinline__ void begin()
     {
-        if (BIAS && threadIdx.x < CH) eg = grid_row(0);
+        if (BIAS)
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const int axis = min(grid_slot(i) / CH, 2);
+                extent[i] = a.extent[6 * seq + axis];
+                lowest[i] = a.extent[6 * seq + 3 + axis];
+            }
+        fetch_rows(0);
         fetch(0);
         issue(0);
         fetch(1);
@@ -437,7 +480,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
     PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
-                                         table.copies_log2 + 2, smem};
+                                         table.copies_log2 + 2, 0.f, nullptr, smem};
     in.begin();
     PmBias bias;
     int point[RT][2][3];
@@ -460,7 +503,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
     for (int k = 0; k < MAPS; ++k)
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
-            m[k][x][0] = m[k][x][1] = PM_LOWEST;
+            m[k][x][0] = m[k][x][1] = PA_LOWEST;
             l[k][x][0] = l[k][x][1] = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -583,8 +626,11 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
                     float v = hsum2(l[k][x][r]);
                     v += __shfl_xor_sync(0xffffffffu, v, 1);
                     v += __shfl_xor_sync(0xffffffffu, v, 2);
-                    if (t == 0 && e >= 0)
-                        a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r]] = m[k][x][r] + log2f(v);
+                    if (t == 0 && e >= 0) {
+                        float* to = a.lse + (int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r];
+                        *to = m[k][x][r];
+                        to[(int64_t)a.H * MAPS * a.n_pad] = 1.f / v;
+                    }
                 }
             if (e < 0) continue;
             const float w0 = 1.f / sum[0][x][2 * r], w2 = 1.f / sum[MAPS - 1][x][2 * r], w1 = lam * w2;
@@ -644,7 +690,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
     PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
-                                         table.copies_log2 + 2, smem};
+                                         table.copies_log2 + 2, 0.f, nullptr, smem};
     in.begin();
     PmBias bias;
     int point[RT][2][3];
@@ -658,7 +704,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
             for (int r = 0; r < 2; ++r) pm_bias_point(a, table, bias, w, own.row[x][r], 1, point[x][r]);
     }
     uint32_t q[RT][W / 16][4], go[RT][W / 16][4];
-    float lse[MAPS][RT][2], shift[MAPS][RT][2], most[RT][2];
+    float ref[MAPS][RT][2], shift[MAPS][RT][2], most[RT][2];
     uint64_t E[MAPS][RT][2], total[MAPS][RT][2];
     const float lam = MAPS == 2 ? pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
     pm_own_rows<W, RT>(own, (const __nv_bfloat16*)a.dout + w.h * W, a.C, 0u, go);
@@ -688,7 +734,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
         for (int k = 0; k < MAPS; ++k)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                lse[k][x][r] = own.e[x][r] >= 0 ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r]]
+                ref[k][x][r] = own.e[x][r] >= 0 ? a.lse[(int64_t)(w.h * MAPS + k) * a.n_pad + w.start + own.row[x][r]]
                                                 : INFINITY;
                 E[k][x][r] = total[k][x][r] = 0;
             }
@@ -741,8 +787,8 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 const uint64_t v = pack2(s[x][k][n][2 * r], s[x][k][n][2 * r + 1]);
-                                const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-lse[k][x][r]))
-                                                                 : fma2(v, pm_both(scale2), pm_both(-lse[k][x][r])));
+                                const uint64_t pr = pm_exp2(BIAS ? add2(v, pm_both(-ref[k][x][r]))
+                                                                 : fma2(v, pm_both(scale2), pm_both(-ref[k][x][r])));
                                 total[k][x][r] = add2(total[k][x][r], pr);
                                 const uint64_t ds = mul2(pr, add2(pack2(G[x][0][n][2 * r], G[x][0][n][2 * r + 1]),
                                                                   pm_both(-shift[k][x][r])));
@@ -773,7 +819,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
             float by[MAPS], eps[MAPS];
 #pragma unroll
             for (int k = 0; k < MAPS; ++k) {
-                // the saved logarithm is rounded to 2^-24 of itself, which a whole row's probabilities share: divided out
+                // (probabilities so far are times their row's sum)
                 const float sum = quad(hsum2(total[k][x][r])), inv = e >= 0 ? 1.f / sum : 0.f;
                 eps[k] = quad(hsum2(E[k][x][r])) * inv;
                 by[k] = inv * a.scale * (k == 1 ? -lam : 1.f);
@@ -804,6 +850,7 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
     using S = PmStage<W, CH>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float part[4 * NT / 32];
+    __shared__ int marks[PM_STAGES];       // (as they come: a chunk taken for marked is as right, and slower)
     const PmPlace w = pm_place(a);
     const int k0 = w.tile * (NT / 2) * RT, L = w.L;
     const bool learns = BIAS && a.bins;
@@ -820,8 +867,9 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::BINS, true);
+    const float minus_lam = MAPS == 2 ? -pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
     PmStream<W, MAPS, true, BIAS, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.seq, w.start, L, w.h, true,
-                                        table.copies_log2 + 2, smem};
+                                        table.copies_log2 + 2, minus_lam, marks, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);
     int* hist = (int*)(tab + (BIAS ? table.entries << table.copies_log2 : 0));
@@ -858,7 +906,6 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
         pm_rows<W>(p[0] ? p[0] + a.C : nullptr, p[1] ? p[1] + a.C : nullptr, 0u, vf[x]);
     }
     const float scale2 = a.scale * PA_LOG2E;
-    const float minus_lam = MAPS == 2 ? -pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
     float dk[RT][W / 8][4], dv[RT][W / 8][4];
 #pragma unroll
     for (int x = 0; x < RT; ++x)
@@ -867,8 +914,73 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
 #pragma unroll
             for (int c = 0; c < 4; ++c) dk[x][n][c] = dv[x][n][c] = 0.f;
 
+    auto chunk = [&](int i, const unsigned char* st, auto clamp, auto far) {
+        constexpr bool CLAMP = decltype(clamp)::value, FAR = decltype(far)::value;
+        const uint32_t qs = smem_u32(st), os = qs + S::TILE;
+        const float* aux = (const float*)(st + S::AUX);
+        const int* gs = (const int*)(st + S::GRID);
+        const int nq = L - i * CH;
+#pragma unroll (2 / RT)
+        for (int j0 = 0; j0 < CH; j0 += 16) {
+            if (j0 >= nq) break;
+            uint32_t p[RT][MAPS][4], pm[RT][1][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int j = j0 + 8 * n + 2 * t;
+                float s[RT][MAPS][4], G[RT][1][4];
+                pm_products8<W, MAPS, RT>(kf, qs, j0 + 8 * n, s);
+                pm_products8<W, 1, RT>(vf, os, j0 + 8 * n, G);
+                int2 g[3];
+                if (BIAS) pm_coords<CH>(gs, j, g);
+                uint64_t ref[MAPS], coef[MAPS], delta[MAPS];
+#pragma unroll
+                for (int k = 0; k < MAPS; ++k) {
+                    ref[k] = *(const uint64_t*)(aux + k * CH + j);
+                    if (FAR) coef[k] = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
+                    delta[k] = *(const uint64_t*)(aux + (2 * MAPS + k) * CH + j);
+                }
+#pragma unroll
+                for (int x = 0; x < RT; ++x) {
+                    uint32_t at[4][3];
+                    if (BIAS) {
+                        pm_places<-1, CLAMP>(bias, point[x], g, at);
+                        pm_bias(at, scale2, s[x][0]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        uint64_t mix = 0;
+#pragma unroll
+                        for (int k = 0; k < MAPS; ++k) {
+                            const uint64_t v = pack2(s[x][k][2 * r], s[x][k][2 * r + 1]);
+                            uint64_t pr = pm_exp2(BIAS ? add2(v, ref[k]) : fma2(v, pm_both(scale2), ref[k]));
+                            if (FAR) pr = mul2(pr, coef[k]);
+                            else if (k == 1) pr = mul2(pr, pm_both(minus_lam));
+                            mix = k == 0 ? pr : add2(mix, pr);
+                            const uint64_t ds = mul2(pr, add2(pack2(G[x][0][2 * r], G[x][0][2 * r + 1]), delta[k]));
+                            float y, z;
+                            unpack2(ds, y, z);
+                            p[x][k][2 * n + r] = pack_bf16(y, z);
+                            // (rows beyond the patch have no key: their lanes add nothing)
+                            if (learns && own.row[x][r] < L) {
+                                const int vy = __float2int_rn(y * per_unit), vz = __float2int_rn(z * per_unit);
+#pragma unroll
+                                for (int c = 0; c < 3; ++c) {
+                                    pm_add_shared((at[2 * r][c] >> fewer) + to_hist, vy);
+                                    pm_add_shared((at[2 * r + 1][c] >> fewer) + to_hist, vz);
+                                }
+                            }
+                        }
+                        float y, z;
+                        unpack2(mix, y, z);
+                        pm[x][0][2 * n + r] = pack_bf16(y, z);
+                    }
+                }
+            }
+            pm_accumulate<W, 1, RT>(pm, os, j0, dv, pm, dv);
+            pm_accumulate<W, MAPS, RT>(p, qs, j0, dk, p, dk);
+        }
+    };
     auto walk = [&](auto clamp) {
-        constexpr bool CLAMP = decltype(clamp)::value;
         for (int i = 0; i * CH < L; ++i) {
             if (learns && i % (PM_WINDOW / CH) == 0) {
                 if (i) {
@@ -880,67 +992,8 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
             }
             const unsigned char* st = in.next(i);
             if (warp0 >= L) continue;
-            const uint32_t qs = smem_u32(st), os = qs + S::TILE;
-            const float* aux = (const float*)(st + S::AUX);
-            const int* gs = (const int*)(st + S::GRID);
-            const int nq = L - i * CH;
-#pragma unroll (2 / RT)
-            for (int j0 = 0; j0 < CH; j0 += 16) {
-                if (j0 >= nq) break;
-                uint32_t p[RT][MAPS][4], pm[RT][1][4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int j = j0 + 8 * n + 2 * t;
-                    float s[RT][MAPS][4], G[RT][1][4];
-                    pm_products8<W, MAPS, RT>(kf, qs, j0 + 8 * n, s);
-                    pm_products8<W, 1, RT>(vf, os, j0 + 8 * n, G);
-                    int2 g[3];
-                    if (BIAS) pm_coords<CH>(gs, j, g);
-                    uint64_t lse[MAPS], delta[MAPS];      // (negated as they are staged)
-#pragma unroll
-                    for (int k = 0; k < MAPS; ++k) {
-                        lse[k] = *(const uint64_t*)(aux + k * CH + j);
-                        delta[k] = *(const uint64_t*)(aux + (MAPS + k) * CH + j);
-                    }
-#pragma unroll
-                    for (int x = 0; x < RT; ++x) {
-                        uint32_t at[4][3];
-                        if (BIAS) {
-                            pm_places<-1, CLAMP>(bias, point[x], g, at);
-                            pm_bias(at, scale2, s[x][0]);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            uint64_t mix = 0;
-#pragma unroll
-                            for (int k = 0; k < MAPS; ++k) {
-                                const uint64_t v = pack2(s[x][k][2 * r], s[x][k][2 * r + 1]);
-                                uint64_t pr = pm_exp2(BIAS ? add2(v, lse[k]) : fma2(v, pm_both(scale2), lse[k]));
-                                if (k == 1) pr = mul2(pr, pm_both(minus_lam));
-                                mix = k == 0 ? pr : add2(mix, pr);
-                                const uint64_t ds = mul2(pr, add2(pack2(G[x][0][2 * r], G[x][0][2 * r + 1]), delta[k]));
-                                float y, z;
-                                unpack2(ds, y, z);
-                                p[x][k][2 * n + r] = pack_bf16(y, z);
-                                // (rows beyond the patch have no key: their lanes add nothing)
-                                if (learns && own.row[x][r] < L) {
-                                    const int vy = __float2int_rn(y * per_unit), vz = __float2int_rn(z * per_unit);
-#pragma unroll
-                                    for (int c = 0; c < 3; ++c) {
-                                        pm_add_shared((at[2 * r][c] >> fewer) + to_hist, vy);
-                                        pm_add_shared((at[2 * r + 1][c] >> fewer) + to_hist, vz);
-                                    }
-                                }
-                            }
-                            float y, z;
-                            unpack2(mix, y, z);
-                            pm[x][0][2 * n + r] = pack_bf16(y, z);
-                        }
-                    }
-                }
-                pm_accumulate<W, 1, RT>(pm, os, j0, dv, pm, dv);
-                pm_accumulate<W, MAPS, RT>(p, qs, j0, dk, p, dk);
-            }
+            if (BIAS || marks[i % PM_STAGES] == i + 1) chunk(i, st, clamp, PmYes());
+            else chunk(i, st, clamp, PmNo());
         }
     };
     if (BIAS && table.clamps) walk(PmYes());

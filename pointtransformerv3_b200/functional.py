@@ -216,7 +216,8 @@ def attention_bias(qkv, order_row, pad, unpad, cu_seqlens, heads, max_seqlen, sc
     the sum over the axes a of table[a * num + bucket(grid_coord[i, a] - grid_coord[j, a]), head]; table (3 num, heads), fp32 or
     bf16, grid_coord (N, 3) integers within 2^22 of zero.  ``buckets`` (2 bound + 1,) int32 gives the bucket of every offset -bound .. bound,
     those beyond going with the outermost (``log_buckets``); without it every offset has its own, num = 2 bound + 1, which is
-    the bias of ``RPE``.  Without a table there is no bias.
+    the bias of ``RPE``.  Without a table there is no bias.  Finite entries beyond 2.9e37 in size count as that: a row whose every key is masked
+    by a type's lowest value attends to its least masked keys, one whose every key is masked by minus infinity is NaN.
 
     status: a device status word of the caller's (``ops.new_status``), in which a plan, coordinates or buckets out of range are reported; the caller
     checks it when the host next waits.  Without one the call checks for itself and waits for the device.

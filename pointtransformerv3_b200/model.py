@@ -258,7 +258,8 @@ class SerializedAttention(PointModule):
                         self.scale)
             if self.lam is not None:
                 return functional.attention_diff(qkv, self.lam, *geometry, status=point.device_status())
-            if learns or (self.enable_rpe and self.rpe.buckets is not None):
+            if learns or (self.enable_rpe and (self.rpe.buckets is not None
+                                               or self.rpe.pos_bnd > ops.ATTENTION_RPE_MAX_BOUND)):
                 bias = {}
                 if self.enable_rpe:
                     bias = dict(grid_coord=point.grid_coord, table=self.rpe.rpe_table, buckets=self.rpe.buckets)

@@ -188,6 +188,9 @@ def attention(qkv, order_row, pad, unpad, cu_seqlens, heads, max_seqlen, scale, 
     return out
 
 
+ATTENTION_RPE_MAX_BOUND = 64       # of ptv3_attention_rpe_fwd's table
+
+
 def attention_rpe(qkv, order_row, pad, unpad, cu_seqlens, grid_coord, rpe_table, pos_bnd, heads, max_seqlen,
                   scale):
     """Patch attention with the relative position bias (see ptv3_attention_rpe_fwd)."""

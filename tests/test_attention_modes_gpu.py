@@ -55,3 +55,20 @@ def test_a_block_does_not_train_its_attention_alone():
     block.attn.train()
     with pytest.raises(AssertionError, match="inference only"):
         block(P.Point(dict(pt)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_a_bias_of_far_offsets_evaluates(dtype):
+    """Patches of 10 000 have a bias for offsets up to 68, more than the inference kernel's table holds: what trains evaluates."""
+    att = module("rpe", dtype, flash=False, K=10000)
+    assert att.rpe.pos_bnd == 68
+    pt, feat, dout = scene([300, 270], 61, 64, dtype)
+    outs = []
+    for training in (True, False):
+        att.train(training)
+        pt.feat = feat
+        with torch.no_grad():
+            outs.append(att(pt).feat)
+    want = reference(att, pt, feat, dout)[0]
+    for out in outs:
+        assert rel_l2(out, want) < (2e-5 if dtype == torch.float32 else 10 ** 0.5 * 2.0 ** -8)

@@ -275,9 +275,19 @@ class SerializedAttention(PointModule):
     def attend(self, point, feat):
         """qkv projection, patch attention and output projection of ``feat``."""
         if self._learns(feat):
-            return self.proj_drop(self.proj(self._core(point, self.qkv(feat), True)))
+            out = self.proj_drop(self.proj(self._core(point, self.qkv(feat), True)))
+            self._report(point)
+            return out
         status = point.device_status()
         return self.proj_drop(_linear_op(self.core(point, _linear_op(feat, self.qkv, status)), self.proj, status))
+
+    def _report(self, point):
+        """Raises for what the kernels found wrong with a plan or coordinates: once for a Point, an order and a patch size, as that
+        waits for the device.  A call that is being captured cannot, and leaves it to the status word."""
+        key, read = (self.order_index, self.patch_size), point.get("_attention_read", ())
+        if key not in read and not torch.cuda.is_current_stream_capturing():
+            point.check_status("SerializedAttention")
+            point["_attention_read"] = read + (key,)
 
     def forward(self, point):
         point.feat = self.attend(point, point.feat)

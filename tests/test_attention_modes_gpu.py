@@ -4,6 +4,7 @@ import torch
 
 import pointtransformerv3_b200 as P
 from helpers import rel_l2
+from pointtransformerv3_b200 import _lib, ops
 from test_attention_options_gpu import OPTIONS, module, reference, scene
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +73,49 @@ def test_a_bias_of_far_offsets_evaluates(dtype):
     want = reference(att, pt, feat, dout)[0]
     for out in outs:
         assert rel_l2(out, want) < (2e-5 if dtype == torch.float32 else 10 ** 0.5 * 2.0 ** -8)
+
+
+def test_what_does_not_hold_is_reported_in_training():
+    """Coordinates that the bias does not take, by the call itself and without a look at the status word."""
+    att = module("buckets", torch.float32, flash=False).train()
+    pt, feat, _ = scene([200, 150], 71, 64, torch.float32)
+    for bad in (True, False):
+        q = P.Point(dict(pt))
+        q["_status"] = ops.new_status("cuda")
+        q.feat = feat
+        if bad:
+            q.grid_coord = pt.grid_coord.clone()
+            q.grid_coord[7, 2] = 2 ** 22 + 1
+            with pytest.raises(_lib.Ptv3Error, match="SerializedAttention.*index or size out of range"):
+                att(q)
+        else:
+            att(q)
+
+
+def test_a_captured_step_does_not_wait():
+    """A Point that has not been reported on yet, in a step that is captured: forward and backward, replayed with other features."""
+    att = module("all_diff", torch.bfloat16, flash=True).train()
+    pt, feat, dout = scene([300, 100], 73, 64, torch.bfloat16)
+    x = feat.clone().requires_grad_()
+
+    def step(point):
+        point.feat = x
+        out = att(point).feat
+        return (out,) + torch.autograd.grad(out, [x] + list(att.parameters()), dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(P.Point(dict(pt)))
+    torch.cuda.current_stream().wait_stream(side)
+    fresh = P.Point(dict(pt))
+    att.get_padding_and_inverse(fresh)
+    fresh.device_status()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(fresh)
+    with torch.no_grad():
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(9)))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, step(P.Point(dict(pt)))))
+    fresh.check_status(force=True)

@@ -65,6 +65,7 @@ struct PatchArgs {
     float* reach;               // H x n_pad: no row's sum of |dS| is larger; or NULL
     float* shared;              // rows of (dK, dV), 2C
     float* bins;                // per block of keys: H x 3 (2 bnd + 1), or NULL
+    int bin_rows;               // rows of such a block, where blocks are numbered by rows (pa_bin_block); 0: by sequence and tile
 };
 
 // rows [start, start + L) of a sequence; L = 0 for what patch_rows_kernel reports
@@ -186,6 +187,30 @@ __device__ __forceinline__ void pa_flush(const PatchTable& t, int* hist, float* 
         sums[i] = fmaf(v, unit, sums[i]);
     }
 }
+// The bins of a block of keys and head; of a tile without keys, zeros are left there where nobody else does, and NULL is returned
+template <int ROWS>
+__device__ __forceinline__ float* pa_bins(const PatchArgs& a, int seq, int tile, int h, int start, int L, int threads)
+{
+    const int64_t size = 3 * (2 * a.bnd + 1);
+    auto at = [&](int64_t block) { return a.bins + (block * a.H + h) * size; };
+    auto clear = [&](int64_t block) {
+        for (int i = threadIdx.x; i < size; i += threads) at(block)[i] = 0.f;
+    };
+    const bool empty = tile * ROWS >= L;
+    if (!a.bin_rows) {
+        const int64_t block = (int64_t)seq * a.tiles + tile;
+        if (empty) clear(block);
+        return empty ? nullptr : at(block);
+    }
+    const int first = min(max(start, 0), a.n_pad);          // (of a sequence that does not hold)
+    const int64_t block = pa_bin_block(first, ROWS, seq, tile);
+    if (empty) {
+        if (tile == 0) clear(block);
+        return nullptr;
+    }
+    if ((tile + 1) * ROWS >= L && pa_bin_end(first + L, ROWS, seq) > block + 1) clear(block + 1);
+    return at(block);
+}
 // a block's sums of all offsets within the bound, those beyond with the outermost
 __device__ __forceinline__ void pa_store_bins(const PatchArgs& a, const PatchTable& t, const float* sums, float* bins, int threads)
 {
@@ -204,7 +229,7 @@ enum { PA_FWD = 0, PA_ROWS = 1, PA_COLS = 2 };
 // fp32 (patch_attn_fma.cu) and bf16 (patch_attn_mma.cu): a pass queued, `tiles` set by the rows that its blocks have
 int launch_patch_fma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
 int launch_patch_mma(const PatchArgs& a, int width, int maps, int pass, cudaStream_t stream);
-// rows of a block of the pass over columns with a bias, whose blocks leave bins
+// rows of a block of the pass over columns with a bias, whose blocks leave bins (PatchArgs::bin_rows)
 int patch_fma_cols_rows(int64_t longest, int width);
 int patch_mma_cols_rows(int64_t n_seq, int64_t longest, int heads, int width);
 

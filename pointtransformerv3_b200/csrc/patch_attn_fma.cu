@@ -464,12 +464,8 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_cols_kernel(const PatchA
     const int L = pa_sequence(a, seq, start);
     const int k0 = tile * S::ROWS, kj = k0 + threadIdx.x / SPLIT;
     const bool learns = BIAS && a.bins;
-    float* bins = learns ? a.bins + ((int64_t)(seq * a.tiles + tile) * a.H + h) * 3 * (2 * a.bnd + 1) : nullptr;
-    if (k0 >= L) {
-        if (learns)
-            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += PF_THREADS) bins[i] = 0.f;
-        return;
-    }
+    float* bins = learns ? pa_bins<S::ROWS>(a, seq, tile, h, start, L, PF_THREADS) : nullptr;
+    if (k0 >= L) return;
     const bool busy = k0 + threadIdx.x / 32 * 32 / SPLIT < L;
     const int64_t stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;

@@ -854,12 +854,8 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
     const PmPlace w = pm_place(a);
     const int k0 = w.tile * (NT / 2) * RT, L = w.L;
     const bool learns = BIAS && a.bins;
-    float* bins = learns ? a.bins + ((int64_t)(w.seq * a.tiles + w.tile) * a.H + w.h) * 3 * (2 * a.bnd + 1) : nullptr;
-    if (k0 >= L) {
-        if (learns)
-            for (int i = threadIdx.x; i < 3 * (2 * a.bnd + 1); i += NT) bins[i] = 0.f;
-        return;
-    }
+    float* bins = learns ? pa_bins<NT / 2 * RT>(a, w.seq, w.tile, w.h, w.start, L, NT) : nullptr;
+    if (k0 >= L) return;
     const int t = threadIdx.x & 3, warp0 = k0 + (int)(threadIdx.x / 32) * 16 * RT;
     PmOwn<RT> own;
     own.load(a, w, k0);

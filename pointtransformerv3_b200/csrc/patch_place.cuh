@@ -1,4 +1,5 @@
-// Where a pair of points looks into a head's table of biases (patch_attn.cuh); plain C++, so that it can be checked on the host.
+// Where a pair of points looks into a head's table of biases, and where a block of keys leaves the table's gradient (patch_attn.cuh); plain
+// C++, so that both can be checked on the host.
 #pragma once
 #include <stdint.h>
 
@@ -21,5 +22,11 @@ PTV3_PLACE int pa_held(int coord, int lowest, int extent)
 // This point's share of an entry's address: subtracting `sign` times pa_other of the other point gives the address
 PTV3_PLACE int pa_mine(int first, int reach, int held, int sign, int step) { return first + ((reach + sign * held) << step); }
 PTV3_PLACE int pa_other(int held, int step) { return held << step; }
+
+// Number of a block of `rows` keys, tile `tile` of a sequence that starts at row `start`: below n_pad / rows + n_seq, whatever the longest
+// sequence is.  Sequences have a number to spare at most, behind their last tile: where pa_bin_end is above that tile's number and one.
+PTV3_PLACE int64_t pa_bin_block(int start, int rows, int seq, int tile) { return (int64_t)(start / rows) + seq + tile; }
+// first number of the next sequence
+PTV3_PLACE int64_t pa_bin_end(int end, int rows, int seq) { return (int64_t)(end / rows) + seq + 1; }
 
 }  // namespace ptv3

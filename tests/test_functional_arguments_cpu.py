@@ -40,11 +40,16 @@ def test_weights_off_their_own_type_are_refused(dtype, step):
 
 
 @pytest.fixture(scope="module")
-def places(tmp_path_factory):
+def place_lib(tmp_path_factory):
     so = str(tmp_path_factory.mktemp("hostmath") / "libpatch_place_host.so")
     subprocess.check_call(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-o", so,
                            os.path.join(ROOT, "tests", "hostmath", "patch_place_host.cpp")])
-    lib = ctypes.CDLL(so)
+    return ctypes.CDLL(so)
+
+
+@pytest.fixture(scope="module")
+def places(place_lib):
+    lib = place_lib
     i, p = ctypes.c_int, ctypes.c_void_p
     lib.host_places.argtypes = [p, p, ctypes.c_int64, i, i, i, i, i, i, p]
 
@@ -74,6 +79,42 @@ def test_look_ups_stay_in_the_table_whatever_the_coordinates_are(places, lowest,
         got = places(outside[0], outside[1], lowest, extent, first, reach, sign, step)
         far = (extent - reach) << step              # (beyond the table only where look-ups are held afterwards)
         assert got.min() >= first - far and got.max() <= first + ((2 * reach) << step) + far
+
+
+@pytest.mark.parametrize("rows", [64, 128, 256])
+def test_blocks_of_keys_have_numbers_of_their_own(place_lib, rows):
+    """Numbered by rows, all blocks that leave a share of a table's gradient, and the numbers that are cleared, are each number below
+    n_pad / rows + n_seq once: the sum behind them reads nothing that was not written."""
+    rng = np.random.default_rng(rows)
+    out = np.empty(4096, dtype=np.int64)
+    for lengths in ([0], [1], [rows], [rows - 1, 1], [0, 0, 5 * rows + 3, 0], [20] * 500 + [1024], list(rng.integers(0, 700, 300)),
+                    list(rng.integers(0, 3, 300)), [rows * 7] * 20):
+        start, got = 0, []
+        for seq, n in enumerate(lengths):
+            count = place_lib.host_bins(start, int(n), rows, seq, ctypes.c_void_p(out.ctypes.data))
+            got += out[:count].tolist()
+            start += int(n)
+        assert got == list(range(start // rows + len(lengths)))
+
+
+def _workspace(n, n_pad, n_seq, longest, heads, bound, dtype):
+    args = _lib.PATCH_ATTENTION_ARGS.pack(n, n_pad, n_seq, longest, 16 * heads, heads, 1, dtype, 0.25, bound, 2 * bound + 1, 0, 0,
+                                          *([1 << 20] * 5), 1 << 20, 0, 1 << 20, 0, *([1 << 20] * 4), 0, 1 << 20, 1 << 20,
+                                          1 << 20, 0, 0, 0)
+    return _lib.load().ptv3_patch_attention_workspace_bytes(args)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_workspace_follows_the_rows(dtype):
+    """Many short sequences beside a long one: the table's gradient takes space for the blocks that there are, a number for each
+    sequence and one for every 64 rows at most; and of whole patches alone no more than their blocks."""
+    n, seqs, heads, bound = 400000 + 1500, 20002, 4, 512
+    entries = heads * 3 * (2 * bound + 1) * 4
+    per_row = 4 * (2 * heads + heads * 16 * 4)
+    got = _workspace(n, n + 548, seqs, 1024, heads, bound, dtype)
+    assert 0 < got <= (seqs + (n + 548) / 64) * entries * 65 / 64 + (n + 548) * per_row
+    got = _workspace(100 * 1024, 100 * 1024, 100, 1024, heads, bound, dtype)
+    assert 0 < got <= 100 * 1024 / 64 * entries * 65 / 64 + 100 * 1024 * per_row
 
 
 class _Cuda(torch.Tensor):

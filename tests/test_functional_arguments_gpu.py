@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import functional_norms as N
 import functional_reference as R
 from pointtransformerv3_b200 import functional as F
 from pointtransformerv3_b200 import ops
@@ -92,3 +93,24 @@ def test_coordinates_that_change_unseen_stay_in_the_table(width, dtype):
         assert all(bool(t.isfinite().all()) for t in grads())
     p["grid"].data.copy_(grid)
     assert all(torch.equal(a, b) for a, b in zip(first, grads()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("counts,patch", [([17] * 200 + [1500], 1024), ([1] * 300 + [700, 2], 512), ([600] + [33] * 90, 300)],
+                         ids=["17s", "1s", "33s"])
+def test_short_sequences_beside_a_long_one(counts, patch, dtype):
+    """Blocks of keys numbered by rows: results, gradients and the table's, and sequences of no rows among them."""
+    p = patches(counts, patch)
+    order, pad, unpad, cu = p["geometry"]
+    ends = cu.tolist()
+    cu = torch.tensor(ends[:1] * 3 + ends[1:40] + ends[39:40] * 2 + ends[40:] + ends[-1:], dtype=torch.int32, device="cuda")
+    for width, H in ((16, 2), (64, 1)):
+        C = width * H
+        qkv, dout = normal(p["n"], 3 * C, seed=1, dtype=dtype), normal(p["n"], C, seed=3, dtype=dtype)
+        buckets, num = F.log_buckets(130, device="cuda")
+        x, table = qkv.clone().requires_grad_(), normal(3 * num, H, seed=2, scale=0.5).requires_grad_()
+        out = F.attention_bias(x, order, pad, unpad, cu, H, p["longest"], grid_coord=p["grid"], table=table, buckets=buckets)
+        got = (out,) + torch.autograd.grad(out, (x, table), dout)
+        ref = R.attention(qkv, order, pad, unpad, cu, H, width ** -0.5, 1, table.detach(), p["grid"], 130, buckets, dout)
+        for name, t in zip(("out", "dqkv", "dparam"), got):
+            N.check(t.detach(), ref, name, qkv, dout, dtype)

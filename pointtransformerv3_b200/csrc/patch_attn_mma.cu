@@ -95,13 +95,14 @@ __device__ __forceinline__ void pm_add_shared(uint32_t addr, int v)
 // The other side's rows: x and y (head h's W values of each), three words of each map (AUX), coordinates (BIAS).  The words are
 // r, f and -delta of P = f 2^(score + r): near zero r takes the logarithm of the softmax's sum in, and f is 1 or -lam; a reference
 // further off has no bits for it, so f is that over the sum, and the chunk is marked.  (100 000 x 64, columns: of two maps 320 us, 364 with f
-// multiplied always.  With a bias, whose tables mask, always: 809 us, 783 without f.)  Words and coordinates are spread over the threads
-// of a block, so that no warp comes late to a chunk (rows 447 -> 432 us).
-template <int W, int MAPS, bool AUX, bool BIAS, int NT>
+// multiplied always.  With a bias, whose tables mask, always: 803 us, 784 without f.)  SPREAD: a thread has one coordinate of a row,
+// not three, so that no warp comes late to a chunk (rows of heads of 16 447 -> 432 us; forward 397 -> 407, rows of heads of 32 293 -> 295).
+template <int W, int MAPS, bool AUX, bool BIAS, bool SPREAD, int NT>
 struct PmStream {
     static constexpr int CH = PmChunk<W, BIAS, NT>::N;
-    static constexpr int RPP = NT / 4, NR = CH / RPP, NG = BIAS ? (3 * CH + NT - 1) / NT : 1;
-    // with a bias a thread has one word at a time, otherwise the three of a row
+    static constexpr int RPP = NT / 4, NR = CH / RPP;
+    // coordinates that a thread has at a time, and how often; with a bias it has one word of a row at a time, otherwise three
+    static constexpr int GA = SPREAD ? 1 : 3, SLOTS = 3 / GA * CH, NG = BIAS ? (SLOTS + NT - 1) / NT : 1;
     static constexpr int NA = !AUX ? 1 : ((BIAS ? 3 : MAPS) * CH + NT - 1) / NT, AW = BIAS ? 1 : 3;
     static_assert(!(BIAS && MAPS == 2), "coordinates lie where the second map's words do");
     using S = PmStage<W, CH>;
@@ -114,7 +115,7 @@ struct PmStream {
     float second;            // factor of the second map
     int* marks;              // of the stages: 1 + the last chunk there with a reference far from zero
     unsigned char* smem;
-    int e[NR], eg[NG], ea[NA], g[NG], lowest[NG], extent[NG];
+    int e[NR], eg[NG], ea[NA], g[NG][GA];
     float aux[NA][AW];
 
     __device__ __forceinline__ int row_of(int chunk, int j) const
@@ -122,7 +123,7 @@ struct PmStream {
         const int r = chunk * CH + j;
         return r < L ? a.rows[start + r] : INT_MIN;
     }
-    // this thread's i-th coordinate of a chunk: of row k % CH along axis k / CH
+    // this thread's i-th coordinates of a chunk: of row k % CH, from axis k / CH on
     static __device__ __forceinline__ int grid_slot(int i) { return threadIdx.x + i * NT; }
     // (of rows beyond the last the last one's: places in the table stay within it)
     __device__ __forceinline__ void fetch_rows(int chunk)
@@ -130,15 +131,17 @@ struct PmStream {
         if (BIAS)
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-                if (grid_slot(i) < 3 * CH) eg[i] = a.rows[start + min(chunk * CH + grid_slot(i) % CH, L - 1)];
+                if (grid_slot(i) < SLOTS) eg[i] = a.rows[start + min(chunk * CH + grid_slot(i) % CH, L - 1)];
     }
     __device__ __forceinline__ void fetch_grid()
     {
         if (BIAS)
 #pragma unroll
             for (int i = 0; i < NG; ++i)
-                if (grid_slot(i) < 3 * CH)
-                    g[i] = a.grid[3 * (int64_t)(eg[i] >= 0 ? eg[i] : -(eg[i] + 1)) + grid_slot(i) / CH];
+                if (grid_slot(i) < SLOTS)
+#pragma unroll
+                    for (int c = 0; c < GA; ++c)
+                        g[i][c] = a.grid[3 * (int64_t)(eg[i] >= 0 ? eg[i] : -(eg[i] + 1)) + grid_slot(i) / CH + c];
     }
     // its i-th word, or three (with a bias other threads than the first have two of these)
     static __device__ __forceinline__ int aux_slot(int i) { return (BIAS ? (threadIdx.x + NT - CH) % NT : threadIdx.x) + i * NT; }
@@ -211,20 +214,16 @@ struct PmStream {
             if (BIAS)
 #pragma unroll
                 for (int i = 0; i < NG; ++i)
-                    if (grid_slot(i) < 3 * CH)
-                        ((int*)(st + S::GRID))[grid_slot(i)] = pa_other(pa_held(g[i], lowest[i], extent[i]), step);
+                    if (grid_slot(i) < SLOTS)
+#pragma unroll
+                        for (int c = 0; c < GA; ++c)
+                            ((int*)(st + S::GRID))[c * CH + grid_slot(i)] =
+                                pa_other(pm_box(a, seq, g[i][c], grid_slot(i) / CH + c), step);
         }
         cp_async_commit();
     }
     __device__ __forceinline__ void begin()
     {
-        if (BIAS)
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int axis = min(grid_slot(i) / CH, 2);
-                extent[i] = a.extent[6 * seq + axis];
-                lowest[i] = a.extent[6 * seq + 3 + axis];
-            }
         fetch_rows(0);
         fetch(0);
         issue(0);
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
-    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
+    PmStream<W, MAPS, false, BIAS, false, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
                                          table.copies_log2 + 2, 0.f, nullptr, smem};
     in.begin();
     PmBias bias;
@@ -689,7 +688,7 @@ __global__ void __launch_bounds__(NT, (W == 64 ? 256 : 512) / NT) patch_mma_rows
     const __nv_bfloat16* base = (const __nv_bfloat16*)a.qkv + w.h * W;
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::TABLE, false);
-    PmStream<W, MAPS, false, BIAS, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
+    PmStream<W, MAPS, false, BIAS, W == 16, NT> in = {a, base + a.C, base + 2 * a.C, stride, stride, w.seq, w.start, L, w.h, false,
                                          table.copies_log2 + 2, 0.f, nullptr, smem};
     in.begin();
     PmBias bias;
@@ -864,7 +863,7 @@ __global__ void __launch_bounds__(NT, (W == 64 || (W == 32 && RT == 2 && BIAS) ?
     PatchTable table = {};
     if (BIAS) table = pa_table(a, w.seq, PmTableBytes<NT>::BINS, true);
     const float minus_lam = MAPS == 2 ? -pa_param(a.lam, w.h, a.lam_bf16) : 0.f;
-    PmStream<W, MAPS, true, BIAS, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.seq, w.start, L, w.h, true,
+    PmStream<W, MAPS, true, BIAS, false, NT> in = {a, base, (const __nv_bfloat16*)a.dout + w.h * W, stride, a.C, w.seq, w.start, L, w.h, true,
                                         table.copies_log2 + 2, minus_lam, marks, smem};
     in.begin();
     float* tab = (float*)(smem + PM_STAGES * S::BYTES);

@@ -205,7 +205,7 @@ int ptv3_attention_rpe_fwd(const void* qkv, const int64_t* order, const int64_t*
  * the same time need one each.
  *   qkv, dqkv   n x 3*channels; out, dout n x channels; 16-byte aligned, dtype PTV3_DTYPE_*
  *   order, pad, unpad, cu_seqlens   as for ptv3_attention_fwd; n_pad <= 2 n, n_pad < 2^30; read by _fwd (cu_seqlens by _bwd too)
- *   rows        2 * n_pad + (n_pad - n) + 1 + 6 * n_seq int32: what the kernels need of the plan, written by _fwd, read by _bwd.
+ *   rows        3 * n_pad + 1 + 6 * n_seq int32: what the kernels need of the plan, written by _fwd, read by _bwd.
  *               Where coordinates, buckets or cu_seqlens have changed in between, the gradients are undefined, and accesses
  *               stay within the tensors all the same
  *   grid_coord  n x 3 int32 within 2^22 of zero; buckets 2 pos_bnd + 1 int32 in [0, num_buckets)

@@ -18,7 +18,7 @@ struct PatchPlan {
     const int64_t *order, *pad, *unpad;
     const int32_t *cu, *grid, *buckets;
     int n, n_pad, n_seq, max_seqlen, n_entries, num, n_extents;
-    int32_t *rows, *slot, *extent;      // slot: n_pad, then a point for each of n_pad - n, then the counter; or NULL
+    int32_t *rows, *slot, *extent, *owner;      // slot: n_pad, then a point for each of n_pad - n, then the counter; or NULL
     uint32_t* status;
 };
 
@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(256) patch_rows_kernel(const PatchPlan p)
                 }
             }
             p.rows[i] = !good ? -1 : own == i ? (int32_t)e : -1 - (int32_t)e;
+            if (good && own == i) p.owner[e] = i;
         }
         if (i < p.n) {
             // every point has one row that answers for it
@@ -327,7 +328,10 @@ static PatchArgs device_args(const ptv3_patch_attention_args* p)
     a.num = p->num_buckets;
     a.bnd = p->pos_bnd;
     a.table_bf16 = p->table_dtype == PTV3_DTYPE_BF16;
-    a.extent = p->grid_coord ? p->rows + 2 * p->n_pad + (p->n_pad - p->n) + 1 : nullptr;
+    int32_t* const extent = p->rows + 2 * p->n_pad + (p->n_pad - p->n) + 1;
+    a.extent = p->grid_coord ? extent : nullptr;
+    a.owner = extent + 6 * (int64_t)p->n_seq;
+    a.status = p->status;
     a.second = p->second;
     a.lam = p->lam;
     a.lam_bf16 = p->lam_dtype == PTV3_DTYPE_BF16;
@@ -346,7 +350,8 @@ static int launch_rows(const ptv3_patch_attention_args* a, cudaStream_t stream)
     const int borrowed = (int)(n_pad - n);
     PatchPlan p = {a->order, a->pad, a->unpad, a->cu_seqlens, a->grid_coord, a->buckets, (int)n, (int)n_pad, a->n_seq,
                    a->max_seqlen, a->buckets ? 2 * a->pos_bnd + 1 : 0, a->num_buckets, a->grid_coord ? a->n_seq : 0, a->rows,
-                   a->lse && borrowed ? a->rows + n_pad : nullptr, a->rows + 2 * n_pad + borrowed + 1, a->status};
+                   a->lse && borrowed ? a->rows + n_pad : nullptr, a->rows + 2 * n_pad + borrowed + 1,
+                   a->rows + 2 * n_pad + borrowed + 1 + 6 * (int64_t)a->n_seq, a->status};
     if (p.slot) {
         const cudaError_t e = cudaMemsetAsync(p.slot, 0xff, (size_t)(n_pad + borrowed + 1) * 4, stream);
         PTV3_REQUIRE(e == cudaSuccess, PTV3_ERR_CUDA, "ptv3_patch_attention_fwd: %s", cudaGetErrorString(e));

@@ -54,6 +54,8 @@ struct PatchArgs {
     const int32_t* buckets;     // 2 bnd + 1, or NULL: every offset its own
     int num, bnd, table_bf16;
     const int32_t* extent;      // n_seq x 6: largest offset within a sequence along each axis, and its lowest coordinates
+    const int32_t* owner;       // of every point: a row that answers for it (one of them, where an order holds it twice)
+    uint32_t* status;           // or NULL
     const void* lam;            // H
     int lam_bf16;
     float* lse;                 // twice (H maps) x n_pad: the softmax's reference value in log2, then one over its sum (not the
@@ -75,6 +77,16 @@ __device__ __forceinline__ int pa_sequence(const PatchArgs& a, int seq, int& sta
     const int end = a.cu[seq + 1];
     const bool ok = start >= 0 && end <= a.n_pad && end - start <= a.max_seqlen && end > start;
     return ok ? end - start : 0;
+}
+
+// Reports a point that more than one of the rows [first, end) answers for, and another therefore none: all but one of its rows find that
+// out.  (A call, so that the kernels' registers stay as they are.)
+static __device__ __noinline__ void pa_check_owners(const int32_t* rows, const int32_t* owner, uint32_t* status, int first, int end)
+{
+    for (int i = first + threadIdx.x; i < end; i += blockDim.x) {
+        const int e = rows[i];
+        if (e >= 0 && owner[e] != i) atomicOr(status, PTV3_STATUS_BAD_INDEX);
+    }
 }
 
 // a coordinate of a bias (patch_rows_kernel reports one out of range; places in the table stay within it all the same)

@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(PF_THREADS) patch_fma_fwd_kernel(const PatchAr
     const int L = pa_sequence(a, seq, start);
     const int q0 = tile * S::ROWS, qi = q0 + threadIdx.x / SPLIT;
     if (q0 >= L) return;
+    if (h == 0 && a.status) pa_check_owners(a.rows, a.owner, a.status, start + q0, start + min(q0 + S::ROWS, L));
     const bool busy = q0 + threadIdx.x / 32 * 32 / SPLIT < L;          // (warps with no row at all only gather)
     const int64_t stride = 3 * (int64_t)a.C;
     const float* base = (const float*)a.qkv + h * W;

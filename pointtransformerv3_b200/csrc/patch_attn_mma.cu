@@ -470,6 +470,7 @@ __global__ void __launch_bounds__(NT, (W == 64 && (MAPS == 2 || RT == 2) ? 256 :
     const PmPlace w = pm_place(a);
     const int q0 = w.tile * (NT / 2) * RT, L = w.L;
     if (q0 >= L) return;
+    if (w.h == 0 && a.status) pa_check_owners(a.rows, a.owner, a.status, w.start + q0, w.start + min(q0 + NT / 2 * RT, L));
     const int t = threadIdx.x & 3;
     PmOwn<RT> own;
     own.load(a, w, q0);

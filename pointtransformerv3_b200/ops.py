@@ -270,7 +270,7 @@ def patch_attention_fwd(qkv, plan, heads, max_seqlen, scale, maps=1, param=None,
     _lib.require_cuda(qkv, *plan, param, status)
     n, c3 = qkv.shape
     n_pad, dev = plan[1].shape[0], qkv.device
-    rows = plan[3].new_empty(3 * n_pad - n + 1 + 6 * (plan[3].shape[0] - 1))       # (int32 too; new_empty is the cheaper call)
+    rows = plan[3].new_empty(3 * n_pad + 1 + 6 * (plan[3].shape[0] - 1))       # (int32 too; new_empty is the cheaper call)
     out = qkv.new_empty((n, c3 // 3))
     lse = torch.empty((2 * heads * maps, n_pad), dtype=torch.float32, device=dev) if keep else None
     second = torch.empty_like(out) if keep and maps == 2 else None

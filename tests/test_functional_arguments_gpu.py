@@ -4,8 +4,8 @@ import torch
 
 import functional_norms as N
 import functional_reference as R
+from pointtransformerv3_b200 import _lib, ops
 from pointtransformerv3_b200 import functional as F
-from pointtransformerv3_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,22 @@ def test_short_sequences_beside_a_long_one(counts, patch, dtype):
         ref = R.attention(qkv, order, pad, unpad, cu, H, width ** -0.5, 1, table.detach(), p["grid"], 130, buckets, dout)
         for name, t in zip(("out", "dqkv", "dparam"), got):
             N.check(t.detach(), ref, name, qkv, dout, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_an_order_that_holds_a_point_twice_is_reported(dtype):
+    """Another point has no row then, and nothing would write its result: in heads alone and together, in the first patch, in the last
+    one and across two, with a graph and without one."""
+    p = patches([130, 90, 1], 64)
+    for width, H in ((16, 1), (32, 2), (64, 1)):
+        qkv = normal(p["n"], 3 * width * H, seed=1, dtype=dtype)
+        lam, rest = torch.ones(H, device="cuda"), p["geometry"][1:]
+        for at, instead in ((3, 4), (0, 129), (200, 70), (219, 131)):
+            order = p["geometry"][0].clone()
+            order[at] = order[instead]
+            for x in (qkv, qkv.clone().requires_grad_()):
+                with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):
+                    F.attention_diff(x, lam, order, *rest, H, 64)
+                with pytest.raises(_lib.Ptv3Error, match="index or size out of range"):
+                    F.attention_bias(x, order, *rest, H, 64, grid_coord=p["grid"], table=torch.ones(9, H, device="cuda"))
+        F.attention_diff(qkv, lam, *p["geometry"], H, 64)

@@ -20,6 +20,7 @@ from torch.autograd import forward_ad
 
 from . import _lib, ops
 
+HEAD_WIDTHS = (16, 32, 64)    # of the attention operators
 BUCKETS_MAX_BOUND = 512       # offsets beyond that many cells share the outermost bucket in any case
 
 
@@ -173,7 +174,7 @@ class _PatchAttention(torch.autograd.Function):
 def _attend(qkv, param, order_row, pad, unpad, cu_seqlens, bias, heads, max_seqlen, scale, maps, status):
     _no_tangents(qkv, param)
     n, D = qkv.shape[0], qkv.shape[1] // 3 // heads
-    if D not in (16, 32, 64):
+    if D not in HEAD_WIDTHS:
         raise ValueError("heads of %d values (supported: 16, 32, 64)" % D)
     if order_row.shape != (n,) or unpad.shape != (n,) or pad.dim() != 1 or not n <= pad.shape[0] <= 2 * n:
         raise ValueError("order_row and unpad must be (%d,), pad %d to %d rows" % (n, n, 2 * n))

@@ -216,11 +216,17 @@ class SerializedAttention(PointModule):
         """Whether this is the attention that the one-call block and backbone know."""
         return not (self.enable_rpe or self.enable_rope or self.q_norm is not None or self.lam is not None)
 
+    @property
+    def _options(self):
+        """Whether there are options beyond the reference's."""
+        return (self.q_norm is not None or self.enable_rope or self.lam is not None
+                or (self.enable_rpe and self.rpe.buckets is not None))
+
     def _learns(self, feat):
-        """Whether a call has gradients: in training mode, and with options beyond the reference's wherever autograd asks."""
-        options = (self.q_norm is not None or self.enable_rope or self.lam is not None
-                   or (self.enable_rpe and self.rpe.buckets is not None))
-        return self.training or (options and torch.is_grad_enabled()
+        """Whether a call has gradients: in training mode, and with options beyond the reference's wherever autograd asks and
+        the kernels have them."""
+        return self.training or (self._options and torch.is_grad_enabled()
+                                 and self.channels // self.num_heads in functional.HEAD_WIDTHS
                                  and (feat.requires_grad or any(p.requires_grad for p in self.parameters())))
 
     @torch.no_grad()
@@ -279,7 +285,9 @@ class SerializedAttention(PointModule):
             self._report(point)
             return out
         status = point.device_status()
-        return self.proj_drop(_linear_op(self.core(point, _linear_op(feat, self.qkv, status)), self.proj, status))
+        # (with options a call without gradients has none at all, not those of its last layer)
+        with torch.set_grad_enabled(torch.is_grad_enabled() and not self._options):
+            return self.proj_drop(_linear_op(self.core(point, _linear_op(feat, self.qkv, status)), self.proj, status))
 
     def _report(self, point):
         """Raises for what the kernels found wrong with a plan or coordinates: once for a Point, an order and a patch size, as that

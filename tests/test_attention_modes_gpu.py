@@ -119,3 +119,20 @@ def test_a_captured_step_does_not_wait():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, step(P.Point(dict(pt)))))
     fresh.check_status(force=True)
+
+
+def test_heads_without_gradients_evaluate_without_any():
+    """Heads of 8 have norms and rotation and no gradients: refused in training, and in evaluation no part of the module has one."""
+    att = module("norm_rope", torch.float32, flash=True, C=32, H=4)
+    pt, feat, _ = scene([200, 90], 81, 32, torch.float32)
+    outs = []
+    for grad in (True, False):
+        att.eval()
+        pt.feat = feat.clone().requires_grad_()
+        with torch.set_grad_enabled(grad):
+            outs.append(att(pt).feat)
+        assert not outs[-1].requires_grad
+    assert torch.equal(*outs)
+    pt.feat = feat
+    with pytest.raises(ValueError, match="heads of 8"):
+        att.train()(pt)

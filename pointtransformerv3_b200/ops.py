@@ -236,7 +236,8 @@ def qk_norm_rope_bwd(qkv, dout, heads, grid, q_weight, k_weight, eps, base):
         dq, dk = torch.empty_like(q_weight), torch.empty_like(k_weight)
         nbytes = lib.ptv3_qk_norm_rope_workspace_bytes(n, c3 // 3, heads)
         ws = _lib.workspace(nbytes, dout.device)
-    with timed("qk_norm_rope_bwd", (2.0 + (q_weight is not None)) * dout.numel() * dout.element_size()):
+    # (the gradient in and one out, and with weights the queries and keys)
+    with timed("qk_norm_rope_bwd", (2.0 + 2.0 / 3.0 * (q_weight is not None)) * dout.numel() * dout.element_size()):
         _lib.check(lib.ptv3_qk_norm_rope_bwd(
             _lib.ptr(qkv), _lib.ptr(q_weight), _lib.ptr(k_weight), _lib.dtype_id(dout if q_weight is None else q_weight),
             _lib.ptr(grid), _lib.ptr(dout), _lib.ptr(dqkv), _lib.ptr(dq), _lib.ptr(dk), n, c3 // 3, heads, eps, base,

@@ -1036,11 +1036,11 @@ static int launch(K kern, const PatchArgs& a, size_t smem, cudaStream_t stream)
 
 // What a block is.  Eight warps of a row tile each; two tiles to a warp, so that what it reads of the other side serves twice the
 // rows, where registers allow it, patches fill such blocks and launches are long.  us with one and with two, heads of 16:
-// forward with a bias, 120 000 x 64, 489 and 397; 100 000 x 64, rows with a bias 464 and 452, columns 857 and 784, columns of
-// two maps 347 and 320; not so forward and rows without a bias (312 and 326, 341 and 465).  Heads of 32, 100 000 x 64: columns with a
-// bias, a CTA to an SM, 671 and 523 (10 000 x 64: 110 and 84), of two maps in blocks of four warps, three to an SM, 266 and 233
-// (20 000 x 64: 78 and 68; 10 000 x 64 42 and 41); forward and rows are slower or as fast (with a bias 238 and 281, 289 and 300).  Heads
-// of 64, a CTA to an SM: forward with a bias 231 and 174 (20 000 x 64: 74 and 58); columns with a bias 410 and 383, of two maps 261 and
+// forward with a bias, 120 000 x 64, 489 and 392; 100 000 x 64, rows with a bias 462 and 432, columns 886 and 804, columns of
+// two maps 356 and 319; not so forward and rows without a bias (312 and 326, 341 and 465).  Heads of 32, 100 000 x 64: columns with a
+// bias, a CTA to an SM, 667 and 543 (10 000 x 64: 108 and 87), of two maps in blocks of four warps, three to an SM, 252 and 233
+// (20 000 x 64: 75 and 67; 10 000 x 64 42 and 42); forward and rows are slower or as fast (with a bias 238 and 281, 289 and 300).  Heads
+// of 64, a CTA to an SM: forward with a bias 238 and 178 (20 000 x 64: 76 and 58); columns with a bias 410 and 383, of two maps 261 and
 // 228, but 202 and 247, 122 and 149 at 40 000 x 64, whose 160 blocks are two rounds: one tile.  Four warps where patches are short
 // (60 000 x 64 in patches of 48, two maps, the three passes: 62, 70 and 74 us with eight, 34, 38 and 36) or blocks without a bias
 // few (1 560 x 256 forward 33 and 27.5; with a bias, 6 760 x 128, 68 and 72).

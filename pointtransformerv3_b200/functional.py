@@ -3,8 +3,8 @@
 ``qk_norm_rope`` prepares the rows of a QKV projection (norms of queries and keys for each head, rotation by grid
 coordinates), ``attention_bias`` and ``attention_diff`` are attention cores within the patches of a serialized order, with a
 learned relative position bias by buckets or as the difference of two softmax maps.  They take the index tensors that
-``ops.attention`` takes; ``SerializedAttention`` calls them for its options ``qk_norm``, ``enable_rope``, ``enable_rpe`` (in training) and
-``differential``.
+``ops.attention`` takes; ``SerializedAttention`` calls them for its options ``qk_norm``, ``enable_rope``, ``enable_rpe`` (in training, and
+where its bias is by buckets or reaches beyond 64 cells) and ``differential``.
 
 All of them run on the current stream of the tensors' device, keep nothing between calls, and can be captured into a graph (with a
 ``status`` word of the caller's: one that they make themselves is read at once, which waits for the device).  A backward pass

@@ -648,6 +648,53 @@ int ptv3_seg_head_fwd(const void* feat, const void* weight, const void* bias, vo
                       int64_t n, int channels, int classes, int dtype, void* stream);
 
 /*
+ * What rows of logits answer (behind the segmentation head; no counterpart in the reference, whose file ends with the
+ * backbone, model.py:966-982).  With p = softmax(logits / temperature) of a row:
+ *   log_prob       n: log p of the row's label; 0 where the label is `ignore`, NaN (and PTV3_STATUS_BAD_INDEX) where it is no class
+ *   entropy        n
+ *   top_log_prob, top_class   n x top: the `top` largest logits, the lowest class first among equals, NaN above all;
+ *                  beyond the classes there are: minus infinity and -1
+ * Minus infinity masks a class; a row of nothing else has log p = minus infinity, entropy 0 and a gradient of 0.  A NaN or a plus
+ * infinity makes its row NaN.
+ *   logits         n x classes, PTV3_DTYPE_* dtype, rows ld elements apart (ld >= classes), any alignment of that type
+ *   labels         n int32 or int64 (label_bytes 4 or 8), or NULL with log_prob NULL
+ *   stats          n x 2 fp32 (8-byte aligned) that _bwd takes, or NULL
+ *   dlog_prob, dentropy   gradients of the two outputs, their steps apart (0: one value for all rows), or NULL
+ *   dtop           n x top gradients of top_log_prob, or NULL
+ *   dlogits        n x classes (out), in the logits' type
+ *   status         may be NULL without log_prob
+ * classes up to 262 144, top up to 64, temperature in [1e-6, 1e6], n below 2^31.
+ */
+int ptv3_class_scores_fwd(const void* logits, int64_t ld, const void* labels, int label_bytes, int64_t ignore,
+                          float* log_prob, float* entropy, float* top_log_prob, int32_t* top_class, float* stats, int64_t n,
+                          int classes, int top, float temperature, int dtype, uint32_t* status, void* stream);
+int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void* labels, int label_bytes, int64_t ignore,
+                          const float* entropy, const int32_t* top_class, const float* stats, const float* dlog_prob,
+                          int64_t dlog_prob_step, const float* dentropy, int64_t dentropy_step, const float* dtop,
+                          void* dlogits, int64_t n, int classes, int top, float temperature, int dtype, void* stream);
+
+/*
+ * A student's logits against the best k classes that a teacher kept of each row.  With p = softmax(logits / temperature):
+ *   rest = 0: t = softmax(teacher / temperature) over the row's list;  loss = sum t_i (log t_i - log p_{c_i})
+ *   rest = 1: t = exp(teacher), and what the list leaves, t_r = max(0, 1 - sum t), against the probability p_r of the classes
+ *             outside the list:  loss = sum t_i (log t_i - log p_{c_i}) + t_r (log t_r - log p_r)
+ * A class of -1 is absent; a row without any has loss and gradient 0.  A class outside -1 .. classes - 1 makes its row's loss
+ * NaN and sets PTV3_STATUS_BAD_INDEX.  A class that a list has twice counts as two entries.  Where the list leaves no class that the
+ * student allows (minus infinity masks one), there is no t_r.  A student that allows no class has an infinite loss and a gradient of 0.
+ *   logits     as above; dlogits (out) n x classes in their type
+ *   teacher    n x k, PTV3_DTYPE_* teacher_dtype;  list: n x k int32 or int64 (list_bytes 4 or 8)
+ *   loss       n (out);  dloss: its gradient, dloss_step apart (0: one value for all rows)
+ *   stats      n x 4 fp32 (16-byte aligned) that _bwd takes, or NULL
+ * classes up to 262 144, k in 1 .. 64, temperature in [1e-6, 1e6], n below 2^31.
+ */
+int ptv3_distill_topk_fwd(const void* logits, int64_t ld, const void* teacher, int teacher_dtype, const void* list,
+                          int list_bytes, int k, float* loss, float* stats, int64_t n, int classes, float temperature, int rest,
+                          int dtype, uint32_t* status, void* stream);
+int ptv3_distill_topk_bwd(const void* logits, int64_t ld, const void* teacher, int teacher_dtype, const void* list,
+                          int list_bytes, int k, const float* stats, const float* dloss, int64_t dloss_step, void* dlogits,
+                          int64_t n, int classes, float temperature, int rest, int dtype, void* stream);
+
+/*
  * Stage transitions in one call each (bf16): the Linear projection(s) on the tensor-core
  * Linear kernels (ptv3_linear_fwd or ptv3_gemm_fwd, whichever takes the shape;
  * ptv3_pool_stage_supported tells whether one does), then the kernel of ptv3_pool_fwd /

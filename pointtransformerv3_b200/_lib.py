@@ -141,6 +141,14 @@ SIGNATURES = {
                               c_sz, c_ptr]),
     "ptv3_voxelize_rows": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_f32, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr]),
     "ptv3_seg_head_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int, c_int, c_int, c_ptr]),
+    "ptv3_class_scores_fwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int,
+                                      c_int, c_f32, c_int, c_ptr, c_ptr]),
+    "ptv3_class_scores_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
+                                      c_ptr, c_ptr, c_i64, c_int, c_int, c_f32, c_int, c_ptr]),
+    "ptv3_distill_topk_fwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_ptr, c_int, c_int, c_ptr, c_ptr, c_i64, c_int, c_f32,
+                                      c_int, c_int, c_ptr, c_ptr]),
+    "ptv3_distill_topk_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_ptr, c_int, c_int, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
+                                      c_int, c_f32, c_int, c_int, c_ptr]),
     "ptv3_pool_stage_supported": (c_int, [c_int, c_int, c_int]),
     "ptv3_pool_stage_workspace_bytes": (c_sz, [c_i64, c_int]),
     "ptv3_pool_stage_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_ptr,

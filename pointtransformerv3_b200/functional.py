@@ -1,4 +1,4 @@
-"""Operators of serialized attention that can be trained: functions of tensors with gradients.
+"""Operators that can be trained: functions of tensors with gradients.
 
 ``qk_norm_rope`` prepares the rows of a QKV projection (norms of queries and keys for each head, rotation by grid
 coordinates), ``attention_bias`` and ``attention_diff`` are attention cores within the patches of a serialized order, with a
@@ -6,12 +6,16 @@ learned relative position bias by buckets or as the difference of two softmax ma
 ``ops.attention`` takes; ``SerializedAttention`` calls them for its options ``qk_norm``, ``enable_rope``, ``enable_rpe`` (in training, and
 where its bias is by buckets or reaches beyond 64 cells) and ``differential``.
 
+``class_log_probs`` and ``distill_topk`` stand behind a network's logits: the terms of a cross entropy, uncertainty and the best alternatives of
+every point, and the loss of a student against what a teacher's scoring kept of these.  ``SegHead.log_probs`` gives the first straight from features.
+
 All of them run on the current stream of the tensors' device, keep nothing between calls, and can be captured into a graph (with a
 ``status`` word of the caller's: one that they make themselves is read at once, which waits for the device).  A backward pass
 that is captured wants leaves which no eager graph holds at that time (``x.detach().requires_grad_()``): torch ties a leaf's
 gradient to the stream of the graph that met it first.  Gradients are of first order and backward, and the same bits on every run;
 tensors with a tangent of forward-mode differentiation are refused.
 """
+import collections
 import contextlib
 import math
 
@@ -257,3 +261,164 @@ def attention_diff(qkv, lam, order_row, pad, unpad, cu_seqlens, heads, max_seqle
         raise ValueError("lam must be (%d,), got %s" % (heads, tuple(lam.shape)))
     _lib.dtype_id(lam)
     return _attend(qkv, lam, order_row, pad, unpad, cu_seqlens, None, heads, max_seqlen, scale, 2, status)
+
+
+# --------------------------------------------------------------------------- behind the logits
+CLASSES_MAX = 2 ** 18       # of a row of logits
+LIST_MAX = 64               # alternatives, entries of a teacher's list
+TEMPERATURES = (1e-6, 1e6)
+
+ClassScores = collections.namedtuple("ClassScores", "log_prob entropy top_log_probs top_classes")
+
+
+def _rows(logits):
+    """Rows of neighbouring values, any distance apart."""
+    n, K = logits.shape
+    if (K == 1 or logits.stride(1) == 1) and (n <= 1 or logits.stride(0) >= K):
+        return logits
+    return logits.contiguous()
+
+
+def _check_logits(logits, temperature):
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= CLASSES_MAX:
+        raise ValueError("logits must be (N, 1 to %d classes), got %s" % (CLASSES_MAX, tuple(logits.shape)))
+    _lib.dtype_id(logits)
+    if not TEMPERATURES[0] <= temperature <= TEMPERATURES[1]:
+        raise ValueError("temperature %r, not within %g to %g" % (temperature, *TEMPERATURES))
+
+
+def _check_indices(t, shape, what):
+    if tuple(t.shape) != shape or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s must be int32 or int64 %s, got %s %s" % (what, shape, t.dtype, tuple(t.shape)))
+    return t.contiguous()
+
+
+def _check_labels(labels, n, top, ignore_index):
+    if not 0 <= top <= LIST_MAX:
+        raise ValueError("%d alternatives (0 to %d)" % (top, LIST_MAX))
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index %d" % ignore_index)
+    return labels if labels is None else _check_indices(labels, (n,), "labels")
+
+
+def _status_word(status, device):
+    """The status word of a call, and whether it is the call's own, to be read at once."""
+    if status is not None:
+        if status.dtype != torch.int32 or status.numel() < 1:
+            raise ValueError("status must be an int32 word")
+        return status, False
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a captured call needs a status word of the caller's: one of its own is read at once")
+    return ops.new_status(device), True
+
+
+class _ClassScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top, temperature, ignore_index, status):
+        out = ops.class_scores_fwd(logits, labels, top, temperature, ignore_index, status, True)
+        log_prob, entropy, values, classes, stats = out
+        ctx.save_for_backward(logits, _kept(labels), entropy, classes, stats)
+        ctx.args = temperature, ignore_index
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(classes)
+        return log_prob, entropy, values, classes
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlog_prob, dentropy, dtop, _):
+        logits, labels, entropy, classes, stats = ctx.saved_tensors
+        if dlog_prob is None and dentropy is None and dtop is None:
+            return (None,) * 6
+        with _on(logits.device):
+            dlogits = ops.class_scores_bwd(logits, labels, entropy, classes, stats, *ctx.args, dlog_prob, dentropy,
+                                           None if dtop is None else dtop.contiguous())
+        return dlogits, None, None, None, None, None
+
+
+def class_log_probs(logits, labels=None, top=0, temperature=1.0, ignore_index=-1, status=None):
+    """Log probability of a class, entropy and the best alternatives of every row of logits: ``ClassScores``.
+
+    logits (N, K), bf16 or fp32, K up to 262 144; rows may lie apart (a slice of wider ones is not copied).  p is the softmax of logits /
+    temperature.  All in fp32:
+      log_prob (N,)             log p of ``labels`` (N,), int32 or int64; 0 where the label is ``ignore_index``.  None without labels.
+      entropy (N,)              -sum p log p
+      top_log_probs (N, top)    log p of the ``top`` (up to 64) largest logits, and their classes ``top_classes`` (N, top) int32, the lowest
+                                class first among equals; minus infinity and -1 beyond the classes there are.  None with top = 0.
+    ``-log_prob`` are the terms of a cross entropy; their mean over the rows with a label is the usual loss.
+    Minus infinity masks a class.  A row of masked classes alone has log probabilities of minus infinity, entropy 0 and no gradient; a NaN
+    or a plus infinity makes its row NaN.
+
+    status: a device status word of the caller's (``ops.new_status``), in which labels out of range are reported (their log_prob is
+    NaN, and nothing of them goes into the gradient); the caller checks it when the host next waits.  Without one a call with labels checks
+    for itself and waits for the device.
+    Gradients: logits, from log_prob, entropy and top_log_probs."""
+    _same_device(logits, labels, status)
+    _no_tangents(logits)
+    _check_logits(logits, temperature)
+    labels = _check_labels(labels, logits.shape[0], top, ignore_index)
+    args = int(top), float(temperature), int(ignore_index)
+    with _on(logits.device):
+        own = False
+        if labels is not None:
+            status, own = _status_word(status, logits.device)
+        logits = _rows(logits)
+        if _wants_grad(logits):
+            out = _ClassScores.apply(logits, labels, *args, status)
+        else:
+            out = ops.class_scores_fwd(logits, labels, *args, status)[:4]
+        if own:
+            _lib.raise_on_status(status, "ptv3_class_scores_fwd")
+    return ClassScores(*out)
+
+
+class _DistillTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, classes, temperature, rest, status):
+        loss, stats = ops.distill_topk_fwd(logits, teacher, classes, temperature, rest, status, True)
+        ctx.save_for_backward(logits, _kept(teacher), _kept(classes), stats)
+        ctx.args = temperature, rest
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, teacher, classes, stats = ctx.saved_tensors
+        with _on(logits.device):
+            dlogits = ops.distill_topk_bwd(logits, teacher, classes, stats, *ctx.args, dloss)
+        return dlogits, None, None, None, None, None
+
+
+def distill_topk(logits, teacher, classes, temperature=1.0, rest=False, status=None):
+    """Loss of a student's logits against the best classes that a teacher kept of every row: (N,) fp32, without a factor of temperature ** 2.
+
+    logits (N, K), as for ``class_log_probs``; p is the softmax of logits / temperature.  teacher (N, k), bf16 or fp32, and classes (N, k), int32 or
+    int64, k up to 64: the teacher's values and their classes, in any order, -1 for an entry that is not there (a row without any has loss 0).
+      rest=False   teacher are logits or log probabilities; t = softmax(teacher / temperature) over the row's entries, and the loss is
+                   sum t_i (log t_i - log p_i).
+      rest=True    teacher are log probabilities at this temperature, as ``class_log_probs(..., top=k, temperature=temperature)`` gives them;
+                   t = exp(teacher), and what the list leaves of the teacher's, t_r = 1 - sum t, is one outcome more, against the sum of the
+                   student's probabilities outside the list.  Without a class outside that the student allows there is no such outcome.
+    A class that a list has twice counts as two entries.  A class that the student masks (minus infinity) and the teacher does not makes the
+    loss infinite; where the student masks every class, the gradient is 0.
+
+    status: as for ``class_log_probs``; it reports classes out of range (the row's loss is NaN, its gradient leaves the entry out).
+    Gradients: logits.  The teacher's values are constants, and refused where they ask for a gradient."""
+    _same_device(logits, teacher, classes, status)
+    _no_tangents(logits, teacher)
+    _check_logits(logits, temperature)
+    if classes.dim() != 2 or not 1 <= classes.shape[1] <= LIST_MAX:
+        raise ValueError("classes must be (N, 1 to %d), got %s" % (LIST_MAX, tuple(classes.shape)))
+    classes = _check_indices(classes, (logits.shape[0], classes.shape[1]), "classes")
+    if teacher.shape != classes.shape:
+        raise ValueError("teacher %s, classes %s" % (tuple(teacher.shape), tuple(classes.shape)))
+    _lib.dtype_id(teacher)
+    if _wants_grad(teacher):
+        raise ValueError("no gradient goes to the teacher: detach its values")
+    with _on(logits.device):
+        status, own = _status_word(status, logits.device)
+        args = _rows(logits), teacher.contiguous(), classes, float(temperature), int(bool(rest)), status
+        loss = _DistillTopk.apply(*args) if _wants_grad(logits) else ops.distill_topk_fwd(*args)[0]
+        if own:
+            _lib.raise_on_status(status, "ptv3_distill_topk_fwd")
+    return loss

@@ -981,6 +981,64 @@ def seg_head(feat, weight, bias=None, want_logits=True, want_labels=True):
     return logits, labels
 
 
+def class_scores_fwd(logits, labels, top, temperature, ignore_index, status, keep=False):
+    """See ptv3_class_scores_fwd; ``functional.class_log_probs`` is the checked form with gradients.  logits (N, K) with rows of
+    neighbouring values -> (log_prob or None, entropy, top_log_probs or None, top_classes or None, stats or None)."""
+    n, K = logits.shape
+    dev, f32 = logits.device, torch.float32
+    log_prob = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
+    entropy = torch.empty(n, dtype=f32, device=dev)
+    values = torch.empty((n, top), dtype=f32, device=dev) if top else None
+    classes = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
+    stats = torch.empty((n, 2), dtype=f32, device=dev) if keep else None
+    with timed("class_scores", n * (K * logits.element_size() + 8.0 * top + 8.0)):
+        _lib.check(_lib.load().ptv3_class_scores_fwd(
+            logits.data_ptr(), logits.stride(0) if n > 1 else K, _lib.ptr(labels), 0 if labels is None else labels.element_size(),
+            ignore_index, _lib.ptr(log_prob), entropy.data_ptr(), _lib.ptr(values), _lib.ptr(classes), _lib.ptr(stats), n, K,
+            top, temperature, _lib.dtype_id(logits), _lib.ptr(status), _lib.stream()), "ptv3_class_scores_fwd")
+    return log_prob, entropy, values, classes, stats
+
+
+def class_scores_bwd(logits, labels, entropy, classes, stats, temperature, ignore_index, dlog_prob, dentropy, dtop):
+    """Gradient of the logits (N, K); gradients of outputs that nothing used are None."""
+    n, K = logits.shape
+    dlogits = torch.empty((n, K), dtype=logits.dtype, device=logits.device)
+    with timed("class_scores_bwd", n * (2.0 * K * logits.element_size() + 16.0)):
+        _lib.check(_lib.load().ptv3_class_scores_bwd(
+            logits.data_ptr(), logits.stride(0) if n > 1 else K, _lib.ptr(labels), 0 if labels is None else labels.element_size(),
+            ignore_index, entropy.data_ptr(), _lib.ptr(classes), stats.data_ptr(), _lib.ptr(dlog_prob),
+            0 if dlog_prob is None else dlog_prob.stride(0), _lib.ptr(dentropy), 0 if dentropy is None else dentropy.stride(0),
+            _lib.ptr(dtop), dlogits.data_ptr(), n, K, 0 if classes is None else classes.shape[1], temperature,
+            _lib.dtype_id(logits), _lib.stream()), "ptv3_class_scores_bwd")
+    return dlogits
+
+
+def distill_topk_fwd(logits, teacher, classes, temperature, rest, status, keep=False):
+    """See ptv3_distill_topk_fwd; ``functional.distill_topk`` is the checked form with gradients.  -> (loss (N,), stats or None)."""
+    n, K = logits.shape
+    loss = torch.empty(n, dtype=torch.float32, device=logits.device)
+    stats = torch.empty((n, 4), dtype=torch.float32, device=logits.device) if keep else None
+    k = classes.shape[1]
+    with timed("distill_topk", n * (K * logits.element_size() + 8.0 * k + 4.0)):
+        _lib.check(_lib.load().ptv3_distill_topk_fwd(
+            logits.data_ptr(), logits.stride(0) if n > 1 else K, teacher.data_ptr(), _lib.dtype_id(teacher), classes.data_ptr(),
+            classes.element_size(), k, loss.data_ptr(), _lib.ptr(stats), n, K, temperature, rest, _lib.dtype_id(logits),
+            status.data_ptr(), _lib.stream()), "ptv3_distill_topk_fwd")
+    return loss, stats
+
+
+def distill_topk_bwd(logits, teacher, classes, stats, temperature, rest, dloss):
+    """Gradient of the logits (N, K)."""
+    n, K = logits.shape
+    dlogits = torch.empty((n, K), dtype=logits.dtype, device=logits.device)
+    with timed("distill_topk_bwd", n * (2.0 * K * logits.element_size() + 8.0 * classes.shape[1] + 20.0)):
+        _lib.check(_lib.load().ptv3_distill_topk_bwd(
+            logits.data_ptr(), logits.stride(0) if n > 1 else K, teacher.data_ptr(), _lib.dtype_id(teacher), classes.data_ptr(),
+            classes.element_size(), classes.shape[1], stats.data_ptr(), dloss.data_ptr(), dloss.stride(0), dlogits.data_ptr(), n,
+            K, temperature, rest, _lib.dtype_id(logits), _lib.stream()), "ptv3_distill_topk_bwd")
+    return dlogits
+
+
 def pool_stage_supported(c_in, c_out, dtype):
     """Whether a projection c_in -> c_out can go through the one-call stage transitions."""
     return dtype in _lib.DTYPE_IDS and bool(

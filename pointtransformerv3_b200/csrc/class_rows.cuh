@@ -11,6 +11,7 @@
 #pragma once
 #include "common.cuh"
 #include "convert.cuh"
+#include "mma_util.cuh"
 #include "vec.cuh"
 
 namespace ptv3 {
@@ -48,11 +49,164 @@ __device__ __forceinline__ float load_value(const void* p, bool bf16, int64_t i)
     return bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : ((const float*)p)[i];
 }
 
+// ---- 8 neighbouring logits of a row ---------------------------------------------------------------------------------
+template <typename T> struct Eight;
+template <> struct Eight<__nv_bfloat16> {
+    static constexpr int WORDS = 4;
+    uint32_t w[4];
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+    __device__ __forceinline__ uint64_t pair(int q) const { return unpack_bf16x2(w[q]); }
+    __device__ __forceinline__ void keep_first(int count)       // the others become minus infinity
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i >= count) w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | 0xff800000u : (w[i >> 1] & 0xffff0000u) | 0xff80u;
+    }
+    __device__ __forceinline__ void drop_first(int count)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | 0xff800000u : (w[i >> 1] & 0xffff0000u) | 0xff80u;
+    }
+    __device__ __forceinline__ float largest() const            // NaN if one is
+    {
+        __nv_bfloat162 a = __hmax2_nan(h(0), h(1)), b = __hmax2_nan(h(2), h(3));
+        a = __hmax2_nan(a, b);
+        return max_nan(__low2float(a), __high2float(a));
+    }
+    __device__ __forceinline__ __nv_bfloat162 h(int q) const { return *reinterpret_cast<const __nv_bfloat162*>(&w[q]); }
+    __device__ __forceinline__ void set(int q, float lo, float hi) { w[q] = pack_bf16(lo, hi); }
+};
+template <> struct Eight<float> {
+    static constexpr int WORDS = 8;
+    uint32_t w[8];
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
+    __device__ __forceinline__ uint64_t pair(int q) const { return pack2u(w[2 * q], w[2 * q + 1]); }
+    __device__ __forceinline__ void keep_first(int count)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i >= count) w[i] = 0xff800000u;
+    }
+    __device__ __forceinline__ void drop_first(int count)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < count) w[i] = 0xff800000u;
+    }
+    __device__ __forceinline__ float largest() const
+    {
+        return max_nan(max_nan(max_nan(at(0), at(1)), max_nan(at(2), at(3))), max_nan(max_nan(at(4), at(5)), max_nan(at(6), at(7))));
+    }
+    __device__ __forceinline__ void set(int q, float lo, float hi)
+    {
+        w[2 * q] = __float_as_uint(lo);
+        w[2 * q + 1] = __float_as_uint(hi);
+    }
+};
+
+// S and U = sum e d of a row, in packed pairs
+struct RowSum {
+    uint64_t s, u;
+    __device__ __forceinline__ void clear() { s = u = 0; }
+    template <typename T>
+    __device__ __forceinline__ void add(const Eight<T>& x, uint64_t minus_origin, uint64_t c)
+    {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float lo, hi, e0, e1;
+            unpack2(add2(x.pair(q), minus_origin), lo, hi);
+            const uint64_t d = pack2(max_nan(lo, -1e38f), max_nan(hi, -1e38f));
+            unpack2(mul2(d, c), e0, e1);
+            const uint64_t e = pack2(fast_exp2(e0), fast_exp2(e1));
+            s = add2(s, e);
+            u = fma2(e, d, u);
+        }
+    }
+};
+
+// ---- the largest of a row, kept sorted in a thread's registers ------------------------------------------------------------
+// Keys say value and class: the larger value first, then the lower class, so that no two are equal and the order in which they
+// come does not matter.  bf16: 16 bits of each (rows of up to 2^16 classes); fp32: 32 and 32.  0: no class.
+template <typename T> struct TopKey;
+template <> struct TopKey<__nv_bfloat16> {
+    using Key = uint32_t;
+    // of eight classes from j on
+    __device__ static __forceinline__ void keys(const Eight<__nv_bfloat16>& x, int j, Key* k)
+    {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            // (adding zero: one zero, one NaN)
+            const __nv_bfloat162 one = __hadd2_rn(x.h(q), __nv_bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)));
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(&one);
+            const uint32_t o = w ^ (((w >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u);
+            const uint32_t at = 0xffffu - (j + 2 * q);
+            k[2 * q] = __byte_perm(at, o, 0x5410);
+            k[2 * q + 1] = __byte_perm(at - 1, o, 0x7610);
+        }
+    }
+    __device__ static __forceinline__ int cls(Key k) { return k ? (int)(0xffffu - (k & 0xffffu)) : -1; }
+    __device__ static __forceinline__ float value(Key k) { return order_value((k & 0xffff0000u) | (k >> 31 ? 0 : 0xffffu)); }
+};
+template <> struct TopKey<float> {
+    using Key = unsigned long long;
+    __device__ static __forceinline__ void keys(const Eight<float>& x, int j, Key* k)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = (unsigned long long)order_key(x.at(i)) << 32 | (0xffffffffu - (j + i));
+    }
+    __device__ static __forceinline__ int cls(Key k) { return k ? (int)(0xffffffffu - (uint32_t)k) : -1; }
+    __device__ static __forceinline__ float value(Key k) { return order_value((uint32_t)(k >> 32)); }
+};
+
+template <typename K>
+__device__ __forceinline__ void larger_first(K& a, K& b)
+{
+    const K hi = a > b ? a : b, lo = a > b ? b : a;
+    a = hi;
+    b = lo;
+}
+// B keys in falling order: odd-even merge sort, about B log^2 B / 4 exchanges (recursion, so that every index is a constant)
+template <int LO, int N, int R, typename K>
+__device__ __forceinline__ void merge_halves(K* k)
+{
+    if constexpr (2 * R < N) {
+        merge_halves<LO, N, 2 * R>(k);
+        merge_halves<LO + R, N, 2 * R>(k);
+#pragma unroll
+        for (int i = LO + R; i + R < LO + N; i += 2 * R) larger_first(k[i], k[i + R]);
+    } else {
+        larger_first(k[LO], k[LO + R]);
+    }
+}
+template <int N, int LO = 0, typename K>
+__device__ __forceinline__ void sort_keys(K* k)
+{
+    if constexpr (N > 1) {
+        sort_keys<N / 2, LO>(k);
+        sort_keys<N / 2, LO + N / 2>(k);
+        merge_halves<LO, N, 1>(k);
+    }
+}
+// best, in falling order, becomes the best of itself and k, both in falling order: the larger of each with its opposite is a
+// bitonic row of the best B, which log B half-cleaners sort
+template <int B, typename K>
+__device__ __forceinline__ void merge_keys(K* best, const K* k)
+{
+#pragma unroll
+    for (int i = 0; i < B; ++i) best[i] = best[i] > k[B - 1 - i] ? best[i] : k[B - 1 - i];
+#pragma unroll
+    for (int d = B / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if ((i & d) == 0) larger_first(best[i], best[i + d]);
+}
+
 // ---- G threads to a row: a warp (of several in a block) or a whole block --------------------------------------------
 template <int G>
 struct Group {
     static constexpr int WARPS = G / 32;
-    // scratch: 3 * WARPS floats of shared memory for a block, unused by a warp
+    // scratch: 4 * WARPS floats of shared memory for a block, unused by a warp
     float* scratch;
     __device__ __forceinline__ int rank() const { return G == 32 ? (threadIdx.x & 31) : threadIdx.x; }
     __device__ __forceinline__ void sync() const
@@ -100,83 +254,259 @@ struct Group {
     }
 };
 
-// A row of K logits spread over G threads, in pieces of V values: piece p belongs to thread p % G.  V is what 16 bytes
-// hold where rows start on 16 bytes and end there, else 1.
-template <typename T, int V>
-__device__ __forceinline__ void load_piece(const T* row, int piece, int K, float (&v)[V])
-{
-    if (V == 1) {
-        v[0] = piece < K ? to_f<T>(row[piece]) : -INFINITY;
-    } else {
-        if (piece * V < K) {
-            typename Vec<T>::Raw raw = *reinterpret_cast<const typename Vec<T>::Raw*>(row + (int64_t)piece * V);
-            Vec<T>::unpack(raw, v);
+// A row in pieces of eight logits that start on 16 bytes (32 for fp32: two loads) wherever the row starts: `skip` values of the first
+// piece lie before it.  What a piece holds of its neighbours is masked; the pieces at the two ends of the whole matrix, which may reach
+// beyond it, are read value by value.
+template <typename T>
+struct RowPieces {
+    const T* row;
+    const T* base;           // the first piece, on 16 bytes
+    int skip, K, pieces;
+    bool whole;              // every piece lies within the matrix
+    __device__ __forceinline__ RowPieces(const T* logits, int64_t ld, int64_t n, int64_t r, int k)
+    {
+        row = logits + r * ld;
+        K = k;
+        skip = (int)(((uintptr_t)row & 15) / sizeof(T));
+        base = row - skip;
+        pieces = (skip + K + 7) / 8;
+        whole = base >= logits && base + (int64_t)pieces * 8 <= logits + (n - 1) * ld + K;
+    }
+    // class of the first value of piece p (may be negative)
+    __device__ __forceinline__ int first(int p) const { return p * 8 - skip; }
+    __device__ __forceinline__ Eight<T> load(int p) const
+    {
+        Eight<T> x;
+        const int j = first(p);
+        if (whole) {
+            const uint4* src = reinterpret_cast<const uint4*>(base + (int64_t)p * 8);
+            *reinterpret_cast<uint4*>(&x.w[0]) = src[0];
+            if (Eight<T>::WORDS == 8) *reinterpret_cast<uint4*>(&x.w[Eight<T>::WORDS - 4]) = src[1];
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = -INFINITY;
+            for (int q = 0; q < 4; ++q)
+                x.set(q, j + 2 * q >= 0 && j + 2 * q < K ? to_f<T>(row[j + 2 * q]) : 0.f,
+                      j + 2 * q + 1 >= 0 && j + 2 * q + 1 < K ? to_f<T>(row[j + 2 * q + 1]) : 0.f);
         }
+        if (j < 0) x.drop_first(-j);
+        if (j + 8 > K) x.keep_first(K - j);
+        return x;
     }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_piece(T* row, int piece, int K, const float (&v)[V])
-{
-    if (V == 1) {
-        if (piece < K) row[piece] = from_f<T>(v[0]);
-    } else if (piece * V < K) {
-        *reinterpret_cast<typename Vec<T>::Raw*>(row + (int64_t)piece * V) = Vec<T>::pack(v);
-    }
-}
-
-static inline bool rows_aligned(const void* p, int64_t ld, int K, int size)
-{
-    return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0 && (K * (int64_t)size) % 16 == 0;
-}
-
-// ---- a tile of rows in shared memory, one thread to a row -----------------------------------------------------------
-// Rows of up to SMALL_CLASSES logits, as fp32, an odd number of words apart: a thread reads its row without conflicts.
-constexpr int SMALL_CLASSES = 64;
-constexpr int TILE_ROWS = 128;
-
-__host__ __device__ __forceinline__ int tile_pitch(int K) { return K | 1; }
-
-// Walks the elements idx = first, first + step, ... of rows of K as (row, column) without dividing again.
-struct RowWalk {
-    int row, col, rows_step, cols_step, K;
-    __device__ __forceinline__ RowWalk(int first, int step, int k) : row(first / k), col(first % k), rows_step(step / k), cols_step(step % k), K(k) {}
-    __device__ __forceinline__ void next()
+    // into a row of results that lies as this one does with respect to 16 bytes (`alike`), or elsewhere
+    __device__ __forceinline__ void store(T* out, bool alike, int p, const Eight<T>& x) const
     {
-        row += rows_step;
-        col += cols_step;
-        if (col >= K) {
-            col -= K;
-            ++row;
+        const int j = first(p);
+        if (alike && j >= 0 && j + 8 <= K) {
+            uint4* dst = reinterpret_cast<uint4*>(out + j);
+            dst[0] = *reinterpret_cast<const uint4*>(&x.w[0]);
+            if (Eight<T>::WORDS == 8) dst[1] = *reinterpret_cast<const uint4*>(&x.w[Eight<T>::WORDS - 4]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i >= 0 && j + i < K) out[j + i] = from_f<T>(x.at(i));
         }
     }
 };
 
-template <typename T>
-__device__ __forceinline__ void load_tile(float* tile, const T* logits, int64_t ld, int64_t row0, int rows, int K)
-{
-    const int pitch = tile_pitch(K);
-    const T* src = logits + row0 * ld;
-    RowWalk w(threadIdx.x, TILE_ROWS, K);
-#pragma unroll 8
-    for (int idx = threadIdx.x; idx < rows * K; idx += TILE_ROWS) {
-        tile[w.row * pitch + w.col] = to_f<T>(src[w.row * ld + w.col]);
-        w.next();
+constexpr int WARP_ROWS = 4;    // warps of a block where a warp has a row
+// a row's pieces with G threads: P of each in registers, or none, to be read again for every pass
+template <typename T, int G, int P>
+struct RowValues {
+    Eight<T> x[P > 0 ? P : 1];
+    const RowPieces<T>& pieces;
+    int rank;
+    __device__ __forceinline__ RowValues(const RowPieces<T>& p, int me) : pieces(p), rank(me)
+    {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (i * G + rank < pieces.pieces)
+                x[i] = pieces.load(i * G + rank);
+            else
+                x[i].keep_first(0);
+        }
     }
-}
-template <typename T>
-__device__ __forceinline__ void store_tile(const float* tile, T* out, int64_t row0, int rows, int K)
-{
-    const int pitch = tile_pitch(K);
-    T* dst = out + row0 * K;
-    RowWalk w(threadIdx.x, TILE_ROWS, K);
-#pragma unroll 4
-    for (int idx = threadIdx.x; idx < rows * K; idx += TILE_ROWS) {
-        dst[idx] = from_f<T>(tile[w.row * pitch + w.col]);
-        w.next();
+    // f(eight logits, class of the first; those that are no class are minus infinity)
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const
+    {
+        if (P > 0) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) f(x[i], pieces.first(i * G + rank));
+        } else {
+            for (int p = rank; p < pieces.pieces; p += G) f(pieces.load(p), pieces.first(p));
+        }
     }
+};
+// ---- a tile of rows in shared memory, one thread to a row -----------------------------------------------------------
+// No sums or choices across threads: a row costs the fewest instructions so, and short rows are bound by these.  Rows lie as they do in
+// memory, so that a tile is copied in pieces of 16 bytes whatever K is; a thread reads eight logits at a time, as wide as rows are aligned:
+//   16 bytes  rows of a multiple of 16 bytes; an odd number of such pieces apart, so that eight neighbours' reads fill the banks
+//   8, 4      rows of another multiple of 8 or 4 bytes: an odd number of 8-byte pieces apart, or of words: no conflicts either
+//   2         rows of an odd number of bf16 values: neighbours share words, which are broadcast
+constexpr int TILE_SLACK = 64;      // bytes that the last row's last read may reach beyond it
+
+template <typename T>
+struct RowTile {
+    unsigned char* smem;
+    int K, pitch, width;            // bytes from row to row, bytes of a read
+    __host__ __device__ static int row_width(int K)
+    {
+        const int bytes = K * (int)sizeof(T);
+        return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : bytes % 4 == 0 ? 4 : 2;
+    }
+    __host__ __device__ static int row_pitch(int K)
+    {
+        const int bytes = K * (int)sizeof(T);
+        return bytes % 16 == 0 ? (bytes / 16 | 1) * 16 : bytes;
+    }
+    __device__ __forceinline__ RowTile(unsigned char* s, int k) : smem(s), K(k), pitch(row_pitch(k)), width(row_width(k)) {}
+    __device__ __forceinline__ T* row(int r) const { return reinterpret_cast<T*>(smem + r * pitch); }
+
+    // rows of the matrix into the tile (all threads; ends with a barrier).  wide: they may be read in pieces of 16 bytes, which is where
+    // they lie one behind the other, or each on 16 bytes
+    __device__ __forceinline__ void load(const T* logits, int64_t ld, int64_t row0, int rows, bool wide) const
+    {
+        const int threads = blockDim.x;
+        const T* src = logits + row0 * ld;
+        int done = 0;                // values
+        if (wide && width == 16) {
+            const int per_row = K * (int)sizeof(T) / 16;
+            int r = threadIdx.x / per_row, c = threadIdx.x % per_row;
+            const int dr = threads / per_row, dc = threads % per_row;
+            for (int i = threadIdx.x; i < rows * per_row; i += threads) {
+                copy16(smem + r * pitch + c * 16, reinterpret_cast<const unsigned char*>(src + r * ld) + c * 16);
+                r += dr;
+                c += dc;
+                if (c >= per_row) {
+                    c -= per_row;
+                    ++r;
+                }
+            }
+            done = rows * K;
+        } else if (wide) {
+            const int pieces = rows * K * (int)sizeof(T) / 16;
+            for (int i = threadIdx.x; i < pieces; i += threads) copy16(smem + i * 16, reinterpret_cast<const unsigned char*>(src) + i * 16);
+            done = pieces * (16 / (int)sizeof(T));
+        }
+        for (int i = done + threadIdx.x; i < rows * K; i += threads) {
+            const int r = i / K, c = i - r * K;
+            row(r)[c] = src[r * ld + c];
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+    }
+    // the tile's rows out to rows one behind the other (after a barrier of the caller's)
+    __device__ __forceinline__ void store(T* out, int64_t row0, int rows, bool wide) const
+    {
+        const int threads = blockDim.x;
+        T* dst = out + row0 * K;
+        int done = 0;
+        if (wide && width == 16) {
+            const int per_row = K * (int)sizeof(T) / 16;
+            int r = threadIdx.x / per_row, c = threadIdx.x % per_row;
+            const int dr = threads / per_row, dc = threads % per_row;
+            for (int i = threadIdx.x; i < rows * per_row; i += threads) {
+                reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(smem + r * pitch + c * 16);
+                r += dr;
+                c += dc;
+                if (c >= per_row) {
+                    c -= per_row;
+                    ++r;
+                }
+            }
+            done = rows * K;
+        } else if (wide) {
+            const int pieces = rows * K * (int)sizeof(T) / 16;
+            for (int i = threadIdx.x; i < pieces; i += threads) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(smem)[i];
+            done = pieces * (16 / (int)sizeof(T));
+        }
+        for (int i = done + threadIdx.x; i < rows * K; i += threads) {
+            const int r = i / K;
+            dst[i] = row(r)[i - r * K];
+        }
+    }
+    static __device__ __forceinline__ void copy16(void* to, const void* from)
+    {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+    }
+
+    // W: the tile's width, known to the compiler.  Values beyond the row are minus infinity.
+    template <int W>
+    __device__ __forceinline__ Eight<T> read(const T* r, int j) const
+    {
+        Eight<T> x;
+        const unsigned char* p = reinterpret_cast<const unsigned char*>(r + j);
+        if (W == 16) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS / 4; ++i) *reinterpret_cast<uint4*>(&x.w[4 * i]) = reinterpret_cast<const uint4*>(p)[i];
+        } else if (W == 8) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS / 2; ++i) *reinterpret_cast<uint2*>(&x.w[2 * i]) = reinterpret_cast<const uint2*>(p)[i];
+        } else if (W == 4) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS; ++i) x.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS; ++i) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+                x.w[i] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+            }
+        }
+        if (j + 8 > K) x.keep_first(K - j);
+        return x;
+    }
+    template <int W>
+    __device__ __forceinline__ void write(T* r, int j, const Eight<T>& x) const
+    {
+        unsigned char* p = reinterpret_cast<unsigned char*>(r + j);
+        if (j + 8 > K) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j + i < K) r[j + i] = from_f<T>(x.at(i));
+        } else if (W == 16) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS / 4; ++i) reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(&x.w[4 * i]);
+        } else if (W == 8) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS / 2; ++i) reinterpret_cast<uint2*>(p)[i] = *reinterpret_cast<const uint2*>(&x.w[2 * i]);
+        } else if (W == 4) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS; ++i) reinterpret_cast<uint32_t*>(p)[i] = x.w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::WORDS; ++i) {
+                uint16_t* h = reinterpret_cast<uint16_t*>(p) + 2 * i;
+                h[0] = (uint16_t)x.w[i];
+                h[1] = (uint16_t)(x.w[i] >> 16);
+            }
+        }
+    }
+    template <int W>
+    __device__ __forceinline__ float largest(const T* r) const
+    {
+        float m = -INFINITY;
+        for (int j = 0; j < K; j += 8) m = max_nan(m, read<W>(r, j).largest());
+        return m;
+    }
+    // whether `load` and `store` may take pieces of 16 bytes
+    static bool wide_rows(const void* p, int64_t ld, int K)
+    {
+        return ((uintptr_t)p & 15) == 0 && (ld == K || (ld * sizeof(T) % 16 == 0 && row_width(K) == 16));
+    }
+};
+
+// Rows and shared memory of a block with a tile.
+struct TileShape {
+    int rows;
+    size_t smem;
+};
+constexpr int TILE_ROW_BYTES = 512;       // rows beyond take a warp each
+template <typename T>
+static inline TileShape tile_shape(int K)
+{
+    const int pitch = RowTile<T>::row_pitch(K);
+    const int rows = pitch <= 272 ? 128 : 64;
+    return TileShape{rows, (size_t)rows * pitch + TILE_SLACK};
 }
 
 }  // namespace ptv3

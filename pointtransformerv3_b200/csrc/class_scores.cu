@@ -21,6 +21,7 @@ struct ScoresArgs {
     float2* stats;           // n x {m, log S} or NULL
     int K, top;
     float inv_t;
+    bool wide, wide_out;     // logits, gradient: see RowTile::wide_rows
     uint32_t* status;
     // backward
     const float *g_logp, *g_entropy;     // steps g_logp_step, g_entropy_step apart (0: one value for all), or NULL
@@ -66,196 +67,268 @@ __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, cons
     if (a.stats) a.stats[row] = make_float2(r.m, r.log_s);
 }
 
-// ---- the best classes, kept sorted in registers while a thread reads its row in order --------------------------------
-// bf16 logits and classes below 2^16 share a word, value above (inverted) class: a step of the insertion is a maximum and a
-// minimum.  Otherwise the classes move with the keys; equal keys stay in the order they come in, lowest class first.
-template <int TOP, bool PACKED>
-struct TopList {
-    uint32_t key[TOP > 0 ? TOP : 1];
-    int cls[TOP > 0 && !PACKED ? TOP : 1];
-    __device__ __forceinline__ void clear()
-    {
-#pragma unroll
-        for (int i = 0; i < TOP; ++i) {
-            key[i] = 0;
-            if (!PACKED) cls[i] = -1;
-        }
-    }
-    __device__ __forceinline__ void insert(float x, int j)
-    {
-        uint32_t k = order_key(x);
-        if (PACKED) {
-            k = (k & 0xffff0000u) | (0xffffu - j);
-#pragma unroll
-            for (int i = 0; i < TOP; ++i) {
-                const uint32_t hi = ::max(key[i], k);
-                k = ::min(key[i], k);
-                key[i] = hi;
-            }
-        } else {
-            bool up = false;     // from the first smaller key on, everything moves
-#pragma unroll
-            for (int i = 0; i < TOP; ++i) {
-                up |= k > key[i];
-                const uint32_t k2 = up ? key[i] : k;
-                const int j2 = up ? cls[i] : j;
-                key[i] = up ? k : key[i];
-                cls[i] = up ? j : cls[i];
-                k = k2;
-                j = j2;
-            }
-        }
-    }
-    __device__ __forceinline__ int at(int i) const
-    {
-        if (!PACKED) return cls[i];
-        return key[i] ? (int)(0xffffu - (key[i] & 0xffffu)) : -1;
-    }
-};
-
-// ---- up to SMALL_CLASSES classes: a tile of rows, one thread to a row -------------------------------------------------
-template <typename T, int TOP>
-__global__ void __launch_bounds__(TILE_ROWS) scores_tile_kernel(const ScoresArgs a)
+template <typename T, int TOP, typename Key>
+__device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, const RowSums& r, const Key (&best)[TOP > 0 ? TOP : 1])
 {
-    extern __shared__ __align__(16) float tile[];
-    const int64_t row0 = blockIdx.x * (int64_t)TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, a.n - row0);
-    load_tile(tile, (const T*)a.logits, a.ld, row0, rows, a.K);
-    __syncthreads();
-    if ((int)threadIdx.x >= rows) return;
-    const float* x = tile + threadIdx.x * tile_pitch(a.K);
-    const int64_t row = row0 + threadIdx.x;
-    TopList<TOP, sizeof(T) == 2> best;
-    best.clear();
-    float m = -INFINITY;
-    for (int j = 0; j < a.K; ++j) {
-        m = max_nan(m, x[j]);
-        if (TOP) best.insert(x[j], j);
-    }
-    const float origin = row_origin(m), c = a.inv_t * LOG2E;
-    float s = 0.f, u = 0.f;
-    for (int j = 0; j < a.K; ++j) {
-        const float d = below_max(x[j], origin), e = fast_exp2(d * c);
-        s += e;
-        u = fmaf(e, d, u);
-    }
-    const RowSums r = row_sums(m, s, u, a.inv_t);
-    write_row(a, row, r, [&](int j) { return x[j]; });
+    float v[TOP > 0 ? TOP : 1];
+#pragma unroll
+    for (int i = 0; i < TOP; ++i) v[i] = best[i] ? log_prob_of(r, TopKey<T>::value(best[i]), a.inv_t) : -INFINITY;
+    int32_t* cls = a.top_class + row * a.top;
+    float* val = a.top_logp + row * a.top;
 #pragma unroll
     for (int i = 0; i < TOP; ++i) {
         if (i < a.top) {
-            const int cls = best.at(i);
-            a.top_class[row * a.top + i] = cls;
-            a.top_logp[row * a.top + i] = cls < 0 ? -INFINITY : log_prob_of(r, x[cls], a.inv_t);
+            cls[i] = TopKey<T>::cls(best[i]);
+            val[i] = v[i];
         }
     }
 }
 
-// ---- more classes: G threads to a row -----------------------------------------------------------------------------------
-// The row's values stay in registers, E of each thread; rows beyond G x 32 are read again for every sum (E = 0).
-constexpr int WARP_ROWS = 4;    // warps of a block where a warp has a row
+// ---- short rows: a tile of rows, one thread to a row -----------------------------------------------------------------
+// TOP: 0, or 1, 2, 4, ... 32 alternatives at least.  The row is read twice from shared memory, for the largest (with their keys) and for
+// the sums.
+template <typename T, int W, int TOP>
+__global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
+{
+    using Top = TopKey<T>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const RowTile<T> tile(smem, a.K);
+    const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
+    const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
+    if ((int)threadIdx.x >= rows) return;
+    const T* x = tile.row(threadIdx.x);
+    const int64_t row = row0 + threadIdx.x;
 
-template <typename T, int V, int G, int E>
-struct RowValues {
-    static constexpr int P = E / V;
-    float v[E > 0 ? P : 1][V];
-    const T* row;
-    int K, rank;
-    __device__ __forceinline__ void load(const T* r, int k, int me)
-    {
-        row = r;
-        K = k;
-        rank = me;
-        if (E > 0) {
+    typename Top::Key best[TOP > 0 ? TOP : 1];
+    float m;
+    if (TOP == 0) {
+        m = tile.template largest<W>(x);
+    } else {
+        constexpr int STEP = TOP > 8 ? TOP : 8;        // classes at a time: what a sort takes
 #pragma unroll
-            for (int p = 0; p < P; ++p) load_piece<T, V>(row, p * G + rank, K, v[p]);
-        }
-    }
-    // f(value, class), classes ascending; those of no class are minus infinity
-    template <typename F>
-    __device__ __forceinline__ void each(F&& f) const
-    {
-        if (E > 0) {
+        for (int i = 0; i < TOP; ++i) best[i] = 0;
+        for (int j = 0; j < a.K; j += STEP) {
+            typename Top::Key k[STEP];
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+            for (int b = 0; b < STEP; b += 8) {
+                if (j + b < a.K) {
+                    Top::keys(tile.template read<W>(x, j + b), j + b, k + b);
+                    if (j + b + 8 > a.K) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) f(v[p][i], (p * G + rank) * V + i);
-        } else {
-            for (int p = rank; p * V < K; p += G) {
-                float w[V];
-                load_piece<T, V>(row, p, K, w);
+                        for (int i = 0; i < 8; ++i)
+                            if (j + b + i >= a.K) k[b + i] = 0;
+                    }
+                } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) f(w[i], p * V + i);
+                    for (int i = 0; i < 8; ++i) k[b + i] = 0;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < STEP; b += (TOP > 0 ? TOP : 1)) {
+                sort_keys<TOP>(k + b);
+                merge_keys<TOP>(best, k + b);
             }
         }
+        m = Top::value(best[0]);                       // (of NaN: one)
     }
+    const float origin = row_origin(m);
+    const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
+    RowSum sums;
+    sums.clear();
+    for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
+    const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u), a.inv_t);
+    write_row(a, row, r, [&](int j) { return to_f<T>(x[j]); });
+    write_top<T, TOP>(a, row, r, best);
+}
+
+// ---- longer rows: a warp, or a block of G threads ------------------------------------------------------------------------
+// A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).
+//
+// The alternatives.  Up to FEW: one after another, each a maximum over the row of what comes behind the last one.  More: every thread has
+// the largest of its pieces, 64 (128 for more than 32 alternatives) such maxima of a row are compared by the upper 16 bits of their keys, and the
+// k-th largest of these, found bit by bit, bounds the k-th largest of the row from below; the few logits at or above it (less than twice k
+// of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of few values), one after another again.
+constexpr int FEW = 3, CANDIDATES = 192;
+
+// value and class as one number, below ~0 (NaN of class 0); 0 for none
+__device__ __forceinline__ unsigned long long wide_key(float x, int j, int K)
+{
+    return (unsigned)j < (unsigned)K ? (unsigned long long)order_key(x) << 32 | (0x7fffffffu - j) : 0ull;
+}
+__device__ __forceinline__ int key_class(unsigned long long k) { return k ? (int)(0x7fffffffu - (uint32_t)k) : -1; }
+
+template <int G>
+struct TopScratch {
+    unsigned long long candidate[CANDIDATES];
+    unsigned long long chosen[G / 32];
+    uint16_t maxima[G > 32 ? 128 : 1];
+    uint32_t bound;
+    int count;
 };
 
-template <typename T, int V, int G, int E>
-__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_kernel(const ScoresArgs a)
+__device__ __forceinline__ void write_alternative(const ScoresArgs& a, int64_t row, const RowSums& r, int i, unsigned long long k)
 {
-    __shared__ float scratch[G > 32 ? 3 * (G / 32) : 1];
-    __shared__ unsigned long long chosen[G > 32 ? G / 32 : 1];
-    const Group<G> group{scratch};
-    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.n) return;
-    const int me = group.rank();
-    const T* x = (const T*)a.logits + row * a.ld;
-    RowValues<T, V, G, E> vals;
-    vals.load(x, a.K, me);
-    float m = -INFINITY;
-    vals.each([&](float v, int) { m = max_nan(m, v); });
-    m = group.max(m);
-    const float origin = row_origin(m), c = a.inv_t * LOG2E;
-    float su[2] = {0.f, 0.f};
-    vals.each([&](float v, int) {
-        const float d = below_max(v, origin), e = fast_exp2(d * c);
-        su[0] += e;
-        su[1] = fmaf(e, d, su[1]);
-    });
-    group.sum(su);
-    const RowSums r = row_sums(m, su[0], su[1], a.inv_t);
-    if (me == 0) write_row(a, row, r, [&](int j) { return to_f<T>(x[j]); });
+    a.top_class[row * a.top + i] = key_class(k);
+    a.top_logp[row * a.top + i] = k ? log_prob_of(r, order_value((uint32_t)(k >> 32)), a.inv_t) : -INFINITY;
+}
 
-    // one alternative after another: the largest of (key, lowest class) behind the last one
-    uint32_t last_key = 0xffffffffu;
-    int last_class = -1;
-    uint32_t key = 0;
-    int cls = 0x7fffffff;
+// the k-th largest (k = 1 ..) of N x 32 numbers of 16 bits, N with each lane, from below: the largest that so many reach
+template <int N>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[N], int k)
+{
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x8000; bit; bit >>= 1) {
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) reach += __popc(__ballot_sync(~0u, v[i] >= (bound | bit)));
+        if (reach >= k) bound |= bit;
+    }
+    return bound;
+}
+
+template <typename T, int G, int P>
+__device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, const RowSums& r, const RowValues<T, G, P>& vals,
+                                             const Group<G>& group, TopScratch<G>& scratch, float mine)
+{
+    const int me = group.rank(), lane = threadIdx.x & 31;
+    if (a.top > FEW) {
+        // maxima: of a thread's half or quarter of its pieces where a warp has the row, else of two or four threads
+        uint32_t bound = 0;
+        if (G == 32) {
+            if (a.top <= 32 && P >= 2) {
+                uint32_t v[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float m = vals.x[i].largest();
+                    v[i & 1] = ::max(v[i & 1], i * G + me < vals.pieces.pieces ? order_key(m) >> 16 : 0u);
+                }
+                bound = kth_largest(v, a.top);
+            } else if (a.top <= 32) {
+                const uint32_t v[1] = {me < vals.pieces.pieces ? order_key(mine) >> 16 : 0u};
+                bound = kth_largest(v, a.top);
+            }
+            // (more than 32 of a warp's row: a bound of 0 makes everything a candidate where the row is short, else one after another)
+        } else {
+            const int per = a.top <= 32 ? G / 64 : G / 128;      // threads that share a maximum
+            float m = mine;
+            for (int o = 1; o < per; o *= 2) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
+            if (lane % per == 0) scratch.maxima[me / per] = order_key(m) >> 16;
+            if (me == 0) scratch.count = 0;
+            __syncthreads();
+            if (me < 32) {
+                const uint32_t v[4] = {scratch.maxima[me], scratch.maxima[me + 32], a.top <= 32 ? 0u : scratch.maxima[me + 64],
+                                       a.top <= 32 ? 0u : scratch.maxima[me + 96]};
+                const uint32_t b = kth_largest(v, a.top);
+                if (me == 0) scratch.bound = b;
+            }
+            __syncthreads();
+            bound = scratch.bound;
+        }
+        int count = 0;
+        if (G == 32) {
+            // each lane's number, its place among the lanes', its candidates
+            vals.each([&](const Eight<T>& x, int j) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) count += (unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound;
+            });
+            int at = count;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int up = __shfl_up_sync(~0u, at, o);
+                if (lane >= o) at += up;
+            }
+            const int all = __shfl_sync(~0u, at, 31);
+            at -= count;
+            count = all;
+            if (count <= CANDIDATES) {
+                vals.each([&](const Eight<T>& x, int j) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if ((unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound) scratch.candidate[at++] = wide_key(x.at(i), j + i, a.K);
+                });
+            }
+        } else {
+            vals.each([&](const Eight<T>& x, int j) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound) {
+                        const int at = atomicAdd(&scratch.count, 1);
+                        if (at < CANDIDATES) scratch.candidate[at] = wide_key(x.at(i), j + i, a.K);
+                    }
+            });
+        }
+        group.sync();
+        if (G > 32) count = scratch.count;
+        if (count <= CANDIDATES) {
+            for (int i = me; i < ::max(count, a.top); i += G) {
+                if (i < count) {
+                    const unsigned long long k = scratch.candidate[i];
+                    int before = 0;
+                    for (int q = 0; q < count; ++q) before += scratch.candidate[q] > k;
+                    if (before < a.top) write_alternative(a, row, r, before, k);
+                } else {
+                    write_alternative(a, row, r, i, 0);          // no such class
+                }
+            }
+            return;
+        }
+    }
+    unsigned long long last = ~0ull, key = 0;
     bool again = true;
     for (int i = 0; i < a.top; ++i) {
         if (again) {
             key = 0;
-            cls = 0x7fffffff;
-            vals.each([&](float v, int j) {
-                const uint32_t k = order_key(v);
-                const bool left = j < a.K && (k < last_key || (k == last_key && j > last_class));
-                if (left && k > key) {
-                    key = k;
-                    cls = j;
+            vals.each([&](const Eight<T>& x, int j) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const unsigned long long k = wide_key(x.at(q), j + q, a.K);
+                    if (k < last && k > key) key = k;
                 }
             });
         }
-        uint32_t k = __reduce_max_sync(~0u, key);
-        int j = (int)__reduce_min_sync(~0u, key == k ? (uint32_t)cls : 0x7fffffffu);
+        const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(key >> 32));
+        const uint32_t lo = __reduce_max_sync(~0u, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+        unsigned long long k = (unsigned long long)hi << 32 | lo;
         if (G > 32) {
             __syncthreads();
-            if ((threadIdx.x & 31) == 0) chosen[threadIdx.x >> 5] = (unsigned long long)k << 32 | (0x7fffffffu - j);
+            if (lane == 0) scratch.chosen[threadIdx.x >> 5] = k;
             __syncthreads();
-            unsigned long long best = chosen[0];
+            k = scratch.chosen[0];
 #pragma unroll
-            for (int w = 1; w < G / 32; ++w) best = best > chosen[w] ? best : chosen[w];
-            k = (uint32_t)(best >> 32);
-            j = (int)(0x7fffffffu - (uint32_t)best);
+            for (int w = 1; w < G / 32; ++w) k = k > scratch.chosen[w] ? k : scratch.chosen[w];
         }
-        again = j == cls;
-        last_key = k;
-        last_class = j;
-        if (me == 0) {
-            a.top_class[row * a.top + i] = k ? j : -1;
-            a.top_logp[row * a.top + i] = k ? log_prob_of(r, order_value(k), a.inv_t) : -INFINITY;
-        }
+        again = k == key;
+        last = k;
+        if (me == 0) write_alternative(a, row, r, i, k);
     }
+}
+
+template <typename T, int G, int P, bool TOPS>
+__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_kernel(const ScoresArgs a)
+{
+    constexpr int SLOTS = G == 32 ? WARP_ROWS : 1;
+    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
+    __shared__ TopScratch<G> top_scratch[TOPS ? SLOTS : 1];
+    const Group<G> group{scratch};
+    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= a.n) return;
+    const int me = group.rank();
+    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const RowValues<T, G, P> vals(pieces, me);
+    float mine = -INFINITY;
+    vals.each([&](const Eight<T>& x, int) { mine = max_nan(mine, x.largest()); });
+    const float m = group.max(mine), origin = row_origin(m);
+    const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
+    RowSum sums;
+    sums.clear();
+    vals.each([&](const Eight<T>& x, int) { sums.add(x, minus, c2); });
+    float su[2] = {hsum2(sums.s), hsum2(sums.u)};
+    group.sum(su);
+    const RowSums r = row_sums(m, su[0], su[1], a.inv_t);
+    if (me == 0) write_row(a, row, r, [&](int j) { return to_f<T>(pieces.row[j]); });
+    if (TOPS) alternatives<T, G, P>(a, row, r, vals, group, top_scratch[G == 32 ? threadIdx.x >> 5 : 0], mine);
 }
 
 // ---- gradient -------------------------------------------------------------------------------------------------------------
@@ -299,17 +372,49 @@ __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, fl
     return r;
 }
 
+// the gradient of one class again, with the alternative's own part
 template <typename T>
-__global__ void __launch_bounds__(TILE_ROWS) scores_tile_bwd_kernel(const ScoresArgs a)
+__device__ __forceinline__ T grad_of(const RowGrad& r, const T* logits, int j, float own)
 {
-    extern __shared__ __align__(16) float tile[];
-    const int64_t row0 = blockIdx.x * (int64_t)TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, a.n - row0);
-    load_tile(tile, (const T*)a.logits, a.ld, row0, rows, a.K);
-    __syncthreads();
+    return from_f<T>(fmaf(own, r.inv_t, r.at(to_f<T>(logits[j]), j)));
+}
+// Eight of a row's gradient, without own parts: p A, or p (A + B log p)
+template <typename T>
+__device__ __forceinline__ void grad_eight(const RowGrad& r, Eight<T>& x)
+{
+    const uint64_t c2 = pack2(r.inv_t * LOG2E, r.inv_t * LOG2E), minus = pack2(-r.m, -r.m);
+    const float shift = -r.log_s * LOG2E, a = r.A * r.inv_t;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float d0, d1, t0, t1;
+        unpack2(add2(x.pair(q), minus), d0, d1);
+        d0 = max_nan(d0, -1e38f);
+        d1 = max_nan(d1, -1e38f);
+        unpack2(fma2(pack2(d0, d1), c2, pack2(shift, shift)), t0, t1);
+        const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
+        if (r.B == 0.f) {
+            x.set(q, p0 * a, p1 * a);
+        } else {
+            // p log p of a class without a probability is 0 (p > 0 fails for it; NaN passes by A)
+            const float b0 = p0 > 0.f ? fmaf(r.B, fmaf(d0, r.inv_t, -r.log_s), r.A) : r.A;
+            const float b1 = p1 > 0.f ? fmaf(r.B, fmaf(d1, r.inv_t, -r.log_s), r.A) : r.A;
+            x.set(q, p0 * b0 * r.inv_t, p1 * b1 * r.inv_t);
+        }
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a)
+{
+    extern __shared__ __align__(16) unsigned char smem[];
+    const RowTile<T> tile(smem, a.K);
+    const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
+    const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
     if ((int)threadIdx.x < rows) {
         const int64_t row = row0 + threadIdx.x;
-        float* x = tile + threadIdx.x * tile_pitch(a.K);
+        T* x = tile.row(threadIdx.x);
+        const T* logits = (const T*)a.logits + row * a.ld;
         const float* gt = a.g_top ? a.g_top + row * a.top : nullptr;
         const int32_t* tc = a.g_top ? a.top_class + row * a.top : nullptr;
         float g_sum = 0.f;
@@ -317,25 +422,33 @@ __global__ void __launch_bounds__(TILE_ROWS) scores_tile_bwd_kernel(const Scores
             for (int i = 0; i < a.top; ++i) g_sum += tc[i] >= 0 ? gt[i] : 0.f;
         bool none;
         const RowGrad r = row_grad(a, row, g_sum, none);
-        for (int j = 0; j < a.K; ++j) x[j] = r.at(x[j], j);
+        const T label = r.label >= 0 ? grad_of<T>(r, x, r.label, 0.f) : from_f<T>(0.f);
+        for (int j = 0; j < a.K; j += 8) {
+            Eight<T> e = tile.template read<W>(x, j);
+            grad_eight(r, e);
+            tile.template write<W>(x, j, e);
+        }
+        if (r.label >= 0) x[r.label] = label;
         if (gt && !none)
             for (int i = 0; i < a.top; ++i)
-                if (tc[i] >= 0) x[tc[i]] += gt[i] * a.inv_t;
+                if (tc[i] >= 0) x[tc[i]] = grad_of<T>(r, logits, tc[i], gt[i]);
     }
     __syncthreads();
-    store_tile(tile, (T*)a.dlogits, row0, rows, a.K);
+    tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
-template <typename T, int V, int G>
+template <typename T, int G>
 __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_bwd_kernel(const ScoresArgs a)
 {
-    __shared__ float scratch[G > 32 ? 3 * (G / 32) : 1];
+    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
     const Group<G> group{scratch};
     const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.n) return;
     const int me = group.rank();
-    const T* x = (const T*)a.logits + row * a.ld;
+    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
+    const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
     const float* gt = a.g_top ? a.g_top + row * a.top : nullptr;
     const int32_t* tc = a.g_top ? a.top_class + row * a.top : nullptr;
     float g_sum[1] = {0.f};
@@ -345,92 +458,97 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_bwd_k
     }
     bool none;
     const RowGrad r = row_grad(a, row, g_sum[0], none);
-#pragma unroll 4
-    for (int p = me; p * V < a.K; p += G) {
-        float v[V];
-        load_piece<T, V>(x, p, a.K, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = r.at(v[i], p * V + i);
-        store_piece<T, V>(dx, p, a.K, v);
+#pragma unroll 2
+    for (int p = me; p < pieces.pieces; p += G) {
+        Eight<T> e = pieces.load(p);
+        grad_eight(r, e);
+        pieces.store(dx, alike, p, e);
     }
+    // classes with parts of their own once more: the label, then the alternatives (of which the label may be one)
+    group.sync();
+    if (me == 0 && r.label >= 0) dx[r.label] = grad_of<T>(r, x, r.label, 0.f);
     if (gt && !none) {
-        // the alternatives once more, with their own parts
         group.sync();
         for (int i = me; i < a.top; i += G)
-            if (tc[i] >= 0) dx[tc[i]] = from_f<T>(fmaf(gt[i], a.inv_t, r.at(to_f<T>(x[tc[i]]), tc[i])));
+            if (tc[i] >= 0) dx[tc[i]] = grad_of<T>(r, x, tc[i], gt[i]);
     }
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
-template <typename T>
-static void launch_tile(const ScoresArgs& a, cudaStream_t stream)
+template <typename T, int W>
+static bool launch_tile(const ScoresArgs& a, bool backward, cudaStream_t stream)
 {
-    const unsigned blocks = (unsigned)((a.n + TILE_ROWS - 1) / TILE_ROWS);
-    const size_t smem = (size_t)TILE_ROWS * tile_pitch(a.K) * sizeof(float);
-    if (a.top == 0)
-        scores_tile_kernel<T, 0><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    else if (a.top <= 4)
-        scores_tile_kernel<T, 4><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    else if (a.top <= 8)
-        scores_tile_kernel<T, 8><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    else if (a.top <= 16)
-        scores_tile_kernel<T, 16><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    else if (a.top <= 32)
-        scores_tile_kernel<T, 32><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    else
-        scores_tile_kernel<T, 64><<<blocks, TILE_ROWS, smem, stream>>>(a);
+    const TileShape shape = tile_shape<T>(a.K);
+    const unsigned blocks = (unsigned)((a.n + shape.rows - 1) / shape.rows);
+    auto run = [&](auto kern) {
+        if (shape.smem > 48 * 1024 && allow_smem(kern) != cudaSuccess) return false;
+        kern<<<blocks, shape.rows, shape.smem, stream>>>(a);
+        return true;
+    };
+    if (backward) return run(scores_tile_bwd_kernel<T, W>);
+    if (a.top == 0) return run(scores_tile_kernel<T, W, 0>);
+    if (a.top == 1) return run(scores_tile_kernel<T, W, 1>);
+    if (a.top == 2) return run(scores_tile_kernel<T, W, 2>);
+    if (a.top <= 4) return run(scores_tile_kernel<T, W, 4>);
+    if (a.top <= 8) return run(scores_tile_kernel<T, W, 8>);
+    if (a.top <= 16) return run(scores_tile_kernel<T, W, 16>);
+    return run(scores_tile_kernel<T, W, 32>);
+}
+template <typename T>
+static bool launch_tile_of(const ScoresArgs& a, bool backward, cudaStream_t stream)
+{
+    switch (RowTile<T>::row_width(a.K)) {
+    case 16: return launch_tile<T, 16>(a, backward, stream);
+    case 8: return launch_tile<T, 8>(a, backward, stream);
+    case 4: return launch_tile<T, 4>(a, backward, stream);
+    default: return launch_tile<T, sizeof(T) == 2 ? 2 : 4>(a, backward, stream);
+    }
 }
 
-template <typename T, int V>
+template <typename T, bool TOPS>
 static void launch_rows(const ScoresArgs& a, cudaStream_t stream)
 {
     const unsigned warps = (unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), rows = (unsigned)a.n;
-    if (a.K <= 256)
-        scores_row_kernel<T, V, 32, 8><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (a.K <= 512)
-        scores_row_kernel<T, V, 32, 16><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (a.K <= 1024)
-        scores_row_kernel<T, V, 32, 32><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (a.K <= 2048)
-        scores_row_kernel<T, V, 256, 8><<<rows, 256, 0, stream>>>(a);
-    else if (a.K <= 4096)
-        scores_row_kernel<T, V, 256, 16><<<rows, 256, 0, stream>>>(a);
-    else if (a.K <= 8192)
-        scores_row_kernel<T, V, 256, 32><<<rows, 256, 0, stream>>>(a);
+    const int most = a.K + 16 / (int)sizeof(T) - 1;      // with what the first piece may skip
+    if (most <= 256)
+        scores_row_kernel<T, 32, 1, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
+    else if (most <= 512)
+        scores_row_kernel<T, 32, 2, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
+    else if (most <= 1024)
+        scores_row_kernel<T, 32, 4, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
+    else if (most <= 2048)
+        scores_row_kernel<T, 32, 8, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
+    else if (most <= 4096)
+        scores_row_kernel<T, 256, 2, TOPS><<<rows, 256, 0, stream>>>(a);
+    else if (most <= 8192)
+        scores_row_kernel<T, 256, 4, TOPS><<<rows, 256, 0, stream>>>(a);
+    else if (most <= 16384)
+        scores_row_kernel<T, 512, 4, TOPS><<<rows, 512, 0, stream>>>(a);
     else
-        scores_row_kernel<T, V, 256, 0><<<rows, 256, 0, stream>>>(a);
-}
-
-template <typename T, int V>
-static void launch_rows_bwd(const ScoresArgs& a, cudaStream_t stream)
-{
-    if (a.K <= 1024)
-        scores_row_bwd_kernel<T, V, 32><<<(unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, stream>>>(a);
-    else
-        scores_row_bwd_kernel<T, V, 256><<<(unsigned)a.n, 256, 0, stream>>>(a);
+        scores_row_kernel<T, 1024, 0, TOPS><<<rows, 1024, 0, stream>>>(a);
 }
 
 template <typename T>
-static int launch_scores(const ScoresArgs& a, bool backward, cudaStream_t stream)
+static int launch_scores(ScoresArgs a, bool backward, cudaStream_t stream)
 {
-    const bool wide = rows_aligned(a.logits, a.ld, a.K, sizeof(T)) && (!backward || ((uintptr_t)a.dlogits & 15) == 0);
-    if (backward) {
-        if (a.K <= SMALL_CLASSES)
-            scores_tile_bwd_kernel<T><<<(unsigned)((a.n + TILE_ROWS - 1) / TILE_ROWS), TILE_ROWS,
-                                        (size_t)TILE_ROWS * tile_pitch(a.K) * sizeof(float), stream>>>(a);
-        else if (wide)
-            launch_rows_bwd<T, Vec<T>::N>(a, stream);
+    a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
+    a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
+    const char* what = backward ? "ptv3_class_scores_bwd" : "ptv3_class_scores_fwd";
+    // a thread keeps up to 32 alternatives; beyond, and for longer rows, a warp chooses them
+    if (a.K * sizeof(T) <= TILE_ROW_BYTES && (backward || a.top <= 32)) {
+        if (!launch_tile_of<T>(a, backward, stream)) return check_launch("ptv3_class_scores: shared memory attribute");
+    } else if (backward) {
+        if (a.K <= 2048)
+            scores_row_bwd_kernel<T, 32><<<(unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, stream>>>(a);
         else
-            launch_rows_bwd<T, 1>(a, stream);
-    } else if (a.K <= SMALL_CLASSES) {
-        launch_tile<T>(a, stream);
-    } else if (wide) {
-        launch_rows<T, Vec<T>::N>(a, stream);
+            scores_row_bwd_kernel<T, 256><<<(unsigned)a.n, 256, 0, stream>>>(a);
+    } else if (a.top) {
+        launch_rows<T, true>(a, stream);
     } else {
-        launch_rows<T, 1>(a, stream);
+        launch_rows<T, false>(a, stream);
     }
     count_launches(1);
-    return check_launch(backward ? "ptv3_class_scores_bwd" : "ptv3_class_scores_fwd");
+    return check_launch(what);
 }
 
 static int check_scores(const char* what, const ScoresArgs& a, float temperature, int dtype)

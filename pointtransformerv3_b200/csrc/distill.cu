@@ -20,7 +20,7 @@ struct DistillArgs {
     const void* teacher;      // n x k
     const void* list;         // n x k
     int list_bytes, k, K, rest;
-    bool teacher_bf16;
+    bool teacher_bf16, wide, wide_out;      // wide: logits, gradient: see RowTile::wide_rows
     float* loss;              // n
     float4* stats;            // n x {m, log S, log of the outside's sum or the list's largest, t_r or 1 / the list's sum}, or NULL
     float inv_t;
@@ -37,110 +37,123 @@ __device__ __forceinline__ int list_class(const DistillArgs& a, int64_t i)
     return c >= 0 && c < a.K ? (int)c : (c == -1 ? PLACE_ABSENT : PLACE_BAD);
 }
 
-// what a list says by itself: the largest value, the sum of probabilities, whether there is an entry
-struct ListSums {
-    float top, sum;
-    bool any, bad;
-    // probability of an entry
-    __device__ __forceinline__ float prob(float v, int rest, float inv_t) const
-    {
-        return rest ? fast_exp2(v * LOG2E) : fast_exp2(below_max(v, row_origin(top)) * (inv_t * LOG2E));
-    }
-};
 // t log t - t log p of an entry; nothing where t is 0
 __device__ __forceinline__ float entry_loss(float t, float log_t, float log_p) { return t == 0.f ? 0.f : t * (log_t - log_p); }
 
 // t_r = 1 - sum t: of one large and other small entries the large one's part is taken by expm1
 __device__ __forceinline__ float rest_prob(float top, float others) { return fmaxf(-expm1f(fminf(top, 0.f)) - others, 0.f); }
 
-// ---- up to SMALL_CLASSES classes ------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(TILE_ROWS) distill_tile_kernel(const DistillArgs a)
+// a list entry as it comes: the teacher's probability before its sum is known
+__device__ __forceinline__ float entry_weight(const DistillArgs& a, float v, float top)
 {
-    extern __shared__ __align__(16) float tile[];
-    const int64_t row0 = blockIdx.x * (int64_t)TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, a.n - row0);
-    load_tile(tile, (const T*)a.logits, a.ld, row0, rows, a.K);
-    __syncthreads();
+    return a.rest ? fast_exp2(v * LOG2E) : fast_exp2(below_max(v, row_origin(top)) * (a.inv_t * LOG2E));
+}
+constexpr float GAP_SCALE = 1.f / LIST_MAX;
+// What a row's list adds up to.  With w the entries' weights (t itself, or t times their sum), z = d / T the student's and l the teacher's
+// logits at the temperature (v, or (v - top) / T), the list's part of the loss is  sum w (l - z) / W + log S - log W  for W = sum w.
+struct ListSums {
+    float top;         // the largest value
+    float sum;         // W
+    float others;      // without the largest
+    float gap;         // sum w (l - z), the terms of w = 0 left out; without a rest a 64th of it (W may be 64, l - z the largest number)
+    __device__ __forceinline__ float loss(bool rest, float log_s) const
+    {
+        if (rest) return sum == 0.f ? 0.f : fmaf(sum, log_s, gap);
+        return sum > 0.f ? __fdiv_rn(gap, sum * GAP_SCALE) + log_s - logf(sum) : sum;      // (NaN stays)
+    }
+};
+// log of a sum of the outside's exponentials; `again` takes it from its own maximum
+template <typename F>
+__device__ __forceinline__ float log_outside(float sum, F&& again)
+{
+    return sum >= REST_TOO_SMALL ? logf(sum) : again();
+}
+
+// ---- short rows: a tile of rows, one thread to a row ---------------------------------------------------------------
+// The list is walked twice, for its largest value and for its sums.  With an outcome for the rest, the list's classes are then masked in
+// the tile: one pass over the row gives the outside's sum, and the list's own exponentials make it the row's.
+template <typename T, int W>
+__global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
+{
+    extern __shared__ __align__(16) unsigned char smem[];
+    const RowTile<T> tile(smem, a.K);
+    const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
+    const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
     if ((int)threadIdx.x >= rows) return;
-    const float* x = tile + threadIdx.x * tile_pitch(a.K);
+    T* x = tile.row(threadIdx.x);
     const int64_t row = row0 + threadIdx.x, at = row * a.k;
 
-    float m = -INFINITY;
-    for (int j = 0; j < a.K; ++j) m = max_nan(m, x[j]);
-    const float origin = row_origin(m), c = a.inv_t * LOG2E;
-    ListSums l{-INFINITY, 0.f, false, false};
-    uint64_t inside = 0;
-    int first = 0;
+    const float m = tile.template largest<W>(x), origin = row_origin(m), c = a.inv_t * LOG2E;
+    bool any = false, bad = false;
+    ListSums l{-INFINITY, 0.f, 0.f, 0.f};
+    if (!a.rest)
+        for (int i = 0; i < a.k; ++i)
+            if (list_class(a, at + i) >= 0) l.top = max_nan(l.top, load_value(a.teacher, a.teacher_bf16, at + i));
+    float most = 0.f, inside = 0.f;
     for (int i = 0; i < a.k; ++i) {
         const int cls = list_class(a, at + i);
-        l.bad |= cls == PLACE_BAD;
+        bad |= cls == PLACE_BAD;
         if (cls < 0) continue;
-        const float v = load_value(a.teacher, a.teacher_bf16, at + i);
-        inside |= 1ull << cls;
-        if (!l.any || v > l.top || v != v) {
-            first = i;
-            l.top = v;
+        any = true;
+        const float v = load_value(a.teacher, a.teacher_bf16, at + i), w = entry_weight(a, v, l.top), d = to_f<T>(x[cls]) - origin;
+        l.sum += w;
+        if (a.rest) {
+            if (v > l.top) {
+                l.others += most;
+                most = w;
+                l.top = v;
+            } else {
+                l.others += w;
+            }
         }
-        l.any = true;
+        if (w != 0.f) l.gap = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(l.top)) * a.inv_t) - d * a.inv_t, l.gap);
     }
-    float s = 0.f, out = 0.f, out_max = -INFINITY;
-    for (int j = 0; j < a.K; ++j) {
-        const float e = fast_exp2(below_max(x[j], origin) * c);
-        s += e;
-        if (a.rest && !(inside >> j & 1)) {
-            out += e;
-            out_max = max_nan(out_max, x[j]);
+    if (a.rest) {
+        for (int i = 0; i < a.k; ++i) {
+            const int cls = list_class(a, at + i);
+            if (cls < 0) continue;
+            inside += fast_exp2(below_max(to_f<T>(x[cls]), origin) * c);       // (a class that comes again is masked by then)
+            x[cls] = from_f<T>(-INFINITY);
         }
     }
+    const uint64_t c2 = pack2(c, c), minus = pack2(-origin, -origin);
+    RowSum sums;
+    sums.clear();
+    for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
+    const float outside = hsum2(sums.s), s = outside + inside;
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
-    float log_out = -INFINITY;
-    if (a.rest && out_max != -INFINITY) {
-        if (out >= REST_TOO_SMALL || out != out) {
-            log_out = logf(out);
-        } else {
-            out = 0.f;
-            for (int j = 0; j < a.K; ++j)
-                if (!(inside >> j & 1)) out += fast_exp2(below_max(x[j], out_max) * c);
-            log_out = (out_max - origin) * a.inv_t + logf(out);
+    float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
+    if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
+    if (a.rest) {
+        log_out = log_outside(outside, [&]() {
+            const float om = tile.template largest<W>(x);
+            if (om == -INFINITY) return -INFINITY;
+            RowSum again;
+            again.clear();
+            const uint64_t mo = pack2(-om, -om);
+            for (int j = 0; j < a.K; j += 8) again.add(tile.template read<W>(x, j), mo, c2);
+            return (om - origin) * a.inv_t + logf(hsum2(again.s));
+        });
+        if (any && log_out != -INFINITY) {
+            t_r = rest_prob(l.top, l.others);
+            loss += entry_loss(t_r, logf(t_r), log_out - log_s);
         }
     }
-    // the list's sums, then its part of the loss
-    float others = 0.f, loss = 0.f;
-    for (int i = 0; i < a.k; ++i) {
-        const int cls = list_class(a, at + i);
-        if (cls < 0) continue;
-        const float t = l.prob(load_value(a.teacher, a.teacher_bf16, at + i), a.rest, a.inv_t);
-        l.sum += t;
-        if (i != first) others += t;
-    }
-    const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
-    const float log_scale = a.rest || !(l.sum > 0.f) ? 0.f : logf(l.sum);
-    for (int i = 0; i < a.k; ++i) {
-        const int cls = list_class(a, at + i);
-        if (cls < 0) continue;
-        const float v = load_value(a.teacher, a.teacher_bf16, at + i);
-        const float log_t = a.rest ? v : below_max(v, row_origin(l.top)) * a.inv_t - log_scale;
-        const float log_p = none ? -INFINITY : (x[cls] - origin) * a.inv_t - log_s;
-        loss += entry_loss(l.prob(v, a.rest, a.inv_t) * scale, log_t, log_p);
-    }
-    float t_r = 0.f;
-    if (a.rest && l.any && log_out != -INFINITY) {
-        t_r = rest_prob(l.top, others);
-        loss += entry_loss(t_r, logf(t_r), log_out - log_s);
-    }
-    if (l.bad) {
+    if (bad) {
         loss = NAN;
         atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
     }
     a.loss[row] = loss;
-    if (a.stats) a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r) : make_float4(origin, log_s, row_origin(l.top), scale);
+    if (a.stats)
+        a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
+                              : make_float4(origin, log_s, row_origin(l.top), l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
 }
 
-// ---- more classes: G threads to a row -----------------------------------------------------------------------------------
-constexpr int WARP_ROWS = 4;
-
+// ---- longer rows: a warp, or a block of G threads ------------------------------------------------------------------------
+// A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).  With an outcome
+// for the rest, the list's classes are bits in shared memory, which a piece's eight are cut out of.
 // the list, entry i with thread i % G of the first warp of a row's threads
 template <int G>
 struct ListPart {
@@ -158,116 +171,123 @@ struct ListPart {
     }
 };
 
-template <typename T, int V, int G>
+// words of bits of a row: a piece may begin before class 0 and end behind the last, so one word more on either side
+__host__ __device__ __forceinline__ int bit_words(int K) { return (K + 31) / 32 + 2; }
+
+template <typename T, int G, int P>
 __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_kernel(const DistillArgs a)
 {
-    __shared__ float scratch_s[G > 32 ? 5 * (G / 32) : 1];
-    extern __shared__ uint32_t bits_s[];             // a bit for every class in the list: (K + 31) / 32 words to a row
-    const Group<G> group{scratch_s};
+    __shared__ float scratch[G > 32 ? 5 * (G / 32) : 1];
+    extern __shared__ uint32_t bits_s[];
+    const Group<G> group{scratch};
     const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.n) return;
-    const int me = group.rank(), words = (a.K + 31) / 32;
+    const int me = group.rank(), words = bit_words(a.K);
     uint32_t* bits = bits_s + (G == 32 ? (threadIdx.x >> 5) * words : 0);
-    const T* x = (const T*)a.logits + row * a.ld;
+    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const T* x = pieces.row;
     ListPart<G> list;
     list.load(a, row * a.k, me);
+    const RowValues<T, G, P> vals(pieces, me);
     if (a.rest) {
         for (int w = me; w < words; w += G) bits[w] = 0;
         group.sync();
 #pragma unroll
         for (int q = 0; q < ListPart<G>::N; ++q)
-            if (list.cls[q] >= 0) atomicOr(&bits[list.cls[q] >> 5], 1u << (list.cls[q] & 31));
+            if (list.cls[q] >= 0) atomicOr(&bits[(list.cls[q] >> 5) + 1], 1u << (list.cls[q] & 31));
         group.sync();
     }
     float m = -INFINITY;
-    for (int p = me; p * V < a.K; p += G) {
-        float v[V];
-        load_piece<T, V>(x, p, a.K, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) m = max_nan(m, v[i]);
-    }
+    vals.each([&](const Eight<T>& e, int) { m = max_nan(m, e.largest()); });
     m = group.max(m);
     const float origin = row_origin(m), c = a.inv_t * LOG2E;
-    float out_max = -INFINITY, sums[2] = {0.f, 0.f};
-    for (int p = me; p * V < a.K; p += G) {
-        float v[V];
-        load_piece<T, V>(x, p, a.K, v);
-        const uint32_t in = a.rest ? bits[p * V >> 5] >> (p * V & 31) : 0;
+    const uint64_t c2 = pack2(c, c), minus = pack2(-origin, -origin);
+    // the classes of the list as bits of a piece
+    auto listed = [&](int j) {
+        const int at = j + 32;
+        return __funnelshift_r(bits[at >> 5], bits[(at >> 5) + 1], at & 31) & 0xffu;
+    };
+    auto masked = [&](const Eight<T>& e, int j) {
+        Eight<T> o = e;
+        const uint32_t in = listed(j);
+        if (in) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float e = fast_exp2(below_max(v[i], origin) * c);
-            sums[0] += e;
-            if (a.rest && !(in >> i & 1)) {
-                sums[1] += e;
-                out_max = max_nan(out_max, v[i]);
-            }
+            for (int q = 0; q < 4; ++q) o.set(q, in >> (2 * q) & 1 ? -INFINITY : e.at(2 * q), in >> (2 * q + 1) & 1 ? -INFINITY : e.at(2 * q + 1));
         }
-    }
-    group.sum(sums);
-    const bool none = sums[0] == 0.f;
-    const float log_s = none ? -INFINITY : log1pf(sums[0] - 1.f);
-    float log_out = -INFINITY;
-    if (a.rest) {
-        out_max = group.max(out_max);
-        if (out_max != -INFINITY) {
-            if (sums[1] >= REST_TOO_SMALL || sums[1] != sums[1]) {
-                log_out = logf(sums[1]);
-            } else {
-                float again[1] = {0.f};
-                for (int j = me; j < a.K; j += G)
-                    if (!(bits[j >> 5] >> (j & 31) & 1)) again[0] += fast_exp2(below_max(to_f<T>(x[j]), out_max) * c);
-                group.sum(again);
-                log_out = (out_max - origin) * a.inv_t + logf(again[0]);
+        return o;
+    };
+    RowSum sums;
+    sums.clear();
+    float inside = 0.f;
+    if (a.rest)
+        vals.each([&](const Eight<T>& e, int j) {
+            if (j >= a.K) return;
+            sums.add(masked(e, j), minus, c2);
+            if (const uint32_t in = listed(j)) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (in >> q & 1) inside += fast_exp2(below_max(e.at(q), origin) * c);
             }
-        }
-    }
-    // the list
+        });
+    else
+        vals.each([&](const Eight<T>& e, int) { sums.add(e, minus, c2); });
+
+    // the list: its largest value, then its sums
     float top = -INFINITY;
-    bool any = false, bad = false;
 #pragma unroll
-    for (int q = 0; q < ListPart<G>::N; ++q) {
-        any |= list.cls[q] >= 0;
-        bad |= list.cls[q] == PLACE_BAD;
-        top = max_nan(top, list.v[q]);
-    }
+    for (int q = 0; q < ListPart<G>::N; ++q) top = max_nan(top, list.v[q]);
     top = group.max(top);
-    const ListSums l{top, 0.f, false, false};
-    // sum of t, entries, bad ones, entries that are as large as the largest
-    float ls[4] = {0.f, any ? 1.f : 0.f, bad ? 1.f : 0.f, 0.f};
-    float t[ListPart<G>::N];
+    // the row's (or the outside's) sum; weights but the largest's, all, their gap; entries, bad ones, entries that are as large as the
+    // largest; the inside's sum
+    float all[4] = {hsum2(sums.s), 0.f, 0.f, 0.f}, counts[4] = {0.f, 0.f, 0.f, inside};
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
-        t[q] = list.cls[q] >= 0 ? l.prob(list.v[q], a.rest, a.inv_t) : 0.f;
-        const bool is_top = list.cls[q] >= 0 && list.v[q] == top;
-        ls[0] += a.rest && is_top ? 0.f : t[q];
-        ls[3] += is_top ? 1.f : 0.f;
+        counts[1] += list.cls[q] == PLACE_BAD ? 1.f : 0.f;
+        if (list.cls[q] < 0) continue;
+        counts[0] += 1.f;
+        const float v = list.v[q], w = entry_weight(a, v, top), d = to_f<T>(x[list.cls[q]]) - origin;
+        const bool is_top = a.rest && v == top;
+        all[1] += is_top ? 0.f : w;
+        counts[2] += is_top ? 1.f : 0.f;
+        all[2] += w;
+        if (w != 0.f) all[3] = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(top)) * a.inv_t) - d * a.inv_t, all[3]);
     }
-    group.sum(ls);
-    float scale = 1.f, log_scale = 0.f, t_r = 0.f;
-    if (!a.rest) {
-        scale = ls[0] > 0.f ? __fdiv_rn(1.f, ls[0]) : ls[0];
-        log_scale = ls[0] > 0.f ? logf(ls[0]) : 0.f;
-    } else if (ls[1] > 0.f && log_out != -INFINITY) {
-        t_r = rest_prob(top, ls[0] + (ls[3] - 1.f) * fast_exp2(top * LOG2E));
-    }
-    float loss[1] = {0.f};
-#pragma unroll
-    for (int q = 0; q < ListPart<G>::N; ++q) {
-        if (list.cls[q] >= 0) {
-            const float log_t = a.rest ? list.v[q] : below_max(list.v[q], row_origin(top)) * a.inv_t - log_scale;
-            const float log_p = none ? -INFINITY : (to_f<T>(x[list.cls[q]]) - origin) * a.inv_t - log_s;
-            loss[0] += entry_loss(t[q] * scale, log_t, log_p);
+    group.sum(all);
+    group.sum(counts);
+    const float s = all[0] + counts[3];
+    const bool none = s == 0.f;
+    const float log_s = none ? -INFINITY : log1pf(s - 1.f);
+    ListSums l{top, all[2], all[1] + fmaxf(counts[2] - 1.f, 0.f) * fast_exp2(top * LOG2E), all[3]};
+    float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
+    if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
+    if (a.rest) {
+        log_out = log_outside(all[0], [&]() {
+            float om = -INFINITY;
+            vals.each([&](const Eight<T>& e, int j) { if (j < a.K) om = max_nan(om, masked(e, j).largest()); });
+            om = group.max(om);
+            if (om == -INFINITY) return -INFINITY;
+            RowSum again;
+            again.clear();
+            const uint64_t mo = pack2(-om, -om);
+            vals.each([&](const Eight<T>& e, int j) { if (j < a.K) again.add(masked(e, j), mo, c2); });
+            float o[1] = {hsum2(again.s)};
+            group.sum(o);
+            return (om - origin) * a.inv_t + logf(o[0]);
+        });
+        if (counts[0] > 0.f && log_out != -INFINITY) {
+            t_r = rest_prob(l.top, l.others);
+            loss += entry_loss(t_r, logf(t_r), log_out - log_s);
         }
     }
-    group.sum(loss);
     if (me == 0) {
-        if (a.rest) loss[0] += entry_loss(t_r, logf(t_r), log_out - log_s);
-        if (ls[2] > 0.f) {
-            loss[0] = NAN;
+        if (counts[1] > 0.f) {
+            loss = NAN;
             atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
         }
-        a.loss[row] = loss[0];
-        if (a.stats) a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r) : make_float4(origin, log_s, row_origin(top), scale);
+        a.loss[row] = loss;
+        if (a.stats)
+            a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
+                                  : make_float4(origin, log_s, row_origin(top), l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
     }
 }
 
@@ -307,49 +327,79 @@ __device__ __forceinline__ float entry_prob(const DistillArgs& a, float4 st, flo
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TILE_ROWS) distill_tile_bwd_kernel(const DistillArgs a)
+__device__ __forceinline__ void grad_eight(const DistillGrad& r, Eight<T>& x)
 {
-    extern __shared__ __align__(16) float tile[];
-    const int64_t row0 = blockIdx.x * (int64_t)TILE_ROWS;
-    const int rows = (int)min((int64_t)TILE_ROWS, a.n - row0);
-    load_tile(tile, (const T*)a.logits, a.ld, row0, rows, a.K);
-    __syncthreads();
+    const uint64_t c2 = pack2(r.c, r.c), minus = pack2(-r.m, -r.m), shift = pack2(r.shift, r.shift);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float d0, d1, t0, t1;
+        unpack2(add2(x.pair(q), minus), d0, d1);
+        unpack2(fma2(pack2(max_nan(d0, -1e38f), max_nan(d1, -1e38f)), c2, shift), t0, t1);
+        x.set(q, fast_exp2(t0) * r.factor, fast_exp2(t1) * r.factor);
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs a)
+{
+    extern __shared__ __align__(16) unsigned char smem[];
+    const RowTile<T> tile(smem, a.K);
+    const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
+    const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
     if ((int)threadIdx.x < rows) {
         const int64_t row = row0 + threadIdx.x, at = row * a.k;
-        float* x = tile + threadIdx.x * tile_pitch(a.K);
-        const T* again = (const T*)a.logits + row * a.ld;
+        T* x = tile.row(threadIdx.x);
+        const T* logits = (const T*)a.logits + row * a.ld;
         const float4 st = a.stats[row];
         float mass = 0.f;
         for (int i = 0; i < a.k; ++i)
             if (list_class(a, at + i) >= 0) mass += entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + i));
         const DistillGrad r = distill_grad(a, row, st, mass);
-        for (int j = 0; j < a.K; ++j) x[j] = r.at(x[j]);
-        if (a.rest)
-            for (int i = 0; i < a.k; ++i) {
-                const int cls = list_class(a, at + i);
-                if (cls >= 0) x[cls] = r.in_list(to_f<T>(again[cls]));
-            }
+        for (int j = 0; j < a.K; j += 8) {
+            Eight<T> e = tile.template read<W>(x, j);
+            grad_eight(r, e);
+            tile.template write<W>(x, j, e);
+        }
+        // the list's classes once more.  An entry leaves its number at its class first: where it is another's afterwards, a class comes twice,
+        // and every entry of the row writes the sum over its class.
         for (int i = 0; i < a.k; ++i) {
             const int cls = list_class(a, at + i);
-            if (cls >= 0) x[cls] -= r.g * entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + i));
+            if (cls >= 0) x[cls] = from_f<T>((float)i);
+        }
+        bool twice = false;
+        for (int i = 0; i < a.k; ++i) {
+            const int cls = list_class(a, at + i);
+            if (cls >= 0) twice |= to_f<T>(x[cls]) != (float)i;
+        }
+        for (int i = 0; i < a.k; ++i) {
+            const int cls = list_class(a, at + i);
+            if (cls < 0) continue;
+            float t = twice ? 0.f : entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + i));
+            if (twice)
+                for (int q = 0; q < a.k; ++q)
+                    if (list_class(a, at + q) == cls) t += entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + q));
+            x[cls] = from_f<T>(r.in_list(to_f<T>(logits[cls])) - r.g * t);
         }
     }
     __syncthreads();
-    store_tile(tile, (T*)a.dlogits, row0, rows, a.K);
+    tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
-template <typename T, int V, int G>
+template <typename T, int G>
 __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_bwd_kernel(const DistillArgs a)
 {
-    __shared__ float scratch[G > 32 ? 3 * (G / 32) : 1];
+    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
     __shared__ int list_c[G == 32 ? WARP_ROWS : 1][LIST_MAX];
     __shared__ float list_t[G == 32 ? WARP_ROWS : 1][LIST_MAX];
     const Group<G> group{scratch};
     const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.n) return;
     const int me = group.rank(), slot = G == 32 ? threadIdx.x >> 5 : 0;
-    const T* x = (const T*)a.logits + row * a.ld;
+    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
+    const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
     const float4 st = a.stats[row];
     ListPart<G> list;
     list.load(a, row * a.k, me);
@@ -365,13 +415,11 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_bwd_
     }
     group.sum(mass);
     const DistillGrad r = distill_grad(a, row, st, mass[0]);
-#pragma unroll 4
-    for (int p = me; p * V < a.K; p += G) {
-        float v[V];
-        load_piece<T, V>(x, p, a.K, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = r.at(v[i]);
-        store_piece<T, V>(dx, p, a.K, v);
+#pragma unroll 2
+    for (int p = me; p < pieces.pieces; p += G) {
+        Eight<T> e = pieces.load(p);
+        grad_eight(r, e);
+        pieces.store(dx, alike, p, e);
     }
     // the list's classes once more; one that comes twice is written by its first entry, with the sum of both
     group.sync();
@@ -392,36 +440,56 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_bwd_
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
-template <typename T, int V, int G>
-static int launch_distill_rows(const DistillArgs& a, bool backward, cudaStream_t stream)
+template <typename T, int W>
+static bool launch_tile(const DistillArgs& a, bool backward, cudaStream_t stream)
+{
+    const TileShape shape = tile_shape<T>(a.K);
+    const unsigned blocks = (unsigned)((a.n + shape.rows - 1) / shape.rows);
+    auto run = [&](auto kern) {
+        if (shape.smem > 48 * 1024 && allow_smem(kern) != cudaSuccess) return false;
+        kern<<<blocks, shape.rows, shape.smem, stream>>>(a);
+        return true;
+    };
+    return backward ? run(distill_tile_bwd_kernel<T, W>) : run(distill_tile_kernel<T, W>);
+}
+template <typename T, int G, int P>
+static void launch_rows(const DistillArgs& a, cudaStream_t stream)
 {
     const unsigned blocks = G == 32 ? (unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS) : (unsigned)a.n;
-    const int threads = G == 32 ? 32 * WARP_ROWS : G;
-    if (backward) {
-        distill_row_bwd_kernel<T, V, G><<<blocks, threads, 0, stream>>>(a);
-    } else {
-        const size_t smem = a.rest ? (size_t)((a.K + 31) / 32) * 4 * (G == 32 ? WARP_ROWS : 1) : 0;
-        distill_row_kernel<T, V, G><<<blocks, threads, smem, stream>>>(a);
-    }
-    return 0;
+    const size_t smem = a.rest ? (size_t)bit_words(a.K) * 4 * (G == 32 ? WARP_ROWS : 1) : 0;
+    distill_row_kernel<T, G, P><<<blocks, G == 32 ? 32 * WARP_ROWS : G, smem, stream>>>(a);
 }
 
 template <typename T>
-static int launch_distill(const DistillArgs& a, bool backward, cudaStream_t stream)
+static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
 {
-    const bool wide = rows_aligned(a.logits, a.ld, a.K, sizeof(T)) && (!backward || ((uintptr_t)a.dlogits & 15) == 0);
-    constexpr int V = Vec<T>::N;
-    if (a.K <= SMALL_CLASSES) {
-        const unsigned blocks = (unsigned)((a.n + TILE_ROWS - 1) / TILE_ROWS);
-        const size_t smem = (size_t)TILE_ROWS * tile_pitch(a.K) * sizeof(float);
-        if (backward)
-            distill_tile_bwd_kernel<T><<<blocks, TILE_ROWS, smem, stream>>>(a);
+    a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
+    a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
+    const int most = a.K + 16 / (int)sizeof(T) - 1;      // with what the first piece may skip
+    if (a.K * sizeof(T) <= TILE_ROW_BYTES) {
+        bool ok;
+        switch (RowTile<T>::row_width(a.K)) {
+        case 16: ok = launch_tile<T, 16>(a, backward, stream); break;
+        case 8: ok = launch_tile<T, 8>(a, backward, stream); break;
+        case 4: ok = launch_tile<T, 4>(a, backward, stream); break;
+        default: ok = launch_tile<T, sizeof(T) == 2 ? 2 : 4>(a, backward, stream); break;
+        }
+        if (!ok) return check_launch("ptv3_distill_topk: shared memory attribute");
+    } else if (backward) {
+        if (a.K <= 2048)
+            distill_row_bwd_kernel<T, 32><<<(unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, stream>>>(a);
         else
-            distill_tile_kernel<T><<<blocks, TILE_ROWS, smem, stream>>>(a);
-    } else if (a.K <= 1024) {
-        wide ? launch_distill_rows<T, V, 32>(a, backward, stream) : launch_distill_rows<T, 1, 32>(a, backward, stream);
+            distill_row_bwd_kernel<T, 256><<<(unsigned)a.n, 256, 0, stream>>>(a);
+    } else if (most <= 512) {
+        launch_rows<T, 32, 2>(a, stream);
+    } else if (most <= 1024) {
+        launch_rows<T, 32, 4>(a, stream);
+    } else if (most <= 2048) {
+        launch_rows<T, 32, 8>(a, stream);
+    } else if (most <= 8192) {
+        launch_rows<T, 256, 4>(a, stream);
     } else {
-        wide ? launch_distill_rows<T, V, 256>(a, backward, stream) : launch_distill_rows<T, 1, 256>(a, backward, stream);
+        launch_rows<T, 1024, 0>(a, stream);
     }
     count_launches(1);
     return check_launch(backward ? "ptv3_distill_topk_bwd" : "ptv3_distill_topk_fwd");

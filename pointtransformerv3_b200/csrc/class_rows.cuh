@@ -2,11 +2,11 @@
 //
 // z = x / T, m = max x, S = sum exp((x - m) / T), log p_j = (x_j - m) / T - log S.  The maximum is taken out of the
 // logits themselves, before the division, so that rows of any height keep their differences; a gradient is made from m and
-// log S apart, for the same reason.  Exponentials are 2^(d c), d = x - m, c = log2(e) / T, on the exponential unit
+// log S apart, for the same reason.  Exponentials are 2^t, t = (x - m) c, c = log2(e) / T, on the exponential unit
 // (relative error 2^-22); log S is log1p(S - 1), the accurate function, once per row: near a certain class log S is small, and
 // the fast logarithm has an absolute error there.
 //
-// Masked classes are minus infinity: d is held at -1e38, whose exponential is zero, so that 0 * d is zero too.  NaN and plus
+// Masked classes are minus infinity: t is held at -200, whose power is zero in fp32, so that 0 * t is zero too.  NaN and plus
 // infinity pass through max.NaN and make the row's sums NaN.  A row of minus infinities alone has S = 0.
 #pragma once
 #include "common.cuh"
@@ -105,7 +105,8 @@ template <> struct Eight<float> {
     }
 };
 
-// S and U = sum e d of a row, in packed pairs
+constexpr float NO_POWER = -200.f;
+// S and U = sum e t of a row, in packed pairs
 struct RowSum {
     uint64_t s, u;
     __device__ __forceinline__ void clear() { s = u = 0; }
@@ -114,16 +115,30 @@ struct RowSum {
     {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            float lo, hi, e0, e1;
-            unpack2(add2(x.pair(q), minus_origin), lo, hi);
-            const uint64_t d = pack2(max_nan(lo, -1e38f), max_nan(hi, -1e38f));
-            unpack2(mul2(d, c), e0, e1);
-            const uint64_t e = pack2(fast_exp2(e0), fast_exp2(e1));
+            float lo, hi;
+            unpack2(mul2(add2(x.pair(q), minus_origin), c), lo, hi);
+            lo = max_nan(lo, NO_POWER);
+            hi = max_nan(hi, NO_POWER);
+            const uint64_t e = pack2(fast_exp2(lo), fast_exp2(hi));
             s = add2(s, e);
-            u = fma2(e, d, u);
+            u = fma2(e, pack2(lo, hi), u);
         }
     }
 };
+// Eight of a gradient: p (A + B t) with p = 2^t, t = (x - m) c + shift = log2 p
+template <typename T>
+__device__ __forceinline__ void row_gradient(Eight<T>& x, uint64_t minus_m, uint64_t c, uint64_t shift, uint64_t A, uint64_t B)
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float lo, hi;
+        unpack2(fma2(add2(x.pair(q), minus_m), c, shift), lo, hi);
+        lo = max_nan(lo, NO_POWER);
+        hi = max_nan(hi, NO_POWER);
+        unpack2(mul2(pack2(fast_exp2(lo), fast_exp2(hi)), fma2(pack2(lo, hi), B, A)), lo, hi);
+        x.set(q, lo, hi);
+    }
+}
 
 // ---- the largest of a row, kept sorted in a thread's registers ------------------------------------------------------------
 // Keys say value and class: the larger value first, then the lower class, so that no two are equal and the order in which they
@@ -202,16 +217,20 @@ __device__ __forceinline__ void merge_keys(K* best, const K* k)
             if ((i & d) == 0) larger_first(best[i], best[i + d]);
 }
 
-// ---- G threads to a row: a warp (of several in a block) or a whole block --------------------------------------------
+// ---- G threads to a row: part of a warp, a warp, or a block ----------------------------------------------------------
 template <int G>
 struct Group {
-    static constexpr int WARPS = G / 32;
+    static constexpr int WARPS = G <= 32 ? 1 : G / 32;
+    static constexpr int BLOCK = G <= 32 ? 128 : G;           // threads of a block
+    static constexpr int ROWS = G <= 32 ? 128 / G : 1;        // rows of a block
     // scratch: 4 * WARPS floats of shared memory for a block, unused by a warp
     float* scratch;
-    __device__ __forceinline__ int rank() const { return G == 32 ? (threadIdx.x & 31) : threadIdx.x; }
+    __device__ __forceinline__ int rank() const { return threadIdx.x & (G - 1); }
+    __device__ __forceinline__ int slot() const { return G <= 32 ? threadIdx.x / G : 0; }
+    __device__ __forceinline__ int64_t row() const { return blockIdx.x * (int64_t)ROWS + slot(); }
     __device__ __forceinline__ void sync() const
     {
-        if (G == 32)
+        if (G <= 32)
             __syncwarp();
         else
             __syncthreads();
@@ -219,7 +238,7 @@ struct Group {
     __device__ __forceinline__ float max(float v) const
     {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+        for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
         if (G > 32) {
             __syncthreads();
             if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
@@ -235,7 +254,7 @@ struct Group {
     __device__ __forceinline__ void sum(float (&v)[N]) const
     {
 #pragma unroll
-        for (int o = 16; o; o >>= 1)
+        for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1)
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(~0u, v[i], o);
         if (G > 32) {
@@ -252,6 +271,7 @@ struct Group {
                 for (int i = 0; i < N; ++i) v[i] += scratch[N * w + i];
         }
     }
+    static unsigned blocks(int64_t n) { return (unsigned)((n + ROWS - 1) / ROWS); }
 };
 
 // A row in pieces of eight logits that start on 16 bytes (32 for fp32: two loads) wherever the row starts: `skip` values of the first
@@ -308,7 +328,6 @@ struct RowPieces {
     }
 };
 
-constexpr int WARP_ROWS = 4;    // warps of a block where a warp has a row
 // a row's pieces with G threads: P of each in registers, or none, to be read again for every pass
 template <typename T, int G, int P>
 struct RowValues {
@@ -331,12 +350,20 @@ struct RowValues {
     {
         if (P > 0) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) f(x[i], pieces.first(i * G + rank));
+            for (int i = 0; i < P; ++i)
+                if (i * G < pieces.pieces) f(x[i], pieces.first(i * G + rank));
         } else {
             for (int p = rank; p < pieces.pieces; p += G) f(pieces.load(p), pieces.first(p));
         }
     }
 };
+// logits that a row's first piece may skip
+template <typename T>
+static inline int most_skipped(const void* p, int64_t ld)
+{
+    return ((uintptr_t)p & 15) == 0 && ld * sizeof(T) % 16 == 0 ? 0 : 16 / (int)sizeof(T) - 1;
+}
+
 // ---- a tile of rows in shared memory, one thread to a row -----------------------------------------------------------
 // No sums or choices across threads: a row costs the fewest instructions so, and short rows are bound by these.  Rows lie as they do in
 // memory, so that a tile is copied in pieces of 16 bytes whatever K is; a thread reads eight logits at a time, as wide as rows are aligned:
@@ -500,7 +527,8 @@ struct TileShape {
     int rows;
     size_t smem;
 };
-constexpr int TILE_ROW_BYTES = 512;       // rows beyond take a warp each
+// rows beyond are spread over threads: those of which the best are asked for, and the others
+constexpr size_t TILE_TOP_BYTES = 512, TILE_PLAIN_BYTES = 128;
 template <typename T>
 static inline TileShape tile_shape(int K)
 {

@@ -2,7 +2,7 @@
 // of all three with respect to the logits.  No counterpart in the reference, whose file ends with the backbone
 // (model.py:966-982); the formulas stand in class_rows.cuh and below.
 //
-//     H = log S - (1/S) sum e_j d_j / T,    e_j = exp(d_j / T), d_j = x_j - m
+//     H = log S - (ln 2 / S) sum e_j t_j,    e_j = 2^t_j, t_j = (x_j - m) log2(e) / T
 //     dx_j = 1/T ( p_j (A + B log p_j) + [j = label] g + sum_i [j = t_i] g_i ),   A = -(g + sum g_i) - h H,  B = -h
 // with g, h, g_i the gradients of the three.
 #include "class_rows.cuh"
@@ -34,14 +34,15 @@ struct RowSums {
     float m, log_s, entropy;   // m: what was taken out; log_s: minus infinity for a row without a class
     bool none;
 };
-// S, U = sum e d -> log S and the entropy
-__device__ __forceinline__ RowSums row_sums(float m, float s, float u, float inv_t)
+constexpr float LN2 = 0.693147180559945309f;
+// S, U = sum e t -> log S and the entropy
+__device__ __forceinline__ RowSums row_sums(float m, float s, float u)
 {
     RowSums r;
     r.m = row_origin(m);
     r.none = s == 0.f;
     r.log_s = r.none ? -INFINITY : log1pf(s - 1.f);
-    r.entropy = r.none ? 0.f : r.log_s - __fdiv_rn(u * inv_t, s);
+    r.entropy = r.none ? 0.f : r.log_s - __fdiv_rn(u * LN2, s);
     return r;
 }
 __device__ __forceinline__ float log_prob_of(const RowSums& r, float x, float inv_t)
@@ -70,16 +71,15 @@ __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, cons
 template <typename T, int TOP, typename Key>
 __device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, const RowSums& r, const Key (&best)[TOP > 0 ? TOP : 1])
 {
-    float v[TOP > 0 ? TOP : 1];
-#pragma unroll
-    for (int i = 0; i < TOP; ++i) v[i] = best[i] ? log_prob_of(r, TopKey<T>::value(best[i]), a.inv_t) : -INFINITY;
-    int32_t* cls = a.top_class + row * a.top;
-    float* val = a.top_logp + row * a.top;
+    int32_t* to_class = a.top_class + row * a.top;
+    float* to_value = a.top_logp + row * a.top;
 #pragma unroll
     for (int i = 0; i < TOP; ++i) {
         if (i < a.top) {
-            cls[i] = TopKey<T>::cls(best[i]);
-            val[i] = v[i];
+            const int cls = TopKey<T>::cls(best[i]);
+            const bool is = (unsigned)cls < (unsigned)a.K;
+            to_class[i] = is ? cls : -1;
+            to_value[i] = is ? log_prob_of(r, TopKey<T>::value(best[i]), a.inv_t) : -INFINITY;
         }
     }
 }
@@ -105,20 +105,14 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     if (TOP == 0) {
         m = tile.template largest<W>(x);
     } else {
+        // (the values beyond the row are minus infinity of classes that do not exist: behind every class that does)
         constexpr int STEP = TOP > 8 ? TOP : 8;        // classes at a time: what a sort takes
-#pragma unroll
-        for (int i = 0; i < TOP; ++i) best[i] = 0;
         for (int j = 0; j < a.K; j += STEP) {
             typename Top::Key k[STEP];
 #pragma unroll
             for (int b = 0; b < STEP; b += 8) {
-                if (j + b < a.K) {
+                if (b == 0 || j + b < a.K) {
                     Top::keys(tile.template read<W>(x, j + b), j + b, k + b);
-                    if (j + b + 8 > a.K) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (j + b + i >= a.K) k[b + i] = 0;
-                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) k[b + i] = 0;
@@ -127,7 +121,12 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
 #pragma unroll
             for (int b = 0; b < STEP; b += (TOP > 0 ? TOP : 1)) {
                 sort_keys<TOP>(k + b);
-                merge_keys<TOP>(best, k + b);
+                if (b == 0 && j == 0) {
+#pragma unroll
+                    for (int i = 0; i < TOP; ++i) best[i] = k[i];
+                } else {
+                    merge_keys<TOP>(best, k + b);
+                }
             }
         }
         m = Top::value(best[0]);                       // (of NaN: one)
@@ -137,12 +136,12 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     RowSum sums;
     sums.clear();
     for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
-    const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u), a.inv_t);
+    const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u));
     write_row(a, row, r, [&](int j) { return to_f<T>(x[j]); });
     write_top<T, TOP>(a, row, r, best);
 }
 
-// ---- longer rows: a warp, or a block of G threads ------------------------------------------------------------------------
+// ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------------------
 // A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).
 //
 // The alternatives.  Up to FEW: one after another, each a maximum over the row of what comes behind the last one.  More: every thread has
@@ -226,12 +225,23 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
             __syncthreads();
             bound = scratch.bound;
         }
+        // at or above the bound as logits (NaN is), compared as they are: eight at once, since few pieces have one
+        const float least = order_value(bound << 16);
+        auto any = [&](const Eight<T>& x) {
+            bool yes = bound == 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) yes |= !(x.at(i) < least);
+            return yes;
+        };
+        auto is = [&](float v, int j) { return (unsigned)j < (unsigned)a.K && (bound == 0 || !(v < least)); };
         int count = 0;
         if (G == 32) {
             // each lane's number, its place among the lanes', its candidates
             vals.each([&](const Eight<T>& x, int j) {
+                if (any(x)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) count += (unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound;
+                    for (int i = 0; i < 8; ++i) count += is(x.at(i), j + i);
+                }
             });
             int at = count;
 #pragma unroll
@@ -244,19 +254,23 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
             count = all;
             if (count <= CANDIDATES) {
                 vals.each([&](const Eight<T>& x, int j) {
+                    if (any(x)) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if ((unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound) scratch.candidate[at++] = wide_key(x.at(i), j + i, a.K);
+                        for (int i = 0; i < 8; ++i)
+                            if (is(x.at(i), j + i)) scratch.candidate[at++] = wide_key(x.at(i), j + i, a.K);
+                    }
                 });
             }
         } else {
             vals.each([&](const Eight<T>& x, int j) {
+                if (any(x)) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if ((unsigned)(j + i) < (unsigned)a.K && order_key(x.at(i)) >> 16 >= bound) {
-                        const int at = atomicAdd(&scratch.count, 1);
-                        if (at < CANDIDATES) scratch.candidate[at] = wide_key(x.at(i), j + i, a.K);
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        if (is(x.at(i), j + i)) {
+                            const int at = atomicAdd(&scratch.count, 1);
+                            if (at < CANDIDATES) scratch.candidate[at] = wide_key(x.at(i), j + i, a.K);
+                        }
+                }
             });
         }
         group.sync();
@@ -306,16 +320,14 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
 }
 
 template <typename T, int G, int P, bool TOPS>
-__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_kernel(const ScoresArgs a)
 {
-    constexpr int SLOTS = G == 32 ? WARP_ROWS : 1;
-    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
-    __shared__ TopScratch<G> top_scratch[TOPS ? SLOTS : 1];
+    __shared__ float scratch[4 * Group<G>::WARPS];
+    __shared__ TopScratch<TOPS ? G : 32> top_scratch[TOPS ? Group<G>::ROWS : 1];
     const Group<G> group{scratch};
-    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.n) return;
+    const int64_t row = group.row(), at = min(row, a.n - 1);        // (threads beyond the last row keep it company)
     const int me = group.rank();
-    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, at, a.K);
     const RowValues<T, G, P> vals(pieces, me);
     float mine = -INFINITY;
     vals.each([&](const Eight<T>& x, int) { mine = max_nan(mine, x.largest()); });
@@ -326,23 +338,27 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_kerne
     vals.each([&](const Eight<T>& x, int) { sums.add(x, minus, c2); });
     float su[2] = {hsum2(sums.s), hsum2(sums.u)};
     group.sum(su);
-    const RowSums r = row_sums(m, su[0], su[1], a.inv_t);
-    if (me == 0) write_row(a, row, r, [&](int j) { return to_f<T>(pieces.row[j]); });
-    if (TOPS) alternatives<T, G, P>(a, row, r, vals, group, top_scratch[G == 32 ? threadIdx.x >> 5 : 0], mine);
+    const RowSums r = row_sums(m, su[0], su[1]);
+    if (me == 0 && row < a.n) write_row(a, row, r, [&](int j) { return to_f<T>(pieces.row[j]); });
+    if constexpr (TOPS) {
+        if (row < a.n) alternatives<T, G, P>(a, row, r, vals, group, top_scratch[group.slot()], mine);     // (whole warps)
+    }
 }
 
 // ---- gradient -------------------------------------------------------------------------------------------------------------
 struct RowGrad {
-    float m, log_s, A, B, g, inv_t;
+    float m, c, shift, A, B, g, inv_t;      // A, B, g: with 1 / T in them; B for a logarithm of base 2
     int label;
-    // without the alternatives' own parts
-    __device__ __forceinline__ float at(float x, int j) const
+    template <typename T>
+    __device__ __forceinline__ void eight(Eight<T>& x) const
     {
-        const float d = below_max(x, m);
-        const float p = fast_exp2(fmaf(d, inv_t * LOG2E, -log_s * LOG2E));
-        float v = p * (B != 0.f && p > 0.f ? fmaf(B, fmaf(d, inv_t, -log_s), A) : A);
-        if (j == label) v += g;
-        return v * inv_t;
+        row_gradient(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(A, A), pack2(B, B));
+    }
+    // one class, with the part of its own
+    __device__ __forceinline__ float at(float x, int j, float own) const
+    {
+        const float t = max_nan(fmaf(x - m, c, shift), NO_POWER);
+        return fmaf(fast_exp2(t), fmaf(t, B, A), fmaf(own, inv_t, j == label ? g : 0.f));
     }
 };
 __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, float g_top_sum, bool& none)
@@ -351,56 +367,23 @@ __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, fl
     const float2 st = a.stats[row];
     none = st.y == -INFINITY;
     r.m = st.x;
-    r.log_s = none ? INFINITY : st.y;
+    r.c = a.inv_t * LOG2E;
+    r.shift = none ? -INFINITY : -st.y * LOG2E;
     r.inv_t = a.inv_t;
     r.label = -1;
-    r.g = 0.f;
+    float g = 0.f;
     if (a.g_logp) {
         const int64_t label = load_index(a.labels, a.label_bytes, row);
-        if (label != a.ignore && label >= 0 && label < a.K) {
+        if (label != a.ignore && label >= 0 && label < a.K && !none) {
             r.label = (int)label;
-            r.g = a.g_logp[row * a.g_logp_step];
+            g = a.g_logp[row * a.g_logp_step];
         }
     }
     const float h = a.g_entropy ? a.g_entropy[row * a.g_entropy_step] : 0.f;
-    r.A = -(r.g + g_top_sum) - (a.g_entropy ? h * a.entropy[row] : 0.f);
-    r.B = -h;
-    if (none) {
-        r.A = r.B = r.g = 0.f;
-        r.label = -1;
-    }
+    r.g = g * a.inv_t;
+    r.A = none ? 0.f : (-(g + g_top_sum) - (a.g_entropy ? h * a.entropy[row] : 0.f)) * a.inv_t;
+    r.B = none ? 0.f : -h * a.inv_t * LN2;
     return r;
-}
-
-// the gradient of one class again, with the alternative's own part
-template <typename T>
-__device__ __forceinline__ T grad_of(const RowGrad& r, const T* logits, int j, float own)
-{
-    return from_f<T>(fmaf(own, r.inv_t, r.at(to_f<T>(logits[j]), j)));
-}
-// Eight of a row's gradient, without own parts: p A, or p (A + B log p)
-template <typename T>
-__device__ __forceinline__ void grad_eight(const RowGrad& r, Eight<T>& x)
-{
-    const uint64_t c2 = pack2(r.inv_t * LOG2E, r.inv_t * LOG2E), minus = pack2(-r.m, -r.m);
-    const float shift = -r.log_s * LOG2E, a = r.A * r.inv_t;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float d0, d1, t0, t1;
-        unpack2(add2(x.pair(q), minus), d0, d1);
-        d0 = max_nan(d0, -1e38f);
-        d1 = max_nan(d1, -1e38f);
-        unpack2(fma2(pack2(d0, d1), c2, pack2(shift, shift)), t0, t1);
-        const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
-        if (r.B == 0.f) {
-            x.set(q, p0 * a, p1 * a);
-        } else {
-            // p log p of a class without a probability is 0 (p > 0 fails for it; NaN passes by A)
-            const float b0 = p0 > 0.f ? fmaf(r.B, fmaf(d0, r.inv_t, -r.log_s), r.A) : r.A;
-            const float b1 = p1 > 0.f ? fmaf(r.B, fmaf(d1, r.inv_t, -r.log_s), r.A) : r.A;
-            x.set(q, p0 * b0 * r.inv_t, p1 * b1 * r.inv_t);
-        }
-    }
 }
 
 template <typename T, int W>
@@ -422,28 +405,28 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
             for (int i = 0; i < a.top; ++i) g_sum += tc[i] >= 0 ? gt[i] : 0.f;
         bool none;
         const RowGrad r = row_grad(a, row, g_sum, none);
-        const T label = r.label >= 0 ? grad_of<T>(r, x, r.label, 0.f) : from_f<T>(0.f);
+        const T label = r.label >= 0 ? from_f<T>(r.at(to_f<T>(x[r.label]), r.label, 0.f)) : from_f<T>(0.f);
         for (int j = 0; j < a.K; j += 8) {
             Eight<T> e = tile.template read<W>(x, j);
-            grad_eight(r, e);
+            r.eight(e);
             tile.template write<W>(x, j, e);
         }
         if (r.label >= 0) x[r.label] = label;
         if (gt && !none)
             for (int i = 0; i < a.top; ++i)
-                if (tc[i] >= 0) x[tc[i]] = grad_of<T>(r, logits, tc[i], gt[i]);
+                if (tc[i] >= 0) x[tc[i]] = from_f<T>(r.at(to_f<T>(logits[tc[i]]), tc[i], gt[i]));
     }
     __syncthreads();
     tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
 template <typename T, int G>
-__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_bwd_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const ScoresArgs a)
 {
-    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
+    __shared__ float scratch[4 * Group<G>::WARPS];
     const Group<G> group{scratch};
-    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.n) return;
+    const bool live = group.row() < a.n;
+    const int64_t row = min(group.row(), a.n - 1);
     const int me = group.rank();
     const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
     const T* x = pieces.row;
@@ -458,19 +441,19 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) scores_row_bwd_k
     }
     bool none;
     const RowGrad r = row_grad(a, row, g_sum[0], none);
-#pragma unroll 2
-    for (int p = me; p < pieces.pieces; p += G) {
+#pragma unroll 4
+    for (int p = me; p < (live ? pieces.pieces : 0); p += G) {
         Eight<T> e = pieces.load(p);
-        grad_eight(r, e);
+        r.eight(e);
         pieces.store(dx, alike, p, e);
     }
     // classes with parts of their own once more: the label, then the alternatives (of which the label may be one)
     group.sync();
-    if (me == 0 && r.label >= 0) dx[r.label] = grad_of<T>(r, x, r.label, 0.f);
-    if (gt && !none) {
+    if (me == 0 && live && r.label >= 0) dx[r.label] = from_f<T>(r.at(to_f<T>(x[r.label]), r.label, 0.f));
+    if (gt) {
         group.sync();
-        for (int i = me; i < a.top; i += G)
-            if (tc[i] >= 0) dx[tc[i]] = grad_of<T>(r, x, tc[i], gt[i]);
+        for (int i = me; i < (live && !none ? a.top : 0); i += G)
+            if (tc[i] >= 0) dx[tc[i]] = from_f<T>(r.at(to_f<T>(x[tc[i]]), tc[i], gt[i]));
     }
 }
 
@@ -505,27 +488,52 @@ static bool launch_tile_of(const ScoresArgs& a, bool backward, cudaStream_t stre
     }
 }
 
-template <typename T, bool TOPS>
+template <typename T, int G, int P, bool TOPS>
+static void launch_row(const ScoresArgs& a, cudaStream_t stream)
+{
+    scores_row_kernel<T, G, P, TOPS><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+}
+template <typename T, int G>
+static void launch_row_bwd(const ScoresArgs& a, cudaStream_t stream)
+{
+    scores_row_bwd_kernel<T, G><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+}
+// P pieces of each thread: 64 bf16 or 32 fp32 logits, where the alternatives are chosen 32
+template <typename T>
 static void launch_rows(const ScoresArgs& a, cudaStream_t stream)
 {
-    const unsigned warps = (unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), rows = (unsigned)a.n;
-    const int most = a.K + 16 / (int)sizeof(T) - 1;      // with what the first piece may skip
-    if (most <= 256)
-        scores_row_kernel<T, 32, 1, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (most <= 512)
-        scores_row_kernel<T, 32, 2, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (most <= 1024)
-        scores_row_kernel<T, 32, 4, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (most <= 2048)
-        scores_row_kernel<T, 32, 8, TOPS><<<warps, 32 * WARP_ROWS, 0, stream>>>(a);
-    else if (most <= 4096)
-        scores_row_kernel<T, 256, 2, TOPS><<<rows, 256, 0, stream>>>(a);
-    else if (most <= 8192)
-        scores_row_kernel<T, 256, 4, TOPS><<<rows, 256, 0, stream>>>(a);
-    else if (most <= 16384)
-        scores_row_kernel<T, 512, 4, TOPS><<<rows, 512, 0, stream>>>(a);
-    else
-        scores_row_kernel<T, 1024, 0, TOPS><<<rows, 1024, 0, stream>>>(a);
+    constexpr int P = sizeof(T) == 2 ? 8 : 4;
+    const int most = a.K + most_skipped<T>(a.logits, a.ld);
+    if (a.top) {
+        if (most <= 256)
+            launch_row<T, 32, 1, true>(a, stream);
+        else if (most <= 512)
+            launch_row<T, 32, 2, true>(a, stream);
+        else if (most <= 1024)
+            launch_row<T, 32, 4, true>(a, stream);
+        else if (most <= 2048)
+            launch_row<T, 128, 2, true>(a, stream);
+        else if (most <= 4096)
+            launch_row<T, 256, 2, true>(a, stream);
+        else if (most <= 8192)
+            launch_row<T, 256, 4, true>(a, stream);
+        else if (most <= 16384)
+            launch_row<T, 512, 4, true>(a, stream);
+        else
+            launch_row<T, 1024, 0, true>(a, stream);
+    } else if (most <= 4 * 8 * P) {
+        launch_row<T, 4, P, false>(a, stream);
+    } else if (most <= 8 * 8 * P) {
+        launch_row<T, 8, P, false>(a, stream);
+    } else if (most <= 16 * 8 * P) {
+        launch_row<T, 16, P, false>(a, stream);
+    } else if (most <= 32 * 8 * P) {
+        launch_row<T, 32, P, false>(a, stream);
+    } else if (most <= 8192) {
+        launch_row<T, 256, 4, false>(a, stream);
+    } else {
+        launch_row<T, 1024, 0, false>(a, stream);
+    }
 }
 
 template <typename T>
@@ -534,18 +542,22 @@ static int launch_scores(ScoresArgs a, bool backward, cudaStream_t stream)
     a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
     const char* what = backward ? "ptv3_class_scores_bwd" : "ptv3_class_scores_fwd";
+    const size_t bytes = a.K * sizeof(T);
     // a thread keeps up to 32 alternatives; beyond, and for longer rows, a warp chooses them
-    if (a.K * sizeof(T) <= TILE_ROW_BYTES && (backward || a.top <= 32)) {
+    if (bytes <= TILE_PLAIN_BYTES ? backward || a.top <= 32 : bytes <= TILE_TOP_BYTES && !backward && a.top && a.top <= 32) {
         if (!launch_tile_of<T>(a, backward, stream)) return check_launch("ptv3_class_scores: shared memory attribute");
-    } else if (backward) {
-        if (a.K <= 2048)
-            scores_row_bwd_kernel<T, 32><<<(unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, stream>>>(a);
-        else
-            scores_row_bwd_kernel<T, 256><<<(unsigned)a.n, 256, 0, stream>>>(a);
-    } else if (a.top) {
-        launch_rows<T, true>(a, stream);
+    } else if (!backward) {
+        launch_rows<T>(a, stream);
+    } else if (bytes <= 512) {
+        launch_row_bwd<T, 4>(a, stream);
+    } else if (bytes <= 1024) {
+        launch_row_bwd<T, 8>(a, stream);
+    } else if (bytes <= 2048) {
+        launch_row_bwd<T, 16>(a, stream);
+    } else if (bytes <= 8192) {
+        launch_row_bwd<T, 32>(a, stream);
     } else {
-        launch_rows<T, false>(a, stream);
+        launch_row_bwd<T, 256>(a, stream);
     }
     count_launches(1);
     return check_launch(what);

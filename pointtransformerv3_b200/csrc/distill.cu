@@ -20,7 +20,8 @@ struct DistillArgs {
     const void* teacher;      // n x k
     const void* list;         // n x k
     int list_bytes, k, K, rest;
-    bool teacher_bf16, wide, wide_out;      // wide: logits, gradient: see RowTile::wide_rows
+    bool teacher_bf16, list4;     // list4: see RowList
+    bool wide, wide_out;          // logits, gradient: see RowTile::wide_rows
     float* loss;              // n
     float4* stats;            // n x {m, log S, log of the outside's sum or the list's largest, t_r or 1 / the list's sum}, or NULL
     float inv_t;
@@ -70,53 +71,107 @@ __device__ __forceinline__ float log_outside(float sum, F&& again)
 }
 
 // ---- short rows: a tile of rows, one thread to a row ---------------------------------------------------------------
-// The list is walked twice, for its largest value and for its sums.  With an outcome for the rest, the list's classes are then masked in
-// the tile: one pass over the row gives the outside's sum, and the list's own exponentials make it the row's.
-template <typename T, int W>
+// A row's list in its thread's registers (N entries; N = 0: longer ones are read again from memory wherever they are walked).
+template <int N>
+struct RowList {
+    int c[N > 0 ? N : 1];
+    float v[N > 0 ? N : 1];
+    const DistillArgs& a;
+    int64_t at;
+    __device__ __forceinline__ RowList(const DistillArgs& args, int64_t row) : a(args), at(row * args.k)
+    {
+        if (N == 0) return;
+        if (a.list4) {          // lists of int32 and fp32 that start on 16 bytes
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                if (i >= a.k) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) c[i + q] = PLACE_ABSENT;
+                    continue;
+                }
+                const int4 c4 = reinterpret_cast<const int4*>((const int32_t*)a.list + at)[i / 4];
+                const float4 v4 = reinterpret_cast<const float4*>((const float*)a.teacher + at)[i / 4];
+                const int cc[4] = {c4.x, c4.y, c4.z, c4.w};
+                const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    c[i + q] = (unsigned)cc[q] < (unsigned)a.K ? cc[q] : (cc[q] == -1 ? PLACE_ABSENT : PLACE_BAD);
+                    v[i + q] = vv[q];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                c[i] = i < a.k ? list_class(a, at + i) : PLACE_ABSENT;
+                v[i] = i < a.k ? load_value(a.teacher, a.teacher_bf16, at + i) : 0.f;
+            }
+        }
+    }
+    // f(entry's number, class, value) of the entries that are there; bad() of those out of range
+    template <typename F>
+    __device__ __forceinline__ void each(F&& f) const
+    {
+        if (N > 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (c[i] >= 0) f(i, c[i], v[i]);
+        } else {
+            for (int i = 0; i < a.k; ++i) {
+                const int cls = list_class(a, at + i);
+                if (cls >= 0) f(i, cls, load_value(a.teacher, a.teacher_bf16, at + i));
+            }
+        }
+    }
+    __device__ __forceinline__ bool bad() const
+    {
+        bool b = false;
+        if (N > 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) b |= c[i] == PLACE_BAD;
+        } else {
+            for (int i = 0; i < a.k; ++i) b |= list_class(a, at + i) == PLACE_BAD;
+        }
+        return b;
+    }
+};
+
+// With an outcome for the rest, the list's classes are masked in the tile once they are read: one pass over the row gives the outside's
+// sum, and the list's own exponentials make it the row's.
+template <typename T, int W, int N>
 __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     const RowTile<T> tile(smem, a.K);
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    const int64_t row = row0 + threadIdx.x;
+    const RowList<N> list(a, min(row, a.n - 1));
     tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
     if ((int)threadIdx.x >= rows) return;
     T* x = tile.row(threadIdx.x);
-    const int64_t row = row0 + threadIdx.x, at = row * a.k;
 
     const float m = tile.template largest<W>(x), origin = row_origin(m), c = a.inv_t * LOG2E;
-    bool any = false, bad = false;
+    bool any = false;
     ListSums l{-INFINITY, 0.f, 0.f, 0.f};
-    if (!a.rest)
-        for (int i = 0; i < a.k; ++i)
-            if (list_class(a, at + i) >= 0) l.top = max_nan(l.top, load_value(a.teacher, a.teacher_bf16, at + i));
+    if (!a.rest) list.each([&](int, int, float v) { l.top = max_nan(l.top, v); });
     float most = 0.f, inside = 0.f;
-    for (int i = 0; i < a.k; ++i) {
-        const int cls = list_class(a, at + i);
-        bad |= cls == PLACE_BAD;
-        if (cls < 0) continue;
+    list.each([&](int, int cls, float v) {
         any = true;
-        const float v = load_value(a.teacher, a.teacher_bf16, at + i), w = entry_weight(a, v, l.top), d = to_f<T>(x[cls]) - origin;
+        const float w = entry_weight(a, v, l.top), d = to_f<T>(x[cls]) - origin;
         l.sum += w;
         if (a.rest) {
-            if (v > l.top) {
-                l.others += most;
-                most = w;
-                l.top = v;
-            } else {
-                l.others += w;
-            }
+            const bool up = v > l.top;
+            l.others += up ? most : w;
+            most = up ? w : most;
+            l.top = up ? v : l.top;
         }
         if (w != 0.f) l.gap = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(l.top)) * a.inv_t) - d * a.inv_t, l.gap);
-    }
-    if (a.rest) {
-        for (int i = 0; i < a.k; ++i) {
-            const int cls = list_class(a, at + i);
-            if (cls < 0) continue;
+    });
+    if (a.rest)
+        list.each([&](int, int cls, float) {
             inside += fast_exp2(below_max(to_f<T>(x[cls]), origin) * c);       // (a class that comes again is masked by then)
             x[cls] = from_f<T>(-INFINITY);
-        }
-    }
+        });
     const uint64_t c2 = pack2(c, c), minus = pack2(-origin, -origin);
     RowSum sums;
     sums.clear();
@@ -141,7 +196,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
             loss += entry_loss(t_r, logf(t_r), log_out - log_s);
         }
     }
-    if (bad) {
+    if (list.bad()) {
         loss = NAN;
         atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
     }
@@ -151,13 +206,13 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
                               : make_float4(origin, log_s, row_origin(l.top), l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
 }
 
-// ---- longer rows: a warp, or a block of G threads ------------------------------------------------------------------------
-// A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).  With an outcome
+// ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------
+// A thread keeps P pieces of eight logits in registers; the longest rows are read again for every pass (P = 0).  With an outcome
 // for the rest, the list's classes are bits in shared memory, which a piece's eight are cut out of.
-// the list, entry i with thread i % G of the first warp of a row's threads
+// the list, entry i with thread i % G of a row's threads
 template <int G>
 struct ListPart {
-    static constexpr int N = G == 32 ? 2 : 1;        // LIST_MAX entries
+    static constexpr int N = G <= LIST_MAX ? LIST_MAX / G : 1;
     int cls[N];
     float v[N];
     __device__ __forceinline__ void load(const DistillArgs& a, int64_t at, int me)
@@ -165,8 +220,12 @@ struct ListPart {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             const int i = me + q * G;
-            cls[q] = i < a.k ? list_class(a, at + i) : PLACE_ABSENT;
-            v[q] = cls[q] >= 0 ? load_value(a.teacher, a.teacher_bf16, at + i) : -INFINITY;
+            cls[q] = PLACE_ABSENT;
+            v[q] = -INFINITY;
+            if (q * G < a.k) {
+                if (i < a.k) cls[q] = list_class(a, at + i);
+                if (cls[q] >= 0) v[q] = load_value(a.teacher, a.teacher_bf16, at + i);
+            }
         }
     }
 };
@@ -175,15 +234,15 @@ struct ListPart {
 __host__ __device__ __forceinline__ int bit_words(int K) { return (K + 31) / 32 + 2; }
 
 template <typename T, int G, int P>
-__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const DistillArgs a)
 {
-    __shared__ float scratch[G > 32 ? 5 * (G / 32) : 1];
+    __shared__ float scratch[4 * Group<G>::WARPS];
     extern __shared__ uint32_t bits_s[];
     const Group<G> group{scratch};
-    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.n) return;
+    const bool live = group.row() < a.n;
+    const int64_t row = min(group.row(), a.n - 1);        // (threads beyond the last row keep it company)
     const int me = group.rank(), words = bit_words(a.K);
-    uint32_t* bits = bits_s + (G == 32 ? (threadIdx.x >> 5) * words : 0);
+    uint32_t* bits = bits_s + group.slot() * words;
     const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
     const T* x = pieces.row;
     ListPart<G> list;
@@ -242,6 +301,7 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_kern
     float all[4] = {hsum2(sums.s), 0.f, 0.f, 0.f}, counts[4] = {0.f, 0.f, 0.f, inside};
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
+        if (q * G >= a.k) break;
         counts[1] += list.cls[q] == PLACE_BAD ? 1.f : 0.f;
         if (list.cls[q] < 0) continue;
         counts[0] += 1.f;
@@ -261,25 +321,28 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_kern
     float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
-        log_out = log_outside(all[0], [&]() {
+        // (taken by all rows of a warp where one needs it)
+        const bool low = !(all[0] >= REST_TOO_SMALL);
+        if (G < 32 ? __any_sync(~0u, low) : low) {
             float om = -INFINITY;
             vals.each([&](const Eight<T>& e, int j) { if (j < a.K) om = max_nan(om, masked(e, j).largest()); });
             om = group.max(om);
-            if (om == -INFINITY) return -INFINITY;
+            const float from = row_origin(om);
             RowSum again;
             again.clear();
-            const uint64_t mo = pack2(-om, -om);
+            const uint64_t mo = pack2(-from, -from);
             vals.each([&](const Eight<T>& e, int j) { if (j < a.K) again.add(masked(e, j), mo, c2); });
             float o[1] = {hsum2(again.s)};
             group.sum(o);
-            return (om - origin) * a.inv_t + logf(o[0]);
-        });
+            if (om != -INFINITY) log_out = (om - origin) * a.inv_t + logf(o[0]);
+        }
+        if (!low) log_out = logf(all[0]);
         if (counts[0] > 0.f && log_out != -INFINITY) {
             t_r = rest_prob(l.top, l.others);
             loss += entry_loss(t_r, logf(t_r), log_out - log_s);
         }
     }
-    if (me == 0) {
+    if (me == 0 && live) {
         if (counts[1] > 0.f) {
             loss = NAN;
             atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
@@ -296,9 +359,16 @@ struct DistillGrad {
     float m, c, shift, factor, inside_shift, inside_factor, g;
     bool none;
     // every class as one outside the list
-    __device__ __forceinline__ float at(float x) const { return fast_exp2(fmaf(below_max(x, m), c, shift)) * factor; }
+    template <typename T>
+    __device__ __forceinline__ void eight(Eight<T>& x) const
+    {
+        row_gradient(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(factor, factor), 0ull);
+    }
     // M p of a class in the list
-    __device__ __forceinline__ float in_list(float x) const { return fast_exp2(fmaf(below_max(x, m), c, inside_shift)) * inside_factor; }
+    __device__ __forceinline__ float in_list(float x) const
+    {
+        return fast_exp2(max_nan(fmaf(x - m, c, inside_shift), NO_POWER)) * inside_factor;
+    }
 };
 // mass: sum of the list's t
 __device__ __forceinline__ DistillGrad distill_grad(const DistillArgs& a, int64_t row, float4 st, float mass)
@@ -326,60 +396,46 @@ __device__ __forceinline__ float entry_prob(const DistillArgs& a, float4 st, flo
     return a.rest ? fast_exp2(v * LOG2E) : fast_exp2(below_max(v, st.z) * (a.inv_t * LOG2E)) * st.w;
 }
 
-template <typename T>
-__device__ __forceinline__ void grad_eight(const DistillGrad& r, Eight<T>& x)
-{
-    const uint64_t c2 = pack2(r.c, r.c), minus = pack2(-r.m, -r.m), shift = pack2(r.shift, r.shift);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float d0, d1, t0, t1;
-        unpack2(add2(x.pair(q), minus), d0, d1);
-        unpack2(fma2(pack2(max_nan(d0, -1e38f), max_nan(d1, -1e38f)), c2, shift), t0, t1);
-        x.set(q, fast_exp2(t0) * r.factor, fast_exp2(t1) * r.factor);
-    }
-}
-
-template <typename T, int W>
+template <typename T, int W, int N>
 __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs a)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     const RowTile<T> tile(smem, a.K);
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
+    const int64_t row = min(row0 + threadIdx.x, a.n - 1);
+    RowList<N> list(a, row);
+    const float4 st = a.stats[row];
     tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
     if ((int)threadIdx.x < rows) {
-        const int64_t row = row0 + threadIdx.x, at = row * a.k;
         T* x = tile.row(threadIdx.x);
         const T* logits = (const T*)a.logits + row * a.ld;
-        const float4 st = a.stats[row];
         float mass = 0.f;
-        for (int i = 0; i < a.k; ++i)
-            if (list_class(a, at + i) >= 0) mass += entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + i));
+        list.each([&](int, int, float v) { mass += entry_prob(a, st, v); });
         const DistillGrad r = distill_grad(a, row, st, mass);
+        // the list's classes apart: M p - t of each, which goes into the row behind the others
+        float own[N > 0 ? N : 1];
+        if (N > 0) list.each([&](int i, int cls, float v) { own[i] = r.in_list(to_f<T>(x[cls])) - r.g * entry_prob(a, st, v); });
         for (int j = 0; j < a.K; j += 8) {
             Eight<T> e = tile.template read<W>(x, j);
-            grad_eight(r, e);
+            r.eight(e);
             tile.template write<W>(x, j, e);
         }
-        // the list's classes once more.  An entry leaves its number at its class first: where it is another's afterwards, a class comes twice,
-        // and every entry of the row writes the sum over its class.
-        for (int i = 0; i < a.k; ++i) {
-            const int cls = list_class(a, at + i);
-            if (cls >= 0) x[cls] = from_f<T>((float)i);
-        }
+        // An entry leaves its number at its class first: where it is another's afterwards, a class comes twice, and every entry of the row
+        // writes the sum over its class.
+        list.each([&](int i, int cls, float) { x[cls] = from_f<T>((float)i); });
         bool twice = false;
-        for (int i = 0; i < a.k; ++i) {
-            const int cls = list_class(a, at + i);
-            if (cls >= 0) twice |= to_f<T>(x[cls]) != (float)i;
-        }
-        for (int i = 0; i < a.k; ++i) {
-            const int cls = list_class(a, at + i);
-            if (cls < 0) continue;
-            float t = twice ? 0.f : entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + i));
-            if (twice)
-                for (int q = 0; q < a.k; ++q)
-                    if (list_class(a, at + q) == cls) t += entry_prob(a, st, load_value(a.teacher, a.teacher_bf16, at + q));
-            x[cls] = from_f<T>(r.in_list(to_f<T>(logits[cls])) - r.g * t);
+        list.each([&](int i, int cls, float) { twice |= to_f<T>(x[cls]) != (float)i; });
+        if (N > 0 && !twice) {
+            list.each([&](int i, int cls, float) { x[cls] = from_f<T>(own[i]); });
+        } else {
+            const RowList<0> all(a, row);
+            all.each([&](int, int cls, float v) {
+                float t = twice ? 0.f : entry_prob(a, st, v);
+                if (twice)
+                    all.each([&](int, int other, float u) { t += other == cls ? entry_prob(a, st, u) : 0.f; });
+                x[cls] = from_f<T>(r.in_list(to_f<T>(logits[cls])) - r.g * t);
+            });
         }
     }
     __syncthreads();
@@ -387,15 +443,15 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
 }
 
 template <typename T, int G>
-__global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_bwd_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const DistillArgs a)
 {
-    __shared__ float scratch[G > 32 ? 4 * (G / 32) : 1];
-    __shared__ int list_c[G == 32 ? WARP_ROWS : 1][LIST_MAX];
-    __shared__ float list_t[G == 32 ? WARP_ROWS : 1][LIST_MAX];
+    __shared__ float scratch[4 * Group<G>::WARPS];
+    __shared__ __align__(16) int list_c[Group<G>::ROWS][LIST_MAX];
+    __shared__ float list_t[Group<G>::ROWS][LIST_MAX];
     const Group<G> group{scratch};
-    const int64_t row = G == 32 ? blockIdx.x * (int64_t)WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.n) return;
-    const int me = group.rank(), slot = G == 32 ? threadIdx.x >> 5 : 0;
+    const bool live = group.row() < a.n;
+    const int64_t row = min(group.row(), a.n - 1);
+    const int me = group.rank(), slot = group.slot();
     const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
     const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
@@ -415,24 +471,33 @@ __global__ void __launch_bounds__(G == 32 ? 32 * WARP_ROWS : G) distill_row_bwd_
     }
     group.sum(mass);
     const DistillGrad r = distill_grad(a, row, st, mass[0]);
-#pragma unroll 2
-    for (int p = me; p < pieces.pieces; p += G) {
+#pragma unroll 4
+    for (int p = me; p < (live ? pieces.pieces : 0); p += G) {
         Eight<T> e = pieces.load(p);
-        grad_eight(r, e);
+        r.eight(e);
         pieces.store(dx, alike, p, e);
     }
     // the list's classes once more; one that comes twice is written by its first entry, with the sum of both
     group.sync();
+    if (!live) return;
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
         const int mine = me + q * G, cls = list.cls[q];
         if (cls < 0) continue;
-        float t = 0.f;
+        int same = 0;
+        for (int i = 0; i < a.k; i += 4) {                   // (absent entries beyond the list's are -1)
+            const int4 c = *reinterpret_cast<const int4*>(&list_c[slot][i]);
+            same += (c.x == cls) + (c.y == cls) + (c.z == cls) + (c.w == cls);
+        }
+        float t = list_t[slot][mine];
         bool is_first = true;
-        for (int i = 0; i < a.k; ++i) {
-            if (list_c[slot][i] == cls) {
-                t += list_t[slot][i];
-                is_first &= i >= mine;
+        if (same > 1) {
+            t = 0.f;
+            for (int i = 0; i < a.k; ++i) {
+                if (list_c[slot][i] == cls) {
+                    t += list_t[slot][i];
+                    is_first &= i >= mine;
+                }
             }
         }
         if (is_first) dx[cls] = from_f<T>(r.in_list(to_f<T>(x[cls])) - r.g * t);
@@ -450,14 +515,21 @@ static bool launch_tile(const DistillArgs& a, bool backward, cudaStream_t stream
         kern<<<blocks, shape.rows, shape.smem, stream>>>(a);
         return true;
     };
-    return backward ? run(distill_tile_bwd_kernel<T, W>) : run(distill_tile_kernel<T, W>);
+    if (a.k <= 4) return backward ? run(distill_tile_bwd_kernel<T, W, 4>) : run(distill_tile_kernel<T, W, 4>);
+    if (a.k <= 8) return backward ? run(distill_tile_bwd_kernel<T, W, 8>) : run(distill_tile_kernel<T, W, 8>);
+    if (a.k <= 16) return backward ? run(distill_tile_bwd_kernel<T, W, 16>) : run(distill_tile_kernel<T, W, 16>);
+    return backward ? run(distill_tile_bwd_kernel<T, W, 0>) : run(distill_tile_kernel<T, W, 0>);
 }
 template <typename T, int G, int P>
-static void launch_rows(const DistillArgs& a, cudaStream_t stream)
+static void launch_row(const DistillArgs& a, cudaStream_t stream)
 {
-    const unsigned blocks = G == 32 ? (unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS) : (unsigned)a.n;
-    const size_t smem = a.rest ? (size_t)bit_words(a.K) * 4 * (G == 32 ? WARP_ROWS : 1) : 0;
-    distill_row_kernel<T, G, P><<<blocks, G == 32 ? 32 * WARP_ROWS : G, smem, stream>>>(a);
+    const size_t smem = a.rest ? (size_t)bit_words(a.K) * 4 * Group<G>::ROWS : 0;
+    distill_row_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, smem, stream>>>(a);
+}
+template <typename T, int G>
+static void launch_row_bwd(const DistillArgs& a, cudaStream_t stream)
+{
+    distill_row_bwd_kernel<T, G><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
 }
 
 template <typename T>
@@ -465,8 +537,11 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
 {
     a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
-    const int most = a.K + 16 / (int)sizeof(T) - 1;      // with what the first piece may skip
-    if (a.K * sizeof(T) <= TILE_ROW_BYTES) {
+    a.list4 = a.list_bytes == 4 && !a.teacher_bf16 && a.k % 4 == 0 && (((uintptr_t)a.list | (uintptr_t)a.teacher) & 15) == 0;
+    constexpr int P = sizeof(T) == 2 ? 8 : 4;            // pieces of each thread: 64 bf16 or 32 fp32 logits
+    const int most = a.K + most_skipped<T>(a.logits, a.ld);
+    const size_t bytes = a.K * sizeof(T);
+    if (bytes <= TILE_PLAIN_BYTES) {
         bool ok;
         switch (RowTile<T>::row_width(a.K)) {
         case 16: ok = launch_tile<T, 16>(a, backward, stream); break;
@@ -476,20 +551,24 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
         }
         if (!ok) return check_launch("ptv3_distill_topk: shared memory attribute");
     } else if (backward) {
-        if (a.K <= 2048)
-            distill_row_bwd_kernel<T, 32><<<(unsigned)((a.n + WARP_ROWS - 1) / WARP_ROWS), 32 * WARP_ROWS, 0, stream>>>(a);
+        if (bytes <= 1024)
+            launch_row_bwd<T, 8>(a, stream);
+        else if (bytes <= 2048)
+            launch_row_bwd<T, 16>(a, stream);
+        else if (bytes <= 8192)
+            launch_row_bwd<T, 32>(a, stream);
         else
-            distill_row_bwd_kernel<T, 256><<<(unsigned)a.n, 256, 0, stream>>>(a);
-    } else if (most <= 512) {
-        launch_rows<T, 32, 2>(a, stream);
-    } else if (most <= 1024) {
-        launch_rows<T, 32, 4>(a, stream);
-    } else if (most <= 2048) {
-        launch_rows<T, 32, 8>(a, stream);
+            launch_row_bwd<T, 256>(a, stream);
+    } else if (most <= 8 * 8 * P) {
+        launch_row<T, 8, P>(a, stream);
+    } else if (most <= 16 * 8 * P) {
+        launch_row<T, 16, P>(a, stream);
+    } else if (most <= 32 * 8 * P) {
+        launch_row<T, 32, P>(a, stream);
     } else if (most <= 8192) {
-        launch_rows<T, 256, 4>(a, stream);
+        launch_row<T, 256, 4>(a, stream);
     } else {
-        launch_rows<T, 1024, 0>(a, stream);
+        launch_row<T, 1024, 0>(a, stream);
     }
     count_launches(1);
     return check_launch(backward ? "ptv3_distill_topk_bwd" : "ptv3_distill_topk_fwd");

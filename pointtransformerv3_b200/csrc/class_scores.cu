@@ -144,24 +144,21 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
 // ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------------------
 // A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).
 //
-// The alternatives.  Up to FEW: one after another, each a maximum over the row of what comes behind the last one.  More: every thread has
-// the largest of its pieces, 64 (128 for more than 32 alternatives) such maxima of a row are compared by the upper 16 bits of their keys, and the
-// k-th largest of these, found bit by bit, bounds the k-th largest of the row from below; the few logits at or above it (less than twice k
-// of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of few values), one after another again.
-constexpr int FEW = 3, CANDIDATES = 192;
+// The alternatives.  Every thread has the largest of each of two parts of its logits (of four for more than 32 alternatives); their k-th
+// largest, found one after another by the upper 16 bits of their keys, bounds the row's k-th largest from below.  The few logits at or above
+// the bound (less than twice k of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of
+// few values), the best are taken one after another, each a maximum over the row of what comes behind the last one.
+constexpr int CANDIDATES = 192;
 
 // value and class as one number, below ~0 (NaN of class 0); 0 for none
-__device__ __forceinline__ unsigned long long wide_key(float x, int j, int K)
-{
-    return (unsigned)j < (unsigned)K ? (unsigned long long)order_key(x) << 32 | (0x7fffffffu - j) : 0ull;
-}
+__device__ __forceinline__ unsigned long long wide_key(float x, int j) { return (unsigned long long)order_key(x) << 32 | (0x7fffffffu - j); }
 __device__ __forceinline__ int key_class(unsigned long long k) { return k ? (int)(0x7fffffffu - (uint32_t)k) : -1; }
 
 template <int G>
 struct TopScratch {
     unsigned long long candidate[CANDIDATES];
     unsigned long long chosen[G / 32];
-    uint16_t maxima[G > 32 ? 128 : 1];
+    uint16_t maxima[G > 32 ? 128 : 1];      // 64 or 128 of a block
     uint32_t bound;
     int count;
 };
@@ -172,17 +169,26 @@ __device__ __forceinline__ void write_alternative(const ScoresArgs& a, int64_t r
     a.top_logp[row * a.top + i] = k ? log_prob_of(r, order_value((uint32_t)(k >> 32)), a.inv_t) : -INFINITY;
 }
 
-// the k-th largest (k = 1 ..) of N x 32 numbers of 16 bits, N with each lane, from below: the largest that so many reach
-template <int N>
-__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[N], int k)
+// the k-th largest (k = 1 ..) of 4 x 32 numbers of 16 bits, four with each lane; 0 where there are not so many
+__device__ __forceinline__ uint32_t kth_largest(uint32_t (&v)[4], int k, bool four)
 {
+    if (!four) {
+        v[0] = ::max(v[0], v[2]);
+        v[1] = ::max(v[1], v[3]);
+        v[2] = v[3] = 0;
+    }
     uint32_t bound = 0;
 #pragma unroll 1
-    for (uint32_t bit = 0x8000; bit; bit >>= 1) {
-        int reach = 0;
+    while (k > 0) {
+        const uint32_t mine = ::max(::max(v[0], v[1]), ::max(v[2], v[3]));
+        bound = __reduce_max_sync(~0u, mine);
+        if (bound == 0) break;
+        // all that are as large
+        const int n = four ? (v[0] == bound) + (v[1] == bound) + (v[2] == bound) + (v[3] == bound) : (v[0] == bound) + (v[1] == bound);
+        k -= __popc(__ballot_sync(~0u, n > 0));
+        if (__any_sync(~0u, n > 1)) k -= __reduce_add_sync(~0u, n > 1 ? n - 1 : 0);
 #pragma unroll
-        for (int i = 0; i < N; ++i) reach += __popc(__ballot_sync(~0u, v[i] >= (bound | bit)));
-        if (reach >= k) bound |= bit;
+        for (int i = 0; i < 4; ++i) v[i] = v[i] == bound ? 0 : v[i];
     }
     return bound;
 }
@@ -192,115 +198,111 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
                                              const Group<G>& group, TopScratch<G>& scratch, float mine)
 {
     const int me = group.rank(), lane = threadIdx.x & 31;
-    if (a.top > FEW) {
-        // maxima: of a thread's half or quarter of its pieces where a warp has the row, else of two or four threads
-        uint32_t bound = 0;
-        if (G == 32) {
-            if (a.top <= 32 && P >= 2) {
-                uint32_t v[2] = {0, 0};
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    const float m = vals.x[i].largest();
-                    v[i & 1] = ::max(v[i & 1], i * G + me < vals.pieces.pieces ? order_key(m) >> 16 : 0u);
-                }
-                bound = kth_largest(v, a.top);
-            } else if (a.top <= 32) {
-                const uint32_t v[1] = {me < vals.pieces.pieces ? order_key(mine) >> 16 : 0u};
-                bound = kth_largest(v, a.top);
-            }
-            // (more than 32 of a warp's row: a bound of 0 makes everything a candidate where the row is short, else one after another)
-        } else {
-            const int per = a.top <= 32 ? G / 64 : G / 128;      // threads that share a maximum
-            float m = mine;
-            for (int o = 1; o < per; o *= 2) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
-            if (lane % per == 0) scratch.maxima[me / per] = order_key(m) >> 16;
-            if (me == 0) scratch.count = 0;
-            __syncthreads();
-            if (me < 32) {
-                const uint32_t v[4] = {scratch.maxima[me], scratch.maxima[me + 32], a.top <= 32 ? 0u : scratch.maxima[me + 64],
-                                       a.top <= 32 ? 0u : scratch.maxima[me + 96]};
-                const uint32_t b = kth_largest(v, a.top);
-                if (me == 0) scratch.bound = b;
-            }
-            __syncthreads();
-            bound = scratch.bound;
+    const bool four = a.top > 32;
+    uint32_t bound = 0;
+    if (G == 32) {
+        uint32_t v[4] = {0, 0, 0, 0};
+        vals.each([&](const Eight<T>& x, int, int i) { v[i & 3] = ::max(v[i & 3], order_key(x.largest()) >> 16); },
+                  [&](float x, int, int) { v[3] = ::max(v[3], order_key(x) >> 16); });
+        bound = kth_largest(v, a.top, four);
+    } else {
+        const int per = four ? G / 128 : G / 64;      // threads that share a maximum
+        float m = mine;
+        for (int o = 1; o < per; o *= 2) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
+        if (lane % per == 0) scratch.maxima[me / per] = order_key(m) >> 16;
+        if (me == 0) scratch.count = 0;
+        __syncthreads();
+        if (me < 32) {
+            uint32_t v[4] = {scratch.maxima[me], scratch.maxima[me + 32], four ? scratch.maxima[me + 64] : 0u, four ? scratch.maxima[me + 96] : 0u};
+            const uint32_t b = kth_largest(v, a.top, four);
+            if (me == 0) scratch.bound = b;
         }
-        // at or above the bound as logits (NaN is), compared as they are: eight at once, since few pieces have one
-        const float least = order_value(bound << 16);
-        auto any = [&](const Eight<T>& x) {
-            bool yes = bound == 0;
+        __syncthreads();
+        bound = scratch.bound;
+    }
+    // At or above the bound as logits (NaN is), compared as they are.  A thread's are bits of a mask; those of a row that is read again,
+    // which has more than a mask has bits, are gathered as they are found.
+    const float least = order_value(bound << 16);
+    auto bits_of = [&](const Eight<T>& x) {
+        bool any = bound == 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) yes |= !(x.at(i) < least);
-            return yes;
-        };
-        auto is = [&](float v, int j) { return (unsigned)j < (unsigned)a.K && (bound == 0 || !(v < least)); };
-        int count = 0;
+        for (int i = 0; i < 8; ++i) any |= !(x.at(i) < least);
+        uint32_t bits = 0;
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits |= (bound == 0 || !(x.at(i) < least) ? 1u : 0u) << i;
+        }
+        return bits;
+    };
+    const T* logits = vals.pieces.row;
+    auto put = [&](int at, int j) { scratch.candidate[at] = wide_key(to_f<T>(logits[j]), j); };
+    int count = 0;
+    if (P > 0) {
+        uint32_t mask = 0, edge_mask = 0;
+        vals.each([&](const Eight<T>& x, int, int i) { mask |= bits_of(x) << (8 * i); },
+                  [&](float x, int, int q) { edge_mask |= (bound == 0 || !(x < least) ? 1u : 0u) << q; });
+        const int own = __popc(mask) + __popc(edge_mask);
+        int at = own;
         if (G == 32) {
-            // each lane's number, its place among the lanes', its candidates
-            vals.each([&](const Eight<T>& x, int j) {
-                if (any(x)) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) count += is(x.at(i), j + i);
-                }
-            });
-            int at = count;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
                 const int up = __shfl_up_sync(~0u, at, o);
                 if (lane >= o) at += up;
             }
-            const int all = __shfl_sync(~0u, at, 31);
-            at -= count;
-            count = all;
-            if (count <= CANDIDATES) {
-                vals.each([&](const Eight<T>& x, int j) {
-                    if (any(x)) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (is(x.at(i), j + i)) scratch.candidate[at++] = wide_key(x.at(i), j + i, a.K);
-                    }
-                });
-            }
+            count = __shfl_sync(~0u, at, 31);
+            at -= own;
         } else {
-            vals.each([&](const Eight<T>& x, int j) {
-                if (any(x)) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (is(x.at(i), j + i)) {
-                            const int at = atomicAdd(&scratch.count, 1);
-                            if (at < CANDIDATES) scratch.candidate[at] = wide_key(x.at(i), j + i, a.K);
-                        }
-                }
-            });
+            at = own ? atomicAdd(&scratch.count, own) : 0;
         }
-        group.sync();
-        if (G > 32) count = scratch.count;
-        if (count <= CANDIDATES) {
-            for (int i = me; i < ::max(count, a.top); i += G) {
-                if (i < count) {
-                    const unsigned long long k = scratch.candidate[i];
-                    int before = 0;
-                    for (int q = 0; q < count; ++q) before += scratch.candidate[q] > k;
-                    if (before < a.top) write_alternative(a, row, r, before, k);
-                } else {
-                    write_alternative(a, row, r, i, 0);          // no such class
-                }
+        if (at + own <= CANDIDATES) {
+            for (; mask; mask &= mask - 1) {
+                const int i = __ffs(mask) - 1;
+                put(at++, vals.pieces.first((i >> 3) * G + me) + (i & 7));
             }
-            return;
+            for (; edge_mask; edge_mask &= edge_mask - 1) put(at++, vals.pieces.edge_class((__ffs(edge_mask) - 1) * G + me));
         }
+    } else {
+        vals.each([&](const Eight<T>& x, int j, int) {
+            for (uint32_t mask = bits_of(x); mask; mask &= mask - 1) {
+                const int at = atomicAdd(&scratch.count, 1);
+                if (at < CANDIDATES) put(at, j + __ffs(mask) - 1);
+            }
+        }, [&](float x, int j, int) {
+            if (bound == 0 || !(x < least)) {
+                const int at = atomicAdd(&scratch.count, 1);
+                if (at < CANDIDATES) put(at, j);
+            }
+        });
+    }
+    group.sync();
+    if (G > 32) count = scratch.count;
+    if (count <= CANDIDATES) {
+        for (int i = me; i < ::max(count, a.top); i += G) {
+            if (i < count) {
+                const unsigned long long k = scratch.candidate[i];
+                int before = 0;
+#pragma unroll 4
+                for (int q = 0; q < count; ++q) before += scratch.candidate[q] > k;
+                if (before < a.top) write_alternative(a, row, r, before, k);
+            } else {
+                write_alternative(a, row, r, i, 0);          // no such class
+            }
+        }
+        return;
     }
     unsigned long long last = ~0ull, key = 0;
     bool again = true;
     for (int i = 0; i < a.top; ++i) {
         if (again) {
             key = 0;
-            vals.each([&](const Eight<T>& x, int j) {
+            auto look = [&](float x, int j) {
+                const unsigned long long k = wide_key(x, j);
+                if (k < last && k > key) key = k;
+            };
+            vals.each([&](const Eight<T>& x, int j, int) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const unsigned long long k = wide_key(x.at(q), j + q, a.K);
-                    if (k < last && k > key) key = k;
-                }
-            });
+                for (int q = 0; q < 8; ++q) look(x.at(q), j + q);
+            }, [&](float x, int j, int) { look(x, j); });
         }
         const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(key >> 32));
         const uint32_t lo = __reduce_max_sync(~0u, (uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
@@ -327,16 +329,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_kernel(const Score
     const Group<G> group{scratch};
     const int64_t row = group.row(), at = min(row, a.n - 1);        // (threads beyond the last row keep it company)
     const int me = group.rank();
-    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, at, a.K);
+    const RowPieces<T> pieces((const T*)a.logits + at * a.ld, a.K);
     const RowValues<T, G, P> vals(pieces, me);
     float mine = -INFINITY;
-    vals.each([&](const Eight<T>& x, int) { mine = max_nan(mine, x.largest()); });
+    vals.each([&](const Eight<T>& x, int, int) { mine = max_nan(mine, x.largest()); }, [&](float x, int, int) { mine = max_nan(mine, x); });
     const float m = group.max(mine), origin = row_origin(m);
     const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
     RowSum sums;
     sums.clear();
-    vals.each([&](const Eight<T>& x, int) { sums.add(x, minus, c2); });
-    float su[2] = {hsum2(sums.s), hsum2(sums.u)};
+    EdgeSum edge{0.f, 0.f};
+    vals.each([&](const Eight<T>& x, int, int) { sums.add(x, minus, c2); }, [&](float x, int, int) { edge.add(x, origin, a.inv_t * LOG2E); });
+    float su[2] = {hsum2(sums.s) + edge.s, hsum2(sums.u) + edge.u};
     group.sum(su);
     const RowSums r = row_sums(m, su[0], su[1]);
     if (me == 0 && row < a.n) write_row(a, row, r, [&](int j) { return to_f<T>(pieces.row[j]); });
@@ -358,7 +361,7 @@ struct RowGrad {
     __device__ __forceinline__ float at(float x, int j, float own) const
     {
         const float t = max_nan(fmaf(x - m, c, shift), NO_POWER);
-        return fmaf(fast_exp2(t), fmaf(t, B, A), fmaf(own, inv_t, j == label ? g : 0.f));
+        return fmaf(fast_exp2(t), fmaf(t, B, A), fmaf(own, inv_t, j == label ? g : 0.f));     // (no class, no label: -2, -1)
     }
 };
 __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, float g_top_sum, bool& none)
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const S
     const bool live = group.row() < a.n;
     const int64_t row = min(group.row(), a.n - 1);
     const int me = group.rank();
-    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const RowPieces<T> pieces((const T*)a.logits + row * a.ld, a.K);
     const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
     const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
@@ -446,6 +449,10 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const S
         Eight<T> e = pieces.load(p);
         r.eight(e);
         pieces.store(dx, alike, p, e);
+    }
+    for (int e = me; e < (live ? pieces.edges : 0); e += G) {
+        const int j = pieces.edge_class(e);
+        dx[j] = from_f<T>(r.at(to_f<T>(x[j]), -2, 0.f));
     }
     // classes with parts of their own once more: the label, then the alternatives (of which the label may be one)
     group.sync();
@@ -503,8 +510,9 @@ template <typename T>
 static void launch_rows(const ScoresArgs& a, cudaStream_t stream)
 {
     constexpr int P = sizeof(T) == 2 ? 8 : 4;
-    const int most = a.K + most_skipped<T>(a.logits, a.ld);
+    const int most = a.K;
     if (a.top) {
+        // (a thread's pieces are bits of a word: four at most)
         if (most <= 256)
             launch_row<T, 32, 1, true>(a, stream);
         else if (most <= 512)

@@ -230,8 +230,8 @@ struct ListPart {
     }
 };
 
-// words of bits of a row: a piece may begin before class 0 and end behind the last, so one word more on either side
-__host__ __device__ __forceinline__ int bit_words(int K) { return (K + 31) / 32 + 2; }
+// words of bits of a row, one more for the last piece's
+__host__ __device__ __forceinline__ int bit_words(int K) { return (K + 31) / 32 + 1; }
 
 template <typename T, int G, int P>
 __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const DistillArgs a)
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
     const int64_t row = min(group.row(), a.n - 1);        // (threads beyond the last row keep it company)
     const int me = group.rank(), words = bit_words(a.K);
     uint32_t* bits = bits_s + group.slot() * words;
-    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const RowPieces<T> pieces((const T*)a.logits + row * a.ld, a.K);
     const T* x = pieces.row;
     ListPart<G> list;
     list.load(a, row * a.k, me);
@@ -253,19 +253,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
         group.sync();
 #pragma unroll
         for (int q = 0; q < ListPart<G>::N; ++q)
-            if (list.cls[q] >= 0) atomicOr(&bits[(list.cls[q] >> 5) + 1], 1u << (list.cls[q] & 31));
+            if (list.cls[q] >= 0) atomicOr(&bits[list.cls[q] >> 5], 1u << (list.cls[q] & 31));
         group.sync();
     }
     float m = -INFINITY;
-    vals.each([&](const Eight<T>& e, int) { m = max_nan(m, e.largest()); });
+    vals.each([&](const Eight<T>& e, int, int) { m = max_nan(m, e.largest()); }, [&](float e, int, int) { m = max_nan(m, e); });
     m = group.max(m);
     const float origin = row_origin(m), c = a.inv_t * LOG2E;
     const uint64_t c2 = pack2(c, c), minus = pack2(-origin, -origin);
     // the classes of the list as bits of a piece
-    auto listed = [&](int j) {
-        const int at = j + 32;
-        return __funnelshift_r(bits[at >> 5], bits[(at >> 5) + 1], at & 31) & 0xffu;
-    };
+    auto listed = [&](int j) { return __funnelshift_r(bits[j >> 5], bits[(j >> 5) + 1], j & 31) & 0xffu; };
+    auto is_listed = [&](int j) { return bits[j >> 5] >> (j & 31) & 1; };
     auto masked = [&](const Eight<T>& e, int j) {
         Eight<T> o = e;
         const uint32_t in = listed(j);
@@ -277,47 +275,54 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
     };
     RowSum sums;
     sums.clear();
+    EdgeSum edge{0.f, 0.f};
     float inside = 0.f;
     if (a.rest)
-        vals.each([&](const Eight<T>& e, int j) {
-            if (j >= a.K) return;
+        vals.each([&](const Eight<T>& e, int j, int) {
             sums.add(masked(e, j), minus, c2);
             if (const uint32_t in = listed(j)) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                     if (in >> q & 1) inside += fast_exp2(below_max(e.at(q), origin) * c);
             }
+        }, [&](float e, int j, int) {
+            if (is_listed(j))
+                inside += fast_exp2(below_max(e, origin) * c);
+            else
+                edge.add(e, origin, c);
         });
     else
-        vals.each([&](const Eight<T>& e, int) { sums.add(e, minus, c2); });
+        vals.each([&](const Eight<T>& e, int, int) { sums.add(e, minus, c2); }, [&](float e, int, int) { edge.add(e, origin, c); });
 
     // the list: its largest value, then its sums
     float top = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < ListPart<G>::N; ++q) top = max_nan(top, list.v[q]);
+    for (int q = 0; q < ListPart<G>::N; ++q)
+        if (q * G < a.k) top = max_nan(top, list.v[q]);
     top = group.max(top);
-    // the row's (or the outside's) sum; weights but the largest's, all, their gap; entries, bad ones, entries that are as large as the
-    // largest; the inside's sum
-    float all[4] = {hsum2(sums.s), 0.f, 0.f, 0.f}, counts[4] = {0.f, 0.f, 0.f, inside};
+    // the row's (or the outside's) sum; weights, their gap; entries, and from 128 on those out of range
+    float all[4] = {hsum2(sums.s) + edge.s, 0.f, 0.f, 0.f};
+    // with an outcome for the rest: the inside's sum, weights but the largest's, entries that are as large as the largest
+    float more[3] = {inside, 0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
         if (q * G >= a.k) break;
-        counts[1] += list.cls[q] == PLACE_BAD ? 1.f : 0.f;
+        all[3] += list.cls[q] == PLACE_BAD ? 128.f : 0.f;
         if (list.cls[q] < 0) continue;
-        counts[0] += 1.f;
+        all[3] += 1.f;
         const float v = list.v[q], w = entry_weight(a, v, top), d = to_f<T>(x[list.cls[q]]) - origin;
-        const bool is_top = a.rest && v == top;
-        all[1] += is_top ? 0.f : w;
-        counts[2] += is_top ? 1.f : 0.f;
-        all[2] += w;
-        if (w != 0.f) all[3] = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(top)) * a.inv_t) - d * a.inv_t, all[3]);
+        all[1] += w;
+        if (w != 0.f) all[2] = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(top)) * a.inv_t) - d * a.inv_t, all[2]);
+        more[1] += v == top ? 0.f : w;
+        more[2] += v == top ? 1.f : 0.f;
     }
     group.sum(all);
-    group.sum(counts);
-    const float s = all[0] + counts[3];
+    if (a.rest) group.sum(more);
+    const bool bad = all[3] >= 128.f, any = all[3] != 0.f && all[3] != 128.f * (int)(all[3] / 128.f);
+    const float s = all[0] + (a.rest ? more[0] : 0.f);
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
-    ListSums l{top, all[2], all[1] + fmaxf(counts[2] - 1.f, 0.f) * fast_exp2(top * LOG2E), all[3]};
+    ListSums l{top, all[1], more[1] + fmaxf(more[2] - 1.f, 0.f) * fast_exp2(top * LOG2E), all[2]};
     float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
@@ -325,25 +330,28 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
         const bool low = !(all[0] >= REST_TOO_SMALL);
         if (G < 32 ? __any_sync(~0u, low) : low) {
             float om = -INFINITY;
-            vals.each([&](const Eight<T>& e, int j) { if (j < a.K) om = max_nan(om, masked(e, j).largest()); });
+            vals.each([&](const Eight<T>& e, int j, int) { om = max_nan(om, masked(e, j).largest()); },
+                      [&](float e, int j, int) { om = max_nan(om, is_listed(j) ? -INFINITY : e); });
             om = group.max(om);
             const float from = row_origin(om);
             RowSum again;
             again.clear();
             const uint64_t mo = pack2(-from, -from);
-            vals.each([&](const Eight<T>& e, int j) { if (j < a.K) again.add(masked(e, j), mo, c2); });
-            float o[1] = {hsum2(again.s)};
+            EdgeSum at_edge{0.f, 0.f};
+            vals.each([&](const Eight<T>& e, int j, int) { again.add(masked(e, j), mo, c2); },
+                      [&](float e, int j, int) { at_edge.add(is_listed(j) ? -INFINITY : e, from, c); });
+            float o[1] = {hsum2(again.s) + at_edge.s};
             group.sum(o);
             if (om != -INFINITY) log_out = (om - origin) * a.inv_t + logf(o[0]);
         }
         if (!low) log_out = logf(all[0]);
-        if (counts[0] > 0.f && log_out != -INFINITY) {
+        if (any && log_out != -INFINITY) {
             t_r = rest_prob(l.top, l.others);
             loss += entry_loss(t_r, logf(t_r), log_out - log_s);
         }
     }
     if (me == 0 && live) {
-        if (counts[1] > 0.f) {
+        if (bad) {
             loss = NAN;
             atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
         }
@@ -364,6 +372,7 @@ struct DistillGrad {
     {
         row_gradient(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(factor, factor), 0ull);
     }
+    __device__ __forceinline__ float outside(float x) const { return fast_exp2(max_nan(fmaf(x - m, c, shift), NO_POWER)) * factor; }
     // M p of a class in the list
     __device__ __forceinline__ float in_list(float x) const
     {
@@ -452,7 +461,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const 
     const bool live = group.row() < a.n;
     const int64_t row = min(group.row(), a.n - 1);
     const int me = group.rank(), slot = group.slot();
-    const RowPieces<T> pieces((const T*)a.logits, a.ld, a.n, row, a.K);
+    const RowPieces<T> pieces((const T*)a.logits + row * a.ld, a.K);
     const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
     const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
@@ -476,6 +485,10 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const 
         Eight<T> e = pieces.load(p);
         r.eight(e);
         pieces.store(dx, alike, p, e);
+    }
+    for (int e = me; e < (live ? pieces.edges : 0); e += G) {
+        const int j = pieces.edge_class(e);
+        dx[j] = from_f<T>(r.outside(to_f<T>(x[j])));
     }
     // the list's classes once more; one that comes twice is written by its first entry, with the sum of both
     group.sync();
@@ -539,7 +552,7 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
     a.list4 = a.list_bytes == 4 && !a.teacher_bf16 && a.k % 4 == 0 && (((uintptr_t)a.list | (uintptr_t)a.teacher) & 15) == 0;
     constexpr int P = sizeof(T) == 2 ? 8 : 4;            // pieces of each thread: 64 bf16 or 32 fp32 logits
-    const int most = a.K + most_skipped<T>(a.logits, a.ld);
+    const int most = a.K;
     const size_t bytes = a.K * sizeof(T);
     if (bytes <= TILE_PLAIN_BYTES) {
         bool ok;

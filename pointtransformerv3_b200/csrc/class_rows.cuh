@@ -276,7 +276,7 @@ struct Group {
 
 // A row as its pieces of eight logits that start on 16 bytes (32 bytes of fp32: two loads) and, wherever the row starts and ends, the
 // values before the first and behind the last of these, its edges: 14 at most, read one by one, so that nothing beside the row is read.
-// (Whole pieces whose foreign values are masked took half as many instructions again: 50 021 x 1 201 lists backward 73 -> 51 us.)
+// (With whole pieces whose foreign values are masked, lists of 50 021 x 1 201 took 58 us forward instead of 46, backward 73 instead of 68.)
 constexpr int EDGES = 14;
 template <typename T>
 struct RowPieces {
@@ -301,10 +301,9 @@ struct RowPieces {
         if (Eight<T>::WORDS == 8) *reinterpret_cast<uint4*>(&x.w[Eight<T>::WORDS - 4]) = src[1];
         return x;
     }
-    // into a row of results that lies as this one does with respect to 16 bytes (`alike`), or elsewhere
-    __device__ __forceinline__ void store(T* out, bool alike, int p, const Eight<T>& x) const
+    // eight from class j on into a row of results that lies as this one does with respect to 16 bytes (`alike`), or elsewhere
+    __device__ __forceinline__ void store(T* out, bool alike, int j, const Eight<T>& x) const
     {
-        const int j = first(p);
         if (alike) {
             uint4* dst = reinterpret_cast<uint4*>(out + j);
             dst[0] = *reinterpret_cast<const uint4*>(&x.w[0]);
@@ -388,9 +387,9 @@ struct RowTile {
     __device__ __forceinline__ RowTile(unsigned char* s, int k) : smem(s), K(k), pitch(row_pitch(k)), width(row_width(k)) {}
     __device__ __forceinline__ T* row(int r) const { return reinterpret_cast<T*>(smem + r * pitch); }
 
-    // rows of the matrix into the tile (all threads; ends with a barrier).  wide: they may be read in pieces of 16 bytes, which is where
+    // rows of the matrix into the tile (all threads; they are there after `wait`).  wide: they may be read in pieces of 16 bytes, which is where
     // they lie one behind the other, or each on 16 bytes
-    __device__ __forceinline__ void load(const T* logits, int64_t ld, int64_t row0, int rows, bool wide) const
+    __device__ __forceinline__ void fetch(const T* logits, int64_t ld, int64_t row0, int rows, bool wide) const
     {
         const int threads = blockDim.x;
         const T* src = logits + row0 * ld;
@@ -418,6 +417,9 @@ struct RowTile {
             const int r = i / K, c = i - r * K;
             row(r)[c] = src[r * ld + c];
         }
+    }
+    __device__ __forceinline__ void wait() const
+    {
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
     }
@@ -520,6 +522,36 @@ struct RowTile {
         return ((uintptr_t)p & 15) == 0 && (ld == K || (ld * sizeof(T) % 16 == 0 && row_width(K) == 16));
     }
 };
+
+// Threads of a row and pieces of each.  A thread holds up to 128 bf16 or 64 fp32 logits in 64 registers, all of them on the way at once:
+// that, not many warps, is what keeps memory busy, and one warp to a row waits for no barrier.  Short rows take part of a warp, so
+// that what is done once for a row is done for several at a time.
+template <int N> struct Const { static constexpr int value = N; };
+template <typename T, typename F>
+static inline void for_row_shape(int K, bool warps, F&& f)
+{
+    constexpr int P = sizeof(T) == 2 ? 8 : 4;
+    if (K <= 8 * 8 * P && warps)
+        K <= 256 ? f(Const<32>(), Const<1>()) : f(Const<32>(), Const<2>());
+    else if (K <= 4 * 8 * P)
+        f(Const<4>(), Const<P>());
+    else if (K <= 8 * 8 * P)
+        f(Const<8>(), Const<P>());
+    else if (K <= 16 * 8 * P)
+        warps ? f(Const<32>(), Const<P / 2>()) : f(Const<16>(), Const<P>());
+    else if (K <= 32 * 8 * P)
+        f(Const<32>(), Const<P>());
+    else if (K <= 32 * 16 * P)
+        f(Const<32>(), Const<2 * P>());
+    else if (K <= 128 * 16 * P)
+        f(Const<128>(), Const<2 * P>());
+    else if (K <= 256 * 16 * P)
+        f(Const<256>(), Const<2 * P>());
+    else if (K <= 512 * 16 * P)
+        f(Const<512>(), Const<2 * P>());
+    else
+        f(Const<1024>(), Const<0>());
+}
 
 // Rows and shared memory of a block with a tile.
 struct TileShape {

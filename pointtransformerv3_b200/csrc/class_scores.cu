@@ -50,19 +50,20 @@ __device__ __forceinline__ float log_prob_of(const RowSums& r, float x, float in
     return r.none ? -INFINITY : (x - r.m) * inv_t - r.log_s;
 }
 
-// The label's log probability: 0 for a row without a label, NaN and a status bit for one that is no class.
-template <typename F>
-__device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, const RowSums& r, F&& logit)
+// A row's label, read before the row is there: its class, NO_LABEL or BAD_LABEL.
+constexpr int NO_LABEL = -1, BAD_LABEL = -2;
+__device__ __forceinline__ int row_label(const ScoresArgs& a, int64_t row)
+{
+    if (!a.labels) return NO_LABEL;
+    const int64_t label = load_index(a.labels, a.label_bytes, row);
+    return label == a.ignore ? NO_LABEL : (label >= 0 && label < a.K ? (int)label : BAD_LABEL);
+}
+// The label's log probability is 0 for a row without one, NaN with a status bit for one that is no class.  x: the label's logit
+__device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, const RowSums& r, int label, float x)
 {
     if (a.logp) {
-        const int64_t label = load_index(a.labels, a.label_bytes, row);
-        float lp = 0.f;
-        if (label != a.ignore) {
-            const bool is = label >= 0 && label < a.K;
-            lp = is ? log_prob_of(r, logit((int)label), a.inv_t) : NAN;
-            if (!is) atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
-        }
-        a.logp[row] = lp;
+        a.logp[row] = label >= 0 ? log_prob_of(r, x, a.inv_t) : (label == NO_LABEL ? 0.f : NAN);
+        if (label == BAD_LABEL) atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
     }
     if (a.entropy) a.entropy[row] = r.entropy;
     if (a.stats) a.stats[row] = make_float2(r.m, r.log_s);
@@ -95,10 +96,12 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     const RowTile<T> tile(smem, a.K);
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
-    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
+    const int64_t row = row0 + threadIdx.x;
+    tile.fetch((const T*)a.logits, a.ld, row0, rows, a.wide);
+    const int label = row_label(a, min(row, a.n - 1));
+    tile.wait();
     if ((int)threadIdx.x >= rows) return;
     const T* x = tile.row(threadIdx.x);
-    const int64_t row = row0 + threadIdx.x;
 
     typename Top::Key best[TOP > 0 ? TOP : 1];
     float m;
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     sums.clear();
     for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
     const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u));
-    write_row(a, row, r, [&](int j) { return to_f<T>(x[j]); });
+    write_row(a, row, r, label, label >= 0 ? to_f<T>(x[label]) : 0.f);
     write_top<T, TOP>(a, row, r, best);
 }
 
@@ -158,7 +161,7 @@ template <int G>
 struct TopScratch {
     unsigned long long candidate[CANDIDATES];
     unsigned long long chosen[G / 32];
-    uint16_t maxima[G > 32 ? 128 : 1];      // 64 or 128 of a block
+    uint4 maxima[G > 32 ? 32 : 1];          // 64 or 128 of a block, four to a vector
     uint32_t bound;
     int count;
 };
@@ -195,27 +198,34 @@ __device__ __forceinline__ uint32_t kth_largest(uint32_t (&v)[4], int k, bool fo
 
 template <typename T, int G, int P>
 __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, const RowSums& r, const RowValues<T, G, P>& vals,
-                                             const Group<G>& group, TopScratch<G>& scratch, float mine)
+                                             const Group<G>& group, TopScratch<G>& scratch, const float (&part)[4])
 {
     const int me = group.rank(), lane = threadIdx.x & 31;
     const bool four = a.top > 32;
     uint32_t bound = 0;
     if (G == 32) {
-        uint32_t v[4] = {0, 0, 0, 0};
-        vals.each([&](const Eight<T>& x, int, int i) { v[i & 3] = ::max(v[i & 3], order_key(x.largest()) >> 16); },
-                  [&](float x, int, int) { v[3] = ::max(v[3], order_key(x) >> 16); });
+        // (a part without a logit: minus infinity, which is no more than any)
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = part[i] == -INFINITY ? 0u : order_key(part[i]) >> 16;
         bound = kth_largest(v, a.top, four);
     } else {
-        const int per = four ? G / 128 : G / 64;      // threads that share a maximum
-        float m = mine;
+        // a block's threads count how many reach each of 64 (128) maxima: in a tenth of the time that one warp takes for 32 of them in turn
+        const int per = four ? G / 128 : G / 64, all = four ? 128 : 64;      // threads that share a maximum
+        float m = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
         for (int o = 1; o < per; o *= 2) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
-        if (lane % per == 0) scratch.maxima[me / per] = order_key(m) >> 16;
-        if (me == 0) scratch.count = 0;
+        const uint32_t key = order_key(m) >> 16;
+        if (lane % per == 0) reinterpret_cast<uint32_t*>(scratch.maxima)[me / per] = key;
+        if (me == 0) scratch.count = scratch.bound = 0;
         __syncthreads();
-        if (me < 32) {
-            uint32_t v[4] = {scratch.maxima[me], scratch.maxima[me + 32], four ? scratch.maxima[me + 64] : 0u, four ? scratch.maxima[me + 96] : 0u};
-            const uint32_t b = kth_largest(v, a.top, four);
-            if (me == 0) scratch.bound = b;
+        if (lane % per == 0) {
+            int reach = 0;
+#pragma unroll 4
+            for (int i = 0; i < all / 4; ++i) {
+                const uint4 v = scratch.maxima[i];
+                reach += (v.x >= key) + (v.y >= key) + (v.z >= key) + (v.w >= key);
+            }
+            if (reach >= a.top) atomicMax(&scratch.bound, key);
         }
         __syncthreads();
         bound = scratch.bound;
@@ -238,10 +248,13 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
     auto put = [&](int at, int j) { scratch.candidate[at] = wide_key(to_f<T>(logits[j]), j); };
     int count = 0;
     if (P > 0) {
-        uint32_t mask = 0, edge_mask = 0;
-        vals.each([&](const Eight<T>& x, int, int i) { mask |= bits_of(x) << (8 * i); },
+        constexpr int WORDS = (P + 3) / 4 > 0 ? (P + 3) / 4 : 1;
+        uint32_t mask[WORDS] = {}, edge_mask = 0;
+        vals.each([&](const Eight<T>& x, int, int i) { mask[i / 4] |= bits_of(x) << (8 * (i & 3)); },
                   [&](float x, int, int q) { edge_mask |= (bound == 0 || !(x < least) ? 1u : 0u) << q; });
-        const int own = __popc(mask) + __popc(edge_mask);
+        int own = __popc(edge_mask);
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) own += __popc(mask[w]);
         int at = own;
         if (G == 32) {
 #pragma unroll
@@ -255,9 +268,12 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
             at = own ? atomicAdd(&scratch.count, own) : 0;
         }
         if (at + own <= CANDIDATES) {
-            for (; mask; mask &= mask - 1) {
-                const int i = __ffs(mask) - 1;
-                put(at++, vals.pieces.first((i >> 3) * G + me) + (i & 7));
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                for (uint32_t b = mask[w]; b; b &= b - 1) {
+                    const int i = __ffs(b) - 1;
+                    put(at++, vals.pieces.first((4 * w + (i >> 3)) * G + me) + (i & 7));
+                }
             }
             for (; edge_mask; edge_mask &= edge_mask - 1) put(at++, vals.pieces.edge_class((__ffs(edge_mask) - 1) * G + me));
         }
@@ -331,8 +347,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_kernel(const Score
     const int me = group.rank();
     const RowPieces<T> pieces((const T*)a.logits + at * a.ld, a.K);
     const RowValues<T, G, P> vals(pieces, me);
-    float mine = -INFINITY;
-    vals.each([&](const Eight<T>& x, int, int) { mine = max_nan(mine, x.largest()); }, [&](float x, int, int) { mine = max_nan(mine, x); });
+    const int label = row_label(a, at);
+    const float label_x = label >= 0 ? to_f<T>(pieces.row[label]) : 0.f;
+    // the largest of a thread's logits, in four parts
+    float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    vals.each([&](const Eight<T>& x, int, int i) {
+        if (P > 0)
+            part[i & 3] = max_nan(part[i & 3], x.largest());
+        else
+            part[0] = max_nan(part[0], x.largest());
+    }, [&](float x, int, int) { part[3] = max_nan(part[3], x); });
+    const float mine = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
     const float m = group.max(mine), origin = row_origin(m);
     const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
     RowSum sums;
@@ -342,9 +367,9 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_kernel(const Score
     float su[2] = {hsum2(sums.s) + edge.s, hsum2(sums.u) + edge.u};
     group.sum(su);
     const RowSums r = row_sums(m, su[0], su[1]);
-    if (me == 0 && row < a.n) write_row(a, row, r, [&](int j) { return to_f<T>(pieces.row[j]); });
+    if (me == 0 && row < a.n) write_row(a, row, r, label, label_x);
     if constexpr (TOPS) {
-        if (row < a.n) alternatives<T, G, P>(a, row, r, vals, group, top_scratch[group.slot()], mine);     // (whole warps)
+        if (row < a.n) alternatives<T, G, P>(a, row, r, vals, group, top_scratch[group.slot()], part);     // (whole warps)
     }
 }
 
@@ -361,7 +386,7 @@ struct RowGrad {
     __device__ __forceinline__ float at(float x, int j, float own) const
     {
         const float t = max_nan(fmaf(x - m, c, shift), NO_POWER);
-        return fmaf(fast_exp2(t), fmaf(t, B, A), fmaf(own, inv_t, j == label ? g : 0.f));     // (no class, no label: -2, -1)
+        return fmaf(fast_exp2(t), fmaf(t, B, A), fmaf(own, inv_t, j == label ? g : 0.f));
     }
 };
 __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, float g_top_sum, bool& none)
@@ -396,18 +421,19 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
     const RowTile<T> tile(smem, a.K);
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
-    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
+    tile.fetch((const T*)a.logits, a.ld, row0, rows, a.wide);
+    const int64_t row = min(row0 + threadIdx.x, a.n - 1);
+    const float* gt = a.g_top ? a.g_top + row * a.top : nullptr;
+    const int32_t* tc = a.g_top ? a.top_class + row * a.top : nullptr;
+    float g_sum = 0.f;
+    if (gt)
+        for (int i = 0; i < a.top; ++i) g_sum += tc[i] >= 0 ? gt[i] : 0.f;
+    bool none;
+    const RowGrad r = row_grad(a, row, g_sum, none);
+    tile.wait();
     if ((int)threadIdx.x < rows) {
-        const int64_t row = row0 + threadIdx.x;
         T* x = tile.row(threadIdx.x);
         const T* logits = (const T*)a.logits + row * a.ld;
-        const float* gt = a.g_top ? a.g_top + row * a.top : nullptr;
-        const int32_t* tc = a.g_top ? a.top_class + row * a.top : nullptr;
-        float g_sum = 0.f;
-        if (gt)
-            for (int i = 0; i < a.top; ++i) g_sum += tc[i] >= 0 ? gt[i] : 0.f;
-        bool none;
-        const RowGrad r = row_grad(a, row, g_sum, none);
         const T label = r.label >= 0 ? from_f<T>(r.at(to_f<T>(x[r.label]), r.label, 0.f)) : from_f<T>(0.f);
         for (int j = 0; j < a.K; j += 8) {
             Eight<T> e = tile.template read<W>(x, j);
@@ -423,7 +449,7 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
     tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
-template <typename T, int G>
+template <typename T, int G, int P>
 __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
@@ -432,6 +458,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const S
     const int64_t row = min(group.row(), a.n - 1);
     const int me = group.rank();
     const RowPieces<T> pieces((const T*)a.logits + row * a.ld, a.K);
+    const RowValues<T, G, P> vals(pieces, me);
     const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
     const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
@@ -444,19 +471,15 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const S
     }
     bool none;
     const RowGrad r = row_grad(a, row, g_sum[0], none);
-#pragma unroll 4
-    for (int p = me; p < (live ? pieces.pieces : 0); p += G) {
-        Eight<T> e = pieces.load(p);
-        r.eight(e);
-        pieces.store(dx, alike, p, e);
-    }
-    for (int e = me; e < (live ? pieces.edges : 0); e += G) {
-        const int j = pieces.edge_class(e);
-        dx[j] = from_f<T>(r.at(to_f<T>(x[j]), -2, 0.f));
-    }
+    const float label_x = r.label >= 0 ? to_f<T>(x[r.label]) : 0.f;       // (on the way with the row)
+    if (live)
+        vals.each([&](Eight<T> e, int j, int) {
+            r.eight(e);
+            pieces.store(dx, alike, j, e);
+        }, [&](float e, int j, int) { dx[j] = from_f<T>(r.at(e, j, 0.f)); });
     // classes with parts of their own once more: the label, then the alternatives (of which the label may be one)
     group.sync();
-    if (me == 0 && live && r.label >= 0) dx[r.label] = from_f<T>(r.at(to_f<T>(x[r.label]), r.label, 0.f));
+    if (me == 0 && live && r.label >= 0) dx[r.label] = from_f<T>(r.at(label_x, r.label, 0.f));
     if (gt) {
         group.sync();
         for (int i = me; i < (live && !none ? a.top : 0); i += G)
@@ -495,53 +518,16 @@ static bool launch_tile_of(const ScoresArgs& a, bool backward, cudaStream_t stre
     }
 }
 
-template <typename T, int G, int P, bool TOPS>
-static void launch_row(const ScoresArgs& a, cudaStream_t stream)
+template <typename T, int G, int P>
+static void launch_row(const ScoresArgs& a, bool backward, cudaStream_t stream)
 {
-    scores_row_kernel<T, G, P, TOPS><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
-}
-template <typename T, int G>
-static void launch_row_bwd(const ScoresArgs& a, cudaStream_t stream)
-{
-    scores_row_bwd_kernel<T, G><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
-}
-// P pieces of each thread: 64 bf16 or 32 fp32 logits, where the alternatives are chosen 32
-template <typename T>
-static void launch_rows(const ScoresArgs& a, cudaStream_t stream)
-{
-    constexpr int P = sizeof(T) == 2 ? 8 : 4;
-    const int most = a.K;
-    if (a.top) {
-        // (a thread's pieces are bits of a word: four at most)
-        if (most <= 256)
-            launch_row<T, 32, 1, true>(a, stream);
-        else if (most <= 512)
-            launch_row<T, 32, 2, true>(a, stream);
-        else if (most <= 1024)
-            launch_row<T, 32, 4, true>(a, stream);
-        else if (most <= 2048)
-            launch_row<T, 128, 2, true>(a, stream);
-        else if (most <= 4096)
-            launch_row<T, 256, 2, true>(a, stream);
-        else if (most <= 8192)
-            launch_row<T, 256, 4, true>(a, stream);
-        else if (most <= 16384)
-            launch_row<T, 512, 4, true>(a, stream);
-        else
-            launch_row<T, 1024, 0, true>(a, stream);
-    } else if (most <= 4 * 8 * P) {
-        launch_row<T, 4, P, false>(a, stream);
-    } else if (most <= 8 * 8 * P) {
-        launch_row<T, 8, P, false>(a, stream);
-    } else if (most <= 16 * 8 * P) {
-        launch_row<T, 16, P, false>(a, stream);
-    } else if (most <= 32 * 8 * P) {
-        launch_row<T, 32, P, false>(a, stream);
-    } else if (most <= 8192) {
-        launch_row<T, 256, 4, false>(a, stream);
-    } else {
-        launch_row<T, 1024, 0, false>(a, stream);
-    }
+    if (backward)
+        scores_row_bwd_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+    else if constexpr (G >= 32)
+        a.top ? scores_row_kernel<T, G, P, true><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a)
+              : scores_row_kernel<T, G, P, false><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+    else
+        scores_row_kernel<T, G, P, false><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
 }
 
 template <typename T>
@@ -554,18 +540,9 @@ static int launch_scores(ScoresArgs a, bool backward, cudaStream_t stream)
     // a thread keeps up to 32 alternatives; beyond, and for longer rows, a warp chooses them
     if (bytes <= TILE_PLAIN_BYTES ? backward || a.top <= 32 : bytes <= TILE_TOP_BYTES && !backward && a.top && a.top <= 32) {
         if (!launch_tile_of<T>(a, backward, stream)) return check_launch("ptv3_class_scores: shared memory attribute");
-    } else if (!backward) {
-        launch_rows<T>(a, stream);
-    } else if (bytes <= 512) {
-        launch_row_bwd<T, 4>(a, stream);
-    } else if (bytes <= 1024) {
-        launch_row_bwd<T, 8>(a, stream);
-    } else if (bytes <= 2048) {
-        launch_row_bwd<T, 16>(a, stream);
-    } else if (bytes <= 8192) {
-        launch_row_bwd<T, 32>(a, stream);
     } else {
-        launch_row_bwd<T, 256>(a, stream);
+        // (where alternatives are chosen, a warp at least)
+        for_row_shape<T>(a.K, !backward && a.top, [&](auto g, auto p) { launch_row<T, decltype(g)::value, decltype(p)::value>(a, backward, stream); });
     }
     count_launches(1);
     return check_launch(what);

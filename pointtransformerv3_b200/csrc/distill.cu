@@ -145,8 +145,9 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
     const int64_t row = row0 + threadIdx.x;
+    tile.fetch((const T*)a.logits, a.ld, row0, rows, a.wide);
     const RowList<N> list(a, min(row, a.n - 1));
-    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
+    tile.wait();
     if ((int)threadIdx.x >= rows) return;
     T* x = tile.row(threadIdx.x);
 
@@ -222,9 +223,10 @@ struct ListPart {
             const int i = me + q * G;
             cls[q] = PLACE_ABSENT;
             v[q] = -INFINITY;
-            if (q * G < a.k) {
-                if (i < a.k) cls[q] = list_class(a, at + i);
-                if (cls[q] >= 0) v[q] = load_value(a.teacher, a.teacher_bf16, at + i);
+            if (q * G < a.k && i < a.k) {
+                const float value = load_value(a.teacher, a.teacher_bf16, at + i);      // (on the way with the class)
+                cls[q] = list_class(a, at + i);
+                v[q] = cls[q] >= 0 ? value : -INFINITY;
             }
         }
     }
@@ -248,6 +250,9 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
     ListPart<G> list;
     list.load(a, row * a.k, me);
     const RowValues<T, G, P> vals(pieces, me);
+    float x_of[ListPart<G>::N];
+#pragma unroll
+    for (int q = 0; q < ListPart<G>::N; ++q) x_of[q] = list.cls[q] >= 0 ? to_f<T>(x[list.cls[q]]) : 0.f;
     if (a.rest) {
         for (int w = me; w < words; w += G) bits[w] = 0;
         group.sync();
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_kernel(const Dist
         all[3] += list.cls[q] == PLACE_BAD ? 128.f : 0.f;
         if (list.cls[q] < 0) continue;
         all[3] += 1.f;
-        const float v = list.v[q], w = entry_weight(a, v, top), d = to_f<T>(x[list.cls[q]]) - origin;
+        const float v = list.v[q], w = entry_weight(a, v, top), d = x_of[q] - origin;
         all[1] += w;
         if (w != 0.f) all[2] = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(top)) * a.inv_t) - d * a.inv_t, all[2]);
         more[1] += v == top ? 0.f : w;
@@ -413,9 +418,10 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
     const int64_t row0 = blockIdx.x * (int64_t)blockDim.x;
     const int rows = (int)min((int64_t)blockDim.x, a.n - row0);
     const int64_t row = min(row0 + threadIdx.x, a.n - 1);
-    RowList<N> list(a, row);
+    tile.fetch((const T*)a.logits, a.ld, row0, rows, a.wide);
+    const RowList<N> list(a, row);
     const float4 st = a.stats[row];
-    tile.load((const T*)a.logits, a.ld, row0, rows, a.wide);
+    tile.wait();
     if ((int)threadIdx.x < rows) {
         T* x = tile.row(threadIdx.x);
         const T* logits = (const T*)a.logits + row * a.ld;
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
     tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
-template <typename T, int G>
+template <typename T, int G, int P>
 __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const DistillArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
@@ -462,47 +468,49 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const 
     const int64_t row = min(group.row(), a.n - 1);
     const int me = group.rank(), slot = group.slot();
     const RowPieces<T> pieces((const T*)a.logits + row * a.ld, a.K);
+    const RowValues<T, G, P> vals(pieces, me);
     const T* x = pieces.row;
     T* dx = (T*)a.dlogits + row * a.K;
     const bool alike = (((uintptr_t)dx ^ (uintptr_t)x) & 15) == 0;
     const float4 st = a.stats[row];
     ListPart<G> list;
     list.load(a, row * a.k, me);
-    float mass[1] = {0.f};
+    float mass[1] = {0.f}, x_of[ListPart<G>::N], t_of[ListPart<G>::N];
+#pragma unroll
+    for (int q = 0; q < ListPart<G>::N; ++q) x_of[q] = list.cls[q] >= 0 ? to_f<T>(x[list.cls[q]]) : 0.f;       // (on the way with the row)
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
-        const float t = list.cls[q] >= 0 ? entry_prob(a, st, list.v[q]) : 0.f;
-        mass[0] += t;
+        t_of[q] = list.cls[q] >= 0 ? entry_prob(a, st, list.v[q]) : 0.f;
+        mass[0] += t_of[q];
         if (me + q * G < LIST_MAX) {
             list_c[slot][me + q * G] = list.cls[q];
-            list_t[slot][me + q * G] = t;
+            list_t[slot][me + q * G] = t_of[q];
         }
     }
     group.sum(mass);
     const DistillGrad r = distill_grad(a, row, st, mass[0]);
-#pragma unroll 4
-    for (int p = me; p < (live ? pieces.pieces : 0); p += G) {
-        Eight<T> e = pieces.load(p);
-        r.eight(e);
-        pieces.store(dx, alike, p, e);
-    }
-    for (int e = me; e < (live ? pieces.edges : 0); e += G) {
-        const int j = pieces.edge_class(e);
-        dx[j] = from_f<T>(r.outside(to_f<T>(x[j])));
-    }
+    if (live)
+        vals.each([&](Eight<T> e, int j, int) {
+            r.eight(e);
+            pieces.store(dx, alike, j, e);
+        }, [&](float e, int j, int) { dx[j] = from_f<T>(r.outside(e)); });
     // the list's classes once more; one that comes twice is written by its first entry, with the sum of both
     group.sync();
-    if (!live) return;
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
+        if (q * G >= a.k) break;
         const int mine = me + q * G, cls = list.cls[q];
-        if (cls < 0) continue;
         int same = 0;
-        for (int i = 0; i < a.k; i += 4) {                   // (absent entries beyond the list's are -1)
-            const int4 c = *reinterpret_cast<const int4*>(&list_c[slot][i]);
-            same += (c.x == cls) + (c.y == cls) + (c.z == cls) + (c.w == cls);
+        if (G == 32 && a.k <= 32) {
+            same = __popc(__match_any_sync(~0u, cls < 0 ? -32 - me : cls));
+        } else if (cls >= 0) {
+            for (int i = 0; i < a.k; i += 4) {                   // (entries beyond the list's are -1)
+                const int4 c = *reinterpret_cast<const int4*>(&list_c[slot][i]);
+                same += (c.x == cls) + (c.y == cls) + (c.z == cls) + (c.w == cls);
+            }
         }
-        float t = list_t[slot][mine];
+        if (cls < 0 || !live) continue;
+        float t = t_of[q];
         bool is_first = true;
         if (same > 1) {
             t = 0.f;
@@ -513,7 +521,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK) distill_row_bwd_kernel(const 
                 }
             }
         }
-        if (is_first) dx[cls] = from_f<T>(r.in_list(to_f<T>(x[cls])) - r.g * t);
+        if (is_first) dx[cls] = from_f<T>(r.in_list(x_of[q]) - r.g * t);
     }
 }
 
@@ -534,15 +542,13 @@ static bool launch_tile(const DistillArgs& a, bool backward, cudaStream_t stream
     return backward ? run(distill_tile_bwd_kernel<T, W, 0>) : run(distill_tile_kernel<T, W, 0>);
 }
 template <typename T, int G, int P>
-static void launch_row(const DistillArgs& a, cudaStream_t stream)
+static void launch_row(const DistillArgs& a, bool backward, cudaStream_t stream)
 {
     const size_t smem = a.rest ? (size_t)bit_words(a.K) * 4 * Group<G>::ROWS : 0;
-    distill_row_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, smem, stream>>>(a);
-}
-template <typename T, int G>
-static void launch_row_bwd(const DistillArgs& a, cudaStream_t stream)
-{
-    distill_row_bwd_kernel<T, G><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+    if (backward)
+        distill_row_bwd_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+    else
+        distill_row_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, smem, stream>>>(a);
 }
 
 template <typename T>
@@ -551,8 +557,6 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
     a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
     a.list4 = a.list_bytes == 4 && !a.teacher_bf16 && a.k % 4 == 0 && (((uintptr_t)a.list | (uintptr_t)a.teacher) & 15) == 0;
-    constexpr int P = sizeof(T) == 2 ? 8 : 4;            // pieces of each thread: 64 bf16 or 32 fp32 logits
-    const int most = a.K;
     const size_t bytes = a.K * sizeof(T);
     if (bytes <= TILE_PLAIN_BYTES) {
         bool ok;
@@ -563,25 +567,12 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
         default: ok = launch_tile<T, sizeof(T) == 2 ? 2 : 4>(a, backward, stream); break;
         }
         if (!ok) return check_launch("ptv3_distill_topk: shared memory attribute");
-    } else if (backward) {
-        if (bytes <= 1024)
-            launch_row_bwd<T, 8>(a, stream);
-        else if (bytes <= 2048)
-            launch_row_bwd<T, 16>(a, stream);
-        else if (bytes <= 8192)
-            launch_row_bwd<T, 32>(a, stream);
-        else
-            launch_row_bwd<T, 256>(a, stream);
-    } else if (most <= 8 * 8 * P) {
-        launch_row<T, 8, P>(a, stream);
-    } else if (most <= 16 * 8 * P) {
-        launch_row<T, 16, P>(a, stream);
-    } else if (most <= 32 * 8 * P) {
-        launch_row<T, 32, P>(a, stream);
-    } else if (most <= 8192) {
-        launch_row<T, 256, 4>(a, stream);
     } else {
-        launch_row<T, 1024, 0>(a, stream);
+        // (a list over 8 threads at least)
+        for_row_shape<T>(a.K, false, [&](auto g, auto p) {
+            constexpr int G = decltype(g)::value, P = decltype(p)::value;
+            launch_row<T, (G < 8 ? 8 : G), (G < 8 ? P / 2 : P)>(a, backward, stream);
+        });
     }
     count_launches(1);
     return check_launch(backward ? "ptv3_distill_topk_bwd" : "ptv3_distill_topk_fwd");

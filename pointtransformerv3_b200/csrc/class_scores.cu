@@ -338,7 +338,7 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
 }
 
 template <typename T, int G, int P, bool TOPS>
-__global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) scores_row_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     __shared__ TopScratch<TOPS ? G : 32> top_scratch[TOPS ? Group<G>::ROWS : 1];
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
 }
 
 template <typename T, int G, int P>
-__global__ void __launch_bounds__(Group<G>::BLOCK) scores_row_bwd_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) scores_row_bwd_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     const Group<G> group{scratch};

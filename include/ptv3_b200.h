@@ -674,6 +674,18 @@ int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void* labels, in
                           void* dlogits, int64_t n, int classes, int top, float temperature, int dtype, void* stream);
 
 /*
+ * The same answers straight from features, without logits in memory: logits = feat W^T + bias in fp32 (tcgen05), any number of classes.
+ *   feat      n x channels bf16, weight classes x channels bf16, both 16-byte aligned; bias: classes bf16 or NULL
+ *   the outputs as above (entropy is required); a row with a NaN has alternatives of NaN and classes of -1
+ * channels a multiple of 8 up to 512, classes up to 262 144, top up to PTV3_HEAD_TOP_MAX, temperature in [1e-6, 1e6].  status is required; it
+ * also reports a wait that ran out (PTV3_STATUS_WAIT_LIMIT).
+ */
+#define PTV3_HEAD_TOP_MAX 32
+int ptv3_seg_head_scores_fwd(const void* feat, const void* weight, const void* bias, const void* labels, int label_bytes,
+                             int64_t ignore, float* log_prob, float* entropy, float* top_log_prob, int32_t* top_class, int64_t n,
+                             int channels, int classes, int top, float temperature, int dtype, uint32_t* status, void* stream);
+
+/*
  * A student's logits against the best k classes that a teacher kept of each row.  With p = softmax(logits / temperature):
  *   rest = 0: t = softmax(teacher / temperature) over the row's list;  loss = sum t_i (log t_i - log p_{c_i})
  *   rest = 1: t = exp(teacher), and what the list leaves, t_r = max(0, 1 - sum t), against the probability p_r of the classes

@@ -145,6 +145,8 @@ SIGNATURES = {
                                       c_int, c_f32, c_int, c_ptr, c_ptr]),
     "ptv3_class_scores_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
                                       c_ptr, c_ptr, c_i64, c_int, c_int, c_f32, c_int, c_ptr]),
+    "ptv3_seg_head_scores_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int,
+                                         c_int, c_int, c_f32, c_int, c_ptr, c_ptr]),
     "ptv3_distill_topk_fwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_ptr, c_int, c_int, c_ptr, c_ptr, c_i64, c_int, c_f32,
                                       c_int, c_int, c_ptr, c_ptr]),
     "ptv3_distill_topk_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_ptr, c_int, c_int, c_ptr, c_ptr, c_i64, c_ptr, c_i64,

@@ -1036,7 +1036,8 @@ class SegHead(PointModule):
     """Per-point classifier on the backbone's output: ``Linear(in_channels,
     num_classes)`` (state_dict keys ``weight`` / ``bias`` like the ``seg_head`` of a
     segmentor around the reference backbone) with the arg max taken in the same pass.
-    ``forward(point)`` stores ``seg_logits`` (unless ``logits=False``) and ``seg_pred``."""
+    ``forward(point)`` stores ``seg_logits`` (unless ``logits=False``) and ``seg_pred``.
+    ``log_probs(point, labels)`` scores a batch instead: log probabilities, entropy, alternatives, with gradients where they are asked for."""
 
     def __init__(self, in_channels, num_classes, logits=True):
         super().__init__()
@@ -1059,6 +1060,19 @@ class SegHead(PointModule):
             point["seg_logits"] = logits
         point["seg_pred"] = labels
         return point
+
+    def log_probs(self, point, labels=None, top=0, temperature=1.0, ignore_index=-1, status=None):
+        """``functional.class_log_probs`` of the head's logits (``ClassScores``), for losses (``-log_prob``), for uncertainty and for the
+        lists that ``functional.distill_topk`` learns from.  Where no gradients are wanted, bf16 features of up to 512 channels (a multiple of 8) go
+        straight to the scores, up to 32 alternatives: logits are fp32 on the way and never stored (``ops.seg_head_log_probs``).
+        Otherwise they are the layer's own, in its type."""
+        feat = point.feat if isinstance(point, Point) else point
+        weight, bias = self.linear.weight, self.linear.bias
+        plain = not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (feat, weight, bias)))
+        if (plain and type(self.linear) is nn.Linear and feat.dim() == 2 and weight.dtype == feat.dtype
+                and ops.head_scores_supported(feat.shape[1], top, feat.dtype)):
+            return ops.seg_head_log_probs(feat, weight, bias, labels, top, temperature, ignore_index, status)
+        return functional.class_log_probs(self.linear(feat), labels, top, temperature, ignore_index, status)
 
 
 def _linear_op(x, linear, status):

@@ -1013,6 +1013,51 @@ def class_scores_bwd(logits, labels, entropy, classes, stats, temperature, ignor
     return dlogits
 
 
+def head_scores_supported(channels, top, dtype):
+    """Whether ``seg_head_log_probs`` takes features of that width and type, and so many alternatives."""
+    return dtype == torch.bfloat16 and channels % 8 == 0 and 8 <= channels <= 512 and 0 <= top <= 32
+
+
+def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=1.0, ignore_index=-1, status=None):
+    """``functional.class_log_probs`` of feat (N, C) @ weight (K, C)^T + bias (K,) without the logits, which are fp32 on the way: log
+    probability of ``labels``, entropy, alternatives (``functional.ClassScores``).  bf16, C a multiple of 8 up to 512, K up to 262 144, top up to
+    32, no gradients.  A masked class (a bias of minus infinity) is no alternative.  status: a device status word of the caller's; without
+    one the call checks for itself and waits for the device."""
+    from .functional import CLASSES_MAX, ClassScores, TEMPERATURES, _aligned, _check_labels, _on, _same_device, _status_word
+    _same_device(feat, weight, bias, labels, status)
+    if feat.dim() != 2 or weight.dim() != 2 or weight.shape[1] != feat.shape[1] or not 1 <= weight.shape[0] <= CLASSES_MAX:
+        raise ValueError("features (N, C) and weights (1 to %d classes, C), got %s and %s" % (
+            CLASSES_MAX, tuple(feat.shape), tuple(weight.shape)))
+    n, C = feat.shape
+    K = weight.shape[0]
+    if bias is not None and bias.shape != (K,):
+        raise ValueError("bias must be (%d,), got %s" % (K, tuple(bias.shape)))
+    if any(t is not None and t.dtype != torch.bfloat16 for t in (feat, weight, bias)):
+        raise ValueError("features, weights and bias must be bf16")
+    if not TEMPERATURES[0] <= temperature <= TEMPERATURES[1]:
+        raise ValueError("temperature %r, not within %g to %g" % (temperature, *TEMPERATURES))
+    labels = _check_labels(labels, n, top, ignore_index)
+    if not head_scores_supported(C, top, feat.dtype):
+        raise ValueError("%d channels (a multiple of 8 up to 512), %d alternatives (up to 32)" % (C, top))
+    dev, f32 = feat.device, torch.float32
+    with _on(dev):
+        status, own = _status_word(status, dev)
+        feat, weight = _aligned(feat), _aligned(weight)
+        bias = None if bias is None else bias.contiguous()
+        log_prob = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
+        entropy = torch.empty(n, dtype=f32, device=dev)
+        values = torch.empty((n, top), dtype=f32, device=dev) if top else None
+        classes = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
+        with timed("seg_head_log_probs", 2.0 * n * C * K):
+            _lib.check(_lib.load().ptv3_seg_head_scores_fwd(
+                feat.data_ptr(), weight.data_ptr(), _lib.ptr(bias), _lib.ptr(labels), 0 if labels is None else labels.element_size(),
+                int(ignore_index), _lib.ptr(log_prob), entropy.data_ptr(), _lib.ptr(values), _lib.ptr(classes), n, C, K, int(top),
+                float(temperature), _lib.dtype_id(feat), status.data_ptr(), _lib.stream()), "ptv3_seg_head_scores_fwd")
+        if own:
+            _lib.raise_on_status(status, "ptv3_seg_head_scores_fwd")
+    return ClassScores(log_prob, entropy, values, classes)
+
+
 def distill_topk_fwd(logits, teacher, classes, temperature, rest, status, keep=False):
     """See ptv3_distill_topk_fwd; ``functional.distill_topk`` is the checked form with gradients.  -> (loss (N,), stats or None)."""
     n, K = logits.shape

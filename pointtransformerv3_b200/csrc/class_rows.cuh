@@ -174,6 +174,18 @@ template <> struct TopKey<float> {
     __device__ static __forceinline__ float value(Key k) { return order_value((uint32_t)(k >> 32)); }
 };
 
+__device__ __forceinline__ void larger_first(int& a, int& b)
+{
+    const int hi = ::max(a, b), lo = ::min(a, b);
+    a = hi;
+    b = lo;
+}
+__device__ __forceinline__ void larger_first(uint32_t& a, uint32_t& b)
+{
+    const uint32_t hi = ::max(a, b), lo = ::min(a, b);
+    a = hi;
+    b = lo;
+}
 template <typename K>
 __device__ __forceinline__ void larger_first(K& a, K& b)
 {

@@ -9,22 +9,6 @@
 
 namespace ptv3 {
 
-template <typename T, int TOP, typename Key>
-__device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, const RowSums& r, const Key (&best)[TOP > 0 ? TOP : 1])
-{
-    int32_t* to_class = a.top_class + row * a.top;
-    float* to_value = a.top_logp + row * a.top;
-#pragma unroll
-    for (int i = 0; i < TOP; ++i) {
-        if (i < a.top) {
-            const int cls = TopKey<T>::cls(best[i]);
-            const bool is = (unsigned)cls < (unsigned)a.K;
-            to_class[i] = is ? cls : -1;
-            to_value[i] = is ? log_prob_of(r, TopKey<T>::value(best[i]), a.inv_t) : -INFINITY;
-        }
-    }
-}
-
 // ---- short rows: a tile of rows, one thread to a row -----------------------------------------------------------------
 // TOP: 0, or 1, 2, 4, ... 32 alternatives at least.  The row is read twice from shared memory, for the largest (with their keys) and for
 // the sums.
@@ -81,7 +65,16 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
     const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u));
     write_row(a, row, r, label, label >= 0 ? to_f<T>(x[label]) : 0.f);
-    write_top<T, TOP>(a, row, r, best);
+    if (TOP > 0) {
+        const bool wide = wide_lists(a);
+        write_list<TOP>(a.top_class + row * a.top, a.top, wide, [&](int i) {
+            const int cls = Top::cls(best[i]);
+            return (unsigned)cls < (unsigned)a.K ? cls : -1;
+        });
+        write_list<TOP>(a.top_logp + row * a.top, a.top, wide, [&](int i) {
+            return (unsigned)Top::cls(best[i]) < (unsigned)a.K ? log_prob_of(r, Top::value(best[i]), a.inv_t) : -INFINITY;
+        });
+    }
 }
 
 // ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------------------

@@ -64,4 +64,28 @@ __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, cons
     if (a.stats) a.stats[row] = make_float2(r.m, r.log_s);
 }
 
+// A row's alternatives out, get(i) the i-th (i < TOP): as wide as lists are aligned.  (Through shared memory, so that a warp's stores are
+// neighbours, they took as long or longer: 407 678 x 20 with 5 alternatives 20.4 us instead of 16.4, with 8 to 64 classes 12.4 and 13.9.)
+template <int TOP, typename V, typename F>
+__device__ __forceinline__ void write_list(V* out, int top, bool wide, F&& get)
+{
+    if (TOP >= 4 && wide) {
+#pragma unroll
+        for (int i = 0; i + 3 < TOP; i += 4) {
+            if (i < top) {
+                const V v[4] = {get(i), get(i + 1), get(i + 2), get(i + 3)};
+                *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(v);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TOP; ++i)
+            if (i < top) out[i] = get(i);
+    }
+}
+__device__ __forceinline__ bool wide_lists(const ScoresArgs& a)
+{
+    return a.top % 4 == 0 && (((uintptr_t)a.top_logp | (uintptr_t)a.top_class) & 15) == 0;
+}
+
 }  // namespace ptv3

@@ -10,9 +10,9 @@
 // classes.  So no value crosses threads, and groups work on different tiles while the next are multiplied.  Where a row has several
 // class tiles, the groups' results of it meet in shared memory.
 //
-// Alternatives.  Up to 64 classes go through a sorting network of 64-bit keys.  With more, a logit above the row's k-th best so far is put
-// into a short list of the row's in shared memory (one predicated store; a row of 1 201 has about 16 + 16 ln(1 201 / 16) such), and when a row of
-// the warp has SPARE places left, every row's list is sorted and merged with its best.
+// Alternatives: 32 logits go through a sorting network of 32-bit keys, the logit without its last five bits and its place instead of
+// them, a maximum and a minimum to an exchange; the best of these, as they are, merge with the row's best so far.  Where logits that differ in
+// those bits alone are among the best of the 32, or beside them, the warp takes 64-bit keys, which hold all of both (three times the time).
 #include "class_scores.cuh"
 #include "tc05.cuh"
 
@@ -23,8 +23,7 @@ using namespace tc05;
 constexpr int HS_ROWS = 128;
 constexpr int HS_BK = 64;                              // one 128-byte swizzle span of bf16
 constexpr int HS_X_BYTES = HS_ROWS * HS_BK * 2;
-constexpr int HS_PENDING = 16, HS_SPARE = 8;           // places of a row's short list; what eight more logits may take
-constexpr int HS_NETWORK = 64;                         // classes up to which a network takes them all
+constexpr int HS_AREA = 32 * 32;                       // words of a warp: 32 logits of its rows
 
 struct HeadArgs {
     ScoresArgs s;                  // n, labels, outputs, K, top, inv_t, status
@@ -34,43 +33,138 @@ struct HeadArgs {
     int x_stages, w_stages;        // w_stages 0: all of W is resident
 };
 
-// the best of a row, sorted, as keys of (logit, lowest class), and the value that another logit has to exceed
+__device__ __forceinline__ unsigned long long head_key(float x, int j) { return x > -INFINITY ? (unsigned long long)order_key(x) << 32 | (0x7fffffffu - j) : 0ull; }
+
+// A row's best logits, sorted, the lowest class first among equals; minus infinity (of any class) where there are no more.
 template <int B>
 struct Best {
-    unsigned long long key[B > 0 ? B : 1];
-    float least;
+    float v[B];
+    int c[B];
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int i = 0; i < B; ++i) key[i] = 0;
-        least = -INFINITY;
-    }
-    __device__ __forceinline__ static unsigned long long key_of(float x, int j) { return (unsigned long long)order_key(x) << 32 | (0x7fffffffu - j); }
-    __device__ __forceinline__ void set_least(int top)
-    {
-        unsigned long long k = 0;
-#pragma unroll
-        for (int i = 0; i < B; ++i) k = i == top - 1 ? key[i] : k;
-        least = k ? order_value((uint32_t)(k >> 32)) : -INFINITY;
-    }
-    // N keys in any order
-    template <int N>
-    __device__ __forceinline__ void absorb(unsigned long long* k)
-    {
-        if constexpr (N >= B) {
-#pragma unroll
-            for (int b = 0; b < N; b += B) {
-                sort_keys<B>(k + b);
-                merge_keys<B>(key, k + b);
-            }
-        } else {
-            unsigned long long wide[B];
-            sort_keys<N>(k);
-#pragma unroll
-            for (int i = 0; i < B; ++i) wide[i] = i < N ? k[i] : 0;
-            merge_keys<B>(key, wide);
+        for (int i = 0; i < B; ++i) {
+            v[i] = -INFINITY;
+            c[i] = -1;
         }
     }
+    __device__ __forceinline__ void from_keys(const unsigned long long* k)
+    {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            v[i] = k[i] ? order_value((uint32_t)(k[i] >> 32)) : -INFINITY;
+            c[i] = (int)(0x7fffffffu - (uint32_t)k[i]);
+        }
+    }
+    // The best of 32 logits, classes from j0 on; those from the `width`-th on and masked ones are minus infinity.  mine: the same, 32 words apart in
+    // shared memory
+    __device__ __forceinline__ void take(const float (&x)[32], int j0, int width, int top, float* mine)
+    {
+        constexpr int STEP = B > 8 ? B : 8;
+        int best[B], lost = INT32_MIN;
+#pragma unroll
+        for (int b = 0; b < 32; b += STEP) {
+            if (b == 0 || b < width) {
+                int k[STEP];
+#pragma unroll
+                for (int i = 0; i < STEP; ++i) {
+                    const int u = __float_as_int(x[b + i]);
+                    k[i] = ((u ^ ((u >> 31) & 0x7fffffff)) & ~31) | (31 - (b + i));
+                }
+#pragma unroll
+                for (int q = 0; q < STEP; q += B) {
+                    sort_keys<B>(k + q);
+                    if (b == 0 && q == 0) {
+#pragma unroll
+                        for (int i = 0; i < B; ++i) best[i] = k[i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < B; ++i) lost = ::max(lost, ::min(best[i], k[q + B - 1 - i]));
+                        merge_keys<B>(best, k + q);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int at = 31 - (best[i] & 31);
+            c[i] = j0 + at;
+            v[i] = mine[32 * at];
+        }
+        // Keys that differ in the place alone: their logits may be in the other order, or one that was left out larger than the last.
+        // (Equal logits are in order: the lower place has the larger key.)
+        bool wrong = false;
+#pragma unroll
+        for (int i = 0; i + 1 < B; ++i) wrong |= v[i] < v[i + 1];
+        const bool edge = (unsigned)(best[B - 1] ^ lost) < 32u && v[B - 1] > -INFINITY;
+        if (__any_sync(~0u, edge)) {
+            int better = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) better += x[i] > v[B - 1];
+            wrong |= edge && better >= B;
+            // (as many as B - 1 are better than the last of the list where it is right)
+        }
+        if (__any_sync(~0u, wrong)) {
+            unsigned long long wide[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) wide[i] = 0;
+#pragma unroll
+            for (int b = 0; b < 32; b += STEP) {
+                if (b == 0 || b < width) {
+                    unsigned long long k[STEP];
+#pragma unroll
+                    for (int i = 0; i < STEP; ++i) k[i] = head_key(x[b + i], j0 + b + i);
+#pragma unroll
+                    for (int q = 0; q < STEP; q += B) {
+                        sort_keys<B>(k + q);
+                        merge_keys<B>(wide, k + q);
+                    }
+                }
+            }
+            from_keys(wide);
+        }
+    }
+    // with the best of later classes
+    __device__ __forceinline__ void merge(const Best& o)
+    {
+        bool equal = false;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const bool up = o.v[B - 1 - i] > v[i];
+            v[i] = up ? o.v[B - 1 - i] : v[i];
+            c[i] = up ? o.c[B - 1 - i] : c[i];
+        }
+#pragma unroll
+        for (int d = B / 2; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if ((i & d) == 0) exchange(i, i + d, v[i + d] > v[i]);
+#pragma unroll
+        for (int i = 0; i + 1 < B; ++i) equal |= v[i] == v[i + 1] && v[i] > -INFINITY;
+        // (the half-cleaners leave equal logits in any order)
+        if (__any_sync(~0u, equal)) {
+#pragma unroll 1
+            for (int r = 0; r < B / 2; ++r) {
+#pragma unroll
+                for (int i = 0; i + 1 < B; i += 2) exchange(i, i + 1, v[i] == v[i + 1] && c[i + 1] < c[i]);
+#pragma unroll
+                for (int i = 1; i + 1 < B; i += 2) exchange(i, i + 1, v[i] == v[i + 1] && c[i + 1] < c[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void exchange(int i, int j, bool swap)
+    {
+        const float vi = v[i];
+        const int ci = c[i];
+        v[i] = swap ? v[j] : vi;
+        c[i] = swap ? c[j] : ci;
+        v[j] = swap ? vi : v[j];
+        c[j] = swap ? ci : c[j];
+    }
+};
+template <>
+struct Best<0> {
+    __device__ __forceinline__ void clear() {}
 };
 
 // a row's running answers
@@ -102,20 +196,20 @@ struct HeadRow {
     }
 };
 
-template <int NG, int B, bool NETWORK>
+template <int NG, int B>
 __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                        const __grid_constant__ CUtensorMap map_w, const HeadArgs a)
 {
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    unsigned char* smem = smem_raw + (-smem_u32_generic(smem_raw) & 1023u);       // (plain arithmetic: it stays known to be shared)
     const uint32_t sbase = smem_u32_generic(smem);
     const int w_bytes = a.N * HS_BK * 2;
     const int w_count = a.w_stages ? a.w_stages : a.col_tiles * a.chunks;
     const uint32_t x_base = sbase, w_base = sbase + a.x_stages * HS_X_BYTES;
     unsigned char* after = smem + a.x_stages * HS_X_BYTES + w_count * w_bytes;
     float* bias_s = reinterpret_cast<float*>(after);                                     // NG x N
-    // short lists; where groups meet, they leave their parts in the same place
-    constexpr int MEET_ROW = 16 + B * 8, PENDING_BYTES = B && !NETWORK ? NG * HS_ROWS * HS_PENDING * 8 : 0, MEET_BYTES = (NG - 1) * HS_ROWS * MEET_ROW;
+    // words of each warp; where groups meet, they leave their parts in the same place
+    constexpr int MEET_ROW = 16 + B * 8, PENDING_BYTES = B ? NG * 4 * HS_AREA * 4 : 0, MEET_BYTES = (NG - 1) * HS_ROWS * MEET_ROW;
     unsigned char* pending = reinterpret_cast<unsigned char*>(bias_s + NG * a.N);
     uint64_t* bars = reinterpret_cast<uint64_t*>(pending + (a.col_tiles > 1 && MEET_BYTES > PENDING_BYTES ? MEET_BYTES : PENDING_BYTES));
     const int nbar = 2 * a.x_stages + 2 * a.w_stages + 2 * NG + 1;
@@ -244,44 +338,34 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
         const uint32_t my_tmem = tmem + group * a.N + ((uint32_t)(quarter * 32) << 16);
         float* my_bias = bias_s + group * a.N;
         // (a row's places are 32 lanes apart, so that a warp's stores meet no conflict)
-        float2* my_pending = reinterpret_cast<float2*>(pending) + (group * 4 + quarter) * 32 * HS_PENDING + lane;
+        uint32_t* area = reinterpret_cast<uint32_t*>(pending) + (group * 4 + quarter) * HS_AREA;
+        float* my_logits = reinterpret_cast<float*>(area) + lane;
         const float c = a.s.inv_t * LOG2E;
         const uint64_t c2 = pack2(c, c);
         int turn = 0, phase = 0;         // class tiles so far, modulo NG; of this group's accumulator
         bool bias_there = false;
         int tile_no = 0;
         for (int rt = blockIdx.x; rt < a.row_tiles; rt += gridDim.x, ++tile_no) {
+            if (a.col_tiles == 1 && tile_no % NG != group) continue;
             const int64_t row = (int64_t)rt * HS_ROWS + r;
             HeadRow h;
             h.clear();
             Best<B> best;
             best.clear();
-            int waiting = 0;                     // places taken of the row's short list
-            int label = NO_LABEL;
+            const int label = row_label(a.s, min(row, a.s.n - 1));       // (read early: it has until the first tile is there)
             bool mine = false;
-            auto settle = [&]() {
-                // the short list of every row of the warp into its best
-                unsigned long long k[HS_PENDING];
-#pragma unroll
-                for (int i = 0; i < HS_PENDING; ++i) {
-                    const float2 e = my_pending[i * 32];
-                    k[i] = i < waiting ? Best<B>::key_of(e.x, __float_as_int(e.y)) : 0ull;
-                }
-                best.template absorb<HS_PENDING>(k);
-                best.set_least(a.s.top);
-                waiting = 0;
-            };
             for (int t = 0; t < a.col_tiles; ++t) {
-                const bool here = turn == group;
-                turn = turn + 1 == NG ? 0 : turn + 1;
-                if (!here) continue;
-                if (!mine) label = row_label(a.s, min(row, a.s.n - 1));
+                if (a.col_tiles > 1) {
+                    const bool here = turn == group;
+                    turn = turn + 1 == NG ? 0 : turn + 1;
+                    if (!here) continue;
+                }
                 mine = true;
                 const int col0 = t * a.N;
                 if (!bias_there || a.col_tiles > 1) {
                     if (bias_there) named_barrier(1 + group, 128);     // every warp has finished with the tile before
                     for (int i = r; i < a.N; i += HS_ROWS)
-                        my_bias[i] = a.bias && col0 + i < a.s.K ? __bfloat162float(a.bias[col0 + i]) : 0.f;
+                        my_bias[i] = a.bias && col0 + i < a.s.K ? __bfloat162float(a.bias[col0 + i]) + 0.f : 0.f;    // (no zero below zero)
                     named_barrier(1 + group, 128);
                     bias_there = true;
                 }
@@ -294,12 +378,6 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
                     tmem_ld32(my_tmem + b, v);
                     tmem_ld_wait();
                     tmem_ld_fence(v);
-                    if (b + 32 >= width) {
-                        // the accumulator may be overwritten
-                        fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_one(acc_empty + 8 * group);
-                    }
                     float x[32];
                     const ulonglong2* bias2 = reinterpret_cast<const ulonglong2*>(my_bias + b);
 #pragma unroll
@@ -311,64 +389,70 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
                     const int j0 = col0 + b;
                     if (b + 32 > width) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (b + i >= width) x[i] = -INFINITY;
+                        for (int i = 0; i < 32; ++i) x[i] = i < width - b ? x[i] : -INFINITY;
                     }
-                    // the label's logit
-                    if ((unsigned)(label - j0) < 32u) {
+                    // running sums, eight classes at a time as far as there are any
+                    float top = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (label == j0 + i) h.label_x = x[i];
+                    for (int q = 0; q < 32; q += 8) {
+                        if (q == 0 || b + q < width) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) top = max_nan(top, x[q + i]);
+                        }
                     }
-                    // running sums
-                    float top = x[0];
-#pragma unroll
-                    for (int i = 1; i < 32; ++i) top = max_nan(top, x[i]);
                     h.rebase(max_nan(h.m, top), c);
                     const float origin = row_origin(h.m);
                     const uint64_t minus = pack2(-origin, -origin);
                     uint64_t s2[2] = {0, 0}, u2[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float lo, hi;
-                        unpack2(mul2(add2(pack2(x[i], x[i + 1]), minus), c2), lo, hi);
-                        lo = max_nan(lo, NO_POWER);
-                        hi = max_nan(hi, NO_POWER);
-                        const uint64_t e = pack2(fast_exp2(lo), fast_exp2(hi));
-                        s2[i / 2 & 1] = add2(s2[i / 2 & 1], e);
-                        u2[i / 2 & 1] = fma2(e, pack2(lo, hi), u2[i / 2 & 1]);
+                    for (int q = 0; q < 32; q += 8) {
+                        if (q == 0 || b + q < width) {
+#pragma unroll
+                            for (int i = q; i < q + 8; i += 2) {
+                                float lo, hi;
+                                unpack2(mul2(add2(pack2(x[i], x[i + 1]), minus), c2), lo, hi);
+                                lo = max_nan(lo, NO_POWER);
+                                hi = max_nan(hi, NO_POWER);
+                                const uint64_t e = pack2(fast_exp2(lo), fast_exp2(hi));
+                                s2[i / 2 & 1] = add2(s2[i / 2 & 1], e);
+                                u2[i / 2 & 1] = fma2(e, pack2(lo, hi), u2[i / 2 & 1]);
+                            }
+                        }
                     }
                     h.s += hsum2(add2(s2[0], s2[1]));
                     h.u += hsum2(add2(u2[0], u2[1]));
                     // alternatives
-                    if (B > 0 && NETWORK) {
+                    if constexpr (B > 0) {
 #pragma unroll
-                        for (int q = 0; q < 32; q += (B > 8 ? B : 8)) {
-                            if (b + q < width) {
-                                unsigned long long k[B > 8 ? B : 8];
+                        for (int i = 0; i < 32; ++i) my_logits[32 * i] = x[i];
+                        if ((unsigned)(label - j0) < 32u) h.label_x = my_logits[32 * (label - j0)];
+                        if (a.s.K <= 32) {
+                            best.take(x, j0, width - b, a.s.top, my_logits);
+                        } else {
+                            // (not where no row of the warp has a logit that is better than its k-th best)
+                            float least = -INFINITY;
 #pragma unroll
-                                for (int i = 0; i < (B > 8 ? B : 8); ++i) k[i] = x[q + i] > -INFINITY ? Best<B>::key_of(x[q + i], j0 + q + i) : 0ull;
-                                best.template absorb<(B > 8 ? B : 8)>(k);
-                            }
-                        }
-                    } else if (B > 0) {
-#pragma unroll
-                        for (int q = 0; q < 32; q += 8) {
-                            float m8 = x[q];
-#pragma unroll
-                            for (int i = 1; i < 8; ++i) m8 = fmaxf(m8, x[q + i]);
-                            if (__any_sync(~0u, m8 > best.least)) {
-                                if (__any_sync(~0u, waiting > HS_PENDING - HS_SPARE)) settle();
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    if (x[q + i] > best.least) my_pending[32 * waiting++] = make_float2(x[q + i], __int_as_float(j0 + q + i));
+                            for (int i = 0; i < B; ++i) least = i == a.s.top - 1 ? best.v[i] : least;
+                            if (__any_sync(~0u, top > least)) {
+                                Best<B> more;
+                                more.take(x, j0, width - b, a.s.top, my_logits);
+                                best.merge(more);
                             }
                         }
                     }
+                    if (b + 32 >= width) {
+                        // the accumulator may be overwritten
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_one(acc_empty + 8 * group);
+                    }
+                    // the label's logit (last: the label has had time to come)
+                    if (B == 0 && (unsigned)(label - j0) < 32u) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (label == j0 + i) h.label_x = x[i];
+                    }
                 }
-            }
-            if (B > 0 && !NETWORK) {
-                if (__any_sync(~0u, waiting > 0)) settle();
             }
             if (a.col_tiles > 1) {
                 // the groups' parts of the row meet where the short lists were: the group whose turn it is collects
@@ -378,46 +462,48 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
                 if (place_no >= 0) {
                     unsigned char* place = pending + (size_t)(place_no * HS_ROWS + r) * MEET_ROW;
                     *reinterpret_cast<float4*>(place) = make_float4(h.m, h.s, h.u, has_label ? h.label_x : 0.f);
+                    if constexpr (B > 0) {
 #pragma unroll
-                    for (int i = 0; i < B; ++i) reinterpret_cast<unsigned long long*>(place + 16)[i] = best.key[i];
+                        for (int i = 0; i < B; ++i) reinterpret_cast<unsigned long long*>(place + 16)[i] = head_key(best.v[i], best.c[i]);
+                    }
                 }
                 named_barrier(1 + NG, NG * 128);
                 if (place_no >= 0) {
                     named_barrier(1 + NG, NG * 128);
                     continue;
                 }
-                label = row_label(a.s, min(row, a.s.n - 1));
                 float label_x = has_label ? h.label_x : 0.f;
+                unsigned long long keys[B > 0 ? B : 1];
+                if constexpr (B > 0) {
+#pragma unroll
+                    for (int i = 0; i < B; ++i) keys[i] = head_key(best.v[i], best.c[i]);
+                }
                 for (int o = 0; o < NG - 1; ++o) {
                     const unsigned char* other = pending + (size_t)(o * HS_ROWS + r) * MEET_ROW;
                     const float4 f = *reinterpret_cast<const float4*>(other);
                     HeadRow oh{f.x, f.y, f.z, 0.f};
                     h.merge(oh, c);
                     label_x += f.w;
-                    if (B > 0) {
-                        unsigned long long k[B > 0 ? B : 1];
+                    if constexpr (B > 0) {
+                        unsigned long long k[B];
 #pragma unroll
                         for (int i = 0; i < B; ++i) k[i] = reinterpret_cast<const unsigned long long*>(other + 16)[i];
-                        merge_keys<(B > 0 ? B : 1)>(best.key, k);
+                        merge_keys<B>(keys, k);
                     }
                 }
+                if constexpr (B > 0) best.from_keys(keys);
                 h.label_x = label_x;
                 named_barrier(1 + NG, NG * 128);           // the place is free
-            } else if (!mine) {
-                continue;
             }
-            if (row >= a.s.n) continue;
             const RowSums sums = row_sums(h.m, h.s, h.u);
-            write_row(a.s, row, sums, label, h.label_x);
-            int32_t* to_class = a.s.top_class + row * a.s.top;
-            float* to_value = a.s.top_logp + row * a.s.top;
-            const bool nan = h.s != h.s;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                if (i < a.s.top) {
-                    const unsigned long long k = best.key[i];
-                    to_class[i] = k && !nan ? (int)(0x7fffffffu - (uint32_t)k) : -1;
-                    to_value[i] = nan ? NAN : (k ? log_prob_of(sums, order_value((uint32_t)(k >> 32)), a.s.inv_t) : -INFINITY);
+            if (row < a.s.n) write_row(a.s, row, sums, label, h.label_x);
+            if constexpr (B > 0) {
+                const bool nan = h.s != h.s, wide = wide_lists(a.s);
+                if (row < a.s.n) {
+                    write_list<B>(a.s.top_class + row * a.s.top, a.s.top, wide, [&](int i) { return nan || best.v[i] == -INFINITY ? -1 : best.c[i]; });
+                    write_list<B>(a.s.top_logp + row * a.s.top, a.s.top, wide, [&](int i) {
+                        return nan ? NAN : (best.v[i] > -INFINITY ? log_prob_of(sums, best.v[i], a.s.inv_t) : -INFINITY);
+                    });
                 }
             }
         }
@@ -432,14 +518,14 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
 }
 
 // shared memory beside the features and W
-static size_t head_extra(int NG, int B, bool network, int N, int col_tiles)
+static size_t head_extra(int NG, int B, int N, int col_tiles)
 {
-    const size_t pending = B && !network ? (size_t)NG * HS_ROWS * HS_PENDING * 8 : 0, meet = col_tiles > 1 ? (size_t)(NG - 1) * HS_ROWS * (16 + B * 8) : 0;
+    const size_t pending = B ? (size_t)NG * 4 * HS_AREA * 4 : 0, meet = col_tiles > 1 ? (size_t)(NG - 1) * HS_ROWS * (16 + B * 8) : 0;
     return (size_t)NG * N * 4 + (pending > meet ? pending : meet) + 8 * (2 * 32 + 2 * 8 + 2 * NG + 1) + 16 + 1024;
 }
 constexpr size_t HS_SMEM = 227 * 1024;
 
-template <int NG, int B, bool NETWORK>
+template <int NG, int B>
 static int launch_head(const void* feat, const void* weight, HeadArgs a, int channels, cudaStream_t stream)
 {
     // Classes of a tile: as many as the accumulators leave, half of it where fewer than four pieces of W would fit beside the features.
@@ -447,7 +533,7 @@ static int launch_head(const void* feat, const void* weight, HeadArgs a, int cha
     size_t room = 0, w_piece = 0;
     for (a.N = a.s.K <= 32 ? 32 : a.s.K <= 64 ? 64 : a.s.K <= 128 ? 128 : NG == 2 ? 256 : 128;; a.N /= 2) {
         a.col_tiles = (a.s.K + a.N - 1) / a.N;
-        room = HS_SMEM - head_extra(NG, B, NETWORK, a.N, a.col_tiles);
+        room = HS_SMEM - head_extra(NG, B, a.N, a.col_tiles);
         w_piece = (size_t)a.N * HS_BK * 2;
         if (a.N <= 128 || x_tile + 4 * w_piece <= room) break;
     }
@@ -465,25 +551,18 @@ static int launch_head(const void* feat, const void* weight, HeadArgs a, int cha
     }
     a.x_stages = a.x_stages > 4 * a.chunks ? 4 * a.chunks : a.x_stages;
     a.x_stages = a.x_stages > 32 ? 32 : a.x_stages;
-    const size_t smem = head_extra(NG, B, NETWORK, a.N, a.col_tiles) + (size_t)a.x_stages * HS_X_BYTES + (a.w_stages ? a.w_stages * w_piece : w_whole);
+    const size_t smem = head_extra(NG, B, a.N, a.col_tiles) + (size_t)a.x_stages * HS_X_BYTES + (a.w_stages ? a.w_stages * w_piece : w_whole);
     CUtensorMap mx, mw;
     int rc = make_tensor_map_bf16(&mx, feat, (uint64_t)a.s.n, (uint64_t)channels, (uint64_t)channels * 2, HS_ROWS, HS_BK);
     if (rc) return rc;
     rc = make_tensor_map_bf16(&mw, weight, (uint64_t)a.s.K, (uint64_t)channels, (uint64_t)channels * 2, (uint32_t)a.N, HS_BK);
     if (rc) return rc;
-    auto kern = head_scores_kernel<NG, B, NETWORK>;
+    auto kern = head_scores_kernel<NG, B>;
     if (allow_smem(kern) != cudaSuccess) return check_launch("ptv3_seg_head_scores_fwd: shared memory attribute");
     const unsigned grid = (unsigned)(a.row_tiles < SMS ? a.row_tiles : SMS);
     launch_dependent(kern, dim3(grid), dim3(64 + NG * 128), smem, stream, mx, mw, a);
     count_launches(1);
     return check_launch("ptv3_seg_head_scores_fwd");
-}
-
-template <int NG, int B>
-static int launch_head_as(const void* feat, const void* weight, HeadArgs a, int channels, cudaStream_t stream)
-{
-    if (B == 0 || a.s.K <= HS_NETWORK) return launch_head<NG, B, true>(feat, weight, a, channels, stream);
-    return launch_head<NG, B, false>(feat, weight, a, channels, stream);
 }
 
 }  // namespace ptv3
@@ -525,12 +604,12 @@ extern "C" int ptv3_seg_head_scores_fwd(const void* feat, const void* weight, co
     a.chunks = (channels + HS_BK - 1) / HS_BK;
     a.last_steps = (channels - (a.chunks - 1) * HS_BK + 15) / 16;
     a.row_tiles = (int)((n + HS_ROWS - 1) / HS_ROWS);
-    // Groups of warps: a thread's best take registers (four groups leave 96 to a thread, three 128), short lists take shared memory
-    // that wide features need for themselves.
+    // Groups of warps: a thread's best take registers (four groups leave 96 to a thread, three 128), the words of
+    // their warps shared memory that wide features need for W.
     const cudaStream_t s = (cudaStream_t)stream;
-    if (top == 0) return launch_head_as<4, 0>(feat, weight, a, channels, s);
-    if (top <= 8 && a.chunks <= 4) return launch_head_as<3, 8>(feat, weight, a, channels, s);
-    if (top <= 8) return launch_head_as<2, 8>(feat, weight, a, channels, s);
-    if (top <= 16) return launch_head_as<2, 16>(feat, weight, a, channels, s);
-    return launch_head_as<2, 32>(feat, weight, a, channels, s);
+    if (top == 0) return launch_head<4, 0>(feat, weight, a, channels, s);
+    if (top <= 8 && a.chunks <= 4) return launch_head<3, 8>(feat, weight, a, channels, s);
+    if (top <= 8) return launch_head<2, 8>(feat, weight, a, channels, s);
+    if (top <= 16) return launch_head<2, 16>(feat, weight, a, channels, s);
+    return launch_head<2, 32>(feat, weight, a, channels, s);
 }

@@ -658,7 +658,7 @@ int ptv3_seg_head_fwd(const void* feat, const void* weight, const void* bias, vo
  * infinity makes its row NaN.
  *   logits         n x classes, PTV3_DTYPE_* dtype, rows ld elements apart (ld >= classes), any alignment of that type
  *   labels         n int32 or int64 (label_bytes 4 or 8), or NULL with log_prob NULL
- *   stats          n x 2 fp32 (8-byte aligned) that _bwd takes, or NULL
+ *   stats          n x 4 fp32 (16-byte aligned) that _bwd takes, or NULL
  *   dlog_prob, dentropy   gradients of the two outputs, their steps apart (0: one value for all rows), or NULL
  *   dtop           n x top gradients of top_log_prob, or NULL
  *   dlogits        n x classes (out), in the logits' type
@@ -669,7 +669,7 @@ int ptv3_class_scores_fwd(const void* logits, int64_t ld, const void* labels, in
                           float* log_prob, float* entropy, float* top_log_prob, int32_t* top_class, float* stats, int64_t n,
                           int classes, int top, float temperature, int dtype, uint32_t* status, void* stream);
 int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void* labels, int label_bytes, int64_t ignore,
-                          const float* entropy, const int32_t* top_class, const float* stats, const float* dlog_prob,
+                          const int32_t* top_class, const float* stats, const float* dlog_prob,
                           int64_t dlog_prob_step, const float* dentropy, int64_t dentropy_step, const float* dtop,
                           void* dlogits, int64_t n, int classes, int top, float temperature, int dtype, void* stream);
 

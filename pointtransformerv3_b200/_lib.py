@@ -3,6 +3,7 @@
 There is no fallback: if the shared library is missing or a call fails, an
 exception is raised."""
 import ctypes
+import importlib.util
 import os
 import struct
 
@@ -143,7 +144,7 @@ SIGNATURES = {
     "ptv3_seg_head_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int, c_int, c_int, c_ptr]),
     "ptv3_class_scores_fwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int,
                                       c_int, c_f32, c_int, c_ptr, c_ptr]),
-    "ptv3_class_scores_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
+    "ptv3_class_scores_bwd": (c_int, [c_ptr, c_i64, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64,
                                       c_ptr, c_ptr, c_i64, c_int, c_int, c_f32, c_int, c_ptr]),
     "ptv3_seg_head_scores_fwd": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_int, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_int,
                                          c_int, c_int, c_f32, c_int, c_ptr, c_ptr]),
@@ -194,6 +195,24 @@ def load():
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_nodes = None
+
+
+def nodes():
+    """The module of autograd nodes (csrc/nodes.cpp)."""
+    global _nodes
+    if _nodes is None:
+        load()
+        path = os.path.join(_HERE, "csrc", "ptv3_nodes.so")
+        if not os.path.exists(path):
+            raise Ptv3Error("%s is not built; run `python -m pointtransformerv3_b200.build`" % path)
+        spec = importlib.util.spec_from_file_location("ptv3_nodes", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _nodes = module
+    return _nodes
 
 
 def check(rc, what):

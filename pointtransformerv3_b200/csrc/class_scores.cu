@@ -325,7 +325,7 @@ struct RowGrad {
 __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, float g_top_sum, bool& none)
 {
     RowGrad r;
-    const float2 st = a.stats[row];
+    const float4 st = a.stats[row];
     none = st.y == -INFINITY;
     r.m = st.x;
     r.c = a.inv_t * LOG2E;
@@ -342,7 +342,7 @@ __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, fl
     }
     const float h = a.g_entropy ? a.g_entropy[row * a.g_entropy_step] : 0.f;
     r.g = g * a.inv_t;
-    r.A = none ? 0.f : (-(g + g_top_sum) - (a.g_entropy ? h * a.entropy[row] : 0.f)) * a.inv_t;
+    r.A = none ? 0.f : (-(g + g_top_sum) - (a.g_entropy ? h * st.z : 0.f)) * a.inv_t;
     r.B = none ? 0.f : -h * a.inv_t * LN2;
     return r;
 }
@@ -515,7 +515,7 @@ extern "C" int ptv3_class_scores_fwd(const void* logits, int64_t ld, const void*
     a.entropy = entropy;
     a.top_logp = top_log_prob;
     a.top_class = top_class;
-    a.stats = (float2*)stats;
+    a.stats = (float4*)stats;
     a.K = classes;
     a.top = top;
     a.inv_t = (float)(1.0 / temperature);
@@ -526,13 +526,13 @@ extern "C" int ptv3_class_scores_fwd(const void* logits, int64_t ld, const void*
     PTV3_REQUIRE(logits && (status || !log_prob) && (entropy || log_prob || top), PTV3_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
     PTV3_REQUIRE(!log_prob || labels, PTV3_ERR_INVALID_ARGUMENT, "%s: log_prob without labels", what);
     PTV3_REQUIRE(top == 0 || (top_log_prob && top_class), PTV3_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-    PTV3_REQUIRE(((uintptr_t)stats & 7) == 0, PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned stats", what);
+    PTV3_REQUIRE(((uintptr_t)stats & 15) == 0, PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned stats", what);
     return dtype == PTV3_DTYPE_F32 ? launch_scores<float>(a, false, (cudaStream_t)stream)
                                    : launch_scores<__nv_bfloat16>(a, false, (cudaStream_t)stream);
 }
 
 extern "C" int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void* labels, int label_bytes, int64_t ignore,
-                                     const float* entropy, const int32_t* top_class, const float* stats,
+                                     const int32_t* top_class, const float* stats,
                                      const float* dlog_prob, int64_t dlog_prob_step, const float* dentropy,
                                      int64_t dentropy_step, const float* dtop, void* dlogits, int64_t n, int classes,
                                      int top, float temperature, int dtype, void* stream)
@@ -546,9 +546,8 @@ extern "C" int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void*
     a.labels = labels;
     a.label_bytes = label_bytes;
     a.ignore = ignore;
-    a.entropy = const_cast<float*>(entropy);
     a.top_class = const_cast<int32_t*>(top_class);
-    a.stats = (float2*)stats;
+    a.stats = (float4*)stats;
     a.K = classes;
     a.top = top;
     a.inv_t = (float)(1.0 / temperature);
@@ -561,9 +560,9 @@ extern "C" int ptv3_class_scores_bwd(const void* logits, int64_t ld, const void*
     const int rc = check_scores(what, a, temperature, dtype);
     if (rc) return rc;
     if (n == 0) return PTV3_OK;
-    PTV3_REQUIRE(logits && stats && dlogits && (!dentropy || entropy) && (!dlog_prob || labels) && (!a.g_top || top_class),
+    PTV3_REQUIRE(logits && stats && dlogits && (!dlog_prob || labels) && (!a.g_top || top_class),
                  PTV3_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-    PTV3_REQUIRE(((uintptr_t)stats & 7) == 0, PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned stats", what);
+    PTV3_REQUIRE(((uintptr_t)stats & 15) == 0, PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned stats", what);
     return dtype == PTV3_DTYPE_F32 ? launch_scores<float>(a, true, (cudaStream_t)stream)
                                    : launch_scores<__nv_bfloat16>(a, true, (cudaStream_t)stream);
 }

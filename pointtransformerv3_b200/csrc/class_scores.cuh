@@ -13,7 +13,7 @@ struct ScoresArgs {
     float *logp, *entropy;   // n
     float* top_logp;         // n x top
     int32_t* top_class;
-    float2* stats;           // n x {m, log S} or NULL
+    float4* stats;           // n x {m, log S, entropy, -} or NULL
     int K, top;
     float inv_t;
     bool wide, wide_out;     // logits, gradient: see RowTile::wide_rows
@@ -61,7 +61,7 @@ __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, cons
         if (label == BAD_LABEL) atomicOr(a.status, PTV3_STATUS_BAD_INDEX);
     }
     if (a.entropy) a.entropy[row] = r.entropy;
-    if (a.stats) a.stats[row] = make_float2(r.m, r.log_s);
+    if (a.stats) a.stats[row] = make_float4(r.m, r.log_s, r.entropy, 0.f);
 }
 
 // A row's alternatives out, get(i) the i-th (i < TOP): as wide as lists are aligned.  (Through shared memory, so that a warp's stores are

@@ -53,7 +53,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device):
     """Makes the tensors' device the current one, where it is another (the guard costs as much as a launch)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _no_tangents(*tensors):
@@ -312,30 +312,6 @@ def _status_word(status, device):
     return ops.new_status(device), True
 
 
-class _ClassScores(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top, temperature, ignore_index, status):
-        out = ops.class_scores_fwd(logits, labels, top, temperature, ignore_index, status, True)
-        log_prob, entropy, values, classes, stats = out
-        ctx.save_for_backward(logits, _kept(labels), entropy, classes, stats)
-        ctx.args = temperature, ignore_index
-        ctx.set_materialize_grads(False)
-        if top:
-            ctx.mark_non_differentiable(classes)
-        return log_prob, entropy, values, classes
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dlog_prob, dentropy, dtop, _):
-        logits, labels, entropy, classes, stats = ctx.saved_tensors
-        if dlog_prob is None and dentropy is None and dtop is None:
-            return (None,) * 6
-        with _on(logits.device):
-            dlogits = ops.class_scores_bwd(logits, labels, entropy, classes, stats, *ctx.args, dlog_prob, dentropy,
-                                           None if dtop is None else dtop.contiguous())
-        return dlogits, None, None, None, None, None
-
-
 def class_log_probs(logits, labels=None, top=0, temperature=1.0, ignore_index=-1, status=None):
     """Log probability of a class, entropy and the best alternatives of every row of logits: ``ClassScores``.
 
@@ -362,31 +338,10 @@ def class_log_probs(logits, labels=None, top=0, temperature=1.0, ignore_index=-1
         own = False
         if labels is not None:
             status, own = _status_word(status, logits.device)
-        logits = _rows(logits)
-        if _wants_grad(logits):
-            out = _ClassScores.apply(logits, labels, *args, status)
-        else:
-            out = ops.class_scores_fwd(logits, labels, *args, status)[:4]
+        out = ops.class_scores(_rows(logits), labels, *args, status)
         if own:
             _lib.raise_on_status(status, "ptv3_class_scores_fwd")
     return ClassScores(*out)
-
-
-class _DistillTopk(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher, classes, temperature, rest, status):
-        loss, stats = ops.distill_topk_fwd(logits, teacher, classes, temperature, rest, status, True)
-        ctx.save_for_backward(logits, _kept(teacher), _kept(classes), stats)
-        ctx.args = temperature, rest
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        logits, teacher, classes, stats = ctx.saved_tensors
-        with _on(logits.device):
-            dlogits = ops.distill_topk_bwd(logits, teacher, classes, stats, *ctx.args, dloss)
-        return dlogits, None, None, None, None, None
 
 
 def distill_topk(logits, teacher, classes, temperature=1.0, rest=False, status=None):
@@ -417,8 +372,7 @@ def distill_topk(logits, teacher, classes, temperature=1.0, rest=False, status=N
         raise ValueError("no gradient goes to the teacher: detach its values")
     with _on(logits.device):
         status, own = _status_word(status, logits.device)
-        args = _rows(logits), teacher.contiguous(), classes, float(temperature), int(bool(rest)), status
-        loss = _DistillTopk.apply(*args) if _wants_grad(logits) else ops.distill_topk_fwd(*args)[0]
+        loss = ops.distill_topk(_rows(logits), teacher.contiguous(), classes, float(temperature), bool(rest), status)
         if own:
             _lib.raise_on_status(status, "ptv3_distill_topk_fwd")
     return loss

@@ -981,36 +981,14 @@ def seg_head(feat, weight, bias=None, want_logits=True, want_labels=True):
     return logits, labels
 
 
-def class_scores_fwd(logits, labels, top, temperature, ignore_index, status, keep=False):
-    """See ptv3_class_scores_fwd; ``functional.class_log_probs`` is the checked form with gradients.  logits (N, K) with rows of
-    neighbouring values -> (log_prob or None, entropy, top_log_probs or None, top_classes or None, stats or None)."""
-    n, K = logits.shape
-    dev, f32 = logits.device, torch.float32
-    log_prob = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
-    entropy = torch.empty(n, dtype=f32, device=dev)
-    values = torch.empty((n, top), dtype=f32, device=dev) if top else None
-    classes = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
-    stats = torch.empty((n, 2), dtype=f32, device=dev) if keep else None
-    with timed("class_scores", n * (K * logits.element_size() + 8.0 * top + 8.0)):
-        _lib.check(_lib.load().ptv3_class_scores_fwd(
-            logits.data_ptr(), logits.stride(0) if n > 1 else K, _lib.ptr(labels), 0 if labels is None else labels.element_size(),
-            ignore_index, _lib.ptr(log_prob), entropy.data_ptr(), _lib.ptr(values), _lib.ptr(classes), _lib.ptr(stats), n, K,
-            top, temperature, _lib.dtype_id(logits), _lib.ptr(status), _lib.stream()), "ptv3_class_scores_fwd")
-    return log_prob, entropy, values, classes, stats
-
-
-def class_scores_bwd(logits, labels, entropy, classes, stats, temperature, ignore_index, dlog_prob, dentropy, dtop):
-    """Gradient of the logits (N, K); gradients of outputs that nothing used are None."""
-    n, K = logits.shape
-    dlogits = torch.empty((n, K), dtype=logits.dtype, device=logits.device)
-    with timed("class_scores_bwd", n * (2.0 * K * logits.element_size() + 16.0)):
-        _lib.check(_lib.load().ptv3_class_scores_bwd(
-            logits.data_ptr(), logits.stride(0) if n > 1 else K, _lib.ptr(labels), 0 if labels is None else labels.element_size(),
-            ignore_index, entropy.data_ptr(), _lib.ptr(classes), stats.data_ptr(), _lib.ptr(dlog_prob),
-            0 if dlog_prob is None else dlog_prob.stride(0), _lib.ptr(dentropy), 0 if dentropy is None else dentropy.stride(0),
-            _lib.ptr(dtop), dlogits.data_ptr(), n, K, 0 if classes is None else classes.shape[1], temperature,
-            _lib.dtype_id(logits), _lib.stream()), "ptv3_class_scores_bwd")
-    return dlogits
+def class_scores(logits, labels, top, temperature, ignore_index, status):
+    """ptv3_class_scores_fwd with its gradient; ``functional.class_log_probs`` is the checked form.  logits (N, K) with rows of neighbouring
+    values -> (log_prob or None, entropy, top_log_probs or None, top_classes or None)."""
+    call = _lib.nodes().class_scores
+    if TIMERS is None:           # (short calls are bounded by the host)
+        return call(logits, labels, top, temperature, ignore_index, status)
+    with timed("class_scores", logits.shape[0] * (logits.shape[1] * logits.element_size() + 8.0 * top + 8.0)):
+        return call(logits, labels, top, temperature, ignore_index, status)
 
 
 def head_scores_supported(channels, top, dtype):
@@ -1039,49 +1017,29 @@ def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=
     labels = _check_labels(labels, n, top, ignore_index)
     if not head_scores_supported(C, top, feat.dtype):
         raise ValueError("%d channels (a multiple of 8 up to 512), %d alternatives (up to 32)" % (C, top))
-    dev, f32 = feat.device, torch.float32
+    dev = feat.device
     with _on(dev):
         status, own = _status_word(status, dev)
         feat, weight = _aligned(feat), _aligned(weight)
         bias = None if bias is None else bias.contiguous()
-        log_prob = torch.empty(n, dtype=f32, device=dev) if labels is not None else None
-        entropy = torch.empty(n, dtype=f32, device=dev)
-        values = torch.empty((n, top), dtype=f32, device=dev) if top else None
-        classes = torch.empty((n, top), dtype=torch.int32, device=dev) if top else None
-        with timed("seg_head_log_probs", 2.0 * n * C * K):
-            _lib.check(_lib.load().ptv3_seg_head_scores_fwd(
-                feat.data_ptr(), weight.data_ptr(), _lib.ptr(bias), _lib.ptr(labels), 0 if labels is None else labels.element_size(),
-                int(ignore_index), _lib.ptr(log_prob), entropy.data_ptr(), _lib.ptr(values), _lib.ptr(classes), n, C, K, int(top),
-                float(temperature), _lib.dtype_id(feat), status.data_ptr(), _lib.stream()), "ptv3_seg_head_scores_fwd")
+        args = feat, weight, bias, labels, int(top), float(temperature), int(ignore_index), status
+        if TIMERS is None:
+            out = _lib.nodes().seg_head_scores(*args)
+        else:
+            with timed("seg_head_log_probs", 2.0 * n * C * K):
+                out = _lib.nodes().seg_head_scores(*args)
         if own:
             _lib.raise_on_status(status, "ptv3_seg_head_scores_fwd")
-    return ClassScores(log_prob, entropy, values, classes)
+    return ClassScores(*out)
 
 
-def distill_topk_fwd(logits, teacher, classes, temperature, rest, status, keep=False):
-    """See ptv3_distill_topk_fwd; ``functional.distill_topk`` is the checked form with gradients.  -> (loss (N,), stats or None)."""
-    n, K = logits.shape
-    loss = torch.empty(n, dtype=torch.float32, device=logits.device)
-    stats = torch.empty((n, 4), dtype=torch.float32, device=logits.device) if keep else None
-    k = classes.shape[1]
-    with timed("distill_topk", n * (K * logits.element_size() + 8.0 * k + 4.0)):
-        _lib.check(_lib.load().ptv3_distill_topk_fwd(
-            logits.data_ptr(), logits.stride(0) if n > 1 else K, teacher.data_ptr(), _lib.dtype_id(teacher), classes.data_ptr(),
-            classes.element_size(), k, loss.data_ptr(), _lib.ptr(stats), n, K, temperature, rest, _lib.dtype_id(logits),
-            status.data_ptr(), _lib.stream()), "ptv3_distill_topk_fwd")
-    return loss, stats
-
-
-def distill_topk_bwd(logits, teacher, classes, stats, temperature, rest, dloss):
-    """Gradient of the logits (N, K)."""
-    n, K = logits.shape
-    dlogits = torch.empty((n, K), dtype=logits.dtype, device=logits.device)
-    with timed("distill_topk_bwd", n * (2.0 * K * logits.element_size() + 8.0 * classes.shape[1] + 20.0)):
-        _lib.check(_lib.load().ptv3_distill_topk_bwd(
-            logits.data_ptr(), logits.stride(0) if n > 1 else K, teacher.data_ptr(), _lib.dtype_id(teacher), classes.data_ptr(),
-            classes.element_size(), classes.shape[1], stats.data_ptr(), dloss.data_ptr(), dloss.stride(0), dlogits.data_ptr(), n,
-            K, temperature, rest, _lib.dtype_id(logits), _lib.stream()), "ptv3_distill_topk_bwd")
-    return dlogits
+def distill_topk(logits, teacher, classes, temperature, rest, status):
+    """ptv3_distill_topk_fwd with its gradient; ``functional.distill_topk`` is the checked form.  -> loss (N,)."""
+    call = _lib.nodes().distill_topk
+    if TIMERS is None:
+        return call(logits, teacher, classes, temperature, rest, status)
+    with timed("distill_topk", logits.shape[0] * (logits.shape[1] * logits.element_size() + 8.0 * classes.shape[1] + 4.0)):
+        return call(logits, teacher, classes, temperature, rest, status)
 
 
 def pool_stage_supported(c_in, c_out, dtype):

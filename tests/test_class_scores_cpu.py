@@ -94,9 +94,9 @@ def scores_fwd(logits=ROWS, ld=20, labels=ROWS, label_bytes=8, ignore=-1, log_pr
                                              temperature, dtype, status, None)
 
 
-def scores_bwd(logits=ROWS, ld=20, labels=ROWS, label_bytes=8, entropy=ROWS, classes=ROWS, stats=ROWS, g=ROWS, h=ROWS, t=ROWS,
+def scores_bwd(logits=ROWS, ld=20, labels=ROWS, label_bytes=8, classes=ROWS, stats=ROWS, g=ROWS, h=ROWS, t=ROWS,
                dlogits=ROWS, n=4, K=20, top=3, temperature=1.0, dtype=0):
-    return _lib.load().ptv3_class_scores_bwd(logits, ld, labels, label_bytes, -1, entropy, classes, stats, g, 1, h, 1, t, dlogits, n, K, top,
+    return _lib.load().ptv3_class_scores_bwd(logits, ld, labels, label_bytes, -1, classes, stats, g, 1, h, 1, t, dlogits, n, K, top,
                                              temperature, dtype, None)
 
 
@@ -116,7 +116,7 @@ SHARED = [dict(n=-1), dict(n=2 ** 31), dict(dtype=2), dict(K=0), dict(K=2 ** 18 
 REFUSED = {
     scores_fwd: SHARED + [dict(top=-1), dict(top=65), dict(label_bytes=2), dict(labels=None), dict(values=None), dict(classes=None),
                           dict(status=None), dict(stats=ROWS + 4), dict(dtype=1, logits=ROWS + 1)],
-    scores_bwd: SHARED + [dict(top=65), dict(stats=None), dict(dlogits=None), dict(entropy=None), dict(labels=None), dict(classes=None),
+    scores_bwd: SHARED + [dict(top=65), dict(stats=None), dict(dlogits=None), dict(labels=None), dict(classes=None), dict(stats=ROWS + 8),
                           dict(dlogits=ROWS + 2), dict(label_bytes=1)],
     distill_fwd: SHARED + [dict(k=0), dict(k=65), dict(teacher_dtype=2), dict(size=2), dict(teacher=None), dict(classes=None), dict(loss=None),
                            dict(status=None), dict(teacher=ROWS + 2), dict(classes=ROWS + 4, size=8), dict(stats=ROWS + 8)],

@@ -354,6 +354,7 @@ struct RowValues {
             for (int i = 0; i < P; ++i)
                 if (i * G + rank < pieces.pieces) f(x[i], pieces.first(i * G + rank), i);
         } else {
+#pragma unroll 2
             for (int p = rank; p < pieces.pieces; p += G) f(pieces.load(p), pieces.first(p), p / G);
         }
         if (pieces.edges) {
@@ -535,13 +536,21 @@ struct RowTile {
     }
 };
 
+// Blocks of these that an SM has at least: 64 registers of a thread for up to 32 words of a row, 102 for 64 (alternatives of 4 099 x 8 192
+// fp32: 53 us with the 168 that the compiler would take, 40 so).
+template <typename T>
+constexpr int row_blocks(int G, int P)
+{
+    return P * Eight<T>::WORDS <= 32 ? (G <= 128 ? 8 : 1) : (G <= 128 ? 5 : G <= 256 ? 2 : 1);
+}
 // Threads of a row and pieces of each.  A thread holds up to 128 bf16 or 64 fp32 logits in 64 registers, all of them on the way at once:
 // that, not many warps, is what keeps memory busy, and one warp to a row waits for no barrier.  Short rows take part of a warp, so
 // that what is done once for a row is done for several at a time.
 template <int N> struct Const { static constexpr int value = N; };
 template <typename T, typename F>
-static inline void for_row_shape(int K, bool warps, F&& f)
+static inline void for_row_shape(int K, bool warps, bool once, F&& f)
 {
+    // (once: the row is passed over once, so that the longest need not be held: 1 500 x 20 001 backward 57 us held, 40 read as they are needed)
     constexpr int P = sizeof(T) == 2 ? 8 : 4;
     if (K <= 8 * 8 * P && warps)
         K <= 256 ? f(Const<32>(), Const<1>()) : f(Const<32>(), Const<2>());
@@ -557,6 +566,8 @@ static inline void for_row_shape(int K, bool warps, F&& f)
         f(Const<32>(), Const<2 * P>());
     else if (K <= 128 * 16 * P)
         f(Const<128>(), Const<2 * P>());
+    else if (once)
+        f(Const<256>(), Const<0>());
     else if (K <= 256 * 16 * P)
         f(Const<256>(), Const<2 * P>());
     else if (K <= 512 * 16 * P)

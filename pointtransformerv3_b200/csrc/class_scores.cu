@@ -271,7 +271,7 @@ __device__ __forceinline__ void alternatives(const ScoresArgs& a, int64_t row, c
 }
 
 template <typename T, int G, int P, bool TOPS>
-__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) scores_row_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_row_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     __shared__ TopScratch<TOPS ? G : 32> top_scratch[TOPS ? Group<G>::ROWS : 1];
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
 }
 
 template <typename T, int G, int P>
-__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) scores_row_bwd_kernel(const ScoresArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_row_bwd_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     const Group<G> group{scratch};
@@ -475,7 +475,7 @@ static int launch_scores(ScoresArgs a, bool backward, cudaStream_t stream)
         if (!launch_tile_of<T>(a, backward, stream)) return check_launch("ptv3_class_scores: shared memory attribute");
     } else {
         // (where alternatives are chosen, a warp at least)
-        for_row_shape<T>(a.K, !backward && a.top, [&](auto g, auto p) { launch_row<T, decltype(g)::value, decltype(p)::value>(a, backward, stream); });
+        for_row_shape<T>(a.K, !backward && a.top, backward, [&](auto g, auto p) { launch_row<T, decltype(g)::value, decltype(p)::value>(a, backward, stream); });
     }
     count_launches(1);
     return check_launch(what);

@@ -236,7 +236,7 @@ struct ListPart {
 __host__ __device__ __forceinline__ int bit_words(int K) { return (K + 31) / 32 + 1; }
 
 template <typename T, int G, int P>
-__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) distill_row_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_row_kernel(const DistillArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     extern __shared__ uint32_t bits_s[];
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
 }
 
 template <typename T, int G, int P>
-__global__ void __launch_bounds__(Group<G>::BLOCK, G <= 32 && P * Eight<T>::WORDS <= 32 ? 8 : 1) distill_row_bwd_kernel(const DistillArgs a)
+__global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_row_bwd_kernel(const DistillArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
     __shared__ __align__(16) int list_c[Group<G>::ROWS][LIST_MAX];
@@ -569,7 +569,7 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
         if (!ok) return check_launch("ptv3_distill_topk: shared memory attribute");
     } else {
         // (a list over 8 threads at least)
-        for_row_shape<T>(a.K, false, [&](auto g, auto p) {
+        for_row_shape<T>(a.K, false, backward, [&](auto g, auto p) {
             constexpr int G = decltype(g)::value, P = decltype(p)::value;
             launch_row<T, (G < 8 ? 8 : G), (G < 8 ? P / 2 : P)>(a, backward, stream);
         });

@@ -37,7 +37,7 @@ __device__ __forceinline__ RowSums row_sums(float m, float s, float u)
     r.m = row_origin(m);
     r.none = s == 0.f;
     r.log_s = r.none ? -INFINITY : log1pf(s - 1.f);
-    r.entropy = r.none ? 0.f : r.log_s - __fdiv_rn(u * LN2, s);
+    r.entropy = r.none ? 0.f : r.log_s - __fdividef(u * LN2, s);
     return r;
 }
 __device__ __forceinline__ float log_prob_of(const RowSums& r, float x, float inv_t)

@@ -592,7 +592,8 @@ static int run_distill(const char* what, DistillArgs& a, int teacher_dtype, floa
     PTV3_REQUIRE(a.list_bytes == 4 || a.list_bytes == 8, PTV3_ERR_INVALID_ARGUMENT, "%s: classes of %d bytes", what, a.list_bytes);
     const int size = dtype == PTV3_DTYPE_F32 ? 4 : 2, tsize = teacher_dtype == PTV3_DTYPE_F32 ? 4 : 2;
     PTV3_REQUIRE((uintptr_t)a.logits % size == 0 && (uintptr_t)a.dlogits % size == 0 && (uintptr_t)a.teacher % tsize == 0 &&
-                     (uintptr_t)a.list % a.list_bytes == 0 && (uintptr_t)a.stats % 16 == 0,
+                     (uintptr_t)a.list % a.list_bytes == 0 && (uintptr_t)a.stats % 16 == 0 &&
+                     (((uintptr_t)a.loss | (uintptr_t)a.g | (uintptr_t)a.status) & 3) == 0,
                  PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned tensor", what);
     a.inv_t = (float)(1.0 / temperature);
     a.teacher_bf16 = teacher_dtype == PTV3_DTYPE_BF16;

@@ -191,7 +191,7 @@ struct Best<0> {
 
 // Of 32 logits behind n, 32 k / n are better than the k-th best on average.  One costs 5 B operations in a warp and the row with most of them
 // decides, the network 28 B and the merge 20 B: from 8 B on one after another is cheaper (100 003 x 64 to 1 201 classes with 16: 506 us with the network
-// alone, @ so).
+// alone, 282 so).
 constexpr int HS_FEW = 8;
 
 // a row's running answers
@@ -336,7 +336,9 @@ __global__ void __launch_bounds__(64 + NG * 128, 1) head_scores_kernel(const __g
                     const uint64_t dw = dw0 + (uint64_t)(a.w_stages ? ws : t * a.chunks + k) * (w_bytes >> 4);
                     const int steps = k == a.chunks - 1 ? a.last_steps : HS_BK / 16;
                     if (elect_one()) {
-                        for (int q = 0; q < steps; ++q) umma_bf16(tmem + g * a.N, dx + 2 * q, dw + 2 * q, idesc, k > 0 || q > 0);
+#pragma unroll
+                        for (int q = 0; q < HS_BK / 16; ++q)
+                            if (q < steps) umma_bf16(tmem + g * a.N, dx + 2 * q, dw + 2 * q, idesc, k > 0 || q > 0);
                         if (a.w_stages) umma_commit(w_empty + 8 * ws);
                         if (t == a.col_tiles - 1) umma_commit(x_empty + 8 * x_at);
                         if (k == a.chunks - 1) umma_commit(acc_full + 8 * g);
@@ -625,6 +627,9 @@ extern "C" int ptv3_seg_head_scores_fwd(const void* feat, const void* weight, co
                  PTV3_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
     PTV3_REQUIRE((((uintptr_t)feat | (uintptr_t)weight) & 15) == 0 && ((uintptr_t)bias & 1) == 0, PTV3_ERR_INVALID_ARGUMENT,
                  "%s: features and weights must be 16-byte aligned", what);
+    PTV3_REQUIRE((((uintptr_t)log_prob | (uintptr_t)entropy | (uintptr_t)top_log_prob | (uintptr_t)top_class | (uintptr_t)status) & 3) == 0 &&
+                     (!labels || (uintptr_t)labels % label_bytes == 0),
+                 PTV3_ERR_INVALID_ARGUMENT, "%s: unaligned labels or outputs", what);
     HeadArgs a{};
     a.s.n = n;
     a.s.labels = log_prob ? labels : nullptr;

@@ -999,9 +999,10 @@ def head_scores_supported(channels, top, dtype):
 def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=1.0, ignore_index=-1, status=None):
     """``functional.class_log_probs`` of feat (N, C) @ weight (K, C)^T + bias (K,) without the logits, which are fp32 on the way: log
     probability of ``labels``, entropy, alternatives (``functional.ClassScores``).  bf16, C a multiple of 8 up to 512, K up to 262 144, top up to
-    32, no gradients.  A masked class (a bias of minus infinity) is no alternative.  status: a device status word of the caller's; without
+    32.  Without gradients, and refused where they are wanted.  A masked class (a bias of minus infinity) is no alternative.  status: a device status word of the caller's; without
     one the call checks for itself and waits for the device."""
-    from .functional import CLASSES_MAX, ClassScores, TEMPERATURES, _aligned, _check_labels, _on, _same_device, _status_word
+    from .functional import (CLASSES_MAX, ClassScores, TEMPERATURES, _aligned, _check_labels, _no_tangents, _on, _same_device, _status_word,
+                             _wants_grad)
     _same_device(feat, weight, bias, labels, status)
     if feat.dim() != 2 or weight.dim() != 2 or weight.shape[1] != feat.shape[1] or not 1 <= weight.shape[0] <= CLASSES_MAX:
         raise ValueError("features (N, C) and weights (1 to %d classes, C), got %s and %s" % (
@@ -1014,6 +1015,9 @@ def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=
         raise ValueError("features, weights and bias must be bf16")
     if not TEMPERATURES[0] <= temperature <= TEMPERATURES[1]:
         raise ValueError("temperature %r, not within %g to %g" % (temperature, *TEMPERATURES))
+    if _wants_grad(feat, weight, bias):
+        raise ValueError("no gradients go through this call: SegHead.log_probs, or a Linear and functional.class_log_probs")
+    _no_tangents(feat, weight, bias)
     labels = _check_labels(labels, n, top, ignore_index)
     if not head_scores_supported(C, top, feat.dtype):
         raise ValueError("%d channels (a multiple of 8 up to 512), %d alternatives (up to 32)" % (C, top))

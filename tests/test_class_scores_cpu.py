@@ -111,15 +111,26 @@ def distill_bwd(logits=ROWS, ld=20, teacher=ROWS, classes=ROWS, size=4, k=3, sta
     return _lib.load().ptv3_distill_topk_bwd(logits, ld, teacher, 0, classes, size, k, stats, g, 1, dlogits, n, K, temperature, rest, dtype, None)
 
 
+def head(feat=ROWS, weight=ROWS, bias=ROWS, labels=ROWS, label_bytes=8, log_prob=ROWS, entropy=ROWS, values=ROWS, classes=ROWS, n=4, C=64, K=20,
+         top=3, temperature=1.0, dtype=1, status=WORD):
+    return _lib.load().ptv3_seg_head_scores_fwd(feat, weight, bias, labels, label_bytes, -1, log_prob, entropy, values, classes, n, C, K, top,
+                                                temperature, dtype, status, None)
+
+
 SHARED = [dict(n=-1), dict(n=2 ** 31), dict(dtype=2), dict(K=0), dict(K=2 ** 18 + 1, ld=2 ** 19), dict(ld=19), dict(temperature=0.0),
           dict(temperature=-1.0), dict(temperature=math.nan), dict(temperature=math.inf), dict(logits=None), dict(logits=ROWS + 2)]
 REFUSED = {
     scores_fwd: SHARED + [dict(top=-1), dict(top=65), dict(label_bytes=2), dict(labels=None), dict(values=None), dict(classes=None),
-                          dict(status=None), dict(stats=ROWS + 4), dict(dtype=1, logits=ROWS + 1)],
+                          dict(status=None), dict(stats=ROWS + 4), dict(dtype=1, logits=ROWS + 1), dict(labels=ROWS + 4), dict(values=ROWS + 2),
+                          dict(entropy=ROWS + 1)],
     scores_bwd: SHARED + [dict(top=65), dict(stats=None), dict(dlogits=None), dict(labels=None), dict(classes=None), dict(stats=ROWS + 8),
-                          dict(dlogits=ROWS + 2), dict(label_bytes=1)],
+                          dict(dlogits=ROWS + 2), dict(label_bytes=1), dict(g=ROWS + 2), dict(labels=ROWS + 2, label_bytes=4)],
     distill_fwd: SHARED + [dict(k=0), dict(k=65), dict(teacher_dtype=2), dict(size=2), dict(teacher=None), dict(classes=None), dict(loss=None),
-                           dict(status=None), dict(teacher=ROWS + 2), dict(classes=ROWS + 4, size=8), dict(stats=ROWS + 8)],
+                           dict(status=None), dict(teacher=ROWS + 2), dict(classes=ROWS + 4, size=8), dict(stats=ROWS + 8), dict(loss=ROWS + 2)],
+    head: [dict(n=-1), dict(n=2 ** 31 - 1), dict(dtype=0), dict(K=0), dict(K=2 ** 18 + 1), dict(C=0), dict(C=60), dict(C=520), dict(top=-1),
+           dict(top=33), dict(temperature=0.0), dict(temperature=math.nan), dict(label_bytes=2), dict(labels=None), dict(feat=None),
+           dict(weight=None), dict(entropy=None), dict(values=None), dict(classes=None), dict(status=None), dict(feat=ROWS + 8),
+           dict(weight=ROWS + 2), dict(bias=ROWS + 1), dict(labels=ROWS + 4), dict(entropy=ROWS + 2)],
     distill_bwd: SHARED + [dict(k=0), dict(stats=None), dict(g=None), dict(dlogits=None), dict(dlogits=ROWS + 2)],
 }
 

@@ -55,6 +55,12 @@ def test_numbers_of_classes(K):
         check(*made(300, 64, K, K + top), labels_of(300, K, K, torch.int32 if K % 2 else torch.int64), top, (1.0, 0.5, 3.0)[K % 3])
 
 
+@pytest.mark.parametrize("C,K", [(8, 20000), (64, 20000), (512, 9001), (64, F.CLASSES_MAX)])
+def test_long_lists_of_classes(C, K):
+    for top in (0, 7, 16, 32):
+        check(*made(70, C, K, top), labels_of(70, K), top)
+
+
 @pytest.mark.parametrize("C", [8, 16, 24, 56, 64, 72, 96, 128, 200, 256, 264, 384, 448, 512])
 def test_numbers_of_channels(C):
     for K, top in ((20, 5), (150, 8), (700, 16), (700, 2), (260, 0), (260, 32)):
@@ -197,6 +203,13 @@ def test_refusals():
             ops.seg_head_log_probs(*args, **kw)
     with pytest.raises(_lib.Ptv3Error, match="CUDA"):
         ops.seg_head_log_probs(feat, weight.cpu(), bias)
+    for t in (feat, weight, bias):
+        t.requires_grad_()
+        with pytest.raises(ValueError, match="gradients"):
+            ops.seg_head_log_probs(feat, weight, bias)
+        with torch.no_grad():
+            assert not ops.seg_head_log_probs(feat, weight, bias).entropy.requires_grad
+        t.requires_grad_(False)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])

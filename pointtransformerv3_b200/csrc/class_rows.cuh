@@ -106,7 +106,8 @@ template <> struct Eight<float> {
 };
 
 constexpr float NO_POWER = -200.f;
-// S and U = sum e t of a row, in packed pairs
+// S and, where they are wanted (U), sum e t of a row, in packed pairs
+template <bool U>
 struct RowSum {
     uint64_t s, u;
     __device__ __forceinline__ void clear() { s = u = 0; }
@@ -117,25 +118,29 @@ struct RowSum {
         for (int q = 0; q < 4; ++q) {
             float lo, hi;
             unpack2(mul2(add2(x.pair(q), minus_origin), c), lo, hi);
-            lo = max_nan(lo, NO_POWER);
-            hi = max_nan(hi, NO_POWER);
+            if (U) {
+                lo = max_nan(lo, NO_POWER);
+                hi = max_nan(hi, NO_POWER);
+            }
             const uint64_t e = pack2(fast_exp2(lo), fast_exp2(hi));
             s = add2(s, e);
-            u = fma2(e, pack2(lo, hi), u);
+            if (U) u = fma2(e, pack2(lo, hi), u);
         }
     }
 };
-// Eight of a gradient: p (A + B t) with p = 2^t, t = (x - m) c + shift = log2 p
-template <typename T>
+// Eight of a gradient: p (A + B t) with p = 2^t, t = (x - m) c + shift = log2 p; without LOG, p A
+template <bool LOG, typename T>
 __device__ __forceinline__ void row_gradient(Eight<T>& x, uint64_t minus_m, uint64_t c, uint64_t shift, uint64_t A, uint64_t B)
 {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         float lo, hi;
         unpack2(fma2(add2(x.pair(q), minus_m), c, shift), lo, hi);
-        lo = max_nan(lo, NO_POWER);
-        hi = max_nan(hi, NO_POWER);
-        unpack2(mul2(pack2(fast_exp2(lo), fast_exp2(hi)), fma2(pack2(lo, hi), B, A)), lo, hi);
+        if (LOG) {
+            lo = max_nan(lo, NO_POWER);
+            hi = max_nan(hi, NO_POWER);
+        }
+        unpack2(mul2(pack2(fast_exp2(lo), fast_exp2(hi)), LOG ? fma2(pack2(lo, hi), B, A) : A), lo, hi);
         x.set(q, lo, hi);
     }
 }
@@ -369,7 +374,7 @@ struct EdgeSum {
     float s, u;
     __device__ __forceinline__ void add(float x, float origin, float c)
     {
-        const float t = max_nan((x - origin) * c, NO_POWER), e = fast_exp2(t);
+        const float t = max_nan((x - origin) * c, NO_POWER), e = fast_exp2(t);       // (few: both, always)
         s += e;
         u = fmaf(e, t, u);
     }

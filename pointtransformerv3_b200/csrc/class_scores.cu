@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
     }
     const float origin = row_origin(m);
     const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
-    RowSum sums;
+    RowSum<true> sums;
     sums.clear();
     each([&](const Eight<T>& e, int) { sums.add(e, minus, c2); });
     const RowSums r = row_sums(m, hsum2(sums.s), hsum2(sums.u));
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_r
     const float mine = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
     const float m = group.max(mine), origin = row_origin(m);
     const uint64_t c2 = pack2(a.inv_t * LOG2E, a.inv_t * LOG2E), minus = pack2(-origin, -origin);
-    RowSum sums;
+    RowSum<true> sums;
     sums.clear();
     EdgeSum edge{0.f, 0.f};
     vals.each([&](const Eight<T>& x, int, int) { sums.add(x, minus, c2); }, [&](float x, int, int) { edge.add(x, origin, a.inv_t * LOG2E); });
@@ -343,10 +343,11 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_r
 struct RowGrad {
     float m, c, shift, A, B, g, inv_t;      // A, B, g: with 1 / T in them; B for a logarithm of base 2
     int label;
-    template <typename T>
+    // LOG: with a gradient of the entropy
+    template <bool LOG, typename T>
     __device__ __forceinline__ void eight(Eight<T>& x) const
     {
-        row_gradient(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(A, A), pack2(B, B));
+        row_gradient<LOG>(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(A, A), pack2(B, B));
     }
     // one class, with the part of its own
     __device__ __forceinline__ float at(float x, int j, float own) const
@@ -380,7 +381,7 @@ __device__ __forceinline__ RowGrad row_grad(const ScoresArgs& a, int64_t row, fl
     return r;
 }
 
-template <typename T, int W>
+template <typename T, int W, bool LOG>
 __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a)
 {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
         const T label = r.label >= 0 ? from_f<T>(r.at(to_f<T>(x[r.label]), r.label, 0.f)) : from_f<T>(0.f);
         for (int j = 0; j < a.K; j += 8) {
             Eight<T> e = tile.template read<W>(x, j);
-            r.eight(e);
+            r.eight<LOG>(e);
             tile.template write<W>(x, j, e);
         }
         if (r.label >= 0) x[r.label] = label;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(128) scores_tile_bwd_kernel(const ScoresArgs a
     tile.store((T*)a.dlogits, row0, rows, a.wide_out);
 }
 
-template <typename T, int G, int P>
+template <typename T, int G, int P, bool LOG>
 __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_row_bwd_kernel(const ScoresArgs a)
 {
     __shared__ float scratch[4 * Group<G>::WARPS];
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) scores_r
     const float label_x = r.label >= 0 ? to_f<T>(x[r.label]) : 0.f;       // (on the way with the row)
     if (live)
         vals.each([&](Eight<T> e, int j, int) {
-            r.eight(e);
+            r.eight<LOG>(e);
             pieces.store(dx, alike, j, e);
         }, [&](float e, int j, int) { dx[j] = from_f<T>(r.at(e, j, 0.f)); });
     // classes with parts of their own once more: the label, then the alternatives (of which the label may be one)
@@ -464,7 +465,7 @@ static bool launch_tile(const ScoresArgs& a, bool backward, cudaStream_t stream)
         kern<<<blocks, shape.rows, shape.smem, stream>>>(a);
         return true;
     };
-    if (backward) return run(scores_tile_bwd_kernel<T, W>);
+    if (backward) return a.g_entropy ? run(scores_tile_bwd_kernel<T, W, true>) : run(scores_tile_bwd_kernel<T, W, false>);
     // (kept in registers a row is read once: 407 678 x 20 with 5 alternatives 16.5 us read twice, 15.8 so)
     const bool few = a.K <= 32;
     if (a.top == 0) return few ? run(scores_tile_kernel<T, W, 0, true>) : run(scores_tile_kernel<T, W, 0, false>);
@@ -490,7 +491,8 @@ template <typename T, int G, int P>
 static void launch_row(const ScoresArgs& a, bool backward, cudaStream_t stream)
 {
     if (backward)
-        scores_row_bwd_kernel<T, G, P><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
+        a.g_entropy ? scores_row_bwd_kernel<T, G, P, true><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a)
+                    : scores_row_bwd_kernel<T, G, P, false><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
     else if constexpr (G >= 32)
         a.top ? scores_row_kernel<T, G, P, true><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a)
               : scores_row_kernel<T, G, P, false><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
             x[cls] = from_f<T>(-INFINITY);
         });
     const uint64_t c2 = pack2(c, c), minus = pack2(-origin, -origin);
-    RowSum sums;
+    RowSum<false> sums;
     sums.clear();
     for (int j = 0; j < a.K; j += 8) sums.add(tile.template read<W>(x, j), minus, c2);
     const float outside = hsum2(sums.s), s = outside + inside;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
         log_out = log_outside(outside, [&]() {
             const float om = tile.template largest<W>(x);
             if (om == -INFINITY) return -INFINITY;
-            RowSum again;
+            RowSum<false> again;
             again.clear();
             const uint64_t mo = pack2(-om, -om);
             for (int j = 0; j < a.K; j += 8) again.add(tile.template read<W>(x, j), mo, c2);
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         }
         return o;
     };
-    RowSum sums;
+    RowSum<false> sums;
     sums.clear();
     EdgeSum edge{0.f, 0.f};
     float inside = 0.f;
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
                       [&](float e, int j, int) { om = max_nan(om, is_listed(j) ? -INFINITY : e); });
             om = group.max(om);
             const float from = row_origin(om);
-            RowSum again;
+            RowSum<false> again;
             again.clear();
             const uint64_t mo = pack2(-from, -from);
             EdgeSum at_edge{0.f, 0.f};
@@ -375,7 +375,7 @@ struct DistillGrad {
     template <typename T>
     __device__ __forceinline__ void eight(Eight<T>& x) const
     {
-        row_gradient(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(factor, factor), 0ull);
+        row_gradient<false>(x, pack2(-m, -m), pack2(c, c), pack2(shift, shift), pack2(factor, factor), 0ull);
     }
     __device__ __forceinline__ float outside(float x) const { return fast_exp2(max_nan(fmaf(x - m, c, shift), NO_POWER)) * factor; }
     // M p of a class in the list

@@ -150,37 +150,91 @@ struct DistillTopk : torch::autograd::Function<DistillTopk> {
 
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// ---- arguments as they ordinarily are: what needs no copy, no message and no read of a status word -------------------------------------
+bool logits_are_plain(const Tensor& t)
+{
+    return t.is_cuda() && t.dim() == 2 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) && t.size(0) > 1 && t.size(1) >= 1 &&
+           t.size(1) <= 1 << 18 && t.stride(1) == 1 && t.stride(0) >= t.size(1);
+}
+bool is_plain(const Tensor& t, const Tensor& like, bool type) { return type && t.device() == like.device() && t.is_contiguous(); }
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+bool status_is_plain(const Tensor& t, const Tensor& like) { return is_plain(t, like, t.scalar_type() == at::kInt) && t.numel() > 0; }
+bool temperature_is_plain(double t) { return t >= 1e-6 && t <= 1e6; }
+
+using Given = std::optional<Tensor>;
+using Answers = std::tuple<Given, Given, Given, Given>;
+
+// -> log_prob (None without labels), entropy, the alternatives' values and classes (None with top = 0)
+Answers class_scores(const Tensor& logits, const Given& labels, int64_t top, double temperature, int64_t ignore, const Given& status)
+{
+    const c10::DeviceGuard guard(logits.device());
+    if (!wants_grad(logits))
+        return run_class_scores(logits, labels.value_or(Tensor()), top, temperature, ignore, status.value_or(Tensor()), Tensor()).all();
+    const variable_list out = ClassScores::apply(logits, labels, top, temperature, ignore, status);
+    const size_t at = labels ? 2 : 1;
+    return {labels ? Given(out[1]) : Given(), out[0], top ? Given(out[at]) : Given(), top ? Given(out[at + 1]) : Given()};
+}
+Tensor distill_topk(const Tensor& logits, const Tensor& teacher, const Tensor& classes, double temperature, bool rest, const Tensor& status)
+{
+    const c10::DeviceGuard guard(logits.device());
+    if (!wants_grad(logits)) return run_distill(logits, teacher, classes, temperature, rest, status, Tensor());
+    return DistillTopk::apply(logits, teacher, classes, temperature, rest, status);
+}
+Answers seg_head_scores(const Tensor& feat, const Tensor& weight, const Given& bias, const Given& given_labels, int64_t top, double temperature,
+                        int64_t ignore, const Tensor& status)
+{
+    const c10::DeviceGuard guard(feat.device());
+    const Tensor labels = given_labels.value_or(Tensor());
+    const Scores s(feat, labels.defined(), top);
+    check(ptv3_seg_head_scores_fwd(feat.data_ptr(), weight.data_ptr(), pointer(bias.value_or(Tensor())), pointer(labels),
+                                   labels.defined() ? (int)labels.element_size() : 0, ignore, (float*)pointer(s.log_prob),
+                                   (float*)pointer(s.entropy), (float*)pointer(s.values), (int32_t*)pointer(s.classes), feat.size(0),
+                                   (int)feat.size(1), (int)weight.size(0), (int)top, (float)temperature, dtype_of(feat),
+                                   (uint32_t*)status.data_ptr(), stream_of(feat)),
+          "ptv3_seg_head_scores_fwd");
+    return s.all();
+}
+bool labels_are_plain(const Given& labels, const Tensor& rows)
+{
+    return !labels || (labels->dim() == 1 && labels->size(0) == rows.size(0) && is_plain(*labels, rows, is_index(*labels)));
+}
+
 }  // namespace
 
+// The functions whose names begin with plain_ return None where an argument is not as ordinary ones are; functional.py and ops.py then check them
+// one by one.
 PYBIND11_MODULE(ptv3_nodes, m)
 {
-    using Given = std::optional<Tensor>;
-    // -> log_prob (None without labels), entropy, the alternatives' values and classes (None with top = 0)
-    m.def("class_scores", [](const Tensor& logits, const Given& labels, int64_t top, double temperature, int64_t ignore, const Given& status) {
-        const c10::DeviceGuard guard(logits.device());
-        if (!wants_grad(logits))
-            return run_class_scores(logits, labels.value_or(Tensor()), top, temperature, ignore, status.value_or(Tensor()), Tensor()).all();
-        const variable_list out = ClassScores::apply(logits, labels, top, temperature, ignore, status);
-        const size_t at = labels ? 2 : 1;
-        return std::tuple<Given, Given, Given, Given>{labels ? Given(out[1]) : Given(), out[0], top ? Given(out[at]) : Given(),
-                                                      top ? Given(out[at + 1]) : Given()};
+    m.def("class_scores", &class_scores);
+    m.def("distill_topk", &distill_topk);
+    m.def("seg_head_scores", &seg_head_scores);
+    m.def("plain_class_scores", [](const Tensor& logits, const Given& labels, int64_t top, double temperature, int64_t ignore,
+                                   const Given& status) -> std::optional<Answers> {
+        if (!logits_are_plain(logits) || !labels_are_plain(labels, logits) || top < 0 || top > 64 || !temperature_is_plain(temperature) ||
+            (labels && !(status && status_is_plain(*status, logits))))
+            return std::nullopt;
+        return class_scores(logits, labels, top, temperature, ignore, status);
     });
-    m.def("distill_topk", [](const Tensor& logits, const Tensor& teacher, const Tensor& classes, double temperature, bool rest, const Tensor& status) {
-        const c10::DeviceGuard guard(logits.device());
-        if (!wants_grad(logits)) return run_distill(logits, teacher, classes, temperature, rest, status, Tensor());
-        return DistillTopk::apply(logits, teacher, classes, temperature, rest, status);
+    m.def("plain_distill_topk", [](const Tensor& logits, const Tensor& teacher, const Tensor& classes, double temperature, bool rest,
+                                   const Given& status) -> Given {
+        if (!logits_are_plain(logits) || classes.dim() != 2 || classes.size(0) != logits.size(0) || classes.size(1) < 1 || classes.size(1) > 64 ||
+            !is_plain(classes, logits, is_index(classes)) || teacher.sizes() != classes.sizes() || wants_grad(teacher) ||
+            !is_plain(teacher, logits, teacher.scalar_type() == at::kFloat || teacher.scalar_type() == at::kBFloat16) ||
+            !temperature_is_plain(temperature) || !status || !status_is_plain(*status, logits))
+            return std::nullopt;
+        return distill_topk(logits, teacher, classes, temperature, rest, *status);
     });
-    m.def("seg_head_scores", [](const Tensor& feat, const Tensor& weight, const Given& bias, const Given& given_labels, int64_t top, double temperature,
-                                int64_t ignore, const Tensor& status) {
-        const c10::DeviceGuard guard(feat.device());
-        const Tensor labels = given_labels.value_or(Tensor());
-        const Scores s(feat, labels.defined(), top);
-        check(ptv3_seg_head_scores_fwd(feat.data_ptr(), weight.data_ptr(), pointer(bias.value_or(Tensor())), pointer(labels),
-                                       labels.defined() ? (int)labels.element_size() : 0, ignore, (float*)pointer(s.log_prob),
-                                       (float*)pointer(s.entropy), (float*)pointer(s.values), (int32_t*)pointer(s.classes), feat.size(0),
-                                       (int)feat.size(1), (int)weight.size(0), (int)top, (float)temperature, dtype_of(feat),
-                                       (uint32_t*)status.data_ptr(), stream_of(feat)),
-              "ptv3_seg_head_scores_fwd");
-        return s.all();
+    m.def("plain_seg_head_scores", [](const Tensor& feat, const Tensor& weight, const Given& bias, const Given& labels, int64_t top, double temperature,
+                                      int64_t ignore, const Given& status) -> std::optional<Answers> {
+        auto bf16 = [&](const Tensor& t, int64_t dim, bool wide) {
+            return t.dim() == dim && is_plain(t, feat, t.scalar_type() == at::kBFloat16) && !wants_grad(t) &&
+                   (!wide || ((uintptr_t)t.data_ptr() & 15) == 0);
+        };
+        if (!feat.is_cuda() || !bf16(feat, 2, true) || !bf16(weight, 2, true) || weight.size(1) != feat.size(1) || weight.size(0) < 1 ||
+            weight.size(0) > 1 << 18 || (bias && !(bf16(*bias, 1, false) && bias->size(0) == weight.size(0))) || feat.size(1) % 8 ||
+            feat.size(1) < 8 || feat.size(1) > 512 || !labels_are_plain(labels, feat) || top < 0 || top > PTV3_HEAD_TOP_MAX ||
+            !temperature_is_plain(temperature) || !status || !status_is_plain(*status, feat))
+            return std::nullopt;
+        return seg_head_scores(feat, weight, bias, labels, top, temperature, ignore, *status);
     });
 }

@@ -271,6 +271,17 @@ TEMPERATURES = (1e-6, 1e6)
 ClassScores = collections.namedtuple("ClassScores", "log_prob entropy top_log_probs top_classes")
 
 
+def _try(call, *args):
+    """A call as it is, in one step (the host bounds short ones), unless something is timed or differentiated forward.  None where an argument is
+    not as ordinary ones are: the caller then looks at them one by one."""
+    if ops.TIMERS is not None or forward_ad._current_level >= 0:
+        return None
+    try:
+        return getattr(_lib.nodes(), call)(*args)
+    except TypeError:            # arguments that are no tensors or numbers
+        return None
+
+
 def _rows(logits):
     """Rows of neighbouring values, any distance apart."""
     n, K = logits.shape
@@ -329,6 +340,9 @@ def class_log_probs(logits, labels=None, top=0, temperature=1.0, ignore_index=-1
     NaN, and nothing of them goes into the gradient); the caller checks it when the host next waits.  Without one a call with labels checks
     for itself and waits for the device.
     Gradients: logits, from log_prob, entropy and top_log_probs."""
+    out = _try("plain_class_scores", logits, labels, top, temperature, ignore_index, status)
+    if out is not None:
+        return ClassScores(*out)
     _same_device(logits, labels, status)
     _no_tangents(logits)
     _check_logits(logits, temperature)
@@ -359,6 +373,9 @@ def distill_topk(logits, teacher, classes, temperature=1.0, rest=False, status=N
 
     status: as for ``class_log_probs``; it reports classes out of range (the row's loss is NaN, its gradient leaves the entry out).
     Gradients: logits.  The teacher's values are constants, and refused where they ask for a gradient."""
+    loss = _try("plain_distill_topk", logits, teacher, classes, temperature, rest, status)
+    if loss is not None:
+        return loss
     _same_device(logits, teacher, classes, status)
     _no_tangents(logits, teacher)
     _check_logits(logits, temperature)

@@ -1002,7 +1002,10 @@ def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=
     32.  Without gradients, and refused where they are wanted.  A masked class (a bias of minus infinity) is no alternative.  status: a device status word of the caller's; without
     one the call checks for itself and waits for the device."""
     from .functional import (CLASSES_MAX, ClassScores, TEMPERATURES, _aligned, _check_labels, _no_tangents, _on, _same_device, _status_word,
-                             _wants_grad)
+                             _try, _wants_grad)
+    out = _try("plain_seg_head_scores", feat, weight, bias, labels, top, temperature, ignore_index, status)
+    if out is not None:
+        return ClassScores(*out)
     _same_device(feat, weight, bias, labels, status)
     if feat.dim() != 2 or weight.dim() != 2 or weight.shape[1] != feat.shape[1] or not 1 <= weight.shape[0] <= CLASSES_MAX:
         raise ValueError("features (N, C) and weights (1 to %d classes, C), got %s and %s" % (

@@ -38,9 +38,6 @@ __device__ __forceinline__ int list_class(const DistillArgs& a, int64_t i)
     return c >= 0 && c < a.K ? (int)c : (c == -1 ? PLACE_ABSENT : PLACE_BAD);
 }
 
-// t log t - t log p of an entry; nothing where t is 0
-__device__ __forceinline__ float entry_loss(float t, float log_t, float log_p) { return t == 0.f ? 0.f : t * (log_t - log_p); }
-
 // t_r = 1 - sum t: of one large and other small entries the large one's part is taken by expm1
 __device__ __forceinline__ float rest_prob(float top, float others) { return fmaxf(-expm1f(fminf(top, 0.f)) - others, 0.f); }
 
@@ -49,25 +46,25 @@ __device__ __forceinline__ float entry_weight(const DistillArgs& a, float v, flo
 {
     return a.rest ? fast_exp2(v * LOG2E) : fast_exp2(below_max(v, row_origin(top)) * (a.inv_t * LOG2E));
 }
-constexpr float GAP_SCALE = 1.f / LIST_MAX;
-// What a row's list adds up to.  With w the entries' weights (t itself, or t times their sum), z = d / T the student's and l the teacher's
-// logits at the temperature (v, or (v - top) / T), the list's part of the loss is  sum w (l - z) / W + log S - log W  for W = sum w.
+// What a row's list adds up to: weights w (t itself, or t times their sum W), the largest value.
 struct ListSums {
-    float top;         // the largest value
-    float sum;         // W
-    float others;      // without the largest
-    float gap;         // sum w (l - z), the terms of w = 0 left out; without a rest a 64th of it (W may be 64, l - z the largest number)
-    __device__ __forceinline__ float loss(bool rest, float log_s) const
-    {
-        if (rest) return sum == 0.f ? 0.f : fmaf(sum, log_s, gap);
-        return sum > 0.f ? __fdiv_rn(gap, sum * GAP_SCALE) + log_s - logf(sum) : sum;      // (NaN stays)
-    }
+    float top, sum, others;      // others: W without the largest
 };
-// log of a sum of the outside's exponentials; `again` takes it from its own maximum
-template <typename F>
-__device__ __forceinline__ float log_outside(float sum, F&& again)
+// t (log t - log p) of an entry.  The three logarithms are subtracted from one another entry by entry, and not as sums over the list: near a student
+// that has learnt its teacher they nearly cancel.  z: the student's logit from the origin, at the temperature
+__device__ __forceinline__ float entry_term(const DistillArgs& a, float w, float scale, float log_sum, float v, float top, float z, float log_s)
 {
-    return sum >= REST_TOO_SMALL ? logf(sum) : again();
+    const float log_t = a.rest ? v : below_max(v, row_origin(top)) * a.inv_t - log_sum;
+    return w == 0.f ? 0.f : w * scale * (log_t - (z - log_s));
+}
+// t_r (log t_r - log p_r).  Both are taken from what is missing to 1 where that is the smaller part, as the list's share is for p_r = outside /
+// (outside + inside); far_log: log p_r of an outside that had to be summed from its own maximum, or 0
+__device__ __forceinline__ float rest_term(float t_r, float list_sum, float inside, float outside, float far_log)
+{
+    if (t_r == 0.f) return 0.f;
+    const float log_t = list_sum < 0.5f ? log1pf(-list_sum) : logf(t_r);
+    const float log_p = far_log != 0.f ? far_log : -log1pf(__fdividef(inside, outside));
+    return t_r * (log_t - log_p);
 }
 
 // ---- short rows: a tile of rows, one thread to a row ---------------------------------------------------------------
@@ -153,12 +150,12 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
 
     const float m = tile.template largest<W>(x), origin = row_origin(m), c = a.inv_t * LOG2E;
     bool any = false;
-    ListSums l{-INFINITY, 0.f, 0.f, 0.f};
+    ListSums l{-INFINITY, 0.f, 0.f};
     if (!a.rest) list.each([&](int, int, float v) { l.top = max_nan(l.top, v); });
-    float most = 0.f, inside = 0.f;
-    list.each([&](int, int cls, float v) {
+    float most = 0.f, inside = 0.f, z[N > 0 ? N : 1];
+    list.each([&](int i, int cls, float v) {
         any = true;
-        const float w = entry_weight(a, v, l.top), d = to_f<T>(x[cls]) - origin;
+        const float w = entry_weight(a, v, l.top);
         l.sum += w;
         if (a.rest) {
             const bool up = v > l.top;
@@ -166,7 +163,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
             most = up ? w : most;
             l.top = up ? v : l.top;
         }
-        if (w != 0.f) l.gap = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(l.top)) * a.inv_t) - d * a.inv_t, l.gap);
+        if (N > 0) z[N > 0 ? i : 0] = (to_f<T>(x[cls]) - origin) * a.inv_t;
     });
     if (a.rest)
         list.each([&](int, int cls, float) {
@@ -180,21 +177,32 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     const float outside = hsum2(sums.s), s = outside + inside;
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
-    float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
+    const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdividef(1.f, l.sum) : l.sum), log_sum = a.rest || !(l.sum > 0.f) ? 0.f : log1pf(l.sum - 1.f);
+    const T* logits = (const T*)a.logits + row * a.ld;
+    float loss = 0.f, log_out = -INFINITY, t_r = 0.f;
+    list.each([&](int i, int cls, float v) {
+        const float zi = N > 0 ? z[N > 0 ? i : 0] : (to_f<T>(logits[cls]) - origin) * a.inv_t;
+        loss += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, zi, log_s);
+    });
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
-        log_out = log_outside(outside, [&]() {
+        float far_log = 0.f;
+        if (outside >= REST_TOO_SMALL) {
+            log_out = logf(outside);
+        } else {
             const float om = tile.template largest<W>(x);
-            if (om == -INFINITY) return -INFINITY;
-            RowSum<false> again;
-            again.clear();
-            const uint64_t mo = pack2(-om, -om);
-            for (int j = 0; j < a.K; j += 8) again.add(tile.template read<W>(x, j), mo, c2);
-            return (om - origin) * a.inv_t + logf(hsum2(again.s));
-        });
+            if (om != -INFINITY) {
+                RowSum<false> again;
+                again.clear();
+                const uint64_t mo = pack2(-om, -om);
+                for (int j = 0; j < a.K; j += 8) again.add(tile.template read<W>(x, j), mo, c2);
+                log_out = (om - origin) * a.inv_t + logf(hsum2(again.s));
+                far_log = log_out - log_s;
+            }
+        }
         if (any && log_out != -INFINITY) {
             t_r = rest_prob(l.top, l.others);
-            loss += entry_loss(t_r, logf(t_r), log_out - log_s);
+            loss += rest_term(t_r, l.sum, inside, outside, far_log);
         }
     }
     if (list.bad()) {
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     a.loss[row] = loss;
     if (a.stats)
         a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
-                              : make_float4(origin, log_s, row_origin(l.top), l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
+                              : make_float4(origin, log_s, row_origin(l.top), scale);
 }
 
 // ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------
@@ -305,32 +313,40 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
     for (int q = 0; q < ListPart<G>::N; ++q)
         if (q * G < a.k) top = max_nan(top, list.v[q]);
     top = group.max(top);
-    // the row's (or the outside's) sum; weights, their gap; entries, and from 128 on those out of range
-    float all[4] = {hsum2(sums.s) + edge.s, 0.f, 0.f, 0.f};
-    // with an outcome for the rest: the inside's sum, weights but the largest's, entries that are as large as the largest
-    float more[3] = {inside, 0.f, 0.f};
+    // the row's (or the outside's) sum; weights; entries, and from 128 on those out of range; the inside's sum
+    float all[4] = {hsum2(sums.s) + edge.s, 0.f, 0.f, inside};
+    // with an outcome for the rest: weights but the largest's, entries that are as large as the largest
+    float more[2] = {0.f, 0.f}, w[ListPart<G>::N];
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
-        if (q * G >= a.k) break;
-        all[3] += list.cls[q] == PLACE_BAD ? 128.f : 0.f;
+        w[q] = 0.f;
+        if (q * G >= a.k) continue;
+        all[2] += list.cls[q] == PLACE_BAD ? 128.f : 0.f;
         if (list.cls[q] < 0) continue;
-        all[3] += 1.f;
-        const float v = list.v[q], w = entry_weight(a, v, top), d = x_of[q] - origin;
-        all[1] += w;
-        if (w != 0.f) all[2] = fmaf(a.rest ? w : w * GAP_SCALE, (a.rest ? v : below_max(v, row_origin(top)) * a.inv_t) - d * a.inv_t, all[2]);
-        more[1] += v == top ? 0.f : w;
-        more[2] += v == top ? 1.f : 0.f;
+        all[2] += 1.f;
+        w[q] = entry_weight(a, list.v[q], top);
+        all[1] += w[q];
+        more[0] += list.v[q] == top ? 0.f : w[q];
+        more[1] += list.v[q] == top ? 1.f : 0.f;
     }
     group.sum(all);
     if (a.rest) group.sum(more);
-    const bool bad = all[3] >= 128.f, any = all[3] != 0.f && all[3] != 128.f * (int)(all[3] / 128.f);
-    const float s = all[0] + (a.rest ? more[0] : 0.f);
+    const bool bad = all[2] >= 128.f, any = all[2] != 0.f && all[2] != 128.f * (int)(all[2] / 128.f);
+    const float s = all[0] + all[3];
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
-    ListSums l{top, all[1], more[1] + fmaxf(more[2] - 1.f, 0.f) * fast_exp2(top * LOG2E), all[2]};
-    float loss = l.loss(a.rest, log_s), log_out = -INFINITY, t_r = 0.f;
+    const ListSums l{top, all[1], more[0] + fmaxf(more[1] - 1.f, 0.f) * fast_exp2(top * LOG2E)};
+    const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdividef(1.f, l.sum) : l.sum), log_sum = a.rest || !(l.sum > 0.f) ? 0.f : log1pf(l.sum - 1.f);
+    float terms[1] = {0.f};
+#pragma unroll
+    for (int q = 0; q < ListPart<G>::N; ++q)
+        if (q * G < a.k && list.cls[q] >= 0)
+            terms[0] += entry_term(a, w[q], scale, log_sum, list.v[q], top, (x_of[q] - origin) * a.inv_t, log_s);
+    group.sum(terms);
+    float loss = terms[0], log_out = -INFINITY, t_r = 0.f;
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
+        float far_log = 0.f;
         // (taken by all rows of a warp where one needs it)
         const bool low = !(all[0] >= REST_TOO_SMALL);
         if (G < 32 ? __any_sync(~0u, low) : low) {
@@ -347,12 +363,18 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
                       [&](float e, int j, int) { at_edge.add(is_listed(j) ? -INFINITY : e, from, c); });
             float o[1] = {hsum2(again.s) + at_edge.s};
             group.sum(o);
-            if (om != -INFINITY) log_out = (om - origin) * a.inv_t + logf(o[0]);
+            if (om != -INFINITY) {
+                log_out = (om - origin) * a.inv_t + logf(o[0]);
+                far_log = log_out - log_s;
+            }
         }
-        if (!low) log_out = logf(all[0]);
+        if (!low) {
+            log_out = logf(all[0]);
+            far_log = 0.f;
+        }
         if (any && log_out != -INFINITY) {
             t_r = rest_prob(l.top, l.others);
-            loss += entry_loss(t_r, logf(t_r), log_out - log_s);
+            loss += rest_term(t_r, l.sum, all[3], all[0], far_log);
         }
     }
     if (me == 0 && live) {
@@ -363,7 +385,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         a.loss[row] = loss;
         if (a.stats)
             a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
-                                  : make_float4(origin, log_s, row_origin(top), l.sum > 0.f ? __fdiv_rn(1.f, l.sum) : l.sum);
+                                  : make_float4(origin, log_s, row_origin(top), scale);
     }
 }
 

@@ -23,7 +23,7 @@ struct DistillArgs {
     bool teacher_bf16, list4;     // list4: see RowList
     bool wide, wide_out;          // logits, gradient: see RowTile::wide_rows
     float* loss;              // n
-    float4* stats;            // n x {m, log S, log of the outside's sum or the list's largest, t_r or 1 / the list's sum}, or NULL
+    float4* stats;            // n x {m, log S, log of the outside's sum or the list's largest, M p_r - t_r or 1 / the list's sum}, or NULL
     float inv_t;
     uint32_t* status;
     const float* g;           // n, g_step apart
@@ -57,15 +57,24 @@ __device__ __forceinline__ float entry_term(const DistillArgs& a, float w, float
     const float log_t = a.rest ? v : below_max(v, row_origin(top)) * a.inv_t - log_sum;
     return w == 0.f ? 0.f : w * scale * (log_t - (z - log_s));
 }
-// t_r (log t_r - log p_r).  Both are taken from what is missing to 1 where that is the smaller part, as the list's share is for p_r = outside /
-// (outside + inside); far_log: log p_r of an outside that had to be summed from its own maximum, or 0
-__device__ __forceinline__ float rest_term(float t_r, float list_sum, float inside, float outside, float far_log)
-{
-    if (t_r == 0.f) return 0.f;
-    const float log_t = list_sum < 0.5f ? log1pf(-list_sum) : logf(t_r);
-    const float log_p = far_log != 0.f ? far_log : -log1pf(__fdividef(inside, outside));
-    return t_r * (log_t - log_p);
-}
+// The outcome for the rest, from the teacher's t_r, the list's sum and the student's sums inside and outside (far_log: log p_r of an outside that had
+// to be summed from its own maximum, or 0).  What is near 1 is taken from what is missing to it: a list that holds a hundredth of both
+// teacher and student leaves differences of hundredths.
+struct Rest {
+    float term;          // t_r (log t_r - log p_r)
+    float surplus;       // M p_r - t_r = W - M (1 - p_r)
+    float log_out;       // log of the outside's sum
+    __device__ __forceinline__ Rest(float t_r, float W, float inside, float outside, float far_log, float log_s)
+    {
+        const float M = W + t_r, p_in = __fdividef(inside, inside + outside);
+        const bool small = p_in < 0.5f;
+        const float log_p = far_log != 0.f ? far_log : (small ? log1pf(-p_in) : -log1pf(__fdividef(inside, outside)));
+        const float log_t = W < 0.5f ? log1pf(-W) : logf(t_r);
+        term = t_r == 0.f ? 0.f : t_r * (log_t - log_p);
+        surplus = small ? W - M * p_in : M * fast_exp2(log_p * LOG2E) - t_r;
+        log_out = log_s + log_p;
+    }
+};
 
 // ---- short rows: a tile of rows, one thread to a row ---------------------------------------------------------------
 // A row's list in its thread's registers (N entries; N = 0: longer ones are read again from memory wherever they are walked).
@@ -179,7 +188,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
     const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdividef(1.f, l.sum) : l.sum), log_sum = a.rest || !(l.sum > 0.f) ? 0.f : log1pf(l.sum - 1.f);
     const T* logits = (const T*)a.logits + row * a.ld;
-    float loss = 0.f, log_out = -INFINITY, t_r = 0.f;
+    float loss = 0.f, log_out = -INFINITY, surplus = 0.f;
     list.each([&](int i, int cls, float v) {
         const float zi = N > 0 ? z[N > 0 ? i : 0] : (to_f<T>(logits[cls]) - origin) * a.inv_t;
         loss += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, zi, log_s);
@@ -187,22 +196,24 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
         float far_log = 0.f;
-        if (outside >= REST_TOO_SMALL) {
-            log_out = logf(outside);
-        } else {
+        bool open = outside >= REST_TOO_SMALL || outside != outside;
+        if (!open) {
             const float om = tile.template largest<W>(x);
-            if (om != -INFINITY) {
+            open = om != -INFINITY;
+            if (open) {
                 RowSum<false> again;
                 again.clear();
                 const uint64_t mo = pack2(-om, -om);
                 for (int j = 0; j < a.K; j += 8) again.add(tile.template read<W>(x, j), mo, c2);
-                log_out = (om - origin) * a.inv_t + logf(hsum2(again.s));
-                far_log = log_out - log_s;
+                far_log = (om - origin) * a.inv_t + logf(hsum2(again.s)) - log_s;
             }
         }
-        if (any && log_out != -INFINITY) {
-            t_r = rest_prob(l.top, l.others);
-            loss += rest_term(t_r, l.sum, inside, outside, far_log);
+        if (open) {
+            const float t_r = any ? rest_prob(l.top, l.others) : 0.f;
+            const Rest r(t_r, l.sum, inside, outside, far_log, log_s);
+            loss += r.term;
+            log_out = r.log_out;
+            surplus = r.surplus;
         }
     }
     if (list.bad()) {
@@ -211,7 +222,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     }
     a.loss[row] = loss;
     if (a.stats)
-        a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
+        a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, surplus)
                               : make_float4(origin, log_s, row_origin(l.top), scale);
 }
 
@@ -343,12 +354,13 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         if (q * G < a.k && list.cls[q] >= 0)
             terms[0] += entry_term(a, w[q], scale, log_sum, list.v[q], top, (x_of[q] - origin) * a.inv_t, log_s);
     group.sum(terms);
-    float loss = terms[0], log_out = -INFINITY, t_r = 0.f;
+    float loss = terms[0], log_out = -INFINITY, surplus = 0.f;
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
         float far_log = 0.f;
         // (taken by all rows of a warp where one needs it)
-        const bool low = !(all[0] >= REST_TOO_SMALL);
+        const bool low = all[0] < REST_TOO_SMALL;
+        bool open = true;
         if (G < 32 ? __any_sync(~0u, low) : low) {
             float om = -INFINITY;
             vals.each([&](const Eight<T>& e, int j, int) { om = max_nan(om, masked(e, j).largest()); },
@@ -363,18 +375,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
                       [&](float e, int j, int) { at_edge.add(is_listed(j) ? -INFINITY : e, from, c); });
             float o[1] = {hsum2(again.s) + at_edge.s};
             group.sum(o);
-            if (om != -INFINITY) {
-                log_out = (om - origin) * a.inv_t + logf(o[0]);
-                far_log = log_out - log_s;
+            if (low) {
+                open = om != -INFINITY;
+                if (open) far_log = (om - origin) * a.inv_t + logf(o[0]) - log_s;
             }
         }
-        if (!low) {
-            log_out = logf(all[0]);
-            far_log = 0.f;
-        }
-        if (any && log_out != -INFINITY) {
-            t_r = rest_prob(l.top, l.others);
-            loss += rest_term(t_r, l.sum, all[3], all[0], far_log);
+        if (open) {
+            const float t_r = any ? rest_prob(l.top, l.others) : 0.f;
+            const Rest r(t_r, l.sum, all[3], all[0], far_log, log_s);
+            loss += r.term;
+            log_out = r.log_out;
+            surplus = r.surplus;
         }
     }
     if (me == 0 && live) {
@@ -384,7 +395,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         }
         a.loss[row] = loss;
         if (a.stats)
-            a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, t_r)
+            a.stats[row] = a.rest ? make_float4(origin, log_s, log_out, surplus)
                                   : make_float4(origin, log_s, row_origin(top), scale);
     }
 }
@@ -418,11 +429,10 @@ __device__ __forceinline__ DistillGrad distill_grad(const DistillArgs& a, int64_
     r.inside_shift = r.shift = -log_s * LOG2E;
     r.inside_factor = r.factor = mass * r.g;
     if (a.rest && st.z != -INFINITY) {
-        // p_j / p_r (M p_r - t_r)
-        const float M = mass + st.w;
-        r.inside_factor = M * r.g;
+        // p_j / p_r (M p_r - t_r);  M = W + max(0, 1 - W)
+        r.inside_factor = max_nan(mass, 1.f) * r.g;
         r.shift = r.none ? -INFINITY : -st.z * LOG2E;
-        r.factor = r.g * (M * fast_exp2((st.z - log_s) * LOG2E) - st.w);
+        r.factor = r.g * st.w;
     }
     return r;
 }

@@ -114,9 +114,9 @@ def distill(logits, teacher, classes, temperature=1.0, rest=False, upstream=None
         s = torch.exp(z).sum(1, keepdim=True)
         log_t = torch.where(s == 0, -INF, z - torch.log(s))
     t = torch.exp(log_t)
-    lt = torch.where(t > 0, log_t, 0.0)
+    lt = torch.where(t == 0, 0.0, log_t)
     lp = logp.gather(1, at)
-    part = torch.where(t > 0, t * (lt - lp), 0.0)
+    part = torch.where(t == 0, 0.0, t * (lt - lp))
     loss = part.sum(1)
     t_tol = t * ((k + 12) * U + 4 * U * lt.abs())
     lp_fin = torch.where(lp == -INF, 0.0, lp)

@@ -98,6 +98,7 @@ def test_lists_beyond_the_ordinary(K, rest):
     values[13] = torch.finfo(torch.float32).min
     values[14, 3], classes[14, 3] = math.nan, -1          # what an absent entry holds is not read
     classes[15, :5] = -1
+    values[16, 2] = math.nan                              # what a present one holds is
     for dtype in DTYPES:
         for temperature in (1.0, 2.0):
             check(normal(n, K, seed=5, scale=2.0, dtype=dtype), values, classes, temperature, rest)
@@ -129,6 +130,21 @@ def test_students_beyond_the_ordinary(K, rest, dtype):
     x[14] = torch.where(inside[14], x[14] + 40.0, x[14])  # about where the sum is taken again
     x[15] = torch.where(inside[15], x[15] + 46.0, x[15])
     check(x.to(dtype), values, classes, 1.0, rest)
+
+
+@pytest.mark.parametrize("K", [30, 400, 3000])
+def test_lists_that_hold_little(K):
+    """Flat teachers and students: the list's share and the rest's differences are small beside 1, and lose nothing to it."""
+    n = 64
+    x, t = normal(n, K, seed=1) / 30, normal(n, K, seed=2) / 30
+    out = F.class_log_probs(t, top=4)
+    for a, b in ((out.top_log_probs, out.top_classes), (out.top_log_probs[:, :1], out.top_classes[:, :1])):
+        check(x, a, b, rest=True)
+        loss = F.distill_topk(x, a, b, rest=True)
+        want = R.distill(x, a, b, 1.0, True, normal(n, seed=77))
+        # the terms of a few hundredths of a flat list: a dozen roundings of the largest of them
+        size = (a.double().exp() * (a.double() - torch.log_softmax(x.double(), 1).gather(1, b.long())).abs()).sum(1)
+        assert ((loss.double() - want["loss"][0]).abs() <= 12 * 2.0 ** -22 * (size + a.double().exp().sum(1))).all()
 
 
 @pytest.mark.parametrize("K", [20, 100, 1100])

@@ -62,12 +62,6 @@ template <> struct Eight<__nv_bfloat16> {
         for (int i = 0; i < 8; ++i)
             if (i >= count) w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | 0xff800000u : (w[i >> 1] & 0xffff0000u) | 0xff80u;
     }
-    __device__ __forceinline__ void drop_first(int count)
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | 0xff800000u : (w[i >> 1] & 0xffff0000u) | 0xff80u;
-    }
     __device__ __forceinline__ float largest() const            // NaN if one is
     {
         __nv_bfloat162 a = __hmax2_nan(h(0), h(1)), b = __hmax2_nan(h(2), h(3));
@@ -87,12 +81,6 @@ template <> struct Eight<float> {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i >= count) w[i] = 0xff800000u;
-    }
-    __device__ __forceinline__ void drop_first(int count)
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < count) w[i] = 0xff800000u;
     }
     __device__ __forceinline__ float largest() const
     {

@@ -111,12 +111,13 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
 }
 
 // ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------------------
-// A thread keeps P pieces of eight logits in registers; rows beyond G x 32 logits are read again for every pass (P = 0).
+// A thread keeps P pieces of eight logits in registers; the longest rows are read again for every pass (P = 0).
 //
-// The alternatives.  Every thread has the largest of each of two parts of its logits (of four for more than 32 alternatives); their k-th
-// largest, found one after another by the upper 16 bits of their keys, bounds the row's k-th largest from below.  The few logits at or above
-// the bound (less than twice k of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of
-// few values), the best are taken one after another, each a maximum over the row of what comes behind the last one.
+// The alternatives.  A row's logits fall into 64 parts (128 for more than 32 alternatives), of which the largest are known: two or four of each
+// lane where a warp has the row, one of neighbouring threads together where a block has it.  Their k-th largest, by the upper 16 bits of their
+// keys, bounds the row's k-th largest from below; a warp takes its parts one after another, a block counts.  The few logits at or above the
+// bound (less than twice k of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of few
+// values), the best are taken one after another, each a maximum over the row of what comes behind the last one.
 constexpr int CANDIDATES = 192;
 
 // value and class as one number, below ~0 (NaN of class 0); 0 for none

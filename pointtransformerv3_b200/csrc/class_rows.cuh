@@ -240,6 +240,13 @@ struct Group {
         else
             __syncthreads();
     }
+    // whether it holds for any of the row's threads, which meet here
+    __device__ __forceinline__ bool any(bool v) const
+    {
+        if (G > 32) return __syncthreads_or(v);
+        const uint32_t all = __ballot_sync(~0u, v);
+        return ((G < 32 ? all >> (threadIdx.x & (32 - G) & 31) & ((1u << (G & 31)) - 1) : all)) != 0;
+    }
     __device__ __forceinline__ float max(float v) const
     {
 #pragma unroll
@@ -574,8 +581,10 @@ struct TileShape {
     int rows;
     size_t smem;
 };
-// rows beyond are spread over threads: those of which the best are asked for, and the others
-constexpr size_t TILE_TOP_BYTES = 512, TILE_PLAIN_BYTES = 128;
+// Rows in tiles or spread over threads.  A thread to a row costs the fewest instructions but wants a tile of 128 rows for every SM (many_rows), and
+// fewer tiles are resident the longer rows are.  Each operator has the bytes up to which that pays, with both sides measured.
+constexpr size_t TILE_BYTES = 128;          // always
+constexpr bool many_rows(int64_t n) { return n >= (int64_t)SMS * 128; }
 template <typename T>
 static inline TileShape tile_shape(int K)
 {

@@ -501,15 +501,28 @@ static void launch_row(const ScoresArgs& a, bool backward, cudaStream_t stream)
         scores_row_kernel<T, G, P, false><<<Group<G>::blocks(a.n), Group<G>::BLOCK, 0, stream>>>(a);
 }
 
+// Sums and gradients: 200 000 x 72 bf16 15.5 and 23.1 us spread, 9.5 and 14.4 in tiles; x 128 16.9 and 29.0, 16.8 and 27.4; x 200 20.5 and 38.0, 24.4 and
+// 43.3.  Alternatives, up to 32 of a thread's: few rows of more than 256 bytes finish sooner spread (2 000 x 200 bf16 with 8: 8.7 us in tiles, 4.3), but
+// for many of them; many are slower so up to 1 024 bytes of bf16 or 704 of fp32, where keys have 64 bits (60 000 x 333 bf16 with 8 and 32: 65.5 and 154 us
+// spread, 37.0 and 52.6 in tiles; x 500 65.8 and 138, 56.5 and 74.0; x 166 fp32 53.2 and 422, 41.6 and 78.0; x 250 with 8 52.5, 61.5).
+template <typename T>
+static bool in_tiles(const ScoresArgs& a, bool backward)
+{
+    const size_t bytes = a.K * sizeof(T);
+    const bool many = many_rows(a.n);
+    if (backward || a.top == 0) return bytes <= (many ? 160 : TILE_BYTES);
+    if (a.top > 32) return false;
+    if (bytes <= 512) return bytes <= 256 || a.top > 16 || a.n >= SMS * 32;
+    return many && bytes <= (sizeof(T) == 2 ? 1024 : 704);
+}
+
 template <typename T>
 static int launch_scores(ScoresArgs a, bool backward, cudaStream_t stream)
 {
     a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
     const char* what = backward ? "ptv3_class_scores_bwd" : "ptv3_class_scores_fwd";
-    const size_t bytes = a.K * sizeof(T);
-    // a thread keeps up to 32 alternatives; beyond, and for longer rows, a warp chooses them
-    if (bytes <= TILE_PLAIN_BYTES ? backward || a.top <= 32 : bytes <= TILE_TOP_BYTES && !backward && a.top && a.top <= 32) {
+    if (in_tiles<T>(a, backward)) {
         if (!launch_tile_of<T>(a, backward, stream)) return check_launch("ptv3_class_scores: shared memory attribute");
     } else {
         // (where alternatives are chosen, a warp at least)

@@ -68,7 +68,8 @@ struct Rest {
     {
         const float M = W + t_r, p_in = __fdividef(inside, inside + outside);
         const bool small = p_in < 0.5f;
-        const float log_p = far_log != 0.f ? far_log : (small ? log1pf(-p_in) : -log1pf(__fdividef(inside, outside)));
+        const float log_near = log1pf(small ? -p_in : __fdividef(inside, outside));        // (one call for both)
+        const float log_p = far_log != 0.f ? far_log : (small ? log_near : -log_near);
         const float log_t = W < 0.5f ? log1pf(-W) : logf(t_r);
         term = t_r == 0.f ? 0.f : t_r * (log_t - log_p);
         surplus = small ? W - M * p_in : M * fast_exp2(log_p * LOG2E) - t_r;
@@ -77,7 +78,7 @@ struct Rest {
 };
 
 // ---- short rows: a tile of rows, one thread to a row ---------------------------------------------------------------
-// A row's list in its thread's registers (N entries; N = 0: longer ones are read again from memory wherever they are walked).
+// A row's list in its thread's registers (N entries; N = 0: read from memory wherever it is walked).
 template <int N>
 struct RowList {
     int c[N > 0 ? N : 1];
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     bool any = false;
     ListSums l{-INFINITY, 0.f, 0.f};
     if (!a.rest) list.each([&](int, int, float v) { l.top = max_nan(l.top, v); });
-    float most = 0.f, inside = 0.f, z[N > 0 ? N : 1];
+    float most = 0.f, inside = 0.f, z[N];
     list.each([&](int i, int cls, float v) {
         any = true;
         const float w = entry_weight(a, v, l.top);
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
             most = up ? w : most;
             l.top = up ? v : l.top;
         }
-        if (N > 0) z[N > 0 ? i : 0] = (to_f<T>(x[cls]) - origin) * a.inv_t;
+        z[i] = (to_f<T>(x[cls]) - origin) * a.inv_t;
     });
     if (a.rest)
         list.each([&](int, int cls, float) {
@@ -187,12 +188,8 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
     const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdividef(1.f, l.sum) : l.sum), log_sum = a.rest || !(l.sum > 0.f) ? 0.f : log1pf(l.sum - 1.f);
-    const T* logits = (const T*)a.logits + row * a.ld;
     float loss = 0.f, log_out = -INFINITY, surplus = 0.f;
-    list.each([&](int i, int cls, float v) {
-        const float zi = N > 0 ? z[N > 0 ? i : 0] : (to_f<T>(logits[cls]) - origin) * a.inv_t;
-        loss += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, zi, log_s);
-    });
+    list.each([&](int i, int, float v) { loss += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, z[i], log_s); });
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
         float far_log = 0.f;
@@ -272,12 +269,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
     float x_of[ListPart<G>::N];
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) x_of[q] = list.cls[q] >= 0 ? to_f<T>(x[list.cls[q]]) : 0.f;
+    bool twice = false;              // a class comes more than once in the list
     if (a.rest) {
         for (int w = me; w < words; w += G) bits[w] = 0;
         group.sync();
 #pragma unroll
         for (int q = 0; q < ListPart<G>::N; ++q)
-            if (list.cls[q] >= 0) atomicOr(&bits[list.cls[q] >> 5], 1u << (list.cls[q] & 31));
+            if (list.cls[q] >= 0) {
+                const uint32_t bit = 1u << (list.cls[q] & 31);
+                twice |= (atomicOr(&bits[list.cls[q] >> 5], bit) & bit) != 0;
+            }
+        twice = group.any(twice);
         group.sync();
     }
     float m = -INFINITY;
@@ -304,19 +306,25 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
     if (a.rest)
         vals.each([&](const Eight<T>& e, int j, int) {
             sums.add(masked(e, j), minus, c2);
-            if (const uint32_t in = listed(j)) {
+            if (const uint32_t in = twice ? listed(j) : 0u) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                     if (in >> q & 1) inside += fast_exp2(below_max(e.at(q), origin) * c);
             }
         }, [&](float e, int j, int) {
-            if (is_listed(j))
-                inside += fast_exp2(below_max(e, origin) * c);
-            else
+            if (!is_listed(j))
                 edge.add(e, origin, c);
+            else if (twice)
+                inside += fast_exp2(below_max(e, origin) * c);
         });
     else
         vals.each([&](const Eight<T>& e, int, int) { sums.add(e, minus, c2); }, [&](float e, int, int) { edge.add(e, origin, c); });
+    // (the sum inside: from the list where every class is there once, else from the row)
+    if (a.rest && !twice) {
+#pragma unroll
+        for (int q = 0; q < ListPart<G>::N; ++q)
+            if (list.cls[q] >= 0) inside += fast_exp2(below_max(x_of[q], origin) * c);
+    }
 
     // the list: its largest value, then its sums
     float top = -INFINITY;
@@ -325,16 +333,17 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         if (q * G < a.k) top = max_nan(top, list.v[q]);
     top = group.max(top);
     // the row's (or the outside's) sum; weights; entries, and from 128 on those out of range; the inside's sum
-    float all[4] = {hsum2(sums.s) + edge.s, 0.f, 0.f, inside};
+    float all[3] = {hsum2(sums.s) + edge.s, 0.f, inside};
+    bool bad = false, any = false;
     // with an outcome for the rest: weights but the largest's, entries that are as large as the largest
     float more[2] = {0.f, 0.f}, w[ListPart<G>::N];
 #pragma unroll
     for (int q = 0; q < ListPart<G>::N; ++q) {
         w[q] = 0.f;
         if (q * G >= a.k) continue;
-        all[2] += list.cls[q] == PLACE_BAD ? 128.f : 0.f;
+        bad |= list.cls[q] == PLACE_BAD;
         if (list.cls[q] < 0) continue;
-        all[2] += 1.f;
+        any = true;
         w[q] = entry_weight(a, list.v[q], top);
         all[1] += w[q];
         more[0] += list.v[q] == top ? 0.f : w[q];
@@ -342,8 +351,9 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
     }
     group.sum(all);
     if (a.rest) group.sum(more);
-    const bool bad = all[2] >= 128.f, any = all[2] != 0.f && all[2] != 128.f * (int)(all[2] / 128.f);
-    const float s = all[0] + all[3];
+    bad = group.any(bad);
+    if (a.rest) any = group.any(any);
+    const float s = all[0] + all[2];
     const bool none = s == 0.f;
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
     const ListSums l{top, all[1], more[0] + fmaxf(more[1] - 1.f, 0.f) * fast_exp2(top * LOG2E)};
@@ -382,7 +392,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
         }
         if (open) {
             const float t_r = any ? rest_prob(l.top, l.others) : 0.f;
-            const Rest r(t_r, l.sum, all[3], all[0], far_log, log_s);
+            const Rest r(t_r, l.sum, all[2], all[0], far_log, log_s);
             loss += r.term;
             log_out = r.log_out;
             surplus = r.surplus;
@@ -461,8 +471,8 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
         list.each([&](int, int, float v) { mass += entry_prob(a, st, v); });
         const DistillGrad r = distill_grad(a, row, st, mass);
         // the list's classes apart: M p - t of each, which goes into the row behind the others
-        float own[N > 0 ? N : 1];
-        if (N > 0) list.each([&](int i, int cls, float v) { own[i] = r.in_list(to_f<T>(x[cls])) - r.g * entry_prob(a, st, v); });
+        float own[N];
+        list.each([&](int i, int cls, float v) { own[i] = r.in_list(to_f<T>(x[cls])) - r.g * entry_prob(a, st, v); });
         for (int j = 0; j < a.K; j += 8) {
             Eight<T> e = tile.template read<W>(x, j);
             r.eight(e);
@@ -473,14 +483,13 @@ __global__ void __launch_bounds__(128) distill_tile_bwd_kernel(const DistillArgs
         list.each([&](int i, int cls, float) { x[cls] = from_f<T>((float)i); });
         bool twice = false;
         list.each([&](int i, int cls, float) { twice |= to_f<T>(x[cls]) != (float)i; });
-        if (N > 0 && !twice) {
+        if (!twice) {
             list.each([&](int i, int cls, float) { x[cls] = from_f<T>(own[i]); });
         } else {
             const RowList<0> all(a, row);
-            all.each([&](int, int cls, float v) {
-                float t = twice ? 0.f : entry_prob(a, st, v);
-                if (twice)
-                    all.each([&](int, int other, float u) { t += other == cls ? entry_prob(a, st, u) : 0.f; });
+            all.each([&](int, int cls, float) {
+                float t = 0.f;
+                all.each([&](int, int other, float u) { t += other == cls ? entry_prob(a, st, u) : 0.f; });
                 x[cls] = from_f<T>(r.in_list(to_f<T>(logits[cls])) - r.g * t);
             });
         }
@@ -571,7 +580,7 @@ static bool launch_tile(const DistillArgs& a, bool backward, cudaStream_t stream
     if (a.k <= 4) return backward ? run(distill_tile_bwd_kernel<T, W, 4>) : run(distill_tile_kernel<T, W, 4>);
     if (a.k <= 8) return backward ? run(distill_tile_bwd_kernel<T, W, 8>) : run(distill_tile_kernel<T, W, 8>);
     if (a.k <= 16) return backward ? run(distill_tile_bwd_kernel<T, W, 16>) : run(distill_tile_kernel<T, W, 16>);
-    return backward ? run(distill_tile_bwd_kernel<T, W, 0>) : run(distill_tile_kernel<T, W, 0>);
+    return backward ? run(distill_tile_bwd_kernel<T, W, 32>) : run(distill_tile_kernel<T, W, 32>);
 }
 template <typename T, int G, int P>
 static void launch_row(const DistillArgs& a, bool backward, cudaStream_t stream)
@@ -589,8 +598,11 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
     a.wide = RowTile<T>::wide_rows(a.logits, a.ld, a.K);
     a.wide_out = RowTile<T>::wide_rows(a.dlogits, a.K, a.K);
     a.list4 = a.list_bytes == 4 && !a.teacher_bf16 && a.k % 4 == 0 && (((uintptr_t)a.list | (uintptr_t)a.teacher) & 15) == 0;
+    // Lists of up to 32 in a thread's registers: 200 000 x 128 bf16 with 8 and a rest 66.6 us forward and 48.0 backward spread, 23.2 and 30.8 in tiles; x 166
+    // fp32 86.3 and 84.2, 36.3 and 60.8; x 250 fp32 92 and 111, 58 and 94, but with 16 of 40 000 rows 25 and 31, 22 and 28; 10 000 x 64 fp32 5.0 and
+    // 4.0, 4.7 and 5.3.
     const size_t bytes = a.K * sizeof(T);
-    if (bytes <= TILE_PLAIN_BYTES) {
+    if (a.k <= 32 && bytes <= (many_rows(a.n) ? 704 : TILE_BYTES)) {
         bool ok;
         switch (RowTile<T>::row_width(a.K)) {
         case 16: ok = launch_tile<T, 16>(a, backward, stream); break;

@@ -94,7 +94,7 @@ template <> struct Eight<float> {
 };
 
 constexpr float NO_POWER = -200.f;
-// S and, where they are wanted (U), sum e t of a row, in packed pairs
+// S and, where they are wanted (U), sum e t of a row, in packed pairs.  Eight are added to one another first: a row's sum is rounded an eighth as often.
 template <bool U>
 struct RowSum {
     uint64_t s, u;
@@ -102,6 +102,7 @@ struct RowSum {
     template <typename T>
     __device__ __forceinline__ void add(const Eight<T>& x, uint64_t minus_origin, uint64_t c)
     {
+        uint64_t e[4], v = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             float lo, hi;
@@ -110,10 +111,11 @@ struct RowSum {
                 lo = max_nan(lo, NO_POWER);
                 hi = max_nan(hi, NO_POWER);
             }
-            const uint64_t e = pack2(fast_exp2(lo), fast_exp2(hi));
-            s = add2(s, e);
-            if (U) u = fma2(e, pack2(lo, hi), u);
+            e[q] = pack2(fast_exp2(lo), fast_exp2(hi));
+            if (U) v = q ? fma2(e[q], pack2(lo, hi), v) : mul2(e[q], pack2(lo, hi));
         }
+        s = add2(s, add2(add2(e[0], e[1]), add2(e[2], e[3])));
+        if (U) u = add2(u, v);
     }
 };
 // Eight of a gradient: p (A + B t) with p = 2^t, t = (x - m) c + shift = log2 p; without LOG, p A

@@ -162,11 +162,11 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     bool any = false;
     ListSums l{-INFINITY, 0.f, 0.f};
     if (!a.rest) list.each([&](int, int, float v) { l.top = max_nan(l.top, v); });
-    float most = 0.f, inside = 0.f, z[N];
+    float most = 0.f, inside = 0.f, z[N], parts[4] = {0.f, 0.f, 0.f, 0.f};
     list.each([&](int i, int cls, float v) {
         any = true;
         const float w = entry_weight(a, v, l.top);
-        l.sum += w;
+        parts[i & 3] += w;
         if (a.rest) {
             const bool up = v > l.top;
             l.others += up ? most : w;
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
         }
         z[i] = (to_f<T>(x[cls]) - origin) * a.inv_t;
     });
+    l.sum = (parts[0] + parts[1]) + (parts[2] + parts[3]);
     if (a.rest)
         list.each([&](int, int cls, float) {
             inside += fast_exp2(below_max(to_f<T>(x[cls]), origin) * c);       // (a class that comes again is masked by then)
@@ -189,7 +190,9 @@ __global__ void __launch_bounds__(128) distill_tile_kernel(const DistillArgs a)
     const float log_s = none ? -INFINITY : log1pf(s - 1.f);
     const float scale = a.rest ? 1.f : (l.sum > 0.f ? __fdividef(1.f, l.sum) : l.sum), log_sum = a.rest || !(l.sum > 0.f) ? 0.f : log1pf(l.sum - 1.f);
     float loss = 0.f, log_out = -INFINITY, surplus = 0.f;
-    list.each([&](int i, int, float v) { loss += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, z[i], log_s); });
+    float terms[4] = {0.f, 0.f, 0.f, 0.f};
+    list.each([&](int i, int, float v) { terms[i & 3] += entry_term(a, entry_weight(a, v, l.top), scale, log_sum, v, l.top, z[i], log_s); });
+    loss = (terms[0] + terms[1]) + (terms[2] + terms[3]);
     if (none) loss = l.sum > 0.f ? INFINITY : l.sum;
     if (a.rest) {
         float far_log = 0.f;

@@ -98,11 +98,13 @@ struct Best {
         for (int i = 0; i + 1 < B; ++i) wrong |= v[i] < v[i + 1];
         const bool edge = (unsigned)(best[B - 1] ^ lost) < 32u && v[B - 1] > -INFINITY;
         if (__any_sync(~0u, edge)) {
-            int better = 0;
+            // (where nothing larger was left out, all that are better than the last are in the list, before those that equal it)
+            int better = 0, kept = 0;
 #pragma unroll
             for (int i = 0; i < 32; ++i) better += x[i] > v[B - 1];
-            wrong |= edge && better >= B;
-            // (as many as B - 1 are better than the last of the list where it is right)
+#pragma unroll
+            for (int i = 0; i + 1 < B; ++i) kept += v[i] > v[B - 1];
+            wrong |= edge && better > kept;
         }
         if (__any_sync(~0u, wrong)) {
             unsigned long long wide[B];

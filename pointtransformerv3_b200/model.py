@@ -1032,6 +1032,14 @@ class PointTransformerV3(PointModule):
         return point
 
 
+def _is_its_product(linear):
+    """Whether calling the module is the product with its present weight and its bias and nothing else.  Hooks may do more, and those of
+    ``weight_norm`` and ``spectral_norm`` make the weight: without them it is that of the last call."""
+    every = nn.modules.module
+    return (type(linear) is nn.Linear and not linear._forward_hooks and not linear._forward_pre_hooks
+            and not every._global_forward_hooks and not every._global_forward_pre_hooks)
+
+
 class SegHead(PointModule):
     """Per-point classifier on the backbone's output: ``Linear(in_channels,
     num_classes)`` (state_dict keys ``weight`` / ``bias`` like the ``seg_head`` of a
@@ -1065,11 +1073,11 @@ class SegHead(PointModule):
         """``functional.class_log_probs`` of the head's logits (``ClassScores``), for losses (``-log_prob``), for uncertainty and for the
         lists that ``functional.distill_topk`` learns from.  Where no gradients are wanted, bf16 features of up to 512 channels (a multiple of 8) go
         straight to the scores, up to 32 alternatives: logits are fp32 on the way and never stored (``ops.seg_head_log_probs``).
-        Otherwise they are the layer's own, in its type."""
+        Otherwise, and where the layer has forward hooks, they are the layer's own, in its type."""
         feat = point.feat if isinstance(point, Point) else point
         weight, bias = self.linear.weight, self.linear.bias
         plain = not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (feat, weight, bias)))
-        if (plain and type(self.linear) is nn.Linear and feat.dim() == 2 and weight.dtype == feat.dtype
+        if (plain and _is_its_product(self.linear) and feat.dim() == 2 and weight.dtype == feat.dtype
                 and ops.head_scores_supported(feat.shape[1], top, feat.dtype)):
             return ops.seg_head_log_probs(feat, weight, bias, labels, top, temperature, ignore_index, status)
         return functional.class_log_probs(self.linear(feat), labels, top, temperature, ignore_index, status)

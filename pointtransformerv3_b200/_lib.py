@@ -6,6 +6,7 @@ import ctypes
 import importlib.util
 import os
 import struct
+import sys
 
 import torch
 
@@ -200,12 +201,19 @@ def load():
 _nodes = None
 
 
+def nodes_path():
+    """Where the module of autograd nodes for this torch and this Python is.  It is compiled against both, and one that was made for others
+    would fail to load, or read their tensors with another layout: so its name says them."""
+    return os.path.join(_HERE, "csrc", "ptv3_nodes.torch-%s.abi%d.%s.so" % (
+        torch.__version__, torch._C._GLIBCXX_USE_CXX11_ABI, sys.implementation.cache_tag))
+
+
 def nodes():
     """The module of autograd nodes (csrc/nodes.cpp)."""
     global _nodes
     if _nodes is None:
         load()
-        path = os.path.join(_HERE, "csrc", "ptv3_nodes.so")
+        path = nodes_path()
         if not os.path.exists(path):
             raise Ptv3Error("%s is not built; run `python -m pointtransformerv3_b200.build`" % path)
         spec = importlib.util.spec_from_file_location("ptv3_nodes", path)

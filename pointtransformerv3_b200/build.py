@@ -4,11 +4,12 @@ import os
 import subprocess
 import sys
 
+from . import _lib
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libptv3_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-NODES = os.path.join(CSRC, "ptv3_nodes.so")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "--use_fast_math", "-Xcompiler", "-fPIC"]
 
@@ -33,7 +34,7 @@ def nodes_command():
     include = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(NVCC), "..", "include")]
     return (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
             + [f for i in include for f in ("-isystem", i)]
-            + [os.path.join(CSRC, "nodes.cpp"), "-o", NODES, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            + [os.path.join(CSRC, "nodes.cpp"), "-o", _lib.nodes_path(), "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
                "-ltorch_python", "-L", CSRC, "-l:libptv3_b200.so", "-Wl,-rpath,$ORIGIN"])
 
 
@@ -58,7 +59,7 @@ def build(force=False, verbose=False):
         raise RuntimeError("nvcc failed")
     if jobs or not os.path.exists(LIB):
         subprocess.check_call([NVCC, "-shared", "-Wno-deprecated-gpu-targets", "-o", LIB] + objs + ["-lcudart"])
-    if force or _stale(NODES, os.path.join(CSRC, "nodes.cpp"), glob.glob(os.path.join(HERE, "..", "include", "*.h"))):
+    if force or _stale(_lib.nodes_path(), os.path.join(CSRC, "nodes.cpp"), glob.glob(os.path.join(HERE, "..", "include", "*.h"))):
         subprocess.check_call(nodes_command())
     return LIB
 

@@ -984,6 +984,8 @@ def seg_head(feat, weight, bias=None, want_logits=True, want_labels=True):
 def class_scores(logits, labels, top, temperature, ignore_index, status):
     """ptv3_class_scores_fwd with its gradient; ``functional.class_log_probs`` is the checked form.  logits (N, K) with rows of neighbouring
     values -> (log_prob or None, entropy, top_log_probs or None, top_classes or None)."""
+    _lib.require_cuda(logits, labels, status)
+    _lib.dtype_id(logits)
     call = _lib.nodes().class_scores
     if TIMERS is None:           # (short calls are bounded by the host)
         return call(logits, labels, top, temperature, ignore_index, status)
@@ -1042,6 +1044,8 @@ def seg_head_log_probs(feat, weight, bias=None, labels=None, top=0, temperature=
 
 def distill_topk(logits, teacher, classes, temperature, rest, status):
     """ptv3_distill_topk_fwd with its gradient; ``functional.distill_topk`` is the checked form.  -> loss (N,)."""
+    _lib.require_cuda(logits, teacher, classes, status)
+    _lib.dtype_id(logits), _lib.dtype_id(teacher)
     call = _lib.nodes().distill_topk
     if TIMERS is None:
         return call(logits, teacher, classes, temperature, rest, status)

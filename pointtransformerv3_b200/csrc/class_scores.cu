@@ -113,11 +113,16 @@ __global__ void __launch_bounds__(128) scores_tile_kernel(const ScoresArgs a)
 // ---- longer rows: G threads, some of a warp, a warp or a block ------------------------------------------------------------------------
 // A thread keeps P pieces of eight logits in registers; the longest rows are read again for every pass (P = 0).
 //
-// The alternatives.  A row's logits fall into 64 parts (128 for more than 32 alternatives), of which the largest are known: two or four of each
-// lane where a warp has the row, one of neighbouring threads together where a block has it.  Their k-th largest, by the upper 16 bits of their
+// The alternatives.  A row's logits fall into up to 64 parts (128 for more than 32 alternatives), of which the largest are known: two or four of
+// each lane where a warp has the row, one of neighbouring threads together where a block has it.  Their k-th largest, by the upper 16 bits of their
 // keys, bounds the row's k-th largest from below; a warp takes its parts one after another, a block counts.  The few logits at or above the
-// bound (less than twice k of most rows) are gathered and ranked by counting.  Where more than CANDIDATES are (rows of equal logits, of few
-// values), the best are taken one after another, each a maximum over the row of what comes behind the last one.
+// bound (less than twice k of most long rows) are gathered and ranked by counting.  Where more than CANDIDATES are, the best are taken one after
+// another, each a maximum over the row of what comes behind the last one.
+//
+// That is so for rows of equal logits or of few values, and for lists that are long beside the row.  Rows of up to 256 classes have a part for
+// every eight of them and one for each lane with values at the edges, not 64: with more alternatives than parts there is no bound and all
+// logits are candidates.  From there to 512 and more, 64 of 128 parts still let a large share of the row pass.  60 000 rows of bf16: x 200 with 32,
+// 48 and 64 alternatives 348, 480 and 608 us, x 300 with 64 786, x 500 with 64 952, x 600 with 64 400; fp32 the same.
 constexpr int CANDIDATES = 192;
 
 // value and class as one number, below ~0 (NaN of class 0); 0 for none
@@ -505,6 +510,10 @@ static void launch_row(const ScoresArgs& a, bool backward, cudaStream_t stream)
 // 43.3.  Alternatives, up to 32 of a thread's: few rows of more than 256 bytes finish sooner spread (2 000 x 200 bf16 with 8: 8.7 us in tiles, 4.3), but
 // for many of them; many are slower so up to 1 024 bytes of bf16 or 704 of fp32, where keys have 64 bits (60 000 x 333 bf16 with 8 and 32: 65.5 and 154 us
 // spread, 37.0 and 52.6 in tiles; x 500 65.8 and 138, 56.5 and 74.0; x 166 fp32 53.2 and 422, 41.6 and 78.0; x 250 with 8 52.5, 61.5).
+// These bounds are those of few alternatives.  With 32 the spread form, which is taken, is the slower one beyond them: 10 000 x 166 fp32 78 us, 31 in
+// tiles; 60 000 x 250 fp32 275 and 112; 10 000 x 333 bf16 32 and 21; 60 000 x 600 bf16 156 and 112; with 8 of 100 000 x 200 fp32 84 and 74.  The other
+// way round, tiles are taken and slower for 2 000 x 100 fp32 with 32 (18.5 us, 14.4 spread) and 20 000 x 500 bf16 with 8 (28.8 and 24.7).  More than 32
+// alternatives have the spread form alone.
 template <typename T>
 static bool in_tiles(const ScoresArgs& a, bool backward)
 {

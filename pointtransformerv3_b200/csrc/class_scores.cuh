@@ -30,7 +30,7 @@ struct RowSums {
     bool none;
 };
 constexpr float LN2 = 0.693147180559945309f;
-// S, U = sum e t -> log S and the entropy
+// S, U = sum e t -> log S and the entropy (__fdividef: two units in the last place of a quotient that is as exact as S and U)
 __device__ __forceinline__ RowSums row_sums(float m, float s, float u)
 {
     RowSums r;

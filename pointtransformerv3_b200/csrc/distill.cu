@@ -59,7 +59,8 @@ __device__ __forceinline__ float entry_term(const DistillArgs& a, float w, float
 }
 // The outcome for the rest, from the teacher's t_r, the list's sum and the student's sums inside and outside (far_log: log p_r of an outside that had
 // to be summed from its own maximum, or 0).  What is near 1 is taken from what is missing to it: a list that holds a hundredth of both
-// teacher and student leaves differences of hundredths.
+// teacher and student leaves differences of hundredths.  logf is the fast one of the compiler's flag, off by 2^-21 near 1 and by 3 units in the last
+// place elsewhere: here its argument is at most a half, and for far_log what it adds to is beyond 46 in size.
 struct Rest {
     float term;          // t_r (log t_r - log p_r)
     float surplus;       // M p_r - t_r = W - M (1 - p_r)
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(Group<G>::BLOCK, row_blocks<T>(G, P)) distill_
     for (int q = 0; q < ListPart<G>::N; ++q)
         if (q * G < a.k) top = max_nan(top, list.v[q]);
     top = group.max(top);
-    // the row's (or the outside's) sum; weights; entries, and from 128 on those out of range; the inside's sum
+    // the row's (or the outside's) sum; the list's weights; the inside's sum
     float all[3] = {hsum2(sums.s) + edge.s, 0.f, inside};
     bool bad = false, any = false;
     // with an outcome for the rest: weights but the largest's, entries that are as large as the largest
@@ -603,7 +604,7 @@ static int launch_distill(DistillArgs a, bool backward, cudaStream_t stream)
     a.list4 = a.list_bytes == 4 && !a.teacher_bf16 && a.k % 4 == 0 && (((uintptr_t)a.list | (uintptr_t)a.teacher) & 15) == 0;
     // Lists of up to 32 in a thread's registers: 200 000 x 128 bf16 with 8 and a rest 66.6 us forward and 48.0 backward spread, 23.2 and 30.8 in tiles; x 166
     // fp32 86.3 and 84.2, 36.3 and 60.8; x 250 fp32 92 and 111, 58 and 94, but with 16 of 40 000 rows 25 and 31, 22 and 28; 10 000 x 64 fp32 5.0 and
-    // 4.0, 4.7 and 5.3.
+    // 4.0, 4.7 and 5.3.  Longer lists have the spread form alone.
     const size_t bytes = a.K * sizeof(T);
     if (a.k <= 32 && bytes <= (many_rows(a.n) ? 704 : TILE_BYTES)) {
         bool ok;

@@ -1,6 +1,6 @@
 // Calls and autograd nodes of the operators behind a network's logits (functional.py, ops.py): outputs and the forward call of the C ABI, and, on
 // the engine's thread, the backward call, without Python on the way.  Short calls are bounded by the host: a training step on 64 x 20 logits
-// took 104 us with a node in Python, most of it in a thread that has just woken up, and takes 64 so (one of torch's own log_softmax: 49).
+// took 104 us with a node in Python, most of it in a thread that has just woken up, and takes 56 so (one of torch's own log_softmax: 49).
 //
 // The checks of arguments stand in functional.py, ahead of these calls.  Gradients are of first order: one that is to be differentiated again
 // is an error node, as torch's once_differentiable leaves it.

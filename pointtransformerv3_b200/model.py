@@ -1044,7 +1044,8 @@ class SegHead(PointModule):
     """Per-point classifier on the backbone's output: ``Linear(in_channels,
     num_classes)`` (state_dict keys ``weight`` / ``bias`` like the ``seg_head`` of a
     segmentor around the reference backbone) with the arg max taken in the same pass.
-    ``forward(point)`` stores ``seg_logits`` (unless ``logits=False``) and ``seg_pred``.
+    ``forward(point)`` stores ``seg_logits`` (unless ``logits=False``) and ``seg_pred``, from the layer's weight and bias as they are: it calls
+    no hooks of the layer.
     ``log_probs(point, labels)`` scores a batch instead: log probabilities, entropy, alternatives, with gradients where they are asked for."""
 
     def __init__(self, in_channels, num_classes, logits=True):
